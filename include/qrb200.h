@@ -44,8 +44,10 @@ enum {
   QRB200_ERR_CUDA = 3,       /* a CUDA runtime call or kernel launch failed          */
   QRB200_ERR_DEVICE = 4,     /* current device is not an sm_100 (B200-class) GPU     */
   QRB200_ERR_TIMEOUT = 5,    /* a device-side bounded wait expired (see device_status) */
-  QRB200_ERR_SCRATCH_LIMIT = 6 /* qrb200_geqrf_f32_noalloc: problem needs more scratch than
+  QRB200_ERR_SCRATCH_LIMIT = 6, /* qrb200_geqrf_f32_noalloc: problem needs more scratch than
                                   QRB200_NOALLOC_SCRATCH_BYTES                           */
+  QRB200_ERR_INDEX = 7       /* a cache slot, block table entry or length was out of range
+                                (see qrb200_last_status); it was skipped, not followed   */
 };
 
 /* Bytes of scratch that qrb200_geqrf_f32 needs for (batch, n).
@@ -91,18 +93,19 @@ int qrb200_version(void);
  * records the failure, skips its outputs and returns (the results of that call are invalid).
  * The record lands in a device word and in a mapped pinned host word per device.
  *
- * qrb200_last_status: QRB200_ERR_TIMEOUT if a kernel on the current device has recorded a
+ * qrb200_last_status: QRB200_ERR_TIMEOUT (an expired wait) or QRB200_ERR_INDEX (a slot, block
+ * table entry or length outside a cache) if a kernel on the current device has recorded a
  * failure since the last read, else QRB200_OK; the host word is cleared by the read. It makes
  * no CUDA call beyond cudaGetDevice and never waits, so it sees failures of work that has
  * already executed (read it after synchronising, or before the next call as the Python operator
  * does). *site_out (may be NULL) receives the wait site: 1 tensor-core mbarrier, 2 whole-matrix
- * hand-off, 3 cluster-panel exchange, 4 self-test. No counterpart in the reference (its only
+ * hand-off, 3 cluster-panel exchange, 4 self-test, 5 cache index. No counterpart in the reference (its only
  * failure mechanism is the exception fallback of submission.py:572-596). */
 int qrb200_last_status(int* site_out);
 
 /* Synchronous variant: reads (and clears) the device word of the current device with a symbol
  * copy (which waits for prior work on the legacy default stream) and clears the host word;
- * *status_out = QRB200_ERR_TIMEOUT or QRB200_OK. */
+ * *status_out = QRB200_ERR_TIMEOUT, QRB200_ERR_INDEX or QRB200_OK. */
 int qrb200_device_status(int* status_out);
 
 /* Test hook: one warp waits `polls` times on a barrier that nothing completes, so the wait runs
@@ -137,6 +140,80 @@ int qrb200_selftest_wait_timeout(uint32_t polls, void* stream);
  *     them on one stream, or with events. */
 int qrb200_geqrf_f32_noalloc(const float* A, float* H, float* tau, int64_t batch, int64_t n,
                              int64_t a_batch_stride, void* stream);
+
+/* ---- data in 8 and 4 bits (no counterpart in the reference) ---------------------------
+ *
+ * What a consumer of Q needs next to it: activations and weights rotated by an orthogonal matrix
+ * hold no outlying channels, and are kept in 8 bits, keys and values in 4. All entries are
+ * asynchronous on `stream`, allocate nothing, return a status, and first report (launching
+ * nothing) a failure that a kernel of an earlier call has recorded, as qrb200_last_status does. */
+
+enum { QRB200_F32 = 0, QRB200_BF16 = 1, QRB200_F16 = 2 }; /* element types */
+
+/* Rows into 8 bits. h = x + residual (x alone when residual is NULL); t = h * weight (h alone when
+ * weight is NULL); code_j = rint(t_j * 127 / a) with a = max |t_j|;
+ * scale = a * (mean(h^2) + eps)^-1/2 / 127, so code * scale is the norm's output. h, rounded to
+ * dtype, goes to h_out (rows x cols, contiguous; NULL exactly when residual is).
+ * x, residual: rows x cols of dtype with row strides in elements; weight: cols of dtype or of
+ * QRB200_F32; q: row stride q_stride bytes; scale: rows. cols <= 32768. A row with a NaN or an
+ * infinity gets codes 0 and a NaN scale; one whose a is below 2^-100 gets codes and scale 0. */
+int qrb200_rms_norm_int8(const void* x, int64_t x_stride, const void* residual, int64_t residual_stride,
+                         const void* weight, int weight_type, int8_t* q, int64_t q_stride, float* scale, void* h_out,
+                         int64_t rows, int64_t cols, float eps, int dtype, void* stream);
+
+/* The same without the norm: code = rint(x * 127 / max|x|), scale = max|x| / 127. */
+int qrb200_quantize_int8(const void* x, int64_t x_stride, int8_t* q, int64_t q_stride, float* scale, int64_t rows,
+                         int64_t cols, int dtype, void* stream);
+
+/* out (rows x cols of dtype, contiguous) = q * scale of its row. */
+int qrb200_dequantize_int8(const int8_t* q, int64_t q_stride, const float* scale, void* out, int64_t rows,
+                           int64_t cols, int dtype, void* stream);
+
+/* y[i, n] = (sum_k x[i, k] w[n, k]) x_scale[i] w_scale[n] + bias[n]: y rows x outs of dtype,
+ * contiguous; bias (may be NULL) of dtype; row strides of x and w in bytes. The sum is exact in
+ * 32-bit integers for depth <= QRB200_INT8_MAX_DEPTH. */
+#define QRB200_INT8_MAX_DEPTH 131071
+int qrb200_int8_linear(const int8_t* x, int64_t x_stride, const float* x_scale, const int8_t* w, int64_t w_stride,
+                       const float* w_scale, const void* bias, void* y, int64_t rows, int64_t outs, int64_t depth,
+                       int dtype, void* stream);
+
+/* A paged key/value cache in 4 bits: pages x kv_heads blocks of qrb200_kv4_block_bytes bytes,
+ * contiguous, 16-byte aligned. Each group of head_dim / groups channels of a token holds 4-bit
+ * codes and a step and minimum of type dtype (QRB200_BF16 or QRB200_F16). head_dim 64 or 128;
+ * groups of 32, 64 or 128 channels; page_size a power of two from 16 to 1024. */
+typedef struct qrb200_kv4_shape {
+  int64_t pages;
+  int32_t kv_heads, page_size, head_dim, groups, dtype;
+} qrb200_kv4_shape;
+int64_t qrb200_kv4_block_bytes(int64_t page_size, int64_t head_dim, int64_t group_size);
+
+/* Quantises keys and values (tokens x kv_heads x head_dim of the cache's type, channels
+ * contiguous, other strides in elements) into the cache at slots (page * page_size + offset). A
+ * negative slot is skipped; slots of one call must differ. A group's step and minimum are its
+ * range / 15 and its least entry, its codes the nearest steps; a group with a NaN or an infinity
+ * reads back as NaN. */
+int qrb200_kv4_write(void* cache, const qrb200_kv4_shape* shape, const void* k, int64_t k_token_stride,
+                     int64_t k_head_stride, const void* v, int64_t v_token_stride, int64_t v_head_stride,
+                     const int64_t* slots, int64_t tokens, void* stream);
+
+/* The values at slots, as tokens x kv_heads x head_dim, contiguous; zeros for a negative slot. */
+int qrb200_kv4_read(const void* cache, const qrb200_kv4_shape* shape, void* k, void* v, const int64_t* slots,
+                    int64_t tokens, void* stream);
+
+/* Attention of `queries` new tokens of each sequence over the cache. q: batch x queries x q_heads x
+ * head_dim of the cache's type, channels contiguous, q_strides = {batch, query, head} in elements;
+ * q_heads a multiple of kv_heads (head h reads key head h / (q_heads / kv_heads)). block_table:
+ * batch x max_pages pages, rows table_stride apart; entries past a sequence's length are not read.
+ * lengths: batch, tokens in the cache, the queries' own among them: query i stands at position
+ * lengths - queries + i. It sees the tokens up to its position (all of them when causal is 0),
+ * and of those the last `window` up to its position when window > 0. out: batch x queries x q_heads x head_dim,
+ * contiguous; zeros where nothing is seen. Workspace as the query says, 256-byte aligned. */
+size_t qrb200_kv4_attention_workspace_bytes(const qrb200_kv4_shape* shape, int64_t batch, int64_t queries,
+                                            int64_t q_heads, int64_t max_pages);
+int qrb200_kv4_attention(const void* q, const int64_t* q_strides, const void* cache, const qrb200_kv4_shape* shape,
+                         const int32_t* block_table, int64_t table_stride, const int32_t* lengths, void* out,
+                         int64_t batch, int64_t queries, int64_t q_heads, int64_t max_pages, int64_t window,
+                         int causal, float scale, void* workspace, size_t workspace_bytes, void* stream);
 
 /* ---- diagnostics (no counterpart in the reference; used by bench.py) ---------------- */
 

@@ -8,10 +8,16 @@ Public API (the reference's drop-in operator, ``submission.py:560-596``)::
     Q = householder_product(H, tau)    # explicit Q (sorgqr), on the tensor cores
     X = ormqr(H, tau, B, transpose=True)   # Q^T B (sormqr)
 
+Operators on data in 8 and 4 bits, which an orthogonal ``Q`` makes fit for them (``quant``):
+``rms_norm_int8``, ``quantize_int8``, ``dequantize_int8``, ``int8_linear``, ``kv4_cache``,
+``kv4_write``, ``kv4_read``, ``kv4_attention``.
+
 Helpers: ``gen`` (seeded inputs), ``checker`` (the FP64 correctness gate),
 ``sharding`` (host-side batch split over several GPUs).
 """
 
 from .api import custom_kernel, custom_kernel_host, geqrf, householder_product, ormqr, workspace_bytes  # noqa: F401
+from .quant import (KV4Cache, dequantize_int8, int8_linear, kv4_attention, kv4_cache, kv4_read,  # noqa: F401
+                    kv4_write, quantize_int8, rms_norm_int8)
 
 __version__ = "0.1.0"

@@ -19,6 +19,7 @@ QRB200_ERR_CUDA = 3
 QRB200_ERR_DEVICE = 4
 QRB200_ERR_TIMEOUT = 5
 QRB200_ERR_SCRATCH_LIMIT = 6
+QRB200_ERR_INDEX = 7
 NOALLOC_SCRATCH_BYTES = 32 << 20  # QRB200_NOALLOC_SCRATCH_BYTES
 
 class KernelStat(ctypes.Structure):
@@ -27,6 +28,15 @@ class KernelStat(ctypes.Structure):
     _fields_ = [("name", ctypes.c_char * 32), ("launches", ctypes.c_int32), ("tensor_bound", ctypes.c_int32),
                 ("ms", ctypes.c_double), ("flops", ctypes.c_double), ("bytes", ctypes.c_double)]
 
+
+class KV4Shape(ctypes.Structure):
+    """``qrb200_kv4_shape`` of include/qrb200.h."""
+
+    _fields_ = [("pages", ctypes.c_int64), ("kv_heads", ctypes.c_int32), ("page_size", ctypes.c_int32),
+                ("head_dim", ctypes.c_int32), ("groups", ctypes.c_int32), ("dtype", ctypes.c_int32)]
+
+
+_P, _I64, _INT, _F32, _SIZE = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_float, ctypes.c_size_t
 
 # Every symbol include/qrb200.h declares, with its ctypes signature.
 SIGNATURES = {
@@ -56,6 +66,16 @@ SIGNATURES = {
                                                 ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p,
                                                 ctypes.POINTER(KernelStat), ctypes.c_int,
                                                 ctypes.POINTER(ctypes.c_int)]),
+    "qrb200_rms_norm_int8": (_INT, [_P, _I64, _P, _I64, _P, _INT, _P, _I64, _P, _P, _I64, _I64, _F32, _INT, _P]),
+    "qrb200_quantize_int8": (_INT, [_P, _I64, _P, _I64, _P, _I64, _I64, _INT, _P]),
+    "qrb200_dequantize_int8": (_INT, [_P, _I64, _P, _P, _I64, _I64, _INT, _P]),
+    "qrb200_int8_linear": (_INT, [_P, _I64, _P, _P, _I64, _P, _P, _P, _I64, _I64, _I64, _INT, _P]),
+    "qrb200_kv4_block_bytes": (_I64, [_I64, _I64, _I64]),
+    "qrb200_kv4_write": (_INT, [_P, _P, _P, _I64, _I64, _P, _I64, _I64, _P, _I64, _P]),
+    "qrb200_kv4_read": (_INT, [_P, _P, _P, _P, _P, _I64, _P]),
+    "qrb200_kv4_attention_workspace_bytes": (_SIZE, [_P, _I64, _I64, _I64, _I64]),
+    "qrb200_kv4_attention": (_INT, [_P, _P, _P, _P, _P, _I64, _P, _P, _I64, _I64, _I64, _I64, _I64, _INT, _F32, _P,
+                                    _SIZE, _P]),
 }
 
 _lock = threading.Lock()

@@ -17,7 +17,7 @@ REPO_DIR = os.path.dirname(PKG_DIR)
 CSRC = os.path.join(PKG_DIR, "csrc")
 LIB_NAME = "libqrb200.so"
 LIB_PATH = os.path.join(PKG_DIR, LIB_NAME)
-SOURCES = ["qrb200.cu", "noalloc.cu"]
+SOURCES = ["qrb200.cu", "quant.cu", "noalloc.cu"]
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 
@@ -45,7 +45,7 @@ def build(force: bool = False, verbose: bool = False) -> str:
     """Compile ``libqrb200.so`` next to this file if any source is newer; return its path."""
     if not force and up_to_date():
         return LIB_PATH
-    cmd = [nvcc_path(), *ARCH_FLAGS, "-O3", "-lineinfo", "-std=c++17", "-shared",
+    cmd = [nvcc_path(), *ARCH_FLAGS, "-O3", "-lineinfo", "-std=c++17", "-shared", "--threads", "0",
            "-Xcompiler", "-fPIC", "-Xptxas", "-v" if verbose else "-O3",
            "-I", os.path.join(REPO_DIR, "include"), "-o", LIB_PATH + ".tmp"]
     cmd += [os.path.join(CSRC, s) for s in SOURCES]

@@ -86,7 +86,7 @@ constexpr float kRescaleUp = 0x1p100f, kRescaleDown = 0x1p-100f;
 
 // Out of line: the hot loops keep a plain branch to a call that ordinary inputs never take
 // (inlined, the precise square root and reciprocals of this path slowed the reflector chain).
-__device__ __noinline__ Reflector make_reflector_outside(float alpha, float xnorm2, float xnorm2_up) {
+static __device__ __noinline__ Reflector make_reflector_outside(float alpha, float xnorm2, float xnorm2_up) {
   if (fmaf(alpha, alpha, xnorm2) < kRescaleDown) {
     Reflector r = make_reflector(alpha * kRescaleUp, xnorm2_up);
     r.diag *= kRescaleDown;

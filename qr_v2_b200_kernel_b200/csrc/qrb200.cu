@@ -23,6 +23,7 @@
 #include <mutex>
 #include <vector>
 
+#include "internal.h"
 #include "qrb200.h"
 #include "panel.cuh"
 #include "panel_fw.cuh"
@@ -228,6 +229,11 @@ static int check_device() {
   }
   ok.mark(dev);
   return QRB200_OK;
+}
+
+// A recorded wait site as a status: sites from kSiteIndex on are indexes out of range.
+static int site_status(int site) {
+  return site == 0 ? QRB200_OK : site >= kSiteIndex ? QRB200_ERR_INDEX : QRB200_ERR_TIMEOUT;
 }
 
 // Launch with an optional cluster shape and, for kernels that begin with griddep_launch_wait(),
@@ -1124,6 +1130,17 @@ __global__ void selftest_wait_kernel(uint32_t polls) {
 
 using namespace qrb200;
 
+int qrb200_internal_check_device() { return check_device(); }
+int* qrb200_internal_status_word(int dev) {
+  void* d = nullptr;
+  std::lock_guard<std::mutex> lk(g_status_mu);
+  if (!g_status_host || dev < 0 || dev >= kStatusWords ||
+      cudaHostGetDevicePointer(&d, g_status_host + dev, 0) != cudaSuccess)
+    return nullptr;
+  return static_cast<int*>(d);
+}
+void qrb200_internal_count_launch() { g_launches.fetch_add(1, std::memory_order_relaxed); }
+
 static int geqrf_impl(const float* A, float* H, float* tau, int64_t batch, int64_t n,
                       int64_t a_batch_stride, void* workspace, size_t workspace_bytes, void* stream);
 int qrb200_noalloc_scratch(void** out);  // noalloc.cu: static scratch of the current device
@@ -1286,6 +1303,7 @@ const char* qrb200_status_string(int status) {
     case QRB200_ERR_CUDA: return "CUDA runtime error or kernel launch failure";
     case QRB200_ERR_DEVICE: return "current device is not an sm_100 (B200-class) GPU";
     case QRB200_ERR_TIMEOUT: return "device-side bounded wait expired";
+    case QRB200_ERR_INDEX: return "a slot, block table entry or length pointed outside the cache";
     case QRB200_ERR_SCRATCH_LIMIT:
       return "problem needs more than the 32 MiB static scratch of qrb200_geqrf_f32_noalloc; "
              "call qrb200_geqrf_f32 with a workspace";
@@ -1299,6 +1317,8 @@ int qrb200_device_status(int* status_out) {
   if (!status_out) return QRB200_ERR_ARG;
   int v = 0;
   if (cudaMemcpyFromSymbol(&v, g_device_status, sizeof(int)) != cudaSuccess) return QRB200_ERR_CUDA;
+  const int q = qrb200_internal_quant_site();
+  if (q < 0) return QRB200_ERR_CUDA;
   const int zero = 0;
   if (v != 0 && cudaMemcpyToSymbol(g_device_status, &zero, sizeof(int)) != cudaSuccess) return QRB200_ERR_CUDA;
   int dev = 0;
@@ -1306,7 +1326,7 @@ int qrb200_device_status(int* status_out) {
     std::lock_guard<std::mutex> lk(g_status_mu);
     if (g_status_host) reinterpret_cast<volatile int*>(g_status_host)[dev] = 0;
   }
-  *status_out = v != 0 ? QRB200_ERR_TIMEOUT : QRB200_OK;
+  *status_out = site_status(v != 0 ? v : q);
   return QRB200_OK;
 }
 
@@ -1323,7 +1343,7 @@ int qrb200_last_status(int* site_out) {
     }
   }
   if (site_out) *site_out = v;
-  return v != 0 ? QRB200_ERR_TIMEOUT : QRB200_OK;
+  return site_status(v);
 }
 
 int qrb200_selftest_wait_timeout(uint32_t polls, void* stream) {

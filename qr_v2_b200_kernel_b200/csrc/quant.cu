@@ -1,0 +1,238 @@
+// C ABI of the operators on data in 8 and 4 bits: argument checks, choice of kernel, launches.
+#include <cuda.h>
+#include <cudaTypedefs.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <atomic>
+#include <cstdint>
+#include <mutex>
+
+#include "internal.h"
+#include "qrb200.h"
+#include "i8_linear.cuh"
+#include "kv4.cuh"
+#include "quant_rows.cuh"
+
+namespace qrb200 {
+
+// This translation unit's failure words, registered once per device after the library's own check.
+static int quant_ready() {
+  static std::atomic<unsigned long long> ready{0};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return QRB200_ERR_CUDA;
+  if (dev < 64 && ((ready.load(std::memory_order_acquire) >> dev) & 1ull)) return qrb200_last_status(nullptr);
+  const int st = qrb200_internal_check_device();
+  if (st != QRB200_OK) return st;
+  int* word = qrb200_internal_status_word(dev);
+  if (word && cudaMemcpyToSymbol(g_status_mapped, &word, sizeof(word)) != cudaSuccess) return QRB200_ERR_CUDA;
+  if (dev < 64) ready.fetch_or(1ull << dev, std::memory_order_acq_rel);
+  return qrb200_last_status(nullptr);
+}
+
+static int launched() {
+  qrb200_internal_count_launch();
+  return cudaGetLastError() == cudaSuccess ? QRB200_OK : QRB200_ERR_CUDA;
+}
+
+static bool type_ok(int t) { return t == QRB200_F32 || t == QRB200_BF16 || t == QRB200_F16; }
+static bool type16_ok(int t) { return t == QRB200_BF16 || t == QRB200_F16; }
+
+constexpr int kMaxCols = 32768;
+constexpr int64_t kMaxRows = (1ll << 31) - 1;
+
+template <typename T, bool kNorm>
+static int launch_rows(const RowsParams& p, int weight_type, int dtype, cudaStream_t s) {
+  const unsigned grid = (unsigned)p.rows;
+  if (p.weight && weight_type == QRB200_F32 && dtype != QRB200_F32)
+    rows_int8_kernel<T, float, kNorm><<<grid, 256, 0, s>>>(p);
+  else
+    rows_int8_kernel<T, T, kNorm><<<grid, 256, 0, s>>>(p);
+  return launched();
+}
+
+template <bool kNorm>
+static int rows_int8(const RowsParams& p, int weight_type, int dtype, cudaStream_t s) {
+  switch (dtype) {
+    case QRB200_BF16: return launch_rows<__nv_bfloat16, kNorm>(p, weight_type, dtype, s);
+    case QRB200_F16: return launch_rows<__half, kNorm>(p, weight_type, dtype, s);
+    default: return launch_rows<float, kNorm>(p, weight_type, dtype, s);
+  }
+}
+
+static bool shape_ok(const Kv4Shape& h) {
+  return h.pages >= 0 && h.pages <= (1ll << 31) - 1 && h.heads > 0 && h.heads <= 65535 && (h.dim == 64 || h.dim == 128) &&
+         h.page >= 16 && h.page <= 1024 && (h.page & (h.page - 1)) == 0 && h.groups > 0 && h.dim % h.groups == 0 &&
+         (h.dim / h.groups == 32 || h.dim / h.groups == 64 || h.dim / h.groups == 128);
+}
+
+}  // namespace qrb200
+
+using namespace qrb200;
+
+int qrb200_internal_quant_site() {
+  int v = 0;
+  const int zero = 0;
+  if (cudaMemcpyFromSymbol(&v, g_device_status, sizeof(int)) != cudaSuccess) return -1;
+  if (v != 0 && cudaMemcpyToSymbol(g_device_status, &zero, sizeof(int)) != cudaSuccess) return -1;
+  return v;
+}
+
+extern "C" {
+
+int qrb200_rms_norm_int8(const void* x, int64_t x_stride, const void* residual, int64_t residual_stride,
+                         const void* weight, int weight_type, int8_t* q, int64_t q_stride, float* scale, void* h_out,
+                         int64_t rows, int64_t cols, float eps, int dtype, void* stream) {
+  if (rows < 0 || cols < 0 || rows > kMaxRows || cols > kMaxCols || !type_ok(dtype)) return QRB200_ERR_ARG;
+  if (rows == 0 || cols == 0) return QRB200_OK;
+  if (!x || !q || !scale || (residual != nullptr) != (h_out != nullptr) || !(eps >= 0.f)) return QRB200_ERR_ARG;
+  if (weight && weight_type != dtype && weight_type != QRB200_F32) return QRB200_ERR_ARG;
+  if (rows > 1 && (x_stride < cols || q_stride < cols || (residual && residual_stride < cols))) return QRB200_ERR_ARG;
+  const int st = quant_ready();
+  if (st != QRB200_OK) return st;
+  RowsParams p{x, residual, weight, h_out, q, scale, rows, x_stride, residual_stride, q_stride, (int)cols, eps};
+  return rows_int8<true>(p, weight_type, dtype, static_cast<cudaStream_t>(stream));
+}
+
+int qrb200_quantize_int8(const void* x, int64_t x_stride, int8_t* q, int64_t q_stride, float* scale, int64_t rows,
+                         int64_t cols, int dtype, void* stream) {
+  if (rows < 0 || cols < 0 || rows > kMaxRows || cols > kMaxCols || !type_ok(dtype)) return QRB200_ERR_ARG;
+  if (rows == 0 || cols == 0) return QRB200_OK;
+  if (!x || !q || !scale || (rows > 1 && (x_stride < cols || q_stride < cols))) return QRB200_ERR_ARG;
+  const int st = quant_ready();
+  if (st != QRB200_OK) return st;
+  RowsParams p{x, nullptr, nullptr, nullptr, q, scale, rows, x_stride, 0, q_stride, (int)cols, 0.f};
+  return rows_int8<false>(p, dtype, dtype, static_cast<cudaStream_t>(stream));
+}
+
+int qrb200_dequantize_int8(const int8_t* q, int64_t q_stride, const float* scale, void* out, int64_t rows,
+                           int64_t cols, int dtype, void* stream) {
+  if (rows < 0 || cols < 0 || rows > kMaxRows || cols > kMaxCols || !type_ok(dtype)) return QRB200_ERR_ARG;
+  if (rows == 0 || cols == 0) return QRB200_OK;
+  if (!q || !scale || !out || (rows > 1 && q_stride < cols)) return QRB200_ERR_ARG;
+  const int st = quant_ready();
+  if (st != QRB200_OK) return st;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const unsigned grid = (unsigned)rows;
+  if (dtype == QRB200_BF16)
+    dequant_rows_kernel<<<grid, 256, 0, s>>>(q, q_stride, scale, static_cast<__nv_bfloat16*>(out), rows, (int)cols);
+  else if (dtype == QRB200_F16)
+    dequant_rows_kernel<<<grid, 256, 0, s>>>(q, q_stride, scale, static_cast<__half*>(out), rows, (int)cols);
+  else
+    dequant_rows_kernel<<<grid, 256, 0, s>>>(q, q_stride, scale, static_cast<float*>(out), rows, (int)cols);
+  return launched();
+}
+
+int qrb200_int8_linear(const int8_t* x, int64_t x_stride, const float* x_scale, const int8_t* w, int64_t w_stride,
+                       const float* w_scale, const void* bias, void* y, int64_t rows, int64_t outs, int64_t depth,
+                       int dtype, void* stream) {
+  if (rows < 0 || outs < 0 || depth <= 0 || depth > QRB200_INT8_MAX_DEPTH || !type_ok(dtype)) return QRB200_ERR_ARG;
+  if (rows > kMaxRows || outs > kMaxRows) return QRB200_ERR_ARG;
+  if (rows == 0 || outs == 0) return QRB200_OK;
+  if (!x || !w || !x_scale || !w_scale || !y) return QRB200_ERR_ARG;
+  if ((rows > 1 && x_stride < depth) || (outs > 1 && w_stride < depth)) return QRB200_ERR_ARG;
+  const int st = quant_ready();
+  if (st != QRB200_OK) return st;
+  I8Params p{x, w, x_scale, w_scale, bias, y, rows, outs, x_stride, w_stride, (int)depth};
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const dim3 grid((unsigned)((outs + 63) / 64), (unsigned)((rows + 63) / 64));
+  if (grid.y > 65535) return QRB200_ERR_ARG;
+  if (dtype == QRB200_BF16)
+    i8_linear_simple_kernel<__nv_bfloat16><<<grid, 256, 0, s>>>(p);
+  else if (dtype == QRB200_F16)
+    i8_linear_simple_kernel<__half><<<grid, 256, 0, s>>>(p);
+  else
+    i8_linear_simple_kernel<float><<<grid, 256, 0, s>>>(p);
+  return launched();
+}
+
+int64_t qrb200_kv4_block_bytes(int64_t page_size, int64_t head_dim, int64_t group_size) {
+  if (group_size <= 0 || page_size < 0 || page_size > 1024 || head_dim < 0 || head_dim > 128) return 0;
+  const Kv4Shape h{1, (int)page_size, (int)head_dim, (int)(head_dim / std::min<int64_t>(group_size, 1024)), 0};
+  return shape_ok(h) && head_dim % group_size == 0 ? h.block_bytes() : 0;
+}
+
+int qrb200_kv4_write(void* cache, const qrb200_kv4_shape* shape, const void* k, int64_t k_token_stride,
+                     int64_t k_head_stride, const void* v, int64_t v_token_stride, int64_t v_head_stride,
+                     const int64_t* slots, int64_t tokens, void* stream) {
+  if (!shape || tokens < 0 || !type16_ok(shape->dtype)) return QRB200_ERR_ARG;
+  const Kv4Shape h{shape->kv_heads, shape->page_size, shape->head_dim, shape->groups, shape->pages};
+  if (!shape_ok(h) || tokens > kMaxRows / h.heads) return QRB200_ERR_ARG;
+  if (tokens == 0) return QRB200_OK;
+  if (!cache || !k || !v || !slots || (reinterpret_cast<uintptr_t>(cache) & 15u)) return QRB200_ERR_ARG;
+  const int st = quant_ready();
+  if (st != QRB200_OK) return st;
+  Kv4IoParams p{static_cast<unsigned char*>(cache), k, v, nullptr, nullptr, reinterpret_cast<const long long*>(slots),
+                tokens, k_token_stride, k_head_stride, v_token_stride, v_head_stride, h};
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const unsigned grid = (unsigned)((tokens * h.heads + 3) / 4);
+  const bool bf = shape->dtype == QRB200_BF16;
+  if (h.dim == 128) {
+    if (bf) kv4_write_kernel<__nv_bfloat16, 4><<<grid, 128, 0, s>>>(p);
+    else kv4_write_kernel<__half, 4><<<grid, 128, 0, s>>>(p);
+  } else {
+    if (bf) kv4_write_kernel<__nv_bfloat16, 2><<<grid, 128, 0, s>>>(p);
+    else kv4_write_kernel<__half, 2><<<grid, 128, 0, s>>>(p);
+  }
+  return launched();
+}
+
+int qrb200_kv4_read(const void* cache, const qrb200_kv4_shape* shape, void* k, void* v, const int64_t* slots,
+                    int64_t tokens, void* stream) {
+  if (!shape || tokens < 0 || !type16_ok(shape->dtype)) return QRB200_ERR_ARG;
+  const Kv4Shape h{shape->kv_heads, shape->page_size, shape->head_dim, shape->groups, shape->pages};
+  if (!shape_ok(h) || tokens > kMaxRows / h.heads) return QRB200_ERR_ARG;
+  if (tokens == 0) return QRB200_OK;
+  if (!cache || !k || !v || !slots || (reinterpret_cast<uintptr_t>(cache) & 15u)) return QRB200_ERR_ARG;
+  const int st = quant_ready();
+  if (st != QRB200_OK) return st;
+  Kv4IoParams p{static_cast<unsigned char*>(const_cast<void*>(cache)), nullptr, nullptr, k, v,
+                reinterpret_cast<const long long*>(slots), tokens, 0, 0, 0, 0, h};
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const unsigned grid = (unsigned)((tokens * h.heads * h.dim + 255) / 256);
+  if (shape->dtype == QRB200_BF16) kv4_read_kernel<__nv_bfloat16><<<grid, 256, 0, s>>>(p);
+  else kv4_read_kernel<__half><<<grid, 256, 0, s>>>(p);
+  return launched();
+}
+
+size_t qrb200_kv4_attention_workspace_bytes(const qrb200_kv4_shape* shape, int64_t batch, int64_t queries,
+                                            int64_t q_heads, int64_t max_pages) {
+  (void)shape, (void)batch, (void)queries, (void)q_heads, (void)max_pages;
+  return 0;
+}
+
+int qrb200_kv4_attention(const void* q, const int64_t* q_strides, const void* cache, const qrb200_kv4_shape* shape,
+                         const int32_t* block_table, int64_t table_stride, const int32_t* lengths, void* out,
+                         int64_t batch, int64_t queries, int64_t q_heads, int64_t max_pages, int64_t window,
+                         int causal, float scale, void* workspace, size_t workspace_bytes, void* stream) {
+  (void)workspace, (void)workspace_bytes;
+  if (!shape || !q_strides || batch < 0 || queries < 0 || q_heads < 0 || max_pages < 0 || window < 0 ||
+      !type16_ok(shape->dtype))
+    return QRB200_ERR_ARG;
+  const Kv4Shape h{shape->kv_heads, shape->page_size, shape->head_dim, shape->groups, shape->pages};
+  if (!shape_ok(h) || q_heads % h.heads != 0 || batch > 65535 || queries > kMaxRows || q_heads > 65535 ||
+      batch * queries > kMaxRows / std::max<int64_t>(1, q_heads) || max_pages > kMaxRows / h.page || window > kMaxRows)
+    return QRB200_ERR_ARG;
+  if (batch == 0 || queries == 0 || q_heads == 0) return QRB200_OK;
+  if (!q || !out || !lengths || (max_pages > 0 && !block_table) || (reinterpret_cast<uintptr_t>(cache) & 15u) ||
+      (h.pages > 0 && !cache) || table_stride < 0)
+    return QRB200_ERR_ARG;
+  const int st = quant_ready();
+  if (st != QRB200_OK) return st;
+  Kv4AttnParams p{static_cast<const unsigned char*>(cache), q, out, block_table, lengths, q_strides[0], q_strides[1],
+                  q_strides[2], table_stride, (int)batch, (int)queries, (int)q_heads, (int)max_pages, (int)window,
+                  causal, scale, h};
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const unsigned grid = (unsigned)((batch * queries * q_heads + 3) / 4);
+  const bool bf = shape->dtype == QRB200_BF16;
+  if (h.dim == 128) {
+    if (bf) kv4_attention_simple_kernel<__nv_bfloat16, 4><<<grid, 128, 0, s>>>(p);
+    else kv4_attention_simple_kernel<__half, 4><<<grid, 128, 0, s>>>(p);
+  } else {
+    if (bf) kv4_attention_simple_kernel<__nv_bfloat16, 2><<<grid, 128, 0, s>>>(p);
+    else kv4_attention_simple_kernel<__half, 2><<<grid, 128, 0, s>>>(p);
+  }
+  return launched();
+}
+
+}  // extern "C"

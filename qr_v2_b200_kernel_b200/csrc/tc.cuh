@@ -41,10 +41,11 @@ constexpr int kSiteMbarrier = 1;    // mbarrier wait of a tensor-core kernel (MM
 constexpr int kSiteHandoff = 2;     // hand-off flag of the whole-matrix kernel
 constexpr int kSiteCluster = 3;     // partial-sum exchange of the cluster panel
 constexpr int kSiteSelfTest = 4;    // qrb200_selftest_wait_timeout
+constexpr int kSiteIndex = 5;       // a cache slot, block table entry or length out of range (no wait)
 __device__ int g_device_status = 0;
 __device__ int* g_status_mapped = nullptr;
 
-__device__ __noinline__ void report_device_failure(int site) {
+static __device__ __noinline__ void report_device_failure(int site) {
   atomicExch(&g_device_status, site);
   int* h = g_status_mapped;
   if (h != nullptr) {
