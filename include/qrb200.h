@@ -170,7 +170,8 @@ int qrb200_dequantize_int8(const int8_t* q, int64_t q_stride, const float* scale
                            int64_t cols, int dtype, void* stream);
 
 /* y[i, n] = (sum_k x[i, k] w[n, k]) x_scale[i] w_scale[n] + bias[n]: y rows x outs of dtype,
- * contiguous; bias (may be NULL) of dtype; row strides of x and w in bytes. The sum is exact in
+ * contiguous; bias (may be NULL) of dtype; row strides of x and w in bytes; x, w, y and the
+ * strides (where there is more than one row) multiples of 16 bytes, else QRB200_ERR_ARG. The sum is exact in
  * 32-bit integers for depth <= QRB200_INT8_MAX_DEPTH. */
 #define QRB200_INT8_MAX_DEPTH 131071
 int qrb200_int8_linear(const int8_t* x, int64_t x_stride, const float* x_scale, const int8_t* w, int64_t w_stride,

@@ -5,51 +5,418 @@
 // the result is rounded once.
 #pragma once
 
+#include <cuda.h>
+
 #include "quant_rows.cuh"
+#include "tc.cuh"
 
 namespace qrb200 {
 
 struct I8Params {
-  const int8_t* x;
-  const int8_t* w;
   const float* sx;
   const float* sw;
   const void* bias;  // may be null; y's type
   void* y;
-  long long rows, outs, x_stride, w_stride;
-  int depth;
+  int rows, outs, depth;
+  int tiles_n, tiles;  // wide kernel: channel tiles, all tiles
 };
 
-// 64 x 64 outputs per CTA, 16 threads a side with 4 x 4 outputs each; any alignment.
-template <typename T>
-__global__ void __launch_bounds__(256) i8_linear_simple_kernel(I8Params P) {
-  __shared__ __align__(4) int8_t xs[64][68], ws[64][68];
-  const long long i0 = (long long)blockIdx.y * 64, n0 = (long long)blockIdx.x * 64;
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  int acc[4][4] = {};
-  for (int k0 = 0; k0 < P.depth; k0 += 64) {
-    for (int e = threadIdx.x; e < 64 * 64; e += 256) {
-      const int r = e >> 6, c = e & 63;
-      const bool k = k0 + c < P.depth;
-      xs[r][c] = k && i0 + r < P.rows ? P.x[(i0 + r) * P.x_stride + k0 + c] : 0;
-      ws[r][c] = k && n0 + r < P.outs ? P.w[(n0 + r) * P.w_stride + k0 + c] : 0;
+constexpr int kI8Depth = 128;  // codes of one row per stage: one 128-byte swizzled row
+
+// One box of a 2D tensor map into shared memory, completing on an mbarrier of this CTA.
+__device__ __forceinline__ void i8_load(uint32_t dst, const CUtensorMap* map, uint32_t mbar, int x, int y) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
+          dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(mbar)
+      : "memory");
+}
+__device__ __forceinline__ void i8_expect(uint32_t mbar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(mbar), "r"(bytes) : "memory");
+}
+// Descriptor of a K-major tile of 128-byte rows in the 128-byte swizzle (layout type 2): groups of 8 rows 1024 bytes
+// apart; a step of 32 codes advances the start address by 32 bytes.
+__device__ __forceinline__ uint64_t i8_sdesc(uint32_t saddr) { return make_sdesc(saddr, 16, 1024) | ((uint64_t)2 << 61); }
+// kind::i8: signed 8-bit operands, both K-major, 32-bit integer accumulator.
+__host__ __device__ constexpr uint32_t i8_idesc(int M, int N) {
+  return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
+}
+__device__ __forceinline__ void i8_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}\n"
+      :
+      : "r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate ? 1u : 0u)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, int (&v)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
+        "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+      : "r"(taddr));
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ int ld_cluster(uint32_t addr, uint32_t rank) {
+  uint32_t a;
+  int v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(addr), "r"(rank));
+  asm volatile("ld.shared::cluster.b32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
+  return v;
+}
+
+// ---- few rows ------------------------------------------------------------------------------
+//
+// With few rows the weights are the traffic, so they are the 128-row operand (M = output
+// channels) and the rows of x the narrow one (N = kBN): no tensor-core row is wasted on padding.
+// The depth is cut over the cluster's CTAs so that every SM streams weights, and their integer
+// sums are added through distributed shared memory, exactly, in the one launch.
+//
+// Warp 0 issues the loads, warp 1 the MMAs, warps 2-5 hold one output channel a lane.
+template <int kBN>
+struct I8Few {
+  static constexpr int kStage = 128 * kI8Depth + kBN * kI8Depth;
+  static constexpr int kStages = kBN <= 32 ? 4 : 3;
+  static constexpr int kCols = kBN < 32 ? 32 : kBN;  // TMEM columns
+  static constexpr size_t smem() { return 1024 + (size_t)kStages * kStage; }
+};
+
+template <typename T, int kBN>
+__global__ void __launch_bounds__(192) i8_few_kernel(I8Params P, const __grid_constant__ CUtensorMap tm_w,
+                                                     const __grid_constant__ CUtensorMap tm_x) {
+  using C = I8Few<kBN>;
+  extern __shared__ __align__(1024) unsigned char smem_raw[];
+  __shared__ uint64_t full[C::kStages], empty[C::kStages], done;
+  __shared__ uint32_t s_tmem;
+  __shared__ int s_bad;
+  unsigned char* ring = align1024(smem_raw);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int n0 = blockIdx.x * 128, i0 = blockIdx.y * kBN;
+  const int split = gridDim.z, part = blockIdx.z;
+  const int nk = (P.depth + kI8Depth - 1) / kI8Depth;
+  const int k_lo = (int)((long long)nk * part / split), k_hi = (int)((long long)nk * (part + 1) / split);
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < C::kStages; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
     }
-    __syncthreads();
-    for (int c = 0; c < 64; c += 4)
-      for (int a = 0; a < 4; ++a)
-        for (int b = 0; b < 4; ++b)
-          acc[a][b] = __dp4a(*reinterpret_cast<const int*>(&xs[4 * ty + a][c]),
-                             *reinterpret_cast<const int*>(&ws[tx + 16 * b][c]), acc[a][b]);
-    __syncthreads();
+    mbar_init(&done, 1);
+    s_bad = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    fence_async_smem();
   }
-  for (int a = 0; a < 4; ++a)
-    for (int b = 0; b < 4; ++b) {
-      const long long i = i0 + 4 * ty + a, n = n0 + tx + 16 * b;
-      if (i >= P.rows || n >= P.outs) continue;
-      float v = (float)acc[a][b] * P.sx[i] * P.sw[n];
-      if (P.bias) v += to_f32(static_cast<const T*>(P.bias)[n]);
-      static_cast<T*>(P.y)[i * P.outs + n] = from_f32<T>(v);
+  griddep_launch_wait();  // before TMEM is taken: a kernel still running may need it
+  if (warp == 1) tmem_alloc(&s_tmem, C::kCols);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = s_tmem;
+
+  if (warp == 0 && lane == 0) {
+    int issued = 0;
+    for (int k = k_lo; k < k_hi; ++k, ++issued) {
+      const int s = issued % C::kStages, turn = issued / C::kStages;
+      if (turn > 0 && !mbar_wait(&empty[s], (turn - 1) & 1)) {
+        s_bad = 1;
+        break;
+      }
+      const uint32_t at = smem_u32(ring) + s * C::kStage, bar = smem_u32(&full[s]);
+      i8_expect(bar, C::kStage);
+      i8_load(at, &tm_w, bar, k * kI8Depth, n0);
+      i8_load(at + 128 * kI8Depth, &tm_x, bar, k * kI8Depth, i0);
     }
+    // Whatever happened, no load is in flight when this CTA ends.
+    for (int j = max(0, issued - C::kStages); j < issued; ++j)
+      if (!mbar_wait(&full[j % C::kStages], (j / C::kStages) & 1)) s_bad = 1;
+  } else if (warp == 1 && lane == 0) {
+    constexpr uint32_t idesc = i8_idesc(128, kBN);
+    int j = 0;
+    for (int k = k_lo; k < k_hi; ++k, ++j) {
+      const int s = j % C::kStages;
+      if (!mbar_wait(&full[s], (j / C::kStages) & 1)) {
+        s_bad = 1;
+        break;
+      }
+      tc_fence_after();
+      const uint32_t at = smem_u32(ring) + s * C::kStage;
+#pragma unroll
+      for (int c = 0; c < kI8Depth / 32; ++c)
+        i8_mma(tmem, i8_sdesc(at + 32 * c), i8_sdesc(at + 128 * kI8Depth + 32 * c), idesc, j > 0 || c > 0);
+      mma_commit(&empty[s]);
+    }
+    mma_commit(&done);
+  }
+  __syncwarp();
+  const int ch = ((warp & 3) << 5) + lane;  // the channel, and the TMEM lane, of warps 2-5
+  const bool epi = warp >= 2;
+  const int n = n0 + ch;
+  const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+  float sw = 0.f, b = 0.f;
+  if (epi && n < P.outs) {
+    sw = P.sw[n];
+    if (P.bias) b = to_f32(static_cast<const T*>(P.bias)[n]);
+  }
+  T* y = static_cast<T*>(P.y);
+  auto put = [&](int j, int acc) {
+    if (n < P.outs && i0 + j < P.rows)
+      y[(long long)(i0 + j) * P.outs + n] = from_f32<T>(fmaf((float)acc * P.sx[i0 + j], sw, b));
+  };
+  if (epi && !mbar_wait(&done, 0)) s_bad = 1;
+  tc_fence_after();
+  if (split == 1) {
+    __syncthreads();
+    if (epi && !s_bad)
+#pragma unroll 1
+      for (int j = 0; j < kBN && i0 + j < P.rows; j += 16) {
+        int v[16];
+        tmem_ld16(lanes + j, v);
+#pragma unroll
+        for (int q = 0; q < 16; ++q) put(j + q, v[q]);
+      }
+  } else {
+    // The ring is free: every load has landed and every MMA is done. Sums as [row][channel].
+    int* sums = reinterpret_cast<int*>(ring);
+    if (epi)
+#pragma unroll 1
+      for (int j = 0; j < kBN && i0 + j < P.rows; j += 16) {
+        int v[16];
+        tmem_ld16(lanes + j, v);
+#pragma unroll
+        for (int q = 0; q < 16; ++q) sums[(j + q) * 128 + ch] = v[q];
+      }
+    __syncthreads();
+    cluster_sync();
+    bool bad = false;
+    for (int r = 0; r < split; ++r) bad = ld_cluster(smem_u32(&s_bad), r) != 0 || bad;
+    if (epi && !bad)
+      for (int j = part; j < kBN && i0 + j < P.rows; j += split) {
+        int acc = 0;
+        for (int r = 0; r < split; ++r) acc += ld_cluster(smem_u32(&sums[j * 128 + ch]), r);
+        put(j, acc);
+      }
+    cluster_sync();  // nobody leaves while its sums are being read
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) tmem_dealloc(tmem, C::kCols);
+}
+
+// ---- many rows -----------------------------------------------------------------------------
+//
+// 256 rows x 256 channels per pair of CTAs (cta_group::2: each CTA holds 128 rows of x, 128 of the
+// channels' weights and its rows' 128 x 256 sums), persistent, with two accumulators in TMEM so
+// that a tile's epilogue runs under the next tile's products. Warp 0 loads its CTA's halves, warp
+// 1 of the pair's first CTA issues the MMAs, warps 4-7 scale, round and store.
+constexpr int kI8WideStage = 2 * 128 * kI8Depth;  // bytes per CTA and stage
+constexpr int kI8WideStages = 5;
+constexpr int kI8Pitch = 144;  // bytes of a staged output row (128 and 16 to spread the banks)
+constexpr size_t i8_wide_smem() { return 1024 + (size_t)kI8WideStages * kI8WideStage + 4 * 32 * kI8Pitch; }
+
+__device__ __forceinline__ uint32_t pair_leader(uint32_t addr) {  // the same address in the pair's first CTA
+  uint32_t a;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(a) : "r"(addr));
+  return a;
+}
+__device__ __forceinline__ void i8_load_pair(uint32_t dst, const CUtensorMap* map, uint32_t leader_bar, int x, int y) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], "
+      "[%4];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(leader_bar)
+      : "memory");
+}
+__device__ __forceinline__ void i8_mma_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}\n"
+      :
+      : "r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate ? 1u : 0u)
+      : "memory");
+}
+__device__ __forceinline__ void commit_pair(uint64_t* mbar) {  // arrives on this barrier of both CTAs
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
+      :
+      : "r"(smem_u32(mbar)), "h"((uint16_t)3)
+      : "memory");
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256, 1) __cluster_dims__(2, 1, 1)
+    i8_wide_kernel(I8Params P, const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w) {
+  extern __shared__ __align__(1024) unsigned char smem_raw[];
+  __shared__ uint64_t full[kI8WideStages], empty[kI8WideStages], acc_full[2], acc_empty[2];
+  __shared__ uint32_t s_tmem;
+  __shared__ __align__(16) float s_sw[256], s_b[256];
+  unsigned char* ring = align1024(smem_raw);
+  unsigned char* staged = ring + kI8WideStages * kI8WideStage;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_rank();
+  const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+  const int nk = (P.depth + kI8Depth - 1) / kI8Depth;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kI8WideStages; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&acc_full[s], 1);
+      mbar_init(&acc_empty[s], 8);  // the four epilogue warps of both CTAs
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    fence_async_smem();
+  }
+  griddep_launch_wait();  // before TMEM is taken: a kernel still running may need it
+  if (warp == 2) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&s_tmem)) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();  // both CTAs' barriers are initialised
+  tc_fence_after();
+  const uint32_t tmem = s_tmem;
+  // Tiles run down the rows within bands of kBand channel tiles, so that the tiles in flight share both operands in L2.
+  constexpr int kBand = 8;
+  const int tiles_m = P.tiles / P.tiles_n;
+  auto place = [&](int tile, int& m, int& n) {
+    const int band = tile / (kBand * tiles_m), in = tile - band * kBand * tiles_m;
+    const int width = min(kBand, P.tiles_n - band * kBand);
+    m = in / width;
+    n = band * kBand + in % width;
+  };
+
+  if (warp == 0 && lane == 0) {
+    int issued = 0;
+    bool ok = true;
+    for (int tile = pair; tile < P.tiles && ok; tile += pairs) {
+      int m, n;
+      place(tile, m, n);
+      for (int k = 0; k < nk; ++k, ++issued) {
+        const int s = issued % kI8WideStages, turn = issued / kI8WideStages;
+        if (turn > 0 && !mbar_wait(&empty[s], (turn - 1) & 1)) {
+          ok = false;
+          break;
+        }
+        const uint32_t at = smem_u32(ring) + s * kI8WideStage, bar = pair_leader(smem_u32(&full[s]));
+        if (rank == 0) i8_expect(smem_u32(&full[s]), 2 * kI8WideStage);
+        i8_load_pair(at, &tm_x, bar, k * kI8Depth, m * 256 + (int)rank * 128);
+        i8_load_pair(at + 128 * kI8Depth, &tm_w, bar, k * kI8Depth, n * 256 + (int)rank * 128);
+      }
+    }
+    // No load is in flight when the pair ends: the loads of both CTAs land on the leader's
+    // barriers, and `empty` says that the last use of each stage is over.
+    for (int j = max(0, issued - kI8WideStages); j < issued; ++j)
+      mbar_wait(&empty[j % kI8WideStages], (j / kI8WideStages) & 1);
+  } else if (warp == 1 && lane == 0 && rank == 0) {
+    constexpr uint32_t idesc = i8_idesc(256, 256);
+    int j = 0, t = 0;
+    bool ok = true;
+    for (int tile = pair; tile < P.tiles && ok; tile += pairs, ++t) {
+      const int buf = t & 1;
+      if (t >= 2 && !mbar_wait(&acc_empty[buf], ((t >> 1) - 1) & 1)) break;
+      tc_fence_after();
+      for (int k = 0; k < nk; ++k, ++j) {
+        const int s = j % kI8WideStages;
+        if (!mbar_wait(&full[s], (j / kI8WideStages) & 1)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const uint32_t at = smem_u32(ring) + s * kI8WideStage;
+#pragma unroll
+        for (int c = 0; c < kI8Depth / 32; ++c)
+          i8_mma_pair(tmem + buf * 256, i8_sdesc(at + 32 * c), i8_sdesc(at + 128 * kI8Depth + 32 * c), idesc,
+                      k > 0 || c > 0);
+        commit_pair(&empty[s]);
+      }
+      if (ok) commit_pair(&acc_full[buf]);
+    }
+  } else if (warp >= 4) {
+    constexpr int kPer = 128 / sizeof(T);  // outputs in a staged row of 128 bytes
+    const int ew = warp - 4, et = threadIdx.x - 128;
+    unsigned char* mine = staged + ew * 32 * kI8Pitch;
+    const uint32_t lanes = tmem + ((uint32_t)(ew * 32) << 16);
+    const bool wide = P.outs % (16 / (int)sizeof(T)) == 0;  // 16-byte rows of y (y itself is 16-byte aligned)
+    T* y = static_cast<T*>(P.y);
+    int t = 0;
+    bool bad = false;  // a wait ran out: keep to the barriers, touch nothing
+    for (int tile = pair; tile < P.tiles; tile += pairs, ++t) {
+      int m, n;
+      place(tile, m, n);
+      const int n0 = n * 256, row0 = m * 256 + (int)rank * 128 + ew * 32;
+      asm volatile("bar.sync 1, 128;" ::: "memory");  // the last tile's scales have been read
+      for (int c = et; c < 256; c += 128) {
+        const bool in = n0 + c < P.outs;
+        s_sw[c] = in ? P.sw[n0 + c] : 0.f;
+        s_b[c] = in && P.bias ? to_f32(static_cast<const T*>(P.bias)[n0 + c]) : 0.f;
+      }
+      asm volatile("bar.sync 1, 128;" ::: "memory");
+      const float sx = row0 + lane < P.rows ? P.sx[row0 + lane] : 0.f;
+      bad = bad || !__all_sync(kFullMask, mbar_wait(&acc_full[t & 1], (t >> 1) & 1));
+      tc_fence_after();
+      if (bad) continue;
+#pragma unroll 1
+      for (int c0 = 0; c0 < 256; c0 += kPer) {
+        __syncwarp();
+#pragma unroll
+        for (int h = 0; h < kPer; h += 16) {
+          int v[16];
+          tmem_ld16(lanes + (t & 1) * 256 + c0 + h, v);
+          T out[16];
+#pragma unroll
+          for (int q = 0; q < 16; q += 4) {
+            const float4 w4 = *reinterpret_cast<const float4*>(&s_sw[c0 + h + q]);
+            const float4 b4 = *reinterpret_cast<const float4*>(&s_b[c0 + h + q]);
+            out[q] = from_f32<T>(fmaf((float)v[q] * sx, w4.x, b4.x));
+            out[q + 1] = from_f32<T>(fmaf((float)v[q + 1] * sx, w4.y, b4.y));
+            out[q + 2] = from_f32<T>(fmaf((float)v[q + 2] * sx, w4.z, b4.z));
+            out[q + 3] = from_f32<T>(fmaf((float)v[q + 3] * sx, w4.w, b4.w));
+          }
+#pragma unroll
+          for (int q = 0; q < 16 * (int)sizeof(T) / 16; ++q)
+            *reinterpret_cast<uint4*>(mine + lane * kI8Pitch + h * sizeof(T) + 16 * q) = reinterpret_cast<uint4*>(out)[q];
+        }
+        if (c0 + kPer >= 256) {  // every sum of this warp is in registers: the accumulator is free
+          tc_fence_before();
+          if (lane == 0)
+            asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(
+                             pair_leader(smem_u32(&acc_empty[t & 1])))
+                         : "memory");
+        }
+        __syncwarp();
+        const int left = P.outs - n0 - c0;  // columns of this chunk that exist
+        if (left <= 0) continue;
+        if (wide) {
+          const int piece = lane & 7, col = piece * (16 / (int)sizeof(T));
+#pragma unroll
+          for (int r = lane >> 3; r < 32; r += 4)
+            if (row0 + r < P.rows && col < left)
+              *reinterpret_cast<uint4*>(y + (long long)(row0 + r) * P.outs + n0 + c0 + col) =
+                  *reinterpret_cast<const uint4*>(mine + r * kI8Pitch + 16 * piece);
+        } else {
+          for (int r = 0; r < 32 && row0 + r < P.rows; ++r)
+            for (int c = lane; c < min(kPer, left); c += 32)
+              y[(long long)(row0 + r) * P.outs + n0 + c0 + c] = reinterpret_cast<const T*>(mine + r * kI8Pitch)[c];
+        }
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();  // the pair's products, loads and arrivals are over in both CTAs
+  if (warp == 2) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
 }
 
 }  // namespace qrb200

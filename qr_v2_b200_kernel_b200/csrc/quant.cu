@@ -60,6 +60,131 @@ static int rows_int8(const RowsParams& p, int weight_type, int dtype, cudaStream
   }
 }
 
+static PFN_cuTensorMapEncodeTiled_v12000 map_encoder() {
+  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q{};
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
+  });
+  return fn;
+}
+
+struct I8Operand {
+  const int8_t* base;
+  uint64_t rows, stride;
+};
+
+// Boxes of 128 codes x `box_rows` rows, 128-byte swizzle; what lies outside the operand reads as zero.
+static bool encode_codes(CUtensorMap* map, const I8Operand& o, uint64_t depth, uint32_t box_rows) {
+  const PFN_cuTensorMapEncodeTiled_v12000 fn = map_encoder();
+  if (fn == nullptr) return false;
+  const cuuint64_t dims[2] = {depth, o.rows};
+  const cuuint64_t strides[1] = {o.rows > 1 ? o.stride : (depth + 15) / 16 * 16};
+  const cuuint32_t box[2] = {(cuuint32_t)kI8Depth, box_rows};
+  const cuuint32_t estr[2] = {1, 1};
+  return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<int8_t*>(o.base), dims, strides, box, estr,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+struct LaunchShape {
+  cudaLaunchConfig_t cfg{};
+  cudaLaunchAttribute attr[2];
+  // A kernel that begins with griddep_launch_wait() may be set up while its predecessor ends.
+  LaunchShape(dim3 grid, unsigned threads, size_t smem, cudaStream_t s, unsigned cluster_z = 0) {
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.numAttrs = 1;
+    if (cluster_z > 1) {
+      attr[1].id = cudaLaunchAttributeClusterDimension;
+      attr[1].val.clusterDim.x = 1;
+      attr[1].val.clusterDim.y = 1;
+      attr[1].val.clusterDim.z = cluster_z;
+      cfg.numAttrs = 2;
+    }
+    cfg.attrs = attr;
+  }
+};
+
+// Whether a one-time set-up of a kernel has been done on the current device; the caller marks it.
+struct OncePerDevice {
+  std::atomic<unsigned long long> bits{0};
+  template <typename F>
+  cudaError_t run(F&& set_up) {
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (dev < 64 && ((bits.load(std::memory_order_acquire) >> dev) & 1ull)) return cudaSuccess;
+    const cudaError_t e = set_up();
+    if (e == cudaSuccess && dev < 64) bits.fetch_or(1ull << dev, std::memory_order_acq_rel);
+    return e;
+  }
+};
+
+static int sm_count() {
+  static std::atomic<int> sms[64];
+  int dev = 0, n = 0;
+  cudaGetDevice(&dev);
+  if (dev < 64 && (n = sms[dev].load(std::memory_order_relaxed)) > 0) return n;
+  cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
+  if (dev < 64) sms[dev].store(n, std::memory_order_relaxed);
+  return n;
+}
+
+static int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
+
+template <typename T, int kBN>
+static cudaError_t launch_i8_few(const I8Params& p, const I8Operand& x, const I8Operand& w, cudaStream_t s) {
+  using C = I8Few<kBN>;
+  static OncePerDevice once;
+  const cudaError_t e = once.run([] {
+    return cudaFuncSetAttribute(i8_few_kernel<T, kBN>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::smem());
+  });
+  if (e != cudaSuccess) return e;
+  CUtensorMap tw, tx;
+  if (!encode_codes(&tw, w, p.depth, 128) || !encode_codes(&tx, x, p.depth, kBN)) return cudaErrorInvalidValue;
+  const int tn = ceil_div(p.outs, 128), tm = ceil_div(p.rows, kBN), nk = ceil_div(p.depth, kI8Depth);
+  if (tm > 65535) return cudaErrorInvalidValue;
+  unsigned split = 1;
+  while (split < 8 && 2 * split <= (unsigned)nk && (int64_t)tn * tm * split < sm_count()) split *= 2;
+  LaunchShape l(dim3(tn, tm, split), 192, C::smem(), s, split);
+  return cudaLaunchKernelEx(&l.cfg, i8_few_kernel<T, kBN>, p, tw, tx);
+}
+
+template <typename T>
+static cudaError_t launch_i8_wide(I8Params p, const I8Operand& x, const I8Operand& w, cudaStream_t s) {
+  static OncePerDevice once;
+  const cudaError_t e = once.run([] {
+    return cudaFuncSetAttribute(i8_wide_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)i8_wide_smem());
+  });
+  if (e != cudaSuccess) return e;
+  CUtensorMap tw, tx;
+  if (!encode_codes(&tw, w, p.depth, 128) || !encode_codes(&tx, x, p.depth, 128)) return cudaErrorInvalidValue;
+  p.tiles_n = ceil_div(p.outs, 256);
+  const int64_t tiles = (int64_t)p.tiles_n * ceil_div(p.rows, 256);
+  if (tiles > (1 << 30)) return cudaErrorInvalidValue;
+  p.tiles = (int)tiles;
+  const int pairs = std::min(p.tiles, sm_count() / 2);
+  LaunchShape l(dim3(2 * pairs), 256, i8_wide_smem(), s);
+  return cudaLaunchKernelEx(&l.cfg, i8_wide_kernel<T>, p, tx, tw);
+}
+
+template <typename T>
+static cudaError_t launch_i8(const I8Params& p, const I8Operand& x, const I8Operand& w, cudaStream_t s) {
+  if (p.rows <= 16) return launch_i8_few<T, 16>(p, x, w, s);
+  if (p.rows <= 32) return launch_i8_few<T, 32>(p, x, w, s);
+  if (p.rows <= 64) return launch_i8_few<T, 64>(p, x, w, s);
+  if ((int64_t)ceil_div(p.rows, 256) * ceil_div(p.outs, 256) < sm_count() / 4) return launch_i8_few<T, 128>(p, x, w, s);
+  return launch_i8_wide<T>(p, x, w, s);
+}
+
 static bool shape_ok(const Kv4Shape& h) {
   return h.pages >= 0 && h.pages <= (1ll << 31) - 1 && h.heads > 0 && h.heads <= 65535 && (h.dim == 64 || h.dim == 128) &&
          h.page >= 16 && h.page <= 1024 && (h.page & (h.page - 1)) == 0 && h.groups > 0 && h.dim % h.groups == 0 &&
@@ -127,22 +252,24 @@ int qrb200_int8_linear(const int8_t* x, int64_t x_stride, const float* x_scale, 
                        const float* w_scale, const void* bias, void* y, int64_t rows, int64_t outs, int64_t depth,
                        int dtype, void* stream) {
   if (rows < 0 || outs < 0 || depth <= 0 || depth > QRB200_INT8_MAX_DEPTH || !type_ok(dtype)) return QRB200_ERR_ARG;
-  if (rows > kMaxRows || outs > kMaxRows) return QRB200_ERR_ARG;
+  if (rows > kMaxRows / 2 || outs > kMaxRows / 2) return QRB200_ERR_ARG;
   if (rows == 0 || outs == 0) return QRB200_OK;
   if (!x || !w || !x_scale || !w_scale || !y) return QRB200_ERR_ARG;
   if ((rows > 1 && x_stride < depth) || (outs > 1 && w_stride < depth)) return QRB200_ERR_ARG;
+  const auto off16 = [](const void* p, int64_t stride, int64_t n) {
+    return (reinterpret_cast<uintptr_t>(p) & 15u) || (n > 1 && stride % 16);
+  };
+  if (off16(x, x_stride, rows) || off16(w, w_stride, outs) || off16(y, 0, 1)) return QRB200_ERR_ARG;
   const int st = quant_ready();
   if (st != QRB200_OK) return st;
-  I8Params p{x, w, x_scale, w_scale, bias, y, rows, outs, x_stride, w_stride, (int)depth};
+  const I8Params p{x_scale, w_scale, bias, y, (int)rows, (int)outs, (int)depth, 0, 0};
+  const I8Operand xo{x, (uint64_t)rows, (uint64_t)x_stride}, wo{w, (uint64_t)outs, (uint64_t)w_stride};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const dim3 grid((unsigned)((outs + 63) / 64), (unsigned)((rows + 63) / 64));
-  if (grid.y > 65535) return QRB200_ERR_ARG;
-  if (dtype == QRB200_BF16)
-    i8_linear_simple_kernel<__nv_bfloat16><<<grid, 256, 0, s>>>(p);
-  else if (dtype == QRB200_F16)
-    i8_linear_simple_kernel<__half><<<grid, 256, 0, s>>>(p);
-  else
-    i8_linear_simple_kernel<float><<<grid, 256, 0, s>>>(p);
+  cudaError_t e;
+  if (dtype == QRB200_BF16) e = launch_i8<__nv_bfloat16>(p, xo, wo, s);
+  else if (dtype == QRB200_F16) e = launch_i8<__half>(p, xo, wo, s);
+  else e = launch_i8<float>(p, xo, wo, s);
+  if (e != cudaSuccess) return QRB200_ERR_CUDA;
   return launched();
 }
 

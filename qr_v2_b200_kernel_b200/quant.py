@@ -68,6 +68,13 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
     return r
 
 
+def _loadable(t: torch.Tensor) -> torch.Tensor:
+    """8-bit rows as the tensor-core product loads them: from 16-byte boundaries, copied only where they are not."""
+    if t.data_ptr() % 16 == 0 and (t.stride(0) % 16 == 0 or t.shape[0] == 1):
+        return t
+    return _codes(t.shape[0], t.shape[1], t).copy_(t)
+
+
 def _codes(rows: int, cols: int, like: torch.Tensor) -> torch.Tensor:
     """An int8 (rows, cols) tensor whose rows start on 16-byte boundaries, as the tensor-core product loads them."""
     padded = -(-cols // 16) * 16
@@ -171,7 +178,7 @@ def int8_linear(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor, we
     ``x`` int8 (..., depth) with a float32 scale for each row (token), ``weight`` int8 (outs, depth) with a
     float32 scale for each output channel, as :func:`rms_norm_int8` and :func:`quantize_int8` make them;
     ``bias`` (outs,) of ``dtype``. 1 <= depth <= 131071. The products are summed exactly, in 32-bit integers, and the
-    result is rounded once.
+    result is rounded once. Operands whose rows do not start on 16-byte boundaries are copied first.
     """
     _operand(x, "x", (torch.int8,))
     _operand(weight, "weight", (torch.int8,), x)
@@ -198,6 +205,7 @@ def int8_linear(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor, we
     y = torch.empty((*x.shape[:-1], outs), dtype=dtype, device=x.device)
     if rows == 0 or outs == 0:
         return y
+    xr, wr = _loadable(xr), _loadable(wr)
     x_scale, weight_scale = x_scale.contiguous(), weight_scale.contiguous()
     _call("int8_linear", x, _lib.load().qrb200_int8_linear, xr.data_ptr(), xr.stride(0), x_scale.data_ptr(),
           wr.data_ptr(), wr.stride(0), weight_scale.data_ptr(), bias.data_ptr() if bias is not None else None,
