@@ -166,66 +166,4 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(Kv4IoParams P) {
   static_cast<T*>(P.v_out)[e] = from_f32<T>(out[1]);
 }
 
-struct Kv4AttnParams {
-  const unsigned char* cache;
-  const void* q;
-  void* out;
-  const int* table;
-  const int* lengths;
-  long long q_bs, q_ts, q_hs, table_stride;  // strides in elements
-  int batch, queries, q_heads, max_pages, window, causal;
-  float scale;
-  Kv4Shape sh;
-};
-
-// One warp per query row: lanes hold kN channels each and walk the visible tokens with a running
-// maximum and sum. The simplest form.
-template <typename T, int kN>
-__global__ void __launch_bounds__(128) kv4_attention_simple_kernel(Kv4AttnParams P) {
-  const int lane = threadIdx.x & 31;
-  const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
-  if (row >= (long long)P.batch * P.queries * P.q_heads) return;
-  const int qh = (int)(row % P.q_heads), qi = (int)(row / P.q_heads % P.queries), b = (int)(row / P.q_heads / P.queries);
-  const int head = qh / (P.q_heads / P.sh.heads), dim = P.sh.dim;
-  int len = P.lengths[b];
-  if (len < 0 || len > (long long)P.max_pages * P.sh.page) {
-    if (lane == 0) report_device_failure(kSiteIndex);
-    len = 0;
-  }
-  const int pos = P.causal ? len - P.queries + qi : len - 1;
-  const int first = P.window > 0 ? max(0, len - P.queries + qi - P.window + 1) : 0;
-  const T* q = static_cast<const T*>(P.q) + b * P.q_bs + qi * P.q_ts + qh * P.q_hs;
-  float qv[kN], acc[kN] = {}, top = __int_as_float(0xff800000), sum = 0.f;
-  for (int i = 0; i < kN; ++i) qv[i] = to_f32(q[lane * kN + i]) * P.scale;
-  for (int tok = first; tok <= pos; ++tok) {
-    const int page = P.table[b * P.table_stride + tok / P.sh.page], at = tok % P.sh.page;
-    if (page < 0 || page >= P.sh.pages) {
-      if (lane == 0) report_device_failure(kSiteIndex);
-      continue;
-    }
-    const unsigned char* block = P.cache + ((long long)page * P.sh.heads + head) * P.sh.block_bytes();
-    float x[2][kN];
-    for (int part = 0; part < 2; ++part)
-      for (int i = 0; i < kN; ++i) {
-        const int d = lane * kN + i;
-        int shift;
-        const int byte = part ? kv4_value_byte(dim, at, d, &shift) : kv4_key_byte(dim, at, d, &shift);
-        const int code = (block[(part ? P.sh.v_codes() : 0) + byte] >> shift) & 15;
-        const Pair16<T> pr = reinterpret_cast<const Pair16<T>*>(
-            block + (part ? P.sh.v_pairs() : P.sh.k_pairs()))[at * P.sh.groups + d / (dim / P.sh.groups)];
-        x[part][i] = fmaf(to_f32(pr.s), (float)code, to_f32(pr.m));
-      }
-    float score = 0.f;
-    for (int i = 0; i < kN; ++i) score = fmaf(qv[i], x[0][i], score);
-    for (int o = 16; o; o >>= 1) score += __shfl_xor_sync(kFullMask, score, o);
-    const float up = fmaxf(top, score);
-    const float keep = __expf(top - up), p = __expf(score - up);
-    sum = fmaf(sum, keep, p);
-    for (int i = 0; i < kN; ++i) acc[i] = fmaf(acc[i], keep, p * x[1][i]);
-    top = up;
-  }
-  T* out = static_cast<T*>(P.out) + row * dim;
-  for (int i = 0; i < kN; ++i) out[lane * kN + i] = from_f32<T>(pos >= first ? acc[i] / sum : 0.f);
-}
-
 }  // namespace qrb200

@@ -11,7 +11,7 @@
 #include "internal.h"
 #include "qrb200.h"
 #include "i8_linear.cuh"
-#include "kv4.cuh"
+#include "kv4_attention.cuh"
 #include "quant_rows.cuh"
 
 namespace qrb200 {
@@ -191,6 +191,45 @@ static bool shape_ok(const Kv4Shape& h) {
          (h.dim / h.groups == 32 || h.dim / h.groups == 64 || h.dim / h.groups == 128);
 }
 
+// How an attention call is cut: query rows per tile, and the token range over `splits` CTAs.
+struct AttnPlan {
+  int tile_rows, tiles, splits;
+  size_t bytes;  // workspace: the parts and their (maximum, sum) pairs
+};
+
+// Eight rows a tile where a key head has no more than eight query rows, else sixteen. The token range is cut until the
+// GPU is full (three CTAs of four warps per SM), each warp keeping at least one step.
+static AttnPlan attn_plan(const Kv4Shape& h, int64_t batch, int64_t queries, int64_t q_heads, int64_t max_pages) {
+  AttnPlan p{};
+  const int64_t rows = queries * (q_heads / h.heads);
+  p.tile_rows = rows <= 8 ? 8 : 16;
+  p.tiles = ceil_div(rows, p.tile_rows);
+  const int64_t ctas = batch * h.heads * p.tiles, units = (max_pages * h.page + 16 * kv_runs(h.dim) - 1) / (16 * kv_runs(h.dim));
+  const int64_t want = (3 * (int64_t)sm_count() + ctas - 1) / ctas;
+  p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({want, (units + kKvWarps - 1) / kKvWarps, 128}));
+  if (p.splits > 1) p.bytes = (size_t)(ctas * p.splits * p.tile_rows) * (h.dim * sizeof(float) + sizeof(float2));
+  return p;
+}
+
+template <typename T, int kDim, int kGroups>
+static cudaError_t launch_attention(Kv4AttnParams p, const AttnPlan& plan, cudaStream_t s) {
+  const dim3 grid(plan.splits, p.sh.heads * plan.tiles, p.batch);
+  LaunchShape l(grid, 32 * kKvWarps, 0, s);
+  const cudaError_t e = plan.tile_rows == 8 ? cudaLaunchKernelEx(&l.cfg, kv4_attention_kernel<T, kDim, kGroups, 1>, p)
+                                            : cudaLaunchKernelEx(&l.cfg, kv4_attention_kernel<T, kDim, kGroups, 2>, p);
+  if (e != cudaSuccess || plan.splits == 1) return e;
+  qrb200_internal_count_launch();
+  LaunchShape j(dim3(ceil_div((int64_t)p.batch * p.queries * p.q_heads, 4)), 128, 0, s);
+  return cudaLaunchKernelEx(&j.cfg, kv4_join_kernel<T, kDim>, p, plan.tile_rows);
+}
+
+template <typename T>
+static cudaError_t launch_attention_of(const Kv4AttnParams& p, const AttnPlan& plan, cudaStream_t s) {
+  if (p.sh.dim == 64) return p.sh.groups == 1 ? launch_attention<T, 64, 1>(p, plan, s) : launch_attention<T, 64, 2>(p, plan, s);
+  if (p.sh.groups == 1) return launch_attention<T, 128, 1>(p, plan, s);
+  return p.sh.groups == 2 ? launch_attention<T, 128, 2>(p, plan, s) : launch_attention<T, 128, 4>(p, plan, s);
+}
+
 }  // namespace qrb200
 
 using namespace qrb200;
@@ -322,23 +361,29 @@ int qrb200_kv4_read(const void* cache, const qrb200_kv4_shape* shape, void* k, v
   return launched();
 }
 
+// The launch grid is splits x (key heads x row tiles) x batch.
+static bool attention_args(const qrb200_kv4_shape* shape, int64_t batch, int64_t queries, int64_t q_heads,
+                           int64_t max_pages, Kv4Shape* h) {
+  if (!shape || batch < 0 || queries < 0 || q_heads < 0 || max_pages < 0 || !type16_ok(shape->dtype)) return false;
+  *h = Kv4Shape{shape->kv_heads, shape->page_size, shape->head_dim, shape->groups, shape->pages};
+  return shape_ok(*h) && q_heads % h->heads == 0 && batch <= 65535 && q_heads <= 65535 && queries <= (1 << 24) &&
+         queries * (q_heads / h->heads) <= (1 << 24) && (queries * (q_heads / h->heads) + 15) / 16 * h->heads <= 65535 &&
+         batch * queries * q_heads <= kMaxRows && max_pages <= kMaxRows / h->page - 64 * (kKvWarps + 1);
+}
+
 size_t qrb200_kv4_attention_workspace_bytes(const qrb200_kv4_shape* shape, int64_t batch, int64_t queries,
                                             int64_t q_heads, int64_t max_pages) {
-  (void)shape, (void)batch, (void)queries, (void)q_heads, (void)max_pages;
-  return 0;
+  Kv4Shape h;
+  if (!attention_args(shape, batch, queries, q_heads, max_pages, &h) || batch * queries * q_heads == 0) return 0;
+  return attn_plan(h, batch, queries, q_heads, max_pages).bytes;
 }
 
 int qrb200_kv4_attention(const void* q, const int64_t* q_strides, const void* cache, const qrb200_kv4_shape* shape,
                          const int32_t* block_table, int64_t table_stride, const int32_t* lengths, void* out,
                          int64_t batch, int64_t queries, int64_t q_heads, int64_t max_pages, int64_t window,
                          int causal, float scale, void* workspace, size_t workspace_bytes, void* stream) {
-  (void)workspace, (void)workspace_bytes;
-  if (!shape || !q_strides || batch < 0 || queries < 0 || q_heads < 0 || max_pages < 0 || window < 0 ||
-      !type16_ok(shape->dtype))
-    return QRB200_ERR_ARG;
-  const Kv4Shape h{shape->kv_heads, shape->page_size, shape->head_dim, shape->groups, shape->pages};
-  if (!shape_ok(h) || q_heads % h.heads != 0 || batch > 65535 || queries > kMaxRows || q_heads > 65535 ||
-      batch * queries > kMaxRows / std::max<int64_t>(1, q_heads) || max_pages > kMaxRows / h.page || window > kMaxRows)
+  Kv4Shape h;
+  if (!q_strides || window < 0 || window > kMaxRows || !attention_args(shape, batch, queries, q_heads, max_pages, &h))
     return QRB200_ERR_ARG;
   if (batch == 0 || queries == 0 || q_heads == 0) return QRB200_OK;
   if (!q || !out || !lengths || (max_pages > 0 && !block_table) || (reinterpret_cast<uintptr_t>(cache) & 15u) ||
@@ -346,19 +391,27 @@ int qrb200_kv4_attention(const void* q, const int64_t* q_strides, const void* ca
     return QRB200_ERR_ARG;
   const int st = quant_ready();
   if (st != QRB200_OK) return st;
-  Kv4AttnParams p{static_cast<const unsigned char*>(cache), q, out, block_table, lengths, q_strides[0], q_strides[1],
-                  q_strides[2], table_stride, (int)batch, (int)queries, (int)q_heads, (int)max_pages, (int)window,
-                  causal, scale, h};
+  const AttnPlan plan = attn_plan(h, batch, queries, q_heads, max_pages);
+  if (plan.bytes > 0 && (!workspace || workspace_bytes < plan.bytes || (reinterpret_cast<uintptr_t>(workspace) & 255u)))
+    return QRB200_ERR_WORKSPACE;
+  Kv4AttnParams p{};
+  p.cache = static_cast<const unsigned char*>(cache);
+  p.q = q;
+  p.out = out;
+  p.part_o = static_cast<float*>(workspace);
+  p.table = block_table;
+  p.lengths = lengths;
+  p.q_bs = q_strides[0], p.q_ts = q_strides[1], p.q_hs = q_strides[2], p.table_stride = table_stride;
+  p.batch = (int)batch, p.queries = (int)queries, p.q_heads = (int)q_heads, p.share = (int)(q_heads / h.heads);
+  p.max_pages = (int)max_pages, p.window = (int)window, p.causal = causal, p.splits = plan.splits, p.tiles = plan.tiles;
+  p.scale2 = scale * 1.4426950408889634f;
+  p.sh = h;
+  if (plan.splits > 1)
+    p.part_ml = reinterpret_cast<float2*>(p.part_o + batch * h.heads * plan.tiles * plan.splits * plan.tile_rows * h.dim);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const unsigned grid = (unsigned)((batch * queries * q_heads + 3) / 4);
-  const bool bf = shape->dtype == QRB200_BF16;
-  if (h.dim == 128) {
-    if (bf) kv4_attention_simple_kernel<__nv_bfloat16, 4><<<grid, 128, 0, s>>>(p);
-    else kv4_attention_simple_kernel<__half, 4><<<grid, 128, 0, s>>>(p);
-  } else {
-    if (bf) kv4_attention_simple_kernel<__nv_bfloat16, 2><<<grid, 128, 0, s>>>(p);
-    else kv4_attention_simple_kernel<__half, 2><<<grid, 128, 0, s>>>(p);
-  }
+  const cudaError_t e = shape->dtype == QRB200_BF16 ? launch_attention_of<__nv_bfloat16>(p, plan, s)
+                                                    : launch_attention_of<__half>(p, plan, s);
+  if (e != cudaSuccess) return QRB200_ERR_CUDA;
   return launched();
 }
 
