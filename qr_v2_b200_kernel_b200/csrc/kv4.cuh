@@ -8,16 +8,17 @@
 // reader sees what the writer meant. s < 2^-126 has no reciprocal: codes 0. A group that holds a
 // NaN or an infinity reads back as NaN.
 //
-// Layout. One block per (page, head), P tokens of D channels, NG = D / G groups:
-//   [key codes P D/2 B][value codes P D/2 B][key (s, m) P NG 4 B][value (s, m) P NG 4 B]
+// Layout. One block per (page, head): P / 16 runs of 16 tokens, D channels, NG = D / G groups. A run is
+//   [key codes 8 D B][value codes 8 D B][key (s, m) 64 NG B][value (s, m) 64 NG B]
+// so that a run's loads share one address, and what is read together lies together (a multiple of 128 bytes).
 // The codes lie the way the 16 x 8 x 16 matrix instruction's left operand wants them, so that
 // the attention loads them straight into registers, 16 bytes at a time, and no shared memory or
 // transposition stands between the cache and the product. Lane (g, t) = (lane / 4, lane % 4) of
 // that operand holds rows g and g + 8, columns {2t, 2t+1, 2t+8, 2t+9}:
 //   keys: rows are tokens, columns channels (their order is free: queries are permuted alike).
-//     A token's D/2 bytes are four runs, one for each t; word w of a run holds the steps
+//     A token's D/2 bytes are four parts, one for each t; word w of a part holds the steps
 //     j = 2w, 2w + 1, channels 16 j + 4 t + e, e = 0..3, at nibble 2 (j & 1) + (e >> 1) + 4 (e & 1);
-//   values: rows are channels, columns tokens. Each 16 tokens are D/16 tiles of 32 words, one for
+//   values: rows are channels, columns tokens. The run is D/16 tiles of 32 words, one for
 //     each lane, stored as [tile / 4][lane][tile % 4]; word bytes 0, 2, 1, 3 are tokens 2t, 2t+1,
 //     2t+8, 2t+9, low nibble channel 16 tile + g, high nibble + 8. A byte belongs to one token:
 //     tokens written at the same time by different threads never share one.
@@ -31,26 +32,9 @@ namespace qrb200 {
 struct Kv4Shape {
   int heads, page, dim, groups;  // groups per head
   long long pages;
-  __host__ __device__ int block_bytes() const { return page * (dim + 8 * groups); }
-  __host__ __device__ int v_codes() const { return page * dim / 2; }
-  __host__ __device__ int k_pairs() const { return page * dim; }
-  __host__ __device__ int v_pairs() const { return page * (dim + 4 * groups); }
+  __host__ __device__ int run_bytes() const { return 16 * dim + 128 * groups; }
+  __host__ __device__ int block_bytes() const { return page / 16 * run_bytes(); }
 };
-
-// Byte and shift of a key's and a value's code inside its block's code section.
-__device__ __forceinline__ int kv4_key_byte(int dim, int tok, int d, int* shift) {
-  const int j = d >> 4, t = (d >> 2) & 3, e = d & 3;
-  const int nib = 2 * (j & 1) + (e >> 1) + 4 * (e & 1);
-  *shift = 4 * (nib & 1);
-  return tok * (dim / 2) + t * (dim / 8) + (j >> 1) * 4 + (nib >> 1);
-}
-__device__ __forceinline__ int kv4_value_byte(int dim, int tok, int d, int* shift) {
-  const int kk = tok & 15, tile = d >> 4, r = d & 15;
-  const int lane = (r & 7) * 4 + ((kk & 7) >> 1);
-  const int byte = 2 * (kk & 1) + (kk >> 3);
-  *shift = 4 * (r >> 3);
-  return (tok >> 4) * 8 * dim + (tile >> 2) * 512 + lane * 16 + (tile & 3) * 4 + byte;
-}
 
 template <typename T>
 struct Pair16 {
@@ -68,37 +52,56 @@ struct Kv4IoParams {
   Kv4Shape sh;
 };
 
-// One warp quantises one token's key or value of one head: kN = D / 32 channels to a lane, neighbouring
-// ones, so a group is a run of G / kN lanes.
-template <typename T, int kN>
-__global__ void __launch_bounds__(128) kv4_write_kernel(Kv4IoParams P) {
-  const int lane = threadIdx.x & 31;
-  const long long unit = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
-  const long long tok = unit / P.sh.heads;
-  const int head = (int)(unit % P.sh.heads);
-  if (tok >= P.tokens) return;
-  const long long slot = P.slots[tok];
-  if (slot < 0) return;
+// Where a token's run lies, or null for a slot that is skipped; an index past the cache is reported.
+__device__ __forceinline__ unsigned char* kv4_run(const Kv4IoParams& P, long long slot, int head, bool report) {
+  if (slot < 0) return nullptr;
   const long long page = slot / P.sh.page;
   if (page >= P.sh.pages) {
-    if (lane == 0) report_device_failure(kSiteIndex);
-    return;
+    if (report) report_device_failure(kSiteIndex);
+    return nullptr;
   }
-  const int at = (int)(slot % P.sh.page);
-  unsigned char* block = P.cache + (page * P.sh.heads + head) * (long long)P.sh.block_bytes();
-  const int span = 32 / P.sh.groups;  // lanes of a group
+  return P.cache + (page * P.sh.heads + head) * P.sh.block_bytes() + (int)(slot % P.sh.page) / 16 * P.sh.run_bytes();
+}
+
+// Sixteen tokens of one head to a CTA, kDim / 8 threads to a token, 8 channels (16 bytes) to a thread. Bandwidth
+// bounds it: everything a thread reads is asked for before anything is computed. When the sixteen fill a run, as
+// prompts do, the run is put together in shared memory and stored whole; otherwise each thread stores its words (keys) and
+// bytes (values).
+template <typename T, int kDim, bool kVec>
+__global__ void __launch_bounds__(2 * kDim) kv4_write_kernel(Kv4IoParams P) {
+  constexpr int kChunks = kDim / 8;
+  extern __shared__ uint4 s_run[];
+  griddep_launch_wait();
+  const int chunk = threadIdx.x % kChunks, mine = threadIdx.x / kChunks, head = blockIdx.y;
+  const long long first = (long long)blockIdx.x * 16, tok = first + mine;
+  const bool in = tok < P.tokens;
+  T x[2][8];
+#pragma unroll
   for (int part = 0; part < 2; ++part) {
-    const T* src = part ? static_cast<const T*>(P.v) + tok * P.v_ts + head * P.v_hs
-                        : static_cast<const T*>(P.k) + tok * P.k_ts + head * P.k_hs;
-    float x[kN];
-    float lo = __int_as_float(0x7f800000), hi = -lo;
+    const T* src = (part ? static_cast<const T*>(P.v) + tok * P.v_ts + head * P.v_hs
+                         : static_cast<const T*>(P.k) + tok * P.k_ts + head * P.k_hs) + 8 * chunk;
+    if constexpr (kVec) {
+      *reinterpret_cast<uint4*>(x[part]) = in ? *reinterpret_cast<const uint4*>(src) : uint4{};
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[part][i] = in ? src[i] : from_f32<T>(0.f);
+    }
+  }
+  const long long slot = in ? P.slots[tok] : -1, slot0 = P.slots[first];
+  const bool whole = __syncthreads_and(in && slot == slot0 + mine && (slot0 & 15) == 0);
+  unsigned char* run = kv4_run(P, slot, head, chunk == 0);
+  unsigned char* out = whole ? reinterpret_cast<unsigned char*>(s_run) : run;
+  const int at = whole ? mine : (int)(slot & 15), span = kChunks / P.sh.groups;  // threads of a group
+#pragma unroll
+  for (int part = 0; part < 2; ++part) {
+    float f[8], lo, hi;
     bool fine = true;
 #pragma unroll
-    for (int i = 0; i < kN; ++i) {
-      x[i] = to_f32(src[lane * kN + i]);
-      fine = fine && fabsf(x[i]) < __int_as_float(0x7f800000);
-      lo = fminf(lo, x[i]);
-      hi = fmaxf(hi, x[i]);
+    for (int i = 0; i < 8; ++i) {
+      f[i] = to_f32(x[part][i]);
+      fine = fine && fabsf(f[i]) < __int_as_float(0x7f800000);
+      lo = i ? fminf(lo, f[i]) : f[i];
+      hi = i ? fmaxf(hi, f[i]) : f[i];
     }
     for (int o = span >> 1; o; o >>= 1) {
       lo = fminf(lo, __shfl_xor_sync(kFullMask, lo, o));
@@ -112,58 +115,94 @@ __global__ void __launch_bounds__(128) kv4_write_kernel(Kv4IoParams P) {
     pr.m = from_f32<T>(fine ? lo : nan);
     const float s = to_f32(pr.s), m = to_f32(pr.m);
     const float inv = s >= 0x1p-126f ? __frcp_rn(s) : 0.f;
-    if (lane % span == 0)
-      reinterpret_cast<Pair16<T>*>(block + (part ? P.sh.v_pairs() : P.sh.k_pairs()))[at * P.sh.groups + lane / span] = pr;
-    int code[kN];
+    uint32_t code[8];
 #pragma unroll
-    for (int i = 0; i < kN; ++i)
-      code[i] = fine ? (int)fminf(fmaxf(rintf(__fmul_rn(__fsub_rn(x[i], m), inv)), 0.f), 15.f) : 0;
-    // Each byte is put together and stored by the lane that holds its low nibble.
-    unsigned char* codes = block + (part ? P.sh.v_codes() : 0);
+    for (int i = 0; i < 8; ++i)
+      code[i] = fine ? (uint32_t)fminf(fmaxf(rintf(__fmul_rn(__fsub_rn(f[i], m), inv)), 0.f), 15.f) : 0u;
+    if (part == 0) {
+      // Step j = chunk / 2, t = 2 (chunk & 1) and the next; the other half of each word, step j ^ 1, is chunk ^ 2's.
+      const int up = (chunk & 2) ? 8 : 0;
+      const uint32_t a = (code[0] | code[1] << 16 | code[2] << 4 | code[3] << 20) << up;
+      const uint32_t b = (code[4] | code[5] << 16 | code[6] << 4 | code[7] << 20) << up;
+      const uint32_t got = __shfl_xor_sync(kFullMask, up ? a : b, 2), word = (up ? b : a) | got;
+      const int t = 2 * (chunk & 1) + (up ? 1 : 0);
+      if (out) *reinterpret_cast<uint32_t*>(out + at * (kDim / 2) + t * (kDim / 8) + (chunk >> 2) * 4) = word;
+    } else {
+      // Tile chunk / 2; an even chunk has the low nibbles of its 8 bytes, its odd neighbour the high ones.
+      const bool odd = chunk & 1;
+      const uint32_t a = code[0] | code[1] << 8 | code[2] << 16 | code[3] << 24;
+      const uint32_t b = code[4] | code[5] << 8 | code[6] << 16 | code[7] << 24;
+      const uint32_t got = __shfl_xor_sync(kFullMask, odd ? a : b, 1), bytes = odd ? got | b << 4 : a | got << 4;
+      const int tile = chunk >> 1, byte = 2 * (at & 1) + (at >> 3), lane = (odd ? 16 : 0) + ((at & 7) >> 1);
+      if (out) {
+        unsigned char* v = out + 8 * kDim + (tile >> 2) * 512 + lane * 16 + (tile & 3) * 4 + byte;
 #pragma unroll
-    for (int i = 0; i < kN; ++i) {
-      const int d = lane * kN + i;
-      const int partner = part ? d + 8 : (d & 2 ? -1 : d + 2);  // the channel of the byte's high nibble
-      const int pl = (partner < 0 ? 0 : partner / kN) & 31;
-      int high = 0;
-#pragma unroll
-      for (int q = 0; q < kN; ++q) {
-        const int got = __shfl_sync(kFullMask, code[q], pl);
-        if (partner >= 0 && partner % kN == q) high = got;
+        for (int i = 0; i < 4; ++i) v[64 * i] = (unsigned char)(bytes >> (8 * i));
       }
-      int shift;
-      const int byte = part ? kv4_value_byte(P.sh.dim, at, d, &shift) : kv4_key_byte(P.sh.dim, at, d, &shift);
-      if (shift == 0) codes[byte] = (unsigned char)(code[i] | high << 4);
     }
+    if (out && chunk % span == 0)
+      reinterpret_cast<Pair16<T>*>(out + 16 * kDim + part * 64 * P.sh.groups)[at * P.sh.groups + chunk / span] = pr;
+  }
+  if (whole) {
+    __syncthreads();
+    unsigned char* to = kv4_run(P, slot0, head, false);
+    const int pieces = P.sh.run_bytes() / 16;
+    if (to)
+      for (int i = threadIdx.x; i < pieces; i += 2 * kDim) reinterpret_cast<uint4*>(to)[i] = s_run[i];
   }
 }
 
-// Values at slots; a negative slot reads as zeros. One thread per channel of a token and head.
-template <typename T>
-__global__ void __launch_bounds__(256) kv4_read_kernel(Kv4IoParams P) {
-  const long long e = (long long)blockIdx.x * 256 + threadIdx.x;
-  const int dim = P.sh.dim;
-  const long long unit = e / dim, tok = unit / P.sh.heads;
-  if (tok >= P.tokens) return;
-  const int d = (int)(e % dim), head = (int)(unit % P.sh.heads);
-  const long long slot = P.slots[tok], page = slot / P.sh.page;
-  const bool there = slot >= 0 && page < P.sh.pages;
-  if (slot >= 0 && !there && d == 0) report_device_failure(kSiteIndex);
-  float out[2] = {0.f, 0.f};
-  if (there) {
-    const int at = (int)(slot % P.sh.page), g = d / (dim / P.sh.groups);
-    const unsigned char* block = P.cache + (page * P.sh.heads + head) * (long long)P.sh.block_bytes();
-    for (int part = 0; part < 2; ++part) {
-      int shift;
-      const int byte = part ? kv4_value_byte(dim, at, d, &shift) : kv4_key_byte(dim, at, d, &shift);
-      const int code = (block[(part ? P.sh.v_codes() : 0) + byte] >> shift) & 15;
-      const Pair16<T> pr =
-          reinterpret_cast<const Pair16<T>*>(block + (part ? P.sh.v_pairs() : P.sh.k_pairs()))[at * P.sh.groups + g];
-      out[part] = fmaf(to_f32(pr.s), (float)code, to_f32(pr.m));
-    }
+// The values at slots, as kv4_write_kernel cuts them; a negative slot reads as zeros.
+template <typename T, int kDim>
+__global__ void __launch_bounds__(2 * kDim) kv4_read_kernel(Kv4IoParams P) {
+  constexpr int kChunks = kDim / 8;
+  extern __shared__ uint4 s_run[];
+  griddep_launch_wait();
+  const int chunk = threadIdx.x % kChunks, mine = threadIdx.x / kChunks, head = blockIdx.y;
+  const long long first = (long long)blockIdx.x * 16, tok = first + mine;
+  const bool in = tok < P.tokens;
+  const long long slot = in ? P.slots[tok] : -1, slot0 = P.slots[first];
+  const bool whole = __syncthreads_and(in && slot == slot0 + mine && (slot0 & 15) == 0);
+  const unsigned char* run = kv4_run(P, slot, head, chunk == 0);
+  if (whole) {
+    const uint4* from = reinterpret_cast<const uint4*>(kv4_run(P, slot0, head, false));
+    const int pieces = P.sh.run_bytes() / 16;
+    if (from)
+      for (int i = threadIdx.x; i < pieces; i += 2 * kDim) s_run[i] = from[i];
+    __syncthreads();
+    if (run) run = reinterpret_cast<const unsigned char*>(s_run);
   }
-  static_cast<T*>(P.k_out)[e] = from_f32<T>(out[0]);
-  static_cast<T*>(P.v_out)[e] = from_f32<T>(out[1]);
+  if (!in) return;
+  const int at = (int)(slot & 15), group = chunk * P.sh.groups / kChunks;
+  const long long to = (tok * P.sh.heads + head) * kDim + 8 * chunk;
+#pragma unroll
+  for (int part = 0; part < 2; ++part) {
+    uint32_t code[8];
+    T out[8];
+    if (run) {
+      if (part == 0) {
+        const unsigned char* w = run + at * (kDim / 2) + 2 * (chunk & 1) * (kDim / 8) + (chunk >> 2) * 4;
+        const int up = (chunk & 2) ? 8 : 0;
+        const uint32_t a = *reinterpret_cast<const uint32_t*>(w) >> up, b = *reinterpret_cast<const uint32_t*>(w + kDim / 8) >> up;
+        code[0] = a & 15, code[1] = a >> 16 & 15, code[2] = a >> 4 & 15, code[3] = a >> 20 & 15;
+        code[4] = b & 15, code[5] = b >> 16 & 15, code[6] = b >> 4 & 15, code[7] = b >> 20 & 15;
+      } else {
+        const int tile = chunk >> 1, byte = 2 * (at & 1) + (at >> 3), shift = 4 * (chunk & 1);
+        const unsigned char* v = run + 8 * kDim + (tile >> 2) * 512 + ((at & 7) >> 1) * 16 + (tile & 3) * 4 + byte;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) code[i] = v[64 * i] >> shift & 15;
+      }
+      const Pair16<T> pr =
+          reinterpret_cast<const Pair16<T>*>(run + 16 * kDim + part * 64 * P.sh.groups)[at * P.sh.groups + group];
+      const float s = to_f32(pr.s), m = to_f32(pr.m);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) out[i] = from_f32<T>(fmaf(s, (float)code[i], m));
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) out[i] = from_f32<T>(0.f);
+    }
+    *reinterpret_cast<uint4*>(static_cast<T*>(part ? P.v_out : P.k_out) + to) = *reinterpret_cast<uint4*>(out);
+  }
 }
 
 }  // namespace qrb200

@@ -1,17 +1,28 @@
 // Attention of a few queries over the 4-bit cache (layout and formulas: kv4.cuh).
 //
-// With c the centred code (code - 8, exact in 16 bits) and mid = m + 8 s:
-//   q . k_t = sum_groups s_t (q . c_t) + mid_t sum(q),     o = sum_t (p_t s_t) c_t + sum_t p_t mid_t.
-// So the codes themselves are the matrix operands: no key or value is ever rounded to 16 bits, steps and
-// minima are applied in 32. Keys (and values transposed) are the 16-row left operand, 8 query rows that share the key
-// head the right one, so a head with few query rows wastes little of the matrix instruction. The weights p_t s_t are the
-// only rounded operand: each is two bf16 halves, high and low, 16 bits of significand in all.
+// With m_t and s_t a token's minimum and step, c_t its codes:
+//   q . k_t = sum_groups s_t (q . c_t) + m_t sum(q),     o = sum_t (p_t s_t) c_t + sum_t p_t m_t.
+// So the codes themselves are the matrix operands, exact in 16 bits: no key or value is ever rounded, steps
+// and minima are applied in 32 bits. Keys (and values transposed) are the 16-row left operand, 8 query rows that
+// share the key head the right one, so a head with few query rows wastes little of the matrix instruction.
 //
-// A warp takes 32 or 64 tokens at a time: scores, running maximum (base 2), weights, output. Codes go from global memory
-// straight to registers; the next tokens' keys load while the current ones' softmax and output run.
+// Instructions bound it before the memory does, so the inner loop is kept short:
+// * a key's nibble needs one logical operation: left in place in an otherwise empty 16-bit number it is a subnormal (or
+//   the first normal binade, which continues them), worth code 2^-133 in bf16 and code 2^-24 in fp16, 16 times that four
+//   bits higher. The factors are powers of two: 1/16 goes to the queries of those channels, 2^64 to bf16 queries (whose
+//   products would otherwise be subnormal in 32 bits; |q| < 2^63 keeps them finite), the rest to the scores.
+//   A value's nibble is placed under fp16's exponent of 1024 and brought to code - 8, which keeps sums over many tokens from cancelling.
+// * the weights p_t s_t are the only rounded operand: two fp16 numbers each, high and low, 22 bits in all (one alone
+//   would add an error the size of the result's own rounding). They are scaled by a power of two that puts the largest
+//   step near 2^11, so that a weight keeps its leading bits down to 2^-25 of the largest.
+// * the running maximum and that scale move only when a score exceeds the reference by 2^4 or a step its bound, so
+//   that the output is rarely rescaled and the warp rarely reduces.
+// Codes go from global memory straight to registers; the next tokens' keys load while the current ones' softmax and output run.
 // The token range is cut over CTAs (blockIdx.x) and over a CTA's four warps; the parts are joined through shared memory and,
 // between CTAs, by kv4_join_kernel, in a fixed order.
 #pragma once
+
+#include <type_traits>
 
 #include "kv4.cuh"
 
@@ -50,25 +61,37 @@ __device__ __forceinline__ void kv_mma<__half>(float (&d)[4], const uint32_t (&a
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// Nibbles p and p + 4 of w as a pair of 16-bit numbers, less 8. Placed under an exponent whose unit is
-// 1 (128 in bf16, 1024 in fp16), a nibble is that power of two plus its code, exactly; the subtraction is exact too.
-template <typename T>
-__device__ __forceinline__ uint32_t kv_pair(uint32_t w, int p);
-template <>
-__device__ __forceinline__ uint32_t kv_pair<__nv_bfloat16>(uint32_t w, int p) {
-  const uint32_t x = ((w >> (4 * p)) & 0x000f000fu) | 0x43004300u;
-  const __nv_bfloat162 r = __hsub2(reinterpret_cast<const __nv_bfloat162&>(x), __floats2bfloat162_rn(136.f, 136.f));
-  return reinterpret_cast<const uint32_t&>(r);
+// Nibbles p and p + 4 of w as a pair of 16-bit numbers: bare (the integer code, times 16 for odd p, as a subnormal
+// of either 16-bit type), and as code - 8 in fp16.
+__device__ __forceinline__ uint32_t kv_pair_bare(uint32_t w, int p) {
+  if (p & 2) w >>= 8;
+  return w & (p & 1 ? 0x00f000f0u : 0x000f000fu);
 }
-template <>
-__device__ __forceinline__ uint32_t kv_pair<__half>(uint32_t w, int p) {
-  const uint32_t x = ((w >> (4 * p)) & 0x000f000fu) | 0x64006400u;
+__device__ __forceinline__ uint32_t kv_pair_fp16(uint32_t w, int p) {
+  if (p & 2) w >>= 8;
+  if (p & 1) {  // 16 code + 1024: brought to code + 64, less 72, in one fused step
+    const uint32_t x = (w & 0x00f000f0u) | 0x64006400u;
+    const __half2 r = __hfma2(reinterpret_cast<const __half2&>(x), __floats2half2_rn(0.0625f, 0.0625f),
+                              __floats2half2_rn(-72.f, -72.f));
+    return reinterpret_cast<const uint32_t&>(r);
+  }
+  const uint32_t x = (w & 0x000f000fu) | 0x64006400u;
   const __half2 r = __hsub2(reinterpret_cast<const __half2&>(x), __floats2half2_rn(1032.f, 1032.f));
   return reinterpret_cast<const uint32_t&>(r);
 }
+template <typename T>
+struct KvKey;  // what queries are multiplied by, and what gives back q . c from the product with bare codes
+template <>
+struct KvKey<__nv_bfloat16> {
+  static constexpr float kQuery = 0x1p64f, kBack = 0x1p69f;
+};
+template <>
+struct KvKey<__half> {
+  static constexpr float kQuery = 1.f, kBack = 0x1p24f;
+};
 
-__device__ __forceinline__ uint32_t kv_pack_bf16(float lo, float hi) {
-  const __nv_bfloat162 r = __floats2bfloat162_rn(lo, hi);
+__device__ __forceinline__ uint32_t kv_pack(float2 x) {
+  const __half2 r = __float22half2_rn(x);
   return reinterpret_cast<const uint32_t&>(r);
 }
 __device__ __forceinline__ uint32_t kv_transpose(uint32_t x) {  // an 8 x 8 matrix of 16-bit numbers over the warp
@@ -93,13 +116,16 @@ __device__ __forceinline__ void kv_load(uint32_t (&w)[kWords], const unsigned ch
     w[0] = __ldg(reinterpret_cast<const uint32_t*>(p));
   }
 }
-// A (step, minimum) word as (step, minimum + 8 steps).
+// A (step, minimum) word.
 template <typename T>
-__device__ __forceinline__ float2 kv_step_mid(uint32_t w) {
+__device__ __forceinline__ float2 kv_step_low(uint32_t w) {
   const Pair16<T> pr = reinterpret_cast<const Pair16<T>&>(w);
-  const float s = to_f32(pr.s);
-  return make_float2(s, fmaf(8.f, s, to_f32(pr.m)));
+  return make_float2(to_f32(pr.s), to_f32(pr.m));
 }
+__device__ __forceinline__ float2 kv_both(float x) { return make_float2(x, x); }
+
+constexpr float kKvLazy = 4.f;      // powers of two that a score may stand above the reference
+constexpr int kKvStepExp = 11;      // the largest step's place: weights stay below 2^(11 + 4) in fp16
 
 template <typename T, int kDim, int kGroups, int kNT>
 __global__ void __launch_bounds__(32 * kKvWarps, kNT == 1 ? 3 : 2) kv4_attention_kernel(Kv4AttnParams P) {
@@ -120,7 +146,7 @@ __global__ void __launch_bounds__(32 * kKvWarps, kNT == 1 ? 3 : 2) kv4_attention
 
   griddep_launch_wait();
   int len = P.lengths[b];
-  if (len < 0 || len > (long long)P.max_pages * P.sh.page) {
+  if (len < 0 || len > (long long)P.max_pages * P.sh.page || (len > 0 && P.sh.pages == 0)) {
     if (threadIdx.x == 0) report_device_failure(kSiteIndex);
     len = 0;
   }
@@ -154,7 +180,7 @@ __global__ void __launch_bounds__(32 * kKvWarps, kNT == 1 ? 3 : 2) kv4_attention
 
   // Queries as the right operand: step j wants channels 16 j + 4 t + {0, 1} and {2, 3} of row g.
   uint32_t qf[kNT][kSteps][2];
-  float qsum[kNT][kGroups][2];
+  float2 qsum[kNT][kGroups];
 #pragma unroll
   for (int n = 0; n < kNT; ++n) {
     const int r = row0 + 8 * n + g;
@@ -168,229 +194,272 @@ __global__ void __launch_bounds__(32 * kKvWarps, kNT == 1 ? 3 : 2) kv4_attention
         T x[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          x[e] = r < rows ? q[16 * j + e] : from_f32<T>(0.f);
-          sum += to_f32(x[e]);
+          const float v = r < rows ? to_f32(q[16 * j + e]) : 0.f;
+          x[e] = from_f32<T>(v * (e < 2 ? KvKey<T>::kQuery : KvKey<T>::kQuery / 16));
+          sum += v;
         }
         qf[n][j][0] = reinterpret_cast<uint32_t*>(x)[0];
         qf[n][j][1] = reinterpret_cast<uint32_t*>(x)[1];
       }
       sum += __shfl_xor_sync(kFullMask, sum, 1);
       sum += __shfl_xor_sync(kFullMask, sum, 2);  // row g's sum, in its four lanes
-      qsum[n][gr][0] = __shfl_sync(kFullMask, sum, 8 * t);
-      qsum[n][gr][1] = __shfl_sync(kFullMask, sum, 8 * t + 4);
+      qsum[n][gr].x = __shfl_sync(kFullMask, sum, 8 * t);
+      qsum[n][gr].y = __shfl_sync(kFullMask, sum, 8 * t + 4);
     }
   }
 
-  float o[kNT][kSteps][4] = {};
-  float top[kNT][2], sum[kNT][2] = {}, mids[kNT][kGroups][2] = {};
+  float o[kNT][kSteps][4] = {};  // scaled by `unit`
+  float2 sum[kNT] = {}, mids[kNT][kGroups] = {};
+  // Weights are 2^(score scale2 + less); bound is where a score moves that reference. cap bounds the steps, unit scales them.
+  float2 less[kNT] = {};
+  float bound[kNT][2], cap = 0.f, unit = 1.f;
 #pragma unroll
-  for (int n = 0; n < kNT; ++n) top[n][0] = top[n][1] = kNone;
+  for (int n = 0; n < kNT; ++n) bound[n][0] = bound[n][1] = kNone;
 
-  // Where a unit's runs of 16 tokens lie: the block of each run's page, or null past the range.
-  const unsigned char* blocks[kRuns];
+  // Where a step's runs of 16 tokens lie; a run past the range or without a page is read from the cache's first block and
+  // masked.
+  const unsigned char* runs[kRuns];
+  unsigned gone = 0;  // those runs
+  const int run_bytes = P.sh.run_bytes(), page_runs = P.sh.page / 16, page_shift = 31 - __clz(page_runs);
   auto locate = [&](int u) {
-    const int tok = u * kUnit + 16 * (t & (kRuns - 1));
+    const int run = u * kRuns + (t & (kRuns - 1));
     int page = -1;
-    if (u < u_hi && tok < len) {
-      page = __ldg(P.table + b * P.table_stride + tok / P.sh.page);
+    if (u < u_hi && 16 * run < len) {
+      page = __ldg(P.table + b * P.table_stride + (run >> page_shift));
       if (page < 0 || page >= P.sh.pages) {
         if (g == 0 && t < kRuns) report_device_failure(kSiteIndex);
         page = -1;
       }
     }
+    gone = 0;
 #pragma unroll
     for (int i = 0; i < kRuns; ++i) {
       const int pg = __shfl_sync(kFullMask, page, i);
-      blocks[i] = pg < 0 ? nullptr : P.cache + ((long long)pg * P.sh.heads + head) * block_bytes;
+      gone |= pg < 0 ? 1u << i : 0u;
+      runs[i] = P.cache + (pg < 0 ? 0ll : ((long long)pg * P.sh.heads + head) * block_bytes +
+                                              ((u * kRuns + i) & (page_runs - 1)) * run_bytes);
     }
   };
   uint32_t kc[kRuns][2][kKW], kp[kRuns][2][kGroups];
-  auto load_keys = [&](int u) {
+  auto load_keys = [&]() {
 #pragma unroll
     for (int i = 0; i < kRuns; ++i) {
-      const int at = (u * kUnit + 16 * i) & (P.sh.page - 1);
+      const unsigned char* codes = runs[i] + g * (kDim / 2) + t * (kDim / 8);
+      const unsigned char* pairs = runs[i] + 16 * kDim + g * (4 * kGroups);
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        if (blocks[i]) {
-          const int tok = at + g + 8 * h;
-          kv_load(kc[i][h], blocks[i] + tok * (kDim / 2) + t * (kDim / 8));
-          kv_load(kp[i][h], blocks[i] + P.sh.k_pairs() + tok * (4 * kGroups));
-        } else {
-#pragma unroll
-          for (int w = 0; w < kKW; ++w) kc[i][h][w] = 0;
-#pragma unroll
-          for (int w = 0; w < kGroups; ++w) kp[i][h][w] = 0;
-        }
+        kv_load(kc[i][h], codes + h * (4 * kDim));
+        kv_load(kp[i][h], pairs + h * (32 * kGroups));
       }
     }
   };
 
   int u = u_lo + warp;
-  locate(u);
-  load_keys(u);
+  if (u < u_hi) {
+    locate(u);
+    load_keys();
+  }
   for (; u < u_hi; u += kKvWarps) {
     const int tok0 = u * kUnit;
     uint32_t vc[kRuns][kVC][4], vp[kRuns][2][kGroups];
-    bool there = true;
 #pragma unroll
     for (int i = 0; i < kRuns; ++i) {
-      const int at = (tok0 + 16 * i) & (P.sh.page - 1);
-      there = there && blocks[i];
 #pragma unroll
-      for (int c = 0; c < kVC; ++c) {
-        if (blocks[i]) kv_load(vc[i][c], blocks[i] + P.sh.v_codes() + (at >> 4) * (8 * kDim) + c * 512 + lane * 16);
-        else vc[i][c][0] = vc[i][c][1] = vc[i][c][2] = vc[i][c][3] = 0;
-      }
+      for (int c = 0; c < kVC; ++c) kv_load(vc[i][c], runs[i] + 8 * kDim + c * 512 + lane * 16);
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        if (blocks[i]) kv_load(vp[i][h], blocks[i] + P.sh.v_pairs() + (at + g + 8 * h) * (4 * kGroups));
-        else
-#pragma unroll
-          for (int w = 0; w < kGroups; ++w) vp[i][h][w] = 0;
-      }
+      for (int h = 0; h < 2; ++h) kv_load(vp[i][h], runs[i] + 16 * kDim + 64 * kGroups + (g + 8 * h) * (4 * kGroups));
     }
-    // Scores, in base 2: s[i][n][2 h + c] is token tok0 + 16 i + 8 h + g against row 8 n + 2 t + c.
-    float s[kRuns][kNT][4];
-    unsigned gone = 0;  // runs whose page is missing
+    // Scores before scaling: s[i][n][h] holds token tok0 + 16 i + 8 h + g against rows 8 n + 2 t and the next.
+    float2 s[kRuns][kNT][2];
 #pragma unroll
     for (int i = 0; i < kRuns; ++i) {
-      gone |= blocks[i] ? 0u : 1u << i;
-#pragma unroll
-      for (int n = 0; n < kNT; ++n) s[i][n][0] = s[i][n][1] = s[i][n][2] = s[i][n][3] = 0.f;
 #pragma unroll
       for (int gr = 0; gr < kGroups; ++gr) {
         float acc[kNT][4] = {};
 #pragma unroll
         for (int j = gr * kPer; j < (gr + 1) * kPer; ++j) {
           const int p = 2 * (j & 1);
-          const uint32_t a[4] = {kv_pair<T>(kc[i][0][j >> 1], p), kv_pair<T>(kc[i][1][j >> 1], p),
-                                 kv_pair<T>(kc[i][0][j >> 1], p + 1), kv_pair<T>(kc[i][1][j >> 1], p + 1)};
+          const uint32_t a[4] = {kv_pair_bare(kc[i][0][j >> 1], p), kv_pair_bare(kc[i][1][j >> 1], p),
+                                 kv_pair_bare(kc[i][0][j >> 1], p + 1), kv_pair_bare(kc[i][1][j >> 1], p + 1)};
 #pragma unroll
           for (int n = 0; n < kNT; ++n) kv_mma<T>(acc[n], a, qf[n][j][0], qf[n][j][1]);
         }
-        const float2 k0 = kv_step_mid<T>(kp[i][0][gr]), k1 = kv_step_mid<T>(kp[i][1][gr]);
 #pragma unroll
-        for (int n = 0; n < kNT; ++n) {
-          s[i][n][0] += fmaf(k0.x, acc[n][0], k0.y * qsum[n][gr][0]);
-          s[i][n][1] += fmaf(k0.x, acc[n][1], k0.y * qsum[n][gr][1]);
-          s[i][n][2] += fmaf(k1.x, acc[n][2], k1.y * qsum[n][gr][0]);
-          s[i][n][3] += fmaf(k1.x, acc[n][3], k1.y * qsum[n][gr][1]);
+        for (int h = 0; h < 2; ++h) {
+          const float2 k = kv_step_low<T>(kp[i][h][gr]);
+#pragma unroll
+          for (int n = 0; n < kNT; ++n) {
+            const float2 dot = __fmul2_rn(make_float2(acc[n][2 * h], acc[n][2 * h + 1]), kv_both(KvKey<T>::kBack));
+            const float2 base = gr ? __ffma2_rn(kv_both(k.y), qsum[n][gr], s[i][n][h]) : __fmul2_rn(kv_both(k.y), qsum[n][gr]);
+            s[i][n][h] = __ffma2_rn(kv_both(k.x), dot, base);
+          }
         }
       }
     }
-    locate(u + kKvWarps);  // the next unit's keys are under way while this one's softmax and output run
-    load_keys(u + kKvWarps);
-
-    const bool full = !gone && tok0 >= in_lo && tok0 + kUnit <= in_hi;  // every row sees every token
+    const unsigned missing = gone;
+    if (u + kKvWarps < u_hi) {  // the next keys are under way while this step's softmax and output run
+      locate(u + kKvWarps);
+      load_keys();
+    }
+    const bool full = !missing && tok0 >= in_lo && tok0 + kUnit <= in_hi;  // every row sees every token
     uint32_t seen[kNT];
+    if (!full) {
 #pragma unroll
-    for (int n = 0; n < kNT; ++n) {
-      seen[n] = 0xffffu;
-      if (!full) {
+      for (int n = 0; n < kNT; ++n) {
+        seen[n] = 0;
 #pragma unroll
         for (int i = 0; i < kRuns; ++i)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int tok = tok0 + 16 * i + 8 * (e >> 1) + g;
-            if (tok < lo[n][e & 1] || tok >= hi[n][e & 1] || (gone >> i & 1)) seen[n] &= ~(1u << (4 * i + e));
+          for (int h = 0; h < 2; ++h) {
+            const int tok = tok0 + 16 * i + 8 * h + g;
+            const bool x = tok >= lo[n][0] && tok < hi[n][0] && !(missing >> i & 1);
+            const bool y = tok >= lo[n][1] && tok < hi[n][1] && !(missing >> i & 1);
+            seen[n] |= (x ? 1u : 0u) << (4 * i + 2 * h) | (y ? 2u : 0u) << (4 * i + 2 * h);
+            if (!x) s[i][n][h].x = kNone;
+            if (!y) s[i][n][h].y = kNone;
+            if (n == 0 && (tok < all_lo || tok >= all_hi || (missing >> i & 1)))
+#pragma unroll
+              for (int gr = 0; gr < kGroups; ++gr) vp[i][h][gr] = 0;  // seen by no row: may hold anything
           }
       }
     }
+    float2 val[kRuns][2][kGroups];  // step, and minimum + 8 steps
+    float up[kNT][2], steps = 0.f;
+#pragma unroll
+    for (int i = 0; i < kRuns; ++i)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int gr = 0; gr < kGroups; ++gr) {
+          float2 v = kv_step_low<T>(vp[i][h][gr]);
+          v.y = fmaf(8.f, v.x, v.y);
+          val[i][h][gr] = v;
+          steps = fmaxf(steps, v.x);
+        }
+    bool move = steps > cap;
 #pragma unroll
     for (int n = 0; n < kNT; ++n) {
-      float up[2] = {top[n][0], top[n][1]}, ref[2], keep[2];
+      up[n][0] = s[0][n][0].x;
+      up[n][1] = s[0][n][0].y;
 #pragma unroll
       for (int i = 0; i < kRuns; ++i)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          s[i][n][e] = (seen[n] >> (4 * i + e) & 1) ? s[i][n][e] * P.scale2 : kNone;
-          up[e & 1] = fmaxf(up[e & 1], s[i][n][e]);
+        for (int h = 0; h < 2; ++h) {
+          up[n][0] = fmaxf(up[n][0], s[i][n][h].x);
+          up[n][1] = fmaxf(up[n][1], s[i][n][h].y);
         }
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-#pragma unroll
-        for (int x = 4; x < 32; x <<= 1) up[c] = fmaxf(up[c], __shfl_xor_sync(kFullMask, up[c], x));
-        ref[c] = up[c] == kNone ? 0.f : up[c];  // nothing seen yet: every weight is 2^-inf
-        keep[c] = kv_exp2(top[n][c] - ref[c]);
-        sum[n][c] *= keep[c];
+        up[n][c] *= P.scale2;
+        move = move || up[n][c] > bound[n][c];
       }
-      if (__any_sync(kFullMask, up[0] != top[n][0] || up[1] != top[n][1])) {
+    }
+    if (__any_sync(kFullMask, move)) {
+      steps = fmaxf(steps, cap);
+#pragma unroll
+      for (int x = 1; x < 32; x <<= 1) steps = fmaxf(steps, __shfl_xor_sync(kFullMask, steps, x));
+      float ratio = 1.f;
+      if (steps > cap) {  // the power of two above the largest step, and the scale that puts it at 2^11
+        const int e = max(-100, min(126, (int)(__float_as_uint(steps) >> 23) - 126));
+        cap = __int_as_float((e + 127) << 23);
+        const float fresh = __int_as_float((kKvStepExp - e + 127) << 23);
+        ratio = fresh / unit;
+        unit = fresh;
+      }
+#pragma unroll
+      for (int n = 0; n < kNT; ++n) {
+        float keep[2];
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+#pragma unroll
+          for (int x = 4; x < 32; x <<= 1) up[n][c] = fmaxf(up[n][c], __shfl_xor_sync(kFullMask, up[n][c], x));
+          const float last = bound[n][c] - kKvLazy, next = fmaxf(up[n][c], last);
+          keep[c] = next == kNone ? 0.f : kv_exp2(last - next);
+          bound[n][c] = next + kKvLazy;
+          // A row that has seen nothing has the reference -inf: its weights, 2^-inf, come from any finite one.
+          (c ? less[n].y : less[n].x) = next == kNone ? 0.f : -next;
+        }
+        sum[n] = __fmul2_rn(sum[n], make_float2(keep[0], keep[1]));
+#pragma unroll
+        for (int gr = 0; gr < kGroups; ++gr) mids[n][gr] = __fmul2_rn(mids[n][gr], make_float2(keep[0], keep[1]));
 #pragma unroll
         for (int j = 0; j < kSteps; ++j)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) o[n][j][e] *= keep[e & 1];
-#pragma unroll
-        for (int gr = 0; gr < kGroups; ++gr) {
-          mids[n][gr][0] *= keep[0];
-          mids[n][gr][1] *= keep[1];
-        }
+          for (int e = 0; e < 4; ++e) o[n][j][e] *= keep[e & 1] * ratio;
       }
-      top[n][0] = up[0];
-      top[n][1] = up[1];
-#pragma unroll
-      for (int i = 0; i < kRuns; ++i)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          s[i][n][e] = kv_exp2(s[i][n][e] - ref[e & 1]);
-          sum[n][e & 1] += s[i][n][e];
-        }
     }
+    // Weights and output; kAll: every row sees every token (no tests in the common case).
+    auto finish = [&](auto all) {
+      constexpr bool kAll = decltype(all)::value;
 #pragma unroll
-    for (int i = 0; i < kRuns; ++i) {
+      for (int i = 0; i < kRuns; ++i) {
 #pragma unroll
-      for (int gr = 0; gr < kGroups; ++gr) {
-        const float2 v0 = kv_step_mid<T>(vp[i][0][gr]), v1 = kv_step_mid<T>(vp[i][1][gr]);
-        uint32_t high[kNT][2], low[kNT][2];
-#pragma unroll
-        for (int n = 0; n < kNT; ++n) {
-          float w[4], m[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            w[e] = s[i][n][e] * (e < 2 ? v0.x : v1.x);
-            m[e] = s[i][n][e] * (e < 2 ? v0.y : v1.y);
-            if (!full && !(seen[n] >> (4 * i + e) & 1)) w[e] = m[e] = 0.f;  // what is masked may be NaN
-          }
-          mids[n][gr][0] += m[0] + m[2];
-          mids[n][gr][1] += m[1] + m[3];
+        for (int n = 0; n < kNT; ++n)
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            const uint32_t hw = kv_pack_bf16(w[2 * h], w[2 * h + 1]);
-            const float r0 = w[2 * h] - __uint_as_float(hw << 16), r1 = w[2 * h + 1] - __uint_as_float(hw & 0xffff0000u);
-            high[n][h] = kv_transpose(hw);
-            low[n][h] = kv_transpose(kv_pack_bf16(r0, r1));
+            float2 p = __ffma2_rn(s[i][n][h], kv_both(P.scale2), less[n]);
+            p.x = kv_exp2(p.x);
+            p.y = kv_exp2(p.y);
+            sum[n] = __fadd2_rn(sum[n], p);
+            s[i][n][h] = p;
           }
-        }
 #pragma unroll
-        for (int j = gr * kPer; j < (gr + 1) * kPer; ++j) {
-          const uint32_t word = vc[i][j >> 2][j & 3];
-          const uint32_t a[4] = {kv_pair<__nv_bfloat16>(word, 0), kv_pair<__nv_bfloat16>(word, 1),
-                                 kv_pair<__nv_bfloat16>(word, 2), kv_pair<__nv_bfloat16>(word, 3)};
+        for (int gr = 0; gr < kGroups; ++gr) {
+          uint32_t w[2][kNT][2];
 #pragma unroll
-          for (int n = 0; n < kNT; ++n) {
-            kv_mma<__nv_bfloat16>(o[n][j], a, high[n][0], high[n][1]);
-            kv_mma<__nv_bfloat16>(o[n][j], a, low[n][0], low[n][1]);
+          for (int h = 0; h < 2; ++h) {
+            const float scaled = val[i][h][gr].x * unit;
+#pragma unroll
+            for (int n = 0; n < kNT; ++n) {
+              const float2 p = s[i][n][h];
+              float2 x = __fmul2_rn(p, kv_both(scaled)), m = __fmul2_rn(p, kv_both(val[i][h][gr].y));
+              if constexpr (!kAll) {  // what a row does not see may be NaN
+                if (!(seen[n] >> (4 * i + 2 * h) & 1)) x.x = m.x = 0.f;
+                if (!(seen[n] >> (4 * i + 2 * h) & 2)) x.y = m.y = 0.f;
+              }
+              mids[n][gr] = __fadd2_rn(mids[n][gr], m);
+              const uint32_t high = kv_pack(x);
+              w[0][n][h] = kv_transpose(high);
+              const float2 top = __half22float2(reinterpret_cast<const __half2&>(high));
+              w[1][n][h] = kv_transpose(kv_pack(make_float2(x.x - top.x, x.y - top.y)));
+            }
+          }
+#pragma unroll
+          for (int j = gr * kPer; j < (gr + 1) * kPer; ++j) {
+            const uint32_t word = vc[i][j >> 2][j & 3];
+            const uint32_t a[4] = {kv_pair_fp16(word, 0), kv_pair_fp16(word, 1), kv_pair_fp16(word, 2), kv_pair_fp16(word, 3)};
+#pragma unroll
+            for (int n = 0; n < kNT; ++n)
+#pragma unroll
+              for (int half = 0; half < 2; ++half) kv_mma<__half>(o[n][j], a, w[half][n][0], w[half][n][1]);
           }
         }
       }
-    }
+    };
+    if (full) finish(std::true_type{});
+    else finish(std::false_type{});
   }
 
+  const float back = 1.f / unit;
   // The warps' parts: o[n][j][e] is channel 16 j + g + 8 (e / 2) of row 8 n + 2 t + e % 2.
 #pragma unroll
   for (int n = 0; n < kNT; ++n)
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
+      float l = c ? sum[n].y : sum[n].x, add[kGroups];
+#pragma unroll
+      for (int gr = 0; gr < kGroups; ++gr) add[gr] = c ? mids[n][gr].y : mids[n][gr].x;
 #pragma unroll
       for (int x = 4; x < 32; x <<= 1) {
-        sum[n][c] += __shfl_xor_sync(kFullMask, sum[n][c], x);
+        l += __shfl_xor_sync(kFullMask, l, x);
 #pragma unroll
-        for (int gr = 0; gr < kGroups; ++gr) mids[n][gr][c] += __shfl_xor_sync(kFullMask, mids[n][gr][c], x);
+        for (int gr = 0; gr < kGroups; ++gr) add[gr] += __shfl_xor_sync(kFullMask, add[gr], x);
       }
-      if (g == 0) s_ml[warp][8 * n + 2 * t + c] = make_float2(top[n][c], sum[n][c]);
+      if (g == 0) s_ml[warp][8 * n + 2 * t + c] = make_float2(bound[n][c] - kKvLazy, l);
 #pragma unroll
       for (int j = 0; j < kSteps; ++j) {
-        s_o[warp][8 * n + 2 * t + c][16 * j + g] = o[n][j][c] + mids[n][j / kPer][c];
-        s_o[warp][8 * n + 2 * t + c][16 * j + g + 8] = o[n][j][2 + c] + mids[n][j / kPer][c];
+        s_o[warp][8 * n + 2 * t + c][16 * j + g] = fmaf(o[n][j][c], back, add[j / kPer]);
+        s_o[warp][8 * n + 2 * t + c][16 * j + g + 8] = fmaf(o[n][j][2 + c], back, add[j / kPer]);
       }
     }
   __syncthreads();

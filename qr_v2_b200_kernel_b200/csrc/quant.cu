@@ -191,22 +191,48 @@ static bool shape_ok(const Kv4Shape& h) {
          (h.dim / h.groups == 32 || h.dim / h.groups == 64 || h.dim / h.groups == 128);
 }
 
+template <typename T>
+static cudaError_t launch_write(const Kv4IoParams& p, bool vec, cudaStream_t s) {
+  LaunchShape l(dim3(ceil_div(p.tokens, 16), p.sh.heads), 2 * p.sh.dim, p.sh.run_bytes(), s);
+  if (p.sh.dim == 128)
+    return vec ? cudaLaunchKernelEx(&l.cfg, kv4_write_kernel<T, 128, true>, p)
+               : cudaLaunchKernelEx(&l.cfg, kv4_write_kernel<T, 128, false>, p);
+  return vec ? cudaLaunchKernelEx(&l.cfg, kv4_write_kernel<T, 64, true>, p)
+             : cudaLaunchKernelEx(&l.cfg, kv4_write_kernel<T, 64, false>, p);
+}
+
+template <typename T>
+static cudaError_t launch_read(const Kv4IoParams& p, cudaStream_t s) {
+  LaunchShape l(dim3(ceil_div(p.tokens, 16), p.sh.heads), 2 * p.sh.dim, p.sh.run_bytes(), s);
+  return p.sh.dim == 128 ? cudaLaunchKernelEx(&l.cfg, kv4_read_kernel<T, 128>, p)
+                         : cudaLaunchKernelEx(&l.cfg, kv4_read_kernel<T, 64>, p);
+}
+
 // How an attention call is cut: query rows per tile, and the token range over `splits` CTAs.
 struct AttnPlan {
   int tile_rows, tiles, splits;
   size_t bytes;  // workspace: the parts and their (maximum, sum) pairs
 };
 
-// Eight rows a tile where a key head has no more than eight query rows, else sixteen. The token range is cut until the
-// GPU is full (three CTAs of four warps per SM), each warp keeping at least one step.
+// Eight rows a tile where a key head has no more than eight query rows, else sixteen. The token range
+// is cut so that the CTAs, which the GPU holds `slots` of at a time, fill their last round: the estimated time is rounds x
+// (steps of a warp + what a CTA costs besides, about six steps), over the table's capacity, the one length the host knows.
 static AttnPlan attn_plan(const Kv4Shape& h, int64_t batch, int64_t queries, int64_t q_heads, int64_t max_pages) {
   AttnPlan p{};
   const int64_t rows = queries * (q_heads / h.heads);
   p.tile_rows = rows <= 8 ? 8 : 16;
   p.tiles = ceil_div(rows, p.tile_rows);
-  const int64_t ctas = batch * h.heads * p.tiles, units = (max_pages * h.page + 16 * kv_runs(h.dim) - 1) / (16 * kv_runs(h.dim));
-  const int64_t want = (3 * (int64_t)sm_count() + ctas - 1) / ctas;
-  p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({want, (units + kKvWarps - 1) / kKvWarps, 128}));
+  const int64_t ctas = batch * h.heads * p.tiles, unit = 16 * kv_runs(h.dim);
+  const int64_t steps = std::max<int64_t>(1, (max_pages * h.page + unit * kKvWarps - 1) / (unit * kKvWarps));
+  const int64_t slots = (int64_t)sm_count() * (p.tile_rows == 8 ? 3 : 2);
+  int64_t best = -1;
+  for (int64_t n = 1; n <= std::min<int64_t>(steps, 64); ++n) {
+    const int64_t time = (ctas * n + slots - 1) / slots * ((steps + n - 1) / n + 6);
+    if (best < 0 || time < best) {
+      best = time;
+      p.splits = (int)n;
+    }
+  }
   if (p.splits > 1) p.bytes = (size_t)(ctas * p.splits * p.tile_rows) * (h.dim * sizeof(float) + sizeof(float2));
   return p;
 }
@@ -331,15 +357,12 @@ int qrb200_kv4_write(void* cache, const qrb200_kv4_shape* shape, const void* k, 
   Kv4IoParams p{static_cast<unsigned char*>(cache), k, v, nullptr, nullptr, reinterpret_cast<const long long*>(slots),
                 tokens, k_token_stride, k_head_stride, v_token_stride, v_head_stride, h};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const unsigned grid = (unsigned)((tokens * h.heads + 3) / 4);
   const bool bf = shape->dtype == QRB200_BF16;
-  if (h.dim == 128) {
-    if (bf) kv4_write_kernel<__nv_bfloat16, 4><<<grid, 128, 0, s>>>(p);
-    else kv4_write_kernel<__half, 4><<<grid, 128, 0, s>>>(p);
-  } else {
-    if (bf) kv4_write_kernel<__nv_bfloat16, 2><<<grid, 128, 0, s>>>(p);
-    else kv4_write_kernel<__half, 2><<<grid, 128, 0, s>>>(p);
-  }
+  // 16-byte loads where every (token, head) starts on such a boundary.
+  const bool vec = ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15u) == 0 &&
+                   ((k_token_stride | k_head_stride | v_token_stride | v_head_stride) & 7) == 0;
+  const cudaError_t e = bf ? launch_write<__nv_bfloat16>(p, vec, s) : launch_write<__half>(p, vec, s);
+  if (e != cudaSuccess) return QRB200_ERR_CUDA;
   return launched();
 }
 
@@ -355,9 +378,9 @@ int qrb200_kv4_read(const void* cache, const qrb200_kv4_shape* shape, void* k, v
   Kv4IoParams p{static_cast<unsigned char*>(const_cast<void*>(cache)), nullptr, nullptr, k, v,
                 reinterpret_cast<const long long*>(slots), tokens, 0, 0, 0, 0, h};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const unsigned grid = (unsigned)((tokens * h.heads * h.dim + 255) / 256);
-  if (shape->dtype == QRB200_BF16) kv4_read_kernel<__nv_bfloat16><<<grid, 256, 0, s>>>(p);
-  else kv4_read_kernel<__half><<<grid, 256, 0, s>>>(p);
+  if ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15u) return QRB200_ERR_ARG;
+  const cudaError_t e = shape->dtype == QRB200_BF16 ? launch_read<__nv_bfloat16>(p, s) : launch_read<__half>(p, s);
+  if (e != cudaSuccess) return QRB200_ERR_CUDA;
   return launched();
 }
 
@@ -383,7 +406,7 @@ int qrb200_kv4_attention(const void* q, const int64_t* q_strides, const void* ca
                          int64_t batch, int64_t queries, int64_t q_heads, int64_t max_pages, int64_t window,
                          int causal, float scale, void* workspace, size_t workspace_bytes, void* stream) {
   Kv4Shape h;
-  if (!q_strides || window < 0 || window > kMaxRows || !attention_args(shape, batch, queries, q_heads, max_pages, &h))
+  if (!q_strides || !(scale >= 0.f) || !(scale <= 3.0e38f) || window < 0 || window > kMaxRows || !attention_args(shape, batch, queries, q_heads, max_pages, &h))
     return QRB200_ERR_ARG;
   if (batch == 0 || queries == 0 || q_heads == 0) return QRB200_OK;
   if (!q || !out || !lengths || (max_pages > 0 && !block_table) || (reinterpret_cast<uintptr_t>(cache) & 15u) ||
@@ -404,7 +427,7 @@ int qrb200_kv4_attention(const void* q, const int64_t* q_strides, const void* ca
   p.q_bs = q_strides[0], p.q_ts = q_strides[1], p.q_hs = q_strides[2], p.table_stride = table_stride;
   p.batch = (int)batch, p.queries = (int)queries, p.q_heads = (int)q_heads, p.share = (int)(q_heads / h.heads);
   p.max_pages = (int)max_pages, p.window = (int)window, p.causal = causal, p.splits = plan.splits, p.tiles = plan.tiles;
-  p.scale2 = scale * 1.4426950408889634f;
+  p.scale2 = std::max(scale * 1.4426950408889634f, 1e-30f);  // not 0: masked scores, -inf, must stay that
   p.sh = h;
   if (plan.splits > 1)
     p.part_ml = reinterpret_cast<float2*>(p.part_o + batch * h.heads * plan.tiles * plan.splits * plan.tile_rows * h.dim);

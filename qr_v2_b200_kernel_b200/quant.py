@@ -337,6 +337,8 @@ def kv4_attention(q: torch.Tensor, cache: KV4Cache, block_table: torch.Tensor, l
         raise ValueError(f"lengths must be ({batch},), got {tuple(lengths.shape)}")
     if window is not None and window < 1:
         raise ValueError(f"window must be at least 1, got {window}")
+    if scale is not None and not 0 <= scale < 3e38:
+        raise ValueError(f"scale must be finite and not negative, got {scale}")
     if q.stride(3) != 1:
         q = q.contiguous()
     if block_table.stride(1) != 1 and block_table.shape[1] > 1:

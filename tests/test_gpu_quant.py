@@ -197,20 +197,20 @@ def test_int8_linear_offsets_past_32_bits():
 
 def _decode(cache):
     """(codes, steps, minima) of keys and of values, from the bytes, by the documented layout."""
-    P, D, G = cache.page_size, cache.head_dim, cache.group_size
-    tok, d = torch.meshgrid(torch.arange(P), torch.arange(D), indexing="ij")
+    P, D, NG = cache.page_size, cache.head_dim, cache.head_dim // cache.group_size
+    runs = cache.data.reshape(*cache.data.shape[:2], P // 16, 16 * D + 128 * NG)
+    tok, d = torch.meshgrid(torch.arange(16), torch.arange(D), indexing="ij")
     j, t, e = d // 16, d // 4 % 4, d % 4
     nib = 2 * (j % 2) + e // 2 + 4 * (e % 2)
     k_at = (tok * (D // 2) + t * (D // 8) + j // 2 * 4 + nib // 2, nib % 2)
-    kk, tile, r = tok % 16, d // 16, d % 16
-    lane, byte = (r % 8) * 4 + kk % 8 // 2, 2 * (kk % 2) + kk // 8
-    v_at = (tok // 16 * 8 * D + tile // 4 * 512 + lane * 16 + tile % 4 * 4 + byte + P * D // 2, r // 8)
+    lane, byte, r = (d % 8) * 4 + tok % 8 // 2, 2 * (tok % 2) + tok // 8, d % 16
+    v_at = (8 * D + d // 64 * 512 + lane * 16 + d // 16 % 4 * 4 + byte, r // 8)
     out = []
-    for (at, nibble), pairs in ((k_at, P * D), (v_at, P * D + P * (D // G) * 4)):
-        codes = cache.data[:, :, at.cuda()].int() >> (4 * nibble.cuda()) & 15  # pages, heads, P, D
-        raw = cache.data[:, :, pairs : pairs + P * (D // G) * 4].contiguous().view(cache.dtype).double()
-        raw = raw.reshape(*raw.shape[:2], P, D // G, 2)
-        out.append((codes.double(), raw[..., 0], raw[..., 1]))
+    for (at, nibble), pairs in ((k_at, 16 * D), (v_at, 16 * D + 64 * NG)):
+        codes = runs[..., at.cuda()].int() >> (4 * nibble.cuda()) & 15  # pages, heads, runs, 16, D
+        raw = runs[..., pairs : pairs + 64 * NG].contiguous().view(cache.dtype).double()
+        raw = raw.reshape(*runs.shape[:2], P, NG, 2)
+        out.append((codes.flatten(2, 3).double(), raw[..., 0], raw[..., 1]))
     return out
 
 
@@ -486,7 +486,8 @@ def test_cache_refusals():
                  lambda: qr.kv4_write(cache, k, k, slots[None]), lambda: qr.kv4_attention(q[..., :32], cache, table, n),
                  lambda: qr.kv4_attention(q[:, :, :3], cache, table, n), lambda: qr.kv4_attention(q[0], cache, table, n),
                  lambda: qr.kv4_attention(q, cache, table[:1], n), lambda: qr.kv4_attention(q, cache, table, n[:1]),
-                 lambda: qr.kv4_attention(q, cache, table, n, window=0)):
+                 lambda: qr.kv4_attention(q, cache, table, n, window=0),
+                 lambda: qr.kv4_attention(q, cache, table, n, scale=-1.0), lambda: qr.kv4_attention(q, cache, table, n, scale=float("nan"))):
         with pytest.raises(ValueError):
             call()
     for call in (lambda: qr.kv4_write(cache, k.half(), k, slots), lambda: qr.kv4_write(cache, k, k, slots.int()),
