@@ -17,7 +17,8 @@
 //   step near 2^11, so that a weight keeps its leading bits down to 2^-25 of the largest.
 // * the running maximum and that scale move only when a score exceeds the reference by 2^4 or a step its bound, so
 //   that the output is rarely rescaled and the warp rarely reduces.
-// Codes go from global memory straight to registers; the next tokens' keys load while the current ones' softmax and output run.
+// Each warp walks its own stretch of tokens, a step of 32 or 64 at a time, through a ring of three steps in shared memory
+// that bulk asynchronous copies fill: a run's bytes are already in the order of the operand's registers.
 // The token range is cut over CTAs (blockIdx.x) and over a CTA's four warps; the parts are joined through shared memory and,
 // between CTAs, by kv4_join_kernel, in a fixed order.
 #pragma once
@@ -105,16 +106,21 @@ __device__ __forceinline__ float kv_exp2(float x) {
   return r;
 }
 template <int kWords>
-__device__ __forceinline__ void kv_load(uint32_t (&w)[kWords], const unsigned char* p) {
+__device__ __forceinline__ void kv_load(uint32_t (&w)[kWords], const unsigned char* p) {  // from shared memory
   if constexpr (kWords == 4) {
-    const uint4 v = __ldg(reinterpret_cast<const uint4*>(p));
+    const uint4 v = *reinterpret_cast<const uint4*>(p);
     w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
   } else if constexpr (kWords == 2) {
-    const uint2 v = __ldg(reinterpret_cast<const uint2*>(p));
+    const uint2 v = *reinterpret_cast<const uint2*>(p);
     w[0] = v.x, w[1] = v.y;
   } else {
-    w[0] = __ldg(reinterpret_cast<const uint32_t*>(p));
+    w[0] = *reinterpret_cast<const uint32_t*>(p);
   }
+}
+__device__ __forceinline__ void kv_copy(uint32_t dst, const void* src, uint32_t bytes, uint32_t mbar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src),
+               "r"(bytes), "r"(mbar)
+               : "memory");
 }
 // A (step, minimum) word.
 template <typename T>
@@ -127,86 +133,153 @@ __device__ __forceinline__ float2 kv_both(float x) { return make_float2(x, x); }
 constexpr float kKvLazy = 4.f;      // powers of two that a score may stand above the reference
 constexpr int kKvStepExp = 11;      // the largest step's place: weights stay below 2^(11 + 4) in fp16
 
+constexpr int kKvStages = 3;
+// Dynamic shared memory: the warps' rings, reused at the end for their parts of the output.
+__host__ __device__ constexpr int kv_stage_bytes(int dim, int groups) { return kv_runs(dim) * (16 * dim + 128 * groups); }
+__host__ __device__ constexpr int kv_smem_bytes(int dim, int groups, int nt) {
+  const int ring = kKvWarps * kKvStages * kv_stage_bytes(dim, groups), parts = kKvWarps * 8 * nt * (dim + 4) * 4;
+  return ring > parts ? ring : parts;
+}
+
 template <typename T, int kDim, int kGroups, int kNT>
-__global__ void __launch_bounds__(32 * kKvWarps, kNT == 1 ? 3 : 2) kv4_attention_kernel(Kv4AttnParams P) {
+__global__ void __launch_bounds__(32 * kKvWarps, kNT == 1 ? 4 : 2) kv4_attention_kernel(Kv4AttnParams P) {
   constexpr int kRows = 8 * kNT;           // query rows of a tile
   constexpr int kSteps = kDim / 16;        // 16-channel steps of q . k; also 16-channel tiles of the output
   constexpr int kPer = kSteps / kGroups;   // steps of a group
   constexpr int kKW = kDim / 32;           // words of a lane's key codes, for one token
   constexpr int kVC = kDim / 64;           // 16-byte pieces of a lane's value codes, for 16 tokens
   constexpr int kRuns = kv_runs(kDim), kUnit = 16 * kRuns;
+  constexpr int kRunBytes = 16 * kDim + 128 * kGroups, kStage = kRuns * kRunBytes;
   constexpr float kNone = -INFINITY;
-  __shared__ float s_o[kKvWarps][kRows][kDim + 4];
+  extern __shared__ __align__(128) unsigned char s_ring[];
+  __shared__ uint2 s_q[kNT][kSteps][32];
+  __shared__ float s_qsum[kKvWarps][kNT][8][kGroups];
   __shared__ float2 s_ml[kKvWarps][kRows];
+  __shared__ uint64_t s_full[kKvWarps][kKvStages];
+  __shared__ int s_bad;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int split = blockIdx.x, head = blockIdx.y % P.sh.heads, tile = blockIdx.y / P.sh.heads, b = blockIdx.z;
   const int rows = P.queries * P.share, row0 = tile * kRows;
-  const int block_bytes = P.sh.block_bytes();
 
+  if (threadIdx.x == 0) s_bad = 0;
+  if (lane == 0) {
+    for (int i = 0; i < kKvStages; ++i) mbar_init(&s_full[warp][i], 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    fence_async_smem();
+  }
+  __syncwarp();
   griddep_launch_wait();
   int len = P.lengths[b];
   if (len < 0 || len > (long long)P.max_pages * P.sh.page || (len > 0 && P.sh.pages == 0)) {
     if (threadIdx.x == 0) report_device_failure(kSiteIndex);
     len = 0;
   }
-  // Tokens [lo, hi) that a query row sees; those of this thread's two columns of each 8.
-  auto range = [&](int r, int& lo, int& hi) {
-    const int pos = len - P.queries + r / P.share;
-    hi = r >= rows ? 0 : P.causal ? max(0, pos + 1) : len;
-    lo = P.window > 0 ? max(0, pos - P.window + 1) : 0;
-  };
-  int lo[kNT][2], hi[kNT][2], all_lo = 0x7fffffff, all_hi = 0, in_lo = 0, in_hi = 0x7fffffff;
-#pragma unroll
-  for (int r = 0; r < kRows; ++r) {
-    int l, h;
-    range(row0 + r, l, h);
-    if (h > l) {
-      all_lo = min(all_lo, l);
-      all_hi = max(all_hi, h);
-    }
-    if (row0 + r < rows) {
-      in_lo = max(in_lo, l);
-      in_hi = min(in_hi, h);
-    }
+  // Tokens [lo, hi) that each row sees (lane r holds row r's), all rows together, and every row.
+  int my_lo = 0, my_hi = 0;
+  const bool real = lane < kRows && row0 + lane < rows;
+  if (real) {
+    const int pos = len - P.queries + (row0 + lane) / P.share;
+    my_hi = P.causal ? max(0, pos + 1) : len;
+    my_lo = P.window > 0 ? max(0, pos - P.window + 1) : 0;
   }
-#pragma unroll
-  for (int n = 0; n < kNT; ++n)
-#pragma unroll
-    for (int c = 0; c < 2; ++c) range(row0 + 8 * n + 2 * t + c, lo[n][c], hi[n][c]);
+  const bool sees = my_hi > my_lo;
+  const int all_lo = __reduce_min_sync(kFullMask, sees ? my_lo : 0x7fffffff);
+  const int all_hi = __reduce_max_sync(kFullMask, sees ? my_hi : 0);
+  const int in_lo = __reduce_max_sync(kFullMask, my_lo), in_hi = __reduce_min_sync(kFullMask, real ? my_hi : 0x7fffffff);
+  // This warp's steps [u, u_hi) of its CTA's share of the range.
   const int u0 = all_hi > 0 ? all_lo / kUnit : 0, u1 = (all_hi + kUnit - 1) / kUnit;
   const int per = (u1 - u0 + P.splits - 1) / P.splits;
-  const int u_lo = u0 + split * per, u_hi = min(u1, u_lo + per);
+  const int cta_lo = min(u1, u0 + split * per), cta_hi = min(u1, cta_lo + per);
+  const int per_warp = (cta_hi - cta_lo + kKvWarps - 1) / kKvWarps;
+  int u = min(cta_hi, cta_lo + warp * per_warp);
+  const int u_hi = min(cta_hi, u + per_warp);
 
-  // Queries as the right operand: step j wants channels 16 j + 4 t + {0, 1} and {2, 3} of row g.
-  uint32_t qf[kNT][kSteps][2];
-  float2 qsum[kNT][kGroups];
+  // The ring. Lane i of `page` holds the page of run `page_base` + i, -1 past the range or where the table is wrong.
+  unsigned char* ring = s_ring + warp * (kKvStages * kStage);
+  const int page_runs = P.sh.page / 16, page_shift = 31 - __clz(page_runs);
+  const int last_run = min(u_hi * kRuns, (len + 15) / 16);
+  int page_base = u * kRuns, page = -1;
+  auto look_up = [&]() {
+    page = -1;
+    if (page_base + lane < last_run) {
+      page = __ldg(P.table + b * P.table_stride + ((page_base + lane) >> page_shift));
+      if (page < 0 || page >= P.sh.pages) {
+        report_device_failure(kSiteIndex);
+        page = -1;
+      }
+    }
+  };
+  unsigned missing = 0;  // kRuns bits a stage: its runs without a page
+  auto issue = [&](int unit, int stage) {
+    if (unit * kRuns >= page_base + 32) {
+      page_base = unit * kRuns;
+      look_up();
+    }
+    unsigned gone = 0;
+    const unsigned char* src[kRuns];
+#pragma unroll
+    for (int i = 0; i < kRuns; ++i) {
+      const int run = unit * kRuns + i, pg = __shfl_sync(kFullMask, page, run - page_base);
+      gone |= pg < 0 ? 1u << i : 0u;
+      src[i] = P.cache + ((long long)pg * P.sh.heads + head) * P.sh.block_bytes() + (run & (page_runs - 1)) * kRunBytes;
+    }
+    missing = (missing & ~(((1u << kRuns) - 1) << (8 * stage))) | gone << (8 * stage);
+    if (lane == 0) {
+      const uint32_t bar = smem_u32(&s_full[warp][stage]), dst = smem_u32(ring + stage * kStage);
+      asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar),
+                   "r"((kRuns - __popc(gone)) * kRunBytes)
+                   : "memory");
+#pragma unroll
+      for (int i = 0; i < kRuns; ++i)
+        if (!(gone >> i & 1)) kv_copy(dst + i * kRunBytes, src[i], kRunBytes, bar);
+    }
+  };
+  const int count = u_hi - u;
+  if (count > 0) look_up();
+  for (int i = 0; i < kKvStages && i < count; ++i) issue(u + i, i);
+
+  // Queries as the right operand: step j wants channels 16 j + 4 t + {0, 1} and {2, 3} of row g. The warps share the work.
 #pragma unroll
   for (int n = 0; n < kNT; ++n) {
     const int r = row0 + 8 * n + g;
     const T* q = static_cast<const T*>(P.q) + b * P.q_bs + (long long)(r / P.share) * P.q_ts +
                  (head * P.share + r % P.share) * P.q_hs + 4 * t;
+    float part[kGroups] = {};
+#pragma unroll
+    for (int i = 0; i < kSteps / kKvWarps; ++i) {
+      const int j = i * kKvWarps + warp;
+      T x[4];
+      float add = 0.f;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float v = r < rows ? to_f32(q[16 * j + e]) : 0.f;
+        x[e] = from_f32<T>(v * (e < 2 ? KvKey<T>::kQuery : KvKey<T>::kQuery / 16));
+        add += v;
+      }
+      s_q[n][j][lane] = *reinterpret_cast<uint2*>(x);
+#pragma unroll
+      for (int gr = 0; gr < kGroups; ++gr) part[gr] += j / kPer == gr ? add : 0.f;
+    }
 #pragma unroll
     for (int gr = 0; gr < kGroups; ++gr) {
-      float sum = 0.f;
-#pragma unroll
-      for (int j = gr * kPer; j < (gr + 1) * kPer; ++j) {
-        T x[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float v = r < rows ? to_f32(q[16 * j + e]) : 0.f;
-          x[e] = from_f32<T>(v * (e < 2 ? KvKey<T>::kQuery : KvKey<T>::kQuery / 16));
-          sum += v;
-        }
-        qf[n][j][0] = reinterpret_cast<uint32_t*>(x)[0];
-        qf[n][j][1] = reinterpret_cast<uint32_t*>(x)[1];
-      }
-      sum += __shfl_xor_sync(kFullMask, sum, 1);
-      sum += __shfl_xor_sync(kFullMask, sum, 2);  // row g's sum, in its four lanes
-      qsum[n][gr].x = __shfl_sync(kFullMask, sum, 8 * t);
-      qsum[n][gr].y = __shfl_sync(kFullMask, sum, 8 * t + 4);
+      part[gr] += __shfl_xor_sync(kFullMask, part[gr], 1);
+      part[gr] += __shfl_xor_sync(kFullMask, part[gr], 2);
+      if (t == 0) s_qsum[warp][n][g][gr] = part[gr];
     }
   }
+  __syncthreads();
+  float2 qsum[kNT][kGroups];
+#pragma unroll
+  for (int n = 0; n < kNT; ++n)
+#pragma unroll
+    for (int gr = 0; gr < kGroups; ++gr) {
+      qsum[n][gr] = make_float2(0.f, 0.f);
+      for (int w = 0; w < kKvWarps; ++w) {
+        qsum[n][gr].x += s_qsum[w][n][2 * t][gr];
+        qsum[n][gr].y += s_qsum[w][n][2 * t + 1][gr];
+      }
+    }
 
   float o[kNT][kSteps][4] = {};  // scaled by `unit`
   float2 sum[kNT] = {}, mids[kNT][kGroups] = {};
@@ -216,108 +289,86 @@ __global__ void __launch_bounds__(32 * kKvWarps, kNT == 1 ? 3 : 2) kv4_attention
 #pragma unroll
   for (int n = 0; n < kNT; ++n) bound[n][0] = bound[n][1] = kNone;
 
-  // Where a step's runs of 16 tokens lie; a run past the range or without a page is read from the cache's first block and
-  // masked.
-  const unsigned char* runs[kRuns];
-  unsigned gone = 0;  // those runs
-  const int run_bytes = P.sh.run_bytes(), page_runs = P.sh.page / 16, page_shift = 31 - __clz(page_runs);
-  auto locate = [&](int u) {
-    const int run = u * kRuns + (t & (kRuns - 1));
-    int page = -1;
-    if (u < u_hi && 16 * run < len) {
-      page = __ldg(P.table + b * P.table_stride + (run >> page_shift));
-      if (page < 0 || page >= P.sh.pages) {
-        if (g == 0 && t < kRuns) report_device_failure(kSiteIndex);
-        page = -1;
-      }
-    }
-    gone = 0;
-#pragma unroll
-    for (int i = 0; i < kRuns; ++i) {
-      const int pg = __shfl_sync(kFullMask, page, i);
-      gone |= pg < 0 ? 1u << i : 0u;
-      runs[i] = P.cache + (pg < 0 ? 0ll : ((long long)pg * P.sh.heads + head) * block_bytes +
-                                              ((u * kRuns + i) & (page_runs - 1)) * run_bytes);
-    }
-  };
-  uint32_t kc[kRuns][2][kKW], kp[kRuns][2][kGroups];
-  auto load_keys = [&]() {
-#pragma unroll
-    for (int i = 0; i < kRuns; ++i) {
-      const unsigned char* codes = runs[i] + g * (kDim / 2) + t * (kDim / 8);
-      const unsigned char* pairs = runs[i] + 16 * kDim + g * (4 * kGroups);
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        kv_load(kc[i][h], codes + h * (4 * kDim));
-        kv_load(kp[i][h], pairs + h * (32 * kGroups));
-      }
-    }
-  };
-
-  int u = u_lo + warp;
-  if (u < u_hi) {
-    locate(u);
-    load_keys();
-  }
-  for (; u < u_hi; u += kKvWarps) {
+  bool ok = true;
+  int stage = 0, turn = 0;
+  for (int k = 0; k < count; ++k, ++u) {
     const int tok0 = u * kUnit;
-    uint32_t vc[kRuns][kVC][4], vp[kRuns][2][kGroups];
-#pragma unroll
-    for (int i = 0; i < kRuns; ++i) {
-#pragma unroll
-      for (int c = 0; c < kVC; ++c) kv_load(vc[i][c], runs[i] + 8 * kDim + c * 512 + lane * 16);
-#pragma unroll
-      for (int h = 0; h < 2; ++h) kv_load(vp[i][h], runs[i] + 16 * kDim + 64 * kGroups + (g + 8 * h) * (4 * kGroups));
-    }
+    const unsigned char* runs = ring + stage * kStage;
+    const unsigned gone = missing >> (8 * stage) & ((1u << kRuns) - 1);
+    ok = ok && __all_sync(kFullMask, mbar_wait(&s_full[warp][stage], turn));
+    if (!ok) break;
     // Scores before scaling: s[i][n][h] holds token tok0 + 16 i + 8 h + g against rows 8 n + 2 t and the next.
     float2 s[kRuns][kNT][2];
+    {
+      float acc[kRuns][kNT][4];
+      uint32_t kc[kRuns][2][kKW];
 #pragma unroll
-    for (int i = 0; i < kRuns; ++i) {
+      for (int i = 0; i < kRuns; ++i)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) kv_load(kc[i][h], runs + i * kRunBytes + h * (4 * kDim) + lane * (kDim / 8));
 #pragma unroll
       for (int gr = 0; gr < kGroups; ++gr) {
-        float acc[kNT][4] = {};
+#pragma unroll
+        for (int i = 0; i < kRuns; ++i)
+#pragma unroll
+          for (int n = 0; n < kNT; ++n) acc[i][n][0] = acc[i][n][1] = acc[i][n][2] = acc[i][n][3] = 0.f;
 #pragma unroll
         for (int j = gr * kPer; j < (gr + 1) * kPer; ++j) {
           const int p = 2 * (j & 1);
-          const uint32_t a[4] = {kv_pair_bare(kc[i][0][j >> 1], p), kv_pair_bare(kc[i][1][j >> 1], p),
-                                 kv_pair_bare(kc[i][0][j >> 1], p + 1), kv_pair_bare(kc[i][1][j >> 1], p + 1)};
+          uint2 q[kNT];
 #pragma unroll
-          for (int n = 0; n < kNT; ++n) kv_mma<T>(acc[n], a, qf[n][j][0], qf[n][j][1]);
-        }
+          for (int n = 0; n < kNT; ++n) q[n] = s_q[n][j][lane];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const float2 k = kv_step_low<T>(kp[i][h][gr]);
+          for (int i = 0; i < kRuns; ++i) {
+            const uint32_t a[4] = {kv_pair_bare(kc[i][0][j >> 1], p), kv_pair_bare(kc[i][1][j >> 1], p),
+                                   kv_pair_bare(kc[i][0][j >> 1], p + 1), kv_pair_bare(kc[i][1][j >> 1], p + 1)};
 #pragma unroll
-          for (int n = 0; n < kNT; ++n) {
-            const float2 dot = __fmul2_rn(make_float2(acc[n][2 * h], acc[n][2 * h + 1]), kv_both(KvKey<T>::kBack));
-            const float2 base = gr ? __ffma2_rn(kv_both(k.y), qsum[n][gr], s[i][n][h]) : __fmul2_rn(kv_both(k.y), qsum[n][gr]);
-            s[i][n][h] = __ffma2_rn(kv_both(k.x), dot, base);
+            for (int n = 0; n < kNT; ++n) kv_mma<T>(acc[i][n], a, q[n].x, q[n].y);
           }
         }
+#pragma unroll
+        for (int i = 0; i < kRuns; ++i)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const float2 k = kv_step_low<T>(
+                *reinterpret_cast<const uint32_t*>(runs + i * kRunBytes + 16 * kDim + ((g + 8 * h) * kGroups + gr) * 4));
+#pragma unroll
+            for (int n = 0; n < kNT; ++n) {
+              const float2 dot = __fmul2_rn(make_float2(acc[i][n][2 * h], acc[i][n][2 * h + 1]), kv_both(KvKey<T>::kBack));
+              const float2 base = gr ? __ffma2_rn(kv_both(k.y), qsum[n][gr], s[i][n][h]) : __fmul2_rn(kv_both(k.y), qsum[n][gr]);
+              s[i][n][h] = __ffma2_rn(kv_both(k.x), dot, base);
+            }
+          }
       }
     }
-    const unsigned missing = gone;
-    if (u + kKvWarps < u_hi) {  // the next keys are under way while this step's softmax and output run
-      locate(u + kKvWarps);
-      load_keys();
-    }
-    const bool full = !missing && tok0 >= in_lo && tok0 + kUnit <= in_hi;  // every row sees every token
+    uint32_t vp[kRuns][2][kGroups];
+#pragma unroll
+    for (int i = 0; i < kRuns; ++i)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) kv_load(vp[i][h], runs + i * kRunBytes + 16 * kDim + 64 * kGroups + (g + 8 * h) * (4 * kGroups));
+    const bool full = !gone && tok0 >= in_lo && tok0 + kUnit <= in_hi;  // every row sees every token
     uint32_t seen[kNT];
     if (!full) {
 #pragma unroll
       for (int n = 0; n < kNT; ++n) {
+        int lo[2], hi[2];
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          lo[c] = __shfl_sync(kFullMask, my_lo, 8 * n + 2 * t + c);
+          hi[c] = __shfl_sync(kFullMask, my_hi, 8 * n + 2 * t + c);
+        }
         seen[n] = 0;
 #pragma unroll
         for (int i = 0; i < kRuns; ++i)
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             const int tok = tok0 + 16 * i + 8 * h + g;
-            const bool x = tok >= lo[n][0] && tok < hi[n][0] && !(missing >> i & 1);
-            const bool y = tok >= lo[n][1] && tok < hi[n][1] && !(missing >> i & 1);
+            const bool x = tok >= lo[0] && tok < hi[0] && !(gone >> i & 1);
+            const bool y = tok >= lo[1] && tok < hi[1] && !(gone >> i & 1);
             seen[n] |= (x ? 1u : 0u) << (4 * i + 2 * h) | (y ? 2u : 0u) << (4 * i + 2 * h);
             if (!x) s[i][n][h].x = kNone;
             if (!y) s[i][n][h].y = kNone;
-            if (n == 0 && (tok < all_lo || tok >= all_hi || (missing >> i & 1)))
+            if (n == 0 && (tok < all_lo || tok >= all_hi || (gone >> i & 1)))
 #pragma unroll
               for (int gr = 0; gr < kGroups; ++gr) vp[i][h][gr] = 0;  // seen by no row: may hold anything
           }
@@ -393,6 +444,9 @@ __global__ void __launch_bounds__(32 * kKvWarps, kNT == 1 ? 3 : 2) kv4_attention
       constexpr bool kAll = decltype(all)::value;
 #pragma unroll
       for (int i = 0; i < kRuns; ++i) {
+        uint32_t vc[kVC][4];
+#pragma unroll
+        for (int c = 0; c < kVC; ++c) kv_load(vc[c], runs + i * kRunBytes + 8 * kDim + c * 512 + lane * 16);
 #pragma unroll
         for (int n = 0; n < kNT; ++n)
 #pragma unroll
@@ -426,7 +480,7 @@ __global__ void __launch_bounds__(32 * kKvWarps, kNT == 1 ? 3 : 2) kv4_attention
           }
 #pragma unroll
           for (int j = gr * kPer; j < (gr + 1) * kPer; ++j) {
-            const uint32_t word = vc[i][j >> 2][j & 3];
+            const uint32_t word = vc[j >> 2][j & 3];
             const uint32_t a[4] = {kv_pair_fp16(word, 0), kv_pair_fp16(word, 1), kv_pair_fp16(word, 2), kv_pair_fp16(word, 3)};
 #pragma unroll
             for (int n = 0; n < kNT; ++n)
@@ -438,7 +492,20 @@ __global__ void __launch_bounds__(32 * kKvWarps, kNT == 1 ? 3 : 2) kv4_attention
     };
     if (full) finish(std::true_type{});
     else finish(std::false_type{});
+    __syncwarp();  // every lane has read this stage
+    if (k + kKvStages < count) issue(u + kKvStages, stage);
+    if (++stage == kKvStages) {
+      stage = 0;
+      turn ^= 1;
+    }
   }
+  if (!ok) {
+    // A copy did not arrive in time: nothing is written, and what is under way is waited for (with a limit) first.
+    for (int i = 0; i < kKvStages; ++i) mbar_wait(&s_full[warp][i], i < stage ? turn ^ 1 : turn);
+    s_bad = 1;
+  }
+  __syncthreads();  // the rings are free
+  float(*s_o)[kRows][kDim + 4] = reinterpret_cast<float(*)[kRows][kDim + 4]>(s_ring);
 
   const float back = 1.f / unit;
   // The warps' parts: o[n][j][e] is channel 16 j + g + 8 (e / 2) of row 8 n + 2 t + e % 2.
@@ -465,7 +532,7 @@ __global__ void __launch_bounds__(32 * kKvWarps, kNT == 1 ? 3 : 2) kv4_attention
   __syncthreads();
   constexpr int kLanesRow = 32 * kKvWarps / kRows;  // threads of a row
   const int r = threadIdx.x / kLanesRow, d0 = threadIdx.x % kLanesRow;
-  if (row0 + r >= rows) return;
+  if (row0 + r >= rows || s_bad) return;
   float m = kNone, l = 0.f, f[kKvWarps];
 #pragma unroll
   for (int w = 0; w < kKvWarps; ++w) m = fmaxf(m, s_ml[w][r].x);

@@ -224,7 +224,7 @@ static AttnPlan attn_plan(const Kv4Shape& h, int64_t batch, int64_t queries, int
   p.tiles = ceil_div(rows, p.tile_rows);
   const int64_t ctas = batch * h.heads * p.tiles, unit = 16 * kv_runs(h.dim);
   const int64_t steps = std::max<int64_t>(1, (max_pages * h.page + unit * kKvWarps - 1) / (unit * kKvWarps));
-  const int64_t slots = (int64_t)sm_count() * (p.tile_rows == 8 ? 3 : 2);
+  const int64_t slots = (int64_t)sm_count() * (p.tile_rows == 8 ? 4 : 2);
   int64_t best = -1;
   for (int64_t n = 1; n <= std::min<int64_t>(steps, 64); ++n) {
     const int64_t time = (ctas * n + slots - 1) / slots * ((steps + n - 1) / n + 6);
@@ -237,12 +237,22 @@ static AttnPlan attn_plan(const Kv4Shape& h, int64_t batch, int64_t queries, int
   return p;
 }
 
+template <typename T, int kDim, int kGroups, int kNT>
+static cudaError_t launch_attention_tile(const Kv4AttnParams& p, const AttnPlan& plan, cudaStream_t s) {
+  constexpr int kSmem = kv_smem_bytes(kDim, kGroups, kNT);
+  static OncePerDevice once;
+  const cudaError_t e = once.run([] {
+    return cudaFuncSetAttribute(kv4_attention_kernel<T, kDim, kGroups, kNT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+  });
+  if (e != cudaSuccess) return e;
+  LaunchShape l(dim3(plan.splits, p.sh.heads * plan.tiles, p.batch), 32 * kKvWarps, kSmem, s);
+  return cudaLaunchKernelEx(&l.cfg, kv4_attention_kernel<T, kDim, kGroups, kNT>, p);
+}
+
 template <typename T, int kDim, int kGroups>
 static cudaError_t launch_attention(Kv4AttnParams p, const AttnPlan& plan, cudaStream_t s) {
-  const dim3 grid(plan.splits, p.sh.heads * plan.tiles, p.batch);
-  LaunchShape l(grid, 32 * kKvWarps, 0, s);
-  const cudaError_t e = plan.tile_rows == 8 ? cudaLaunchKernelEx(&l.cfg, kv4_attention_kernel<T, kDim, kGroups, 1>, p)
-                                            : cudaLaunchKernelEx(&l.cfg, kv4_attention_kernel<T, kDim, kGroups, 2>, p);
+  const cudaError_t e = plan.tile_rows == 8 ? launch_attention_tile<T, kDim, kGroups, 1>(p, plan, s)
+                                            : launch_attention_tile<T, kDim, kGroups, 2>(p, plan, s);
   if (e != cudaSuccess || plan.splits == 1) return e;
   qrb200_internal_count_launch();
   LaunchShape j(dim3(ceil_div((int64_t)p.batch * p.queries * p.q_heads, 4)), 128, 0, s);
