@@ -128,10 +128,12 @@ __device__ __forceinline__ float2 kv_step_low(uint32_t w) {
   const Pair16<T> pr = reinterpret_cast<const Pair16<T>&>(w);
   return make_float2(to_f32(pr.s), to_f32(pr.m));
 }
-__device__ __forceinline__ float2 kv_both(float x) { return make_float2(x, x); }
-
 constexpr float kKvLazy = 4.f;      // powers of two that a score may stand above the reference
 constexpr int kKvStepExp = 11;      // the largest step's place: weights stay below 2^(11 + 4) in fp16
+
+__device__ __forceinline__ void mbar_expect(uint32_t mbar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(mbar), "r"(bytes) : "memory");
+}
 
 constexpr int kKvStages = 3;
 // Dynamic shared memory: the warps' rings, reused at the end for their parts of the output.
@@ -216,24 +218,27 @@ __global__ void __launch_bounds__(32 * kKvWarps, kNT == 1 ? 4 : 2) kv4_attention
       page_base = unit * kRuns;
       look_up();
     }
+    const uint32_t bar = smem_u32(&s_full[warp][stage]), dst = smem_u32(ring + stage * kStage);
+    const auto at = [&](int pg, int run) {
+      return P.cache + ((long long)pg * P.sh.heads + head) * P.sh.block_bytes() + (run & (page_runs - 1)) * kRunBytes;
+    };
     unsigned gone = 0;
-    const unsigned char* src[kRuns];
-#pragma unroll
-    for (int i = 0; i < kRuns; ++i) {
-      const int run = unit * kRuns + i, pg = __shfl_sync(kFullMask, page, run - page_base);
-      gone |= pg < 0 ? 1u << i : 0u;
-      src[i] = P.cache + ((long long)pg * P.sh.heads + head) * P.sh.block_bytes() + (run & (page_runs - 1)) * kRunBytes;
+    if (page_runs >= kRuns && (unit + 1) * kRuns <= last_run) {  // one page holds the step: one copy
+      const int run = unit * kRuns, pg = __shfl_sync(kFullMask, page, run - page_base);
+      if (pg < 0) gone = (1u << kRuns) - 1;
+      if (lane == 0) {
+        mbar_expect(bar, pg < 0 ? 0 : kStage);
+        if (pg >= 0) kv_copy(dst, at(pg, run), kStage, bar);
+      }
+    } else {
+      for (int i = 0; i < kRuns; ++i) gone |= __shfl_sync(kFullMask, page, unit * kRuns + i - page_base) < 0 ? 1u << i : 0u;
+      if (lane == 0) mbar_expect(bar, (kRuns - __popc(gone)) * kRunBytes);
+      for (int i = 0; i < kRuns; ++i) {
+        const int run = unit * kRuns + i, pg = __shfl_sync(kFullMask, page, run - page_base);
+        if (lane == 0 && pg >= 0) kv_copy(dst + i * kRunBytes, at(pg, run), kRunBytes, bar);
+      }
     }
     missing = (missing & ~(((1u << kRuns) - 1) << (8 * stage))) | gone << (8 * stage);
-    if (lane == 0) {
-      const uint32_t bar = smem_u32(&s_full[warp][stage]), dst = smem_u32(ring + stage * kStage);
-      asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar),
-                   "r"((kRuns - __popc(gone)) * kRunBytes)
-                   : "memory");
-#pragma unroll
-      for (int i = 0; i < kRuns; ++i)
-        if (!(gone >> i & 1)) kv_copy(dst + i * kRunBytes, src[i], kRunBytes, bar);
-    }
   };
   const int count = u_hi - u;
   if (count > 0) look_up();
@@ -334,9 +339,8 @@ __global__ void __launch_bounds__(32 * kKvWarps, kNT == 1 ? 4 : 2) kv4_attention
                 *reinterpret_cast<const uint32_t*>(runs + i * kRunBytes + 16 * kDim + ((g + 8 * h) * kGroups + gr) * 4));
 #pragma unroll
             for (int n = 0; n < kNT; ++n) {
-              const float2 dot = __fmul2_rn(make_float2(acc[i][n][2 * h], acc[i][n][2 * h + 1]), kv_both(KvKey<T>::kBack));
-              const float2 base = gr ? __ffma2_rn(kv_both(k.y), qsum[n][gr], s[i][n][h]) : __fmul2_rn(kv_both(k.y), qsum[n][gr]);
-              s[i][n][h] = __ffma2_rn(kv_both(k.x), dot, base);
+              s[i][n][h].x = fmaf(k.x, acc[i][n][2 * h] * KvKey<T>::kBack, fmaf(k.y, qsum[n][gr].x, gr ? s[i][n][h].x : 0.f));
+              s[i][n][h].y = fmaf(k.x, acc[i][n][2 * h + 1] * KvKey<T>::kBack, fmaf(k.y, qsum[n][gr].y, gr ? s[i][n][h].y : 0.f));
             }
           }
       }
@@ -430,9 +434,9 @@ __global__ void __launch_bounds__(32 * kKvWarps, kNT == 1 ? 4 : 2) kv4_attention
           // A row that has seen nothing has the reference -inf: its weights, 2^-inf, come from any finite one.
           (c ? less[n].y : less[n].x) = next == kNone ? 0.f : -next;
         }
-        sum[n] = __fmul2_rn(sum[n], make_float2(keep[0], keep[1]));
+        sum[n] = make_float2(sum[n].x * keep[0], sum[n].y * keep[1]);
 #pragma unroll
-        for (int gr = 0; gr < kGroups; ++gr) mids[n][gr] = __fmul2_rn(mids[n][gr], make_float2(keep[0], keep[1]));
+        for (int gr = 0; gr < kGroups; ++gr) mids[n][gr] = make_float2(mids[n][gr].x * keep[0], mids[n][gr].y * keep[1]);
 #pragma unroll
         for (int j = 0; j < kSteps; ++j)
 #pragma unroll
@@ -451,10 +455,10 @@ __global__ void __launch_bounds__(32 * kKvWarps, kNT == 1 ? 4 : 2) kv4_attention
         for (int n = 0; n < kNT; ++n)
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            float2 p = __ffma2_rn(s[i][n][h], kv_both(P.scale2), less[n]);
-            p.x = kv_exp2(p.x);
-            p.y = kv_exp2(p.y);
-            sum[n] = __fadd2_rn(sum[n], p);
+            const float2 p = make_float2(kv_exp2(fmaf(s[i][n][h].x, P.scale2, less[n].x)),
+                                         kv_exp2(fmaf(s[i][n][h].y, P.scale2, less[n].y)));
+            sum[n].x += p.x;
+            sum[n].y += p.y;
             s[i][n][h] = p;
           }
 #pragma unroll
@@ -466,12 +470,16 @@ __global__ void __launch_bounds__(32 * kKvWarps, kNT == 1 ? 4 : 2) kv4_attention
 #pragma unroll
             for (int n = 0; n < kNT; ++n) {
               const float2 p = s[i][n][h];
-              float2 x = __fmul2_rn(p, kv_both(scaled)), m = __fmul2_rn(p, kv_both(val[i][h][gr].y));
-              if constexpr (!kAll) {  // what a row does not see may be NaN
-                if (!(seen[n] >> (4 * i + 2 * h) & 1)) x.x = m.x = 0.f;
-                if (!(seen[n] >> (4 * i + 2 * h) & 2)) x.y = m.y = 0.f;
+              float2 x = make_float2(p.x * scaled, p.y * scaled);
+              if constexpr (kAll) {
+                mids[n][gr].x = fmaf(p.x, val[i][h][gr].y, mids[n][gr].x);
+                mids[n][gr].y = fmaf(p.y, val[i][h][gr].y, mids[n][gr].y);
+              } else {  // what a row does not see may be NaN
+                if (seen[n] >> (4 * i + 2 * h) & 1) mids[n][gr].x = fmaf(p.x, val[i][h][gr].y, mids[n][gr].x);
+                else x.x = 0.f;
+                if (seen[n] >> (4 * i + 2 * h) & 2) mids[n][gr].y = fmaf(p.y, val[i][h][gr].y, mids[n][gr].y);
+                else x.y = 0.f;
               }
-              mids[n][gr] = __fadd2_rn(mids[n][gr], m);
               const uint32_t high = kv_pack(x);
               w[0][n][h] = kv_transpose(high);
               const float2 top = __half22float2(reinterpret_cast<const __half2&>(high));

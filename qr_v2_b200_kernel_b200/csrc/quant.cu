@@ -214,20 +214,19 @@ struct AttnPlan {
   size_t bytes;  // workspace: the parts and their (maximum, sum) pairs
 };
 
-// Eight rows a tile where a key head has no more than eight query rows, else sixteen. The token range
-// is cut so that the CTAs, which the GPU holds `slots` of at a time, fill their last round: the estimated time is rounds x
-// (steps of a warp + what a CTA costs besides, about six steps), over the table's capacity, the one length the host knows.
+// Eight rows a tile where a key head has no more than eight query rows, else sixteen. The token range is cut so that the
+// SMs, which instructions keep busy, get even shares: the estimated time is the most CTAs on one SM x (steps of a warp + what
+// a CTA costs besides, about four steps), and four more for joining, over the table's capacity, the one length the host knows.
 static AttnPlan attn_plan(const Kv4Shape& h, int64_t batch, int64_t queries, int64_t q_heads, int64_t max_pages) {
   AttnPlan p{};
   const int64_t rows = queries * (q_heads / h.heads);
   p.tile_rows = rows <= 8 ? 8 : 16;
   p.tiles = ceil_div(rows, p.tile_rows);
-  const int64_t ctas = batch * h.heads * p.tiles, unit = 16 * kv_runs(h.dim);
+  const int64_t ctas = batch * h.heads * p.tiles, unit = 16 * kv_runs(h.dim), sms = sm_count();
   const int64_t steps = std::max<int64_t>(1, (max_pages * h.page + unit * kKvWarps - 1) / (unit * kKvWarps));
-  const int64_t slots = (int64_t)sm_count() * (p.tile_rows == 8 ? 4 : 2);
   int64_t best = -1;
   for (int64_t n = 1; n <= std::min<int64_t>(steps, 64); ++n) {
-    const int64_t time = (ctas * n + slots - 1) / slots * ((steps + n - 1) / n + 6);
+    const int64_t time = (ctas * n + sms - 1) / sms * ((steps + n - 1) / n + 4) + (n > 1 ? 4 : 0);
     if (best < 0 || time < best) {
       best = time;
       p.splits = (int)n;
