@@ -41,25 +41,6 @@ static bool type16_ok(int t) { return t == QRB200_BF16 || t == QRB200_F16; }
 constexpr int kMaxCols = 32768;
 constexpr int64_t kMaxRows = (1ll << 31) - 1;
 
-template <typename T, bool kNorm>
-static int launch_rows(const RowsParams& p, int weight_type, int dtype, cudaStream_t s) {
-  const unsigned grid = (unsigned)p.rows;
-  if (p.weight && weight_type == QRB200_F32 && dtype != QRB200_F32)
-    rows_int8_kernel<T, float, kNorm><<<grid, 256, 0, s>>>(p);
-  else
-    rows_int8_kernel<T, T, kNorm><<<grid, 256, 0, s>>>(p);
-  return launched();
-}
-
-template <bool kNorm>
-static int rows_int8(const RowsParams& p, int weight_type, int dtype, cudaStream_t s) {
-  switch (dtype) {
-    case QRB200_BF16: return launch_rows<__nv_bfloat16, kNorm>(p, weight_type, dtype, s);
-    case QRB200_F16: return launch_rows<__half, kNorm>(p, weight_type, dtype, s);
-    default: return launch_rows<float, kNorm>(p, weight_type, dtype, s);
-  }
-}
-
 static PFN_cuTensorMapEncodeTiled_v12000 map_encoder() {
   static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
   static std::once_flag once;
@@ -139,6 +120,65 @@ static int sm_count() {
 }
 
 static int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
+
+// Packs of a row to a thread, by the row's length: four (enough loads in flight, few threads at the two reductions), fewer
+// where that would leave a warp idle. Short rows go several to a block, a warp each, where there are rows enough.
+template <typename T, typename W, bool kNorm, bool kAligned>
+static cudaError_t launch_rows_of(const RowsParams& p, cudaStream_t s) {
+  const int packs = ceil_div(p.cols, 16 / sizeof(T));
+  const int items = packs <= 32 ? 1 : packs <= 64 ? 2 : packs <= 4096 ? 4 : 8;
+  const int threads = ceil_div(ceil_div(packs, items), 32) * 32;
+  const int y = threads == 32 && p.rows > 4 * sm_count() ? 8 : 1;
+  LaunchShape l(dim3(ceil_div(p.rows, y)), threads, 0, s);
+  l.cfg.blockDim.y = y;
+  switch (items) {
+    case 1: return cudaLaunchKernelEx(&l.cfg, rows_int8_kernel<T, W, kNorm, kAligned, 1>, p);
+    case 2: return cudaLaunchKernelEx(&l.cfg, rows_int8_kernel<T, W, kNorm, kAligned, 2>, p);
+    case 4: return cudaLaunchKernelEx(&l.cfg, rows_int8_kernel<T, W, kNorm, kAligned, 4>, p);
+  }
+  if constexpr (sizeof(T) == 4) return cudaLaunchKernelEx(&l.cfg, rows_int8_kernel<T, W, kNorm, kAligned, 8>, p);
+  return cudaErrorInvalidValue;  // 16-bit rows of up to 32768 have 4096 packs
+}
+
+template <typename T, bool kNorm>
+static int launch_rows(const RowsParams& p, int weight_type, int dtype, cudaStream_t s) {
+  constexpr int kVec = 16 / sizeof(T);
+  const auto off = [](const void* q) { return (reinterpret_cast<uintptr_t>(q) & 15u) != 0; };
+  const bool aligned = p.cols % kVec == 0 && !off(p.x) && !off(p.residual) && !off(p.weight) && !off(p.h_out) && !off(p.q) &&
+                       p.x_stride % kVec == 0 && p.r_stride % kVec == 0 && p.q_stride % 16 == 0;
+  cudaError_t e;
+  if (p.weight && weight_type == QRB200_F32 && dtype != QRB200_F32)
+    e = aligned ? launch_rows_of<T, float, kNorm, true>(p, s) : launch_rows_of<T, float, kNorm, false>(p, s);
+  else
+    e = aligned ? launch_rows_of<T, T, kNorm, true>(p, s) : launch_rows_of<T, T, kNorm, false>(p, s);
+  if (e != cudaSuccess) return QRB200_ERR_CUDA;
+  return launched();
+}
+
+template <typename T>
+static int launch_dequant(const int8_t* q, int64_t q_stride, const float* scale, void* out, int64_t rows, int64_t cols,
+                          cudaStream_t s) {
+  const bool vec = cols % 16 == 0 && q_stride % 16 == 0 &&
+                   ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) & 15u) == 0;
+  const int64_t packs = rows * (vec ? cols / 16 : cols);
+  if (packs > ((int64_t)1 << 38)) return QRB200_ERR_ARG;
+  LaunchShape l(dim3(ceil_div(packs, 256)), 256, 0, s);
+  const cudaError_t e =
+      vec ? cudaLaunchKernelEx(&l.cfg, dequant_rows_kernel<T, 16>, q, (long long)q_stride, scale, static_cast<T*>(out), (long long)rows, (int)cols)
+          : cudaLaunchKernelEx(&l.cfg, dequant_rows_kernel<T, 1>, q, (long long)q_stride, scale, static_cast<T*>(out), (long long)rows, (int)cols);
+  if (e != cudaSuccess) return QRB200_ERR_CUDA;
+  return launched();
+}
+
+template <bool kNorm>
+static int rows_int8(const RowsParams& p, int weight_type, int dtype, cudaStream_t s) {
+  switch (dtype) {
+    case QRB200_BF16: return launch_rows<__nv_bfloat16, kNorm>(p, weight_type, dtype, s);
+    case QRB200_F16: return launch_rows<__half, kNorm>(p, weight_type, dtype, s);
+    default: return launch_rows<float, kNorm>(p, weight_type, dtype, s);
+  }
+}
+
 
 template <typename T, int kBN>
 static cudaError_t launch_i8_few(const I8Params& p, const I8Operand& x, const I8Operand& w, cudaStream_t s) {
@@ -312,14 +352,9 @@ int qrb200_dequantize_int8(const int8_t* q, int64_t q_stride, const float* scale
   const int st = quant_ready();
   if (st != QRB200_OK) return st;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const unsigned grid = (unsigned)rows;
-  if (dtype == QRB200_BF16)
-    dequant_rows_kernel<<<grid, 256, 0, s>>>(q, q_stride, scale, static_cast<__nv_bfloat16*>(out), rows, (int)cols);
-  else if (dtype == QRB200_F16)
-    dequant_rows_kernel<<<grid, 256, 0, s>>>(q, q_stride, scale, static_cast<__half*>(out), rows, (int)cols);
-  else
-    dequant_rows_kernel<<<grid, 256, 0, s>>>(q, q_stride, scale, static_cast<float*>(out), rows, (int)cols);
-  return launched();
+  if (dtype == QRB200_BF16) return launch_dequant<__nv_bfloat16>(q, q_stride, scale, out, rows, cols, s);
+  if (dtype == QRB200_F16) return launch_dequant<__half>(q, q_stride, scale, out, rows, cols, s);
+  return launch_dequant<float>(q, q_stride, scale, out, rows, cols, s);
 }
 
 int qrb200_int8_linear(const int8_t* x, int64_t x_stride, const float* x_scale, const int8_t* w, int64_t w_stride,

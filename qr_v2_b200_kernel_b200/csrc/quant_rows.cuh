@@ -44,66 +44,154 @@ struct RowsParams {
   float eps;
 };
 
-// One CTA per row, any alignment: the simplest form.
-template <typename T, typename W, bool kNorm>
-__global__ void __launch_bounds__(256) rows_int8_kernel(RowsParams P) {
-  const long long row = blockIdx.x;
-  const T* x = static_cast<const T*>(P.x) + row * P.x_stride;
-  const T* r = P.residual ? static_cast<const T*>(P.residual) + row * P.r_stride : nullptr;
-  const W* w = static_cast<const W*>(P.weight);
-  T* ho = P.h_out ? static_cast<T*>(P.h_out) + row * P.cols : nullptr;
-  int8_t* q = P.q + row * P.q_stride;
-  __shared__ float s_sum[8];
-  __shared__ unsigned s_top[8];
-  float sum = 0.f;
-  unsigned top = 0;  // bits of the largest |t|: ordered as unsigned, with NaN above infinity
-  auto value = [&](int c, float& h) {
-    h = to_f32(x[c]);
-    if (r) h += to_f32(r[c]);
-    return w ? h * to_f32(w[c]) : h;
-  };
-  for (int c = threadIdx.x; c < P.cols; c += 256) {
-    float h;
-    const float t = value(c, h);
-    if (ho) ho[c] = from_f32<T>(h);
-    sum = fmaf(h, h, sum);
-    top = max(top, __float_as_uint(t) & 0x7fffffffu);
+// A pack is 16 bytes of consecutive elements: one load or store where all rows start on 16-byte boundaries and hold whole
+// packs (kAligned), else its `n` elements one by one.
+template <bool kAligned, typename T, int kVec>
+__device__ __forceinline__ void load_pack(T (&v)[kVec], const T* p, int n) {
+  if constexpr (kAligned) {
+#pragma unroll
+    for (int i = 0; i < kVec; i += 16 / sizeof(T))
+      *reinterpret_cast<uint4*>(v + i) = __ldg(reinterpret_cast<const uint4*>(p + i));
+  } else {
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) v[i] = i < n ? __ldg(p + i) : from_f32<T>(0.f);
   }
-  top = __reduce_max_sync(kFullMask, top);
-  for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(kFullMask, sum, o);
-  if ((threadIdx.x & 31) == 0) {
-    s_sum[threadIdx.x >> 5] = sum;
-    s_top[threadIdx.x >> 5] = top;
-  }
-  __syncthreads();
-  sum = 0.f;
-  top = 0;
-  for (int i = 0; i < 8; ++i) {
-    sum += s_sum[i];
-    top = max(top, s_top[i]);
-  }
-  const float a = __uint_as_float(top);
-  const bool finite = top < 0x7f800000u, tiny = a < kTinyRow;
-  const float inv = finite && !tiny ? __fmul_rn(__frcp_rn(a), 127.f) : 0.f;
-  if (threadIdx.x == 0) {
-    const float rms = kNorm ? rsqrtf(sum / (float)P.cols + P.eps) : 1.f;
-    P.scale[row] = !finite ? __int_as_float(0x7fffffff) : tiny ? 0.f : a * rms / 127.f;
-  }
-  for (int c = threadIdx.x; c < P.cols; c += 256) {
-    float h;
-    const float t = value(c, h);
-    q[c] = finite ? (int8_t)__float2int_rn(__fmul_rn(t, inv)) : 0;
+}
+template <bool kAligned, typename T, int kVec>
+__device__ __forceinline__ void store_pack(T* p, const T (&v)[kVec], int n) {
+  if constexpr (kAligned) {
+#pragma unroll
+    for (int i = 0; i < kVec; i += 16 / sizeof(T)) *reinterpret_cast<uint4*>(p + i) = *reinterpret_cast<const uint4*>(v + i);
+  } else {
+#pragma unroll
+    for (int i = 0; i < kVec; ++i)
+      if (i < n) p[i] = v[i];
   }
 }
 
-// value = code * scale of its row, rounded once.
-template <typename T>
+// A row lives in the registers of blockDim.x threads, kItems packs each, a block's y rows beside one another:
+// memory is read once and written once, and bounds it. Every load of the row is asked for before the first is used. Which
+// thread holds which element depends on the row's length alone, so a row's result, bit for bit, depends on
+// neither its neighbours, their number nor anybody's alignment.
+template <typename T, typename W, bool kNorm, bool kAligned, int kItems>
+__global__ void __launch_bounds__(1024) rows_int8_kernel(RowsParams P) {
+  constexpr int kVec = 16 / sizeof(T);
+  __shared__ float s_sum[32];
+  __shared__ unsigned s_top[32];
+  griddep_launch_wait();
+  const long long row = (long long)blockIdx.x * blockDim.y + threadIdx.y;
+  const bool in = row < P.rows;
+  const int packs = (P.cols + kVec - 1) / kVec, tid = threadIdx.x, threads = blockDim.x;
+  const T* x = static_cast<const T*>(P.x) + row * P.x_stride;
+  const T* r = static_cast<const T*>(P.residual) + row * P.r_stride;
+  const W* w = static_cast<const W*>(P.weight);
+  T xv[kItems][kVec], rv[kItems][kVec];
+  float t[kItems][kVec];
+#pragma unroll
+  for (int i = 0; i < kItems; ++i) {
+    const int c = tid + i * threads;
+    if (!in || c >= packs) continue;
+    load_pack<kAligned>(xv[i], x + c * kVec, P.cols - c * kVec);
+    if (kNorm && P.residual) load_pack<kAligned>(rv[i], r + c * kVec, P.cols - c * kVec);
+  }
+  float sum = 0.f;
+  unsigned top = 0;  // bits of the largest |t|: ordered as unsigned, with NaN above infinity
+#pragma unroll
+  for (int i = 0; i < kItems; ++i) {
+    const int c = tid + i * threads;
+    if (!in || c >= packs) continue;
+#pragma unroll
+    for (int e = 0; e < kVec; ++e) t[i][e] = to_f32(xv[i][e]);
+    if constexpr (kNorm) {
+      if (P.residual) {
+#pragma unroll
+        for (int e = 0; e < kVec; ++e) {
+          t[i][e] += to_f32(rv[i][e]);
+          rv[i][e] = from_f32<T>(t[i][e]);
+        }
+        store_pack<kAligned>(static_cast<T*>(P.h_out) + row * P.cols + c * kVec, rv[i], P.cols - c * kVec);
+      }
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) sum = fmaf(t[i][e], t[i][e], sum);
+      if (w) {
+        W wv[kVec];
+        load_pack<kAligned>(wv, w + c * kVec, P.cols - c * kVec);
+#pragma unroll
+        for (int e = 0; e < kVec; ++e) t[i][e] *= to_f32(wv[e]);
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < kVec; ++e) top = max(top, __float_as_uint(t[i][e]) & 0x7fffffffu);
+  }
+  top = __reduce_max_sync(kFullMask, top);
+  if constexpr (kNorm)
+    for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(kFullMask, sum, o);
+  if (threads > 32) {  // one row to the block
+    const int warps = threads >> 5;
+    if ((tid & 31) == 0) {
+      s_sum[tid >> 5] = sum;
+      s_top[tid >> 5] = top;
+    }
+    __syncthreads();
+    sum = (tid & 31) < warps ? s_sum[tid & 31] : 0.f;
+    top = __reduce_max_sync(kFullMask, (tid & 31) < warps ? s_top[tid & 31] : 0u);
+    for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(kFullMask, sum, o);
+  }
+  if (!in) return;
+  const float a = __uint_as_float(top);
+  const bool finite = top < 0x7f800000u, tiny = a < kTinyRow;
+  const float inv = finite && !tiny ? __fmul_rn(__frcp_rn(a), 127.f) : 0.f;
+  if (tid == 0) {
+    const float rms = kNorm ? rsqrtf(sum / (float)P.cols + P.eps) : 1.f;
+    P.scale[row] = !finite ? __int_as_float(0x7fffffff) : tiny ? 0.f : a * rms / 127.f;
+  }
+  int8_t* q = P.q + row * P.q_stride;
+#pragma unroll
+  for (int i = 0; i < kItems; ++i) {
+    const int c = tid + i * threads;
+    if (c >= packs) continue;
+    uint32_t word[kVec / 4] = {};
+#pragma unroll
+    for (int e = 0; e < kVec; ++e) {
+      const int code = finite ? __float2int_rn(__fmul_rn(t[i][e], inv)) : 0;
+      word[e / 4] |= (uint32_t)(code & 255) << (8 * (e & 3));
+    }
+    if constexpr (!kAligned) {
+      store_pack<false>(q + c * kVec, reinterpret_cast<const int8_t(&)[kVec]>(word), P.cols - c * kVec);
+    } else if constexpr (kVec == 8) {
+      *reinterpret_cast<uint2*>(q + c * 8) = make_uint2(word[0], word[1]);
+    } else {
+      *reinterpret_cast<uint32_t*>(q + c * 4) = word[0];
+    }
+  }
+}
+
+// value = code * scale of its row, rounded once. One pack of kVec codes to a thread, rows end to end.
+template <typename T, int kVec>
 __global__ void __launch_bounds__(256) dequant_rows_kernel(const int8_t* q, long long q_stride, const float* scale,
                                                            T* out, long long rows, int cols) {
-  const long long row = blockIdx.x;
+  griddep_launch_wait();
+  const int packs = cols / kVec;
+  const long long at = (long long)blockIdx.x * 256 + threadIdx.x;
+  // The division is in 32 bits where the index fits it.
+  const long long row = at <= 0xffffffffll ? (long long)((uint32_t)at / (uint32_t)packs) : at / packs;
+  if (row >= rows) return;
+  const int c = (int)(at - row * packs) * kVec;
   const float s = scale[row];
-  for (int c = threadIdx.x; c < cols; c += 256)
+  if constexpr (kVec == 16) {
+    const int4 codes = __ldg(reinterpret_cast<const int4*>(q + row * q_stride + c));
+    const int8_t* code = reinterpret_cast<const int8_t*>(&codes);
+    constexpr int kPart = 16 / sizeof(T);
+#pragma unroll
+    for (int h = 0; h < 16; h += kPart) {
+      T v[kPart];
+#pragma unroll
+      for (int e = 0; e < kPart; ++e) v[e] = from_f32<T>((float)code[h + e] * s);
+      store_pack<true>(out + row * cols + c + h, v, kPart);
+    }
+  } else {
     out[row * cols + c] = from_f32<T>((float)q[row * q_stride + c] * s);
+  }
 }
 
 }  // namespace qrb200
