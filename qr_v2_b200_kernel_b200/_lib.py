@@ -73,7 +73,7 @@ SIGNATURES = {
     "qrb200_kv4_block_bytes": (_I64, [_I64, _I64, _I64]),
     "qrb200_kv4_write": (_INT, [_P, _P, _P, _I64, _I64, _P, _I64, _I64, _P, _I64, _P]),
     "qrb200_kv4_read": (_INT, [_P, _P, _P, _P, _P, _I64, _P]),
-    "qrb200_kv4_attention_workspace_bytes": (_SIZE, [_P, _I64, _I64, _I64, _I64]),
+    "qrb200_kv4_attention_workspace_bytes": (_SIZE, [_P, _I64, _I64, _I64, _I64, _I64]),
     "qrb200_kv4_attention": (_INT, [_P, _P, _P, _P, _P, _I64, _P, _P, _I64, _I64, _I64, _I64, _I64, _INT, _F32, _P,
                                     _SIZE, _P]),
 }

@@ -7,8 +7,8 @@
 
 #include <cuda.h>
 
+#include "cluster.cuh"
 #include "quant_rows.cuh"
-#include "tc.cuh"
 
 namespace qrb200 {
 
@@ -58,28 +58,12 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, int (&v)[16]) {
       : "r"(taddr));
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
-__device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-__device__ __forceinline__ uint32_t cluster_rank() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-  return r;
-}
-__device__ __forceinline__ int ld_cluster(uint32_t addr, uint32_t rank) {
-  uint32_t a;
-  int v;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(addr), "r"(rank));
-  asm volatile("ld.shared::cluster.b32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
-  return v;
-}
-
 // ---- few rows ------------------------------------------------------------------------------
 //
 // With few rows the weights are the traffic, so they are the 128-row operand (M = output
 // channels) and the rows of x the narrow one (N = kBN): no tensor-core row is wasted on padding.
-// The depth is cut over the cluster's CTAs so that every SM streams weights, and their integer
-// sums are added through distributed shared memory, exactly, in the one launch.
+// The depth is cut over the cluster's CTAs so that every SM streams weights; each CTA then adds all the CTAs' integer sums
+// of some rows of x, exactly, through distributed shared memory, in the one launch.
 //
 // Warp 0 issues the loads, warp 1 the MMAs, warps 2-5 hold one output channel a lane.
 template <int kBN>
@@ -88,6 +72,7 @@ struct I8Few {
   static constexpr int kStages = kBN <= 32 ? 4 : 3;
   static constexpr int kCols = kBN < 32 ? 32 : kBN;  // TMEM columns
   static constexpr size_t smem() { return 1024 + (size_t)kStages * kStage; }
+  static_assert(kBN * 128 * 4 <= kStages * kStage, "the sums take the ring's place");
 };
 
 template <typename T, int kBN>
@@ -173,8 +158,8 @@ __global__ void __launch_bounds__(192) i8_few_kernel(I8Params P, const __grid_co
   };
   if (epi && !mbar_wait(&done, 0)) s_bad = 1;
   tc_fence_after();
+  __syncthreads();
   if (split == 1) {
-    __syncthreads();
     if (epi && !s_bad)
 #pragma unroll 1
       for (int j = 0; j < kBN && i0 + j < P.rows; j += 16) {
@@ -184,7 +169,7 @@ __global__ void __launch_bounds__(192) i8_few_kernel(I8Params P, const __grid_co
         for (int q = 0; q < 16; ++q) put(j + q, v[q]);
       }
   } else {
-    // The ring is free: every load has landed and every MMA is done. Sums as [row][channel].
+    // The ring is free (every load has landed, every MMA is done): sums as [row][channel]. Row j is CTA j % split's to add.
     int* sums = reinterpret_cast<int*>(ring);
     if (epi)
 #pragma unroll 1
@@ -194,16 +179,43 @@ __global__ void __launch_bounds__(192) i8_few_kernel(I8Params P, const __grid_co
 #pragma unroll
         for (int q = 0; q < 16; ++q) sums[(j + q) * 128 + ch] = v[q];
       }
-    __syncthreads();
     cluster_sync();
     bool bad = false;
     for (int r = 0; r < split; ++r) bad = ld_cluster(smem_u32(&s_bad), r) != 0 || bad;
-    if (epi && !bad)
-      for (int j = part; j < kBN && i0 + j < P.rows; j += split) {
-        int acc = 0;
-        for (int r = 0; r < split; ++r) acc += ld_cluster(smem_u32(&sums[j * 128 + ch]), r);
-        put(j, acc);
+    if (epi && !bad) {
+      // A warp to a row, four channels a lane.
+      const int c4 = 4 * lane, et = threadIdx.x >> 5;
+      float w4[4], b4[4];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const bool in = n0 + c4 + c < P.outs;
+        w4[c] = in ? P.sw[n0 + c4 + c] : 0.f;
+        b4[c] = in && P.bias ? to_f32(static_cast<const T*>(P.bias)[n0 + c4 + c]) : 0.f;
       }
+      for (int j = part + split * (et - 2); j < kBN && i0 + j < P.rows; j += 4 * split) {
+        int4 acc = make_int4(0, 0, 0, 0);
+#pragma unroll
+        for (int r = 0; r < 8; ++r)
+          if (r < split) {
+            const int4 v = ld_cluster4(smem_u32(&sums[j * 128 + c4]), r);
+            acc.x += v.x, acc.y += v.y, acc.z += v.z, acc.w += v.w;
+          }
+        const float sx = P.sx[i0 + j];
+        alignas(16) T out[4] = {from_f32<T>(fmaf((float)acc.x * sx, w4[0], b4[0])), from_f32<T>(fmaf((float)acc.y * sx, w4[1], b4[1])),
+                                from_f32<T>(fmaf((float)acc.z * sx, w4[2], b4[2])), from_f32<T>(fmaf((float)acc.w * sx, w4[3], b4[3]))};
+        T* to = y + (long long)(i0 + j) * P.outs + n0 + c4;
+        if (P.outs % 4 == 0) {
+          if (n0 + c4 < P.outs) {
+            if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4*>(to) = *reinterpret_cast<const uint4*>(out);
+            else *reinterpret_cast<uint2*>(to) = *reinterpret_cast<const uint2*>(out);
+          }
+        } else {
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+            if (n0 + c4 + c < P.outs) to[c] = out[c];
+        }
+      }
+    }
     cluster_sync();  // nobody leaves while its sums are being read
   }
   tc_fence_before();

@@ -24,13 +24,15 @@
 //     tokens written at the same time by different threads never share one.
 #pragma once
 
+#include <type_traits>
+
 #include "quant_rows.cuh"
 #include "tc.cuh"
 
 namespace qrb200 {
 
 struct Kv4Shape {
-  int heads, page, dim, groups;  // groups per head
+  int heads, page, dim, groups, shift;  // groups per head; page = 2^shift
   long long pages;
   __host__ __device__ int run_bytes() const { return 16 * dim + 128 * groups; }
   __host__ __device__ int block_bytes() const { return page / 16 * run_bytes(); }
@@ -40,6 +42,34 @@ template <typename T>
 struct Pair16 {
   T s, m;
 };
+
+template <typename T>
+struct Two;
+template <>
+struct Two<__nv_bfloat16> {
+  using type = __nv_bfloat162;
+};
+template <>
+struct Two<__half> {
+  using type = __half2;
+};
+// (least, -greatest) of eight numbers, NaN if one is.
+template <typename T>
+__device__ __forceinline__ typename Two<T>::type kv4_ends(const T (&x)[8]) {
+  using T2 = typename Two<T>::type;
+  const T2* p = reinterpret_cast<const T2*>(x);
+  const T2 lo = __hmin2_nan(__hmin2_nan(p[0], p[1]), __hmin2_nan(p[2], p[3]));
+  const T2 hi = __hmax2_nan(__hmax2_nan(p[0], p[1]), __hmax2_nan(p[2], p[3]));
+  T2 r;
+  r.x = __hmin_nan(lo.x, lo.y);
+  r.y = __hneg(__hmax_nan(hi.x, hi.y));
+  return r;
+}
+// Nibble codes at bits 0 and 16 of w as two numbers.
+__device__ __forceinline__ float2 kv4_codes(uint32_t w) {
+  const uint32_t x = (w & 0x000f000fu) | 0x64006400u;
+  return __half22float2(__hsub2(reinterpret_cast<const __half2&>(x), __floats2half2_rn(1024.f, 1024.f)));
+}
 
 struct Kv4IoParams {
   unsigned char* cache;
@@ -55,27 +85,28 @@ struct Kv4IoParams {
 // Where a token's run lies, or null for a slot that is skipped; an index past the cache is reported.
 __device__ __forceinline__ unsigned char* kv4_run(const Kv4IoParams& P, long long slot, int head, bool report) {
   if (slot < 0) return nullptr;
-  const long long page = slot / P.sh.page;
+  const long long page = slot >> P.sh.shift;
   if (page >= P.sh.pages) {
     if (report) report_device_failure(kSiteIndex);
     return nullptr;
   }
-  return P.cache + (page * P.sh.heads + head) * P.sh.block_bytes() + (int)(slot % P.sh.page) / 16 * P.sh.run_bytes();
+  return P.cache + (page * P.sh.heads + head) * P.sh.block_bytes() + ((int)slot & (P.sh.page - 1)) / 16 * P.sh.run_bytes();
 }
 
 // Sixteen tokens of one head to a CTA, kDim / 8 threads to a token, 8 channels (16 bytes) to a thread. Bandwidth
 // bounds it: everything a thread reads is asked for before anything is computed. When the sixteen fill a run, as
 // prompts do, the run is put together in shared memory and stored whole; otherwise each thread stores its words (keys) and
-// bytes (values).
-template <typename T, int kDim, bool kVec>
+// bytes (values). Long prompts are bound by instructions: codes come out of the 32-bit floating sum's bits, packed as they lie.
+template <typename T, int kDim, int kGroups, bool kVec>
 __global__ void __launch_bounds__(2 * kDim) kv4_write_kernel(Kv4IoParams P) {
-  constexpr int kChunks = kDim / 8;
-  extern __shared__ uint4 s_run[];
+  constexpr int kChunks = kDim / 8, kSpan = kChunks / kGroups;  // threads of a token, of a group
+  constexpr int kRunBytes = 16 * kDim + 128 * kGroups;
+  __shared__ uint4 s_run[kRunBytes / 16];
   griddep_launch_wait();
   const int chunk = threadIdx.x % kChunks, mine = threadIdx.x / kChunks, head = blockIdx.y;
   const long long first = (long long)blockIdx.x * 16, tok = first + mine;
   const bool in = tok < P.tokens;
-  T x[2][8];
+  alignas(16) T x[2][8];
 #pragma unroll
   for (int part = 0; part < 2; ++part) {
     const T* src = (part ? static_cast<const T*>(P.v) + tok * P.v_ts + head * P.v_hs
@@ -91,23 +122,19 @@ __global__ void __launch_bounds__(2 * kDim) kv4_write_kernel(Kv4IoParams P) {
   const bool whole = __syncthreads_and(in && slot == slot0 + mine && (slot0 & 15) == 0);
   unsigned char* run = kv4_run(P, slot, head, chunk == 0);
   unsigned char* out = whole ? reinterpret_cast<unsigned char*>(s_run) : run;
-  const int at = whole ? mine : (int)(slot & 15), span = kChunks / P.sh.groups;  // threads of a group
+  const int at = whole ? mine : (int)(slot & 15);
 #pragma unroll
   for (int part = 0; part < 2; ++part) {
-    float f[8], lo, hi;
-    bool fine = true;
+    // The group's ends, exact in 16 bits: this thread's eight channels two at a time, then (lo, -hi) over the group's threads.
+    // NaN carries through; infinity shows at an end.
+    typename Two<T>::type ends = kv4_ends(x[part]);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      f[i] = to_f32(x[part][i]);
-      fine = fine && fabsf(f[i]) < __int_as_float(0x7f800000);
-      lo = i ? fminf(lo, f[i]) : f[i];
-      hi = i ? fmaxf(hi, f[i]) : f[i];
+    for (int o = kSpan >> 1; o; o >>= 1) {
+      const uint32_t other = __shfl_xor_sync(kFullMask, reinterpret_cast<const uint32_t&>(ends), o);
+      ends = __hmin2_nan(ends, reinterpret_cast<const typename Two<T>::type&>(other));
     }
-    for (int o = span >> 1; o; o >>= 1) {
-      lo = fminf(lo, __shfl_xor_sync(kFullMask, lo, o));
-      hi = fmaxf(hi, __shfl_xor_sync(kFullMask, hi, o));
-      fine = __shfl_xor_sync(kFullMask, (int)fine, o) && fine;
-    }
+    const float lo = to_f32(ends.x), hi = -to_f32(ends.y);
+    const bool fine = fabsf(lo) < __int_as_float(0x7f800000) && fabsf(hi) < __int_as_float(0x7f800000);
     constexpr float kFifteenth = 1.f / 15.f;
     const float nan = __int_as_float(0x7fffffff);
     Pair16<T> pr;
@@ -115,23 +142,31 @@ __global__ void __launch_bounds__(2 * kDim) kv4_write_kernel(Kv4IoParams P) {
     pr.m = from_f32<T>(fine ? lo : nan);
     const float s = to_f32(pr.s), m = to_f32(pr.m);
     const float inv = s >= 0x1p-126f ? __frcp_rn(s) : 0.f;
+    // x - m is never negative. Added to 1.5 2^23, a number below 2^22 leaves its nearest whole number (ties to even) in the
+    // low bits, above a constant that the packing takes off. Where s is normal, its rounding keeps every code below 15.5.
     uint32_t code[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      code[i] = fine ? (uint32_t)fminf(fmaxf(rintf(__fmul_rn(__fsub_rn(f[i], m), inv)), 0.f), 15.f) : 0u;
+    for (int i = 0; i < 8; ++i) {
+      float steps = __fmul_rn(__fsub_rn(to_f32(x[part][i]), m), inv);
+      if constexpr (std::is_same<T, __half>::value) steps = fminf(steps, 15.f);  // subnormal steps
+      code[i] = __float_as_uint(__fadd_rn(fine ? steps : 0.f, 0x1.8p23f));
+    }
+    constexpr uint32_t kBits = 0x4b400000u;
     if (part == 0) {
       // Step j = chunk / 2, t = 2 (chunk & 1) and the next; the other half of each word, step j ^ 1, is chunk ^ 2's.
       const int up = (chunk & 2) ? 8 : 0;
-      const uint32_t a = (code[0] | code[1] << 16 | code[2] << 4 | code[3] << 20) << up;
-      const uint32_t b = (code[4] | code[5] << 16 | code[6] << 4 | code[7] << 20) << up;
+      constexpr uint32_t kAll = kBits + (kBits << 16) + (kBits << 4) + (kBits << 20);
+      const uint32_t a = (code[0] + (code[1] << 16) + (code[2] << 4) + (code[3] << 20) - kAll) << up;
+      const uint32_t b = (code[4] + (code[5] << 16) + (code[6] << 4) + (code[7] << 20) - kAll) << up;
       const uint32_t got = __shfl_xor_sync(kFullMask, up ? a : b, 2), word = (up ? b : a) | got;
       const int t = 2 * (chunk & 1) + (up ? 1 : 0);
       if (out) *reinterpret_cast<uint32_t*>(out + at * (kDim / 2) + t * (kDim / 8) + (chunk >> 2) * 4) = word;
     } else {
       // Tile chunk / 2; an even chunk has the low nibbles of its 8 bytes, its odd neighbour the high ones.
       const bool odd = chunk & 1;
-      const uint32_t a = code[0] | code[1] << 8 | code[2] << 16 | code[3] << 24;
-      const uint32_t b = code[4] | code[5] << 8 | code[6] << 16 | code[7] << 24;
+      constexpr uint32_t kAll = kBits + (kBits << 8) + (kBits << 16) + (kBits << 24);
+      const uint32_t a = code[0] + (code[1] << 8) + (code[2] << 16) + (code[3] << 24) - kAll;
+      const uint32_t b = code[4] + (code[5] << 8) + (code[6] << 16) + (code[7] << 24) - kAll;
       const uint32_t got = __shfl_xor_sync(kFullMask, odd ? a : b, 1), bytes = odd ? got | b << 4 : a | got << 4;
       const int tile = chunk >> 1, byte = 2 * (at & 1) + (at >> 3), lane = (odd ? 16 : 0) + ((at & 7) >> 1);
       if (out) {
@@ -140,23 +175,23 @@ __global__ void __launch_bounds__(2 * kDim) kv4_write_kernel(Kv4IoParams P) {
         for (int i = 0; i < 4; ++i) v[64 * i] = (unsigned char)(bytes >> (8 * i));
       }
     }
-    if (out && chunk % span == 0)
-      reinterpret_cast<Pair16<T>*>(out + 16 * kDim + part * 64 * P.sh.groups)[at * P.sh.groups + chunk / span] = pr;
+    if (out && chunk % kSpan == 0)
+      reinterpret_cast<Pair16<T>*>(out + 16 * kDim + part * 64 * kGroups)[at * kGroups + chunk / kSpan] = pr;
   }
   if (whole) {
     __syncthreads();
     unsigned char* to = kv4_run(P, slot0, head, false);
-    const int pieces = P.sh.run_bytes() / 16;
     if (to)
-      for (int i = threadIdx.x; i < pieces; i += 2 * kDim) reinterpret_cast<uint4*>(to)[i] = s_run[i];
+      for (int i = threadIdx.x; i < kRunBytes / 16; i += 2 * kDim) reinterpret_cast<uint4*>(to)[i] = s_run[i];
   }
 }
 
 // The values at slots, as kv4_write_kernel cuts them; a negative slot reads as zeros.
-template <typename T, int kDim>
+template <typename T, int kDim, int kGroups>
 __global__ void __launch_bounds__(2 * kDim) kv4_read_kernel(Kv4IoParams P) {
-  constexpr int kChunks = kDim / 8;
-  extern __shared__ uint4 s_run[];
+  constexpr int kChunks = kDim / 8, kSpan = kChunks / kGroups;  // threads of a token, of a group
+  constexpr int kRunBytes = 16 * kDim + 128 * kGroups;
+  __shared__ uint4 s_run[kRunBytes / 16];
   griddep_launch_wait();
   const int chunk = threadIdx.x % kChunks, mine = threadIdx.x / kChunks, head = blockIdx.y;
   const long long first = (long long)blockIdx.x * 16, tok = first + mine;
@@ -166,37 +201,38 @@ __global__ void __launch_bounds__(2 * kDim) kv4_read_kernel(Kv4IoParams P) {
   const unsigned char* run = kv4_run(P, slot, head, chunk == 0);
   if (whole) {
     const uint4* from = reinterpret_cast<const uint4*>(kv4_run(P, slot0, head, false));
-    const int pieces = P.sh.run_bytes() / 16;
     if (from)
-      for (int i = threadIdx.x; i < pieces; i += 2 * kDim) s_run[i] = from[i];
+      for (int i = threadIdx.x; i < kRunBytes / 16; i += 2 * kDim) s_run[i] = from[i];
     __syncthreads();
     if (run) run = reinterpret_cast<const unsigned char*>(s_run);
   }
   if (!in) return;
-  const int at = (int)(slot & 15), group = chunk * P.sh.groups / kChunks;
+  const int at = (int)(slot & 15);
   const long long to = (tok * P.sh.heads + head) * kDim + 8 * chunk;
 #pragma unroll
   for (int part = 0; part < 2; ++part) {
-    uint32_t code[8];
-    T out[8];
+    float2 code[4];
+    alignas(16) T out[8];
     if (run) {
       if (part == 0) {
         const unsigned char* w = run + at * (kDim / 2) + 2 * (chunk & 1) * (kDim / 8) + (chunk >> 2) * 4;
         const int up = (chunk & 2) ? 8 : 0;
         const uint32_t a = *reinterpret_cast<const uint32_t*>(w) >> up, b = *reinterpret_cast<const uint32_t*>(w + kDim / 8) >> up;
-        code[0] = a & 15, code[1] = a >> 16 & 15, code[2] = a >> 4 & 15, code[3] = a >> 20 & 15;
-        code[4] = b & 15, code[5] = b >> 16 & 15, code[6] = b >> 4 & 15, code[7] = b >> 20 & 15;
+        code[0] = kv4_codes(a), code[1] = kv4_codes(a >> 4), code[2] = kv4_codes(b), code[3] = kv4_codes(b >> 4);
       } else {
         const int tile = chunk >> 1, byte = 2 * (at & 1) + (at >> 3), shift = 4 * (chunk & 1);
         const unsigned char* v = run + 8 * kDim + (tile >> 2) * 512 + ((at & 7) >> 1) * 16 + (tile & 3) * 4 + byte;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) code[i] = v[64 * i] >> shift & 15;
+        for (int i = 0; i < 4; ++i) code[i] = kv4_codes((v[128 * i] | (uint32_t)v[128 * i + 64] << 16) >> shift);
       }
       const Pair16<T> pr =
-          reinterpret_cast<const Pair16<T>*>(run + 16 * kDim + part * 64 * P.sh.groups)[at * P.sh.groups + group];
+          reinterpret_cast<const Pair16<T>*>(run + 16 * kDim + part * 64 * kGroups)[at * kGroups + chunk / kSpan];
       const float s = to_f32(pr.s), m = to_f32(pr.m);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) out[i] = from_f32<T>(fmaf(s, (float)code[i], m));
+      for (int i = 0; i < 4; ++i) {
+        out[2 * i] = from_f32<T>(fmaf(s, code[i].x, m));
+        out[2 * i + 1] = from_f32<T>(fmaf(s, code[i].y, m));
+      }
     } else {
 #pragma unroll
       for (int i = 0; i < 8; ++i) out[i] = from_f32<T>(0.f);

@@ -20,11 +20,12 @@
 // Each warp walks its own stretch of tokens, a step of 32 or 64 at a time, through a ring of three steps in shared memory
 // that bulk asynchronous copies fill: a run's bytes are already in the order of the operand's registers.
 // The token range is cut over CTAs (blockIdx.x) and over a CTA's four warps; the parts are joined through shared memory and,
-// between CTAs, by kv4_join_kernel, in a fixed order.
+// between CTAs, through the cluster's shared memory (up to eight) or by kv4_join_kernel, always in a fixed order.
 #pragma once
 
 #include <type_traits>
 
+#include "cluster.cuh"
 #include "kv4.cuh"
 
 namespace qrb200 {
@@ -33,17 +34,19 @@ struct Kv4AttnParams {
   const unsigned char* cache;
   const void* q;
   void* out;
-  float* part_o;       // [batch][head][tile][split][rows of a tile][dim], unnormalised, when splits > 1
+  float* part_o;       // [batch][head][tile][split][rows of a tile][dim], unnormalised, when splits > kKvCluster
   float2* part_ml;     // [...][rows of a tile]: maximum (base 2) and sum
   const int* table;
   const int* lengths;
   long long q_bs, q_ts, q_hs, table_stride;  // strides in elements
   int batch, queries, q_heads, share, max_pages, window, causal, splits, tiles;
+  int q_wide;  // four channels of q lie on an 8-byte boundary
   float scale2;  // scale times log2(e)
   Kv4Shape sh;
 };
 
 constexpr int kKvWarps = 4;
+constexpr int kKvCluster = 8;  // the most CTAs that join their parts within a cluster (the portable size)
 // Runs of 16 tokens in a warp's step: as many as the registers hold beside the output (twice the channels, half the runs).
 __host__ __device__ constexpr int kv_runs(int dim) { return dim == 64 ? 4 : 2; }
 
@@ -104,6 +107,11 @@ __device__ __forceinline__ float kv_exp2(float x) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
+}
+// What a part with this (maximum, sum) counts against the maximum m of all: nothing where it saw nothing, NaN where its
+// scores were.
+__device__ __forceinline__ float kv_part_weight(float2 ml, float m) {
+  return ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : ml.y) : kv_exp2(ml.x - m);
 }
 template <int kWords>
 __device__ __forceinline__ void kv_load(uint32_t (&w)[kWords], const unsigned char* p) {  // from shared memory
@@ -173,6 +181,24 @@ __global__ void __launch_bounds__(32 * kKvWarps, kNT == 1 ? 4 : 2) kv4_attention
   __syncwarp();
   griddep_launch_wait();
   int len = P.lengths[b];
+  // The queries, asked for before anything waits: step j wants channels 16 j + 4 t + {0, 1} and {2, 3} of row g.
+  T qv[kNT][kSteps / kKvWarps][4];
+#pragma unroll
+  for (int n = 0; n < kNT; ++n) {
+    const int r = row0 + 8 * n + g;
+    const T* q = static_cast<const T*>(P.q) + b * P.q_bs + (long long)(r / P.share) * P.q_ts +
+                 (head * P.share + r % P.share) * P.q_hs + 4 * t;
+#pragma unroll
+    for (int i = 0; i < kSteps / kKvWarps; ++i) {
+      const T* at = q + 16 * (i * kKvWarps + warp);
+      if (P.q_wide) {
+        *reinterpret_cast<uint2*>(qv[n][i]) = r < rows ? __ldg(reinterpret_cast<const uint2*>(at)) : make_uint2(0, 0);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) qv[n][i][e] = r < rows ? at[e] : from_f32<T>(0.f);
+      }
+    }
+  }
   if (len < 0 || len > (long long)P.max_pages * P.sh.page || (len > 0 && P.sh.pages == 0)) {
     if (threadIdx.x == 0) report_device_failure(kSiteIndex);
     len = 0;
@@ -199,7 +225,7 @@ __global__ void __launch_bounds__(32 * kKvWarps, kNT == 1 ? 4 : 2) kv4_attention
 
   // The ring. Lane i of `page` holds the page of run `page_base` + i, -1 past the range or where the table is wrong.
   unsigned char* ring = s_ring + warp * (kKvStages * kStage);
-  const int page_runs = P.sh.page / 16, page_shift = 31 - __clz(page_runs);
+  const int page_runs = P.sh.page / 16, page_shift = P.sh.shift - 4;
   const int last_run = min(u_hi * kRuns, (len + 15) / 16);
   int page_base = u * kRuns, page = -1;
   auto look_up = [&]() {
@@ -244,12 +270,9 @@ __global__ void __launch_bounds__(32 * kKvWarps, kNT == 1 ? 4 : 2) kv4_attention
   if (count > 0) look_up();
   for (int i = 0; i < kKvStages && i < count; ++i) issue(u + i, i);
 
-  // Queries as the right operand: step j wants channels 16 j + 4 t + {0, 1} and {2, 3} of row g. The warps share the work.
+  // Queries as the right operand. The warps share the work.
 #pragma unroll
   for (int n = 0; n < kNT; ++n) {
-    const int r = row0 + 8 * n + g;
-    const T* q = static_cast<const T*>(P.q) + b * P.q_bs + (long long)(r / P.share) * P.q_ts +
-                 (head * P.share + r % P.share) * P.q_hs + 4 * t;
     float part[kGroups] = {};
 #pragma unroll
     for (int i = 0; i < kSteps / kKvWarps; ++i) {
@@ -258,7 +281,7 @@ __global__ void __launch_bounds__(32 * kKvWarps, kNT == 1 ? 4 : 2) kv4_attention
       float add = 0.f;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const float v = r < rows ? to_f32(q[16 * j + e]) : 0.f;
+        const float v = to_f32(qv[n][i][e]);
         x[e] = from_f32<T>(v * (e < 2 ? KvKey<T>::kQuery : KvKey<T>::kQuery / 16));
         add += v;
       }
@@ -540,27 +563,78 @@ __global__ void __launch_bounds__(32 * kKvWarps, kNT == 1 ? 4 : 2) kv4_attention
   __syncthreads();
   constexpr int kLanesRow = 32 * kKvWarps / kRows;  // threads of a row
   const int r = threadIdx.x / kLanesRow, d0 = threadIdx.x % kLanesRow;
-  if (row0 + r >= rows || s_bad) return;
   float m = kNone, l = 0.f, f[kKvWarps];
 #pragma unroll
   for (int w = 0; w < kKvWarps; ++w) m = fmaxf(m, s_ml[w][r].x);
 #pragma unroll
   for (int w = 0; w < kKvWarps; ++w) {
-    f[w] = s_ml[w][r].x == kNone ? (s_ml[w][r].y == 0.f ? 0.f : s_ml[w][r].y) : kv_exp2(s_ml[w][r].x - m);
+    f[w] = kv_part_weight(s_ml[w][r], m);
     l = fmaf(f[w], s_ml[w][r].y, l);
   }
-  const long long part = (((long long)b * P.sh.heads + head) * P.tiles + tile) * P.splits + split;
-  T* out = static_cast<T*>(P.out) +
-           (((long long)b * P.queries + (row0 + r) / P.share) * P.q_heads + head * P.share + (row0 + r) % P.share) * kDim;
-  const float inv = l == 0.f ? 0.f : 1.f / l;  // nothing seen: zeros
-  for (int d = d0; d < kDim; d += kLanesRow) {
+  const auto out_row = [&](int row) {
+    return static_cast<T*>(P.out) +
+           (((long long)b * P.queries + (row0 + row) / P.share) * P.q_heads + head * P.share + (row0 + row) % P.share) * kDim;
+  };
+  const auto joined = [&](int d) {
     float x = 0.f;
 #pragma unroll
     for (int w = 0; w < kKvWarps; ++w) x = f[w] == 0.f ? x : fmaf(f[w], s_o[w][r][d], x);
-    if (P.splits == 1) out[d] = from_f32<T>(x * inv);
-    else P.part_o[(part * kRows + r) * kDim + d] = x;
+    return x;
+  };
+  if (P.splits == 1) {
+    const float inv = l == 0.f ? 0.f : 1.f / l;  // nothing seen: zeros
+    if (row0 + r < rows && !s_bad)
+      for (int d = d0; d < kDim; d += kLanesRow) out_row(r)[d] = from_f32<T>(joined(d) * inv);
+  } else if (P.splits <= kKvCluster) {
+    // The CTA's part takes its first warp's place; each CTA then joins every splits-th row of all of them.
+    for (int d = d0; d < kDim; d += kLanesRow) s_o[0][r][d] = joined(d);
+    __syncthreads();  // every warp's (maximum, sum) has been read
+    if (d0 == 0) s_ml[0][r] = make_float2(m, l);
+    cluster_sync();
+    // What each CTA's part of a row counts, and the whole row's sum: a thread to a row.
+    float(*s_w)[kKvCluster + 1] = reinterpret_cast<float(*)[kKvCluster + 1]>(s_q);
+    bool bad = false;
+    for (int c = 0; c < P.splits; ++c) bad = ld_cluster(smem_u32(&s_bad), c) != 0 || bad;
+    if (threadIdx.x < kRows) {
+      float2 ml[kKvCluster];
+      float top = kNone, total = 0.f;
+#pragma unroll
+      for (int c = 0; c < kKvCluster; ++c) {
+        ml[c] = make_float2(kNone, 0.f);
+        if (c < P.splits) {
+          ml[c].x = __int_as_float(ld_cluster(smem_u32(&s_ml[0][threadIdx.x].x), c));
+          ml[c].y = __int_as_float(ld_cluster(smem_u32(&s_ml[0][threadIdx.x].y), c));
+        }
+        top = fmaxf(top, ml[c].x);
+      }
+#pragma unroll
+      for (int c = 0; c < kKvCluster; ++c) {
+        const float w = kv_part_weight(ml[c], top);
+        total = fmaf(w, ml[c].y, total);
+        s_w[threadIdx.x][c] = w;
+      }
+      s_w[threadIdx.x][kKvCluster] = total == 0.f ? 0.f : 1.f / total;
+    }
+    __syncthreads();
+    const int own = bad ? 0 : (min(kRows, rows - row0) - split + P.splits - 1) / P.splits;  // rows split, split + splits, ...
+    for (int e = threadIdx.x; e < own * kDim; e += 32 * kKvWarps) {
+      const int row = split + e / kDim * P.splits, d = e % kDim;
+      float v[kKvCluster], x = 0.f;
+#pragma unroll
+      for (int c = 0; c < kKvCluster; ++c) v[c] = c < P.splits ? __int_as_float(ld_cluster(smem_u32(&s_o[0][row][d]), c)) : 0.f;
+#pragma unroll
+      for (int c = 0; c < kKvCluster; ++c) {
+        const float w = s_w[row][c];
+        x = w == 0.f ? x : fmaf(w, v[c], x);
+      }
+      out_row(row)[d] = from_f32<T>(x * s_w[row][kKvCluster]);
+    }
+    cluster_sync();  // nobody leaves while its part is being read
+  } else if (row0 + r < rows && !s_bad) {
+    const long long part = (((long long)b * P.sh.heads + head) * P.tiles + tile) * P.splits + split;
+    for (int d = d0; d < kDim; d += kLanesRow) P.part_o[(part * kRows + r) * kDim + d] = joined(d);
+    if (d0 == 0) P.part_ml[part * kRows + r] = make_float2(m, l);
   }
-  if (P.splits > 1 && d0 == 0) P.part_ml[part * kRows + r] = make_float2(m, l);
 }
 
 // One warp per query row: the splits' parts against their common maximum, in order.
@@ -579,7 +653,7 @@ __global__ void __launch_bounds__(128) kv4_join_kernel(Kv4AttnParams P, int tile
 #pragma unroll 4
   for (int s = 0; s < P.splits; ++s) {
     const float2 ml = P.part_ml[part + (long long)s * tile_rows];
-    const float f = ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : ml.y) : kv_exp2(ml.x - m);
+    const float f = kv_part_weight(ml, m);
     l = fmaf(f, ml.y, l);
     const float* o = P.part_o + (part + (long long)s * tile_rows) * kDim;
 #pragma unroll

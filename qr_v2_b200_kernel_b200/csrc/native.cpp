@@ -267,7 +267,7 @@ Tensor kv4_attention(Tensor q, const Cache& c, Tensor table, Tensor lengths, std
   const Tensor out = empty(q.sizes(), c.type, c.data);
   if (out.numel() == 0) return out;
   const int64_t pages = table.size(1);
-  const size_t need = qrb200_kv4_attention_workspace_bytes(&c.shape, batch, queries, heads, pages);
+  const size_t need = qrb200_kv4_attention_workspace_bytes(&c.shape, batch, queries, heads, pages, window.value_or(0));
   Tensor ws;
   if (need > 0) ws = empty({(int64_t)need}, at::kByte, c.data);
   const int64_t strides[3] = {q.stride(0), q.stride(1), q.stride(2)};

@@ -7,6 +7,7 @@
 #include <atomic>
 #include <cstdint>
 #include <mutex>
+#include <type_traits>
 
 #include "internal.h"
 #include "qrb200.h"
@@ -76,7 +77,7 @@ struct LaunchShape {
   cudaLaunchConfig_t cfg{};
   cudaLaunchAttribute attr[2];
   // A kernel that begins with griddep_launch_wait() may be set up while its predecessor ends.
-  LaunchShape(dim3 grid, unsigned threads, size_t smem, cudaStream_t s, unsigned cluster_z = 0) {
+  LaunchShape(dim3 grid, unsigned threads, size_t smem, cudaStream_t s) {
     cfg.gridDim = grid;
     cfg.blockDim = dim3(threads);
     cfg.dynamicSmemBytes = smem;
@@ -84,14 +85,14 @@ struct LaunchShape {
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.numAttrs = 1;
-    if (cluster_z > 1) {
-      attr[1].id = cudaLaunchAttributeClusterDimension;
-      attr[1].val.clusterDim.x = 1;
-      attr[1].val.clusterDim.y = 1;
-      attr[1].val.clusterDim.z = cluster_z;
-      cfg.numAttrs = 2;
-    }
     cfg.attrs = attr;
+  }
+  void cluster(unsigned x, unsigned y, unsigned z) {
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = x;
+    attr[1].val.clusterDim.y = y;
+    attr[1].val.clusterDim.z = z;
+    cfg.numAttrs = 2;
   }
 };
 
@@ -158,14 +159,15 @@ static int launch_rows(const RowsParams& p, int weight_type, int dtype, cudaStre
 template <typename T>
 static int launch_dequant(const int8_t* q, int64_t q_stride, const float* scale, void* out, int64_t rows, int64_t cols,
                           cudaStream_t s) {
-  const bool vec = cols % 16 == 0 && q_stride % 16 == 0 &&
-                   ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) & 15u) == 0;
-  const int64_t packs = rows * (vec ? cols / 16 : cols);
-  if (packs > ((int64_t)1 << 38)) return QRB200_ERR_ARG;
-  LaunchShape l(dim3(ceil_div(packs, 256)), 256, 0, s);
+  // Sixteen codes to a thread where rows start on 16-byte boundaries on both sides, else eight, a warp's side by side.
+  const bool aligned = (cols * sizeof(T)) % 16 == 0 && q_stride % 16 == 0 &&
+                       ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) & 15u) == 0;
+  const int64_t units = aligned ? rows * ceil_div(cols, 16) : rows * ceil_div(cols, 256) * 32;
+  if (units > ((int64_t)1 << 38)) return QRB200_ERR_ARG;
+  LaunchShape l(dim3(ceil_div(units, 256)), 256, 0, s);
   const cudaError_t e =
-      vec ? cudaLaunchKernelEx(&l.cfg, dequant_rows_kernel<T, 16>, q, (long long)q_stride, scale, static_cast<T*>(out), (long long)rows, (int)cols)
-          : cudaLaunchKernelEx(&l.cfg, dequant_rows_kernel<T, 1>, q, (long long)q_stride, scale, static_cast<T*>(out), (long long)rows, (int)cols);
+      cudaLaunchKernelEx(&l.cfg, aligned ? dequant_rows_kernel<T, true> : dequant_rows_kernel<T, false>, q, (long long)q_stride,
+                         scale, static_cast<T*>(out), (long long)rows, (int)cols);
   if (e != cudaSuccess) return QRB200_ERR_CUDA;
   return launched();
 }
@@ -181,7 +183,7 @@ static int rows_int8(const RowsParams& p, int weight_type, int dtype, cudaStream
 
 
 template <typename T, int kBN>
-static cudaError_t launch_i8_few(const I8Params& p, const I8Operand& x, const I8Operand& w, cudaStream_t s) {
+static cudaError_t launch_i8_few(const I8Params& p, const I8Operand& x, const I8Operand& w, unsigned split, cudaStream_t s) {
   using C = I8Few<kBN>;
   static OncePerDevice once;
   const cudaError_t e = once.run([] {
@@ -190,11 +192,10 @@ static cudaError_t launch_i8_few(const I8Params& p, const I8Operand& x, const I8
   if (e != cudaSuccess) return e;
   CUtensorMap tw, tx;
   if (!encode_codes(&tw, w, p.depth, 128) || !encode_codes(&tx, x, p.depth, kBN)) return cudaErrorInvalidValue;
-  const int tn = ceil_div(p.outs, 128), tm = ceil_div(p.rows, kBN), nk = ceil_div(p.depth, kI8Depth);
+  const int tn = ceil_div(p.outs, 128), tm = ceil_div(p.rows, kBN);
   if (tm > 65535) return cudaErrorInvalidValue;
-  unsigned split = 1;
-  while (split < 8 && 2 * split <= (unsigned)nk && (int64_t)tn * tm * split < sm_count()) split *= 2;
-  LaunchShape l(dim3(tn, tm, split), 192, C::smem(), s, split);
+  LaunchShape l(dim3(tn, tm, split), 192, C::smem(), s);
+  if (split > 1) l.cluster(1, 1, split);
   return cudaLaunchKernelEx(&l.cfg, i8_few_kernel<T, kBN>, p, tw, tx);
 }
 
@@ -216,13 +217,50 @@ static cudaError_t launch_i8_wide(I8Params p, const I8Operand& x, const I8Operan
   return cudaLaunchKernelEx(&l.cfg, i8_wide_kernel<T>, p, tx, tw);
 }
 
+// Which kernel, with how many rows a tile (`rows`) and over how many CTAs of the depth: the least of the estimated clocks. A CTA
+// takes in its stages at about 64 bytes a clock; joining a split costs two cluster barriers (about 1500 clocks) and reading
+// the sums at about 16 bytes a clock. The wide kernel's pair takes 512 clocks a stage and a tile's last epilogue is bare.
+struct I8Plan {
+  int rows;  // 16, 32, 64 or 128 (few), 256 (wide)
+  unsigned split;
+};
+static I8Plan i8_plan(int64_t rows, int64_t outs, int64_t depth) {
+  const int64_t sms = sm_count(), nk = (depth + kI8Depth - 1) / kI8Depth;
+  const int64_t pairs = (rows + 255) / 256 * ((outs + 255) / 256);
+  I8Plan best{256, 1};
+  int64_t least = (pairs + sms / 2 - 1) / (sms / 2) * nk * 512 + 3000;
+  for (int bn = 16; bn <= 128; bn *= 2) {
+    const int64_t tiles = (rows + bn - 1) / bn * ((outs + 127) / 128);
+    if ((rows + bn - 1) / bn > 65535) continue;
+    for (unsigned split = 1; split <= 8 && split <= nk; split *= 2) {
+      const int64_t clocks = (tiles * split + sms - 1) / sms * ((nk + split - 1) / split) * (128 + bn) * 2 +
+                             (split > 1 ? 1500 + bn * 32 : bn * 8);
+      if (clocks < least) {
+        least = clocks;
+        best = I8Plan{bn, split};
+      }
+    }
+    if (rows <= bn) break;
+  }
+  return best;
+}
+
 template <typename T>
 static cudaError_t launch_i8(const I8Params& p, const I8Operand& x, const I8Operand& w, cudaStream_t s) {
-  if (p.rows <= 16) return launch_i8_few<T, 16>(p, x, w, s);
-  if (p.rows <= 32) return launch_i8_few<T, 32>(p, x, w, s);
-  if (p.rows <= 64) return launch_i8_few<T, 64>(p, x, w, s);
-  if ((int64_t)ceil_div(p.rows, 256) * ceil_div(p.outs, 256) < sm_count() / 4) return launch_i8_few<T, 128>(p, x, w, s);
-  return launch_i8_wide<T>(p, x, w, s);
+  const I8Plan plan = i8_plan(p.rows, p.outs, p.depth);
+  switch (plan.rows) {
+    case 16: return launch_i8_few<T, 16>(p, x, w, plan.split, s);
+    case 32: return launch_i8_few<T, 32>(p, x, w, plan.split, s);
+    case 64: return launch_i8_few<T, 64>(p, x, w, plan.split, s);
+    case 128: return launch_i8_few<T, 128>(p, x, w, plan.split, s);
+    default: return launch_i8_wide<T>(p, x, w, s);
+  }
+}
+
+static int page_shift(int page) {
+  int s = 0;
+  while (s < 10 && (1 << s) < page) ++s;
+  return s;
 }
 
 static bool shape_ok(const Kv4Shape& h) {
@@ -231,21 +269,28 @@ static bool shape_ok(const Kv4Shape& h) {
          (h.dim / h.groups == 32 || h.dim / h.groups == 64 || h.dim / h.groups == 128);
 }
 
+// f(dim, groups) with both as types, for the layouts that shape_ok admits.
+template <int kValue>
+using Int = std::integral_constant<int, kValue>;
+template <typename F>
+static cudaError_t with_layout(const Kv4Shape& h, F&& f) {
+  if (h.dim == 64) return h.groups == 1 ? f(Int<64>{}, Int<1>{}) : f(Int<64>{}, Int<2>{});
+  if (h.groups == 1) return f(Int<128>{}, Int<1>{});
+  return h.groups == 2 ? f(Int<128>{}, Int<2>{}) : f(Int<128>{}, Int<4>{});
+}
+
 template <typename T>
 static cudaError_t launch_write(const Kv4IoParams& p, bool vec, cudaStream_t s) {
-  LaunchShape l(dim3(ceil_div(p.tokens, 16), p.sh.heads), 2 * p.sh.dim, p.sh.run_bytes(), s);
-  if (p.sh.dim == 128)
-    return vec ? cudaLaunchKernelEx(&l.cfg, kv4_write_kernel<T, 128, true>, p)
-               : cudaLaunchKernelEx(&l.cfg, kv4_write_kernel<T, 128, false>, p);
-  return vec ? cudaLaunchKernelEx(&l.cfg, kv4_write_kernel<T, 64, true>, p)
-             : cudaLaunchKernelEx(&l.cfg, kv4_write_kernel<T, 64, false>, p);
+  LaunchShape l(dim3(ceil_div(p.tokens, 16), p.sh.heads), 2 * p.sh.dim, 0, s);
+  return with_layout(p.sh, [&](auto dim, auto groups) {
+    return cudaLaunchKernelEx(&l.cfg, vec ? kv4_write_kernel<T, dim(), groups(), true> : kv4_write_kernel<T, dim(), groups(), false>, p);
+  });
 }
 
 template <typename T>
 static cudaError_t launch_read(const Kv4IoParams& p, cudaStream_t s) {
-  LaunchShape l(dim3(ceil_div(p.tokens, 16), p.sh.heads), 2 * p.sh.dim, p.sh.run_bytes(), s);
-  return p.sh.dim == 128 ? cudaLaunchKernelEx(&l.cfg, kv4_read_kernel<T, 128>, p)
-                         : cudaLaunchKernelEx(&l.cfg, kv4_read_kernel<T, 64>, p);
+  LaunchShape l(dim3(ceil_div(p.tokens, 16), p.sh.heads), 2 * p.sh.dim, 0, s);
+  return with_layout(p.sh, [&](auto dim, auto groups) { return cudaLaunchKernelEx(&l.cfg, kv4_read_kernel<T, dim(), groups()>, p); });
 }
 
 // How an attention call is cut: query rows per tile, and the token range over `splits` CTAs.
@@ -256,23 +301,24 @@ struct AttnPlan {
 
 // Eight rows a tile where a key head has no more than eight query rows, else sixteen. The token range is cut so that the
 // SMs, which instructions keep busy, get even shares: the estimated time is the most CTAs on one SM x (steps of a warp + what
-// a CTA costs besides, about four steps), and four more for joining, over the table's capacity, the one length the host knows.
-static AttnPlan attn_plan(const Kv4Shape& h, int64_t batch, int64_t queries, int64_t q_heads, int64_t max_pages) {
+// a CTA costs besides, about two steps), and for joining one more in a cluster, four through memory. The length is the table's
+// capacity or what a window leaves of it, all that the host knows.
+static AttnPlan attn_plan(const Kv4Shape& h, int64_t batch, int64_t queries, int64_t q_heads, int64_t max_pages, int64_t span) {
   AttnPlan p{};
   const int64_t rows = queries * (q_heads / h.heads);
   p.tile_rows = rows <= 8 ? 8 : 16;
   p.tiles = ceil_div(rows, p.tile_rows);
   const int64_t ctas = batch * h.heads * p.tiles, unit = 16 * kv_runs(h.dim), sms = sm_count();
-  const int64_t steps = std::max<int64_t>(1, (max_pages * h.page + unit * kKvWarps - 1) / (unit * kKvWarps));
+  const int64_t steps = std::max<int64_t>(1, (std::min(max_pages * h.page, span) + unit * kKvWarps - 1) / (unit * kKvWarps));
   int64_t best = -1;
   for (int64_t n = 1; n <= std::min<int64_t>(steps, 64); ++n) {
-    const int64_t time = (ctas * n + sms - 1) / sms * ((steps + n - 1) / n + 4) + (n > 1 ? 4 : 0);
+    const int64_t time = (ctas * n + sms - 1) / sms * ((steps + n - 1) / n + 2) + (n > kKvCluster ? 4 : n > 1 ? 1 : 0);
     if (best < 0 || time < best) {
       best = time;
       p.splits = (int)n;
     }
   }
-  if (p.splits > 1) p.bytes = (size_t)(ctas * p.splits * p.tile_rows) * (h.dim * sizeof(float) + sizeof(float2));
+  if (p.splits > kKvCluster) p.bytes = (size_t)(ctas * p.splits * p.tile_rows) * (h.dim * sizeof(float) + sizeof(float2));
   return p;
 }
 
@@ -285,6 +331,7 @@ static cudaError_t launch_attention_tile(const Kv4AttnParams& p, const AttnPlan&
   });
   if (e != cudaSuccess) return e;
   LaunchShape l(dim3(plan.splits, p.sh.heads * plan.tiles, p.batch), 32 * kKvWarps, kSmem, s);
+  if (plan.splits > 1 && plan.splits <= kKvCluster) l.cluster(plan.splits, 1, 1);
   return cudaLaunchKernelEx(&l.cfg, kv4_attention_kernel<T, kDim, kGroups, kNT>, p);
 }
 
@@ -292,7 +339,7 @@ template <typename T, int kDim, int kGroups>
 static cudaError_t launch_attention(Kv4AttnParams p, const AttnPlan& plan, cudaStream_t s) {
   const cudaError_t e = plan.tile_rows == 8 ? launch_attention_tile<T, kDim, kGroups, 1>(p, plan, s)
                                             : launch_attention_tile<T, kDim, kGroups, 2>(p, plan, s);
-  if (e != cudaSuccess || plan.splits == 1) return e;
+  if (e != cudaSuccess || plan.splits <= kKvCluster) return e;
   qrb200_internal_count_launch();
   LaunchShape j(dim3(ceil_div((int64_t)p.batch * p.queries * p.q_heads, 4)), 128, 0, s);
   return cudaLaunchKernelEx(&j.cfg, kv4_join_kernel<T, kDim>, p, plan.tile_rows);
@@ -300,9 +347,7 @@ static cudaError_t launch_attention(Kv4AttnParams p, const AttnPlan& plan, cudaS
 
 template <typename T>
 static cudaError_t launch_attention_of(const Kv4AttnParams& p, const AttnPlan& plan, cudaStream_t s) {
-  if (p.sh.dim == 64) return p.sh.groups == 1 ? launch_attention<T, 64, 1>(p, plan, s) : launch_attention<T, 64, 2>(p, plan, s);
-  if (p.sh.groups == 1) return launch_attention<T, 128, 1>(p, plan, s);
-  return p.sh.groups == 2 ? launch_attention<T, 128, 2>(p, plan, s) : launch_attention<T, 128, 4>(p, plan, s);
+  return with_layout(p.sh, [&](auto dim, auto groups) { return launch_attention<T, dim(), groups()>(p, plan, s); });
 }
 
 }  // namespace qrb200
@@ -384,7 +429,7 @@ int qrb200_int8_linear(const int8_t* x, int64_t x_stride, const float* x_scale, 
 
 int64_t qrb200_kv4_block_bytes(int64_t page_size, int64_t head_dim, int64_t group_size) {
   if (group_size <= 0 || page_size < 0 || page_size > 1024 || head_dim < 0 || head_dim > 128) return 0;
-  const Kv4Shape h{1, (int)page_size, (int)head_dim, (int)(head_dim / std::min<int64_t>(group_size, 1024)), 0};
+  const Kv4Shape h{1, (int)page_size, (int)head_dim, (int)(head_dim / std::min<int64_t>(group_size, 1024)), 0, 0};
   return shape_ok(h) && head_dim % group_size == 0 ? h.block_bytes() : 0;
 }
 
@@ -392,7 +437,7 @@ int qrb200_kv4_write(void* cache, const qrb200_kv4_shape* shape, const void* k, 
                      int64_t k_head_stride, const void* v, int64_t v_token_stride, int64_t v_head_stride,
                      const int64_t* slots, int64_t tokens, void* stream) {
   if (!shape || tokens < 0 || !type16_ok(shape->dtype)) return QRB200_ERR_ARG;
-  const Kv4Shape h{shape->kv_heads, shape->page_size, shape->head_dim, shape->groups, shape->pages};
+  const Kv4Shape h{shape->kv_heads, shape->page_size, shape->head_dim, shape->groups, page_shift(shape->page_size), shape->pages};
   if (!shape_ok(h) || tokens > kMaxRows / h.heads) return QRB200_ERR_ARG;
   if (tokens == 0) return QRB200_OK;
   if (!cache || !k || !v || !slots || (reinterpret_cast<uintptr_t>(cache) & 15u)) return QRB200_ERR_ARG;
@@ -413,7 +458,7 @@ int qrb200_kv4_write(void* cache, const qrb200_kv4_shape* shape, const void* k, 
 int qrb200_kv4_read(const void* cache, const qrb200_kv4_shape* shape, void* k, void* v, const int64_t* slots,
                     int64_t tokens, void* stream) {
   if (!shape || tokens < 0 || !type16_ok(shape->dtype)) return QRB200_ERR_ARG;
-  const Kv4Shape h{shape->kv_heads, shape->page_size, shape->head_dim, shape->groups, shape->pages};
+  const Kv4Shape h{shape->kv_heads, shape->page_size, shape->head_dim, shape->groups, page_shift(shape->page_size), shape->pages};
   if (!shape_ok(h) || tokens > kMaxRows / h.heads) return QRB200_ERR_ARG;
   if (tokens == 0) return QRB200_OK;
   if (!cache || !k || !v || !slots || (reinterpret_cast<uintptr_t>(cache) & 15u)) return QRB200_ERR_ARG;
@@ -428,21 +473,25 @@ int qrb200_kv4_read(const void* cache, const qrb200_kv4_shape* shape, void* k, v
   return launched();
 }
 
+// The most tokens that a sequence's queries see between them.
+static int64_t token_span(int64_t queries, int64_t window) { return window > 0 ? window + queries : kMaxRows; }
+
 // The launch grid is splits x (key heads x row tiles) x batch.
 static bool attention_args(const qrb200_kv4_shape* shape, int64_t batch, int64_t queries, int64_t q_heads,
                            int64_t max_pages, Kv4Shape* h) {
   if (!shape || batch < 0 || queries < 0 || q_heads < 0 || max_pages < 0 || !type16_ok(shape->dtype)) return false;
-  *h = Kv4Shape{shape->kv_heads, shape->page_size, shape->head_dim, shape->groups, shape->pages};
+  *h = Kv4Shape{shape->kv_heads, shape->page_size, shape->head_dim, shape->groups, page_shift(shape->page_size), shape->pages};
   return shape_ok(*h) && q_heads % h->heads == 0 && batch <= 65535 && q_heads <= 65535 && queries <= (1 << 24) &&
          queries * (q_heads / h->heads) <= (1 << 24) && (queries * (q_heads / h->heads) + 15) / 16 * h->heads <= 65535 &&
          batch * queries * q_heads <= kMaxRows && max_pages <= kMaxRows / h->page - 64 * (kKvWarps + 1);
 }
 
 size_t qrb200_kv4_attention_workspace_bytes(const qrb200_kv4_shape* shape, int64_t batch, int64_t queries,
-                                            int64_t q_heads, int64_t max_pages) {
+                                            int64_t q_heads, int64_t max_pages, int64_t window) {
   Kv4Shape h;
+  if (window < 0 || window > kMaxRows) return 0;
   if (!attention_args(shape, batch, queries, q_heads, max_pages, &h) || batch * queries * q_heads == 0) return 0;
-  return attn_plan(h, batch, queries, q_heads, max_pages).bytes;
+  return attn_plan(h, batch, queries, q_heads, max_pages, token_span(queries, window)).bytes;
 }
 
 int qrb200_kv4_attention(const void* q, const int64_t* q_strides, const void* cache, const qrb200_kv4_shape* shape,
@@ -458,7 +507,7 @@ int qrb200_kv4_attention(const void* q, const int64_t* q_strides, const void* ca
     return QRB200_ERR_ARG;
   const int st = quant_ready();
   if (st != QRB200_OK) return st;
-  const AttnPlan plan = attn_plan(h, batch, queries, q_heads, max_pages);
+  const AttnPlan plan = attn_plan(h, batch, queries, q_heads, max_pages, token_span(queries, window));
   if (plan.bytes > 0 && (!workspace || workspace_bytes < plan.bytes || (reinterpret_cast<uintptr_t>(workspace) & 255u)))
     return QRB200_ERR_WORKSPACE;
   Kv4AttnParams p{};
@@ -473,7 +522,8 @@ int qrb200_kv4_attention(const void* q, const int64_t* q_strides, const void* ca
   p.max_pages = (int)max_pages, p.window = (int)window, p.causal = causal, p.splits = plan.splits, p.tiles = plan.tiles;
   p.scale2 = std::max(scale * 1.4426950408889634f, 1e-30f);  // not 0: masked scores, -inf, must stay that
   p.sh = h;
-  if (plan.splits > 1)
+  p.q_wide = (reinterpret_cast<uintptr_t>(q) & 7u) == 0 && ((q_strides[0] | q_strides[1] | q_strides[2]) & 3) == 0;
+  if (plan.splits > kKvCluster)
     p.part_ml = reinterpret_cast<float2*>(p.part_o + batch * h.heads * plan.tiles * plan.splits * plan.tile_rows * h.dim);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const cudaError_t e = shape->dtype == QRB200_BF16 ? launch_attention_of<__nv_bfloat16>(p, plan, s)

@@ -166,31 +166,51 @@ __global__ void __launch_bounds__(1024) rows_int8_kernel(RowsParams P) {
   }
 }
 
-// value = code * scale of its row, rounded once. One pack of kVec codes to a thread, rows end to end.
-template <typename T, int kVec>
+// value = code * scale of its row, rounded once: sixteen codes of a row to a thread, or (kAligned false) eight, 32 apart, with
+// a warp on 256 neighbouring ones.
+template <typename T, bool kAligned>
 __global__ void __launch_bounds__(256) dequant_rows_kernel(const int8_t* q, long long q_stride, const float* scale,
                                                            T* out, long long rows, int cols) {
+  constexpr int kSpan = kAligned ? 16 : 256;
   griddep_launch_wait();
-  const int packs = cols / kVec;
-  const long long at = (long long)blockIdx.x * 256 + threadIdx.x;
+  const int spans = (cols + kSpan - 1) / kSpan;
+  const long long at = ((long long)blockIdx.x * 256 + threadIdx.x) / (kAligned ? 1 : 32);
   // The division is in 32 bits where the index fits it.
-  const long long row = at <= 0xffffffffll ? (long long)((uint32_t)at / (uint32_t)packs) : at / packs;
+  const long long row = at <= 0xffffffffll ? (long long)((uint32_t)at / (uint32_t)spans) : at / spans;
   if (row >= rows) return;
-  const int c = (int)(at - row * packs) * kVec;
+  const int c = (int)(at - row * spans) * kSpan;
   const float s = scale[row];
-  if constexpr (kVec == 16) {
-    const int4 codes = __ldg(reinterpret_cast<const int4*>(q + row * q_stride + c));
-    const int8_t* code = reinterpret_cast<const int8_t*>(&codes);
+  q += row * q_stride + c;
+  out += row * cols + c;
+  if constexpr (kAligned) {
+    const int n = cols - c;  // a multiple of a store's elements
+    uint32_t word[4] = {};
+    if (n >= 16) {
+      *reinterpret_cast<uint4*>(word) = __ldg(reinterpret_cast<const uint4*>(q));
+    } else {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) word[e / 4] |= e < n ? (uint32_t)(uint8_t)q[e] << (8 * (e & 3)) : 0u;
+    }
     constexpr int kPart = 16 / sizeof(T);
 #pragma unroll
     for (int h = 0; h < 16; h += kPart) {
-      T v[kPart];
+      alignas(16) T v[kPart];
 #pragma unroll
-      for (int e = 0; e < kPart; ++e) v[e] = from_f32<T>((float)code[h + e] * s);
-      store_pack<true>(out + row * cols + c + h, v, kPart);
+      for (int e = 0; e < kPart; ++e) {
+        // A byte plus 128, under the exponent of 2^23: exact, and cheaper than a conversion.
+        const uint32_t bits = __byte_perm(word[(h + e) / 4] ^ 0x80808080u, 0x4b000000u, 0x7440 + ((h + e) & 3));
+        v[e] = from_f32<T>((__uint_as_float(bits) - 8388736.f) * s);
+      }
+      if (h < n) store_pack<true>(out + h, v, kPart);
     }
   } else {
-    out[row * cols + c] = from_f32<T>((float)q[row * q_stride + c] * s);
+    const int lane = threadIdx.x & 31, n = cols - c;
+    int code[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) code[i] = lane + 32 * i < n ? __ldg(q + lane + 32 * i) : 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (lane + 32 * i < n) out[lane + 32 * i] = from_f32<T>((float)code[i] * s);
   }
 }
 
