@@ -80,6 +80,7 @@ struct Kv4IoParams {
   const long long* slots;
   long long tokens, k_ts, k_hs, v_ts, v_hs;  // strides in elements
   Kv4Shape sh;
+  int span;  // heads to a CTA
 };
 
 // Where a token's run lies, or null for a slot that is skipped; an index past the cache is reported.
@@ -93,151 +94,193 @@ __device__ __forceinline__ unsigned char* kv4_run(const Kv4IoParams& P, long lon
   return P.cache + (page * P.sh.heads + head) * P.sh.block_bytes() + ((int)slot & (P.sh.page - 1)) / 16 * P.sh.run_bytes();
 }
 
-// Sixteen tokens of one head to a CTA, kDim / 8 threads to a token, 8 channels (16 bytes) to a thread. Bandwidth
-// bounds it: everything a thread reads is asked for before anything is computed. When the sixteen fill a run, as
+// Sixteen tokens to a CTA, kDim / 8 threads to a token, 8 channels (16 bytes) to a thread, head after head of P.span of them;
+// the next head's loads are under way while one is quantised. When the sixteen fill a run, as
 // prompts do, the run is put together in shared memory and stored whole; otherwise each thread stores its words (keys) and
 // bytes (values). Long prompts are bound by instructions: codes come out of the 32-bit floating sum's bits, packed as they lie.
 template <typename T, int kDim, int kGroups, bool kVec>
 __global__ void __launch_bounds__(2 * kDim) kv4_write_kernel(Kv4IoParams P) {
   constexpr int kChunks = kDim / 8, kSpan = kChunks / kGroups;  // threads of a token, of a group
   constexpr int kRunBytes = 16 * kDim + 128 * kGroups;
-  __shared__ uint4 s_run[kRunBytes / 16];
+  __shared__ uint4 s_run[2][kRunBytes / 16];
   griddep_launch_wait();
-  const int chunk = threadIdx.x % kChunks, mine = threadIdx.x / kChunks, head = blockIdx.y;
+  const int chunk = threadIdx.x % kChunks, mine = threadIdx.x / kChunks;
+  const int head0 = blockIdx.y * P.span, heads = min(P.span, P.sh.heads - head0);
   const long long first = (long long)blockIdx.x * 16, tok = first + mine;
   const bool in = tok < P.tokens;
-  alignas(16) T x[2][8];
-#pragma unroll
-  for (int part = 0; part < 2; ++part) {
-    const T* src = (part ? static_cast<const T*>(P.v) + tok * P.v_ts + head * P.v_hs
-                         : static_cast<const T*>(P.k) + tok * P.k_ts + head * P.k_hs) + 8 * chunk;
+  const T* k = static_cast<const T*>(P.k) + tok * P.k_ts + head0 * P.k_hs + 8 * chunk;
+  const T* v = static_cast<const T*>(P.v) + tok * P.v_ts + head0 * P.v_hs + 8 * chunk;
+  const auto load = [&](T(&x)[8], const T* src) {
     if constexpr (kVec) {
-      *reinterpret_cast<uint4*>(x[part]) = in ? *reinterpret_cast<const uint4*>(src) : uint4{};
+      *reinterpret_cast<uint4*>(x) = in ? __ldg(reinterpret_cast<const uint4*>(src)) : uint4{};
     } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[part][i] = in ? src[i] : from_f32<T>(0.f);
+      for (int i = 0; i < 8; ++i) x[i] = in ? src[i] : from_f32<T>(0.f);
     }
-  }
+  };
+  alignas(16) T x[2][8];
+  load(x[0], k);
+  load(x[1], v);
   const long long slot = in ? P.slots[tok] : -1, slot0 = P.slots[first];
   const bool whole = __syncthreads_and(in && slot == slot0 + mine && (slot0 & 15) == 0);
-  unsigned char* run = kv4_run(P, slot, head, chunk == 0);
-  unsigned char* out = whole ? reinterpret_cast<unsigned char*>(s_run) : run;
-  const int at = whole ? mine : (int)(slot & 15);
+  unsigned char* run = kv4_run(P, whole ? slot0 : slot, head0, chunk == 0);
+  const int block = P.sh.block_bytes();
+  // Quantises both parts into the run at `out` (null: nowhere), as its token `at`.
+  const auto quantise = [&](unsigned char* out, int at) {
 #pragma unroll
-  for (int part = 0; part < 2; ++part) {
-    // The group's ends, exact in 16 bits: this thread's eight channels two at a time, then (lo, -hi) over the group's threads.
-    // NaN carries through; infinity shows at an end.
-    typename Two<T>::type ends = kv4_ends(x[part]);
+    for (int part = 0; part < 2; ++part) {
+      // The group's ends, exact in 16 bits: this thread's eight channels two at a time, then (lo, -hi) over the group's threads.
+      // NaN carries through; infinity shows at an end.
+      typename Two<T>::type ends = kv4_ends(x[part]);
 #pragma unroll
-    for (int o = kSpan >> 1; o; o >>= 1) {
-      const uint32_t other = __shfl_xor_sync(kFullMask, reinterpret_cast<const uint32_t&>(ends), o);
-      ends = __hmin2_nan(ends, reinterpret_cast<const typename Two<T>::type&>(other));
-    }
-    const float lo = to_f32(ends.x), hi = -to_f32(ends.y);
-    const bool fine = fabsf(lo) < __int_as_float(0x7f800000) && fabsf(hi) < __int_as_float(0x7f800000);
-    constexpr float kFifteenth = 1.f / 15.f;
-    const float nan = __int_as_float(0x7fffffff);
-    Pair16<T> pr;
-    pr.s = from_f32<T>(fine ? __fsub_rn(__fmul_rn(hi, kFifteenth), __fmul_rn(lo, kFifteenth)) : nan);
-    pr.m = from_f32<T>(fine ? lo : nan);
-    const float s = to_f32(pr.s), m = to_f32(pr.m);
-    const float inv = s >= 0x1p-126f ? __frcp_rn(s) : 0.f;
-    // x - m is never negative. Added to 1.5 2^23, a number below 2^22 leaves its nearest whole number (ties to even) in the
-    // low bits, above a constant that the packing takes off. Where s is normal, its rounding keeps every code below 15.5.
-    uint32_t code[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      float steps = __fmul_rn(__fsub_rn(to_f32(x[part][i]), m), inv);
-      if constexpr (std::is_same<T, __half>::value) steps = fminf(steps, 15.f);  // subnormal steps
-      code[i] = __float_as_uint(__fadd_rn(fine ? steps : 0.f, 0x1.8p23f));
-    }
-    constexpr uint32_t kBits = 0x4b400000u;
-    if (part == 0) {
-      // Step j = chunk / 2, t = 2 (chunk & 1) and the next; the other half of each word, step j ^ 1, is chunk ^ 2's.
-      const int up = (chunk & 2) ? 8 : 0;
-      constexpr uint32_t kAll = kBits + (kBits << 16) + (kBits << 4) + (kBits << 20);
-      const uint32_t a = (code[0] + (code[1] << 16) + (code[2] << 4) + (code[3] << 20) - kAll) << up;
-      const uint32_t b = (code[4] + (code[5] << 16) + (code[6] << 4) + (code[7] << 20) - kAll) << up;
-      const uint32_t got = __shfl_xor_sync(kFullMask, up ? a : b, 2), word = (up ? b : a) | got;
-      const int t = 2 * (chunk & 1) + (up ? 1 : 0);
-      if (out) *reinterpret_cast<uint32_t*>(out + at * (kDim / 2) + t * (kDim / 8) + (chunk >> 2) * 4) = word;
-    } else {
-      // Tile chunk / 2; an even chunk has the low nibbles of its 8 bytes, its odd neighbour the high ones.
-      const bool odd = chunk & 1;
-      constexpr uint32_t kAll = kBits + (kBits << 8) + (kBits << 16) + (kBits << 24);
-      const uint32_t a = code[0] + (code[1] << 8) + (code[2] << 16) + (code[3] << 24) - kAll;
-      const uint32_t b = code[4] + (code[5] << 8) + (code[6] << 16) + (code[7] << 24) - kAll;
-      const uint32_t got = __shfl_xor_sync(kFullMask, odd ? a : b, 1), bytes = odd ? got | b << 4 : a | got << 4;
-      const int tile = chunk >> 1, byte = 2 * (at & 1) + (at >> 3), lane = (odd ? 16 : 0) + ((at & 7) >> 1);
-      if (out) {
-        unsigned char* v = out + 8 * kDim + (tile >> 2) * 512 + lane * 16 + (tile & 3) * 4 + byte;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[64 * i] = (unsigned char)(bytes >> (8 * i));
+      for (int o = kSpan >> 1; o; o >>= 1) {
+        const uint32_t other = __shfl_xor_sync(kFullMask, reinterpret_cast<const uint32_t&>(ends), o);
+        ends = __hmin2_nan(ends, reinterpret_cast<const typename Two<T>::type&>(other));
       }
+      const float lo = to_f32(ends.x), hi = -to_f32(ends.y);
+      const bool fine = fabsf(lo) < __int_as_float(0x7f800000) && fabsf(hi) < __int_as_float(0x7f800000);
+      constexpr float kFifteenth = 1.f / 15.f;
+      const float nan = __int_as_float(0x7fffffff);
+      Pair16<T> pr;
+      pr.s = from_f32<T>(fine ? __fsub_rn(__fmul_rn(hi, kFifteenth), __fmul_rn(lo, kFifteenth)) : nan);
+      pr.m = from_f32<T>(fine ? lo : nan);
+      const float s = to_f32(pr.s), m = to_f32(pr.m);
+      const float inv = s >= 0x1p-126f ? __frcp_rn(s) : 0.f;
+      // x - m is never negative. Added to 1.5 2^23, a number below 2^22 leaves its nearest whole number (ties to even) in
+      // the low bits, above a constant that the packing takes off. Where s is normal, its rounding keeps every code below 15.5.
+      uint32_t code[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        float steps = __fmul_rn(__fsub_rn(to_f32(x[part][i]), m), inv);
+        if constexpr (std::is_same<T, __half>::value) steps = fminf(steps, 15.f);  // subnormal steps
+        code[i] = __float_as_uint(__fadd_rn(fine ? steps : 0.f, 0x1.8p23f));
+      }
+      constexpr uint32_t kBits = 0x4b400000u;
+      if (part == 0) {
+        // Step j = chunk / 2, t = 2 (chunk & 1) and the next; the other half of each word, step j ^ 1, is chunk ^ 2's.
+        const int up = (chunk & 2) ? 8 : 0;
+        constexpr uint32_t kAll = kBits + (kBits << 16) + (kBits << 4) + (kBits << 20);
+        const uint32_t a = (code[0] + (code[1] << 16) + (code[2] << 4) + (code[3] << 20) - kAll) << up;
+        const uint32_t b = (code[4] + (code[5] << 16) + (code[6] << 4) + (code[7] << 20) - kAll) << up;
+        const uint32_t got = __shfl_xor_sync(kFullMask, up ? a : b, 2), word = (up ? b : a) | got;
+        const int t = 2 * (chunk & 1) + (up ? 1 : 0);
+        if (out) *reinterpret_cast<uint32_t*>(out + at * (kDim / 2) + t * (kDim / 8) + (chunk >> 2) * 4) = word;
+      } else {
+        // Tile chunk / 2; an even chunk has the low nibbles of its 8 bytes, its odd neighbour the high ones.
+        const bool odd = chunk & 1;
+        constexpr uint32_t kAll = kBits + (kBits << 8) + (kBits << 16) + (kBits << 24);
+        const uint32_t a = code[0] + (code[1] << 8) + (code[2] << 16) + (code[3] << 24) - kAll;
+        const uint32_t b = code[4] + (code[5] << 8) + (code[6] << 16) + (code[7] << 24) - kAll;
+        const uint32_t got = __shfl_xor_sync(kFullMask, odd ? a : b, 1), bytes = odd ? got | b << 4 : a | got << 4;
+        const int tile = chunk >> 1, byte = 2 * (at & 1) + (at >> 3), lane = (odd ? 16 : 0) + ((at & 7) >> 1);
+        if (out) {
+          unsigned char* to = out + 8 * kDim + (tile >> 2) * 512 + lane * 16 + (tile & 3) * 4 + byte;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) to[64 * i] = (unsigned char)(bytes >> (8 * i));
+        }
+      }
+      if (out && chunk % kSpan == 0)
+        reinterpret_cast<Pair16<T>*>(out + 16 * kDim + part * 64 * kGroups)[at * kGroups + chunk / kSpan] = pr;
     }
-    if (out && chunk % kSpan == 0)
-      reinterpret_cast<Pair16<T>*>(out + 16 * kDim + part * 64 * kGroups)[at * kGroups + chunk / kSpan] = pr;
-  }
-  if (whole) {
-    __syncthreads();
-    unsigned char* to = kv4_run(P, slot0, head, false);
-    if (to)
-      for (int i = threadIdx.x; i < kRunBytes / 16; i += 2 * kDim) reinterpret_cast<uint4*>(to)[i] = s_run[i];
+  };
+  for (int h = 0; h < heads; ++h) {
+    alignas(16) T next[2][8];
+    if (h + 1 < heads) {
+      load(next[0], k + (h + 1) * P.k_hs);
+      load(next[1], v + (h + 1) * P.v_hs);
+    }
+    if (whole) {
+      quantise(reinterpret_cast<unsigned char*>(s_run[h & 1]), mine);
+      __syncthreads();  // also: the other buffer has been stored
+      if (run)
+        for (int i = threadIdx.x; i < kRunBytes / 16; i += 2 * kDim) reinterpret_cast<uint4*>(run)[i] = s_run[h & 1][i];
+    } else {
+      quantise(run, (int)(slot & 15));
+    }
+    if (run) run += block;
+#pragma unroll
+    for (int part = 0; part < 2; ++part)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[part][i] = next[part][i];
   }
 }
 
-// The values at slots, as kv4_write_kernel cuts them; a negative slot reads as zeros.
+// The values at slots, as kv4_write_kernel cuts them; a negative slot reads as zeros. A whole run goes through shared memory.
 template <typename T, int kDim, int kGroups>
 __global__ void __launch_bounds__(2 * kDim) kv4_read_kernel(Kv4IoParams P) {
   constexpr int kChunks = kDim / 8, kSpan = kChunks / kGroups;  // threads of a token, of a group
   constexpr int kRunBytes = 16 * kDim + 128 * kGroups;
-  __shared__ uint4 s_run[kRunBytes / 16];
+  __shared__ uint4 s_run[2][kRunBytes / 16];
   griddep_launch_wait();
-  const int chunk = threadIdx.x % kChunks, mine = threadIdx.x / kChunks, head = blockIdx.y;
+  const int chunk = threadIdx.x % kChunks, mine = threadIdx.x / kChunks;
+  const int head0 = blockIdx.y * P.span, heads = min(P.span, P.sh.heads - head0);
   const long long first = (long long)blockIdx.x * 16, tok = first + mine;
   const bool in = tok < P.tokens;
   const long long slot = in ? P.slots[tok] : -1, slot0 = P.slots[first];
   const bool whole = __syncthreads_and(in && slot == slot0 + mine && (slot0 & 15) == 0);
-  const unsigned char* run = kv4_run(P, slot, head, chunk == 0);
-  if (whole) {
-    const uint4* from = reinterpret_cast<const uint4*>(kv4_run(P, slot0, head, false));
-    if (from)
-      for (int i = threadIdx.x; i < kRunBytes / 16; i += 2 * kDim) s_run[i] = from[i];
-    __syncthreads();
-    if (run) run = reinterpret_cast<const unsigned char*>(s_run);
-  }
-  if (!in) return;
-  const int at = (int)(slot & 15);
-  const long long to = (tok * P.sh.heads + head) * kDim + 8 * chunk;
+  const unsigned char* run = kv4_run(P, whole ? slot0 : slot, head0, chunk == 0);
+  const int block = P.sh.block_bytes();
+  T* k = static_cast<T*>(P.k_out) + (tok * P.sh.heads + head0) * kDim + 8 * chunk;
+  T* v = static_cast<T*>(P.v_out) + (tok * P.sh.heads + head0) * kDim + 8 * chunk;
+  // Both parts of token `at` of the run at `from` (null: zeros).
+  const auto values = [&](const unsigned char* from, int at) {
 #pragma unroll
-  for (int part = 0; part < 2; ++part) {
-    float2 code[4];
-    alignas(16) T out[8];
-    if (run) {
-      if (part == 0) {
-        const unsigned char* w = run + at * (kDim / 2) + 2 * (chunk & 1) * (kDim / 8) + (chunk >> 2) * 4;
-        const int up = (chunk & 2) ? 8 : 0;
-        const uint32_t a = *reinterpret_cast<const uint32_t*>(w) >> up, b = *reinterpret_cast<const uint32_t*>(w + kDim / 8) >> up;
-        code[0] = kv4_codes(a), code[1] = kv4_codes(a >> 4), code[2] = kv4_codes(b), code[3] = kv4_codes(b >> 4);
+    for (int part = 0; part < 2; ++part) {
+      float2 code[4];
+      alignas(16) T out[8];
+      if (from) {
+        if (part == 0) {
+          const unsigned char* w = from + at * (kDim / 2) + 2 * (chunk & 1) * (kDim / 8) + (chunk >> 2) * 4;
+          const int up = (chunk & 2) ? 8 : 0;
+          const uint32_t a = *reinterpret_cast<const uint32_t*>(w) >> up, b = *reinterpret_cast<const uint32_t*>(w + kDim / 8) >> up;
+          code[0] = kv4_codes(a), code[1] = kv4_codes(a >> 4), code[2] = kv4_codes(b), code[3] = kv4_codes(b >> 4);
+        } else {
+          const int tile = chunk >> 1, byte = 2 * (at & 1) + (at >> 3), shift = 4 * (chunk & 1);
+          const unsigned char* c = from + 8 * kDim + (tile >> 2) * 512 + ((at & 7) >> 1) * 16 + (tile & 3) * 4 + byte;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) code[i] = kv4_codes((c[128 * i] | (uint32_t)c[128 * i + 64] << 16) >> shift);
+        }
+        const Pair16<T> pr =
+            reinterpret_cast<const Pair16<T>*>(from + 16 * kDim + part * 64 * kGroups)[at * kGroups + chunk / kSpan];
+        const float s = to_f32(pr.s), m = to_f32(pr.m);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          out[2 * i] = from_f32<T>(fmaf(s, code[i].x, m));
+          out[2 * i + 1] = from_f32<T>(fmaf(s, code[i].y, m));
+        }
       } else {
-        const int tile = chunk >> 1, byte = 2 * (at & 1) + (at >> 3), shift = 4 * (chunk & 1);
-        const unsigned char* v = run + 8 * kDim + (tile >> 2) * 512 + ((at & 7) >> 1) * 16 + (tile & 3) * 4 + byte;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) code[i] = kv4_codes((v[128 * i] | (uint32_t)v[128 * i + 64] << 16) >> shift);
+        for (int i = 0; i < 8; ++i) out[i] = from_f32<T>(0.f);
       }
-      const Pair16<T> pr =
-          reinterpret_cast<const Pair16<T>*>(run + 16 * kDim + part * 64 * kGroups)[at * kGroups + chunk / kSpan];
-      const float s = to_f32(pr.s), m = to_f32(pr.m);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        out[2 * i] = from_f32<T>(fmaf(s, code[i].x, m));
-        out[2 * i + 1] = from_f32<T>(fmaf(s, code[i].y, m));
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) out[i] = from_f32<T>(0.f);
+      if (in) *reinterpret_cast<uint4*>(part ? v : k) = *reinterpret_cast<uint4*>(out);
     }
-    *reinterpret_cast<uint4*>(static_cast<T*>(part ? P.v_out : P.k_out) + to) = *reinterpret_cast<uint4*>(out);
+    k += kDim;
+    v += kDim;
+  };
+  if (!whole || !run) {
+    for (int h = 0; h < heads; ++h) {
+      values(run, (int)(slot & 15));
+      if (run) run += block;
+    }
+    return;
+  }
+  constexpr int kPieces = kRunBytes / 16, kThreads = 2 * kDim;  // at most two pieces a thread
+  static_assert(kPieces <= 2 * kThreads, "");
+  uint4 piece[2];
+  const auto fetch = [&]() {
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      if (threadIdx.x + i * kThreads < kPieces) piece[i] = __ldg(reinterpret_cast<const uint4*>(run) + threadIdx.x + i * kThreads);
+    run += block;
+  };
+  fetch();
+  for (int h = 0; h < heads; ++h) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      if (threadIdx.x + i * kThreads < kPieces) s_run[h & 1][threadIdx.x + i * kThreads] = piece[i];
+    __syncthreads();  // also: the other buffer has been read
+    if (h + 1 < heads) fetch();
+    values(reinterpret_cast<const unsigned char*>(s_run[h & 1]), mine);
   }
 }
 

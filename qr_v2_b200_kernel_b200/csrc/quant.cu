@@ -166,7 +166,7 @@ static int launch_dequant(const int8_t* q, int64_t q_stride, const float* scale,
   if (units > ((int64_t)1 << 38)) return QRB200_ERR_ARG;
   LaunchShape l(dim3(ceil_div(units, 256)), 256, 0, s);
   const cudaError_t e =
-      cudaLaunchKernelEx(&l.cfg, aligned ? dequant_rows_kernel<T, true> : dequant_rows_kernel<T, false>, q, (long long)q_stride,
+      cudaLaunchKernelEx(&l.cfg, !aligned ? dequant_rows_kernel<T, false, true> : cols % 16 ? dequant_rows_kernel<T, true, true> : dequant_rows_kernel<T, true, false>, q, (long long)q_stride,
                          scale, static_cast<T*>(out), (long long)rows, (int)cols);
   if (e != cudaSuccess) return QRB200_ERR_CUDA;
   return launched();
@@ -279,17 +279,26 @@ static cudaError_t with_layout(const Kv4Shape& h, F&& f) {
   return h.groups == 2 ? f(Int<128>{}, Int<2>{}) : f(Int<128>{}, Int<4>{});
 }
 
+// Heads to a CTA of the write and the read: as many as leave sixteen CTAs to an SM, so that a CTA's set-up is shared by more
+// work without idling the GPU.
+static int head_span(int64_t tokens, int heads) {
+  const int64_t ctas = (tokens + 15) / 16 * heads;
+  return (int)std::max<int64_t>(1, std::min<int64_t>(heads, ctas / (16 * sm_count())));
+}
+
 template <typename T>
-static cudaError_t launch_write(const Kv4IoParams& p, bool vec, cudaStream_t s) {
-  LaunchShape l(dim3(ceil_div(p.tokens, 16), p.sh.heads), 2 * p.sh.dim, 0, s);
+static cudaError_t launch_write(Kv4IoParams p, bool vec, cudaStream_t s) {
+  p.span = head_span(p.tokens, p.sh.heads);
+  LaunchShape l(dim3(ceil_div(p.tokens, 16), ceil_div(p.sh.heads, p.span)), 2 * p.sh.dim, 0, s);
   return with_layout(p.sh, [&](auto dim, auto groups) {
     return cudaLaunchKernelEx(&l.cfg, vec ? kv4_write_kernel<T, dim(), groups(), true> : kv4_write_kernel<T, dim(), groups(), false>, p);
   });
 }
 
 template <typename T>
-static cudaError_t launch_read(const Kv4IoParams& p, cudaStream_t s) {
-  LaunchShape l(dim3(ceil_div(p.tokens, 16), p.sh.heads), 2 * p.sh.dim, 0, s);
+static cudaError_t launch_read(Kv4IoParams p, cudaStream_t s) {
+  p.span = head_span(p.tokens, p.sh.heads);
+  LaunchShape l(dim3(ceil_div(p.tokens, 16), ceil_div(p.sh.heads, p.span)), 2 * p.sh.dim, 0, s);
   return with_layout(p.sh, [&](auto dim, auto groups) { return cudaLaunchKernelEx(&l.cfg, kv4_read_kernel<T, dim(), groups()>, p); });
 }
 

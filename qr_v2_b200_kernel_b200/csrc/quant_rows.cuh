@@ -167,8 +167,8 @@ __global__ void __launch_bounds__(1024) rows_int8_kernel(RowsParams P) {
 }
 
 // value = code * scale of its row, rounded once: sixteen codes of a row to a thread, or (kAligned false) eight, 32 apart, with
-// a warp on 256 neighbouring ones.
-template <typename T, bool kAligned>
+// a warp on 256 neighbouring ones. kTail: the last of a row are fewer.
+template <typename T, bool kAligned, bool kTail>
 __global__ void __launch_bounds__(256) dequant_rows_kernel(const int8_t* q, long long q_stride, const float* scale,
                                                            T* out, long long rows, int cols) {
   constexpr int kSpan = kAligned ? 16 : 256;
@@ -183,7 +183,7 @@ __global__ void __launch_bounds__(256) dequant_rows_kernel(const int8_t* q, long
   q += row * q_stride + c;
   out += row * cols + c;
   if constexpr (kAligned) {
-    const int n = cols - c;  // a multiple of a store's elements
+    const int n = kTail ? cols - c : 16;  // a multiple of a store's elements
     uint32_t word[4] = {};
     if (n >= 16) {
       *reinterpret_cast<uint4*>(word) = __ldg(reinterpret_cast<const uint4*>(q));
