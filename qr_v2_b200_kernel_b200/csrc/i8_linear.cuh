@@ -58,6 +58,75 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, int (&v)[16]) {
       : "r"(taddr));
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
+// ---- one to four rows ----------------------------------------------------------------------
+//
+// The time is that of reading the weights once, and at these sizes mostly latency: no tiles, barriers or tensor memory, just
+// wide loads into four-way dot products. A warp takes two channels, a lane 16 codes of each 512; sums are joined by the
+// warp's integer reduction. (1 x 4096 x 4096: 6.6 us a call through the tensor cores, 4.4 us here, of which the host takes 4.2.)
+struct I8RowsParams {
+  I8Params p;
+  const int8_t* x;
+  const int8_t* w;
+  long long x_stride, w_stride;
+};
+
+// 16 codes from k on, zeros past the row's end.
+__device__ __forceinline__ uint4 i8_codes16(const int8_t* row, int k, int depth) {
+  if (k + 16 <= depth) return __ldg(reinterpret_cast<const uint4*>(row + k));
+  uint32_t w[4] = {};
+  for (int i = 0; k + i < depth; ++i) w[i >> 2] |= (uint32_t)(uint8_t)__ldg(row + k + i) << (8 * (i & 3));
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+template <typename T, int kM>
+__global__ void __launch_bounds__(128) i8_rows_kernel(I8RowsParams R) {
+  constexpr int kUnroll = 4;
+  griddep_launch_wait();
+  const I8Params& P = R.p;
+  const int lane = threadIdx.x & 31, n = (blockIdx.x * 4 + (threadIdx.x >> 5)) * 2;
+  if (n >= P.outs) return;
+  const int8_t* w0 = R.w + n * R.w_stride;
+  const int8_t* w1 = n + 1 < P.outs ? w0 + R.w_stride : w0;
+  int acc[kM][2] = {};
+  for (int k0 = 16 * lane; k0 < P.depth; k0 += 512 * kUnroll) {
+    uint4 w[kUnroll][2], x[kUnroll][kM];
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      const int k = k0 + 512 * u;
+      if (k >= P.depth) {
+        w[u][0] = w[u][1] = make_uint4(0, 0, 0, 0);
+      } else {
+        w[u][0] = i8_codes16(w0, k, P.depth);
+        w[u][1] = i8_codes16(w1, k, P.depth);
+      }
+#pragma unroll
+      for (int m = 0; m < kM; ++m)
+        x[u][m] = k < P.depth && m < P.rows ? i8_codes16(R.x + m * R.x_stride, k, P.depth) : make_uint4(0, 0, 0, 0);
+    }
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u)
+#pragma unroll
+      for (int m = 0; m < kM; ++m)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          acc[m][c] = __dp4a((int)w[u][c].x, (int)x[u][m].x, acc[m][c]);
+          acc[m][c] = __dp4a((int)w[u][c].y, (int)x[u][m].y, acc[m][c]);
+          acc[m][c] = __dp4a((int)w[u][c].z, (int)x[u][m].z, acc[m][c]);
+          acc[m][c] = __dp4a((int)w[u][c].w, (int)x[u][m].w, acc[m][c]);
+        }
+  }
+#pragma unroll
+  for (int m = 0; m < kM; ++m)
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      const int sum = __reduce_add_sync(kFullMask, acc[m][c]);
+      if (lane == 2 * m + c && m < P.rows && n + c < P.outs) {
+        const float b = P.bias ? to_f32(static_cast<const T*>(P.bias)[n + c]) : 0.f;
+        static_cast<T*>(P.y)[(long long)m * P.outs + n + c] = from_f32<T>(fmaf((float)sum * P.sx[m], P.sw[n + c], b));
+      }
+    }
+}
+
 // ---- few rows ------------------------------------------------------------------------------
 //
 // With few rows the weights are the traffic, so they are the 128-row operand (M = output

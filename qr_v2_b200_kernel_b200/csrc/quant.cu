@@ -246,7 +246,18 @@ static I8Plan i8_plan(int64_t rows, int64_t outs, int64_t depth) {
 }
 
 template <typename T>
+static cudaError_t launch_i8_rows(const I8Params& p, const I8Operand& x, const I8Operand& w, cudaStream_t s) {
+  const I8RowsParams r{p, x.base, w.base, (long long)x.stride, (long long)w.stride};
+  LaunchShape l(dim3(ceil_div(p.outs, 8)), 128, 0, s);
+  if (p.rows == 1) return cudaLaunchKernelEx(&l.cfg, i8_rows_kernel<T, 1>, r);
+  if (p.rows == 2) return cudaLaunchKernelEx(&l.cfg, i8_rows_kernel<T, 2>, r);
+  return cudaLaunchKernelEx(&l.cfg, i8_rows_kernel<T, 4>, r);
+}
+
+template <typename T>
 static cudaError_t launch_i8(const I8Params& p, const I8Operand& x, const I8Operand& w, cudaStream_t s) {
+  // A warp walks its channels' whole depth, so a long one is left to the split of the tensor-core kernel.
+  if (p.rows <= 4 && p.depth <= 8192) return launch_i8_rows<T>(p, x, w, s);
   const I8Plan plan = i8_plan(p.rows, p.outs, p.depth);
   switch (plan.rows) {
     case 16: return launch_i8_few<T, 16>(p, x, w, plan.split, s);
