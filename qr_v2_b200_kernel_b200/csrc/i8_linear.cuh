@@ -34,6 +34,9 @@ __device__ __forceinline__ void i8_load(uint32_t dst, const CUtensorMap* map, ui
 __device__ __forceinline__ void i8_expect(uint32_t mbar, uint32_t bytes) {
   asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(mbar), "r"(bytes) : "memory");
 }
+__device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
+  asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
+}
 // Descriptor of a K-major tile of 128-byte rows in the 128-byte swizzle (layout type 2): groups of 8 rows 1024 bytes
 // apart; a step of 32 codes advances the start address by 32 bytes.
 __device__ __forceinline__ uint64_t i8_sdesc(uint32_t saddr) { return make_sdesc(saddr, 16, 1024) | ((uint64_t)2 << 61); }
@@ -58,6 +61,13 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, int (&v)[16]) {
       : "r"(taddr));
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
+__device__ __forceinline__ void tmem_ld32i(uint32_t taddr, int (&v)[32]) {
+  float f[32];
+  tmem_ld32(taddr, f);
+#pragma unroll
+  for (int i = 0; i < 32; ++i) v[i] = __float_as_int(f[i]);
+}
+
 // ---- one to four rows ----------------------------------------------------------------------
 //
 // The time is that of reading the weights once, and at these sizes mostly latency: no tiles, barriers or tensor memory, just
@@ -135,10 +145,13 @@ __global__ void __launch_bounds__(128) i8_rows_kernel(I8RowsParams R) {
 // of some rows of x, exactly, through distributed shared memory, in the one launch.
 //
 // Warp 0 issues the loads, warp 1 the MMAs, warps 2-5 hold one output channel a lane.
+constexpr int kI8Split = 4;  // the most CTAs that share a tile's depth
 template <int kBN>
 struct I8Few {
   static constexpr int kStage = 128 * kI8Depth + kBN * kI8Depth;
-  static constexpr int kStages = kBN <= 32 ? 4 : 3;
+  // Loads in flight hide their latency: about 100 KB, which leaves room for the next kernel's set-up, or, for the largest
+  // tile, what one CTA can have.
+  static constexpr int kStages = kBN <= 32 ? 6 : kBN == 64 ? 5 : 6;
   static constexpr int kCols = kBN < 32 ? 32 : kBN;  // TMEM columns
   static constexpr size_t smem() { return 1024 + (size_t)kStages * kStage; }
   static_assert(kBN * 128 * 4 <= kStages * kStage, "the sums take the ring's place");
@@ -152,6 +165,7 @@ __global__ void __launch_bounds__(192) i8_few_kernel(I8Params P, const __grid_co
   __shared__ uint64_t full[C::kStages], empty[C::kStages], done;
   __shared__ uint32_t s_tmem;
   __shared__ int s_bad;
+  __shared__ float s_sx[kBN];
   unsigned char* ring = align1024(smem_raw);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int n0 = blockIdx.x * 128, i0 = blockIdx.y * kBN;
@@ -168,6 +182,8 @@ __global__ void __launch_bounds__(192) i8_few_kernel(I8Params P, const __grid_co
     s_bad = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     fence_async_smem();
+    prefetch_map(&tm_w);
+    prefetch_map(&tm_x);
   }
   griddep_launch_wait();  // before TMEM is taken: a kernel still running may need it
   if (warp == 1) tmem_alloc(&s_tmem, C::kCols);
@@ -213,80 +229,73 @@ __global__ void __launch_bounds__(192) i8_few_kernel(I8Params P, const __grid_co
   __syncwarp();
   const int ch = ((warp & 3) << 5) + lane;  // the channel, and the TMEM lane, of warps 2-5
   const bool epi = warp >= 2;
-  const int n = n0 + ch;
   const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-  float sw = 0.f, b = 0.f;
-  if (epi && n < P.outs) {
-    sw = P.sw[n];
-    if (P.bias) b = to_f32(static_cast<const T*>(P.bias)[n]);
+  // Four channels a lane for the way out, their scales and bias asked for while the products run.
+  const int c4 = 4 * lane;
+  float w4[4] = {}, b4[4] = {};
+  if (epi) {
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const bool in = n0 + c4 + c < P.outs;
+      w4[c] = in ? P.sw[n0 + c4 + c] : 0.f;
+      b4[c] = in && P.bias ? to_f32(static_cast<const T*>(P.bias)[n0 + c4 + c]) : 0.f;
+    }
+    for (int j = threadIdx.x - 64; j < kBN; j += 128) s_sx[j] = i0 + j < P.rows ? P.sx[i0 + j] : 0.f;
+    if (!mbar_wait(&done, 0)) s_bad = 1;
   }
-  T* y = static_cast<T*>(P.y);
-  auto put = [&](int j, int acc) {
-    if (n < P.outs && i0 + j < P.rows)
-      y[(long long)(i0 + j) * P.outs + n] = from_f32<T>(fmaf((float)acc * P.sx[i0 + j], sw, b));
-  };
-  if (epi && !mbar_wait(&done, 0)) s_bad = 1;
   tc_fence_after();
   __syncthreads();
-  if (split == 1) {
-    if (epi && !s_bad)
+  // The ring is free (every load has landed, every MMA is done): sums as [row][channel]. Row j is CTA j % split's to add and
+  // to write, a warp to a row.
+  int* sums = reinterpret_cast<int*>(ring);
+  if (epi)
 #pragma unroll 1
-      for (int j = 0; j < kBN && i0 + j < P.rows; j += 16) {
-        int v[16];
-        tmem_ld16(lanes + j, v);
+    for (int j = 0; j < kBN && i0 + j < P.rows; j += 16) {
+      int v[16];
+      tmem_ld16(lanes + j, v);
 #pragma unroll
-        for (int q = 0; q < 16; ++q) put(j + q, v[q]);
-      }
-  } else {
-    // The ring is free (every load has landed, every MMA is done): sums as [row][channel]. Row j is CTA j % split's to add.
-    int* sums = reinterpret_cast<int*>(ring);
-    if (epi)
-#pragma unroll 1
-      for (int j = 0; j < kBN && i0 + j < P.rows; j += 16) {
-        int v[16];
-        tmem_ld16(lanes + j, v);
-#pragma unroll
-        for (int q = 0; q < 16; ++q) sums[(j + q) * 128 + ch] = v[q];
-      }
+      for (int q = 0; q < 16; ++q) sums[(j + q) * 128 + ch] = v[q];
+    }
+  bool bad = false;
+  if (split > 1) {
     cluster_sync();
-    bool bad = false;
     for (int r = 0; r < split; ++r) bad = ld_cluster(smem_u32(&s_bad), r) != 0 || bad;
-    if (epi && !bad) {
-      // A warp to a row, four channels a lane.
-      const int c4 = 4 * lane, et = threadIdx.x >> 5;
-      float w4[4], b4[4];
+  } else {
+    __syncthreads();
+    bad = s_bad != 0;
+  }
+  if (epi && !bad) {
+    T* y = static_cast<T*>(P.y);
+    const bool whole = P.outs % 4 == 0;
+    for (int j = part + split * (warp - 2); j < kBN && i0 + j < P.rows; j += 4 * split) {
+      int4 acc = make_int4(0, 0, 0, 0);
+      if (split == 1) {
+        acc = *reinterpret_cast<const int4*>(&sums[j * 128 + c4]);
+      } else {
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        const bool in = n0 + c4 + c < P.outs;
-        w4[c] = in ? P.sw[n0 + c4 + c] : 0.f;
-        b4[c] = in && P.bias ? to_f32(static_cast<const T*>(P.bias)[n0 + c4 + c]) : 0.f;
-      }
-      for (int j = part + split * (et - 2); j < kBN && i0 + j < P.rows; j += 4 * split) {
-        int4 acc = make_int4(0, 0, 0, 0);
-#pragma unroll
-        for (int r = 0; r < 8; ++r)
+        for (int r = 0; r < kI8Split; ++r)
           if (r < split) {
             const int4 v = ld_cluster4(smem_u32(&sums[j * 128 + c4]), r);
             acc.x += v.x, acc.y += v.y, acc.z += v.z, acc.w += v.w;
           }
-        const float sx = P.sx[i0 + j];
-        alignas(16) T out[4] = {from_f32<T>(fmaf((float)acc.x * sx, w4[0], b4[0])), from_f32<T>(fmaf((float)acc.y * sx, w4[1], b4[1])),
-                                from_f32<T>(fmaf((float)acc.z * sx, w4[2], b4[2])), from_f32<T>(fmaf((float)acc.w * sx, w4[3], b4[3]))};
-        T* to = y + (long long)(i0 + j) * P.outs + n0 + c4;
-        if (P.outs % 4 == 0) {
-          if (n0 + c4 < P.outs) {
-            if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4*>(to) = *reinterpret_cast<const uint4*>(out);
-            else *reinterpret_cast<uint2*>(to) = *reinterpret_cast<const uint2*>(out);
-          }
-        } else {
-#pragma unroll
-          for (int c = 0; c < 4; ++c)
-            if (n0 + c4 + c < P.outs) to[c] = out[c];
+      }
+      const float sx = s_sx[j];
+      alignas(16) T out[4] = {from_f32<T>(fmaf((float)acc.x * sx, w4[0], b4[0])), from_f32<T>(fmaf((float)acc.y * sx, w4[1], b4[1])),
+                              from_f32<T>(fmaf((float)acc.z * sx, w4[2], b4[2])), from_f32<T>(fmaf((float)acc.w * sx, w4[3], b4[3]))};
+      T* to = y + (long long)(i0 + j) * P.outs + n0 + c4;
+      if (whole) {
+        if (n0 + c4 < P.outs) {
+          if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4*>(to) = *reinterpret_cast<const uint4*>(out);
+          else *reinterpret_cast<uint2*>(to) = *reinterpret_cast<const uint2*>(out);
         }
+      } else {
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          if (n0 + c4 + c < P.outs) to[c] = out[c];
       }
     }
-    cluster_sync();  // nobody leaves while its sums are being read
   }
+  if (split > 1) cluster_sync();  // nobody leaves while its sums are being read
   tc_fence_before();
   __syncthreads();
   if (warp == 1) tmem_dealloc(tmem, C::kCols);
@@ -297,11 +306,12 @@ __global__ void __launch_bounds__(192) i8_few_kernel(I8Params P, const __grid_co
 // 256 rows x 256 channels per pair of CTAs (cta_group::2: each CTA holds 128 rows of x, 128 of the
 // channels' weights and its rows' 128 x 256 sums), persistent, with two accumulators in TMEM so
 // that a tile's epilogue runs under the next tile's products. Warp 0 loads its CTA's halves, warp
-// 1 of the pair's first CTA issues the MMAs, warps 4-7 scale, round and store.
+// 1 of the pair's first CTA issues the MMAs, warps 4-11 scale, round and store, half of a tile's channels each four.
 constexpr int kI8WideStage = 2 * 128 * kI8Depth;  // bytes per CTA and stage
 constexpr int kI8WideStages = 5;
+constexpr int kI8WideEpi = 8;  // epilogue warps
 constexpr int kI8Pitch = 144;  // bytes of a staged output row (128 and 16 to spread the banks)
-constexpr size_t i8_wide_smem() { return 1024 + (size_t)kI8WideStages * kI8WideStage + 4 * 32 * kI8Pitch; }
+constexpr size_t i8_wide_smem() { return 1024 + (size_t)kI8WideStages * kI8WideStage + kI8WideEpi * 32 * kI8Pitch; }
 
 __device__ __forceinline__ uint32_t pair_leader(uint32_t addr) {  // the same address in the pair's first CTA
   uint32_t a;
@@ -333,7 +343,7 @@ __device__ __forceinline__ void commit_pair(uint64_t* mbar) {  // arrives on thi
 }
 
 template <typename T>
-__global__ void __launch_bounds__(256, 1) __cluster_dims__(2, 1, 1)
+__global__ void __launch_bounds__(128 + 32 * kI8WideEpi, 1) __cluster_dims__(2, 1, 1)
     i8_wide_kernel(I8Params P, const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w) {
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   __shared__ uint64_t full[kI8WideStages], empty[kI8WideStages], acc_full[2], acc_empty[2];
@@ -353,10 +363,12 @@ __global__ void __launch_bounds__(256, 1) __cluster_dims__(2, 1, 1)
     }
     for (int s = 0; s < 2; ++s) {
       mbar_init(&acc_full[s], 1);
-      mbar_init(&acc_empty[s], 8);  // the four epilogue warps of both CTAs
+      mbar_init(&acc_empty[s], 2 * kI8WideEpi);  // the epilogue warps of both CTAs
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     fence_async_smem();
+    prefetch_map(&tm_w);
+    prefetch_map(&tm_x);
   }
   griddep_launch_wait();  // before TMEM is taken: a kernel still running may need it
   if (warp == 2) {
@@ -426,8 +438,8 @@ __global__ void __launch_bounds__(256, 1) __cluster_dims__(2, 1, 1)
     }
   } else if (warp >= 4) {
     constexpr int kPer = 128 / sizeof(T);  // outputs in a staged row of 128 bytes
-    const int ew = warp - 4, et = threadIdx.x - 128;
-    unsigned char* mine = staged + ew * 32 * kI8Pitch;
+    const int ew = warp & 3, half = (warp - 4) >> 2, et = threadIdx.x - 128;
+    unsigned char* mine = staged + (warp - 4) * 32 * kI8Pitch;
     const uint32_t lanes = tmem + ((uint32_t)(ew * 32) << 16);
     const bool wide = P.outs % (16 / (int)sizeof(T)) == 0;  // 16-byte rows of y (y itself is 16-byte aligned)
     T* y = static_cast<T*>(P.y);
@@ -437,27 +449,27 @@ __global__ void __launch_bounds__(256, 1) __cluster_dims__(2, 1, 1)
       int m, n;
       place(tile, m, n);
       const int n0 = n * 256, row0 = m * 256 + (int)rank * 128 + ew * 32;
-      asm volatile("bar.sync 1, 128;" ::: "memory");  // the last tile's scales have been read
-      for (int c = et; c < 256; c += 128) {
+      named_sync(1, 32 * kI8WideEpi);  // the last tile's scales have been read
+      for (int c = et; c < 256; c += 32 * kI8WideEpi) {
         const bool in = n0 + c < P.outs;
         s_sw[c] = in ? P.sw[n0 + c] : 0.f;
         s_b[c] = in && P.bias ? to_f32(static_cast<const T*>(P.bias)[n0 + c]) : 0.f;
       }
-      asm volatile("bar.sync 1, 128;" ::: "memory");
+      named_sync(1, 32 * kI8WideEpi);
       const float sx = row0 + lane < P.rows ? P.sx[row0 + lane] : 0.f;
       bad = bad || !__all_sync(kFullMask, mbar_wait(&acc_full[t & 1], (t >> 1) & 1));
       tc_fence_after();
       if (bad) continue;
 #pragma unroll 1
-      for (int c0 = 0; c0 < 256; c0 += kPer) {
+      for (int c0 = 128 * half; c0 < 128 * half + 128; c0 += kPer) {
         __syncwarp();
 #pragma unroll
-        for (int h = 0; h < kPer; h += 16) {
-          int v[16];
-          tmem_ld16(lanes + (t & 1) * 256 + c0 + h, v);
-          T out[16];
+        for (int h = 0; h < kPer; h += 32) {
+          int v[32];
+          tmem_ld32i(lanes + (t & 1) * 256 + c0 + h, v);
+          alignas(16) T out[32];
 #pragma unroll
-          for (int q = 0; q < 16; q += 4) {
+          for (int q = 0; q < 32; q += 4) {
             const float4 w4 = *reinterpret_cast<const float4*>(&s_sw[c0 + h + q]);
             const float4 b4 = *reinterpret_cast<const float4*>(&s_b[c0 + h + q]);
             out[q] = from_f32<T>(fmaf((float)v[q] * sx, w4.x, b4.x));
@@ -466,10 +478,10 @@ __global__ void __launch_bounds__(256, 1) __cluster_dims__(2, 1, 1)
             out[q + 3] = from_f32<T>(fmaf((float)v[q + 3] * sx, w4.w, b4.w));
           }
 #pragma unroll
-          for (int q = 0; q < 16 * (int)sizeof(T) / 16; ++q)
+          for (int q = 0; q < 32 * (int)sizeof(T) / 16; ++q)
             *reinterpret_cast<uint4*>(mine + lane * kI8Pitch + h * sizeof(T) + 16 * q) = reinterpret_cast<uint4*>(out)[q];
         }
-        if (c0 + kPer >= 256) {  // every sum of this warp is in registers: the accumulator is free
+        if (c0 + kPer >= 128 * half + 128) {  // every sum of this warp is in registers: the accumulator is free
           tc_fence_before();
           if (lane == 0)
             asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(

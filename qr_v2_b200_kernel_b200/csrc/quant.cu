@@ -213,13 +213,13 @@ static cudaError_t launch_i8_wide(I8Params p, const I8Operand& x, const I8Operan
   if (tiles > (1 << 30)) return cudaErrorInvalidValue;
   p.tiles = (int)tiles;
   const int pairs = std::min(p.tiles, sm_count() / 2);
-  LaunchShape l(dim3(2 * pairs), 256, i8_wide_smem(), s);
+  LaunchShape l(dim3(2 * pairs), 128 + 32 * kI8WideEpi, i8_wide_smem(), s);
   return cudaLaunchKernelEx(&l.cfg, i8_wide_kernel<T>, p, tx, tw);
 }
 
 // Which kernel, with how many rows a tile (`rows`) and over how many CTAs of the depth: the least of the estimated clocks. A CTA
-// takes in its stages at about 64 bytes a clock; joining a split costs two cluster barriers (about 1500 clocks) and reading
-// the sums at about 16 bytes a clock. The wide kernel's pair takes 512 clocks a stage and a tile's last epilogue is bare.
+// takes in its stages at about 40 bytes a clock; joining a split costs two cluster barriers (about 1500 clocks) and reading
+// the sums at about 16 bytes a clock. Clusters of eight lose: a GPC holds two at best (64 x 1000 x 2048: 12 us against 9). The wide kernel's pair takes 512 clocks a stage and a tile's last epilogue is bare.
 struct I8Plan {
   int rows;  // 16, 32, 64 or 128 (few), 256 (wide)
   unsigned split;
@@ -232,9 +232,9 @@ static I8Plan i8_plan(int64_t rows, int64_t outs, int64_t depth) {
   for (int bn = 16; bn <= 128; bn *= 2) {
     const int64_t tiles = (rows + bn - 1) / bn * ((outs + 127) / 128);
     if ((rows + bn - 1) / bn > 65535) continue;
-    for (unsigned split = 1; split <= 8 && split <= nk; split *= 2) {
-      const int64_t clocks = (tiles * split + sms - 1) / sms * ((nk + split - 1) / split) * (128 + bn) * 2 +
-                             (split > 1 ? 1500 + bn * 32 : bn * 8);
+    for (unsigned split = 1; split <= kI8Split && split <= nk; split *= 2) {
+      const int64_t clocks = (tiles * split + sms - 1) / sms *
+                             ((nk + split - 1) / split * (128 + bn) * 128 / 40 + (split > 1 ? 1500 + bn * 32 : bn * 8));
       if (clocks < least) {
         least = clocks;
         best = I8Plan{bn, split};
