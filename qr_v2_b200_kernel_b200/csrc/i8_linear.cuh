@@ -280,8 +280,9 @@ __global__ void __launch_bounds__(192) i8_few_kernel(I8Params P, const __grid_co
           }
       }
       const float sx = s_sx[j];
-      alignas(16) T out[4] = {from_f32<T>(fmaf((float)acc.x * sx, w4[0], b4[0])), from_f32<T>(fmaf((float)acc.y * sx, w4[1], b4[1])),
-                              from_f32<T>(fmaf((float)acc.z * sx, w4[2], b4[2])), from_f32<T>(fmaf((float)acc.w * sx, w4[3], b4[3]))};
+      alignas(16) T out[4];
+      put2(out, fmaf((float)acc.x * sx, w4[0], b4[0]), fmaf((float)acc.y * sx, w4[1], b4[1]));
+      put2(out + 2, fmaf((float)acc.z * sx, w4[2], b4[2]), fmaf((float)acc.w * sx, w4[3], b4[3]));
       T* to = y + (long long)(i0 + j) * P.outs + n0 + c4;
       if (whole) {
         if (n0 + c4 < P.outs) {
@@ -348,7 +349,7 @@ __global__ void __launch_bounds__(128 + 32 * kI8WideEpi, 1) __cluster_dims__(2, 
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   __shared__ uint64_t full[kI8WideStages], empty[kI8WideStages], acc_full[2], acc_empty[2];
   __shared__ uint32_t s_tmem;
-  __shared__ __align__(16) float s_sw[256], s_b[256];
+  __shared__ __align__(16) float s_sw[2][256], s_b[2][256];
   unsigned char* ring = align1024(smem_raw);
   unsigned char* staged = ring + kI8WideStages * kI8WideStage;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -445,18 +446,30 @@ __global__ void __launch_bounds__(128 + 32 * kI8WideEpi, 1) __cluster_dims__(2, 
     T* y = static_cast<T*>(P.y);
     int t = 0;
     bool bad = false;  // a wait ran out: keep to the barriers, touch nothing
+    // A tile's scales are asked for while the tile before it is scaled: a channel's to each thread, its own row's to each lane.
+    float next_sw = 0.f, next_b = 0.f, next_sx = 0.f;
+    const auto ask = [&](int tile) {
+      if (tile >= P.tiles) return;
+      int m, n;
+      place(tile, m, n);
+      const int c = n * 256 + et, r = m * 256 + (int)rank * 128 + ew * 32 + lane;
+      next_sw = c < P.outs ? P.sw[c] : 0.f;
+      next_b = c < P.outs && P.bias ? to_f32(static_cast<const T*>(P.bias)[c]) : 0.f;
+      next_sx = r < P.rows ? P.sx[r] : 0.f;
+    };
+    static_assert(32 * kI8WideEpi == 256, "a channel to a thread");
+    ask(pair);
     for (int tile = pair; tile < P.tiles; tile += pairs, ++t) {
       int m, n;
       place(tile, m, n);
       const int n0 = n * 256, row0 = m * 256 + (int)rank * 128 + ew * 32;
-      named_sync(1, 32 * kI8WideEpi);  // the last tile's scales have been read
-      for (int c = et; c < 256; c += 32 * kI8WideEpi) {
-        const bool in = n0 + c < P.outs;
-        s_sw[c] = in ? P.sw[n0 + c] : 0.f;
-        s_b[c] = in && P.bias ? to_f32(static_cast<const T*>(P.bias)[n0 + c]) : 0.f;
-      }
-      named_sync(1, 32 * kI8WideEpi);
-      const float sx = row0 + lane < P.rows ? P.sx[row0 + lane] : 0.f;
+      const float* sw = s_sw[t & 1];
+      const float* sb = s_b[t & 1];
+      s_sw[t & 1][et] = next_sw;
+      s_b[t & 1][et] = next_b;
+      const float sx = next_sx;
+      named_sync(1, 32 * kI8WideEpi);  // also: the tile before the last has been scaled, so the other buffer is free
+      ask(tile + pairs);
       bad = bad || !__all_sync(kFullMask, mbar_wait(&acc_full[t & 1], (t >> 1) & 1));
       tc_fence_after();
       if (bad) continue;
@@ -470,12 +483,10 @@ __global__ void __launch_bounds__(128 + 32 * kI8WideEpi, 1) __cluster_dims__(2, 
           alignas(16) T out[32];
 #pragma unroll
           for (int q = 0; q < 32; q += 4) {
-            const float4 w4 = *reinterpret_cast<const float4*>(&s_sw[c0 + h + q]);
-            const float4 b4 = *reinterpret_cast<const float4*>(&s_b[c0 + h + q]);
-            out[q] = from_f32<T>(fmaf((float)v[q] * sx, w4.x, b4.x));
-            out[q + 1] = from_f32<T>(fmaf((float)v[q + 1] * sx, w4.y, b4.y));
-            out[q + 2] = from_f32<T>(fmaf((float)v[q + 2] * sx, w4.z, b4.z));
-            out[q + 3] = from_f32<T>(fmaf((float)v[q + 3] * sx, w4.w, b4.w));
+            const float4 w4 = *reinterpret_cast<const float4*>(&sw[c0 + h + q]);
+            const float4 b4 = *reinterpret_cast<const float4*>(&sb[c0 + h + q]);
+            put2(out + q, fmaf((float)v[q] * sx, w4.x, b4.x), fmaf((float)v[q + 1] * sx, w4.y, b4.y));
+            put2(out + q + 2, fmaf((float)v[q + 2] * sx, w4.z, b4.z), fmaf((float)v[q + 3] * sx, w4.w, b4.w));
           }
 #pragma unroll
           for (int q = 0; q < 32 * (int)sizeof(T) / 16; ++q)

@@ -244,10 +244,7 @@ __global__ void __launch_bounds__(2 * kDim) kv4_read_kernel(Kv4IoParams P) {
             reinterpret_cast<const Pair16<T>*>(from + 16 * kDim + part * 64 * kGroups)[at * kGroups + chunk / kSpan];
         const float s = to_f32(pr.s), m = to_f32(pr.m);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          out[2 * i] = from_f32<T>(fmaf(s, code[i].x, m));
-          out[2 * i + 1] = from_f32<T>(fmaf(s, code[i].y, m));
-        }
+        for (int i = 0; i < 4; ++i) put2(out + 2 * i, fmaf(s, code[i].x, m), fmaf(s, code[i].y, m));
       } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i) out[i] = from_f32<T>(0.f);

@@ -32,6 +32,13 @@ __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { retu
 template <>
 __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
 
+// Two neighbouring results, rounded by one instruction where T has 16 bits.
+__device__ __forceinline__ void put2(float* p, float a, float b) { *reinterpret_cast<float2*>(p) = make_float2(a, b); }
+__device__ __forceinline__ void put2(__nv_bfloat16* p, float a, float b) {
+  *reinterpret_cast<__nv_bfloat162*>(p) = __floats2bfloat162_rn(a, b);
+}
+__device__ __forceinline__ void put2(__half* p, float a, float b) { *reinterpret_cast<__half2*>(p) = __floats2half2_rn(a, b); }
+
 struct RowsParams {
   const void* x;
   const void* residual;  // may be null
@@ -85,7 +92,7 @@ __global__ void __launch_bounds__(1024) rows_int8_kernel(RowsParams P) {
   const T* x = static_cast<const T*>(P.x) + row * P.x_stride;
   const T* r = static_cast<const T*>(P.residual) + row * P.r_stride;
   const W* w = static_cast<const W*>(P.weight);
-  T xv[kItems][kVec], rv[kItems][kVec];
+  alignas(16) T xv[kItems][kVec], rv[kItems][kVec];
   float t[kItems][kVec];
 #pragma unroll
   for (int i = 0; i < kItems; ++i) {
@@ -105,9 +112,10 @@ __global__ void __launch_bounds__(1024) rows_int8_kernel(RowsParams P) {
     if constexpr (kNorm) {
       if (P.residual) {
 #pragma unroll
-        for (int e = 0; e < kVec; ++e) {
+        for (int e = 0; e < kVec; e += 2) {
           t[i][e] += to_f32(rv[i][e]);
-          rv[i][e] = from_f32<T>(t[i][e]);
+          t[i][e + 1] += to_f32(rv[i][e + 1]);
+          put2(&rv[i][e], t[i][e], t[i][e + 1]);
         }
         store_pack<kAligned>(static_cast<T*>(P.h_out) + row * P.cols + c * kVec, rv[i], P.cols - c * kVec);
       }
@@ -196,10 +204,13 @@ __global__ void __launch_bounds__(256) dequant_rows_kernel(const int8_t* q, long
     for (int h = 0; h < 16; h += kPart) {
       alignas(16) T v[kPart];
 #pragma unroll
-      for (int e = 0; e < kPart; ++e) {
+      for (int e = 0; e < kPart; e += 2) {
         // A byte plus 128, under the exponent of 2^23: exact, and cheaper than a conversion.
-        const uint32_t bits = __byte_perm(word[(h + e) / 4] ^ 0x80808080u, 0x4b000000u, 0x7440 + ((h + e) & 3));
-        v[e] = from_f32<T>((__uint_as_float(bits) - 8388736.f) * s);
+        const auto value = [&](int i) {
+          const uint32_t bits = __byte_perm(word[i / 4] ^ 0x80808080u, 0x4b000000u, 0x7440 + (i & 3));
+          return (__uint_as_float(bits) - 8388736.f) * s;
+        };
+        put2(&v[e], value(h + e), value(h + e + 1));
       }
       if (h < n) store_pack<true>(out + h, v, kPart);
     }
