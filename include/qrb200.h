@@ -170,13 +170,16 @@ int qrb200_dequantize_int8(const int8_t* q, int64_t q_stride, const float* scale
                            int64_t cols, int dtype, void* stream);
 
 /* y[i, n] = (sum_k x[i, k] w[n, k]) x_scale[i] w_scale[n] + bias[n]: y rows x outs of dtype,
- * contiguous; bias (may be NULL) of dtype; row strides of x and w in bytes; x, w, y and the
- * strides (where there is more than one row) multiples of 16 bytes, else QRB200_ERR_ARG. The sum is exact in
- * 32-bit integers for depth <= QRB200_INT8_MAX_DEPTH. */
+ * contiguous, 16-byte aligned; bias (may be NULL) of dtype; row strides of x and w in bytes. The sum is
+ * exact in 32-bit integers for depth <= QRB200_INT8_MAX_DEPTH. Operands whose rows start on 16-byte
+ * boundaries are read as they lie; others are first laid out in the workspace (256-byte aligned, its
+ * size from the query; 0 for the former). */
 #define QRB200_INT8_MAX_DEPTH 131071
+size_t qrb200_int8_linear_workspace_bytes(const int8_t* x, int64_t x_stride, const int8_t* w, int64_t w_stride,
+                                          int64_t rows, int64_t outs, int64_t depth);
 int qrb200_int8_linear(const int8_t* x, int64_t x_stride, const float* x_scale, const int8_t* w, int64_t w_stride,
                        const float* w_scale, const void* bias, void* y, int64_t rows, int64_t outs, int64_t depth,
-                       int dtype, void* stream);
+                       int dtype, void* workspace, size_t workspace_bytes, void* stream);
 
 /* A paged key/value cache in 4 bits: pages x kv_heads blocks of qrb200_kv4_block_bytes bytes,
  * contiguous, 16-byte aligned. Each group of head_dim / groups channels of a token holds 4-bit

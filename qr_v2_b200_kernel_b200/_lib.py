@@ -69,7 +69,8 @@ SIGNATURES = {
     "qrb200_rms_norm_int8": (_INT, [_P, _I64, _P, _I64, _P, _INT, _P, _I64, _P, _P, _I64, _I64, _F32, _INT, _P]),
     "qrb200_quantize_int8": (_INT, [_P, _I64, _P, _I64, _P, _I64, _I64, _INT, _P]),
     "qrb200_dequantize_int8": (_INT, [_P, _I64, _P, _P, _I64, _I64, _INT, _P]),
-    "qrb200_int8_linear": (_INT, [_P, _I64, _P, _P, _I64, _P, _P, _P, _I64, _I64, _I64, _INT, _P]),
+    "qrb200_int8_linear_workspace_bytes": (_SIZE, [_P, _I64, _P, _I64, _I64, _I64, _I64]),
+    "qrb200_int8_linear": (_INT, [_P, _I64, _P, _P, _I64, _P, _P, _P, _I64, _I64, _I64, _INT, _P, _SIZE, _P]),
     "qrb200_kv4_block_bytes": (_I64, [_I64, _I64, _I64]),
     "qrb200_kv4_write": (_INT, [_P, _P, _P, _I64, _I64, _P, _I64, _I64, _P, _I64, _P]),
     "qrb200_kv4_read": (_INT, [_P, _P, _P, _P, _P, _I64, _P]),

@@ -68,25 +68,63 @@ __device__ __forceinline__ void tmem_ld32i(uint32_t taddr, int (&v)[32]) {
   for (int i = 0; i < 32; ++i) v[i] = __float_as_int(f[i]);
 }
 
+// ---- rows off 16-byte boundaries -----------------------------------------------------------
+
+struct I8Operand {
+  const int8_t* base;
+  long long rows, stride;  // bytes
+  bool aligned;            // base and stride are multiples of 16
+};
+
+// Sixteen codes of a row from column k on, zeros past the row's end, from any address: neighbouring aligned words, shifted,
+// where those lie within the operand, else byte by byte.
+__device__ __forceinline__ uint4 i8_codes16(const I8Operand& o, long long row, int k, int depth) {
+  const int8_t* p = o.base + row * o.stride + k;
+  const int n = depth - k;
+  if (o.aligned && n >= 16) return __ldg(reinterpret_cast<const uint4*>(p));
+  uint32_t w[4] = {};
+  const uintptr_t at = reinterpret_cast<uintptr_t>(p);
+  const uint32_t* word = reinterpret_cast<const uint32_t*>(at & ~(uintptr_t)3);
+  const int8_t* end = o.base + (o.rows - 1) * o.stride + depth;
+  if (reinterpret_cast<const int8_t*>(word) >= o.base && reinterpret_cast<const int8_t*>(word + 5) <= end) {
+    const int shift = 8 * (int)(at & 3);
+    uint32_t v[5];
+#pragma unroll
+    for (int i = 0; i < 5; ++i) v[i] = __ldg(word + i);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      w[i] = __funnelshift_r(v[i], v[i + 1], shift);
+      const int keep = n - 4 * i;  // bytes of this word inside the row
+      if (keep < 4) w[i] = keep > 0 ? w[i] & (0xffffffffu >> (32 - 8 * keep)) : 0u;
+    }
+  } else {
+    for (int i = 0; i < n && i < 16; ++i) w[i >> 2] |= (uint32_t)(uint8_t)__ldg(p + i) << (8 * (i & 3));
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// Lays an operand out for the tensor-core kernels, which load by TMA: rows of `packs` 16-byte packs.
+__global__ void __launch_bounds__(256) i8_pad_kernel(I8Operand a, uint4* to_a, I8Operand b, uint4* to_b, int depth, int packs) {
+  griddep_launch_wait();
+  long long at = (long long)blockIdx.x * 256 + threadIdx.x;
+  const long long first = to_a ? a.rows * packs : 0;
+  const bool second = at >= first;
+  if (second) at -= first;
+  const I8Operand o = second ? b : a;
+  uint4* to = second ? to_b : to_a;
+  if (!to || at >= o.rows * packs) return;
+  to[at] = i8_codes16(o, at / packs, (int)(at % packs) * 16, depth);
+}
+
 // ---- one to four rows ----------------------------------------------------------------------
 //
 // The time is that of reading the weights once, and at these sizes mostly latency: no tiles, barriers or tensor memory, just
-// wide loads into four-way dot products. A warp takes two channels, a lane 16 codes of each 512; sums are joined by the
-// warp's integer reduction. (1 x 4096 x 4096: 6.6 us a call through the tensor cores, 4.4 us here, of which the host takes 4.2.)
+// wide loads into four-way dot products, and operands as they lie. A warp takes two channels, a lane 16 codes of each 512; sums are joined by the
+// warp's integer reduction. (1 x 4096 x 4096: 6.6 us through the tensor cores, 3.2 us here, 5.2 TB/s of weights that L2 holds.)
 struct I8RowsParams {
   I8Params p;
-  const int8_t* x;
-  const int8_t* w;
-  long long x_stride, w_stride;
+  I8Operand x, w;
 };
-
-// 16 codes from k on, zeros past the row's end.
-__device__ __forceinline__ uint4 i8_codes16(const int8_t* row, int k, int depth) {
-  if (k + 16 <= depth) return __ldg(reinterpret_cast<const uint4*>(row + k));
-  uint32_t w[4] = {};
-  for (int i = 0; k + i < depth; ++i) w[i >> 2] |= (uint32_t)(uint8_t)__ldg(row + k + i) << (8 * (i & 3));
-  return make_uint4(w[0], w[1], w[2], w[3]);
-}
 
 template <typename T, int kM>
 __global__ void __launch_bounds__(128) i8_rows_kernel(I8RowsParams R) {
@@ -95,8 +133,7 @@ __global__ void __launch_bounds__(128) i8_rows_kernel(I8RowsParams R) {
   const I8Params& P = R.p;
   const int lane = threadIdx.x & 31, n = (blockIdx.x * 4 + (threadIdx.x >> 5)) * 2;
   if (n >= P.outs) return;
-  const int8_t* w0 = R.w + n * R.w_stride;
-  const int8_t* w1 = n + 1 < P.outs ? w0 + R.w_stride : w0;
+  const int n1 = min(n + 1, P.outs - 1);
   int acc[kM][2] = {};
   for (int k0 = 16 * lane; k0 < P.depth; k0 += 512 * kUnroll) {
     uint4 w[kUnroll][2], x[kUnroll][kM];
@@ -106,12 +143,12 @@ __global__ void __launch_bounds__(128) i8_rows_kernel(I8RowsParams R) {
       if (k >= P.depth) {
         w[u][0] = w[u][1] = make_uint4(0, 0, 0, 0);
       } else {
-        w[u][0] = i8_codes16(w0, k, P.depth);
-        w[u][1] = i8_codes16(w1, k, P.depth);
+        w[u][0] = i8_codes16(R.w, n, k, P.depth);
+        w[u][1] = i8_codes16(R.w, n1, k, P.depth);
       }
 #pragma unroll
       for (int m = 0; m < kM; ++m)
-        x[u][m] = k < P.depth && m < P.rows ? i8_codes16(R.x + m * R.x_stride, k, P.depth) : make_uint4(0, 0, 0, 0);
+        x[u][m] = k < P.depth && m < P.rows ? i8_codes16(R.x, m, k, P.depth) : make_uint4(0, 0, 0, 0);
     }
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u)

@@ -70,10 +70,6 @@ Tensor empty_codes(int64_t rows, int64_t cols, const Tensor& like) {
   Tensor q = empty({rows, padded}, at::kChar, like);
   return padded == cols ? q : q.slice(1, 0, cols);
 }
-Tensor loadable(const Tensor& t) {
-  if (reinterpret_cast<uintptr_t>(t.const_data_ptr()) % 16 == 0 && (t.size(0) == 1 || t.stride(0) % 16 == 0)) return t;
-  return empty_codes(t.size(0), t.size(1), t).copy_(t);
-}
 Tensor shaped(const Tensor& q, const Tensor& x) {
   if (x.dim() == 2) return q;
   return x.dim() == 1 ? q.select(0, 0) : q.unflatten(0, x.sizes().slice(0, x.dim() - 1));
@@ -183,18 +179,19 @@ Tensor int8_linear(const Tensor& x, const Tensor& x_scale, const Tensor& weight,
     bias = bias->contiguous();
   }
   OnDevice on(x);
-  Tensor xr = as_rows(x), wr = as_rows(weight);
+  const Tensor xr = as_rows(x), wr = as_rows(weight);
   const int64_t rows = xr.size(0);
   c10::SmallVector<int64_t, 5> sizes(x.sizes().begin(), x.sizes().end());
   sizes.back() = outs;
   const Tensor y = empty(sizes, dtype, x);
   if (rows == 0 || outs == 0) return y;
-  xr = loadable(xr);
-  wr = loadable(wr);
+  const int8_t *xp = xr.const_data_ptr<int8_t>(), *wp = wr.const_data_ptr<int8_t>();
+  const size_t need = qrb200_int8_linear_workspace_bytes(xp, xr.stride(0), wp, wr.stride(0), rows, outs, depth);
+  Tensor ws;
+  if (need > 0) ws = empty({(int64_t)need}, at::kByte, x);
   const Tensor sx = x_scale.contiguous(), sw = weight_scale.contiguous();
-  check(qrb200_int8_linear(xr.const_data_ptr<int8_t>(), xr.stride(0), sx.const_data_ptr<float>(), wr.const_data_ptr<int8_t>(),
-                           wr.stride(0), sw.const_data_ptr<float>(), ptr(bias), y.data_ptr(), rows, outs, depth,
-                           type_code(dtype), on.stream),
+  check(qrb200_int8_linear(xp, xr.stride(0), sx.const_data_ptr<float>(), wp, wr.stride(0), sw.const_data_ptr<float>(), ptr(bias),
+                           y.data_ptr(), rows, outs, depth, type_code(dtype), need > 0 ? ws.data_ptr() : nullptr, need, on.stream),
         "int8_linear");
   return y;
 }

@@ -55,17 +55,12 @@ static PFN_cuTensorMapEncodeTiled_v12000 map_encoder() {
   return fn;
 }
 
-struct I8Operand {
-  const int8_t* base;
-  uint64_t rows, stride;
-};
-
 // Boxes of 128 codes x `box_rows` rows, 128-byte swizzle; what lies outside the operand reads as zero.
 static bool encode_codes(CUtensorMap* map, const I8Operand& o, uint64_t depth, uint32_t box_rows) {
   const PFN_cuTensorMapEncodeTiled_v12000 fn = map_encoder();
   if (fn == nullptr) return false;
-  const cuuint64_t dims[2] = {depth, o.rows};
-  const cuuint64_t strides[1] = {o.rows > 1 ? o.stride : (depth + 15) / 16 * 16};
+  const cuuint64_t dims[2] = {depth, (cuuint64_t)o.rows};
+  const cuuint64_t strides[1] = {o.rows > 1 ? (cuuint64_t)o.stride : (depth + 15) / 16 * 16};
   const cuuint32_t box[2] = {(cuuint32_t)kI8Depth, box_rows};
   const cuuint32_t estr[2] = {1, 1};
   return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<int8_t*>(o.base), dims, strides, box, estr,
@@ -247,17 +242,35 @@ static I8Plan i8_plan(int64_t rows, int64_t outs, int64_t depth) {
 
 template <typename T>
 static cudaError_t launch_i8_rows(const I8Params& p, const I8Operand& x, const I8Operand& w, cudaStream_t s) {
-  const I8RowsParams r{p, x.base, w.base, (long long)x.stride, (long long)w.stride};
+  const I8RowsParams r{p, x, w};
   LaunchShape l(dim3(ceil_div(p.outs, 8)), 128, 0, s);
   if (p.rows == 1) return cudaLaunchKernelEx(&l.cfg, i8_rows_kernel<T, 1>, r);
   if (p.rows == 2) return cudaLaunchKernelEx(&l.cfg, i8_rows_kernel<T, 2>, r);
   return cudaLaunchKernelEx(&l.cfg, i8_rows_kernel<T, 4>, r);
 }
 
+// A warp walks its channels' whole depth, so a long one is left to the split of the tensor-core kernel.
+static bool i8_by_rows(int64_t rows, int64_t depth) { return rows <= 4 && depth <= 8192; }
+
+static I8Operand i8_operand(const int8_t* base, int64_t rows, int64_t stride) {
+  return {base, rows, stride, (reinterpret_cast<uintptr_t>(base) & 15u) == 0 && (rows == 1 || stride % 16 == 0)};
+}
+
 template <typename T>
-static cudaError_t launch_i8(const I8Params& p, const I8Operand& x, const I8Operand& w, cudaStream_t s) {
-  // A warp walks its channels' whole depth, so a long one is left to the split of the tensor-core kernel.
-  if (p.rows <= 4 && p.depth <= 8192) return launch_i8_rows<T>(p, x, w, s);
+static cudaError_t launch_i8(const I8Params& p, I8Operand x, I8Operand w, uint4* ws, cudaStream_t s) {
+  if (i8_by_rows(p.rows, p.depth)) return launch_i8_rows<T>(p, x, w, s);
+  if (!x.aligned || !w.aligned) {  // laid out anew in the workspace, x before w
+    const int packs = ceil_div(p.depth, 16);
+    uint4* to_x = x.aligned ? nullptr : ws;
+    uint4* to_w = w.aligned ? nullptr : ws + (x.aligned ? 0 : x.rows * packs);
+    const int64_t count = (to_x ? x.rows * packs : 0) + (to_w ? w.rows * packs : 0);
+    LaunchShape l(dim3(ceil_div(count, 256)), 256, 0, s);
+    const cudaError_t e = cudaLaunchKernelEx(&l.cfg, i8_pad_kernel, x, to_x, w, to_w, p.depth, packs);
+    if (e != cudaSuccess) return e;
+    qrb200_internal_count_launch();
+    if (to_x) x = {reinterpret_cast<const int8_t*>(to_x), x.rows, 16ll * packs, true};
+    if (to_w) w = {reinterpret_cast<const int8_t*>(to_w), w.rows, 16ll * packs, true};
+  }
   const I8Plan plan = i8_plan(p.rows, p.outs, p.depth);
   switch (plan.rows) {
     case 16: return launch_i8_few<T, 16>(p, x, w, plan.split, s);
@@ -422,27 +435,34 @@ int qrb200_dequantize_int8(const int8_t* q, int64_t q_stride, const float* scale
   return launch_dequant<float>(q, q_stride, scale, out, rows, cols, s);
 }
 
+size_t qrb200_int8_linear_workspace_bytes(const int8_t* x, int64_t x_stride, const int8_t* w, int64_t w_stride,
+                                          int64_t rows, int64_t outs, int64_t depth) {
+  if (rows <= 0 || outs <= 0 || depth <= 0 || depth > QRB200_INT8_MAX_DEPTH || i8_by_rows(rows, depth)) return 0;
+  const size_t pitch = (size_t)(depth + 15) / 16 * 16;
+  return (i8_operand(x, rows, x_stride).aligned ? 0 : rows * pitch) + (i8_operand(w, outs, w_stride).aligned ? 0 : outs * pitch);
+}
+
 int qrb200_int8_linear(const int8_t* x, int64_t x_stride, const float* x_scale, const int8_t* w, int64_t w_stride,
                        const float* w_scale, const void* bias, void* y, int64_t rows, int64_t outs, int64_t depth,
-                       int dtype, void* stream) {
+                       int dtype, void* workspace, size_t workspace_bytes, void* stream) {
   if (rows < 0 || outs < 0 || depth <= 0 || depth > QRB200_INT8_MAX_DEPTH || !type_ok(dtype)) return QRB200_ERR_ARG;
   if (rows > kMaxRows / 2 || outs > kMaxRows / 2) return QRB200_ERR_ARG;
   if (rows == 0 || outs == 0) return QRB200_OK;
-  if (!x || !w || !x_scale || !w_scale || !y) return QRB200_ERR_ARG;
+  if (!x || !w || !x_scale || !w_scale || !y || (reinterpret_cast<uintptr_t>(y) & 15u)) return QRB200_ERR_ARG;
   if ((rows > 1 && x_stride < depth) || (outs > 1 && w_stride < depth)) return QRB200_ERR_ARG;
-  const auto off16 = [](const void* p, int64_t stride, int64_t n) {
-    return (reinterpret_cast<uintptr_t>(p) & 15u) || (n > 1 && stride % 16);
-  };
-  if (off16(x, x_stride, rows) || off16(w, w_stride, outs) || off16(y, 0, 1)) return QRB200_ERR_ARG;
   const int st = quant_ready();
   if (st != QRB200_OK) return st;
+  const size_t need = qrb200_int8_linear_workspace_bytes(x, x_stride, w, w_stride, rows, outs, depth);
+  if (need > 0 && (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 255u)))
+    return QRB200_ERR_WORKSPACE;
   const I8Params p{x_scale, w_scale, bias, y, (int)rows, (int)outs, (int)depth, 0, 0};
-  const I8Operand xo{x, (uint64_t)rows, (uint64_t)x_stride}, wo{w, (uint64_t)outs, (uint64_t)w_stride};
+  const I8Operand xo = i8_operand(x, rows, x_stride), wo = i8_operand(w, outs, w_stride);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
+  uint4* ws = static_cast<uint4*>(workspace);
   cudaError_t e;
-  if (dtype == QRB200_BF16) e = launch_i8<__nv_bfloat16>(p, xo, wo, s);
-  else if (dtype == QRB200_F16) e = launch_i8<__half>(p, xo, wo, s);
-  else e = launch_i8<float>(p, xo, wo, s);
+  if (dtype == QRB200_BF16) e = launch_i8<__nv_bfloat16>(p, xo, wo, ws, s);
+  else if (dtype == QRB200_F16) e = launch_i8<__half>(p, xo, wo, ws, s);
+  else e = launch_i8<float>(p, xo, wo, ws, s);
   if (e != cudaSuccess) return QRB200_ERR_CUDA;
   return launched();
 }

@@ -40,12 +40,16 @@ def test_rows_entries_check_their_arguments(lib):
 
 def test_linear_entry_checks_its_arguments(lib):
     def linear(x=P, xs=16, sx=P, w=P, ws=16, sw=P, b=None, y=P, rows=2, outs=3, depth=16, dtype=1):
-        return lib.qrb200_int8_linear(x, xs, sx, w, ws, sw, b, y, rows, outs, depth, dtype, None)
+        return lib.qrb200_int8_linear(x, xs, sx, w, ws, sw, b, y, rows, outs, depth, dtype, None, 0, None)
 
     assert linear(rows=0) == OK and linear(outs=0) == OK
     assert linear(depth=0) == ARG and linear(depth=131072) == ARG and linear(dtype=7) == ARG
     assert linear(x=None) == ARG and linear(sw=None) == ARG and linear(y=None) == ARG
     assert linear(xs=15) == ARG and linear(ws=15) == ARG and linear(rows=-1) == ARG
+    need = lib.qrb200_int8_linear_workspace_bytes
+    assert need(P, 112, P, 112, 50, 70, 100) == 0  # rows on 16-byte boundaries
+    assert need(P, 100, P, 112, 50, 70, 100) == 50 * 112 and need(ctypes.c_void_p(257), 112, P, 100, 50, 70, 100) == 120 * 112
+    assert need(P, 100, P, 100, 4, 70, 100) == 0 and need(P, 100, P, 112, 0, 70, 100) == 0  # few rows are read as they lie
 
 
 def test_cache_entries_check_their_arguments(lib):
