@@ -9,8 +9,8 @@
 // Instructions bound it before the memory does, so the inner loop is kept short:
 // * a key's nibble needs one logical operation: left in place in an otherwise empty 16-bit number it is a subnormal (or
 //   the first normal binade, which continues them), worth code 2^-133 in bf16 and code 2^-24 in fp16, 16 times that four
-//   bits higher. The factors are powers of two: 1/16 goes to the queries of those channels, 2^64 to bf16 queries (whose
-//   products would otherwise be subnormal in 32 bits; |q| < 2^63 keeps them finite), the rest to the scores.
+//   bits higher. The factors are powers of two: 1/16 goes to the queries of those channels; each query row is brought
+//   by another to the top of its type's range, where neither it nor the products lose bits; the scores take both back.
 //   A value's nibble is placed under fp16's exponent of 1024 and brought to code - 8, which keeps sums over many tokens from cancelling.
 // * the weights p_t s_t are the only rounded operand: two fp16 numbers each, high and low, 22 bits in all (one alone
 //   would add an error the size of the result's own rounding). They are scaled by a power of two that puts the largest
@@ -83,16 +83,21 @@ __device__ __forceinline__ uint32_t kv_pair_fp16(uint32_t w, int p) {
   const __half2 r = __hsub2(reinterpret_cast<const __half2&>(x), __floats2half2_rn(1032.f, 1032.f));
   return reinterpret_cast<const uint32_t&>(r);
 }
+// Where a query row's largest entry is put (its exponent), and what its type makes of the code 1 (the negative exponent).
 template <typename T>
-struct KvKey;  // what queries are multiplied by, and what gives back q . c from the product with bare codes
+struct KvKey;
 template <>
 struct KvKey<__nv_bfloat16> {
-  static constexpr float kQuery = 0x1p64f, kBack = 0x1p69f;
+  static constexpr int kTop = 100, kOne = 133;
 };
 template <>
 struct KvKey<__half> {
-  static constexpr float kQuery = 1.f, kBack = 0x1p24f;
+  static constexpr int kTop = 13, kOne = 24;
 };
+__device__ __forceinline__ float kv_power(int e) { return __int_as_float((max(-126, min(127, e)) + 127) << 23); }
+// The power of two that brings a row whose largest entry has these bits (32-bit float, no sign) to kTop.
+template <typename T>
+__device__ __forceinline__ int kv_lift(unsigned top) { return min(120, KvKey<T>::kTop + 127 - (int)(top >> 23)); }
 
 __device__ __forceinline__ uint32_t kv_pack(float2 x) {
   const __half2 r = __float22half2_rn(x);
@@ -144,6 +149,9 @@ __device__ __forceinline__ void mbar_expect(uint32_t mbar, uint32_t bytes) {
 }
 
 constexpr int kKvStages = 3;
+// CTAs to an SM that registers are kept for. Four (128 registers) beat three wherever nothing spills (64 x 8192 tokens, one group:
+// 139 against 152 us); four groups of steps would (131 against 118 us).
+__host__ __device__ constexpr int kv_ctas(int groups, int nt) { return nt > 1 ? 2 : groups < 4 ? 4 : 3; }
 // Dynamic shared memory: the warps' rings, reused at the end for their parts of the output.
 __host__ __device__ constexpr int kv_stage_bytes(int dim, int groups) { return kv_runs(dim) * (16 * dim + 128 * groups); }
 __host__ __device__ constexpr int kv_smem_bytes(int dim, int groups, int nt) {
@@ -152,7 +160,7 @@ __host__ __device__ constexpr int kv_smem_bytes(int dim, int groups, int nt) {
 }
 
 template <typename T, int kDim, int kGroups, int kNT>
-__global__ void __launch_bounds__(32 * kKvWarps, kNT == 1 ? 4 : 2) kv4_attention_kernel(Kv4AttnParams P) {
+__global__ void __launch_bounds__(32 * kKvWarps, kv_ctas(kGroups, kNT)) kv4_attention_kernel(Kv4AttnParams P) {
   constexpr int kRows = 8 * kNT;           // query rows of a tile
   constexpr int kSteps = kDim / 16;        // 16-channel steps of q . k; also 16-channel tiles of the output
   constexpr int kPer = kSteps / kGroups;   // steps of a group
@@ -164,6 +172,7 @@ __global__ void __launch_bounds__(32 * kKvWarps, kNT == 1 ? 4 : 2) kv4_attention
   extern __shared__ __align__(128) unsigned char s_ring[];
   __shared__ uint2 s_q[kNT][kSteps][32];
   __shared__ float s_qsum[kKvWarps][kNT][8][kGroups];
+  __shared__ unsigned s_qtop[kKvWarps][kNT][8];
   __shared__ float2 s_ml[kKvWarps][kRows];
   __shared__ uint64_t s_full[kKvWarps][kKvStages];
   __shared__ int s_bad;
@@ -270,36 +279,54 @@ __global__ void __launch_bounds__(32 * kKvWarps, kNT == 1 ? 4 : 2) kv4_attention
   if (count > 0) look_up();
   for (int i = 0; i < kKvStages && i < count; ++i) issue(u + i, i);
 
-  // Queries as the right operand. The warps share the work.
+  // Queries as the right operand. The warps share the work; first each row's largest entry and each group's sum.
 #pragma unroll
   for (int n = 0; n < kNT; ++n) {
     float part[kGroups] = {};
+    unsigned top = 0;
 #pragma unroll
     for (int i = 0; i < kSteps / kKvWarps; ++i) {
       const int j = i * kKvWarps + warp;
-      T x[4];
       float add = 0.f;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const float v = to_f32(qv[n][i][e]);
-        x[e] = from_f32<T>(v * (e < 2 ? KvKey<T>::kQuery : KvKey<T>::kQuery / 16));
         add += v;
+        top = max(top, __float_as_uint(v) & 0x7fffffffu);
       }
-      s_q[n][j][lane] = *reinterpret_cast<uint2*>(x);
 #pragma unroll
       for (int gr = 0; gr < kGroups; ++gr) part[gr] += j / kPer == gr ? add : 0.f;
     }
 #pragma unroll
-    for (int gr = 0; gr < kGroups; ++gr) {
-      part[gr] += __shfl_xor_sync(kFullMask, part[gr], 1);
-      part[gr] += __shfl_xor_sync(kFullMask, part[gr], 2);
-      if (t == 0) s_qsum[warp][n][g][gr] = part[gr];
+    for (int x = 1; x <= 2; x <<= 1) {
+      top = max(top, __shfl_xor_sync(kFullMask, top, x));
+#pragma unroll
+      for (int gr = 0; gr < kGroups; ++gr) part[gr] += __shfl_xor_sync(kFullMask, part[gr], x);
+    }
+    if (t == 0) {
+      s_qtop[warp][n][g] = top;
+#pragma unroll
+      for (int gr = 0; gr < kGroups; ++gr) s_qsum[warp][n][g][gr] = part[gr];
     }
   }
   __syncthreads();
-  float2 qsum[kNT][kGroups];
+  const auto lift = [&](int n, int row) {
+    unsigned top = 0;
+    for (int w = 0; w < kKvWarps; ++w) top = max(top, s_qtop[w][n][row]);
+    return kv_lift<T>(top);
+  };
+  float2 qsum[kNT][kGroups], back[kNT];  // back: what gives q . c from the product with bare codes
 #pragma unroll
-  for (int n = 0; n < kNT; ++n)
+  for (int n = 0; n < kNT; ++n) {
+    const float up = kv_power(lift(n, g));
+#pragma unroll
+    for (int i = 0; i < kSteps / kKvWarps; ++i) {
+      alignas(8) T x[4];
+      put2(x, to_f32(qv[n][i][0]) * up, to_f32(qv[n][i][1]) * up);
+      put2(x + 2, to_f32(qv[n][i][2]) * (up / 16), to_f32(qv[n][i][3]) * (up / 16));
+      s_q[n][i * kKvWarps + warp][lane] = *reinterpret_cast<uint2*>(x);
+    }
+    back[n] = make_float2(kv_power(KvKey<T>::kOne - lift(n, 2 * t)), kv_power(KvKey<T>::kOne - lift(n, 2 * t + 1)));
 #pragma unroll
     for (int gr = 0; gr < kGroups; ++gr) {
       qsum[n][gr] = make_float2(0.f, 0.f);
@@ -308,6 +335,8 @@ __global__ void __launch_bounds__(32 * kKvWarps, kNT == 1 ? 4 : 2) kv4_attention
         qsum[n][gr].y += s_qsum[w][n][2 * t + 1][gr];
       }
     }
+  }
+  __syncthreads();
 
   float o[kNT][kSteps][4] = {};  // scaled by `unit`
   float2 sum[kNT] = {}, mids[kNT][kGroups] = {};
@@ -362,8 +391,8 @@ __global__ void __launch_bounds__(32 * kKvWarps, kNT == 1 ? 4 : 2) kv4_attention
                 *reinterpret_cast<const uint32_t*>(runs + i * kRunBytes + 16 * kDim + ((g + 8 * h) * kGroups + gr) * 4));
 #pragma unroll
             for (int n = 0; n < kNT; ++n) {
-              s[i][n][h].x = fmaf(k.x, acc[i][n][2 * h] * KvKey<T>::kBack, fmaf(k.y, qsum[n][gr].x, gr ? s[i][n][h].x : 0.f));
-              s[i][n][h].y = fmaf(k.x, acc[i][n][2 * h + 1] * KvKey<T>::kBack, fmaf(k.y, qsum[n][gr].y, gr ? s[i][n][h].y : 0.f));
+              s[i][n][h].x = fmaf(k.x, acc[i][n][2 * h] * back[n].x, fmaf(k.y, qsum[n][gr].x, gr ? s[i][n][h].x : 0.f));
+              s[i][n][h].y = fmaf(k.x, acc[i][n][2 * h + 1] * back[n].y, fmaf(k.y, qsum[n][gr].y, gr ? s[i][n][h].y : 0.f));
             }
           }
       }
@@ -538,7 +567,7 @@ __global__ void __launch_bounds__(32 * kKvWarps, kNT == 1 ? 4 : 2) kv4_attention
   __syncthreads();  // the rings are free
   float(*s_o)[kRows][kDim + 4] = reinterpret_cast<float(*)[kRows][kDim + 4]>(s_ring);
 
-  const float back = 1.f / unit;
+  const float lower = 1.f / unit;
   // The warps' parts: o[n][j][e] is channel 16 j + g + 8 (e / 2) of row 8 n + 2 t + e % 2.
 #pragma unroll
   for (int n = 0; n < kNT; ++n)
@@ -556,8 +585,8 @@ __global__ void __launch_bounds__(32 * kKvWarps, kNT == 1 ? 4 : 2) kv4_attention
       if (g == 0) s_ml[warp][8 * n + 2 * t + c] = make_float2(bound[n][c] - kKvLazy, l);
 #pragma unroll
       for (int j = 0; j < kSteps; ++j) {
-        s_o[warp][8 * n + 2 * t + c][16 * j + g] = fmaf(o[n][j][c], back, add[j / kPer]);
-        s_o[warp][8 * n + 2 * t + c][16 * j + g + 8] = fmaf(o[n][j][2 + c], back, add[j / kPer]);
+        s_o[warp][8 * n + 2 * t + c][16 * j + g] = fmaf(o[n][j][c], lower, add[j / kPer]);
+        s_o[warp][8 * n + 2 * t + c][16 * j + g + 8] = fmaf(o[n][j][2 + c], lower, add[j / kPer]);
       }
     }
   __syncthreads();
@@ -637,36 +666,45 @@ __global__ void __launch_bounds__(32 * kKvWarps, kNT == 1 ? 4 : 2) kv4_attention
   }
 }
 
-// One warp per query row: the splits' parts against their common maximum, in order.
+// One CTA per query row: the splits' parts against their common maximum, a warp every eighth, then the warps' sums in order.
+constexpr int kKvJoinWarps = 8;
 template <typename T, int kDim>
-__global__ void __launch_bounds__(128) kv4_join_kernel(Kv4AttnParams P, int tile_rows) {
+__global__ void __launch_bounds__(32 * kKvJoinWarps) kv4_join_kernel(Kv4AttnParams P, int tile_rows) {
+  __shared__ float s_x[kKvJoinWarps][kDim], s_l[kKvJoinWarps];
   griddep_launch_wait();
-  const int lane = threadIdx.x & 31, rows = P.queries * P.share;
-  const long long unit = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
-  if (unit >= (long long)P.batch * P.sh.heads * rows) return;
-  const int r = (int)(unit % rows), head = (int)(unit / rows % P.sh.heads), b = (int)(unit / rows / P.sh.heads);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rows = P.queries * P.share;
+  const int unit = blockIdx.x, r = unit % rows, head = unit / rows % P.sh.heads, b = unit / rows / P.sh.heads;
   const long long part =
       (((long long)b * P.sh.heads + head) * P.tiles + r / tile_rows) * P.splits * tile_rows + r % tile_rows;
   float m = -INFINITY, l = 0.f, x[kDim / 32] = {};
   for (int s = lane; s < P.splits; s += 32) m = fmaxf(m, P.part_ml[part + (long long)s * tile_rows].x);
   for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(kFullMask, m, o));
-#pragma unroll 4
-  for (int s = 0; s < P.splits; ++s) {
+#pragma unroll 8
+  for (int s = warp; s < P.splits; s += kKvJoinWarps) {
     const float2 ml = P.part_ml[part + (long long)s * tile_rows];
+    const float* o = P.part_o + (part + (long long)s * tile_rows) * kDim;
     const float f = kv_part_weight(ml, m);
     l = fmaf(f, ml.y, l);
-    const float* o = P.part_o + (part + (long long)s * tile_rows) * kDim;
 #pragma unroll
     for (int i = 0; i < kDim / 32; ++i) {
       const float v = o[32 * i + lane];
       x[i] = f == 0.f ? x[i] : fmaf(f, v, x[i]);
     }
   }
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  T* out = static_cast<T*>(P.out) +
-           (((long long)b * P.queries + r / P.share) * P.q_heads + head * P.share + r % P.share) * kDim;
 #pragma unroll
-  for (int i = 0; i < kDim / 32; ++i) out[32 * i + lane] = from_f32<T>(x[i] * inv);
+  for (int i = 0; i < kDim / 32; ++i) s_x[warp][32 * i + lane] = x[i];
+  if (lane == 0) s_l[warp] = l;
+  __syncthreads();
+  if (threadIdx.x >= kDim) return;
+  l = 0.f;
+  float y = 0.f;
+#pragma unroll
+  for (int w = 0; w < kKvJoinWarps; ++w) {
+    l += s_l[w];
+    y += s_x[w][threadIdx.x];
+  }
+  static_cast<T*>(P.out)[(((long long)b * P.queries + r / P.share) * P.q_heads + head * P.share + r % P.share) * kDim + threadIdx.x] =
+      from_f32<T>(l == 0.f ? 0.f : y * (1.f / l));
 }
 
 }  // namespace qrb200

@@ -332,10 +332,10 @@ struct AttnPlan {
   size_t bytes;  // workspace: the parts and their (maximum, sum) pairs
 };
 
-// Eight rows a tile where a key head has no more than eight query rows, else sixteen. The token range is cut so that the
-// SMs, which instructions keep busy, get even shares: the estimated time is the most CTAs on one SM x (steps of a warp + what
-// a CTA costs besides, about two steps), and for joining one more in a cluster, four through memory. The length is the table's
-// capacity or what a window leaves of it, all that the host knows.
+// Eight rows a tile where a key head has no more than eight query rows, else sixteen. The token range is cut over the CTAs that
+// make the least estimated time, in fifths of a step's share of a busy SM (0.63 us): a CTA alone takes 2.4 such shares for a
+// step (1.8 with sixteen rows), so up to that many share an SM for nothing, and its set-up takes two steps; joining costs 1.5 in
+// a cluster and 6 through memory. The length is the table's capacity or what a window leaves of it, all that the host knows.
 static AttnPlan attn_plan(const Kv4Shape& h, int64_t batch, int64_t queries, int64_t q_heads, int64_t max_pages, int64_t span) {
   AttnPlan p{};
   const int64_t rows = queries * (q_heads / h.heads);
@@ -344,8 +344,9 @@ static AttnPlan attn_plan(const Kv4Shape& h, int64_t batch, int64_t queries, int
   const int64_t ctas = batch * h.heads * p.tiles, unit = 16 * kv_runs(h.dim), sms = sm_count();
   const int64_t steps = std::max<int64_t>(1, (std::min(max_pages * h.page, span) + unit * kKvWarps - 1) / (unit * kKvWarps));
   int64_t best = -1;
-  for (int64_t n = 1; n <= std::min<int64_t>(steps, 64); ++n) {
-    const int64_t time = (ctas * n + sms - 1) / sms * ((steps + n - 1) / n + 2) + (n > kKvCluster ? 4 : n > 1 ? 1 : 0);
+  for (int64_t n = 1; n <= std::min<int64_t>(steps, 128); ++n) {
+    const int64_t share = std::max<int64_t>(p.tile_rows == 8 ? 12 : 9, 5 * ((ctas * n + sms - 1) / sms));
+    const int64_t time = share * ((steps + n - 1) / n + 2) + (n > kKvCluster ? 30 : n > 1 ? 8 : 0);
     if (best < 0 || time < best) {
       best = time;
       p.splits = (int)n;
@@ -374,7 +375,7 @@ static cudaError_t launch_attention(Kv4AttnParams p, const AttnPlan& plan, cudaS
                                             : launch_attention_tile<T, kDim, kGroups, 2>(p, plan, s);
   if (e != cudaSuccess || plan.splits <= kKvCluster) return e;
   qrb200_internal_count_launch();
-  LaunchShape j(dim3(ceil_div((int64_t)p.batch * p.queries * p.q_heads, 4)), 128, 0, s);
+  LaunchShape j(dim3(p.batch * p.queries * p.q_heads), 32 * kKvJoinWarps, 0, s);
   return cudaLaunchKernelEx(&j.cfg, kv4_join_kernel<T, kDim>, p, plan.tile_rows);
 }
 

@@ -450,6 +450,24 @@ def test_attention_weights_that_underflow_and_dominate():
     assert torch.equal(got[0, 0], values[:, 0])
 
 
+@pytest.mark.parametrize("dtype, size", [(HF, 2.0**-13), (HF, 2.0**10), (BF, 2.0**-100), (BF, 2.0**90)])
+def test_attention_queries_of_any_size(dtype, size):
+    """Small and large queries keep their bits: the scores only scale (a power of two, exactly)."""
+    q, cache, table, lengths = _case([150, 40], 2, 2, 3, 16, 128, 64, dtype)
+    q = q * 0.9  # an odd significand
+    wide = q * size
+    if dtype == HF:
+        wide[..., 5] = 0.75 * size  # small entries beside large ones
+        q = (wide.double() / size).to(HF)
+        assert torch.equal(q.double() * size, wide.double())
+    # the scale takes the size back, as far as 32 bits go
+    a = _check_attention(q, cache, table, lengths, scale=0.1)
+    if size < 2.0**40 and size > 2.0**-40:
+        _check_attention(wide, cache, table, lengths, scale=0.1 / size)
+    b = qr.kv4_attention(wide, cache, table, lengths, scale=0.1 / size)
+    assert torch.all((a.double() - b.double()).abs() <= 2 * U[dtype] * a.double().abs() + 2.0**-14)
+
+
 # ---- refusals -------------------------------------------------------------------------------
 
 
