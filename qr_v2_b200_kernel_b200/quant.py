@@ -90,13 +90,15 @@ def int8_linear(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor, we
 class KV4Cache:
     """A paged key/value cache in 4 bits (see :func:`kv4_cache`).
 
-    ``data``: uint8 (pages, kv_heads, bytes of a block), the whole state; a copy of it, made by any means, is a
-    copy of the cache. A token occupies head_dim + 8 head_dim / group_size bytes a head for its key and value.
+    ``data``: uint8 (pages, kv_heads, bytes of a block), the whole state, written in place; ``KV4Cache(data.clone(), ...)``
+    is a copy of the cache. A token occupies head_dim + 8 head_dim / group_size bytes a head for its key and value.
     """
 
     __slots__ = ("data", "pages", "page_size", "kv_heads", "head_dim", "group_size", "dtype", "_handle")
 
     def __init__(self, data: torch.Tensor, page_size: int, head_dim: int, group_size: int, dtype: torch.dtype):
+        if group_size < 1 or head_dim % group_size:
+            raise ValueError(f"group_size must divide head_dim, got {group_size} and {head_dim}")
         self.data, self.page_size, self.head_dim, self.group_size, self.dtype = data, page_size, head_dim, group_size, dtype
         self.pages, self.kv_heads = int(data.shape[0]), int(data.shape[1])
         self._handle = _native().Cache(data, page_size, head_dim, head_dim // group_size, dtype)

@@ -398,6 +398,14 @@ def test_attention_options(options):
     _check_attention(*_case([500, 0, 1], 1, 1, 4, 64, 128, 128, HF), **options)
 
 
+def test_attention_window_beyond_every_position():
+    args = _case([3, 40], 6, 1, 2, 16, 64, 32, BF)
+    for causal in (True, False):
+        want = _check_attention(*args, causal=causal)
+        for window in (54, 1 << 30, (1 << 31) - 1):
+            assert torch.equal(want, qr.kv4_attention(*args, causal=causal, window=window))
+
+
 @pytest.mark.parametrize("lengths, heads, share, dim", [([20000], 1, 8, 128), ([9001, 12345], 2, 1, 64), ([5000] * 3, 8, 8, 128)])
 def test_attention_over_long_contexts(lengths, heads, share, dim):
     args = _case(lengths, 1, heads, share, 64, dim, 64, BF)
@@ -495,6 +503,19 @@ def test_refusals():
         qr.rms_norm_int8(g)
     with torch.no_grad():
         qr.rms_norm_int8(g)
+
+
+def test_cache_from_bytes():
+    """A cache's bytes are its whole state; bytes that do not fit the layout are refused."""
+    q, cache, table, n = _case([20, 30], 1, 2, 2, 16, 64, 32, BF)
+    copy = qr.KV4Cache(cache.data.clone(), 16, 64, 32, BF)
+    assert torch.equal(qr.kv4_attention(q, cache, table, n), qr.kv4_attention(q, copy, table, n))
+    for bad in (lambda: qr.KV4Cache(cache.data[..., :-16], 16, 64, 32, BF), lambda: qr.KV4Cache(cache.data, 32, 64, 32, BF),
+                lambda: qr.KV4Cache(cache.data[0], 16, 64, 32, BF), lambda: qr.KV4Cache(cache.data, 16, 64, 24, BF)):
+        with pytest.raises(ValueError):
+            bad()
+    with pytest.raises(TypeError):
+        qr.KV4Cache(cache.data.int(), 16, 64, 32, BF)
 
 
 def test_cache_refusals():
