@@ -76,17 +76,18 @@ struct I8Operand {
   bool aligned;            // base and stride are multiples of 16
 };
 
-// Sixteen codes of a row from column k on, zeros past the row's end, from any address: neighbouring aligned words, shifted,
-// where those lie within the operand, else byte by byte.
+// Sixteen codes of a row from column k on, zeros past the row's end: one load from an aligned row; from any other address
+// neighbouring aligned words, shifted, where those lie within the operand; else byte by byte.
+template <bool kAligned>
 __device__ __forceinline__ uint4 i8_codes16(const I8Operand& o, long long row, int k, int depth) {
   const int8_t* p = o.base + row * o.stride + k;
   const int n = depth - k;
-  if (o.aligned && n >= 16) return __ldg(reinterpret_cast<const uint4*>(p));
+  if (kAligned && n >= 16) return __ldg(reinterpret_cast<const uint4*>(p));
   uint32_t w[4] = {};
   const uintptr_t at = reinterpret_cast<uintptr_t>(p);
   const uint32_t* word = reinterpret_cast<const uint32_t*>(at & ~(uintptr_t)3);
   const int8_t* end = o.base + (o.rows - 1) * o.stride + depth;
-  if (reinterpret_cast<const int8_t*>(word) >= o.base && reinterpret_cast<const int8_t*>(word + 5) <= end) {
+  if (!kAligned && reinterpret_cast<const int8_t*>(word) >= o.base && reinterpret_cast<const int8_t*>(word + 5) <= end) {
     const int shift = 8 * (int)(at & 3);
     uint32_t v[5];
 #pragma unroll
@@ -113,7 +114,7 @@ __global__ void __launch_bounds__(256) i8_pad_kernel(I8Operand a, uint4* to_a, I
   const I8Operand o = second ? b : a;
   uint4* to = second ? to_b : to_a;
   if (!to || at >= o.rows * packs) return;
-  to[at] = i8_codes16(o, at / packs, (int)(at % packs) * 16, depth);
+  to[at] = i8_codes16<false>(o, at / packs, (int)(at % packs) * 16, depth);
 }
 
 // ---- one to four rows ----------------------------------------------------------------------
@@ -126,29 +127,38 @@ struct I8RowsParams {
   I8Operand x, w;
 };
 
-template <typename T, int kM>
+template <typename T, int kM, bool kAligned>  // kM rows, or fewer of four
 __global__ void __launch_bounds__(128) i8_rows_kernel(I8RowsParams R) {
-  constexpr int kUnroll = 4;
+  constexpr int kUnroll = kM <= 2 ? 4 : 2;
   griddep_launch_wait();
   const I8Params& P = R.p;
   const int lane = threadIdx.x & 31, n = (blockIdx.x * 4 + (threadIdx.x >> 5)) * 2;
   if (n >= P.outs) return;
   const int n1 = min(n + 1, P.outs - 1);
+  const int8_t* w0 = R.w.base + n * R.w.stride;
+  const int8_t* w1 = R.w.base + n1 * R.w.stride;
   int acc[kM][2] = {};
   for (int k0 = 16 * lane; k0 < P.depth; k0 += 512 * kUnroll) {
     uint4 w[kUnroll][2], x[kUnroll][kM];
+    if (kAligned && k0 - 16 * lane + 512 * kUnroll <= P.depth) {  // all in range: every load is asked for at once
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      const int k = k0 + 512 * u;
-      if (k >= P.depth) {
-        w[u][0] = w[u][1] = make_uint4(0, 0, 0, 0);
-      } else {
-        w[u][0] = i8_codes16(R.w, n, k, P.depth);
-        w[u][1] = i8_codes16(R.w, n1, k, P.depth);
+      for (int u = 0; u < kUnroll; ++u) {
+        w[u][0] = __ldg(reinterpret_cast<const uint4*>(w0 + k0 + 512 * u));
+        w[u][1] = __ldg(reinterpret_cast<const uint4*>(w1 + k0 + 512 * u));
+#pragma unroll
+        for (int m = 0; m < kM; ++m)
+          x[u][m] = __ldg(reinterpret_cast<const uint4*>(R.x.base + (kM <= 2 ? m : min(m, P.rows - 1)) * R.x.stride + k0 + 512 * u));
       }
+    } else {
 #pragma unroll
-      for (int m = 0; m < kM; ++m)
-        x[u][m] = k < P.depth && m < P.rows ? i8_codes16(R.x, m, k, P.depth) : make_uint4(0, 0, 0, 0);
+      for (int u = 0; u < kUnroll; ++u) {
+        const int k = k0 + 512 * u;
+        const bool in = k < P.depth;
+        w[u][0] = in ? i8_codes16<kAligned>(R.w, n, k, P.depth) : make_uint4(0, 0, 0, 0);
+        w[u][1] = in ? i8_codes16<kAligned>(R.w, n1, k, P.depth) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int m = 0; m < kM; ++m) x[u][m] = in && m < P.rows ? i8_codes16<kAligned>(R.x, m, k, P.depth) : make_uint4(0, 0, 0, 0);
+      }
     }
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u)

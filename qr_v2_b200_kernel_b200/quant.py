@@ -81,7 +81,7 @@ def int8_linear(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor, we
     ``x`` int8 (..., depth) with a float32 scale for each row (token), ``weight`` int8 (outs, depth) with a
     float32 scale for each output channel, as :func:`rms_norm_int8` and :func:`quantize_int8` make them;
     ``bias`` (outs,) of ``dtype``. 1 <= depth <= 131071. The products are summed exactly, in 32-bit integers, and the
-    result is rounded once. Beyond four rows, operands whose rows do not start on 16-byte boundaries are laid out
+    result is rounded once. Beyond two rows, operands whose rows do not start on 16-byte boundaries are laid out
     anew first; those that the quantising functions return do.
     """
     return (_module or _native()).int8_linear(x, x_scale, weight, weight_scale, bias, dtype)
