@@ -137,11 +137,12 @@ static cudaError_t launch_rows_of(const RowsParams& p, cudaStream_t s) {
 }
 
 template <typename T, bool kNorm>
-static int launch_rows(const RowsParams& p, int weight_type, int dtype, cudaStream_t s) {
+static int launch_rows(RowsParams p, int weight_type, int dtype, cudaStream_t s) {
   constexpr int kVec = 16 / sizeof(T);
   const auto off = [](const void* q) { return (reinterpret_cast<uintptr_t>(q) & 15u) != 0; };
   const bool aligned = p.cols % kVec == 0 && !off(p.x) && !off(p.residual) && !off(p.weight) && !off(p.h_out) && !off(p.q) &&
                        p.x_stride % kVec == 0 && p.r_stride % kVec == 0 && p.q_stride % 16 == 0;
+  p.q_aligned = !off(p.q) && p.q_stride % 16 == 0;
   cudaError_t e;
   if (p.weight && weight_type == QRB200_F32 && dtype != QRB200_F32)
     e = aligned ? launch_rows_of<T, float, kNorm, true>(p, s) : launch_rows_of<T, float, kNorm, false>(p, s);
@@ -155,14 +156,16 @@ template <typename T>
 static int launch_dequant(const int8_t* q, int64_t q_stride, const float* scale, void* out, int64_t rows, int64_t cols,
                           cudaStream_t s) {
   // Sixteen codes to a thread where rows start on 16-byte boundaries on both sides, else eight, a warp's side by side.
-  const bool aligned = (cols * sizeof(T)) % 16 == 0 && q_stride % 16 == 0 &&
-                       ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) & 15u) == 0;
-  const int64_t units = aligned ? rows * ceil_div(cols, 16) : rows * ceil_div(cols, 256) * 32;
+  const bool packed = (cols * sizeof(T)) % 16 == 0 && q_stride % 16 == 0 &&
+                      ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) & 15u) == 0;
+  const int64_t units = packed ? rows * ceil_div(cols, 16) : rows * ceil_div(cols, 256) * 32;
   if (units > ((int64_t)1 << 38)) return QRB200_ERR_ARG;
   LaunchShape l(dim3(ceil_div(units, 256)), 256, 0, s);
-  const cudaError_t e =
-      cudaLaunchKernelEx(&l.cfg, !aligned ? dequant_rows_kernel<T, false, true> : cols % 16 ? dequant_rows_kernel<T, true, true> : dequant_rows_kernel<T, true, false>, q, (long long)q_stride,
-                         scale, static_cast<T*>(out), (long long)rows, (int)cols);
+  const auto kernel = !packed     ? dequant_rows_kernel<T, false, true>
+                      : cols % 16 ? dequant_rows_kernel<T, true, true>
+                                  : dequant_rows_kernel<T, true, false>;
+  const cudaError_t e = cudaLaunchKernelEx(
+      &l.cfg, kernel, q, (long long)q_stride, scale, static_cast<T*>(out), (long long)rows, (int)cols);
   if (e != cudaSuccess) return QRB200_ERR_CUDA;
   return launched();
 }
@@ -411,7 +414,7 @@ int qrb200_rms_norm_int8(const void* x, int64_t x_stride, const void* residual, 
   if (rows > 1 && (x_stride < cols || q_stride < cols || (residual && residual_stride < cols))) return QRB200_ERR_ARG;
   const int st = quant_ready();
   if (st != QRB200_OK) return st;
-  RowsParams p{x, residual, weight, h_out, q, scale, rows, x_stride, residual_stride, q_stride, (int)cols, eps};
+  RowsParams p{x, residual, weight, h_out, q, scale, rows, x_stride, residual_stride, q_stride, (int)cols, eps, 0};
   return rows_int8<true>(p, weight_type, dtype, static_cast<cudaStream_t>(stream));
 }
 
@@ -422,7 +425,7 @@ int qrb200_quantize_int8(const void* x, int64_t x_stride, int8_t* q, int64_t q_s
   if (!x || !q || !scale || (rows > 1 && (x_stride < cols || q_stride < cols))) return QRB200_ERR_ARG;
   const int st = quant_ready();
   if (st != QRB200_OK) return st;
-  RowsParams p{x, nullptr, nullptr, nullptr, q, scale, rows, x_stride, 0, q_stride, (int)cols, 0.f};
+  RowsParams p{x, nullptr, nullptr, nullptr, q, scale, rows, x_stride, 0, q_stride, (int)cols, 0.f, 0};
   return rows_int8<false>(p, dtype, dtype, static_cast<cudaStream_t>(stream));
 }
 

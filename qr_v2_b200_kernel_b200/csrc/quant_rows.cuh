@@ -49,27 +49,71 @@ struct RowsParams {
   long long rows, x_stride, r_stride, q_stride;
   int cols;
   float eps;
+  int q_aligned;  // rows of q start on 16-byte boundaries
 };
 
-// A pack is 16 bytes of consecutive elements: one load or store where all rows start on 16-byte boundaries and hold whole
-// packs (kAligned), else its `n` elements one by one.
+// A pack is 16 bytes of consecutive elements. Where all rows start on 16-byte boundaries and hold whole packs (kAligned) it is one
+// load or store. Elsewhere a load takes the two aligned blocks around it and shifts, if both lie within the operand ([lo, hi)),
+// else it goes element by element; elements from n on read as zero. A store goes by aligned pairs.
+struct Span {
+  const char* lo;
+  const char* hi;
+};
 template <bool kAligned, typename T, int kVec>
-__device__ __forceinline__ void load_pack(T (&v)[kVec], const T* p, int n) {
+__device__ __forceinline__ void load_pack(T (&v)[kVec], const T* p, int n, Span in) {
+  static_assert(kVec * sizeof(T) == 16, "a pack");
   if constexpr (kAligned) {
-#pragma unroll
-    for (int i = 0; i < kVec; i += 16 / sizeof(T))
-      *reinterpret_cast<uint4*>(v + i) = __ldg(reinterpret_cast<const uint4*>(p + i));
+    *reinterpret_cast<uint4*>(v) = __ldg(reinterpret_cast<const uint4*>(p));
   } else {
+    const uintptr_t at = reinterpret_cast<uintptr_t>(p);
+    const uint4* block = reinterpret_cast<const uint4*>(at & ~(uintptr_t)15);
+    const int off = (int)(at & 15);
+    if (reinterpret_cast<const char*>(block) >= in.lo && reinterpret_cast<const char*>(block + (off ? 2 : 1)) <= in.hi) {
+      uint32_t w[8] = {};
+      *reinterpret_cast<uint4*>(w) = __ldg(block);
+      if (off) *reinterpret_cast<uint4*>(w + 4) = __ldg(block + 1);
+      if (off & 8) {
 #pragma unroll
-    for (int i = 0; i < kVec; ++i) v[i] = i < n ? __ldg(p + i) : from_f32<T>(0.f);
+        for (int i = 0; i < 6; ++i) w[i] = w[i + 2];
+      }
+      if (off & 4) {
+#pragma unroll
+        for (int i = 0; i < 5; ++i) w[i] = w[i + 1];
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) reinterpret_cast<uint32_t*>(v)[i] = __funnelshift_r(w[i], w[i + 1], 8 * (off & 3));
+      if (n < kVec) {
+#pragma unroll
+        for (int i = 0; i < kVec; ++i)
+          if (i >= n) v[i] = from_f32<T>(0.f);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < kVec; ++i) v[i] = i < n ? __ldg(p + i) : from_f32<T>(0.f);
+    }
   }
 }
 template <bool kAligned, typename T, int kVec>
 __device__ __forceinline__ void store_pack(T* p, const T (&v)[kVec], int n) {
   if constexpr (kAligned) {
-#pragma unroll
-    for (int i = 0; i < kVec; i += 16 / sizeof(T)) *reinterpret_cast<uint4*>(p + i) = *reinterpret_cast<const uint4*>(v + i);
+    static_assert(kVec * sizeof(T) == 16, "a pack");
+    *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(v);
   } else {
+    if constexpr (sizeof(T) == 2) {
+      if (n >= kVec) {
+        const uint32_t* w = reinterpret_cast<const uint32_t*>(v);
+        if (reinterpret_cast<uintptr_t>(p) & 2) {  // the first and the last element stand alone
+          p[0] = v[0];
+#pragma unroll
+          for (int i = 0; i + 1 < kVec / 2; ++i) *reinterpret_cast<uint32_t*>(p + 2 * i + 1) = __funnelshift_r(w[i], w[i + 1], 16);
+          p[kVec - 1] = v[kVec - 1];
+        } else {
+#pragma unroll
+          for (int i = 0; i < kVec / 2; ++i) *reinterpret_cast<uint32_t*>(p + 2 * i) = w[i];
+        }
+        return;
+      }
+    }
 #pragma unroll
     for (int i = 0; i < kVec; ++i)
       if (i < n) p[i] = v[i];
@@ -77,7 +121,8 @@ __device__ __forceinline__ void store_pack(T* p, const T (&v)[kVec], int n) {
 }
 
 // A row lives in the registers of blockDim.x threads, kItems packs each, a block's y rows beside one another:
-// memory is read once and written once, and bounds it. Every load of the row is asked for before the first is used. Which
+// memory is read once and written once, and bounds it. (16384 x 4096 bf16: 79 us, 5.9 TB/s; rows off
+// 16-byte boundaries cost twice that, 16384 x 2047 65 us; storing those through shared memory, element beside element, lost, 74 us.) Every load of the row is asked for before the first is used. Which
 // thread holds which element depends on the row's length alone, so a row's result, bit for bit, depends on
 // neither its neighbours, their number nor anybody's alignment.
 template <typename T, typename W, bool kNorm, bool kAligned, int kItems>
@@ -92,14 +137,21 @@ __global__ void __launch_bounds__(1024) rows_int8_kernel(RowsParams P) {
   const T* x = static_cast<const T*>(P.x) + row * P.x_stride;
   const T* r = static_cast<const T*>(P.residual) + row * P.r_stride;
   const W* w = static_cast<const W*>(P.weight);
+  // The operands' extents, for loads off 16-byte boundaries.
+  const auto extent = [&](const void* base, long long stride) {
+    const char* lo = static_cast<const char*>(base);
+    return Span{lo, lo + ((P.rows - 1) * stride + P.cols) * (long long)sizeof(T)};
+  };
+  const Span xs = extent(P.x, P.x_stride), rs = extent(P.residual, P.r_stride);
+  const Span ws{static_cast<const char*>(P.weight), static_cast<const char*>(P.weight) + P.cols * sizeof(W)};
   alignas(16) T xv[kItems][kVec], rv[kItems][kVec];
   float t[kItems][kVec];
 #pragma unroll
   for (int i = 0; i < kItems; ++i) {
     const int c = tid + i * threads;
     if (!in || c >= packs) continue;
-    load_pack<kAligned>(xv[i], x + c * kVec, P.cols - c * kVec);
-    if (kNorm && P.residual) load_pack<kAligned>(rv[i], r + c * kVec, P.cols - c * kVec);
+    load_pack<kAligned>(xv[i], x + c * kVec, P.cols - c * kVec, xs);
+    if (kNorm && P.residual) load_pack<kAligned>(rv[i], r + c * kVec, P.cols - c * kVec, rs);
   }
   float sum = 0.f;
   unsigned top = 0;  // bits of the largest |t|: ordered as unsigned, with NaN above infinity
@@ -122,10 +174,14 @@ __global__ void __launch_bounds__(1024) rows_int8_kernel(RowsParams P) {
 #pragma unroll
       for (int e = 0; e < kVec; ++e) sum = fmaf(t[i][e], t[i][e], sum);
       if (w) {
-        W wv[kVec];
-        load_pack<kAligned>(wv, w + c * kVec, P.cols - c * kVec);
+        constexpr int kPart = 16 / sizeof(W);  // a 32-bit weight beside 16-bit rows takes two packs
 #pragma unroll
-        for (int e = 0; e < kVec; ++e) t[i][e] *= to_f32(wv[e]);
+        for (int h = 0; h < kVec; h += kPart) {
+          alignas(16) W wv[kPart];
+          load_pack<kAligned>(wv, w + c * kVec + h, P.cols - c * kVec - h, ws);
+#pragma unroll
+          for (int e = 0; e < kPart; ++e) t[i][h + e] *= to_f32(wv[e]);
+        }
       }
     }
 #pragma unroll
@@ -164,25 +220,24 @@ __global__ void __launch_bounds__(1024) rows_int8_kernel(RowsParams P) {
       const int code = finite ? __float2int_rn(__fmul_rn(t[i][e], inv)) : 0;
       word[e / 4] |= (uint32_t)(code & 255) << (8 * (e & 3));
     }
-    if constexpr (!kAligned) {
-      store_pack<false>(q + c * kVec, reinterpret_cast<const int8_t(&)[kVec]>(word), P.cols - c * kVec);
-    } else if constexpr (kVec == 8) {
-      *reinterpret_cast<uint2*>(q + c * 8) = make_uint2(word[0], word[1]);
+    if (kAligned || (P.q_aligned && (c + 1) * kVec <= P.cols)) {
+      if constexpr (kVec == 8) *reinterpret_cast<uint2*>(q + c * 8) = make_uint2(word[0], word[1]);
+      else *reinterpret_cast<uint32_t*>(q + c * 4) = word[0];
     } else {
-      *reinterpret_cast<uint32_t*>(q + c * 4) = word[0];
+      store_pack<false>(q + c * kVec, reinterpret_cast<const int8_t(&)[kVec]>(word), P.cols - c * kVec);
     }
   }
 }
 
-// value = code * scale of its row, rounded once: sixteen codes of a row to a thread, or (kAligned false) eight, 32 apart, with
-// a warp on 256 neighbouring ones. kTail: the last of a row are fewer.
-template <typename T, bool kAligned, bool kTail>
+// value = code * scale of its row, rounded once: sixteen codes of a row to a thread (kPacked: their rows start on 16-byte
+// boundaries, and the values'; kTail: the last of a row may be fewer), or eight, 32 apart, with a warp on 256 neighbouring ones.
+template <typename T, bool kPacked, bool kTail>
 __global__ void __launch_bounds__(256) dequant_rows_kernel(const int8_t* q, long long q_stride, const float* scale,
                                                            T* out, long long rows, int cols) {
-  constexpr int kSpan = kAligned ? 16 : 256;
+  constexpr int kSpan = kPacked ? 16 : 256;
   griddep_launch_wait();
   const int spans = (cols + kSpan - 1) / kSpan;
-  const long long at = ((long long)blockIdx.x * 256 + threadIdx.x) / (kAligned ? 1 : 32);
+  const long long at = ((long long)blockIdx.x * 256 + threadIdx.x) / (kPacked ? 1 : 32);
   // The division is in 32 bits where the index fits it.
   const long long row = at <= 0xffffffffll ? (long long)((uint32_t)at / (uint32_t)spans) : at / spans;
   if (row >= rows) return;
@@ -190,8 +245,8 @@ __global__ void __launch_bounds__(256) dequant_rows_kernel(const int8_t* q, long
   const float s = scale[row];
   q += row * q_stride + c;
   out += row * cols + c;
-  if constexpr (kAligned) {
-    const int n = kTail ? cols - c : 16;  // a multiple of a store's elements
+  if constexpr (kPacked) {
+    const int n = kTail ? cols - c : 16;
     uint32_t word[4] = {};
     if (n >= 16) {
       *reinterpret_cast<uint4*>(word) = __ldg(reinterpret_cast<const uint4*>(q));
@@ -212,7 +267,7 @@ __global__ void __launch_bounds__(256) dequant_rows_kernel(const int8_t* q, long
         };
         put2(&v[e], value(h + e), value(h + e + 1));
       }
-      if (h < n) store_pack<true>(out + h, v, kPart);
+      if (!kTail || h < n) store_pack<true>(out + h, v, kPart);  // n is a multiple of a pack
     }
   } else {
     const int lane = threadIdx.x & 31, n = cols - c;
