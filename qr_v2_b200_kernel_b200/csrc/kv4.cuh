@@ -148,12 +148,16 @@ __global__ void __launch_bounds__(2 * kDim) kv4_write_kernel(Kv4IoParams P) {
       const float inv = s >= 0x1p-126f ? __frcp_rn(s) : 0.f;
       // x - m is never negative. Added to 1.5 2^23, a number below 2^22 leaves its nearest whole number (ties to even) in
       // the low bits, above a constant that the packing takes off. Where s is normal, its rounding keeps every code below 15.5.
+      // (In a group that is not finite the codes come out as anything: they share no byte or word with another group's.)
       uint32_t code[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        float steps = __fmul_rn(__fsub_rn(to_f32(x[part][i]), m), inv);
-        if constexpr (std::is_same<T, __half>::value) steps = fminf(steps, 15.f);  // subnormal steps
-        code[i] = __float_as_uint(__fadd_rn(fine ? steps : 0.f, 0x1.8p23f));
+      for (int i = 0; i < 8; i += 2) {
+        float2 steps = __fadd2_rn(make_float2(to_f32(x[part][i]), to_f32(x[part][i + 1])), make_float2(-m, -m));
+        steps = __fmul2_rn(steps, make_float2(inv, inv));
+        if constexpr (std::is_same<T, __half>::value) steps = make_float2(fminf(steps.x, 15.f), fminf(steps.y, 15.f));  // subnormal steps
+        steps = __fadd2_rn(steps, make_float2(0x1.8p23f, 0x1.8p23f));
+        code[i] = __float_as_uint(steps.x);
+        code[i + 1] = __float_as_uint(steps.y);
       }
       constexpr uint32_t kBits = 0x4b400000u;
       if (part == 0) {
