@@ -47,8 +47,11 @@ struct Kv4AttnParams {
 
 constexpr int kKvWarps = 4;
 constexpr int kKvCluster = 8;  // the most CTAs that join their parts within a cluster (the portable size)
-// Runs of 16 tokens in a warp's step: as many as the registers hold beside the output (twice the channels, half the runs).
-__host__ __device__ constexpr int kv_runs(int dim) { return dim == 64 ? 4 : 2; }
+// Runs of 16 tokens in a warp's step: as many as the registers hold beside the output (twice the channels, half the runs). With 64
+// channels a warp that has no more than two such steps takes them in halves: its time is that of code running for the first
+// time, and there is half as much (12 x 2047 tokens, five drafts, window 1000: 12.2 against 10.0 us; 64 x 8192 tokens in
+// halves would take 63 against 56 us; with 128 channels halves lose, 6.8 against 6.4 us for one sequence of 513).
+__host__ __device__ constexpr int kv_runs(int dim, bool brief) { return dim == 64 && !brief ? 4 : 2; }
 
 template <typename T>
 __device__ __forceinline__ void kv_mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
@@ -153,20 +156,22 @@ constexpr int kKvStages = 3;
 // 139 against 152 us); four groups of steps would (131 against 118 us).
 __host__ __device__ constexpr int kv_ctas(int groups, int nt) { return nt > 1 ? 2 : groups < 4 ? 4 : 3; }
 // Dynamic shared memory: the warps' rings, reused at the end for their parts of the output.
-__host__ __device__ constexpr int kv_stage_bytes(int dim, int groups) { return kv_runs(dim) * (16 * dim + 128 * groups); }
-__host__ __device__ constexpr int kv_smem_bytes(int dim, int groups, int nt) {
-  const int ring = kKvWarps * kKvStages * kv_stage_bytes(dim, groups), parts = kKvWarps * 8 * nt * (dim + 4) * 4;
+__host__ __device__ constexpr int kv_stage_bytes(int dim, int groups, bool brief) {
+  return kv_runs(dim, brief) * (16 * dim + 128 * groups);
+}
+__host__ __device__ constexpr int kv_smem_bytes(int dim, int groups, int nt, bool brief) {
+  const int ring = kKvWarps * kKvStages * kv_stage_bytes(dim, groups, brief), parts = kKvWarps * 8 * nt * (dim + 4) * 4;
   return ring > parts ? ring : parts;
 }
 
-template <typename T, int kDim, int kGroups, int kNT>
+template <typename T, int kDim, int kGroups, int kNT, bool kBrief>
 __global__ void __launch_bounds__(32 * kKvWarps, kv_ctas(kGroups, kNT)) kv4_attention_kernel(Kv4AttnParams P) {
   constexpr int kRows = 8 * kNT;           // query rows of a tile
   constexpr int kSteps = kDim / 16;        // 16-channel steps of q . k; also 16-channel tiles of the output
   constexpr int kPer = kSteps / kGroups;   // steps of a group
   constexpr int kKW = kDim / 32;           // words of a lane's key codes, for one token
   constexpr int kVC = kDim / 64;           // 16-byte pieces of a lane's value codes, for 16 tokens
-  constexpr int kRuns = kv_runs(kDim), kUnit = 16 * kRuns;
+  constexpr int kRuns = kv_runs(kDim, kBrief), kUnit = 16 * kRuns;
   constexpr int kRunBytes = 16 * kDim + 128 * kGroups, kStage = kRuns * kRunBytes;
   constexpr float kNone = -INFINITY;
   extern __shared__ __align__(128) unsigned char s_ring[];

@@ -335,6 +335,7 @@ static cudaError_t launch_read(Kv4IoParams p, cudaStream_t s) {
 // How an attention call is cut: query rows per tile, and the token range over `splits` CTAs.
 struct AttnPlan {
   int tile_rows, tiles, splits;
+  bool brief;  // steps of half the size (kv_runs)
   size_t bytes;  // workspace: the parts and their (maximum, sum) pairs
 };
 
@@ -347,38 +348,48 @@ static AttnPlan attn_plan(const Kv4Shape& h, int64_t batch, int64_t queries, int
   const int64_t rows = queries * (q_heads / h.heads);
   p.tile_rows = rows <= 8 ? 8 : 16;
   p.tiles = ceil_div(rows, p.tile_rows);
-  const int64_t ctas = batch * h.heads * p.tiles, unit = 16 * kv_runs(h.dim), sms = sm_count();
-  const int64_t steps = std::max<int64_t>(1, (std::min(max_pages * h.page, span) + unit * kKvWarps - 1) / (unit * kKvWarps));
-  int64_t best = -1;
-  for (int64_t n = 1; n <= std::min<int64_t>(steps, 128); ++n) {
-    const int64_t share = std::max<int64_t>(p.tile_rows == 8 ? 12 : 9, 5 * ((ctas * n + sms - 1) / sms));
-    const int64_t time = share * ((steps + n - 1) / n + 2) + (n > kKvCluster ? 30 : n > 1 ? 8 : 0);
-    if (best < 0 || time < best) {
-      best = time;
-      p.splits = (int)n;
+  const int64_t ctas = batch * h.heads * p.tiles, tokens = std::min(max_pages * h.page, span), sms = sm_count();
+  const auto plan = [&](bool brief) {  // steps of a warp
+    const int64_t unit = 16 * kv_runs(h.dim, brief) * kKvWarps, steps = std::max<int64_t>(1, (tokens + unit - 1) / unit);
+    int64_t best = -1, left = 0;
+    for (int64_t n = 1; n <= std::min<int64_t>(steps, 128); ++n) {
+      const int64_t share = std::max<int64_t>(p.tile_rows == 8 ? 12 : 9, 5 * ((ctas * n + sms - 1) / sms));
+      const int64_t time = share * ((steps + n - 1) / n + 2) + (n > kKvCluster ? 30 : n > 1 ? 8 : 0);
+      if (best < 0 || time < best) {
+        best = time;
+        left = (steps + n - 1) / n;
+        p.splits = (int)n;
+      }
     }
-  }
+    return left;
+  };
+  p.brief = plan(false) <= 2 && h.dim == 64;
+  if (p.brief) plan(true);
   if (p.splits > kKvCluster) p.bytes = (size_t)(ctas * p.splits * p.tile_rows) * (h.dim * sizeof(float) + sizeof(float2));
   return p;
 }
 
-template <typename T, int kDim, int kGroups, int kNT>
+template <typename T, int kDim, int kGroups, int kNT, bool kBrief>
 static cudaError_t launch_attention_tile(const Kv4AttnParams& p, const AttnPlan& plan, cudaStream_t s) {
-  constexpr int kSmem = kv_smem_bytes(kDim, kGroups, kNT);
+  constexpr int kSmem = kv_smem_bytes(kDim, kGroups, kNT, kBrief);
   static OncePerDevice once;
   const cudaError_t e = once.run([] {
-    return cudaFuncSetAttribute(kv4_attention_kernel<T, kDim, kGroups, kNT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+    return cudaFuncSetAttribute(kv4_attention_kernel<T, kDim, kGroups, kNT, kBrief>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
   });
   if (e != cudaSuccess) return e;
   LaunchShape l(dim3(plan.splits, p.sh.heads * plan.tiles, p.batch), 32 * kKvWarps, kSmem, s);
   if (plan.splits > 1 && plan.splits <= kKvCluster) l.cluster(plan.splits, 1, 1);
-  return cudaLaunchKernelEx(&l.cfg, kv4_attention_kernel<T, kDim, kGroups, kNT>, p);
+  return cudaLaunchKernelEx(&l.cfg, kv4_attention_kernel<T, kDim, kGroups, kNT, kBrief>, p);
 }
 
 template <typename T, int kDim, int kGroups>
 static cudaError_t launch_attention(Kv4AttnParams p, const AttnPlan& plan, cudaStream_t s) {
-  const cudaError_t e = plan.tile_rows == 8 ? launch_attention_tile<T, kDim, kGroups, 1>(p, plan, s)
-                                            : launch_attention_tile<T, kDim, kGroups, 2>(p, plan, s);
+  const auto tile = [&](auto nt) {
+    if constexpr (kDim == 64)
+      if (plan.brief) return launch_attention_tile<T, kDim, kGroups, nt(), true>(p, plan, s);
+    return launch_attention_tile<T, kDim, kGroups, nt(), false>(p, plan, s);
+  };
+  const cudaError_t e = plan.tile_rows == 8 ? tile(Int<1>{}) : tile(Int<2>{});
   if (e != cudaSuccess || plan.splits <= kKvCluster) return e;
   qrb200_internal_count_launch();
   LaunchShape j(dim3(p.batch * p.queries * p.q_heads), 32 * kKvJoinWarps, 0, s);
