@@ -557,9 +557,25 @@ __global__ void __launch_bounds__(128 + 32 * kI8WideEpi, 1) __cluster_dims__(2, 
               *reinterpret_cast<uint4*>(y + (long long)(row0 + r) * P.outs + n0 + c0 + col) =
                   *reinterpret_cast<const uint4*>(mine + r * kI8Pitch + 16 * piece);
         } else {
-          for (int r = 0; r < 32 && row0 + r < P.rows; ++r)
-            for (int c = lane; c < min(kPer, left); c += 32)
-              y[(long long)(row0 + r) * P.outs + n0 + c0 + c] = reinterpret_cast<const T*>(mine + r * kI8Pitch)[c];
+          // Rows off 16-byte boundaries: a row's chunk by aligned pairs (16-bit results), or element beside element.
+          const int count = min(kPer, left);
+#pragma unroll 4
+          for (int r = 0; r < 32 && row0 + r < P.rows; ++r) {
+            const T* from = reinterpret_cast<const T*>(mine + r * kI8Pitch);
+            T* to = y + (long long)(row0 + r) * P.outs + n0 + c0;
+            if constexpr (sizeof(T) == 2) {
+              const int odd = (int)(reinterpret_cast<uintptr_t>(to) >> 1 & 1), c = 2 * lane + odd;
+              if (odd && lane == 0) to[0] = from[0];
+              if (c + 1 < count) {
+                alignas(4) const T two[2] = {from[c], from[c + 1]};
+                *reinterpret_cast<uint32_t*>(to + c) = *reinterpret_cast<const uint32_t*>(two);
+              } else if (c < count) {
+                to[c] = from[c];
+              }
+            } else if (lane < count) {
+              to[lane] = from[lane];
+            }
+          }
         }
       }
     }
