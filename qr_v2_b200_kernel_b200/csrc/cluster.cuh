@@ -1,4 +1,5 @@
-// Thread-block cluster helpers of the quantised operators: barrier, rank, loads from another CTA's shared memory.
+// Thread-block cluster helpers of the quantised operators: barrier, rank, loads from another CTA's
+// shared memory.
 #pragma once
 
 #include "tc.cuh"

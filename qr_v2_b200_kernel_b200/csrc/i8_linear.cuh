@@ -37,8 +37,8 @@ __device__ __forceinline__ void i8_expect(uint32_t mbar, uint32_t bytes) {
 __device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
 }
-// Descriptor of a K-major tile of 128-byte rows in the 128-byte swizzle (layout type 2): groups of 8 rows 1024 bytes
-// apart; a step of 32 codes advances the start address by 32 bytes.
+// Descriptor of a K-major tile of 128-byte rows in the 128-byte swizzle (layout type 2): groups of
+// 8 rows 1024 bytes apart; a step of 32 codes advances the start address by 32 bytes.
 __device__ __forceinline__ uint64_t i8_sdesc(uint32_t saddr) { return make_sdesc(saddr, 16, 1024) | ((uint64_t)2 << 61); }
 // kind::i8: signed 8-bit operands, both K-major, 32-bit integer accumulator.
 __host__ __device__ constexpr uint32_t i8_idesc(int M, int N) {
@@ -76,8 +76,9 @@ struct I8Operand {
   bool aligned;            // base and stride are multiples of 16
 };
 
-// Sixteen codes of a row from column k on, zeros past the row's end: one load from an aligned row; from any other address
-// neighbouring aligned words, shifted, where those lie within the operand; else byte by byte.
+// Sixteen codes of a row from column k on, zeros past the row's end: one load from an aligned row;
+// from any other address neighbouring aligned words, shifted, where those lie within the operand;
+// else byte by byte.
 template <bool kAligned>
 __device__ __forceinline__ uint4 i8_codes16(const I8Operand& o, long long row, int k, int depth) {
   const int8_t* p = o.base + row * o.stride + k;
@@ -119,9 +120,11 @@ __global__ void __launch_bounds__(256) i8_pad_kernel(I8Operand a, uint4* to_a, I
 
 // ---- one to four rows ----------------------------------------------------------------------
 //
-// The time is that of reading the weights once, and at these sizes mostly latency: no tiles, barriers or tensor memory, just
-// wide loads into four-way dot products, and operands as they lie. A warp takes two channels, a lane 16 codes of each 512; sums are joined by the
-// warp's integer reduction. (1 x 4096 x 4096: 6.6 us through the tensor cores, 3.2 us here, 5.2 TB/s of weights that L2 holds.)
+// The time is that of reading the weights once, and at these sizes mostly latency: no tiles,
+// barriers or tensor memory, just wide loads into four-way dot products, and operands as they lie.
+// A warp takes two channels, a lane 16 codes of each 512; sums are joined by the warp's integer
+// reduction. (1 x 4096 x 4096: 6.6 us through the tensor cores, 3.2 us here, 5.2 TB/s of weights
+// that L2 holds.)
 struct I8RowsParams {
   I8Params p;
   I8Operand x, w;
@@ -186,18 +189,18 @@ __global__ void __launch_bounds__(128) i8_rows_kernel(I8RowsParams R) {
 
 // ---- few rows ------------------------------------------------------------------------------
 //
-// With few rows the weights are the traffic, so they are the 128-row operand (M = output
-// channels) and the rows of x the narrow one (N = kBN): no tensor-core row is wasted on padding.
-// The depth is cut over the cluster's CTAs so that every SM streams weights; each CTA then adds all the CTAs' integer sums
-// of some rows of x, exactly, through distributed shared memory, in the one launch.
+// With few rows the weights are the traffic, so they are the 128-row operand (M = output channels)
+// and the rows of x the narrow one (N = kBN): no tensor-core row is wasted on padding. The depth is
+// cut over the cluster's CTAs so that every SM streams weights; each CTA then adds all the CTAs'
+// integer sums of some rows of x, exactly, through distributed shared memory, in the one launch.
 //
 // Warp 0 issues the loads, warp 1 the MMAs, warps 2-5 hold one output channel a lane.
 constexpr int kI8Split = 4;  // the most CTAs that share a tile's depth
 template <int kBN>
 struct I8Few {
   static constexpr int kStage = 128 * kI8Depth + kBN * kI8Depth;
-  // Loads in flight hide their latency: about 100 KB, which leaves room for the next kernel's set-up, or, for the largest
-  // tile, what one CTA can have.
+  // Loads in flight hide their latency: about 100 KB, which leaves room for the next kernel's
+  // set-up, or, for the largest tile, what one CTA can have.
   static constexpr int kStages = kBN <= 32 ? 6 : kBN == 64 ? 5 : 6;
   static constexpr int kCols = kBN < 32 ? 32 : kBN;  // TMEM columns
   static constexpr size_t smem() { return 1024 + (size_t)kStages * kStage; }
@@ -292,8 +295,8 @@ __global__ void __launch_bounds__(192) i8_few_kernel(I8Params P, const __grid_co
   }
   tc_fence_after();
   __syncthreads();
-  // The ring is free (every load has landed, every MMA is done): sums as [row][channel]. Row j is CTA j % split's to add and
-  // to write, a warp to a row.
+  // The ring is free (every load has landed, every MMA is done): sums as [row][channel]. Row j is
+  // CTA j % split's to add and to write, a warp to a row.
   int* sums = reinterpret_cast<int*>(ring);
   if (epi)
 #pragma unroll 1
@@ -353,8 +356,9 @@ __global__ void __launch_bounds__(192) i8_few_kernel(I8Params P, const __grid_co
 //
 // 256 rows x 256 channels per pair of CTAs (cta_group::2: each CTA holds 128 rows of x, 128 of the
 // channels' weights and its rows' 128 x 256 sums), persistent, with two accumulators in TMEM so
-// that a tile's epilogue runs under the next tile's products. Warp 0 loads its CTA's halves, warp
-// 1 of the pair's first CTA issues the MMAs, warps 4-11 scale, round and store, half of a tile's channels each four.
+// that a tile's epilogue runs under the next tile's products. Warp 0 loads its CTA's halves, warp 1
+// of the pair's first CTA issues the MMAs, warps 4-11 scale, round and store, half of a tile's
+// channels each four.
 constexpr int kI8WideStage = 2 * 128 * kI8Depth;  // bytes per CTA and stage
 constexpr int kI8WideStages = 5;
 constexpr int kI8WideEpi = 8;  // epilogue warps
@@ -428,7 +432,8 @@ __global__ void __launch_bounds__(128 + 32 * kI8WideEpi, 1) __cluster_dims__(2, 
   cluster_sync();  // both CTAs' barriers are initialised
   tc_fence_after();
   const uint32_t tmem = s_tmem;
-  // Tiles run down the rows within bands of kBand channel tiles, so that the tiles in flight share both operands in L2.
+  // Tiles run down the rows within bands of kBand channel tiles, so that the tiles in flight share
+  // both operands in L2.
   constexpr int kBand = 8;
   const int tiles_m = P.tiles / P.tiles_n;
   auto place = [&](int tile, int& m, int& n) {
@@ -493,7 +498,8 @@ __global__ void __launch_bounds__(128 + 32 * kI8WideEpi, 1) __cluster_dims__(2, 
     T* y = static_cast<T*>(P.y);
     int t = 0;
     bool bad = false;  // a wait ran out: keep to the barriers, touch nothing
-    // A tile's scales are asked for while the tile before it is scaled: a channel's to each thread, its own row's to each lane.
+    // A tile's scales are asked for while the tile before it is scaled: a channel's to each thread,
+    // its own row's to each lane.
     float next_sw = 0.f, next_b = 0.f, next_sx = 0.f;
     const auto ask = [&](int tile) {
       if (tile >= P.tiles) return;
@@ -557,7 +563,8 @@ __global__ void __launch_bounds__(128 + 32 * kI8WideEpi, 1) __cluster_dims__(2, 
               *reinterpret_cast<uint4*>(y + (long long)(row0 + r) * P.outs + n0 + c0 + col) =
                   *reinterpret_cast<const uint4*>(mine + r * kI8Pitch + 16 * piece);
         } else {
-          // Rows off 16-byte boundaries: a row's chunk by aligned pairs (16-bit results), or element beside element.
+          // Rows off 16-byte boundaries: a row's chunk by aligned pairs (16-bit results), or
+          // element beside element.
           const int count = min(kPer, left);
 #pragma unroll 4
           for (int r = 0; r < 32 && row0 + r < P.rows; ++r) {

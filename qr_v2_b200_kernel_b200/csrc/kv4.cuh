@@ -10,11 +10,12 @@
 //
 // Layout. One block per (page, head): P / 16 runs of 16 tokens, D channels, NG = D / G groups. A run is
 //   [key codes 8 D B][value codes 8 D B][key (s, m) 64 NG B][value (s, m) 64 NG B]
-// so that a run's loads share one address, and what is read together lies together (a multiple of 128 bytes).
-// The codes lie the way the 16 x 8 x 16 matrix instruction's left operand wants them, so that
-// the attention loads them straight into registers, 16 bytes at a time, and no shared memory or
-// transposition stands between the cache and the product. Lane (g, t) = (lane / 4, lane % 4) of
-// that operand holds rows g and g + 8, columns {2t, 2t+1, 2t+8, 2t+9}:
+// so that a run's loads share one address, and what is read together lies together (a multiple of
+// 128 bytes). The codes lie the way the 16 x 8 x 16 matrix instruction's left operand wants them,
+// so that what the attention copies into shared memory is already in the order of its registers,
+// 16 bytes at a time, with nothing to transpose or unpack on the way.
+// Lane (g, t) = (lane / 4, lane % 4) of that operand holds rows g and g + 8, columns
+// {2t, 2t+1, 2t+8, 2t+9}:
 //   keys: rows are tokens, columns channels (their order is free: queries are permuted alike).
 //     A token's D/2 bytes are four parts, one for each t; word w of a part holds the steps
 //     j = 2w, 2w + 1, channels 16 j + 4 t + e, e = 0..3, at nibble 2 (j & 1) + (e >> 1) + 4 (e & 1);
@@ -94,10 +95,11 @@ __device__ __forceinline__ unsigned char* kv4_run(const Kv4IoParams& P, long lon
   return P.cache + (page * P.sh.heads + head) * P.sh.block_bytes() + ((int)slot & (P.sh.page - 1)) / 16 * P.sh.run_bytes();
 }
 
-// Sixteen tokens to a CTA, kDim / 8 threads to a token, 8 channels (16 bytes) to a thread, head after head of P.span of them;
-// the next head's loads are under way while one is quantised. When the sixteen fill a run, as
-// prompts do, the run is put together in shared memory and stored whole; otherwise each thread stores its words (keys) and
-// bytes (values). Long prompts are bound by instructions: codes come out of the 32-bit floating sum's bits, packed as they lie.
+// Sixteen tokens to a CTA, kDim / 8 threads to a token, 8 channels (16 bytes) to a thread, head
+// after head of P.span of them; the next head's loads are under way while one is quantised. When
+// the sixteen fill a run, as prompts do, the run is put together in shared memory and stored whole;
+// otherwise each thread stores its words (keys) and bytes (values). Long prompts are bound by
+// instructions: codes come out of the 32-bit floating sum's bits, packed as they lie.
 template <typename T, int kDim, int kGroups, bool kVec>
 __global__ void __launch_bounds__(2 * kDim) kv4_write_kernel(Kv4IoParams P) {
   constexpr int kChunks = kDim / 8, kSpan = kChunks / kGroups;  // threads of a token, of a group
@@ -129,8 +131,8 @@ __global__ void __launch_bounds__(2 * kDim) kv4_write_kernel(Kv4IoParams P) {
   const auto quantise = [&](unsigned char* out, int at) {
 #pragma unroll
     for (int part = 0; part < 2; ++part) {
-      // The group's ends, exact in 16 bits: this thread's eight channels two at a time, then (lo, -hi) over the group's threads.
-      // NaN carries through; infinity shows at an end.
+      // The group's ends, exact in 16 bits: this thread's eight channels two at a time, then (lo,
+      // -hi) over the group's threads. NaN carries through; infinity shows at an end.
       typename Two<T>::type ends = kv4_ends(x[part]);
 #pragma unroll
       for (int o = kSpan >> 1; o; o >>= 1) {
@@ -146,22 +148,24 @@ __global__ void __launch_bounds__(2 * kDim) kv4_write_kernel(Kv4IoParams P) {
       pr.m = from_f32<T>(fine ? lo : nan);
       const float s = to_f32(pr.s), m = to_f32(pr.m);
       const float inv = s >= 0x1p-126f ? __frcp_rn(s) : 0.f;
-      // x - m is never negative. Added to 1.5 2^23, a number below 2^22 leaves its nearest whole number (ties to even) in
-      // the low bits, above a constant that the packing takes off. Where s is normal, its rounding keeps every code below 15.5.
-      // (In a group that is not finite the codes come out as anything: they share no byte or word with another group's.)
+      // x - m is never negative. Added to 1.5 2^23, a number below 2^22 leaves its nearest whole
+      // number (ties to even) in the low bits, above a constant that the packing takes off. Where s
+      // is normal, its rounding keeps every code below 15.5. (In a group that is not finite the
+      // codes come out as anything: they share no byte or word with another group's.)
       uint32_t code[8];
 #pragma unroll
-      for (int i = 0; i < 8; i += 2) {
-        float2 steps = __fadd2_rn(make_float2(to_f32(x[part][i]), to_f32(x[part][i + 1])), make_float2(-m, -m));
-        steps = __fmul2_rn(steps, make_float2(inv, inv));
-        if constexpr (std::is_same<T, __half>::value) steps = make_float2(fminf(steps.x, 15.f), fminf(steps.y, 15.f));  // subnormal steps
-        steps = __fadd2_rn(steps, make_float2(0x1.8p23f, 0x1.8p23f));
-        code[i] = __float_as_uint(steps.x);
-        code[i + 1] = __float_as_uint(steps.y);
+      for (int i = 0; i < 8; ++i) {
+        // Three roundings, never fused: (x - m) / s often lies midway between two codes, all being
+        // short numbers, and one rounding less would break such ties another way. (The paired forms
+        // of these operations are fused by the compiler.)
+        float steps = __fmul_rn(__fsub_rn(to_f32(x[part][i]), m), inv);
+        if constexpr (std::is_same<T, __half>::value) steps = fminf(steps, 15.f);  // subnormal s
+        code[i] = __float_as_uint(__fadd_rn(steps, 0x1.8p23f));
       }
       constexpr uint32_t kBits = 0x4b400000u;
       if (part == 0) {
-        // Step j = chunk / 2, t = 2 (chunk & 1) and the next; the other half of each word, step j ^ 1, is chunk ^ 2's.
+        // Step j = chunk / 2, t = 2 (chunk & 1) and the next; the other half of each word, step j ^
+        // 1, is chunk ^ 2's.
         const int up = (chunk & 2) ? 8 : 0;
         constexpr uint32_t kAll = kBits + (kBits << 16) + (kBits << 4) + (kBits << 20);
         const uint32_t a = (code[0] + (code[1] << 16) + (code[2] << 4) + (code[3] << 20) - kAll) << up;
@@ -170,7 +174,8 @@ __global__ void __launch_bounds__(2 * kDim) kv4_write_kernel(Kv4IoParams P) {
         const int t = 2 * (chunk & 1) + (up ? 1 : 0);
         if (out) *reinterpret_cast<uint32_t*>(out + at * (kDim / 2) + t * (kDim / 8) + (chunk >> 2) * 4) = word;
       } else {
-        // Tile chunk / 2; an even chunk has the low nibbles of its 8 bytes, its odd neighbour the high ones.
+        // Tile chunk / 2; an even chunk has the low nibbles of its 8 bytes, its odd neighbour the
+        // high ones.
         const bool odd = chunk & 1;
         constexpr uint32_t kAll = kBits + (kBits << 8) + (kBits << 16) + (kBits << 24);
         const uint32_t a = code[0] + (code[1] << 8) + (code[2] << 16) + (code[3] << 24) - kAll;
@@ -209,7 +214,8 @@ __global__ void __launch_bounds__(2 * kDim) kv4_write_kernel(Kv4IoParams P) {
   }
 }
 
-// The values at slots, as kv4_write_kernel cuts them; a negative slot reads as zeros. A whole run goes through shared memory.
+// The values at slots, as kv4_write_kernel cuts them; a negative slot reads as zeros. A whole run
+// goes through shared memory.
 template <typename T, int kDim, int kGroups>
 __global__ void __launch_bounds__(2 * kDim) kv4_read_kernel(Kv4IoParams P) {
   constexpr int kChunks = kDim / 8, kSpan = kChunks / kGroups;  // threads of a token, of a group

@@ -2,25 +2,30 @@
 //
 // With m_t and s_t a token's minimum and step, c_t its codes:
 //   q . k_t = sum_groups s_t (q . c_t) + m_t sum(q),     o = sum_t (p_t s_t) c_t + sum_t p_t m_t.
-// So the codes themselves are the matrix operands, exact in 16 bits: no key or value is ever rounded, steps
-// and minima are applied in 32 bits. Keys (and values transposed) are the 16-row left operand, 8 query rows that
-// share the key head the right one, so a head with few query rows wastes little of the matrix instruction.
+// So the codes themselves are the matrix operands, exact in 16 bits: no key or value is ever
+// rounded, steps and minima are applied in 32 bits. Keys (and values transposed) are the 16-row
+// left operand, 8 query rows that share the key head the right one, so a head with few query rows
+// wastes little of the matrix instruction.
 //
 // Instructions bound it before the memory does, so the inner loop is kept short:
-// * a key's nibble needs one logical operation: left in place in an otherwise empty 16-bit number it is a subnormal (or
-//   the first normal binade, which continues them), worth code 2^-133 in bf16 and code 2^-24 in fp16, 16 times that four
-//   bits higher. The factors are powers of two: 1/16 goes to the queries of those channels; each query row is brought
-//   by another to the top of its type's range, where neither it nor the products lose bits; the scores take both back.
-//   A value's nibble is placed under fp16's exponent of 1024 and brought to code - 8, which keeps sums over many tokens from cancelling.
-// * the weights p_t s_t are the only rounded operand: two fp16 numbers each, high and low, 22 bits in all (one alone
-//   would add an error the size of the result's own rounding). They are scaled by a power of two that puts the largest
-//   step near 2^11, so that a weight keeps its leading bits down to 2^-25 of the largest.
-// * the running maximum and that scale move only when a score exceeds the reference by 2^4 or a step its bound, so
-//   that the output is rarely rescaled and the warp rarely reduces.
-// Each warp walks its own stretch of tokens, a step of 32 or 64 at a time, through a ring of three steps in shared memory
-// that bulk asynchronous copies fill: a run's bytes are already in the order of the operand's registers.
-// The token range is cut over CTAs (blockIdx.x) and over a CTA's four warps; the parts are joined through shared memory and,
-// between CTAs, through the cluster's shared memory (up to eight) or by kv4_join_kernel, always in a fixed order.
+// * a key's nibble needs one logical operation: left in place in an otherwise empty 16-bit number
+//   it is a subnormal (or the first normal binade, which continues them), worth code 2^-133 in bf16
+//   and code 2^-24 in fp16, 16 times that four bits higher. The factors are powers of two: 1/16
+//   goes to the queries of those channels; each query row is brought by another to the top of its
+//   type's range, where neither it nor the products lose bits; the scores take both back. A value's
+//   nibble is placed under fp16's exponent of 1024 and brought to code - 8, which keeps sums over
+//   many tokens from cancelling.
+// * the weights p_t s_t are the only rounded operand: two fp16 numbers each, high and low, 22 bits
+//   in all (one alone would add an error the size of the result's own rounding). They are scaled by
+//   a power of two that puts the largest step near 2^11, so that a weight keeps its leading bits
+//   down to 2^-25 of the largest.
+// * the running maximum and that scale move only when a score exceeds the reference by 2^4 or a
+//   step its bound, so that the output is rarely rescaled and the warp rarely reduces.
+// Each warp walks its own stretch of tokens, a step of 32 or 64 at a time, through a ring of three
+// steps in shared memory that bulk asynchronous copies fill: a run's bytes are already in the order
+// of the operand's registers. The token range is cut over CTAs (blockIdx.x) and over a CTA's four
+// warps; the parts are joined through shared memory and, between CTAs, through the cluster's shared
+// memory (up to eight) or by kv4_join_kernel, always in a fixed order.
 #pragma once
 
 #include <type_traits>
@@ -47,10 +52,12 @@ struct Kv4AttnParams {
 
 constexpr int kKvWarps = 4;
 constexpr int kKvCluster = 8;  // the most CTAs that join their parts within a cluster (the portable size)
-// Runs of 16 tokens in a warp's step: as many as the registers hold beside the output (twice the channels, half the runs). With 64
-// channels a warp that has no more than two such steps takes them in halves: its time is that of code running for the first
-// time, and there is half as much (12 x 2047 tokens, five drafts, window 1000: 12.2 against 10.0 us; 64 x 8192 tokens in
-// halves would take 63 against 56 us; with 128 channels halves lose, 6.8 against 6.4 us for one sequence of 513).
+// Runs of 16 tokens in a warp's step: as many as the registers hold beside the output (twice the
+// channels, half the runs). With 64 channels a warp that has no more than two such steps takes them
+// in halves: its time is that of code running for the first time, and there is half as much (12 x
+// 2047 tokens, five drafts, window 1000: 12.2 against 10.0 us; 64 x 8192 tokens in halves would
+// take 63 against 56 us; with 128 channels halves lose, 6.8 against 6.4 us for one sequence of
+// 513).
 __host__ __device__ constexpr int kv_runs(int dim, bool brief) { return dim == 64 && !brief ? 4 : 2; }
 
 template <typename T>
@@ -68,8 +75,8 @@ __device__ __forceinline__ void kv_mma<__half>(float (&d)[4], const uint32_t (&a
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// Nibbles p and p + 4 of w as a pair of 16-bit numbers: bare (the integer code, times 16 for odd p, as a subnormal
-// of either 16-bit type), and as code - 8 in fp16.
+// Nibbles p and p + 4 of w as a pair of 16-bit numbers: bare (the integer code, times 16 for odd p,
+// as a subnormal of either 16-bit type), and as code - 8 in fp16.
 __device__ __forceinline__ uint32_t kv_pair_bare(uint32_t w, int p) {
   if (p & 2) w >>= 8;
   return w & (p & 1 ? 0x00f000f0u : 0x000f000fu);
@@ -86,7 +93,8 @@ __device__ __forceinline__ uint32_t kv_pair_fp16(uint32_t w, int p) {
   const __half2 r = __hsub2(reinterpret_cast<const __half2&>(x), __floats2half2_rn(1032.f, 1032.f));
   return reinterpret_cast<const uint32_t&>(r);
 }
-// Where a query row's largest entry is put (its exponent), and what its type makes of the code 1 (the negative exponent).
+// Where a query row's largest entry is put (its exponent), and what its type makes of the code 1
+// (the negative exponent).
 template <typename T>
 struct KvKey;
 template <>
@@ -98,7 +106,8 @@ struct KvKey<__half> {
   static constexpr int kTop = 13, kOne = 24;
 };
 __device__ __forceinline__ float kv_power(int e) { return __int_as_float((max(-126, min(127, e)) + 127) << 23); }
-// The power of two that brings a row whose largest entry has these bits (32-bit float, no sign) to kTop.
+// The power of two that brings a row whose largest entry has these bits (32-bit float, no sign) to
+// kTop.
 template <typename T>
 __device__ __forceinline__ int kv_lift(unsigned top) { return min(120, KvKey<T>::kTop + 127 - (int)(top >> 23)); }
 
@@ -116,8 +125,8 @@ __device__ __forceinline__ float kv_exp2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
-// What a part with this (maximum, sum) counts against the maximum m of all: nothing where it saw nothing, NaN where its
-// scores were.
+// What a part with this (maximum, sum) counts against the maximum m of all: nothing where it saw
+// nothing, NaN where its scores were.
 __device__ __forceinline__ float kv_part_weight(float2 ml, float m) {
   return ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : ml.y) : kv_exp2(ml.x - m);
 }
@@ -152,8 +161,9 @@ __device__ __forceinline__ void mbar_expect(uint32_t mbar, uint32_t bytes) {
 }
 
 constexpr int kKvStages = 3;
-// CTAs to an SM that registers are kept for. Four (128 registers) beat three wherever nothing spills (64 x 8192 tokens, one group:
-// 139 against 152 us); four groups of steps would (131 against 118 us).
+// CTAs to an SM that registers are kept for. Four (128 registers) beat three wherever nothing
+// spills (64 x 8192 tokens, one group: 139 against 152 us); four groups of steps would (131 against
+// 118 us).
 __host__ __device__ constexpr int kv_ctas(int groups, int nt) { return nt > 1 ? 2 : groups < 4 ? 4 : 3; }
 // Dynamic shared memory: the warps' rings, reused at the end for their parts of the output.
 __host__ __device__ constexpr int kv_stage_bytes(int dim, int groups, bool brief) {
@@ -195,7 +205,8 @@ __global__ void __launch_bounds__(32 * kKvWarps, kv_ctas(kGroups, kNT)) kv4_atte
   __syncwarp();
   griddep_launch_wait();
   int len = P.lengths[b];
-  // The queries, asked for before anything waits: step j wants channels 16 j + 4 t + {0, 1} and {2, 3} of row g.
+  // The queries, asked for before anything waits: step j wants channels 16 j + 4 t + {0, 1} and {2,
+  // 3} of row g.
   T qv[kNT][kSteps / kKvWarps][4];
 #pragma unroll
   for (int n = 0; n < kNT; ++n) {
@@ -237,7 +248,8 @@ __global__ void __launch_bounds__(32 * kKvWarps, kv_ctas(kGroups, kNT)) kv4_atte
   int u = min(cta_hi, cta_lo + warp * per_warp);
   const int u_hi = min(cta_hi, u + per_warp);
 
-  // The ring. Lane i of `page` holds the page of run `page_base` + i, -1 past the range or where the table is wrong.
+  // The ring. Lane i of `page` holds the page of run `page_base` + i, -1 past the range or where
+  // the table is wrong.
   unsigned char* ring = s_ring + warp * (kKvStages * kStage);
   const int page_runs = P.sh.page / 16, page_shift = P.sh.shift - 4;
   const int last_run = min(u_hi * kRuns, (len + 15) / 16);
@@ -284,7 +296,8 @@ __global__ void __launch_bounds__(32 * kKvWarps, kv_ctas(kGroups, kNT)) kv4_atte
   if (count > 0) look_up();
   for (int i = 0; i < kKvStages && i < count; ++i) issue(u + i, i);
 
-  // Queries as the right operand. The warps share the work; first each row's largest entry and each group's sum.
+  // Queries as the right operand. The warps share the work; first each row's largest entry and each
+  // group's sum.
 #pragma unroll
   for (int n = 0; n < kNT; ++n) {
     float part[kGroups] = {};
@@ -345,7 +358,8 @@ __global__ void __launch_bounds__(32 * kKvWarps, kv_ctas(kGroups, kNT)) kv4_atte
 
   float o[kNT][kSteps][4] = {};  // scaled by `unit`
   float2 sum[kNT] = {}, mids[kNT][kGroups] = {};
-  // Weights are 2^(score scale2 + less); bound is where a score moves that reference. cap bounds the steps, unit scales them.
+  // Weights are 2^(score scale2 + less); bound is where a score moves that reference. cap bounds
+  // the steps, unit scales them.
   float2 less[kNT] = {};
   float bound[kNT][2], cap = 0.f, unit = 1.f;
 #pragma unroll
@@ -359,7 +373,8 @@ __global__ void __launch_bounds__(32 * kKvWarps, kv_ctas(kGroups, kNT)) kv4_atte
     const unsigned gone = missing >> (8 * stage) & ((1u << kRuns) - 1);
     ok = ok && __all_sync(kFullMask, mbar_wait(&s_full[warp][stage], turn));
     if (!ok) break;
-    // Scores before scaling: s[i][n][h] holds token tok0 + 16 i + 8 h + g against rows 8 n + 2 t and the next.
+    // Scores before scaling: s[i][n][h] holds token tok0 + 16 i + 8 h + g against rows 8 n + 2 t
+    // and the next.
     float2 s[kRuns][kNT][2];
     {
       float acc[kRuns][kNT][4];
@@ -488,7 +503,8 @@ __global__ void __launch_bounds__(32 * kKvWarps, kv_ctas(kGroups, kNT)) kv4_atte
           const float last = bound[n][c] - kKvLazy, next = fmaxf(up[n][c], last);
           keep[c] = next == kNone ? 0.f : kv_exp2(last - next);
           bound[n][c] = next + kKvLazy;
-          // A row that has seen nothing has the reference -inf: its weights, 2^-inf, come from any finite one.
+          // A row that has seen nothing has the reference -inf: its weights, 2^-inf, come from any
+          // finite one.
           (c ? less[n].y : less[n].x) = next == kNone ? 0.f : -next;
         }
         sum[n] = make_float2(sum[n].x * keep[0], sum[n].y * keep[1]);
@@ -565,7 +581,8 @@ __global__ void __launch_bounds__(32 * kKvWarps, kv_ctas(kGroups, kNT)) kv4_atte
     }
   }
   if (!ok) {
-    // A copy did not arrive in time: nothing is written, and what is under way is waited for (with a limit) first.
+    // A copy did not arrive in time: nothing is written, and what is under way is waited for (with
+    // a limit) first.
     for (int i = 0; i < kKvStages; ++i) mbar_wait(&s_full[warp][i], i < stage ? turn ^ 1 : turn);
     s_bad = 1;
   }
@@ -620,7 +637,8 @@ __global__ void __launch_bounds__(32 * kKvWarps, kv_ctas(kGroups, kNT)) kv4_atte
     if (row0 + r < rows && !s_bad)
       for (int d = d0; d < kDim; d += kLanesRow) out_row(r)[d] = from_f32<T>(joined(d) * inv);
   } else if (P.splits <= kKvCluster) {
-    // The CTA's part takes its first warp's place; each CTA then joins every splits-th row of all of them.
+    // The CTA's part takes its first warp's place; each CTA then joins every splits-th row of all
+    // of them.
     for (int d = d0; d < kDim; d += kLanesRow) s_o[0][r][d] = joined(d);
     __syncthreads();  // every warp's (maximum, sum) has been read
     if (d0 == 0) s_ml[0][r] = make_float2(m, l);
@@ -671,7 +689,8 @@ __global__ void __launch_bounds__(32 * kKvWarps, kv_ctas(kGroups, kNT)) kv4_atte
   }
 }
 
-// One CTA per query row: the splits' parts against their common maximum, a warp every eighth, then the warps' sums in order.
+// One CTA per query row: the splits' parts against their common maximum, a warp every eighth, then
+// the warps' sums in order.
 constexpr int kKvJoinWarps = 8;
 template <typename T, int kDim>
 __global__ void __launch_bounds__(32 * kKvJoinWarps) kv4_join_kernel(Kv4AttnParams P, int tile_rows) {

@@ -117,8 +117,9 @@ static int sm_count() {
 
 static int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 
-// Packs of a row to a thread, by the row's length: four (enough loads in flight, few threads at the two reductions), fewer
-// where that would leave a warp idle. Short rows go several to a block, a warp each, where there are rows enough.
+// Packs of a row to a thread, by the row's length: four (enough loads in flight, few threads at the
+// two reductions), fewer where that would leave a warp idle. Short rows go several to a block, a
+// warp each, where there are rows enough.
 template <typename T, typename W, bool kNorm, bool kAligned>
 static cudaError_t launch_rows_of(const RowsParams& p, cudaStream_t s) {
   const int packs = ceil_div(p.cols, 16 / sizeof(T));
@@ -155,7 +156,8 @@ static int launch_rows(RowsParams p, int weight_type, int dtype, cudaStream_t s)
 template <typename T>
 static int launch_dequant(const int8_t* q, int64_t q_stride, const float* scale, void* out, int64_t rows, int64_t cols,
                           cudaStream_t s) {
-  // Sixteen codes to a thread where rows start on 16-byte boundaries on both sides, else eight, a warp's side by side.
+  // Sixteen codes to a thread where rows start on 16-byte boundaries on both sides, else eight, a
+  // warp's side by side.
   const bool packed = (cols * sizeof(T)) % 16 == 0 && q_stride % 16 == 0 &&
                       ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) & 15u) == 0;
   const int64_t units = packed ? rows * ceil_div(cols, 16) : rows * ceil_div(cols, 256) * 32;
@@ -215,9 +217,11 @@ static cudaError_t launch_i8_wide(I8Params p, const I8Operand& x, const I8Operan
   return cudaLaunchKernelEx(&l.cfg, i8_wide_kernel<T>, p, tx, tw);
 }
 
-// Which kernel, with how many rows a tile (`rows`) and over how many CTAs of the depth: the least of the estimated clocks. A CTA
-// takes in its stages at about 40 bytes a clock; joining a split costs two cluster barriers (about 1500 clocks) and reading
-// the sums at about 16 bytes a clock. Clusters of eight lose: a GPC holds two at best (64 x 1000 x 2048: 12 us against 9). The wide kernel's pair takes 512 clocks a stage and a tile's last epilogue is bare.
+// Which kernel, with how many rows a tile (`rows`) and over how many CTAs of the depth: the least
+// of the estimated clocks. A CTA takes in its stages at about 40 bytes a clock; joining a split
+// costs two cluster barriers (about 1500 clocks) and reading the sums at about 16 bytes a clock.
+// Clusters of eight lose: a GPC holds two at best (64 x 1000 x 2048: 12 us against 9). The wide
+// kernel's pair takes 512 clocks a stage and a tile's last epilogue is bare.
 struct I8Plan {
   int rows;  // 16, 32, 64 or 128 (few), 256 (wide)
   unsigned split;
@@ -253,9 +257,10 @@ static cudaError_t launch_i8_rows(const I8Params& p, const I8Operand& x, const I
   return cudaLaunchKernelEx(&l.cfg, i8_rows_kernel<T, 4, true>, r);  // never unaligned
 }
 
-// Up to four rows by dot products (4096 x 4096: 3.2 us for one or two, 4.5 for four, against 5.7 in tiles); three or four off
-// 16-byte boundaries are better laid out first (3 x 1641 x 1329: 6.6 against 8.4). A warp walks its channels' whole depth, so a long
-// one is left to the split of the tensor-core kernel.
+// Up to four rows by dot products (4096 x 4096: 3.2 us for one or two, 4.5 for four, against 5.7 in
+// tiles); three or four off 16-byte boundaries are better laid out first (3 x 1641 x 1329: 6.6
+// against 8.4). A warp walks its channels' whole depth, so a long one is left to the split of the
+// tensor-core kernel.
 static bool i8_by_rows(int64_t rows, int64_t depth, bool aligned) { return rows <= (aligned ? 4 : 2) && depth <= 8192; }
 
 static I8Operand i8_operand(const int8_t* base, int64_t rows, int64_t stride) {
@@ -309,8 +314,8 @@ static cudaError_t with_layout(const Kv4Shape& h, F&& f) {
   return h.groups == 2 ? f(Int<128>{}, Int<2>{}) : f(Int<128>{}, Int<4>{});
 }
 
-// Heads to a CTA of the write and the read: as many as leave sixteen CTAs to an SM, so that a CTA's set-up is shared by more
-// work without idling the GPU.
+// Heads to a CTA of the write and the read: as many as leave sixteen CTAs to an SM, so that a CTA's
+// set-up is shared by more work without idling the GPU.
 static int head_span(int64_t tokens, int heads) {
   const int64_t ctas = (tokens + 15) / 16 * heads;
   return (int)std::max<int64_t>(1, std::min<int64_t>(heads, ctas / (16 * sm_count())));
@@ -339,10 +344,12 @@ struct AttnPlan {
   size_t bytes;  // workspace: the parts and their (maximum, sum) pairs
 };
 
-// Eight rows a tile where a key head has no more than eight query rows, else sixteen. The token range is cut over the CTAs that
-// make the least estimated time, in fifths of a step's share of a busy SM (0.63 us): a CTA alone takes 2.4 such shares for a
-// step (1.8 with sixteen rows), so up to that many share an SM for nothing, and its set-up takes two steps; joining costs 1.5 in
-// a cluster and 6 through memory. The length is the table's capacity or what a window leaves of it, all that the host knows.
+// Eight rows a tile where a key head has no more than eight query rows, else sixteen. The token
+// range is cut over the CTAs that make the least estimated time, in fifths of a step's share of a
+// busy SM (0.63 us): a CTA alone takes 2.4 such shares for a step (1.8 with sixteen rows), so up to
+// that many share an SM for nothing, and its set-up takes two steps; joining costs 1.5 in a cluster
+// and 6 through memory. The length is the table's capacity or what a window leaves of it, all that
+// the host knows.
 static AttnPlan attn_plan(const Kv4Shape& h, int64_t batch, int64_t queries, int64_t q_heads, int64_t max_pages, int64_t span) {
   AttnPlan p{};
   const int64_t rows = queries * (q_heads / h.heads);

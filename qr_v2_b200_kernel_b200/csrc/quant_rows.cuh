@@ -52,9 +52,10 @@ struct RowsParams {
   int q_aligned;  // rows of q start on 16-byte boundaries
 };
 
-// A pack is 16 bytes of consecutive elements. Where all rows start on 16-byte boundaries and hold whole packs (kAligned) it is one
-// load or store. Elsewhere a load takes the two aligned blocks around it and shifts, if both lie within the operand ([lo, hi)),
-// else it goes element by element; elements from n on read as zero. A store goes by aligned pairs.
+// A pack is 16 bytes of consecutive elements. Where all rows start on 16-byte boundaries and hold
+// whole packs (kAligned) it is one load or store. Elsewhere a load takes the two aligned blocks
+// around it and shifts, if both lie within the operand ([lo, hi)), else it goes element by element;
+// elements from n on read as zero. A store goes by aligned pairs.
 struct Span {
   const char* lo;
   const char* hi;
@@ -120,11 +121,12 @@ __device__ __forceinline__ void store_pack(T* p, const T (&v)[kVec], int n) {
   }
 }
 
-// A row lives in the registers of blockDim.x threads, kItems packs each, a block's y rows beside one another:
-// memory is read once and written once, and bounds it. (16384 x 4096 bf16: 79 us, 5.9 TB/s; rows off
-// 16-byte boundaries cost twice that, 16384 x 2047 65 us; storing those through shared memory, element beside element, lost, 74 us.) Every load of the row is asked for before the first is used. Which
-// thread holds which element depends on the row's length alone, so a row's result, bit for bit, depends on
-// neither its neighbours, their number nor anybody's alignment.
+// A row lives in the registers of blockDim.x threads, kItems packs each, a block's y rows beside
+// one another: memory is read once and written once, and bounds it. (16384 x 4096 bf16: 79 us, 5.9
+// TB/s; rows off 16-byte boundaries cost twice that, 16384 x 2047 65 us; storing those through
+// shared memory, element beside element, lost, 74 us.) Every load of the row is asked for before
+// the first is used. Which thread holds which element depends on the row's length alone, so a row's
+// result, bit for bit, depends on neither its neighbours, their number nor anybody's alignment.
 template <typename T, typename W, bool kNorm, bool kAligned, int kItems>
 __global__ void __launch_bounds__(1024) rows_int8_kernel(RowsParams P) {
   constexpr int kVec = 16 / sizeof(T);
@@ -229,8 +231,9 @@ __global__ void __launch_bounds__(1024) rows_int8_kernel(RowsParams P) {
   }
 }
 
-// value = code * scale of its row, rounded once: sixteen codes of a row to a thread (kPacked: their rows start on 16-byte
-// boundaries, and the values'; kTail: the last of a row may be fewer), or eight, 32 apart, with a warp on 256 neighbouring ones.
+// value = code * scale of its row, rounded once: sixteen codes of a row to a thread (kPacked: their
+// rows start on 16-byte boundaries, and the values'; kTail: the last of a row may be fewer), or
+// eight, 32 apart, with a warp on 256 neighbouring ones.
 template <typename T, bool kPacked, bool kTail>
 __global__ void __launch_bounds__(256) dequant_rows_kernel(const int8_t* q, long long q_stride, const float* scale,
                                                            T* out, long long rows, int cols) {

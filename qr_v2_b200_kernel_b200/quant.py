@@ -11,9 +11,9 @@ bits. These are the operators that make and consume such data:
 
 All run on CUDA tensors only, on the current stream of the operands' device with no host
 synchronisation, and never modify an input (``kv4_write`` writes its cache). Wrong arguments raise
-``TypeError``/``ValueError``, host tensors ``RuntimeError``, and a failing C-ABI call, or one that an
-earlier kernel on the device has reported (an index outside a cache), ``QRB200Error``. Rounding to integers
-has no derivative, so a call that autograd would record raises ``RuntimeError``: use
+``TypeError``/``ValueError``, host tensors ``RuntimeError``, and a failing C-ABI call, or one that
+an earlier kernel on the device has reported (an index outside a cache), ``QRB200Error``. Rounding
+to integers has no derivative, so a call that autograd would record raises ``RuntimeError``: use
 ``torch.no_grad()``. None of them has a counterpart in the reference.
 """
 
@@ -50,22 +50,23 @@ def rms_norm_int8(x: torch.Tensor, weight: torch.Tensor | None = None, residual:
                   eps: float = 1e-6):
     """Root-mean-square norm of ``x + residual`` into 8 bits: ``(codes, scale, h)``.
 
-    ``h = x + residual`` (``x`` itself without a residual), in ``x``'s type; ``codes`` int8 of ``x``'s
-    shape and ``scale`` float32 of its leading shape, with ``codes * scale[..., None]`` the values of
-    ``weight * h / sqrt(mean(h^2) + eps)`` to within half a step of the row's largest / 127. The sums run in 32 bits
-    on ``h`` before its rounding.
+    ``h = x + residual`` (``x`` itself without a residual), in ``x``'s type; ``codes`` int8 of
+    ``x``'s shape and ``scale`` float32 of its leading shape, with ``codes * scale[..., None]`` the
+    values of ``weight * h / sqrt(mean(h^2) + eps)`` to within half a step of the row's largest /
+    127. The sums run in 32 bits on ``h`` before its rounding.
 
     ``x`` (..., cols), cols <= 32768, and ``residual``: bfloat16, float16 or float32, any strides;
-    ``weight`` (cols,) of ``x``'s type or float32. A row with a NaN or an infinity gets a NaN scale. Rows of ``codes`` are
-    16-byte aligned, so ``codes`` is contiguous only where cols is a multiple of 16.
+    ``weight`` (cols,) of ``x``'s type or float32. A row with a NaN or an infinity gets a NaN scale.
+    Rows of ``codes`` are 16-byte aligned, so ``codes`` is contiguous only where cols is a multiple
+    of 16.
     """
     return (_module or _native()).rms_norm_int8(x, weight, residual, eps)
 
 
 def quantize_int8(x: torch.Tensor):
-    """``(codes, scale)``: each row of ``x`` (..., cols) in 8 bits, ``codes * scale[..., None]`` within half a step
-    of its largest / 127. For weights (a scale for each output channel) and for activations that no norm precedes.
-    Types, strides and odd rows as :func:`rms_norm_int8`."""
+    """``(codes, scale)``: each row of ``x`` (..., cols) in 8 bits, ``codes * scale[..., None]`` within
+    half a step of its largest / 127. For weights (a scale for each output channel) and for
+    activations that no norm precedes. Types, strides and odd rows as :func:`rms_norm_int8`."""
     return (_module or _native()).quantize_int8(x)
 
 
@@ -78,11 +79,12 @@ def int8_linear(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor, we
                 bias: torch.Tensor | None = None, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """``(x x_scale[..., None]) (weight weight_scale[:, None])^T + bias`` of 8-bit operands, in ``dtype``.
 
-    ``x`` int8 (..., depth) with a float32 scale for each row (token), ``weight`` int8 (outs, depth) with a
-    float32 scale for each output channel, as :func:`rms_norm_int8` and :func:`quantize_int8` make them;
-    ``bias`` (outs,) of ``dtype``. 1 <= depth <= 131071. The products are summed exactly, in 32-bit integers, and the
-    result is rounded once. Beyond two rows, operands whose rows do not start on 16-byte boundaries are laid out
-    anew first; those that the quantising functions return do.
+    ``x`` int8 (..., depth) with a float32 scale for each row (token), ``weight`` int8 (outs, depth)
+    with a float32 scale for each output channel, as :func:`rms_norm_int8` and :func:`quantize_int8`
+    make them; ``bias`` (outs,) of ``dtype``. 1 <= depth <= 131071. The products are summed exactly,
+    in 32-bit integers, and the result is rounded once. Beyond two rows, operands whose rows do not
+    start on 16-byte boundaries are laid out anew first; those that the quantising functions return
+    do.
     """
     return (_module or _native()).int8_linear(x, x_scale, weight, weight_scale, bias, dtype)
 
@@ -90,8 +92,9 @@ def int8_linear(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor, we
 class KV4Cache:
     """A paged key/value cache in 4 bits (see :func:`kv4_cache`).
 
-    ``data``: uint8 (pages, kv_heads, bytes of a block), the whole state, written in place; ``KV4Cache(data.clone(), ...)``
-    is a copy of the cache. A token occupies head_dim + 8 head_dim / group_size bytes a head for its key and value.
+    ``data``: uint8 (pages, kv_heads, bytes of a block), the whole state, written in place;
+    ``KV4Cache(data.clone(), ...)`` is a copy of the cache. A token occupies head_dim + 8 head_dim /
+    group_size bytes a head for its key and value.
     """
 
     __slots__ = ("data", "pages", "page_size", "kv_heads", "head_dim", "group_size", "dtype", "_handle")
@@ -108,9 +111,9 @@ def kv4_cache(pages: int, page_size: int, kv_heads: int, head_dim: int, group_si
               dtype: torch.dtype = torch.bfloat16, device="cuda") -> KV4Cache:
     """An empty 4-bit cache of ``pages`` pages of ``page_size`` tokens (a power of two from 16 to 1024).
 
-    ``head_dim`` 64 or 128; ``group_size`` channels share a step and a minimum: 32, 64 or 128, at most and by default
-    head_dim. ``dtype``: bfloat16 or float16, of the keys and values written and the queries that read. Fresh slots
-    hold zeros.
+    ``head_dim`` 64 or 128; ``group_size`` channels share a step and a minimum: 32, 64 or 128, at
+    most and by default head_dim. ``dtype``: bfloat16 or float16, of the keys and values written and
+    the queries that read. Fresh slots hold zeros.
     """
     group_size = head_dim if group_size is None else group_size
     if dtype not in (torch.bfloat16, torch.float16):
@@ -140,17 +143,19 @@ def _handle(cache):
 def kv4_write(cache: KV4Cache, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor) -> None:
     """Quantises ``k`` and ``v`` (tokens, kv_heads, head_dim) of the cache's type into its ``slots``.
 
-    ``slots`` int64 (tokens,): page * page_size + offset, each at most once; negative ones are skipped (padding). Channels
-    must be contiguous, the other strides are free. Each group's least entry is kept in the cache's type, its range in fifteen
-    steps; a group with a NaN or an infinity reads back as NaN. A slot past the cache is skipped and reported by the
-    next call as ``QRB200Error``.
+    ``slots`` int64 (tokens,): page * page_size + offset, each at most once; negative ones are
+    skipped (padding). Any strides (copied where channels are not contiguous). Each group's least
+    entry is kept in the cache's type, its range in fifteen steps; a group with a NaN or an infinity
+    reads back as NaN. A slot past the cache is skipped and reported by the next call as
+    ``QRB200Error``.
     """
     (_module or _native()).kv4_write(_handle(cache), k, v, slots)
 
 
 def kv4_read(cache: KV4Cache, slots: torch.Tensor):
-    """``(k, v)``, each (tokens, kv_heads, head_dim): the values that the cache holds at ``slots`` (int64), rounded
-    once to its type; zeros for a negative slot. A slot past the cache reads as zeros and is reported by the next call."""
+    """``(k, v)``, each (tokens, kv_heads, head_dim): the values that the cache holds at ``slots``
+    (int64), rounded once to its type; zeros for a negative slot. A slot past the cache reads as
+    zeros and is reported by the next call."""
     return (_module or _native()).kv4_read(_handle(cache), slots)
 
 
@@ -158,13 +163,15 @@ def kv4_attention(q: torch.Tensor, cache: KV4Cache, block_table: torch.Tensor, l
                   scale: float | None = None, causal: bool = True, window: int | None = None) -> torch.Tensor:
     """Softmax attention of each sequence's newest tokens over its 4-bit cache.
 
-    ``q`` (batch, queries, heads, head_dim) of the cache's type, heads a multiple of kv_heads (head h reads key head
-    h // (heads // kv_heads)). ``block_table`` int32 (batch, max_pages): the pages of each sequence in order; entries past its length are
-    not read. ``lengths`` int32 (batch,): tokens in the cache, the queries' own included, so
-    query i stands at position lengths - queries + i. It sees every token up to its position (all tokens with
-    ``causal=False``), or the last ``window`` of those up to its position. ``scale`` multiplies the scores (default head_dim ** -0.5). Rows that see
-    nothing (an empty sequence, a position before its start) are zero. Returns (batch, queries, heads, head_dim);
-    the scores, the softmax and the sums are in 32 bits, the result is rounded once. A length or page outside
-    the table or the cache is left out and reported by the next call as ``QRB200Error``.
+    ``q`` (batch, queries, heads, head_dim) of the cache's type, heads a multiple of kv_heads (head
+    h reads key head h // (heads // kv_heads)). ``block_table`` int32 (batch, max_pages): the pages
+    of each sequence in order; entries past its length are not read. ``lengths`` int32 (batch,):
+    tokens in the cache, the queries' own included, so query i stands at position lengths - queries
+    + i. It sees every token up to its position (all tokens with ``causal=False``), or the last
+    ``window`` of those up to its position. ``scale`` multiplies the scores (default head_dim **
+    -0.5). Rows that see nothing (an empty sequence, a position before its start) are zero. Returns
+    (batch, queries, heads, head_dim); the scores, the softmax and the sums are in 32 bits, the
+    result is rounded once. A length or page outside the table or the cache is left out and reported
+    by the next call as ``QRB200Error``.
     """
     return (_module or _native()).kv4_attention(q, _handle(cache), block_table, lengths, scale, causal, window)

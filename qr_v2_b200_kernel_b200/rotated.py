@@ -1,19 +1,22 @@
-"""A quantised attention layer in rotated coordinates: what the orthogonal matrices of this package are for.
+"""A quantised attention layer in rotated coordinates: what the orthogonal matrices of this package
+    are for.
 
     python -m qr_v2_b200_kernel_b200.rotated [--hidden 1024] [--tokens 200] [--steps 8]
 
-The residual stream of a transformer has a few channels far larger than the rest, and a scale for a whole row
-then wastes the 8 bits of the others. An orthogonal ``Q`` (hidden x hidden, from :func:`custom_kernel` and
-:func:`householder_product`) spreads them: the stream is kept as ``h Q``, a root-mean-square norm without
-gain commutes with ``Q``, and the weights on either side absorb it (``W diag(gain) Q`` reads the
-stream, ``Q^T W`` writes it). In each head a second one, ``R`` (head_dim x head_dim), does the same for the 4-bit
-cache: ``(q R).(k R) = q.k``, and the output projection takes ``R`` back. Nothing is added to a step:
+    The residual stream of a transformer has a few channels far larger than the rest, and a scale
+    for a whole row then wastes the 8 bits of the others. An orthogonal ``Q`` (hidden x hidden, from
+    :func:`custom_kernel` and :func:`householder_product`) spreads them: the stream is kept as ``h
+    Q``, a root-mean-square norm without gain commutes with ``Q``, and the weights on either side
+    absorb it (``W diag(gain) Q`` reads the stream, ``Q^T W`` writes it). In each head a second one,
+    ``R`` (head_dim x head_dim), does the same for the 4-bit cache: ``(q R).(k R) = q.k``, and the
+    output projection takes ``R`` back. Nothing is added to a step:
 
     rms_norm_int8 -> int8_linear -> kv4_write -> kv4_attention -> quantize_int8 -> int8_linear
 
-The command runs a prompt and some single tokens through one layer, with and without the rotation, and prints
-how far each is from the same layer in 64 bits. (No positional rotation: with one, ``R`` is applied after it.)
-"""
+    The command runs a prompt and some single tokens through one layer, with and without the
+    rotation, and prints how far each is from the same layer in 64 bits. (No positional rotation:
+    with one, ``R`` is applied after it.)
+    """
 
 from __future__ import annotations
 
@@ -31,9 +34,10 @@ __all__ = ["RotatedAttention"]
 class RotatedAttention:
     """One attention layer: int8 projections, a 4-bit cache, one sequence per row of ``block_table``.
 
-    ``wq`` (heads * head_dim, hidden), ``wk`` and ``wv`` (kv_heads * head_dim, hidden), ``wo`` (hidden, heads *
-    head_dim) and ``gain`` (hidden,): floating point, on a CUDA device. ``q_hidden`` (hidden, hidden) and ``q_head``
-    (head_dim, head_dim): orthogonal, or ``None`` for no rotation. Weights are rotated in 64 bits and quantised once.
+    ``wq`` (heads * head_dim, hidden), ``wk`` and ``wv`` (kv_heads * head_dim, hidden), ``wo``
+    (hidden, heads * head_dim) and ``gain`` (hidden,): floating point, on a CUDA device.
+    ``q_hidden`` (hidden, hidden) and ``q_head`` (head_dim, head_dim): orthogonal, or ``None`` for
+    no rotation. Weights are rotated in 64 bits and quantised once.
     """
 
     def __init__(self, wq, wk, wv, wo, gain, head_dim: int, q_hidden=None, q_head=None, dtype=torch.bfloat16):
@@ -55,10 +59,12 @@ class RotatedAttention:
         return kv4_cache(pages, page_size, self.kv_heads, self.head_dim, dtype=self.dtype, device=self.qkv.device)
 
     def __call__(self, x, residual, cache, block_table, lengths, slots):
-        """``(update, residual)`` for ``x`` (batch, queries, hidden), added to ``residual`` first (``None``: x is the stream).
+        """``(update, residual)`` for ``x`` (batch, queries, hidden), added to ``residual`` first (``None``:
+        x is the stream).
 
-        ``slots`` (batch * queries,): where the new tokens go in the cache; ``lengths`` (batch,): tokens with
-        them. ``update`` is the layer's output, to be added to ``residual`` by the next norm.
+        ``slots`` (batch * queries,): where the new tokens go in the cache; ``lengths`` (batch,):
+        tokens with them. ``update`` is the layer's output, to be added to ``residual`` by the next
+        norm.
         """
         batch, queries, _ = x.shape
         codes, scale, stream = rms_norm_int8(x, residual=residual)

@@ -263,6 +263,24 @@ def test_cache_write_and_read(tokens, start, heads, page, dim, group, dtype):
             assert torch.equal(torch.nan_to_num(p, nan=-1.0), torch.nan_to_num(q, nan=-1.0))
 
 
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("dim, group", [(64, 32), (64, 64), (128, 32), (128, 64), (128, 128)])
+def test_cache_codes_are_the_formulas_bit_for_bit(dim, group, dtype):
+    """Steps, minima and codes as elementary 32-bit operations give them, each rounded, ties to even: a 16-bit number often
+    lies midway between two codes."""
+    cache = qr.kv4_cache(8, 64, 3, dim, group, dtype)
+    for at, slots in ((0, torch.arange(500, device="cuda")), (1, torch.arange(7, 507, device="cuda"))):  # whole runs, and not
+        k, v = (_randn(500, 3, dim, seed=60 + at + c, dtype=dtype) * (1 + c) for c in (0, 2))
+        qr.kv4_write(cache, k, v, slots)
+        for x, (codes, s, m) in zip((k, v), _decode(cache)):
+            g = x.float().unflatten(-1, (-1, group))
+            lo, hi = g.amin(-1), g.amax(-1)
+            step = (hi * (1 / 15) - lo * (1 / 15)).to(dtype).float()
+            want = torch.round((g - lo.unsqueeze(-1)) * (1 / step).unsqueeze(-1)).clamp(0, 15).flatten(-2)
+            pick = lambda t: t.transpose(1, 2).flatten(0, 1)[slots].float()  # noqa: E731
+            assert torch.equal(pick(s), step) and torch.equal(pick(m), lo) and torch.equal(pick(codes), want)
+
+
 def test_cache_codes_do_not_depend_on_how_slots_arrive():
     """The same tokens in one call, in a shuffled one, and one by one: the same bytes."""
     k, v = _randn(77, 2, 128, seed=22, dtype=BF), _randn(77, 2, 128, seed=23, dtype=BF)
