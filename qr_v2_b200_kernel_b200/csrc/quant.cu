@@ -219,7 +219,7 @@ static cudaError_t launch_i8_wide(I8Params p, const I8Operand& x, const I8Operan
 
 // Which kernel, with how many rows a tile (`rows`) and over how many CTAs of the depth: the least
 // of the estimated clocks. A CTA takes in its stages at about 40 bytes a clock; joining a split
-// costs two cluster barriers (about 1500 clocks) and reading the sums at about 16 bytes a clock.
+// costs two cluster barriers (about 1500 clocks) and reading the sums at about 20 bytes a clock.
 // Clusters of eight lose: a GPC holds two at best (64 x 1000 x 2048: 12 us against 9). The wide
 // kernel's pair takes 512 clocks a stage and a tile's last epilogue is bare.
 struct I8Plan {
@@ -236,7 +236,7 @@ static I8Plan i8_plan(int64_t rows, int64_t outs, int64_t depth) {
     if ((rows + bn - 1) / bn > 65535) continue;
     for (unsigned split = 1; split <= kI8Split && split <= nk; split *= 2) {
       const int64_t clocks = (tiles * split + sms - 1) / sms *
-                             ((nk + split - 1) / split * (128 + bn) * 128 / 40 + (split > 1 ? 1500 + bn * 32 : bn * 8));
+                             ((nk + split - 1) / split * (128 + bn) * 128 / 40 + (split > 1 ? 1500 + bn * 24 : bn * 8));
       if (clocks < least) {
         least = clocks;
         best = I8Plan{bn, split};
