@@ -281,6 +281,25 @@ def test_cache_codes_are_the_formulas_bit_for_bit(dim, group, dtype):
             assert torch.equal(pick(s), step) and torch.equal(pick(m), lo) and torch.equal(pick(codes), want)
 
 
+def test_cache_groups_wider_than_32_bits_reach():
+    """bf16 ends whose difference overflows 32 bits: the codes are the formula's in 64 bits; ends at 0 and 15."""
+    x = _randn(40, 2, 128, seed=64).mul(2.0**127).clamp(-3.2e38, 3.2e38).to(BF)
+    x[:, :, 0], x[:, :, 64] = -3e38, 3e38  # each group wider than 3.4e38
+    x[:, :, 1], x[:, :, 65] = 2.5e38, -2.5e38
+    cache = qr.kv4_cache(4, 16, 2, 128, 64)
+    slots = torch.arange(3, 43, device="cuda")
+    qr.kv4_write(cache, x, -x, slots)
+    for x, (codes, s, m) in zip((x, -x), _decode(cache)):
+        g = x.double().unflatten(-1, (-1, 64))
+        lo, hi = g.amin(-1), g.amax(-1)
+        pick = lambda t: t.transpose(1, 2).flatten(0, 1)[slots].double()  # noqa: E731
+        step = pick(s)
+        assert torch.equal(pick(m), lo) and bool(((step - (hi - lo) / 15).abs() <= step * 2.0**-8).all())
+        want = (g - lo.unsqueeze(-1)) / step.unsqueeze(-1)
+        # The nearest code; near halfway (within 16 roundings of 2^-24) either.
+        assert bool(((pick(codes).unflatten(-1, (-1, 64)) - want.clamp(0, 15)).abs() <= 0.5 + 15 * 2.0**-20).all())
+
+
 def test_cache_codes_do_not_depend_on_how_slots_arrive():
     """The same tokens in one call, in a shuffled one, and one by one: the same bytes."""
     k, v = _randn(77, 2, 128, seed=22, dtype=BF), _randn(77, 2, 128, seed=23, dtype=BF)
