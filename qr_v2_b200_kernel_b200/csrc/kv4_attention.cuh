@@ -109,9 +109,11 @@ struct KvKey<__half> {
 };
 __device__ __forceinline__ float kv_power(int e) { return __int_as_float((max(-126, min(127, e)) + 127) << 23); }
 // The power of two that brings a row whose largest entry has these bits (32-bit float, no sign) to
-// kTop.
+// kTop, as far as it and what takes it back, 2^(kOne - lift), are numbers.
 template <typename T>
-__device__ __forceinline__ int kv_lift(unsigned top) { return min(120, KvKey<T>::kTop + 127 - (int)(top >> 23)); }
+__device__ __forceinline__ int kv_lift(unsigned top) {
+  return max(KvKey<T>::kOne - 127, min(120, KvKey<T>::kTop + 127 - (int)(top >> 23)));
+}
 
 __device__ __forceinline__ uint32_t kv_pack(float2 x) {
   const __half2 r = __float22half2_rn(x);

@@ -513,6 +513,24 @@ def test_attention_queries_of_any_size(dtype, size):
     assert torch.all((a.double() - b.double()).abs() <= 2 * U[dtype] * a.double().abs() + 2.0**-14)
 
 
+@pytest.mark.parametrize("power", [-90, -60, 60, 100, 110])
+def test_attention_of_large_queries_and_small_keys_is_the_same_and_the_reverse(power):
+    """Queries times 2^p on keys divided by it: every number only changes its exponent, so every bit of the result stays.
+    (Where queries shrink the smallest partial products may leave the normal range: then to its rounding.)"""
+    q, plain, table, lengths = _case([70, 33], 2, 2, 3, 16, 128, 64, BF)
+    k, v = _randn(128, 2, 128, seed=66, dtype=BF), _randn(128, 2, 128, seed=67, dtype=BF)
+    slots = torch.arange(128, device="cuda")
+    shifted = qr.kv4_cache(plain.pages, 16, 2, 128, 64, BF)
+    qr.kv4_write(plain, k, v, slots)
+    qr.kv4_write(shifted, k * 2.0**-power, v, slots)
+    a = qr.kv4_attention(q, plain, table % 8, lengths)
+    b = qr.kv4_attention(q * 2.0**power, shifted, table % 8, lengths)
+    if power > 0:
+        assert torch.equal(a, b)
+    else:
+        assert torch.all((a.double() - b.double()).abs() <= 2 * U[BF] * a.double().abs() + 2.0**-14)
+
+
 # ---- refusals -------------------------------------------------------------------------------
 
 
