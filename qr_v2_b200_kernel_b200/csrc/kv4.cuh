@@ -100,10 +100,11 @@ __device__ __forceinline__ unsigned char* kv4_run(const Kv4IoParams& P, long lon
 // the sixteen fill a run, as prompts do, the run is put together in shared memory and stored whole;
 // otherwise each thread stores its words (keys) and bytes (values). Long prompts are bound by
 // instructions: codes come out of the 32-bit floating sum's bits, packed as they lie.
-// 32768 tokens x 8 heads x 128 channels, bf16: 55 us (2.8 TB/s; 320 instructions of a warp for its
-// 512 elements); walking several heads took it from 63.
+// 32768 tokens x 8 heads x 128 channels, bf16: 54 us (2.8 TB/s; 320 instructions of a warp for its
+// 512 elements, issue slots 77 % busy). Walking several heads took it from 63, registers for 40
+// warps an SM in place of 32 from 56 (48 warps would spill: 56).
 template <typename T, int kDim, int kGroups, bool kVec>
-__global__ void __launch_bounds__(2 * kDim) kv4_write_kernel(Kv4IoParams P) {
+__global__ void __launch_bounds__(2 * kDim, kVec ? 640 / kDim : 1) kv4_write_kernel(Kv4IoParams P) {
   constexpr int kChunks = kDim / 8, kSpan = kChunks / kGroups;  // threads of a token, of a group
   constexpr int kRunBytes = 16 * kDim + 128 * kGroups;
   __shared__ uint4 s_run[2][kRunBytes / 16];
