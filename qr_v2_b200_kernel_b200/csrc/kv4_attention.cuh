@@ -12,9 +12,12 @@
 //   it is a subnormal (or the first normal binade, which continues them), worth code 2^-133 in bf16
 //   and code 2^-24 in fp16, 16 times that four bits higher. The factors are powers of two: 1/16
 //   goes to the queries of those channels; each query row is brought by another to the top of its
-//   type's range, where neither it nor the products lose bits; the scores take both back. A value's
-//   nibble is placed under fp16's exponent of 1024 and brought to code - 8, which keeps sums over
-//   many tokens from cancelling.
+//   type's range, where neither it nor the products lose bits; the scores take both back. Values'
+//   nibbles go the same way as fp16, the weights' powers of two and the output's last step taking
+//   theirs (128 us; 139 with codes brought to code - 8 in fp16 first). Codes are never negative, and
+//   the matrix instruction cuts off where it adds, so the sums would drift as they grow: every
+//   fourth step what a lane's first channel has summed is taken off all of its channels and kept
+//   beside them.
 // * the weights p_t s_t are the only rounded operand: two fp16 numbers each, high and low, 22 bits
 //   in all (one alone would add an error the size of the result's own rounding). They are scaled by
 //   a power of two that puts the largest step near 2^11, so that a weight keeps its leading bits
@@ -26,7 +29,7 @@
 // of the operand's registers. The token range is cut over CTAs (blockIdx.x) and over a CTA's four
 // warps; the parts are joined through shared memory and, between CTAs, through the cluster's shared
 // memory (up to eight) or by kv4_join_kernel, always in a fixed order.
-// 64 sequences x 8192 tokens, 64 heads on 8: 139 us, 4.1 TB/s of cache; 1 x 65536 32 us; one of
+// 64 sequences x 8192 tokens, 64 heads on 8: 126 us, 4.5 TB/s of cache; 1 x 65536 30 us; one of
 // 513 tokens 6.5 us, which is latency from end to end.
 #pragma once
 
@@ -77,23 +80,11 @@ __device__ __forceinline__ void kv_mma<__half>(float (&d)[4], const uint32_t (&a
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// Nibbles p and p + 4 of w as a pair of 16-bit numbers: bare (the integer code, times 16 for odd p,
-// as a subnormal of either 16-bit type), and as code - 8 in fp16.
+// Nibbles p and p + 4 of w as a pair of 16-bit numbers: the integer code, times 16 for odd p, as a
+// subnormal of either 16-bit type.
 __device__ __forceinline__ uint32_t kv_pair_bare(uint32_t w, int p) {
   if (p & 2) w >>= 8;
   return w & (p & 1 ? 0x00f000f0u : 0x000f000fu);
-}
-__device__ __forceinline__ uint32_t kv_pair_fp16(uint32_t w, int p) {
-  if (p & 2) w >>= 8;
-  if (p & 1) {  // 16 code + 1024: brought to code + 64, less 72, in one fused step
-    const uint32_t x = (w & 0x00f000f0u) | 0x64006400u;
-    const __half2 r = __hfma2(reinterpret_cast<const __half2&>(x), __floats2half2_rn(0.0625f, 0.0625f),
-                              __floats2half2_rn(-72.f, -72.f));
-    return reinterpret_cast<const uint32_t&>(r);
-  }
-  const uint32_t x = (w & 0x000f000fu) | 0x64006400u;
-  const __half2 r = __hsub2(reinterpret_cast<const __half2&>(x), __floats2half2_rn(1032.f, 1032.f));
-  return reinterpret_cast<const uint32_t&>(r);
 }
 // Where a query row's largest entry is put (its exponent), and what its type makes of the code 1
 // (the negative exponent).
@@ -166,8 +157,8 @@ __device__ __forceinline__ void mbar_expect(uint32_t mbar, uint32_t bytes) {
 
 constexpr int kKvStages = 3;
 // CTAs to an SM that registers are kept for. Four (128 registers) beat three wherever nothing
-// spills (64 x 8192 tokens, one group: 139 against 152 us); four groups of steps would (131 against
-// 118 us).
+// spills much (64 x 8192 tokens, one group: 126 against 138 us); four groups of steps would (131
+// against 118 us).
 __host__ __device__ constexpr int kv_ctas(int groups, int nt) { return nt > 1 ? 2 : groups < 4 ? 4 : 3; }
 // Dynamic shared memory: the warps' rings, reused at the end for their parts of the output.
 __host__ __device__ constexpr int kv_stage_bytes(int dim, int groups, bool brief) {
@@ -337,7 +328,9 @@ __global__ void __launch_bounds__(32 * kKvWarps, kv_ctas(kGroups, kNT)) kv4_atte
     for (int w = 0; w < kKvWarps; ++w) top = max(top, s_qtop[w][n][row]);
     return kv_lift<T>(top);
   };
-  float2 qsum[kNT][kGroups], back[kNT];  // back: what gives q . c from the product with bare codes
+  // back: what gives q . c from the product with bare codes. Both are in the exponent's units (base
+  // 2), so that the largest score less itself is 0 and its weight 1, exactly.
+  float2 qsum[kNT][kGroups], back[kNT];
 #pragma unroll
   for (int n = 0; n < kNT; ++n) {
     const float up = kv_power(lift(n, g));
@@ -348,7 +341,8 @@ __global__ void __launch_bounds__(32 * kKvWarps, kv_ctas(kGroups, kNT)) kv4_atte
       put2(x + 2, to_f32(qv[n][i][2]) * (up / 16), to_f32(qv[n][i][3]) * (up / 16));
       s_q[n][i * kKvWarps + warp][lane] = *reinterpret_cast<uint2*>(x);
     }
-    back[n] = make_float2(kv_power(KvKey<T>::kOne - lift(n, 2 * t)), kv_power(KvKey<T>::kOne - lift(n, 2 * t + 1)));
+    back[n] = make_float2(kv_power(KvKey<T>::kOne - lift(n, 2 * t)) * P.scale2,
+                          kv_power(KvKey<T>::kOne - lift(n, 2 * t + 1)) * P.scale2);
 #pragma unroll
     for (int gr = 0; gr < kGroups; ++gr) {
       qsum[n][gr] = make_float2(0.f, 0.f);
@@ -356,13 +350,14 @@ __global__ void __launch_bounds__(32 * kKvWarps, kv_ctas(kGroups, kNT)) kv4_atte
         qsum[n][gr].x += s_qsum[w][n][2 * t][gr];
         qsum[n][gr].y += s_qsum[w][n][2 * t + 1][gr];
       }
+      qsum[n][gr] = make_float2(qsum[n][gr].x * P.scale2, qsum[n][gr].y * P.scale2);
     }
   }
   __syncthreads();
 
-  float o[kNT][kSteps][4] = {};  // scaled by `unit`
-  float2 sum[kNT] = {}, mids[kNT][kGroups] = {};
-  // Weights are 2^(score scale2 + less); bound is where a score moves that reference. cap bounds
+  float o[kNT][kSteps][4] = {};  // scaled by `unit`, less `off`; [2] and [3] are 16 times that
+  float2 sum[kNT] = {}, lows[kNT][kGroups] = {}, off[kNT][kGroups] = {};
+  // Weights are 2^(score + less); bound is where a score moves that reference. cap bounds
   // the steps, unit scales them.
   float2 less[kNT] = {};
   float bound[kNT][2], cap = 0.f, unit = 1.f;
@@ -377,7 +372,7 @@ __global__ void __launch_bounds__(32 * kKvWarps, kv_ctas(kGroups, kNT)) kv4_atte
     const unsigned gone = missing >> (8 * stage) & ((1u << kRuns) - 1);
     ok = ok && __all_sync(kFullMask, mbar_wait(&s_full[warp][stage], turn));
     if (!ok) break;
-    // Scores before scaling: s[i][n][h] holds token tok0 + 16 i + 8 h + g against rows 8 n + 2 t
+    // Scores: s[i][n][h] holds token tok0 + 16 i + 8 h + g against rows 8 n + 2 t
     // and the next.
     float2 s[kRuns][kNT][2];
     {
@@ -454,7 +449,7 @@ __global__ void __launch_bounds__(32 * kKvWarps, kv_ctas(kGroups, kNT)) kv4_atte
           }
       }
     }
-    float2 val[kRuns][2][kGroups];  // step, and minimum + 8 steps
+    float2 val[kRuns][2][kGroups];  // step and minimum
     float up[kNT][2], steps = 0.f;
 #pragma unroll
     for (int i = 0; i < kRuns; ++i)
@@ -462,10 +457,8 @@ __global__ void __launch_bounds__(32 * kKvWarps, kv_ctas(kGroups, kNT)) kv4_atte
       for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (int gr = 0; gr < kGroups; ++gr) {
-          float2 v = kv_step_low<T>(vp[i][h][gr]);
-          v.y = fmaf(8.f, v.x, v.y);
-          val[i][h][gr] = v;
-          steps = fmaxf(steps, v.x);
+          val[i][h][gr] = kv_step_low<T>(vp[i][h][gr]);
+          steps = fmaxf(steps, val[i][h][gr].x);
         }
     bool move = steps > cap;
 #pragma unroll
@@ -479,11 +472,7 @@ __global__ void __launch_bounds__(32 * kKvWarps, kv_ctas(kGroups, kNT)) kv4_atte
           up[n][0] = fmaxf(up[n][0], s[i][n][h].x);
           up[n][1] = fmaxf(up[n][1], s[i][n][h].y);
         }
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        up[n][c] *= P.scale2;
-        move = move || up[n][c] > bound[n][c];
-      }
+      move = move || up[n][0] > bound[n][0] || up[n][1] > bound[n][1];
     }
     if (__any_sync(kFullMask, move)) {
       steps = fmaxf(steps, cap);
@@ -513,7 +502,10 @@ __global__ void __launch_bounds__(32 * kKvWarps, kv_ctas(kGroups, kNT)) kv4_atte
         }
         sum[n] = make_float2(sum[n].x * keep[0], sum[n].y * keep[1]);
 #pragma unroll
-        for (int gr = 0; gr < kGroups; ++gr) mids[n][gr] = make_float2(mids[n][gr].x * keep[0], mids[n][gr].y * keep[1]);
+        for (int gr = 0; gr < kGroups; ++gr) {
+          lows[n][gr] = make_float2(lows[n][gr].x * keep[0], lows[n][gr].y * keep[1]);
+          off[n][gr] = make_float2(off[n][gr].x * keep[0] * ratio, off[n][gr].y * keep[1] * ratio);
+        }
 #pragma unroll
         for (int j = 0; j < kSteps; ++j)
 #pragma unroll
@@ -532,8 +524,7 @@ __global__ void __launch_bounds__(32 * kKvWarps, kv_ctas(kGroups, kNT)) kv4_atte
         for (int n = 0; n < kNT; ++n)
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            const float2 p = make_float2(kv_exp2(fmaf(s[i][n][h].x, P.scale2, less[n].x)),
-                                         kv_exp2(fmaf(s[i][n][h].y, P.scale2, less[n].y)));
+            const float2 p = make_float2(kv_exp2(s[i][n][h].x + less[n].x), kv_exp2(s[i][n][h].y + less[n].y));
             sum[n].x += p.x;
             sum[n].y += p.y;
             s[i][n][h] = p;
@@ -549,12 +540,12 @@ __global__ void __launch_bounds__(32 * kKvWarps, kv_ctas(kGroups, kNT)) kv4_atte
               const float2 p = s[i][n][h];
               float2 x = make_float2(p.x * scaled, p.y * scaled);
               if constexpr (kAll) {
-                mids[n][gr].x = fmaf(p.x, val[i][h][gr].y, mids[n][gr].x);
-                mids[n][gr].y = fmaf(p.y, val[i][h][gr].y, mids[n][gr].y);
+                lows[n][gr].x = fmaf(p.x, val[i][h][gr].y, lows[n][gr].x);
+                lows[n][gr].y = fmaf(p.y, val[i][h][gr].y, lows[n][gr].y);
               } else {  // what a row does not see may be NaN
-                if (seen[n] >> (4 * i + 2 * h) & 1) mids[n][gr].x = fmaf(p.x, val[i][h][gr].y, mids[n][gr].x);
+                if (seen[n] >> (4 * i + 2 * h) & 1) lows[n][gr].x = fmaf(p.x, val[i][h][gr].y, lows[n][gr].x);
                 else x.x = 0.f;
-                if (seen[n] >> (4 * i + 2 * h) & 2) mids[n][gr].y = fmaf(p.y, val[i][h][gr].y, mids[n][gr].y);
+                if (seen[n] >> (4 * i + 2 * h) & 2) lows[n][gr].y = fmaf(p.y, val[i][h][gr].y, lows[n][gr].y);
                 else x.y = 0.f;
               }
               const uint32_t high = kv_pack(x);
@@ -566,7 +557,7 @@ __global__ void __launch_bounds__(32 * kKvWarps, kv_ctas(kGroups, kNT)) kv4_atte
 #pragma unroll
           for (int j = gr * kPer; j < (gr + 1) * kPer; ++j) {
             const uint32_t word = vc[j >> 2][j & 3];
-            const uint32_t a[4] = {kv_pair_fp16(word, 0), kv_pair_fp16(word, 1), kv_pair_fp16(word, 2), kv_pair_fp16(word, 3)};
+            const uint32_t a[4] = {kv_pair_bare(word, 0), kv_pair_bare(word, 1), kv_pair_bare(word, 2), kv_pair_bare(word, 3)};
 #pragma unroll
             for (int n = 0; n < kNT; ++n)
 #pragma unroll
@@ -577,6 +568,22 @@ __global__ void __launch_bounds__(32 * kKvWarps, kv_ctas(kGroups, kNT)) kv4_atte
     };
     if (full) finish(std::true_type{});
     else finish(std::false_type{});
+    if ((k & 3) == 3) {  // what a group's first tile has summed is set aside, for all of its tiles
+#pragma unroll
+      for (int n = 0; n < kNT; ++n)
+#pragma unroll
+        for (int gr = 0; gr < kGroups; ++gr) {
+          const float2 d = make_float2(o[n][gr * kPer][0], o[n][gr * kPer][1]);
+          off[n][gr] = make_float2(off[n][gr].x + d.x, off[n][gr].y + d.y);
+#pragma unroll
+          for (int j = gr * kPer; j < (gr + 1) * kPer; ++j) {
+            o[n][j][0] -= d.x;
+            o[n][j][1] -= d.y;
+            o[n][j][2] = fmaf(-16.f, d.x, o[n][j][2]);
+            o[n][j][3] = fmaf(-16.f, d.y, o[n][j][3]);
+          }
+        }
+    }
     __syncwarp();  // every lane has read this stage
     if (k + kKvStages < count) issue(u + kKvStages, stage);
     if (++stage == kKvStages) {
@@ -594,14 +601,18 @@ __global__ void __launch_bounds__(32 * kKvWarps, kv_ctas(kGroups, kNT)) kv4_atte
   float(*s_o)[kRows][kDim + 4] = reinterpret_cast<float(*)[kRows][kDim + 4]>(s_ring);
 
   const float lower = 1.f / unit;
+  constexpr float kOne = 0x1p24f;  // of the bare codes
   // The warps' parts: o[n][j][e] is channel 16 j + g + 8 (e / 2) of row 8 n + 2 t + e % 2.
 #pragma unroll
   for (int n = 0; n < kNT; ++n)
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
-      float l = c ? sum[n].y : sum[n].x, add[kGroups];
+      float l = c ? sum[n].y : sum[n].x, add[kGroups], aside[kGroups];
 #pragma unroll
-      for (int gr = 0; gr < kGroups; ++gr) add[gr] = c ? mids[n][gr].y : mids[n][gr].x;
+      for (int gr = 0; gr < kGroups; ++gr) {
+        add[gr] = c ? lows[n][gr].y : lows[n][gr].x;
+        aside[gr] = c ? off[n][gr].y : off[n][gr].x;
+      }
 #pragma unroll
       for (int x = 4; x < 32; x <<= 1) {
         l += __shfl_xor_sync(kFullMask, l, x);
@@ -611,8 +622,9 @@ __global__ void __launch_bounds__(32 * kKvWarps, kv_ctas(kGroups, kNT)) kv4_atte
       if (g == 0) s_ml[warp][8 * n + 2 * t + c] = make_float2(bound[n][c] - kKvLazy, l);
 #pragma unroll
       for (int j = 0; j < kSteps; ++j) {
-        s_o[warp][8 * n + 2 * t + c][16 * j + g] = fmaf(o[n][j][c], lower, add[j / kPer]);
-        s_o[warp][8 * n + 2 * t + c][16 * j + g + 8] = fmaf(o[n][j][2 + c], lower, add[j / kPer]);
+        const float first = aside[j / kPer] + o[n][j][c], second = fmaf(0.0625f, o[n][j][2 + c], aside[j / kPer]);
+        s_o[warp][8 * n + 2 * t + c][16 * j + g] = fmaf(first * kOne, lower, add[j / kPer]);
+        s_o[warp][8 * n + 2 * t + c][16 * j + g + 8] = fmaf(second * kOne, lower, add[j / kPer]);
       }
     }
   __syncthreads();
