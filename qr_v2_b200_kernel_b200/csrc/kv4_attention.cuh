@@ -24,12 +24,13 @@
 //   down to 2^-25 of the largest.
 // * the running maximum and that scale move only when a score exceeds the reference by 2^4 or a
 //   step its bound, so that the output is rarely rescaled and the warp rarely reduces.
+// * a lane's two query rows go through paired 32-bit operations (127 -> 123 us).
 // Each warp walks its own stretch of tokens, a step of 32 or 64 at a time, through a ring of three
 // steps in shared memory that bulk asynchronous copies fill: a run's bytes are already in the order
 // of the operand's registers. The token range is cut over CTAs (blockIdx.x) and over a CTA's four
 // warps; the parts are joined through shared memory and, between CTAs, through the cluster's shared
 // memory (up to eight) or by kv4_join_kernel, always in a fixed order.
-// 64 sequences x 8192 tokens, 64 heads on 8: 126 us, 4.5 TB/s of cache; 1 x 65536 30 us; one of
+// 64 sequences x 8192 tokens, 64 heads on 8: 123 us, 4.7 TB/s of cache; 1 x 65536 30 us; one of
 // 513 tokens 6.5 us, which is latency from end to end.
 #pragma once
 
@@ -61,7 +62,7 @@ constexpr int kKvCluster = 8;  // the most CTAs that join their parts within a c
 // channels, half the runs). With 64 channels a warp that has no more than two such steps takes them
 // in halves: its time is that of code running for the first time, and there is half as much (12 x
 // 2047 tokens, five drafts, window 1000: 12.2 against 10.0 us; 64 x 8192 tokens in halves would
-// take 63 against 56 us; with 128 channels halves lose, 6.8 against 6.4 us for one sequence of
+// take 58 against 51 us; with 128 channels halves lose, 6.8 against 6.4 us for one sequence of
 // 513).
 __host__ __device__ constexpr int kv_runs(int dim, bool brief) { return dim == 64 && !brief ? 4 : 2; }
 
@@ -156,9 +157,9 @@ __device__ __forceinline__ void mbar_expect(uint32_t mbar, uint32_t bytes) {
 }
 
 constexpr int kKvStages = 3;
-// CTAs to an SM that registers are kept for. Four (128 registers) beat three wherever nothing
-// spills much (64 x 8192 tokens, one group: 126 against 138 us); four groups of steps would (131
-// against 118 us).
+// CTAs to an SM that registers are kept for. Four (128 registers) beat three wherever little spills
+// (64 x 8192 tokens, one group: 126 against 138 us); four groups of steps would (125 against 111
+// us).
 __host__ __device__ constexpr int kv_ctas(int groups, int nt) { return nt > 1 ? 2 : groups < 4 ? 4 : 3; }
 // Dynamic shared memory: the warps' rings, reused at the end for their parts of the output.
 __host__ __device__ constexpr int kv_stage_bytes(int dim, int groups, bool brief) {
@@ -410,8 +411,9 @@ __global__ void __launch_bounds__(32 * kKvWarps, kv_ctas(kGroups, kNT)) kv4_atte
                 *reinterpret_cast<const uint32_t*>(runs + i * kRunBytes + 16 * kDim + ((g + 8 * h) * kGroups + gr) * 4));
 #pragma unroll
             for (int n = 0; n < kNT; ++n) {
-              s[i][n][h].x = fmaf(k.x, acc[i][n][2 * h] * back[n].x, fmaf(k.y, qsum[n][gr].x, gr ? s[i][n][h].x : 0.f));
-              s[i][n][h].y = fmaf(k.x, acc[i][n][2 * h + 1] * back[n].y, fmaf(k.y, qsum[n][gr].y, gr ? s[i][n][h].y : 0.f));
+              const float2 kx = make_float2(k.x, k.x), ky = make_float2(k.y, k.y);
+              const float2 low = gr ? __ffma2_rn(ky, qsum[n][gr], s[i][n][h]) : __fmul2_rn(ky, qsum[n][gr]);
+              s[i][n][h] = __ffma2_rn(kx, __fmul2_rn(make_float2(acc[i][n][2 * h], acc[i][n][2 * h + 1]), back[n]), low);
             }
           }
       }
@@ -524,9 +526,8 @@ __global__ void __launch_bounds__(32 * kKvWarps, kv_ctas(kGroups, kNT)) kv4_atte
         for (int n = 0; n < kNT; ++n)
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            const float2 p = make_float2(kv_exp2(s[i][n][h].x + less[n].x), kv_exp2(s[i][n][h].y + less[n].y));
-            sum[n].x += p.x;
-            sum[n].y += p.y;
+            const float2 e = __fadd2_rn(s[i][n][h], less[n]), p = make_float2(kv_exp2(e.x), kv_exp2(e.y));
+            sum[n] = __fadd2_rn(sum[n], p);
             s[i][n][h] = p;
           }
 #pragma unroll
@@ -538,10 +539,9 @@ __global__ void __launch_bounds__(32 * kKvWarps, kv_ctas(kGroups, kNT)) kv4_atte
 #pragma unroll
             for (int n = 0; n < kNT; ++n) {
               const float2 p = s[i][n][h];
-              float2 x = make_float2(p.x * scaled, p.y * scaled);
+              float2 x = __fmul2_rn(p, make_float2(scaled, scaled));
               if constexpr (kAll) {
-                lows[n][gr].x = fmaf(p.x, val[i][h][gr].y, lows[n][gr].x);
-                lows[n][gr].y = fmaf(p.y, val[i][h][gr].y, lows[n][gr].y);
+                lows[n][gr] = __ffma2_rn(p, make_float2(val[i][h][gr].y, val[i][h][gr].y), lows[n][gr]);
               } else {  // what a row does not see may be NaN
                 if (seen[n] >> (4 * i + 2 * h) & 1) lows[n][gr].x = fmaf(p.x, val[i][h][gr].y, lows[n][gr].x);
                 else x.x = 0.f;
@@ -550,8 +550,8 @@ __global__ void __launch_bounds__(32 * kKvWarps, kv_ctas(kGroups, kNT)) kv4_atte
               }
               const uint32_t high = kv_pack(x);
               w[0][n][h] = kv_transpose(high);
-              const float2 top = __half22float2(reinterpret_cast<const __half2&>(high));
-              w[1][n][h] = kv_transpose(kv_pack(make_float2(x.x - top.x, x.y - top.y)));
+              const float2 top = __half22float2(__hneg2(reinterpret_cast<const __half2&>(high)));
+              w[1][n][h] = kv_transpose(kv_pack(__fadd2_rn(x, top)));
             }
           }
 #pragma unroll
