@@ -101,10 +101,11 @@ struct KvKey<__half> {
 };
 __device__ __forceinline__ float kv_power(int e) { return __int_as_float((max(-126, min(127, e)) + 127) << 23); }
 // The power of two that brings a row whose largest entry has these bits (32-bit float, no sign) to
-// kTop, as far as it and what takes it back, 2^(kOne - lift), are numbers.
+// kTop, as far as it and what takes it back, scale2 2^(kOne - lift), are numbers.
 template <typename T>
-__device__ __forceinline__ int kv_lift(unsigned top) {
-  return max(KvKey<T>::kOne - 127, min(120, KvKey<T>::kTop + 127 - (int)(top >> 23)));
+__device__ __forceinline__ int kv_lift(unsigned top, float scale2) {
+  const int least = KvKey<T>::kOne - 127 + max(0, (__float_as_int(scale2) >> 23) - 126);
+  return max(least, min(120, KvKey<T>::kTop + 127 - (int)(top >> 23)));
 }
 
 __device__ __forceinline__ uint32_t kv_pack(float2 x) {
@@ -327,7 +328,7 @@ __global__ void __launch_bounds__(32 * kKvWarps, kv_ctas(kGroups, kNT)) kv4_atte
   const auto lift = [&](int n, int row) {
     unsigned top = 0;
     for (int w = 0; w < kKvWarps; ++w) top = max(top, s_qtop[w][n][row]);
-    return kv_lift<T>(top);
+    return kv_lift<T>(top, P.scale2);
   };
   // back: what gives q . c from the product with bare codes. Both are in the exponent's units (base
   // 2), so that the largest score less itself is 0 and its weight 1, exactly.

@@ -531,6 +531,19 @@ def test_attention_of_large_queries_and_small_keys_is_the_same_and_the_reverse(p
         assert torch.all((a.double() - b.double()).abs() <= 2 * U[BF] * a.double().abs() + 2.0**-14)
 
 
+@pytest.mark.parametrize("scale", [0.7, 1.0, 5.0])
+def test_attention_of_large_queries_with_a_scale_above_one(scale):
+    """As above, every bit of the result stays; the scale comes in where the queries' size is taken back."""
+    q, plain, table, lengths = _case([70, 33], 2, 2, 3, 16, 128, 64, BF)
+    k, v = _randn(128, 2, 128, seed=68, dtype=BF), _randn(128, 2, 128, seed=69, dtype=BF)
+    slots = torch.arange(128, device="cuda")
+    shifted = qr.kv4_cache(plain.pages, 16, 2, 128, 64, BF)
+    qr.kv4_write(plain, k, v, slots)
+    qr.kv4_write(shifted, k * 2.0**-100, v, slots)
+    a = qr.kv4_attention(q, plain, table % 8, lengths, scale=scale)
+    assert torch.equal(a, qr.kv4_attention(q * 2.0**100, shifted, table % 8, lengths, scale=scale))
+
+
 # ---- refusals -------------------------------------------------------------------------------
 
 
