@@ -13,11 +13,16 @@
 //   and code 2^-24 in fp16, 16 times that four bits higher. The factors are powers of two: 1/16
 //   goes to the queries of those channels; each query row is brought by another to the top of its
 //   type's range, where neither it nor the products lose bits; the scores take both back. Values'
-//   nibbles go the same way as fp16, the weights' powers of two and the output's last step taking
-//   theirs (128 us; 139 with codes brought to code - 8 in fp16 first). Codes are never negative, and
-//   the matrix instruction cuts off where it adds, so the sums would drift as they grow: every
-//   fourth step what a lane's first channel has summed is taken off all of its channels and kept
-//   beside them.
+//   nibbles go the same way as fp16, all at bits 4 to 7 (code 2^-20): the instruction adds its
+//   products on a grid set by their operands' exponent fields, and at bits 0 to 3, with the field of
+//   a number 64 to 1024 times larger, it cuts four bits more off (122 us; 119 without the shifts).
+// * sums of codes do not drift: tokens 8 to 15 of a run count down from the group's top, k = (m + 15 s)
+//   - s (15 - c), for nothing (the complement is part of the mask, the sign of the step), so
+//   that what is summed has no common sign. The instruction still cuts off where it adds, so every
+//   eighth step the sums are set aside: added, rounded to nearest, to sums in shared memory. The
+//   result's error is then some units of 2^-24 of the values at any length (of fp16 outputs over 8192
+//   tokens 0.8 % are not the nearest, 0.3 % of those of 32-bit operations throughout; 20 %
+//   with codes counted up and half the bits cut), for the same time.
 // * the weights p_t s_t are the only rounded operand: two fp16 numbers each, high and low, 22 bits
 //   in all (one alone would add an error the size of the result's own rounding). They are scaled by
 //   a power of two that puts the largest step near 2^11, so that a weight keeps its leading bits
@@ -25,8 +30,8 @@
 // * the running maximum and that scale move only when a score exceeds the reference by 2^4 or a
 //   step its bound, so that the output is rarely rescaled and the warp rarely reduces.
 // * a lane's two query rows go through paired 32-bit operations (127 -> 123 us).
-// Each warp walks its own stretch of tokens, a step of 32 or 64 at a time, through a ring of three
-// steps in shared memory that bulk asynchronous copies fill: a run's bytes are already in the order
+// Each warp walks its own stretch of tokens, a step of 32 or 64 at a time, through a ring of two
+// or three steps in shared memory that bulk asynchronous copies fill: a run's bytes are already in the order
 // of the operand's registers. The token range is cut over CTAs (blockIdx.x) and over a CTA's four
 // warps; the parts are joined through shared memory and, between CTAs, through the cluster's shared
 // memory (up to eight) or by kv4_join_kernel, always in a fixed order.
@@ -86,6 +91,12 @@ __device__ __forceinline__ void kv_mma<__half>(float (&d)[4], const uint32_t (&a
 __device__ __forceinline__ uint32_t kv_pair_bare(uint32_t w, int p) {
   if (p & 2) w >>= 8;
   return w & (p & 1 ? 0x00f000f0u : 0x000f000fu);
+}
+// A lane's word of values as the left operand: sixteen times the code of tokens 0 to 7 (channels g,
+// then g + 8), sixteen times 15 - code of tokens 8 to 15.
+__device__ __forceinline__ void kv_values(uint32_t (&a)[4], uint32_t w) {
+  constexpr uint32_t kMask = 0x00f000f0u;
+  a[0] = w << 4 & kMask, a[1] = w & kMask, a[2] = ~(w >> 4) & kMask, a[3] = ~(w >> 8) & kMask;
 }
 // Where a query row's largest entry is put (its exponent), and what its type makes of the code 1
 // (the negative exponent).
@@ -157,18 +168,25 @@ __device__ __forceinline__ void mbar_expect(uint32_t mbar, uint32_t bytes) {
   asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(mbar), "r"(bytes) : "memory");
 }
 
-constexpr int kKvStages = 3;
+// Steps in a warp's ring. With eight query rows two leave room for the sums set aside of four CTAs
+// an SM, and cost nothing (64 x 8192 tokens 121.3 us, with three 122.1).
+__host__ __device__ constexpr int kv_stages(int nt) { return nt == 1 ? 2 : 3; }
+constexpr int kKvAside = 8;  // steps between settings-aside (every fourth: 1.8 us more of 123)
 // CTAs to an SM that registers are kept for. Four (128 registers) beat three wherever little spills
 // (64 x 8192 tokens, one group: 126 against 138 us); four groups of steps would (125 against 111
 // us).
 __host__ __device__ constexpr int kv_ctas(int groups, int nt) { return nt > 1 ? 2 : groups < 4 ? 4 : 3; }
-// Dynamic shared memory: the warps' rings, reused at the end for their parts of the output.
+// Dynamic shared memory: the warps' rings, reused at the end for their parts of the output, and
+// behind them the sums set aside.
 __host__ __device__ constexpr int kv_stage_bytes(int dim, int groups, bool brief) {
   return kv_runs(dim, brief) * (16 * dim + 128 * groups);
 }
-__host__ __device__ constexpr int kv_smem_bytes(int dim, int groups, int nt, bool brief) {
-  const int ring = kKvWarps * kKvStages * kv_stage_bytes(dim, groups, brief), parts = kKvWarps * 8 * nt * (dim + 4) * 4;
+__host__ __device__ constexpr int kv_ring_bytes(int dim, int groups, int nt, bool brief) {
+  const int ring = kKvWarps * kv_stages(nt) * kv_stage_bytes(dim, groups, brief), parts = kKvWarps * 8 * nt * (dim + 4) * 4;
   return ring > parts ? ring : parts;
+}
+__host__ __device__ constexpr int kv_smem_bytes(int dim, int groups, int nt, bool brief) {
+  return kv_ring_bytes(dim, groups, nt, brief) + kKvWarps * 8 * nt * dim * 4;
 }
 
 template <typename T, int kDim, int kGroups, int kNT, bool kBrief>
@@ -180,13 +198,14 @@ __global__ void __launch_bounds__(32 * kKvWarps, kv_ctas(kGroups, kNT)) kv4_atte
   constexpr int kVC = kDim / 64;           // 16-byte pieces of a lane's value codes, for 16 tokens
   constexpr int kRuns = kv_runs(kDim, kBrief), kUnit = 16 * kRuns;
   constexpr int kRunBytes = 16 * kDim + 128 * kGroups, kStage = kRuns * kRunBytes;
+  constexpr int kStages = kv_stages(kNT);
   constexpr float kNone = -INFINITY;
   extern __shared__ __align__(128) unsigned char s_ring[];
   __shared__ uint2 s_q[kNT][kSteps][32];
   __shared__ float s_qsum[kKvWarps][kNT][8][kGroups];
   __shared__ unsigned s_qtop[kKvWarps][kNT][8];
   __shared__ float2 s_ml[kKvWarps][kRows];
-  __shared__ uint64_t s_full[kKvWarps][kKvStages];
+  __shared__ uint64_t s_full[kKvWarps][kStages];
   __shared__ int s_bad;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -195,7 +214,7 @@ __global__ void __launch_bounds__(32 * kKvWarps, kv_ctas(kGroups, kNT)) kv4_atte
 
   if (threadIdx.x == 0) s_bad = 0;
   if (lane == 0) {
-    for (int i = 0; i < kKvStages; ++i) mbar_init(&s_full[warp][i], 1);
+    for (int i = 0; i < kStages; ++i) mbar_init(&s_full[warp][i], 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     fence_async_smem();
   }
@@ -247,7 +266,7 @@ __global__ void __launch_bounds__(32 * kKvWarps, kv_ctas(kGroups, kNT)) kv4_atte
 
   // The ring. Lane i of `page` holds the page of run `page_base` + i, -1 past the range or where
   // the table is wrong.
-  unsigned char* ring = s_ring + warp * (kKvStages * kStage);
+  unsigned char* ring = s_ring + warp * (kStages * kStage);
   const int page_runs = P.sh.page / 16, page_shift = P.sh.shift - 4;
   const int last_run = min(u_hi * kRuns, (len + 15) / 16);
   int page_base = u * kRuns, page = -1;
@@ -291,7 +310,7 @@ __global__ void __launch_bounds__(32 * kKvWarps, kv_ctas(kGroups, kNT)) kv4_atte
   };
   const int count = u_hi - u;
   if (count > 0) look_up();
-  for (int i = 0; i < kKvStages && i < count; ++i) issue(u + i, i);
+  for (int i = 0; i < kStages && i < count; ++i) issue(u + i, i);
 
   // Queries as the right operand. The warps share the work; first each row's largest entry and each
   // group's sum.
@@ -357,8 +376,8 @@ __global__ void __launch_bounds__(32 * kKvWarps, kv_ctas(kGroups, kNT)) kv4_atte
   }
   __syncthreads();
 
-  float o[kNT][kSteps][4] = {};  // scaled by `unit`, less `off`; [2] and [3] are 16 times that
-  float2 sum[kNT] = {}, lows[kNT][kGroups] = {}, off[kNT][kGroups] = {};
+  float o[kNT][kSteps][4] = {};  // scaled by `unit`
+  float2 sum[kNT] = {}, lows[kNT][kGroups] = {};
   // Weights are 2^(score + less); bound is where a score moves that reference. cap bounds
   // the steps, unit scales them.
   float2 less[kNT] = {};
@@ -366,254 +385,269 @@ __global__ void __launch_bounds__(32 * kKvWarps, kv_ctas(kGroups, kNT)) kv4_atte
 #pragma unroll
   for (int n = 0; n < kNT; ++n) bound[n][0] = bound[n][1] = kNone;
 
-  bool ok = true;
+  // This lane's sums set aside, 32 lanes apart; `aside` once there are some.
+  float4* apart = reinterpret_cast<float4*>(s_ring + kv_ring_bytes(kDim, kGroups, kNT, kBrief)) + warp * (kRows * kDim / 4) + lane;
+  bool ok = true, aside = false;
   int stage = 0, turn = 0;
-  for (int k = 0; k < count; ++k, ++u) {
-    const int tok0 = u * kUnit;
-    const unsigned char* runs = ring + stage * kStage;
-    const unsigned gone = missing >> (8 * stage) & ((1u << kRuns) - 1);
-    ok = ok && __all_sync(kFullMask, mbar_wait(&s_full[warp][stage], turn));
-    if (!ok) break;
-    // Scores: s[i][n][h] holds token tok0 + 16 i + 8 h + g against rows 8 n + 2 t
-    // and the next.
-    float2 s[kRuns][kNT][2];
-    {
-      float acc[kRuns][kNT][4];
-      uint32_t kc[kRuns][2][kKW];
-#pragma unroll
-      for (int i = 0; i < kRuns; ++i)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) kv_load(kc[i][h], runs + i * kRunBytes + h * (4 * kDim) + lane * (kDim / 8));
-#pragma unroll
-      for (int gr = 0; gr < kGroups; ++gr) {
+  for (int k = 0; ok && k < count;) {
+    const int pause = min(count, k + kKvAside);
+    for (; k < pause; ++k, ++u) {
+      const int tok0 = u * kUnit;
+      const unsigned char* runs = ring + stage * kStage;
+      const unsigned gone = missing >> (8 * stage) & ((1u << kRuns) - 1);
+      ok = ok && __all_sync(kFullMask, mbar_wait(&s_full[warp][stage], turn));
+      if (!ok) break;
+      // Scores: s[i][n][h] holds token tok0 + 16 i + 8 h + g against rows 8 n + 2 t
+      // and the next.
+      float2 s[kRuns][kNT][2];
+      {
+        float acc[kRuns][kNT][4];
+        uint32_t kc[kRuns][2][kKW];
 #pragma unroll
         for (int i = 0; i < kRuns; ++i)
 #pragma unroll
-          for (int n = 0; n < kNT; ++n) acc[i][n][0] = acc[i][n][1] = acc[i][n][2] = acc[i][n][3] = 0.f;
-#pragma unroll
-        for (int j = gr * kPer; j < (gr + 1) * kPer; ++j) {
-          const int p = 2 * (j & 1);
-          uint2 q[kNT];
-#pragma unroll
-          for (int n = 0; n < kNT; ++n) q[n] = s_q[n][j][lane];
-#pragma unroll
-          for (int i = 0; i < kRuns; ++i) {
-            const uint32_t a[4] = {kv_pair_bare(kc[i][0][j >> 1], p), kv_pair_bare(kc[i][1][j >> 1], p),
-                                   kv_pair_bare(kc[i][0][j >> 1], p + 1), kv_pair_bare(kc[i][1][j >> 1], p + 1)};
-#pragma unroll
-            for (int n = 0; n < kNT; ++n) kv_mma<T>(acc[i][n], a, q[n].x, q[n].y);
-          }
-        }
-#pragma unroll
-        for (int i = 0; i < kRuns; ++i)
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const float2 k = kv_step_low<T>(
-                *reinterpret_cast<const uint32_t*>(runs + i * kRunBytes + 16 * kDim + ((g + 8 * h) * kGroups + gr) * 4));
-#pragma unroll
-            for (int n = 0; n < kNT; ++n) {
-              const float2 kx = make_float2(k.x, k.x), ky = make_float2(k.y, k.y);
-              const float2 low = gr ? __ffma2_rn(ky, qsum[n][gr], s[i][n][h]) : __fmul2_rn(ky, qsum[n][gr]);
-              s[i][n][h] = __ffma2_rn(kx, __fmul2_rn(make_float2(acc[i][n][2 * h], acc[i][n][2 * h + 1]), back[n]), low);
-            }
-          }
-      }
-    }
-    uint32_t vp[kRuns][2][kGroups];
-#pragma unroll
-    for (int i = 0; i < kRuns; ++i)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) kv_load(vp[i][h], runs + i * kRunBytes + 16 * kDim + 64 * kGroups + (g + 8 * h) * (4 * kGroups));
-    const bool full = !gone && tok0 >= in_lo && tok0 + kUnit <= in_hi;  // every row sees every token
-    uint32_t seen[kNT];
-    if (!full) {
-#pragma unroll
-      for (int n = 0; n < kNT; ++n) {
-        int lo[2], hi[2];
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          lo[c] = __shfl_sync(kFullMask, my_lo, 8 * n + 2 * t + c);
-          hi[c] = __shfl_sync(kFullMask, my_hi, 8 * n + 2 * t + c);
-        }
-        seen[n] = 0;
-#pragma unroll
-        for (int i = 0; i < kRuns; ++i)
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const int tok = tok0 + 16 * i + 8 * h + g;
-            const bool x = tok >= lo[0] && tok < hi[0] && !(gone >> i & 1);
-            const bool y = tok >= lo[1] && tok < hi[1] && !(gone >> i & 1);
-            seen[n] |= (x ? 1u : 0u) << (4 * i + 2 * h) | (y ? 2u : 0u) << (4 * i + 2 * h);
-            if (!x) s[i][n][h].x = kNone;
-            if (!y) s[i][n][h].y = kNone;
-            if (n == 0 && (tok < all_lo || tok >= all_hi || (gone >> i & 1)))
-#pragma unroll
-              for (int gr = 0; gr < kGroups; ++gr) vp[i][h][gr] = 0;  // seen by no row: may hold anything
-          }
-      }
-    }
-    float2 val[kRuns][2][kGroups];  // step and minimum
-    float up[kNT][2], steps = 0.f;
-#pragma unroll
-    for (int i = 0; i < kRuns; ++i)
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
+          for (int h = 0; h < 2; ++h) kv_load(kc[i][h], runs + i * kRunBytes + h * (4 * kDim) + lane * (kDim / 8));
 #pragma unroll
         for (int gr = 0; gr < kGroups; ++gr) {
-          val[i][h][gr] = kv_step_low<T>(vp[i][h][gr]);
-          steps = fmaxf(steps, val[i][h][gr].x);
-        }
-    bool move = steps > cap;
 #pragma unroll
-    for (int n = 0; n < kNT; ++n) {
-      up[n][0] = s[0][n][0].x;
-      up[n][1] = s[0][n][0].y;
+          for (int i = 0; i < kRuns; ++i)
 #pragma unroll
-      for (int i = 0; i < kRuns; ++i)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          up[n][0] = fmaxf(up[n][0], s[i][n][h].x);
-          up[n][1] = fmaxf(up[n][1], s[i][n][h].y);
-        }
-      move = move || up[n][0] > bound[n][0] || up[n][1] > bound[n][1];
-    }
-    if (__any_sync(kFullMask, move)) {
-      steps = fmaxf(steps, cap);
-#pragma unroll
-      for (int x = 1; x < 32; x <<= 1) steps = fmaxf(steps, __shfl_xor_sync(kFullMask, steps, x));
-      float ratio = 1.f;
-      if (steps > cap) {  // the power of two above the largest step, and the scale that puts it at 2^11
-        const int e = max(-100, min(126, (int)(__float_as_uint(steps) >> 23) - 126));
-        cap = __int_as_float((e + 127) << 23);
-        const float fresh = __int_as_float((kKvStepExp - e + 127) << 23);
-        ratio = fresh / unit;
-        unit = fresh;
-      }
-#pragma unroll
-      for (int n = 0; n < kNT; ++n) {
-        float keep[2];
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-#pragma unroll
-          for (int x = 4; x < 32; x <<= 1) up[n][c] = fmaxf(up[n][c], __shfl_xor_sync(kFullMask, up[n][c], x));
-          const float last = bound[n][c] - kKvLazy, next = fmaxf(up[n][c], last);
-          keep[c] = next == kNone ? 0.f : kv_exp2(last - next);
-          bound[n][c] = next + kKvLazy;
-          // A row that has seen nothing has the reference -inf: its weights, 2^-inf, come from any
-          // finite one.
-          (c ? less[n].y : less[n].x) = next == kNone ? 0.f : -next;
-        }
-        sum[n] = make_float2(sum[n].x * keep[0], sum[n].y * keep[1]);
-#pragma unroll
-        for (int gr = 0; gr < kGroups; ++gr) {
-          lows[n][gr] = make_float2(lows[n][gr].x * keep[0], lows[n][gr].y * keep[1]);
-          off[n][gr] = make_float2(off[n][gr].x * keep[0] * ratio, off[n][gr].y * keep[1] * ratio);
-        }
-#pragma unroll
-        for (int j = 0; j < kSteps; ++j)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) o[n][j][e] *= keep[e & 1] * ratio;
-      }
-    }
-    // Weights and output; kAll: every row sees every token (no tests in the common case).
-    auto finish = [&](auto all) {
-      constexpr bool kAll = decltype(all)::value;
-#pragma unroll
-      for (int i = 0; i < kRuns; ++i) {
-        uint32_t vc[kVC][4];
-#pragma unroll
-        for (int c = 0; c < kVC; ++c) kv_load(vc[c], runs + i * kRunBytes + 8 * kDim + c * 512 + lane * 16);
-#pragma unroll
-        for (int n = 0; n < kNT; ++n)
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const float2 e = __fadd2_rn(s[i][n][h], less[n]), p = make_float2(kv_exp2(e.x), kv_exp2(e.y));
-            sum[n] = __fadd2_rn(sum[n], p);
-            s[i][n][h] = p;
-          }
-#pragma unroll
-        for (int gr = 0; gr < kGroups; ++gr) {
-          uint32_t w[2][kNT][2];
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const float scaled = val[i][h][gr].x * unit;
-#pragma unroll
-            for (int n = 0; n < kNT; ++n) {
-              const float2 p = s[i][n][h];
-              float2 x = __fmul2_rn(p, make_float2(scaled, scaled));
-              if constexpr (kAll) {
-                lows[n][gr] = __ffma2_rn(p, make_float2(val[i][h][gr].y, val[i][h][gr].y), lows[n][gr]);
-              } else {  // what a row does not see may be NaN
-                if (seen[n] >> (4 * i + 2 * h) & 1) lows[n][gr].x = fmaf(p.x, val[i][h][gr].y, lows[n][gr].x);
-                else x.x = 0.f;
-                if (seen[n] >> (4 * i + 2 * h) & 2) lows[n][gr].y = fmaf(p.y, val[i][h][gr].y, lows[n][gr].y);
-                else x.y = 0.f;
-              }
-              const uint32_t high = kv_pack(x);
-              w[0][n][h] = kv_transpose(high);
-              const float2 top = __half22float2(__hneg2(reinterpret_cast<const __half2&>(high)));
-              w[1][n][h] = kv_transpose(kv_pack(__fadd2_rn(x, top)));
-            }
-          }
+            for (int n = 0; n < kNT; ++n) acc[i][n][0] = acc[i][n][1] = acc[i][n][2] = acc[i][n][3] = 0.f;
 #pragma unroll
           for (int j = gr * kPer; j < (gr + 1) * kPer; ++j) {
-            const uint32_t word = vc[j >> 2][j & 3];
-            const uint32_t a[4] = {kv_pair_bare(word, 0), kv_pair_bare(word, 1), kv_pair_bare(word, 2), kv_pair_bare(word, 3)};
+            const int p = 2 * (j & 1);
+            uint2 q[kNT];
 #pragma unroll
-            for (int n = 0; n < kNT; ++n)
+            for (int n = 0; n < kNT; ++n) q[n] = s_q[n][j][lane];
 #pragma unroll
-              for (int half = 0; half < 2; ++half) kv_mma<__half>(o[n][j], a, w[half][n][0], w[half][n][1]);
+            for (int i = 0; i < kRuns; ++i) {
+              const uint32_t a[4] = {kv_pair_bare(kc[i][0][j >> 1], p), kv_pair_bare(kc[i][1][j >> 1], p),
+                                     kv_pair_bare(kc[i][0][j >> 1], p + 1), kv_pair_bare(kc[i][1][j >> 1], p + 1)};
+#pragma unroll
+              for (int n = 0; n < kNT; ++n) kv_mma<T>(acc[i][n], a, q[n].x, q[n].y);
+            }
+          }
+#pragma unroll
+          for (int i = 0; i < kRuns; ++i)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const float2 k = kv_step_low<T>(
+                  *reinterpret_cast<const uint32_t*>(runs + i * kRunBytes + 16 * kDim + ((g + 8 * h) * kGroups + gr) * 4));
+#pragma unroll
+              for (int n = 0; n < kNT; ++n) {
+                const float2 kx = make_float2(k.x, k.x), ky = make_float2(k.y, k.y);
+                const float2 low = gr ? __ffma2_rn(ky, qsum[n][gr], s[i][n][h]) : __fmul2_rn(ky, qsum[n][gr]);
+                s[i][n][h] = __ffma2_rn(kx, __fmul2_rn(make_float2(acc[i][n][2 * h], acc[i][n][2 * h + 1]), back[n]), low);
+              }
+            }
+        }
+      }
+      uint32_t vp[kRuns][2][kGroups];
+#pragma unroll
+      for (int i = 0; i < kRuns; ++i)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) kv_load(vp[i][h], runs + i * kRunBytes + 16 * kDim + 64 * kGroups + (g + 8 * h) * (4 * kGroups));
+      const bool full = !gone && tok0 >= in_lo && tok0 + kUnit <= in_hi;  // every row sees every token
+      uint32_t seen[kNT];
+      if (!full) {
+#pragma unroll
+        for (int n = 0; n < kNT; ++n) {
+          int lo[2], hi[2];
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            lo[c] = __shfl_sync(kFullMask, my_lo, 8 * n + 2 * t + c);
+            hi[c] = __shfl_sync(kFullMask, my_hi, 8 * n + 2 * t + c);
+          }
+          seen[n] = 0;
+#pragma unroll
+          for (int i = 0; i < kRuns; ++i)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const int tok = tok0 + 16 * i + 8 * h + g;
+              const bool x = tok >= lo[0] && tok < hi[0] && !(gone >> i & 1);
+              const bool y = tok >= lo[1] && tok < hi[1] && !(gone >> i & 1);
+              seen[n] |= (x ? 1u : 0u) << (4 * i + 2 * h) | (y ? 2u : 0u) << (4 * i + 2 * h);
+              if (!x) s[i][n][h].x = kNone;
+              if (!y) s[i][n][h].y = kNone;
+              if (n == 0 && (tok < all_lo || tok >= all_hi || (gone >> i & 1)))
+#pragma unroll
+                for (int gr = 0; gr < kGroups; ++gr) vp[i][h][gr] = 0;  // seen by no row: may hold anything
+            }
+        }
+      }
+      float2 val[kRuns][2][kGroups];  // step and minimum
+      float up[kNT][2], steps = 0.f;
+#pragma unroll
+      for (int i = 0; i < kRuns; ++i)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int gr = 0; gr < kGroups; ++gr) {
+            val[i][h][gr] = kv_step_low<T>(vp[i][h][gr]);
+            steps = fmaxf(steps, val[i][h][gr].x);
+            if (h) val[i][h][gr].y = fmaf(15.f, val[i][h][gr].x, val[i][h][gr].y);  // codes count down from here
+          }
+      bool move = steps > cap;
+#pragma unroll
+      for (int n = 0; n < kNT; ++n) {
+        up[n][0] = s[0][n][0].x;
+        up[n][1] = s[0][n][0].y;
+#pragma unroll
+        for (int i = 0; i < kRuns; ++i)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            up[n][0] = fmaxf(up[n][0], s[i][n][h].x);
+            up[n][1] = fmaxf(up[n][1], s[i][n][h].y);
+          }
+        move = move || up[n][0] > bound[n][0] || up[n][1] > bound[n][1];
+      }
+      if (__any_sync(kFullMask, move)) {
+        steps = fmaxf(steps, cap);
+#pragma unroll
+        for (int x = 1; x < 32; x <<= 1) steps = fmaxf(steps, __shfl_xor_sync(kFullMask, steps, x));
+        float ratio = 1.f;
+        if (steps > cap) {  // the power of two above the largest step, and the scale that puts it at 2^11
+          const int e = max(-100, min(126, (int)(__float_as_uint(steps) >> 23) - 126));
+          cap = __int_as_float((e + 127) << 23);
+          const float fresh = __int_as_float((kKvStepExp - e + 127) << 23);
+          ratio = fresh / unit;
+          unit = fresh;
+        }
+#pragma unroll
+        for (int n = 0; n < kNT; ++n) {
+          float keep[2];
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+#pragma unroll
+            for (int x = 4; x < 32; x <<= 1) up[n][c] = fmaxf(up[n][c], __shfl_xor_sync(kFullMask, up[n][c], x));
+            const float last = bound[n][c] - kKvLazy, next = fmaxf(up[n][c], last);
+            keep[c] = next == kNone ? 0.f : kv_exp2(last - next);
+            bound[n][c] = next + kKvLazy;
+            // A row that has seen nothing has the reference -inf: its weights, 2^-inf, come from any
+            // finite one.
+            (c ? less[n].y : less[n].x) = next == kNone ? 0.f : -next;
+          }
+          sum[n] = make_float2(sum[n].x * keep[0], sum[n].y * keep[1]);
+#pragma unroll
+          for (int gr = 0; gr < kGroups; ++gr) lows[n][gr] = make_float2(lows[n][gr].x * keep[0], lows[n][gr].y * keep[1]);
+#pragma unroll
+          for (int j = 0; j < kSteps; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[n][j][e] *= keep[e & 1] * ratio;
+          if (aside) {
+#pragma unroll
+            for (int j = 0; j < kSteps; ++j) {
+              float4 a = apart[32 * (n * kSteps + j)];
+              a.x *= keep[0] * ratio, a.y *= keep[1] * ratio, a.z *= keep[0] * ratio, a.w *= keep[1] * ratio;
+              apart[32 * (n * kSteps + j)] = a;
+            }
           }
         }
       }
-    };
-    if (full) finish(std::true_type{});
-    else finish(std::false_type{});
-    if ((k & 3) == 3) {  // what a group's first tile has summed is set aside, for all of its tiles
+      // Weights and output; kAll: every row sees every token (no tests in the common case).
+      auto finish = [&](auto all) {
+        constexpr bool kAll = decltype(all)::value;
+#pragma unroll
+        for (int i = 0; i < kRuns; ++i) {
+          uint32_t vc[kVC][4];
+#pragma unroll
+          for (int c = 0; c < kVC; ++c) kv_load(vc[c], runs + i * kRunBytes + 8 * kDim + c * 512 + lane * 16);
+#pragma unroll
+          for (int n = 0; n < kNT; ++n)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const float2 e = __fadd2_rn(s[i][n][h], less[n]), p = make_float2(kv_exp2(e.x), kv_exp2(e.y));
+              sum[n] = __fadd2_rn(sum[n], p);
+              s[i][n][h] = p;
+            }
+#pragma unroll
+          for (int gr = 0; gr < kGroups; ++gr) {
+            uint32_t w[2][kNT][2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const float scaled = val[i][h][gr].x * (h ? -unit : unit);
+#pragma unroll
+              for (int n = 0; n < kNT; ++n) {
+                const float2 p = s[i][n][h];
+                float2 x = __fmul2_rn(p, make_float2(scaled, scaled));
+                if constexpr (kAll) {
+                  lows[n][gr] = __ffma2_rn(p, make_float2(val[i][h][gr].y, val[i][h][gr].y), lows[n][gr]);
+                } else {  // what a row does not see may be NaN
+                  if (seen[n] >> (4 * i + 2 * h) & 1) lows[n][gr].x = fmaf(p.x, val[i][h][gr].y, lows[n][gr].x);
+                  else x.x = 0.f;
+                  if (seen[n] >> (4 * i + 2 * h) & 2) lows[n][gr].y = fmaf(p.y, val[i][h][gr].y, lows[n][gr].y);
+                  else x.y = 0.f;
+                }
+                const uint32_t high = kv_pack(x);
+                w[0][n][h] = kv_transpose(high);
+                const float2 top = __half22float2(__hneg2(reinterpret_cast<const __half2&>(high)));
+                w[1][n][h] = kv_transpose(kv_pack(__fadd2_rn(x, top)));
+              }
+            }
+#pragma unroll
+            for (int j = gr * kPer; j < (gr + 1) * kPer; ++j) {
+              const uint32_t word = vc[j >> 2][j & 3];
+              uint32_t a[4];
+              kv_values(a, word);
+#pragma unroll
+              for (int n = 0; n < kNT; ++n)
+#pragma unroll
+                for (int half = 0; half < 2; ++half) kv_mma<__half>(o[n][j], a, w[half][n][0], w[half][n][1]);
+            }
+          }
+        }
+      };
+      if (full) finish(std::true_type{});
+      else finish(std::false_type{});
+      __syncwarp();  // every lane has read this stage
+      if (k + kStages < count) issue(u + kStages, stage);
+      if (++stage == kStages) {
+        stage = 0;
+        turn ^= 1;
+      }
+    }
+    if (ok && k < count) {  // set the sums aside
 #pragma unroll
       for (int n = 0; n < kNT; ++n)
 #pragma unroll
-        for (int gr = 0; gr < kGroups; ++gr) {
-          const float2 d = make_float2(o[n][gr * kPer][0], o[n][gr * kPer][1]);
-          off[n][gr] = make_float2(off[n][gr].x + d.x, off[n][gr].y + d.y);
-#pragma unroll
-          for (int j = gr * kPer; j < (gr + 1) * kPer; ++j) {
-            o[n][j][0] -= d.x;
-            o[n][j][1] -= d.y;
-            o[n][j][2] = fmaf(-16.f, d.x, o[n][j][2]);
-            o[n][j][3] = fmaf(-16.f, d.y, o[n][j][3]);
-          }
+        for (int j = 0; j < kSteps; ++j) {
+          float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (aside) a = apart[32 * (n * kSteps + j)];
+          a.x += o[n][j][0], a.y += o[n][j][1], a.z += o[n][j][2], a.w += o[n][j][3];
+          apart[32 * (n * kSteps + j)] = a;
+          o[n][j][0] = o[n][j][1] = o[n][j][2] = o[n][j][3] = 0.f;
         }
-    }
-    __syncwarp();  // every lane has read this stage
-    if (k + kKvStages < count) issue(u + kKvStages, stage);
-    if (++stage == kKvStages) {
-      stage = 0;
-      turn ^= 1;
+      aside = true;
     }
   }
   if (!ok) {
     // A copy did not arrive in time: nothing is written, and what is under way is waited for (with
     // a limit) first.
-    for (int i = 0; i < kKvStages; ++i) mbar_wait(&s_full[warp][i], i < stage ? turn ^ 1 : turn);
+    for (int i = 0; i < kStages; ++i) mbar_wait(&s_full[warp][i], i < stage ? turn ^ 1 : turn);
     s_bad = 1;
+  }
+  if (aside) {
+#pragma unroll
+    for (int n = 0; n < kNT; ++n)
+#pragma unroll
+      for (int j = 0; j < kSteps; ++j) {
+        const float4 a = apart[32 * (n * kSteps + j)];
+        o[n][j][0] += a.x, o[n][j][1] += a.y, o[n][j][2] += a.z, o[n][j][3] += a.w;
+      }
   }
   __syncthreads();  // the rings are free
   float(*s_o)[kRows][kDim + 4] = reinterpret_cast<float(*)[kRows][kDim + 4]>(s_ring);
 
   const float lower = 1.f / unit;
-  constexpr float kOne = 0x1p24f;  // of the bare codes
+  constexpr float kOne = 0x1p20f;  // what a code's unit counts less in the operand
   // The warps' parts: o[n][j][e] is channel 16 j + g + 8 (e / 2) of row 8 n + 2 t + e % 2.
 #pragma unroll
   for (int n = 0; n < kNT; ++n)
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
-      float l = c ? sum[n].y : sum[n].x, add[kGroups], aside[kGroups];
+      float l = c ? sum[n].y : sum[n].x, add[kGroups];
 #pragma unroll
-      for (int gr = 0; gr < kGroups; ++gr) {
-        add[gr] = c ? lows[n][gr].y : lows[n][gr].x;
-        aside[gr] = c ? off[n][gr].y : off[n][gr].x;
-      }
+      for (int gr = 0; gr < kGroups; ++gr) add[gr] = c ? lows[n][gr].y : lows[n][gr].x;
 #pragma unroll
       for (int x = 4; x < 32; x <<= 1) {
         l += __shfl_xor_sync(kFullMask, l, x);
@@ -623,9 +657,8 @@ __global__ void __launch_bounds__(32 * kKvWarps, kv_ctas(kGroups, kNT)) kv4_atte
       if (g == 0) s_ml[warp][8 * n + 2 * t + c] = make_float2(bound[n][c] - kKvLazy, l);
 #pragma unroll
       for (int j = 0; j < kSteps; ++j) {
-        const float first = aside[j / kPer] + o[n][j][c], second = fmaf(0.0625f, o[n][j][2 + c], aside[j / kPer]);
-        s_o[warp][8 * n + 2 * t + c][16 * j + g] = fmaf(first * kOne, lower, add[j / kPer]);
-        s_o[warp][8 * n + 2 * t + c][16 * j + g + 8] = fmaf(second * kOne, lower, add[j / kPer]);
+        s_o[warp][8 * n + 2 * t + c][16 * j + g] = fmaf(o[n][j][c] * kOne, lower, add[j / kPer]);
+        s_o[warp][8 * n + 2 * t + c][16 * j + g + 8] = fmaf(o[n][j][2 + c] * kOne, lower, add[j / kPer]);
       }
     }
   __syncthreads();

@@ -1,0 +1,43 @@
+"""The operators on 8- and 4-bit data at the ends of their ranges: how near long sums are to the 64-bit result,
+numbers at either end of a type, indexes that no query needs, captured calls.
+
+Each check derives its own tolerance; U is the unit roundoff of a type.
+"""
+
+import pytest
+import torch
+from test_gpu_quant import HF, _randn, _values
+
+import qr_v2_b200_kernel_b200 as qr
+
+pytestmark = pytest.mark.gpu
+
+
+def _half_step(x):
+    """The spacing of fp16 numbers at x."""
+    return torch.exp2(torch.floor(torch.log2(x.abs().clamp_min(2.0**-14))) - 10)
+
+
+@pytest.mark.parametrize("batch, heads, share, tokens, dim, group", [
+    (4, 2, 8, 8192, 128, 128), (64, 8, 8, 8192, 128, 128), (64, 8, 8, 8192, 128, 32), (64, 8, 4, 8192, 64, 64), (20, 2, 13, 8192, 128, 64),
+    (2, 8, 8, 65536, 128, 128), (64, 8, 8, 65536, 128, 128), (64, 8, 1, 65536, 64, 32)])
+def test_attention_sums_hold_32_bits_at_any_length(batch, heads, share, tokens, dim, group):
+    """An output that is off by e before its rounding misses the nearest fp16 number with the probability e / step. One
+    unit of 2^-24 of the values' weighted mean size is allowed for e, what a handful of roundings of 32-bit sums come to."""
+    pages = -(-tokens // 64)
+    cache = qr.kv4_cache(pages, 64, heads, dim, group, HF)
+    k, v = _randn(tokens, heads, dim, seed=80, dtype=HF), _randn(tokens, heads, dim, seed=81, dtype=HF)
+    qr.kv4_write(cache, k, v, torch.arange(tokens, device="cuda"))
+    q = _randn(batch, 1, heads * share, dim, seed=82, dtype=HF)
+    table = torch.arange(pages, dtype=torch.int32, device="cuda").expand(batch, pages)  # one context, many questions
+    got = qr.kv4_attention(q, cache, table, torch.full((batch,), tokens, dtype=torch.int32, device="cuda"))
+    k, v = _values(cache)
+    missed, allowed, of = 0, 0.0, 0
+    for b in range(0, batch, max(1, batch // 4)):
+        p = (torch.einsum("hgd,thd->hgt", q[b, 0].double().unflatten(0, (heads, share)), k) * dim**-0.5).softmax(-1)
+        want = torch.einsum("hgt,thd->hgd", p, v).flatten(0, 1)
+        size = torch.einsum("hgt,thd->hgd", p, v.abs()).flatten(0, 1)
+        missed += (got[b, 0] != want.to(HF)).sum().item()
+        allowed += (size * 2.0**-24 / _half_step(want)).clamp_max(1).sum().item()
+        of += want.numel()
+    assert missed <= allowed, f"{missed} of {of} outputs are not the nearest, {allowed:.0f} allowed"
