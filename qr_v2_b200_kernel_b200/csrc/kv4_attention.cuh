@@ -378,12 +378,14 @@ __global__ void __launch_bounds__(32 * kKvWarps, kv_ctas(kGroups, kNT)) kv4_atte
 
   float o[kNT][kSteps][4] = {};  // scaled by `unit`
   float2 sum[kNT] = {}, lows[kNT][kGroups] = {};
-  // Weights are 2^(score + less); bound is where a score moves that reference. cap bounds
-  // the steps, unit scales them.
+  // Weights are 2^(score + less), the reference being -less; bound is where a score moves it: 4
+  // above, rounded down where scores are so large (so the reference cannot be had back from it), and
+  // -inf while nothing has been seen. cap bounds the steps, unit scales them.
   float2 less[kNT] = {};
   float bound[kNT][2], cap = 0.f, unit = 1.f;
 #pragma unroll
   for (int n = 0; n < kNT; ++n) bound[n][0] = bound[n][1] = kNone;
+  const auto reference = [&](int n, int c) { return bound[n][c] == kNone ? kNone : -(c ? less[n].y : less[n].x); };
 
   // This lane's sums set aside, 32 lanes apart; `aside` once there are some.
   float4* apart = reinterpret_cast<float4*>(s_ring + kv_ring_bytes(kDim, kGroups, kNT, kBrief)) + warp * (kRows * kDim / 4) + lane;
@@ -520,9 +522,9 @@ __global__ void __launch_bounds__(32 * kKvWarps, kv_ctas(kGroups, kNT)) kv4_atte
           for (int c = 0; c < 2; ++c) {
 #pragma unroll
             for (int x = 4; x < 32; x <<= 1) up[n][c] = fmaxf(up[n][c], __shfl_xor_sync(kFullMask, up[n][c], x));
-            const float last = bound[n][c] - kKvLazy, next = fmaxf(up[n][c], last);
+            const float last = reference(n, c), next = fmaxf(up[n][c], last);
             keep[c] = next == kNone ? 0.f : kv_exp2(last - next);
-            bound[n][c] = next + kKvLazy;
+            bound[n][c] = __fadd_rd(next, kKvLazy);
             // A row that has seen nothing has the reference -inf: its weights, 2^-inf, come from any
             // finite one.
             (c ? less[n].y : less[n].x) = next == kNone ? 0.f : -next;
@@ -654,7 +656,7 @@ __global__ void __launch_bounds__(32 * kKvWarps, kv_ctas(kGroups, kNT)) kv4_atte
 #pragma unroll
         for (int gr = 0; gr < kGroups; ++gr) add[gr] += __shfl_xor_sync(kFullMask, add[gr], x);
       }
-      if (g == 0) s_ml[warp][8 * n + 2 * t + c] = make_float2(bound[n][c] - kKvLazy, l);
+      if (g == 0) s_ml[warp][8 * n + 2 * t + c] = make_float2(reference(n, c), l);
 #pragma unroll
       for (int j = 0; j < kSteps; ++j) {
         s_o[warp][8 * n + 2 * t + c][16 * j + g] = fmaf(o[n][j][c] * kOne, lower, add[j / kPer]);

@@ -6,7 +6,7 @@ Each check derives its own tolerance; U is the unit roundoff of a type.
 
 import pytest
 import torch
-from test_gpu_quant import HF, _randn, _values
+from test_gpu_quant import BF, HF, U, _randn, _values
 
 import qr_v2_b200_kernel_b200 as qr
 
@@ -41,3 +41,35 @@ def test_attention_sums_hold_32_bits_at_any_length(batch, heads, share, tokens, 
         allowed += (size * 2.0**-24 / _half_step(want)).clamp_max(1).sum().item()
         of += want.numel()
     assert missed <= allowed, f"{missed} of {of} outputs are not the nearest, {allowed:.0f} allowed"
+
+
+@pytest.mark.parametrize("base, dtype", [(b, t) for b in (0, 24, 26, 27, 28) for t in (BF, HF) if b < 28 or t is BF])
+@pytest.mark.parametrize("batch, tokens", [(1, 640), (150, 640), (1, 9000)])
+def test_attention_of_scores_a_rounding_apart(base, batch, tokens, dtype):
+    """Scores 2^base + c 2^(base - 23) in the exponent's units, neighbours in 32 bits from 2^26 on eight or more apart:
+    the weights are powers of two, the sums exact, so an output has its own rounding and no more than 2^-20 of the
+    values' size beside it."""
+    page = 64
+    pages = -(-tokens // page)
+    cache = qr.kv4_cache(pages, page, 1, 64, 32, dtype)
+    unit = max(1.0, 2.0 ** (base - 23))
+    k, v = torch.zeros(tokens, 1, 64, dtype=dtype, device="cuda"), _randn(tokens, 1, 64, seed=83, dtype=dtype)
+    k[..., :32] = 2.0**12 if base else 0.0  # a constant group: q . k = 2^base
+    at = torch.arange(tokens, device="cuda")
+    climb = at * 4 // tokens + (at * 37 % 11 == 0).int()  # rises along the tokens, with single ones ahead
+    k[:, 0, 32], k[:, 0, 33], k[:, 0, 34] = climb.to(dtype) + 1, 0, 15  # codes 1 to 6 of steps of one
+    qr.kv4_write(cache, k, v, at)
+    q = torch.zeros(batch, 1, 3, 64, dtype=dtype, device="cuda")
+    q[..., 0] = 2.0 ** (base - 12) if base else 0.0
+    q[..., 32] = unit
+    q[:, :, 2, 32] = -unit
+    table = torch.arange(pages, dtype=torch.int32, device="cuda").expand(batch, pages)
+    lengths = torch.full((batch,), tokens, dtype=torch.int32, device="cuda")
+    scale = 0.6931472  # times log2(e), in 32 bits, is 1
+    assert float(torch.tensor(scale) * torch.tensor(1.4426950408889634)) == 1.0
+    got = qr.kv4_attention(q, cache, table, lengths, scale=scale)
+    keys, values = _values(cache)
+    s = torch.einsum("gd,td->gt", q[0, 0].double(), keys[:tokens, 0])
+    p = torch.exp2(s - s.amax(-1, keepdim=True))
+    want = (p / p.sum(-1, keepdim=True)) @ values[:tokens, 0]
+    assert bool(((got[:, 0].double() - want).abs() <= U[dtype] * want.abs() + 2.0**-20 * values.abs().max()).all())
