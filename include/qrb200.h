@@ -155,7 +155,9 @@ enum { QRB200_F32 = 0, QRB200_BF16 = 1, QRB200_F16 = 2 }; /* element types */
 /* Rows into 8 bits. h = x + residual (x alone when residual is NULL); t = h * weight (h alone when
  * weight is NULL); code_j = rint(t_j * 127 / a) with a = max |t_j|;
  * scale = a * (mean(h^2) + eps)^-1/2 / 127, so code * scale is the norm's output. h, rounded to
- * dtype, goes to h_out (rows x cols, contiguous; NULL exactly when residual is).
+ * dtype, goes to h_out (rows x cols, contiguous; NULL exactly when residual is). Finite rows of any
+ * size are normalised, through scaled squares where 32 bits do not hold theirs. h_out may be the residual itself, not
+ * overlap an input otherwise (rows off 16-byte boundaries that need scaled squares are then normalised from h as stored).
  * x, residual: rows x cols of dtype with row strides in elements; weight: cols of dtype or of
  * QRB200_F32; q: row stride q_stride bytes; scale: rows. cols <= 32768. A row with a NaN or an
  * infinity gets codes 0 and a NaN scale; one whose a is below 2^-100 gets codes and scale 0. */

@@ -121,15 +121,80 @@ __device__ __forceinline__ void store_pack(T* p, const T (&v)[kVec], int n) {
   }
 }
 
+// A row of finite numbers whose squares' sum left 32 bits' range, or whose h w did (top: infinity):
+// the same formulas on h 2^-k, with 2^k above both the largest |h| and sqrt(eps), which the scale
+// takes back. Out of line, from memory and element by element: the hot path keeps a branch to the end that
+// ordinary rows never take. All threads of the row come here; each takes what it holds there.
+// h_out (null: h is x, or stored already) is written last, as it may be the residual.
+template <typename T, typename W>
+__device__ __noinline__ void rows_outside(const T* x, const T* residual, T* h_out, const W* w, int8_t* q, float* scale, int cols,
+                                          float eps, bool over) {
+  constexpr int kVec = 16 / sizeof(T);
+  __shared__ float s_sum[32];
+  __shared__ unsigned s_top[32];
+  const int tid = threadIdx.x, threads = blockDim.x;
+  const auto each = [&](auto f) {
+#pragma unroll 1
+    for (int c = tid * kVec; c < cols; c += threads * kVec)
+#pragma unroll 1
+      for (int j = c; j < min(c + kVec, cols); ++j) f(j, residual ? to_f32(x[j]) + to_f32(residual[j]) : to_f32(x[j]));
+  };
+  float sum = 0.f;
+  unsigned top = 0;
+  const auto join = [&]() {
+    top = __reduce_max_sync(kFullMask, top);
+    for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(kFullMask, sum, o);
+    if (threads == 32) return;
+    __syncthreads();  // what was joined before has been read
+    if ((tid & 31) == 0) {
+      s_sum[tid >> 5] = sum;
+      s_top[tid >> 5] = top;
+    }
+    __syncthreads();
+    const bool mine = (tid & 31) < threads >> 5;
+    sum = mine ? s_sum[tid & 31] : 0.f;
+    top = __reduce_max_sync(kFullMask, mine ? s_top[tid & 31] : 0u);
+    for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(kFullMask, sum, o);
+  };
+  each([&](int, float h) { top = max(top, __float_as_uint(h) & 0x7fffffffu); });
+  join();
+  bool finite = top < 0x7f800000u;
+  // 2^-k in two factors that are both normal numbers.
+  const int k = max(1, (int)(__float_as_uint(fmaxf(__uint_as_float(top), sqrtf(eps))) >> 23)) - 126;
+  const float down = __int_as_float((127 - (k >> 1)) << 23), rest = __int_as_float((127 - (k - (k >> 1))) << 23);
+  top = 0;
+  each([&](int j, float h) {
+    const float v = h * down * rest, t = w ? (over ? v : h) * to_f32(w[j]) : over ? v : h;
+    sum = fmaf(v, v, sum);
+    top = max(top, __float_as_uint(t) & 0x7fffffffu);
+  });
+  join();
+  finite = finite && top < 0x7f800000u;
+  const float a = __uint_as_float(top), inv = finite ? __fmul_rn(__frcp_rn(a), 127.f) : 0.f;
+  if (tid == 0) {
+    const float rms = rsqrtf(sum / (float)cols + eps * down * down * rest * rest) / 127.f;
+    *scale = finite ? (over ? a * rms : a * down * rms * rest) : __int_as_float(0x7fffffff);
+  }
+  each([&](int j, float h) {
+    const float t = (over ? h * down * rest : h) * (w ? to_f32(w[j]) : 1.f);
+    q[j] = finite ? (int8_t)__float2int_rn(__fmul_rn(t, inv)) : (int8_t)0;
+    if (h_out) h_out[j] = from_f32<T>(h);
+  });
+}
+
 // A row lives in the registers of blockDim.x threads, kItems packs each, a block's y rows beside
-// one another: memory is read once and written once, and bounds it. (16384 x 4096 bf16: 79 us, 5.9
-// TB/s; rows off 16-byte boundaries cost twice that, 16384 x 2047 65 us; storing those through
-// shared memory, element beside element, lost, 74 us.) Every load of the row is asked for before
+// one another: memory is read once and written once, and bounds it. (16384 x 4096 bf16: 71 us, 6.6
+// TB/s; rows off 16-byte boundaries cost twice that, 16384 x 2047 77 us with gain and residual;
+// storing those through shared memory, element beside element, lost.) Every load of the row is asked for before
 // the first is used. Which thread holds which element depends on the row's length alone, so a row's
 // result, bit for bit, depends on neither its neighbours, their number nor anybody's alignment.
+// (Short rows, one pack a thread, go two blocks' worth of threads to an SM: 16384 x 64 5.3 us for 5.7.)
 template <typename T, typename W, bool kNorm, bool kAligned, int kItems>
-__global__ void __launch_bounds__(1024) rows_int8_kernel(RowsParams P) {
+__global__ void __launch_bounds__(1024, kItems == 1 ? 2 : 1) rows_int8_kernel(RowsParams P) {
   constexpr int kVec = 16 / sizeof(T);
+  // h_out may be the residual, so h is stored once nobody needs that any more (which is also faster:
+  // 71.4 us for 77.5), in 32 bits, where what is stored is h, and off 16-byte boundaries (77 us for 85) at once.
+  constexpr bool kLate = sizeof(T) == 2 && kAligned;
   __shared__ float s_sum[32];
   __shared__ unsigned s_top[32];
   griddep_launch_wait();
@@ -139,6 +204,7 @@ __global__ void __launch_bounds__(1024) rows_int8_kernel(RowsParams P) {
   const T* x = static_cast<const T*>(P.x) + row * P.x_stride;
   const T* r = static_cast<const T*>(P.residual) + row * P.r_stride;
   const W* w = static_cast<const W*>(P.weight);
+  T* h_out = static_cast<T*>(P.h_out) + row * P.cols;
   // The operands' extents, for loads off 16-byte boundaries.
   const auto extent = [&](const void* base, long long stride) {
     const char* lo = static_cast<const char*>(base);
@@ -171,7 +237,7 @@ __global__ void __launch_bounds__(1024) rows_int8_kernel(RowsParams P) {
           t[i][e + 1] += to_f32(rv[i][e + 1]);
           put2(&rv[i][e], t[i][e], t[i][e + 1]);
         }
-        store_pack<kAligned>(static_cast<T*>(P.h_out) + row * P.cols + c * kVec, rv[i], P.cols - c * kVec);
+        if constexpr (!kLate) store_pack<kAligned>(h_out + c * kVec, rv[i], P.cols - c * kVec);
       }
 #pragma unroll
       for (int e = 0; e < kVec; ++e) sum = fmaf(t[i][e], t[i][e], sum);
@@ -206,6 +272,22 @@ __global__ void __launch_bounds__(1024) rows_int8_kernel(RowsParams P) {
   if (!in) return;
   const float a = __uint_as_float(top);
   const bool finite = top < 0x7f800000u, tiny = a < kTinyRow;
+  if constexpr (kNorm) {
+    // NaN in the sum is one in the row; a mean from 2^-100 on has lost nothing to squares below 2^-126.
+    if (!tiny && (sum > 0x1.fffffep127f || fmaf((float)P.cols, P.eps, sum) < 0x1p-100f * (float)P.cols || (!finite && sum == sum))) {
+      const bool stored = !kLate && P.residual && (sizeof(T) == 4 || r == h_out);
+      rows_outside<T, W>(stored ? h_out : x, P.residual && !stored ? r : nullptr, kLate && P.residual ? h_out : nullptr, w,
+                         P.q + row * P.q_stride, P.scale + row, P.cols, P.eps, !finite);
+      return;
+    }
+    if (kLate && P.residual) {
+#pragma unroll
+      for (int i = 0; i < kItems; ++i) {
+        const int c = tid + i * threads;
+        if (c < packs) store_pack<kAligned>(h_out + c * kVec, rv[i], P.cols - c * kVec);
+      }
+    }
+  }
   const float inv = finite && !tiny ? __fmul_rn(__frcp_rn(a), 127.f) : 0.f;
   if (tid == 0) {
     const float rms = kNorm ? rsqrtf(sum / (float)P.cols + P.eps) : 1.f;

@@ -6,9 +6,10 @@ Each check derives its own tolerance; U is the unit roundoff of a type.
 
 import pytest
 import torch
-from test_gpu_quant import BF, HF, U, _randn, _values
+from test_gpu_quant import BF, HF, SF, U, _check_rows, _randn, _values
 
 import qr_v2_b200_kernel_b200 as qr
+from qr_v2_b200_kernel_b200 import _lib
 
 pytestmark = pytest.mark.gpu
 
@@ -73,3 +74,57 @@ def test_attention_of_scores_a_rounding_apart(base, batch, tokens, dtype):
     p = torch.exp2(s - s.amax(-1, keepdim=True))
     want = (p / p.sum(-1, keepdim=True)) @ values[:tokens, 0]
     assert bool(((got[:, 0].double() - want).abs() <= U[dtype] * want.abs() + 2.0**-20 * values.abs().max()).all())
+
+
+# Entries' size (a power of two), eps, and the gain's size: squares or products with the gain that 32 bits cannot hold,
+# and, in the last two, ordinary ones.
+ROWS = [(66, 0.0, 0), (66, 1e-6, 0), (100, 1e-6, 0), (120, 1e-6, 6), (124, 0.0, -60), (-83, 0.0, 0), (-83, 1e-40, 0),
+        (-60, 1e-36, 0), (-70, 0.0, 90), (-95, 0.0, 20), (60, 1e-6, 80), (100, 1e6, 100), (0, 0.0, 0), (3, 1e-6, 3)]
+
+
+@pytest.mark.parametrize("dtype", [BF, SF])
+@pytest.mark.parametrize("rows, cols", [(3, 50), (700, 256), (2, 1000), (2, 4096), (2, 4099), (1, 32768)])
+@pytest.mark.parametrize("power, eps, gain", ROWS)
+def test_norm_over_the_whole_range(power, eps, gain, rows, cols, dtype):
+    """Finite rows of any size are normalised as ordinary ones are: the same bounds, and h as it was. (Where the scale
+    itself is below the normal range, to its spacing.)"""
+    x = _randn(rows, cols, seed=90).clamp(-4, 4).mul(2.0**power).to(dtype)
+    r = _randn(rows, cols, seed=91).clamp(-4, 4).mul(2.0**power).to(dtype)
+    w = _randn(cols, seed=92).clamp(-4, 4).mul(2.0**gain)
+    w = w.to(dtype) if cols != 4096 else w
+    for residual, weight in ((r, w), (None, w), (r, None)):
+        if weight is None and gain:
+            continue
+        codes, scale, h = qr.rms_norm_int8(x, weight, residual, eps=eps)
+        h64 = x.double() + residual.double() if residual is not None else x.double()
+        e64 = torch.tensor(eps, dtype=torch.float32, device="cuda").double()
+        y64 = h64 / (h64.square().mean(-1, keepdim=True) + e64).sqrt() * (weight.double() if weight is not None else 1)
+        _check_rows(codes, scale, y64)
+        assert bool(((h.double() - h64).abs() <= U[dtype] * h64.abs()).all())
+
+
+@pytest.mark.parametrize("cols", [200, 4096, 5001])
+def test_norm_of_large_rows_that_are_not_finite(cols):
+    x = _randn(6, cols, seed=93, size=1e20).to(BF)
+    w = _randn(cols, seed=94)
+    x[1, 3], x[2, -1], x[3, 0] = float("inf"), float("nan"), -float("inf")
+    codes, scale, _ = qr.rms_norm_int8(x, w)
+    assert torch.isnan(scale[1:4]).all() and not codes[1:4].any() and torch.isfinite(scale[[0, 4, 5]]).all()
+    for bad in (float("inf"), float("nan")):
+        w[7] = bad
+        codes, scale, _ = qr.rms_norm_int8(x, w)
+        assert torch.isnan(scale).all() and not codes.any()
+
+
+@pytest.mark.parametrize("cols", [48, 4096])
+def test_norm_in_place_of_the_residual(cols):
+    """The C entry may store h where the residual was (rows on 16-byte boundaries), in rows of any size."""
+    lib = _lib.load()
+    for dtype, code in ((BF, 1), (SF, 0)):
+        for size in (1.0, 1e20):
+            x, r = _randn(5, cols, seed=95, size=size).to(dtype), _randn(5, cols, seed=96, size=size).to(dtype)
+            want = qr.rms_norm_int8(x, None, r)
+            q, s = torch.empty(5, cols, dtype=torch.int8, device="cuda"), torch.empty(5, device="cuda")
+            assert lib.qrb200_rms_norm_int8(x.data_ptr(), cols, r.data_ptr(), cols, None, 0, q.data_ptr(), cols, s.data_ptr(), r.data_ptr(),
+                                            5, cols, 1e-6, code, torch.cuda.current_stream().cuda_stream) == 0
+            assert all(torch.equal(a, b) for a, b in zip((q, s, r), want))
