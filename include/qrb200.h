@@ -215,7 +215,9 @@ int qrb200_kv4_read(const void* cache, const qrb200_kv4_shape* shape, void* k, v
  * lengths: batch, tokens in the cache, the queries' own among them: query i stands at position
  * lengths - queries + i. It sees the tokens up to its position (all of them when causal is 0),
  * and of those the last `window` up to its position when window > 0. out: batch x queries x q_heads x head_dim,
- * contiguous; zeros where nothing is seen. scale >= 0. Workspace as the query says, 256-byte aligned. */
+ * contiguous; zeros where nothing is seen. scale >= 0. q_heads <= 65535, queries x q_heads / kv_heads <= 2^24,
+ * batch x queries x q_heads < 2^31, (max_pages + 320) x page_size < 2^31. Workspace as the query says,
+ * 256-byte aligned. */
 size_t qrb200_kv4_attention_workspace_bytes(const qrb200_kv4_shape* shape, int64_t batch, int64_t queries,
                                             int64_t q_heads, int64_t max_pages, int64_t window);
 int qrb200_kv4_attention(const void* q, const int64_t* q_strides, const void* cache, const qrb200_kv4_shape* shape,

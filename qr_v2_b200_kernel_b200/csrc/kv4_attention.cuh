@@ -32,7 +32,7 @@
 // * a lane's two query rows go through paired 32-bit operations (127 -> 123 us).
 // Each warp walks its own stretch of tokens, a step of 32 or 64 at a time, through a ring of two
 // or three steps in shared memory that bulk asynchronous copies fill: a run's bytes are already in the order
-// of the operand's registers. The token range is cut over CTAs (blockIdx.x) and over a CTA's four
+// of the operand's registers. The token range is cut over CTAs (blockIdx.x % splits) and over a CTA's four
 // warps; the parts are joined through shared memory and, between CTAs, through the cluster's shared
 // memory (up to eight) or by kv4_join_kernel, always in a fixed order.
 // 64 sequences x 8192 tokens, 64 heads on 8: 123 us, 4.7 TB/s of cache; 1 x 65536 30 us; one of
@@ -209,7 +209,7 @@ __global__ void __launch_bounds__(32 * kKvWarps, kv_ctas(kGroups, kNT)) kv4_atte
   __shared__ int s_bad;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int split = blockIdx.x, head = blockIdx.y % P.sh.heads, tile = blockIdx.y / P.sh.heads, b = blockIdx.z;
+  const int split = blockIdx.x % P.splits, tile = blockIdx.x / P.splits, head = blockIdx.y, b = blockIdx.z;
   const int rows = P.queries * P.share, row0 = tile * kRows;
 
   if (threadIdx.x == 0) s_bad = 0;

@@ -84,6 +84,7 @@ struct OnDevice {
 };
 
 void check(int status, const char* what) {
+  TORCH_CHECK_VALUE(status != QRB200_ERR_ARG, what, ": a size, stride or alignment is beyond what the library takes (include/qrb200.h)");
   if (status != QRB200_OK) py::module_::import("qr_v2_b200_kernel_b200._lib").attr("check")(status, what);
 }
 

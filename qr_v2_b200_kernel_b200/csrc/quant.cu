@@ -384,7 +384,7 @@ static cudaError_t launch_attention_tile(const Kv4AttnParams& p, const AttnPlan&
     return cudaFuncSetAttribute(kv4_attention_kernel<T, kDim, kGroups, kNT, kBrief>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
   });
   if (e != cudaSuccess) return e;
-  LaunchShape l(dim3(plan.splits, p.sh.heads * plan.tiles, p.batch), 32 * kKvWarps, kSmem, s);
+  LaunchShape l(dim3(plan.splits * plan.tiles, p.sh.heads, p.batch), 32 * kKvWarps, kSmem, s);
   if (plan.splits > 1 && plan.splits <= kKvCluster) l.cluster(plan.splits, 1, 1);
   return cudaLaunchKernelEx(&l.cfg, kv4_attention_kernel<T, kDim, kGroups, kNT, kBrief>, p);
 }
@@ -543,14 +543,15 @@ int qrb200_kv4_read(const void* cache, const qrb200_kv4_shape* shape, void* k, v
 // The most tokens that a sequence's queries see between them.
 static int64_t token_span(int64_t queries, int64_t window) { return window > 0 ? window + queries : kMaxRows; }
 
-// The launch grid is splits x (key heads x row tiles) x batch.
+// The launch grid is (splits x row tiles) x key heads x batch, a large batch in several launches.
+constexpr int64_t kGridZ = 65535;
 static bool attention_args(const qrb200_kv4_shape* shape, int64_t batch, int64_t queries, int64_t q_heads,
                            int64_t max_pages, Kv4Shape* h) {
   if (!shape || batch < 0 || queries < 0 || q_heads < 0 || max_pages < 0 || !type16_ok(shape->dtype)) return false;
   *h = Kv4Shape{shape->kv_heads, shape->page_size, shape->head_dim, shape->groups, page_shift(shape->page_size), shape->pages};
-  return shape_ok(*h) && q_heads % h->heads == 0 && batch <= 65535 && q_heads <= 65535 && queries <= (1 << 24) &&
-         queries * (q_heads / h->heads) <= (1 << 24) && (queries * (q_heads / h->heads) + 15) / 16 * h->heads <= 65535 &&
-         batch * queries * q_heads <= kMaxRows && max_pages <= kMaxRows / h->page - 64 * (kKvWarps + 1);
+  return shape_ok(*h) && q_heads % h->heads == 0 && batch <= kMaxRows && q_heads <= 65535 && queries <= (1 << 24) &&
+         queries * (q_heads / h->heads) <= (1 << 24) && (queries * q_heads == 0 || batch <= kMaxRows / (queries * q_heads)) &&
+         max_pages <= kMaxRows / h->page - 64 * (kKvWarps + 1);
 }
 
 size_t qrb200_kv4_attention_workspace_bytes(const qrb200_kv4_shape* shape, int64_t batch, int64_t queries,
@@ -595,10 +596,22 @@ int qrb200_kv4_attention(const void* q, const int64_t* q_strides, const void* ca
   if (plan.splits > kKvCluster)
     p.part_ml = reinterpret_cast<float2*>(p.part_o + batch * h.heads * plan.tiles * plan.splits * plan.tile_rows * h.dim);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const cudaError_t e = shape->dtype == QRB200_BF16 ? launch_attention_of<__nv_bfloat16>(p, plan, s)
-                                                    : launch_attention_of<__half>(p, plan, s);
-  if (e != cudaSuccess) return QRB200_ERR_CUDA;
-  return launched();
+  for (int64_t b = 0; b < batch; b += kGridZ) {
+    Kv4AttnParams part = p;
+    const int64_t rows = b * queries * q_heads, parts = b * h.heads * plan.tiles * plan.splits * plan.tile_rows;
+    part.batch = (int)std::min(kGridZ, batch - b);
+    part.q = static_cast<const char*>(q) + 2 * b * p.q_bs;
+    part.out = static_cast<char*>(out) + 2 * rows * h.dim;
+    part.table += b * table_stride;
+    part.lengths += b;
+    if (p.part_ml) part.part_o += parts * h.dim, part.part_ml += parts;
+    const cudaError_t e = shape->dtype == QRB200_BF16 ? launch_attention_of<__nv_bfloat16>(part, plan, s)
+                                                      : launch_attention_of<__half>(part, plan, s);
+    if (e != cudaSuccess) return QRB200_ERR_CUDA;
+    const int ended = launched();
+    if (ended != QRB200_OK) return ended;
+  }
+  return QRB200_OK;
 }
 
 }  // extern "C"

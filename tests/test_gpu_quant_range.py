@@ -128,3 +128,44 @@ def test_norm_in_place_of_the_residual(cols):
             assert lib.qrb200_rms_norm_int8(x.data_ptr(), cols, r.data_ptr(), cols, None, 0, q.data_ptr(), cols, s.data_ptr(), r.data_ptr(),
                                             5, cols, 1e-6, code, torch.cuda.current_stream().cuda_stream) == 0
             assert all(torch.equal(a, b) for a, b in zip((q, s, r), want))
+
+
+def test_attention_of_a_prompt_past_65535_row_tiles():
+    """8200 queries, 128 heads on 8: 65600 tiles of 16 rows. Some of them against 64 bits."""
+    queries, heads, share, window = 8200, 8, 16, 40
+    cache = qr.kv4_cache(130, 64, heads, 64, 64, BF)
+    k, v = _randn(queries, heads, 64, seed=100, dtype=BF), _randn(queries, heads, 64, seed=101, dtype=BF)
+    qr.kv4_write(cache, k, v, torch.arange(queries, device="cuda"))
+    q = _randn(1, queries, heads * share, 64, seed=102, dtype=BF)
+    table = torch.arange(130, dtype=torch.int32, device="cuda")[None]
+    got = qr.kv4_attention(q, cache, table, torch.tensor([queries], dtype=torch.int32, device="cuda"), window=window)
+    k, v = _values(cache)
+    for i in (0, 1, 15, 39, 40, 4000, 8190, 8191, 8192, 8199):
+        lo = max(0, i - window + 1)
+        p = (torch.einsum("hgd,thd->hgt", q[0, i].double().unflatten(0, (heads, share)), k[lo : i + 1]) / 8).softmax(-1)
+        want = torch.einsum("hgt,thd->hgd", p, v[lo : i + 1]).flatten(0, 1)
+        assert bool(((got[0, i].double() - want).abs() <= U[BF] * want.abs() + 2.0**-16 * v.abs().max()).all())
+
+
+def test_attention_of_more_sequences_than_a_launch_holds():
+    batch = 70000
+    cache = qr.kv4_cache(500, 16, 1, 64, 64, HF)
+    k, v = _randn(8000, 1, 64, seed=103, dtype=HF), _randn(8000, 1, 64, seed=104, dtype=HF)
+    qr.kv4_write(cache, k, v, torch.arange(8000, device="cuda"))
+    gen = torch.Generator(device="cuda").manual_seed(105)
+    table = torch.randint(0, 500, (batch, 2), generator=gen, device="cuda").int()
+    lengths = torch.randint(0, 33, (batch,), generator=gen, device="cuda").int()
+    q = _randn(batch, 2, 2, 64, seed=106, dtype=HF)
+    got = qr.kv4_attention(q.transpose(0, 1).contiguous().transpose(0, 1), cache, table, lengths)
+    for lo, hi in ((0, 5), (30000, 30005), (65530, 65540), (69995, 70000)):
+        assert torch.equal(got[lo:hi], qr.kv4_attention(q[lo:hi], cache, table[lo:hi], lengths[lo:hi]))
+
+
+def test_sizes_beyond_the_library_are_value_errors():
+    cache = qr.kv4_cache(2, 16, 1, 64, 64, BF)
+    one = torch.zeros(1, 1, 1, 64, dtype=BF, device="cuda")
+    table, n = torch.zeros(1, 1, dtype=torch.int32, device="cuda"), torch.ones(1, dtype=torch.int32, device="cuda")
+    with pytest.raises(ValueError):
+        qr.kv4_attention(one.expand(1, (1 << 24) + 1, 1, 64), cache, table, n)
+    with pytest.raises(ValueError):
+        qr.kv4_attention(one.expand(1, 1, 65536, 64), cache, table, n)
