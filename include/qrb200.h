@@ -211,7 +211,8 @@ int qrb200_kv4_read(const void* cache, const qrb200_kv4_shape* shape, void* k, v
 /* Attention of `queries` new tokens of each sequence over the cache. q: batch x queries x q_heads x
  * head_dim of the cache's type, channels contiguous, q_strides = {batch, query, head} in elements;
  * q_heads a multiple of kv_heads (head h reads key head h / (q_heads / kv_heads)). block_table:
- * batch x max_pages pages, rows table_stride apart; entries past a sequence's length are not read.
+ * batch x max_pages pages, rows table_stride apart; entries past a sequence's length, or behind
+ * every query's window, are not read.
  * lengths: batch, tokens in the cache, the queries' own among them: query i stands at position
  * lengths - queries + i. It sees the tokens up to its position (all of them when causal is 0),
  * and of those the last `window` up to its position when window > 0. out: batch x queries x q_heads x head_dim,

@@ -264,15 +264,15 @@ __global__ void __launch_bounds__(32 * kKvWarps, kv_ctas(kGroups, kNT)) kv4_atte
   int u = min(cta_hi, cta_lo + warp * per_warp);
   const int u_hi = min(cta_hi, u + per_warp);
 
-  // The ring. Lane i of `page` holds the page of run `page_base` + i, -1 past the range or where
-  // the table is wrong.
+  // The ring. Lane i of `page` holds the page of run `page_base` + i, -1 outside the range, before
+  // which pages may be gone from the table, or where the table is wrong.
   unsigned char* ring = s_ring + warp * (kStages * kStage);
   const int page_runs = P.sh.page / 16, page_shift = P.sh.shift - 4;
-  const int last_run = min(u_hi * kRuns, (len + 15) / 16);
+  const int first_run = all_lo / 16, last_run = min(u_hi * kRuns, (len + 15) / 16);
   int page_base = u * kRuns, page = -1;
   auto look_up = [&]() {
     page = -1;
-    if (page_base + lane < last_run) {
+    if (page_base + lane >= first_run && page_base + lane < last_run) {
       page = __ldg(P.table + b * P.table_stride + ((page_base + lane) >> page_shift));
       if (page < 0 || page >= P.sh.pages) {
         report_device_failure(kSiteIndex);
@@ -291,8 +291,8 @@ __global__ void __launch_bounds__(32 * kKvWarps, kv_ctas(kGroups, kNT)) kv4_atte
       return P.cache + ((long long)pg * P.sh.heads + head) * P.sh.block_bytes() + (run & (page_runs - 1)) * kRunBytes;
     };
     unsigned gone = 0;
-    if (page_runs >= kRuns && (unit + 1) * kRuns <= last_run) {  // one page holds the step: one copy
-      const int run = unit * kRuns, pg = __shfl_sync(kFullMask, page, run - page_base);
+    if (page_runs >= kRuns && (unit + 1) * kRuns <= last_run) {  // one page, the last run's, holds the step: one copy
+      const int run = unit * kRuns, pg = __shfl_sync(kFullMask, page, run + kRuns - 1 - page_base);
       if (pg < 0) gone = (1u << kRuns) - 1;
       if (lane == 0) {
         mbar_expect(bar, pg < 0 ? 0 : kStage);

@@ -165,7 +165,7 @@ def kv4_attention(q: torch.Tensor, cache: KV4Cache, block_table: torch.Tensor, l
 
     ``q`` (batch, queries, heads, head_dim) of the cache's type, heads a multiple of kv_heads (head
     h reads key head h // (heads // kv_heads)). ``block_table`` int32 (batch, max_pages): the pages
-    of each sequence in order; entries past its length are not read. ``lengths`` int32 (batch,):
+    of each sequence in order; entries past its length, or behind every query's window, are not read. ``lengths`` int32 (batch,):
     tokens in the cache, the queries' own included, so query i stands at position lengths - queries
     + i. It sees every token up to its position (all tokens with ``causal=False``), or the last
     ``window`` of those up to its position. ``scale`` multiplies the scores (default head_dim **

@@ -6,7 +6,7 @@ Each check derives its own tolerance; U is the unit roundoff of a type.
 
 import pytest
 import torch
-from test_gpu_quant import BF, HF, SF, U, _check_rows, _randn, _values
+from test_gpu_quant import BF, HF, SF, U, _case, _check_rows, _randn, _values
 
 import qr_v2_b200_kernel_b200 as qr
 from qr_v2_b200_kernel_b200 import _lib
@@ -169,3 +169,18 @@ def test_sizes_beyond_the_library_are_value_errors():
         qr.kv4_attention(one.expand(1, (1 << 24) + 1, 1, 64), cache, table, n)
     with pytest.raises(ValueError):
         qr.kv4_attention(one.expand(1, 1, 65536, 64), cache, table, n)
+
+
+@pytest.mark.parametrize("page, dim", [(16, 64), (16, 128), (32, 64), (64, 128)])
+@pytest.mark.parametrize("queries, window, causal", [(1, 20, True), (3, 1, True), (5, 70, True), (4, 33, False)])
+def test_attention_reads_no_page_behind_the_window(queries, window, causal, page, dim):
+    """Pages that the window has left may be gone from the table, wherever its start falls."""
+    lengths = list(range(queries, 230, 3))
+    q, cache, table, n = _case(lengths, queries, 1, 2, page, dim, 64, BF, seed=110)
+    want = qr.kv4_attention(q, cache, table, n, window=window, causal=causal)
+    freed = table.clone()
+    for b, length in enumerate(lengths):
+        freed[b, : max(0, length - queries - window + 1) // page] = -1
+    assert torch.equal(want, qr.kv4_attention(q, cache, freed, n, window=window, causal=causal))
+    torch.cuda.synchronize()
+    qr.kv4_read(cache, torch.zeros(1, dtype=torch.int64, device="cuda"))  # nothing was reported
