@@ -99,7 +99,9 @@ __device__ __forceinline__ void kv_values(uint32_t (&a)[4], uint32_t w) {
   a[0] = w << 4 & kMask, a[1] = w & kMask, a[2] = ~(w >> 4) & kMask, a[3] = ~(w >> 8) & kMask;
 }
 // Where a query row's largest entry is put (its exponent), and what its type makes of the code 1
-// (the negative exponent).
+// (the negative exponent). Scores are built from queries brought to 2^-kKvSpare, so that keys of any
+// size give finite ones, and multiplied by what that takes back, the scale included, as the last step.
+constexpr int kKvSpare = 8;
 template <typename T>
 struct KvKey;
 template <>
@@ -112,10 +114,10 @@ struct KvKey<__half> {
 };
 __device__ __forceinline__ float kv_power(int e) { return __int_as_float((max(-126, min(127, e)) + 127) << 23); }
 // The power of two that brings a row whose largest entry has these bits (32-bit float, no sign) to
-// kTop, as far as it and what takes it back, scale2 2^(kOne - lift), are numbers.
+// kTop, as far as it and what takes it back, scale2 2^(kTop + kKvSpare - lift), are normal numbers.
 template <typename T>
 __device__ __forceinline__ int kv_lift(unsigned top, float scale2) {
-  const int least = KvKey<T>::kOne - 127 + max(0, (__float_as_int(scale2) >> 23) - 126);
+  const int least = KvKey<T>::kTop + kKvSpare - 126 + max(0, (__float_as_int(scale2) >> 23) - 126);
   return max(least, min(120, KvKey<T>::kTop + 127 - (int)(top >> 23)));
 }
 
@@ -199,6 +201,7 @@ __global__ void __launch_bounds__(32 * kKvWarps, kv_ctas(kGroups, kNT)) kv4_atte
   constexpr int kRuns = kv_runs(kDim, kBrief), kUnit = 16 * kRuns;
   constexpr int kRunBytes = 16 * kDim + 128 * kGroups, kStage = kRuns * kRunBytes;
   constexpr int kStages = kv_stages(kNT);
+  const float unbare = kv_power(KvKey<T>::kOne - KvKey<T>::kTop - kKvSpare);  // q . c from the product with bare codes
   constexpr float kNone = -INFINITY;
   extern __shared__ __align__(128) unsigned char s_ring[];
   __shared__ uint2 s_q[kNT][kSteps][32];
@@ -325,7 +328,7 @@ __global__ void __launch_bounds__(32 * kKvWarps, kv_ctas(kGroups, kNT)) kv4_atte
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const float v = to_f32(qv[n][i][e]);
-        add += v;
+        add = fmaf(v, 0x1p-8f, add);  // (a sum of 128 may leave the range that one is in)
         top = max(top, __float_as_uint(v) & 0x7fffffffu);
       }
 #pragma unroll
@@ -349,8 +352,8 @@ __global__ void __launch_bounds__(32 * kKvWarps, kv_ctas(kGroups, kNT)) kv4_atte
     for (int w = 0; w < kKvWarps; ++w) top = max(top, s_qtop[w][n][row]);
     return kv_lift<T>(top, P.scale2);
   };
-  // back: what gives q . c from the product with bare codes. Both are in the exponent's units (base
-  // 2), so that the largest score less itself is 0 and its weight 1, exactly.
+  // qsum: a group's sum at the size that scores are built from; back: what takes that size back, into
+  // the exponent's units (base 2), so that the largest score less itself is 0 and its weight 1, exactly.
   float2 qsum[kNT][kGroups], back[kNT];
 #pragma unroll
   for (int n = 0; n < kNT; ++n) {
@@ -362,8 +365,8 @@ __global__ void __launch_bounds__(32 * kKvWarps, kv_ctas(kGroups, kNT)) kv4_atte
       put2(x + 2, to_f32(qv[n][i][2]) * (up / 16), to_f32(qv[n][i][3]) * (up / 16));
       s_q[n][i * kKvWarps + warp][lane] = *reinterpret_cast<uint2*>(x);
     }
-    back[n] = make_float2(kv_power(KvKey<T>::kOne - lift(n, 2 * t)) * P.scale2,
-                          kv_power(KvKey<T>::kOne - lift(n, 2 * t + 1)) * P.scale2);
+    const int lift0 = lift(n, 2 * t) - KvKey<T>::kTop, lift1 = lift(n, 2 * t + 1) - KvKey<T>::kTop;
+    back[n] = make_float2(kv_power(kKvSpare - lift0) * P.scale2, kv_power(kKvSpare - lift1) * P.scale2);
 #pragma unroll
     for (int gr = 0; gr < kGroups; ++gr) {
       qsum[n][gr] = make_float2(0.f, 0.f);
@@ -371,7 +374,8 @@ __global__ void __launch_bounds__(32 * kKvWarps, kv_ctas(kGroups, kNT)) kv4_atte
         qsum[n][gr].x += s_qsum[w][n][2 * t][gr];
         qsum[n][gr].y += s_qsum[w][n][2 * t + 1][gr];
       }
-      qsum[n][gr] = make_float2(qsum[n][gr].x * P.scale2, qsum[n][gr].y * P.scale2);
+      // 2^8 of the sums' and 2^-kKvSpare cancel.
+      qsum[n][gr] = make_float2(qsum[n][gr].x * kv_power(lift0), qsum[n][gr].y * kv_power(lift1));
     }
   }
   __syncthreads();
@@ -439,7 +443,9 @@ __global__ void __launch_bounds__(32 * kKvWarps, kv_ctas(kGroups, kNT)) kv4_atte
               for (int n = 0; n < kNT; ++n) {
                 const float2 kx = make_float2(k.x, k.x), ky = make_float2(k.y, k.y);
                 const float2 low = gr ? __ffma2_rn(ky, qsum[n][gr], s[i][n][h]) : __fmul2_rn(ky, qsum[n][gr]);
-                s[i][n][h] = __ffma2_rn(kx, __fmul2_rn(make_float2(acc[i][n][2 * h], acc[i][n][2 * h + 1]), back[n]), low);
+                const float2 dot = __fmul2_rn(make_float2(acc[i][n][2 * h], acc[i][n][2 * h + 1]), make_float2(unbare, unbare));
+                s[i][n][h] = __ffma2_rn(kx, dot, low);
+                if (gr == kGroups - 1) s[i][n][h] = __fmul2_rn(s[i][n][h], back[n]);
               }
             }
         }

@@ -590,7 +590,7 @@ int qrb200_kv4_attention(const void* q, const int64_t* q_strides, const void* ca
   // A window that reaches every token from every position is none (and cannot overflow a position).
   p.window = window >= max_pages * h.page + queries ? 0 : (int)window;
   p.max_pages = (int)max_pages, p.causal = causal, p.splits = plan.splits, p.tiles = plan.tiles;
-  p.scale2 = std::max(scale * 1.4426950408889634f, 1e-30f);  // not 0: masked scores, -inf, must stay that
+  p.scale2 = scale * 1.4426950408889634f;
   p.sh = h;
   p.q_wide = (reinterpret_cast<uintptr_t>(q) & 7u) == 0 && ((q_strides[0] | q_strides[1] | q_strides[2]) & 3) == 0;
   if (plan.splits > kKvCluster)

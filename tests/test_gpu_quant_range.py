@@ -6,7 +6,7 @@ Each check derives its own tolerance; U is the unit roundoff of a type.
 
 import pytest
 import torch
-from test_gpu_quant import BF, HF, SF, U, _case, _check_rows, _randn, _values
+from test_gpu_quant import BF, HF, SF, U, _attend64, _case, _check_rows, _randn, _values
 
 import qr_v2_b200_kernel_b200 as qr
 from qr_v2_b200_kernel_b200 import _lib
@@ -184,3 +184,53 @@ def test_attention_reads_no_page_behind_the_window(queries, window, causal, page
     assert torch.equal(want, qr.kv4_attention(q, cache, freed, n, window=window, causal=causal))
     torch.cuda.synchronize()
     qr.kv4_read(cache, torch.zeros(1, dtype=torch.int64, device="cuda"))  # nothing was reported
+
+
+@pytest.mark.parametrize("scale", [0.09, 1.0, 30.0])
+@pytest.mark.parametrize("power", [-100, -20, 112, 118, 125])
+def test_attention_of_keys_as_small_as_queries_are_large(power, scale):
+    """Queries times 2^p on keys divided by it: scores of ordinary size. Products at the bottom of 32 bits' range
+    lose up to 2^-18 of a score's terms. (Where a step falls below the normal range the cache holds minima alone.)"""
+    q, plain, table, lengths = _case([70, 33], 2, 2, 3, 16, 128, 64, BF, seed=120)
+    k, v = _randn(128, 2, 128, seed=121).clamp(-3, 3).to(BF), _randn(128, 2, 128, seed=122, dtype=BF)
+    q = q.clamp(-3.5, 3.5)
+    shifted = qr.kv4_cache(plain.pages, 16, 2, 128, 64, BF)
+    qr.kv4_write(shifted, k * 2.0**-power, v, torch.arange(128, device="cuda"))
+    got = qr.kv4_attention(q * 2.0**power, shifted, table % 8, lengths, scale=scale)
+    want, _ = _attend64(q * 2.0**power, shifted, table % 8, lengths, scale=scale)
+    size = v.double().abs().max() * (scale * q.double().abs().sum(-1).max() * 3)
+    assert bool(((got.double() - want).abs() <= U[BF] * 2 * want.abs() + 2.0**-18 * size).all())
+
+
+@pytest.mark.parametrize("power", [95, 105, 118, 125])
+def test_attention_of_large_queries_with_scales_as_small(power):
+    """Queries times 2^p, the scale divided by it: every bit stays."""
+    q, cache, table, lengths = _case([150, 40], 2, 2, 3, 16, 128, 64, BF, seed=123)
+    q = q.clamp(-3.5, 3.5)
+    a = qr.kv4_attention(q, cache, table, lengths, scale=0.1)
+    assert torch.equal(a, qr.kv4_attention(q * 2.0**power, cache, table, lengths, scale=0.1 * 2.0**-power))
+
+
+def test_attention_with_a_scale_of_zero_is_the_mean():
+    q, cache, table, lengths = _case([150, 0, 41], 1, 2, 3, 16, 128, 64, BF, seed=124)
+    for size in (1.0, 2.0**120):
+        got = qr.kv4_attention(q.clamp(-3.5, 3.5) * size, cache, table, lengths, scale=0.0)
+        _, v = _values(cache)
+        for b, n in enumerate((150, 0, 41)):
+            slots = table[b].long()[torch.arange(n, device="cuda") // 16] * 16 + torch.arange(n, device="cuda") % 16
+            want = v[slots].mean(0).repeat_interleave(3, 0) if n else torch.zeros(6, 128, device="cuda", dtype=torch.float64)
+            assert bool(((got[b, 0].double() - want).abs() <= U[BF] * want.abs() + 2.0**-18).all())
+
+
+def test_attention_of_keys_at_the_top_of_the_type():
+    """Keys of 2^120 with queries of 2^-118: scores of ordinary size."""
+    q, cache, table, lengths = _case([100], 1, 1, 4, 16, 64, 64, BF, seed=125)
+    k, v = _randn(112, 1, 64, seed=126).clamp(-3, 3).to(BF), _randn(112, 1, 64, seed=127, dtype=BF)
+    slots, plain = torch.arange(112, device="cuda"), qr.kv4_cache(cache.pages, 16, 1, 64, 64, BF)
+    qr.kv4_write(plain, k, v, slots)
+    qr.kv4_write(cache, k * 2.0**120, v, slots)
+    table = table % 7
+    for down, scale in ((2.0**-118, 0.1), (1.0, 0.1 * 2.0**-118)):
+        a = qr.kv4_attention(q, plain, table, lengths, scale=0.4)
+        b = qr.kv4_attention(q * down, cache, table, lengths, scale=scale)
+        assert bool(((a.double() - b.double()).abs() <= 2 * U[BF] * a.double().abs() + 2.0**-14).all())
