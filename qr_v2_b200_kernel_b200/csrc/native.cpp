@@ -211,9 +211,9 @@ Cache make_cache(const Tensor& data, int32_t page_size, int32_t head_dim, int32_
   operand(data, "data", {at::kByte});
   const int64_t bytes = groups > 0 ? qrb200_kv4_block_bytes(page_size, head_dim, head_dim / groups) : 0;
   TORCH_CHECK_VALUE(bytes > 0 && head_dim % groups == 0 && data.dim() == 3 && data.size(2) == bytes && data.is_contiguous() &&
-                        data.size(1) >= 1 && data.size(1) <= 65535,
-                    "data must be a contiguous (pages, kv_heads, ", bytes, ") tensor for this page_size, head_dim and group_size, got ",
-                    shape_of(data));
+                        data.size(1) >= 1 && data.size(1) <= 65535 && (reinterpret_cast<uintptr_t>(data.const_data_ptr()) & 15u) == 0,
+                    "data must be a contiguous, 16-byte aligned (pages, kv_heads, ", bytes,
+                    ") tensor for this page_size, head_dim and group_size, got ", shape_of(data));
   return Cache{data, {data.size(0), (int32_t)data.size(1), page_size, head_dim, groups, type_code(type)}, type};
 }
 

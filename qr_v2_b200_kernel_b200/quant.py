@@ -93,8 +93,9 @@ class KV4Cache:
     """A paged key/value cache in 4 bits (see :func:`kv4_cache`).
 
     ``data``: uint8 (pages, kv_heads, bytes of a block), the whole state, written in place;
-    ``KV4Cache(data.clone(), ...)`` is a copy of the cache. A token occupies head_dim + 8 head_dim /
-    group_size bytes a head for its key and value.
+    ``KV4Cache(data.clone(), ...)`` is a copy of the cache. Its attributes cannot be assigned: another
+    tensor's bytes are another cache, or are copied into ``data``. A token occupies head_dim + 8
+    head_dim / group_size bytes a head for its key and value.
     """
 
     __slots__ = ("data", "pages", "page_size", "kv_heads", "head_dim", "group_size", "dtype", "_handle")
@@ -102,9 +103,13 @@ class KV4Cache:
     def __init__(self, data: torch.Tensor, page_size: int, head_dim: int, group_size: int, dtype: torch.dtype):
         if group_size < 1 or head_dim % group_size:
             raise ValueError(f"group_size must divide head_dim, got {group_size} and {head_dim}")
-        self.data, self.page_size, self.head_dim, self.group_size, self.dtype = data, page_size, head_dim, group_size, dtype
-        self.pages, self.kv_heads = int(data.shape[0]), int(data.shape[1])
-        self._handle = _native().Cache(data, page_size, head_dim, head_dim // group_size, dtype)
+        handle = _native().Cache(data, page_size, head_dim, head_dim // group_size, dtype)
+        for name, value in (("data", data), ("pages", int(data.shape[0])), ("page_size", page_size), ("kv_heads", int(data.shape[1])),
+                            ("head_dim", head_dim), ("group_size", group_size), ("dtype", dtype), ("_handle", handle)):
+            object.__setattr__(self, name, value)
+
+    def __setattr__(self, name, value):  # the handle would go on with what it was made of
+        raise AttributeError(f"a KV4Cache's {name} cannot be assigned")
 
 
 def kv4_cache(pages: int, page_size: int, kv_heads: int, head_dim: int, group_size: int | None = None,

@@ -234,3 +234,19 @@ def test_attention_of_keys_at_the_top_of_the_type():
         a = qr.kv4_attention(q, plain, table, lengths, scale=0.4)
         b = qr.kv4_attention(q * down, cache, table, lengths, scale=scale)
         assert bool(((a.double() - b.double()).abs() <= 2 * U[BF] * a.double().abs() + 2.0**-14).all())
+
+
+def test_a_caches_attributes_cannot_be_assigned():
+    """The kernels work on the tensor that the cache was made of; another one in its place would be ignored."""
+    cache = qr.kv4_cache(2, 16, 1, 64, 64, BF)
+    other = cache.data.clone()
+    for name, value in (("data", other), ("pages", 1), ("page_size", 32), ("dtype", HF), ("group_size", 32)):
+        with pytest.raises(AttributeError):
+            setattr(cache, name, value)
+    assert cache.pages == 2 and cache.page_size == 16 and cache.kv_heads == 1 and cache.head_dim == 64 and cache.dtype is BF
+    block = cache.data.numel()
+    unaligned = torch.zeros(block + 16, dtype=torch.uint8, device="cuda")[8 : block + 8].view(cache.data.shape)
+    with pytest.raises(ValueError):
+        qr.KV4Cache(unaligned, 16, 64, 64, BF)
+    with pytest.raises(ValueError):
+        qr.KV4Cache(cache.data.flatten(), 16, 64, 64, BF)
