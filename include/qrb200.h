@@ -198,7 +198,8 @@ int64_t qrb200_kv4_block_bytes(int64_t page_size, int64_t head_dim, int64_t grou
 /* Quantises keys and values (tokens x kv_heads x head_dim of the cache's type, channels
  * contiguous, other strides in elements) into the cache at slots (page * page_size + offset). A
  * negative slot is skipped; slots of one call must differ. A group's step and minimum are its
- * range / 15 and its least entry, its codes the nearest steps; a group with a NaN or an infinity
+ * range / 15 (a step less in the last place if its top would pass the type's largest number) and its
+ * least entry, its codes the nearest steps; a group with a NaN or an infinity
  * reads back as NaN. */
 int qrb200_kv4_write(void* cache, const qrb200_kv4_shape* shape, const void* k, int64_t k_token_stride,
                      int64_t k_head_stride, const void* v, int64_t v_token_stride, int64_t v_head_stride,

@@ -2,7 +2,8 @@
 // the attention of a few queries over it.
 //
 // Per token, head and group of G channels, with lo and hi the group's ends:
-//   s = hi/15 - lo/15 rounded to the cache's type,  m = lo,
+//   s = hi/15 - lo/15 rounded to the cache's type (the next lower number if m + 15 s would round to
+//   infinity there),  m = lo,
 //   code = min(15, max(0, rint((x - m) (1/s)))),  value = m + s code.
 // m is exact (it is one of the inputs) and the codes are taken against the rounded s, so the
 // reader sees what the writer meant. s < 2^-126 has no reciprocal: codes 0. A group that holds a
@@ -143,12 +144,20 @@ __global__ void __launch_bounds__(2 * kDim, kVec ? 640 / kDim : 1) kv4_write_ker
         ends = __hmin2_nan(ends, reinterpret_cast<const typename Two<T>::type&>(other));
       }
       const float lo = to_f32(ends.x), hi = -to_f32(ends.y);
-      const bool fine = fabsf(lo) < __int_as_float(0x7f800000) && fabsf(hi) < __int_as_float(0x7f800000);
       constexpr float kFifteenth = 1.f / 15.f;
-      const float nan = __int_as_float(0x7fffffff);
       Pair16<T> pr;
-      pr.s = from_f32<T>(fine ? __fsub_rn(__fmul_rn(hi, kFifteenth), __fmul_rn(lo, kFifteenth)) : nan);
-      pr.m = from_f32<T>(fine ? lo : nan);
+      pr.s = from_f32<T>(__fsub_rn(__fmul_rn(hi, kFifteenth), __fmul_rn(lo, kFifteenth)));
+      pr.m = from_f32<T>(lo);
+      // Not finite, or near the top of the type, where a step rounded up may put the group's top past the
+      // largest number: then the next lower step.
+      constexpr float kNear = std::is_same<T, __half>::value ? 65000.f : 0x1.f8p127f;
+      constexpr float kBeyond = std::is_same<T, __half>::value ? 65520.f : 0x1.ffp127f;  // rounds to infinity
+      if (!(lo > -__int_as_float(0x7f800000) && hi < kNear)) {
+        if (!(fabsf(lo) < __int_as_float(0x7f800000) && fabsf(hi) < __int_as_float(0x7f800000)))
+          pr.s = pr.m = from_f32<T>(__int_as_float(0x7fffffff));
+        else if (fmaf(15.f, to_f32(pr.s), lo) >= kBeyond)
+          --reinterpret_cast<uint16_t&>(pr.s);
+      }
       const float s = to_f32(pr.s), m = to_f32(pr.m);
       // bf16 ends may be further apart than 32 bits reach: such a group is quantised at half its size.
       const float part_of = std::is_same<T, __nv_bfloat16>::value && hi - lo > 0x1.fffffep127f ? 0.5f : 1.f;

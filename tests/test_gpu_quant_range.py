@@ -250,3 +250,24 @@ def test_a_caches_attributes_cannot_be_assigned():
         qr.KV4Cache(unaligned, 16, 64, 64, BF)
     with pytest.raises(ValueError):
         qr.KV4Cache(cache.data.flatten(), 16, 64, 64, BF)
+
+
+@pytest.mark.parametrize("dtype, largest", [(HF, 65504.0), (BF, 3.3895313892515355e38)])
+@pytest.mark.parametrize("dim, group", [(64, 32), (128, 128)])
+def test_cache_of_groups_that_reach_the_types_largest_number(dim, group, dtype, largest):
+    """They read back finite, within half a step and what the step's rounding, here by up to its last place, moves the
+    top of the range (30 u steps), rounded by u."""
+    x = _randn(300, 2, dim, seed=130).mul(largest / 6).clamp(-largest, largest)
+    low = torch.linspace(-1, 0.9, 300, device="cuda")[:, None] * largest
+    x[:, 0, ::32], x[:, 0, 1::32] = largest, low
+    x[:, 1, ::32], x[:, 1, 1::32] = -largest, -low
+    x = x.to(dtype)
+    slots = torch.arange(3, 303, device="cuda")
+    cache = qr.kv4_cache(5, 64, 2, dim, group, dtype)
+    qr.kv4_write(cache, x, -x, slots)
+    for got, want in zip(qr.kv4_read(cache, slots), (x, -x)):
+        g = want.double().unflatten(-1, (-1, group))
+        step = (g.amax(-1) - g.amin(-1)) / 15
+        assert torch.isfinite(got).all()
+        off = (got.double().unflatten(-1, (-1, group)) - g).abs()
+        assert bool((off <= (step * (0.5 + 30 * U[dtype])).unsqueeze(-1) + U[dtype] * largest).all())
