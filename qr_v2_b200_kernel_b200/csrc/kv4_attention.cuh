@@ -140,6 +140,11 @@ __device__ __forceinline__ float kv_exp2(float x) {
 __device__ __forceinline__ float kv_part_weight(float2 ml, float m) {
   return ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : ml.y) : kv_exp2(ml.x - m);
 }
+// x and a part's sum that counts f. One that counts nothing may have left the range, but a value that
+// is NaN makes the result NaN, wherever the parts are cut.
+__device__ __forceinline__ float kv_join(float x, float f, float part) {
+  return f == 0.f && part == part ? x : fmaf(f, part, x);
+}
 template <int kWords>
 __device__ __forceinline__ void kv_load(uint32_t (&w)[kWords], const unsigned char* p) {  // from shared memory
   if constexpr (kWords == 4) {
@@ -687,7 +692,7 @@ __global__ void __launch_bounds__(32 * kKvWarps, kv_ctas(kGroups, kNT)) kv4_atte
   const auto joined = [&](int d) {
     float x = 0.f;
 #pragma unroll
-    for (int w = 0; w < kKvWarps; ++w) x = f[w] == 0.f ? x : fmaf(f[w], s_o[w][r][d], x);
+    for (int w = 0; w < kKvWarps; ++w) x = kv_join(x, f[w], s_o[w][r][d]);
     return x;
   };
   if (P.splits == 1) {
@@ -734,8 +739,7 @@ __global__ void __launch_bounds__(32 * kKvWarps, kv_ctas(kGroups, kNT)) kv4_atte
       for (int c = 0; c < kKvCluster; ++c) v[c] = c < P.splits ? __int_as_float(ld_cluster(smem_u32(&s_o[0][row][d]), c)) : 0.f;
 #pragma unroll
       for (int c = 0; c < kKvCluster; ++c) {
-        const float w = s_w[row][c];
-        x = w == 0.f ? x : fmaf(w, v[c], x);
+        x = kv_join(x, s_w[row][c], v[c]);
       }
       out_row(row)[d] = from_f32<T>(x * s_w[row][kKvCluster]);
     }
@@ -770,7 +774,7 @@ __global__ void __launch_bounds__(32 * kKvJoinWarps) kv4_join_kernel(Kv4AttnPara
 #pragma unroll
     for (int i = 0; i < kDim / 32; ++i) {
       const float v = o[32 * i + lane];
-      x[i] = f == 0.f ? x[i] : fmaf(f, v, x[i]);
+      x[i] = kv_join(x[i], f, v);
     }
   }
 #pragma unroll

@@ -271,3 +271,24 @@ def test_cache_of_groups_that_reach_the_types_largest_number(dim, group, dtype, 
         assert torch.isfinite(got).all()
         off = (got.double().unflatten(-1, (-1, group)) - g).abs()
         assert bool((off <= (step * (0.5 + 30 * U[dtype])).unsqueeze(-1) + U[dtype] * largest).all())
+
+
+@pytest.mark.parametrize("tokens, batch", [(60, 1), (600, 1), (700, 100), (5000, 1), (60000, 1)])
+def test_attention_keeps_a_nan_value_however_little_it_weighs(tokens, batch):
+    """The first token takes everything; a group of a later one's values is NaN, in whichever part of the tokens."""
+    pages = -(-tokens // 64)
+    cache = qr.kv4_cache(pages, 64, 1, 64, 32, BF)
+    k, v = torch.zeros(tokens, 1, 64, dtype=BF, device="cuda"), _randn(tokens, 1, 64, seed=140, dtype=BF)
+    k[0, 0, 0], k[1:, 0, 0] = 300, -300
+    q = torch.zeros(batch, 1, 2, 64, dtype=BF, device="cuda")
+    q[..., 0] = 4
+    table = torch.arange(pages, dtype=torch.int32, device="cuda").expand(batch, pages)
+    n = torch.full((batch,), tokens, dtype=torch.int32, device="cuda")
+    for at in (1, tokens // 2, tokens - 1):
+        w = v.clone()
+        w[at, 0, 40] = float("nan")
+        qr.kv4_write(cache, k, w, torch.arange(tokens, device="cuda"))
+        got = qr.kv4_attention(q, cache, table, n)
+        assert torch.isnan(got[..., 32:]).all()
+        first = qr.kv4_read(cache, torch.zeros(1, dtype=torch.int64, device="cuda"))[1][0, 0, :32]
+        assert torch.equal(got[..., :32], first.expand(batch, 1, 2, 32))
