@@ -541,7 +541,7 @@ int qrb200_kv4_read(const void* cache, const qrb200_kv4_shape* shape, void* k, v
 }
 
 // The most tokens that a sequence's queries see between them.
-static int64_t token_span(int64_t queries, int64_t window) { return window > 0 ? window + queries : kMaxRows; }
+static int64_t token_span(int64_t queries, int64_t window) { return window > 0 ? std::min(window, kMaxRows) + queries : kMaxRows; }
 
 // The launch grid is (splits x row tiles) x key heads x batch, a large batch in several launches.
 constexpr int64_t kGridZ = 65535;
@@ -557,7 +557,7 @@ static bool attention_args(const qrb200_kv4_shape* shape, int64_t batch, int64_t
 size_t qrb200_kv4_attention_workspace_bytes(const qrb200_kv4_shape* shape, int64_t batch, int64_t queries,
                                             int64_t q_heads, int64_t max_pages, int64_t window) {
   Kv4Shape h;
-  if (window < 0 || window > kMaxRows) return 0;
+  if (window < 0) return 0;
   if (!attention_args(shape, batch, queries, q_heads, max_pages, &h) || batch * queries * q_heads == 0) return 0;
   return attn_plan(h, batch, queries, q_heads, max_pages, token_span(queries, window)).bytes;
 }
@@ -567,7 +567,7 @@ int qrb200_kv4_attention(const void* q, const int64_t* q_strides, const void* ca
                          int64_t batch, int64_t queries, int64_t q_heads, int64_t max_pages, int64_t window,
                          int causal, float scale, void* workspace, size_t workspace_bytes, void* stream) {
   Kv4Shape h;
-  if (!q_strides || !(scale >= 0.f) || !(scale <= 3.0e38f) || window < 0 || window > kMaxRows || !attention_args(shape, batch, queries, q_heads, max_pages, &h))
+  if (!q_strides || !(scale >= 0.f) || !(scale <= 3.0e38f) || window < 0 || !attention_args(shape, batch, queries, q_heads, max_pages, &h))
     return QRB200_ERR_ARG;
   if (batch == 0 || queries == 0 || q_heads == 0) return QRB200_OK;
   if (!q || !out || !lengths || (max_pages > 0 && !block_table) || (reinterpret_cast<uintptr_t>(cache) & 15u) ||

@@ -292,3 +292,11 @@ def test_attention_keeps_a_nan_value_however_little_it_weighs(tokens, batch):
         assert torch.isnan(got[..., 32:]).all()
         first = qr.kv4_read(cache, torch.zeros(1, dtype=torch.int64, device="cuda"))[1][0, 0, :32]
         assert torch.equal(got[..., :32], first.expand(batch, 1, 2, 32))
+
+
+@pytest.mark.parametrize("window", [(1 << 31) - 1, 1 << 31, 10**12, (1 << 63) - 1])
+def test_attention_window_of_any_size(window):
+    q, cache, table, n = _case([30, 5000, 0], 2, 1, 2, 64, 64, 64, BF, seed=150)
+    for causal in (True, False):
+        want = qr.kv4_attention(q, cache, table, n, causal=causal)
+        assert torch.equal(want, qr.kv4_attention(q, cache, table, n, causal=causal, window=window))
