@@ -300,3 +300,88 @@ def test_attention_window_of_any_size(window):
     for causal in (True, False):
         want = qr.kv4_attention(q, cache, table, n, causal=causal)
         assert torch.equal(want, qr.kv4_attention(q, cache, table, n, causal=causal, window=window))
+
+
+# ---- captured calls -------------------------------------------------------------------------
+
+
+def _replayed(call, refill):
+    """`call`'s outputs when it is captured with one content of its operands and replayed with another."""
+    call()  # set-up that a capture cannot hold
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call()
+    refill()
+    for _ in range(2):
+        graph.replay()
+    torch.cuda.synchronize()
+    return out
+
+
+def _same(a, b):
+    a, b = ((x,) if isinstance(x, torch.Tensor) else x for x in (a, b))
+    return all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+@pytest.mark.parametrize("rows, cols", [(1, 4096), (33, 130), (700, 2048)])
+def test_captured_rows(rows, cols):
+    x, r, w = _randn(rows, cols, seed=160, dtype=BF), _randn(rows, cols, seed=161, dtype=BF), _randn(cols, seed=162, dtype=BF)
+    for call in (lambda: qr.rms_norm_int8(x, w, r), lambda: qr.quantize_int8(x), lambda: qr.dequantize_int8(*qr.quantize_int8(x), BF)):
+        got = _replayed(call, lambda: x.copy_(_randn(rows, cols, seed=163, size=5)))
+        assert _same(got, call())
+
+
+@pytest.mark.parametrize("rows, outs, depth", [(1, 512, 1024), (4, 300, 512), (16, 512, 4096), (3, 130, 1001), (64, 130, 1001), (333, 1000, 2048),
+                                               (2048, 2048, 512)])
+def test_captured_product(rows, outs, depth):
+    x, w = (torch.randint(-127, 128, s, device="cuda").to(torch.int8) for s in ((rows, depth), (outs, depth)))
+    sx, sw = torch.rand(rows, device="cuda"), torch.rand(outs, device="cuda")
+    call = lambda: qr.int8_linear(x, sx, w, sw)  # noqa: E731
+    got = _replayed(call, lambda: (x.neg_(), sw.mul_(2), w[0].zero_()))
+    assert _same(got, call())
+
+
+@pytest.mark.parametrize("lengths, queries, heads, share, dim", [([100, 0, 7], 1, 1, 2, 64), ([700], 5, 2, 8, 128), ([3000] * 3, 1, 2, 4, 128),
+                                                                 ([50000], 1, 1, 8, 128), ([600] * 40, 2, 8, 2, 64)])
+def test_captured_cache_and_attention(lengths, queries, heads, share, dim):
+    """A decode step: the new tokens' keys and values go into the cache, and the attention reads them; replayed with other
+    tokens, lengths and pages."""
+    q, cache, table, n = _case([max(lengths)] * len(lengths), queries, heads, share, 64, dim, 64, HF, seed=170)
+    n.copy_(torch.tensor(lengths))
+    k, v = _randn(16, heads, dim, seed=171, dtype=HF), _randn(16, heads, dim, seed=172, dtype=HF)
+    slots = table[0, 0].long() * 64 + torch.arange(16, device="cuda")
+
+    def call():
+        qr.kv4_write(cache, k, v, slots)
+        return (qr.kv4_attention(q, cache, table, n), *qr.kv4_read(cache, slots))
+
+    def refill():
+        q.mul_(0.5), k.neg_(), v.mul_(3)
+        n.copy_(n.clamp_min(1) - 1)
+        full = table[:, : max(lengths) // 64]  # (the last page's unwritten slots hold NaN)
+        full.copy_(full.flip(1))
+
+    got = _replayed(call, refill)
+    assert _same(got, call())
+
+
+def test_operators_take_the_tensors_stream():
+    """On a side stream each operator waits for nothing but that stream's work, and its results are the same."""
+    x, r = _randn(300, 512, seed=180, dtype=BF), _randn(300, 512, seed=181, dtype=BF)
+    q, cache, table, n = _case([300, 40], 2, 2, 2, 16, 64, 64, BF, seed=182)
+
+    def step():
+        codes, scale, h = qr.rms_norm_int8(x, None, r)
+        y = qr.int8_linear(codes, scale, codes[:256], scale[:256])
+        kv = y[:64].unflatten(1, (2, 2, 64))
+        qr.kv4_write(cache, kv[:, 0], kv[:, 1], torch.arange(64, device="cuda"))
+        return (codes, scale, h, y, qr.dequantize_int8(codes, scale, BF), qr.kv4_attention(q, cache, table, n))
+
+    want = step()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = step()
+    side.synchronize()
+    assert _same(got, want)
