@@ -9,13 +9,16 @@
 //
 // Instructions bound it before the memory does, so the inner loop is kept short:
 // * a key's nibble needs one logical operation: left in place in an otherwise empty 16-bit number
-//   it is a subnormal (or the first normal binade, which continues them), worth code 2^-133 in bf16
-//   and code 2^-24 in fp16, 16 times that four bits higher. The factors are powers of two: 1/16
-//   goes to the queries of those channels; each query row is brought by another to the top of its
-//   type's range, where neither it nor the products lose bits; the scores take both back. Values'
-//   nibbles go the same way as fp16, all at bits 4 to 7 (code 2^-20): the instruction adds its
-//   products on a grid set by their operands' exponent fields, and at bits 0 to 3, with the field of
-//   a number 64 to 1024 times larger, it cuts four bits more off (122 us; 119 without the shifts).
+//   it is a subnormal (or the first normal binade, which continues them), worth code 2^-133 in bf16, 16
+//   times that four bits higher. The factors are powers of two: 1/16 goes to the queries of those channels;
+//   each query row is brought by another to the top of its type's range, where neither it nor the
+//   products lose bits; the scores take both back.
+// * the instruction adds its products on a grid set by their operands' exponent fields, and a subnormal's
+//   field is that of a larger number: at bits 0 to 3 of a bf16 8 to 128 times (code 15 to 1), of an fp16 64 to
+//   1024 times, so that what is much smaller than the largest product loses bits. fp16 keys, and all values, which are fp16 here,
+//   are therefore shifted to bits 4 to 7 (code 2^-20), two operations more of each eight nibbles (keys: 123 ->
+//   128 us, and with one channel of the queries 256 times the others an error of 3e-6 for 2.4e-5, that of
+//   32-bit operations being 6e-7 and the result's rounding 1.8e-5; values: 119 -> 122 us).
 // * sums of codes do not drift: tokens 8 to 15 of a run count down from the group's top, k = (m + 15 s)
 //   - s (15 - c), for nothing (the complement is part of the mask, the sign of the step), so
 //   that what is summed has no common sign. The instruction still cuts off where it adds, so every
@@ -86,9 +89,11 @@ __device__ __forceinline__ void kv_mma<__half>(float (&d)[4], const uint32_t (&a
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// Nibbles p and p + 4 of w as a pair of 16-bit numbers: the integer code, times 16 for odd p, as a
-// subnormal of either 16-bit type.
-__device__ __forceinline__ uint32_t kv_pair_bare(uint32_t w, int p) {
+// Nibbles p and p + 4 of a word of keys as a pair of 16-bit numbers, the code as a subnormal (or the first
+// normal binade): in bf16 left where they stand, at bits 0 to 3 or, times 16, 4 to 7; in fp16 all at bits 4 to 7.
+template <typename T>
+__device__ __forceinline__ uint32_t kv_key_pair(uint32_t w, int p) {
+  if constexpr (std::is_same<T, __half>::value) return (p == 0 ? w << 4 : w >> (4 * p - 4)) & 0x00f000f0u;
   if (p & 2) w >>= 8;
   return w & (p & 1 ? 0x00f000f0u : 0x000f000fu);
 }
@@ -98,8 +103,8 @@ __device__ __forceinline__ void kv_values(uint32_t (&a)[4], uint32_t w) {
   constexpr uint32_t kMask = 0x00f000f0u;
   a[0] = w << 4 & kMask, a[1] = w & kMask, a[2] = ~(w >> 4) & kMask, a[3] = ~(w >> 8) & kMask;
 }
-// Where a query row's largest entry is put (its exponent), and what its type makes of the code 1
-// (the negative exponent). Scores are built from queries brought to 2^-kKvSpare, so that keys of any
+// Where a query row's largest entry is put (its exponent), what its type makes of the code 1 (the
+// negative exponent), and the factor of the queries that meet nibbles 1 and 3. Scores are built from queries brought to 2^-kKvSpare, so that keys of any
 // size give finite ones, and multiplied by what that takes back, the scale included, as the last step.
 constexpr int kKvSpare = 8;
 template <typename T>
@@ -107,10 +112,12 @@ struct KvKey;
 template <>
 struct KvKey<__nv_bfloat16> {
   static constexpr int kTop = 100, kOne = 133;
+  static constexpr float kOdd = 0.0625f;
 };
 template <>
 struct KvKey<__half> {
-  static constexpr int kTop = 13, kOne = 24;
+  static constexpr int kTop = 13, kOne = 20;
+  static constexpr float kOdd = 1.f;
 };
 __device__ __forceinline__ float kv_power(int e) { return __int_as_float((max(-126, min(127, e)) + 127) << 23); }
 // The power of two that brings a row whose largest entry has these bits (32-bit float, no sign) to
@@ -130,6 +137,7 @@ __device__ __forceinline__ uint32_t kv_transpose(uint32_t x) {  // an 8 x 8 matr
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
   return r;
 }
+// 2^x to within 2 units in the last place of 32 bits, which is what the scores are good for.
 __device__ __forceinline__ float kv_exp2(float x) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
@@ -367,7 +375,7 @@ __global__ void __launch_bounds__(32 * kKvWarps, kv_ctas(kGroups, kNT)) kv4_atte
     for (int i = 0; i < kSteps / kKvWarps; ++i) {
       alignas(8) T x[4];
       put2(x, to_f32(qv[n][i][0]) * up, to_f32(qv[n][i][1]) * up);
-      put2(x + 2, to_f32(qv[n][i][2]) * (up / 16), to_f32(qv[n][i][3]) * (up / 16));
+      put2(x + 2, to_f32(qv[n][i][2]) * (up * KvKey<T>::kOdd), to_f32(qv[n][i][3]) * (up * KvKey<T>::kOdd));
       s_q[n][i * kKvWarps + warp][lane] = *reinterpret_cast<uint2*>(x);
     }
     const int lift0 = lift(n, 2 * t) - KvKey<T>::kTop, lift1 = lift(n, 2 * t + 1) - KvKey<T>::kTop;
@@ -432,8 +440,8 @@ __global__ void __launch_bounds__(32 * kKvWarps, kv_ctas(kGroups, kNT)) kv4_atte
             for (int n = 0; n < kNT; ++n) q[n] = s_q[n][j][lane];
 #pragma unroll
             for (int i = 0; i < kRuns; ++i) {
-              const uint32_t a[4] = {kv_pair_bare(kc[i][0][j >> 1], p), kv_pair_bare(kc[i][1][j >> 1], p),
-                                     kv_pair_bare(kc[i][0][j >> 1], p + 1), kv_pair_bare(kc[i][1][j >> 1], p + 1)};
+              const uint32_t a[4] = {kv_key_pair<T>(kc[i][0][j >> 1], p), kv_key_pair<T>(kc[i][1][j >> 1], p),
+                                     kv_key_pair<T>(kc[i][0][j >> 1], p + 1), kv_key_pair<T>(kc[i][1][j >> 1], p + 1)};
 #pragma unroll
               for (int n = 0; n < kNT; ++n) kv_mma<T>(acc[i][n], a, q[n].x, q[n].y);
             }

@@ -385,3 +385,26 @@ def test_operators_take_the_tensors_stream():
         got = step()
     side.synchronize()
     assert _same(got, want)
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("large", [1.0, 256.0, 4096.0])
+def test_attention_with_one_large_channel(large, dtype):
+    """One channel of the queries far above the others, over keys that hold the same there: it takes no part in the softmax,
+    but the small channels' products must keep their bits beside it. A score is off by 16 units of 2^-24 of its terms'
+    sum at the most (128 products, each cut or rounded: the root of that, and some more), and an output by so
+    much of its size, beside its own rounding; as root mean squares."""
+    tokens, dim = 400, 128
+    cache = qr.kv4_cache(7, 64, 1, dim, 128, dtype)
+    k, v = _randn(tokens, 1, dim, seed=190, dtype=dtype).clamp(-3, 3), _randn(tokens, 1, dim, seed=191, dtype=dtype)
+    k[..., 5], k[..., 7] = 3, -3
+    qr.kv4_write(cache, k, v, torch.arange(tokens, device="cuda"))
+    q = _randn(1, 1, 32, dim, seed=192, dtype=dtype)
+    q[..., 5] = large
+    table = torch.arange(7, dtype=torch.int32, device="cuda")[None]
+    got = qr.kv4_attention(q, cache, table, torch.tensor([tokens], dtype=torch.int32, device="cuda"))[0, 0].double()
+    keys, values = (x[:tokens, 0] for x in _values(cache))
+    want = ((q[0, 0].double() @ keys.T) * dim**-0.5).softmax(-1) @ values
+    terms = ((q[0, 0].double().abs() @ keys.abs().T) * dim**-0.5).max()
+    rms = lambda x: x.square().mean().sqrt()  # noqa: E731
+    assert rms(got - want) <= (rms(want.to(dtype).double() - want).square() + (16 * 2.0**-24 * terms * rms(want)).square()).sqrt() * 1.02
