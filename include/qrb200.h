@@ -175,7 +175,7 @@ int qrb200_dequantize_int8(const int8_t* q, int64_t q_stride, const float* scale
 
 /* y[i, n] = (sum_k x[i, k] w[n, k]) x_scale[i] w_scale[n] + bias[n]: y rows x outs of dtype,
  * contiguous, 16-byte aligned; bias (may be NULL) of dtype; row strides of x and w in bytes. The sum is
- * exact in 32-bit integers for depth <= QRB200_INT8_MAX_DEPTH. Operands whose rows start on 16-byte
+ * exact in 32-bit integers for depth <= QRB200_INT8_MAX_DEPTH, and scaled in 32 bits. Operands whose rows start on 16-byte
  * boundaries are read as they lie; others are first laid out in the workspace (256-byte aligned, its
  * size from the query; 0 for the former). */
 #define QRB200_INT8_MAX_DEPTH 131071
@@ -215,8 +215,8 @@ int qrb200_kv4_read(const void* cache, const qrb200_kv4_shape* shape, void* k, v
  * batch x max_pages pages, rows table_stride apart; entries past a sequence's length, or behind
  * every query's window, are not read.
  * lengths: batch, tokens in the cache, the queries' own among them: query i stands at position
- * lengths - queries + i. It sees the tokens up to its position (all of them when causal is 0),
- * and of those the last `window` up to its position when window > 0. out: batch x queries x q_heads x head_dim,
+ * lengths - queries + i. It sees the tokens up to its position (to the end when causal is 0), when
+ * window > 0 only from its position - window + 1 on. out: batch x queries x q_heads x head_dim,
  * contiguous; zeros where nothing is seen. scale >= 0. q_heads <= 65535, queries x q_heads / kv_heads <= 2^24,
  * batch x queries x q_heads < 2^31, (max_pages + 320) x page_size < 2^31. Workspace as the query says,
  * 256-byte aligned. */

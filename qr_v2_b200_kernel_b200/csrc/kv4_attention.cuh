@@ -24,7 +24,7 @@
 //   that what is summed has no common sign. The instruction still cuts off where it adds, so every
 //   eighth step the sums are set aside: added, rounded to nearest, to sums in shared memory. The
 //   result's error is then some units of 2^-24 of the values at any length (of fp16 outputs over 8192
-//   tokens 0.8 % are not the nearest, 0.3 % of those of 32-bit operations throughout; 20 %
+//   tokens 0.7 % are not the nearest, 0.3 % of those of 32-bit operations throughout; 20 %
 //   with codes counted up and half the bits cut), for the same time.
 // * the weights p_t s_t are the only rounded operand: two fp16 numbers each, high and low, 22 bits
 //   in all (one alone would add an error the size of the result's own rounding). They are scaled by
@@ -38,8 +38,8 @@
 // of the operand's registers. The token range is cut over CTAs (blockIdx.x % splits) and over a CTA's four
 // warps; the parts are joined through shared memory and, between CTAs, through the cluster's shared
 // memory (up to eight) or by kv4_join_kernel, always in a fixed order.
-// 64 sequences x 8192 tokens, 64 heads on 8: 123 us, 4.7 TB/s of cache; 1 x 65536 30 us; one of
-// 513 tokens 6.5 us, which is latency from end to end.
+// 64 sequences x 8192 tokens, 64 heads on 8: 124 us, 4.6 TB/s of cache; 1 x 65536 30 us; one of
+// 513 tokens 6.6 us, which is latency from end to end.
 #pragma once
 
 #include <type_traits>

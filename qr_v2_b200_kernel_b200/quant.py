@@ -82,7 +82,8 @@ def int8_linear(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor, we
     ``x`` int8 (..., depth) with a float32 scale for each row (token), ``weight`` int8 (outs, depth)
     with a float32 scale for each output channel, as :func:`rms_norm_int8` and :func:`quantize_int8`
     make them; ``bias`` (outs,) of ``dtype``. 1 <= depth <= 131071. The products are summed exactly,
-    in 32-bit integers, and the result is rounded once. Beyond two rows, operands whose rows do not
+    in 32-bit integers; the sum is converted, scaled and given the bias in 32-bit floating point, and the result
+    rounded once to ``dtype``. Beyond two rows, operands whose rows do not
     start on 16-byte boundaries are laid out anew first; those that the quantising functions return
     do.
     """
@@ -170,13 +171,15 @@ def kv4_attention(q: torch.Tensor, cache: KV4Cache, block_table: torch.Tensor, l
 
     ``q`` (batch, queries, heads, head_dim) of the cache's type, heads a multiple of kv_heads (head
     h reads key head h // (heads // kv_heads)). ``block_table`` int32 (batch, max_pages): the pages
-    of each sequence in order; entries past its length, or behind every query's window, are not read. ``lengths`` int32 (batch,):
-    tokens in the cache, the queries' own included, so query i stands at position lengths - queries
-    + i. It sees every token up to its position (all tokens with ``causal=False``), or the last
-    ``window`` of those up to its position. ``scale`` multiplies the scores (default head_dim **
-    -0.5). Rows that see nothing (an empty sequence, a position before its start) are zero. Returns
-    (batch, queries, heads, head_dim); the scores, the softmax and the sums are in 32 bits, the
-    result is rounded once. A length or page outside the table or the cache is left out and reported
-    by the next call as ``QRB200Error``.
+    of each sequence in order; entries past its length, or behind every query's window, are not
+    read. ``lengths`` int32 (batch,): tokens in the cache, the queries' own included, so query i
+    stands at position lengths - queries + i. It sees every token up to its position (to the end with
+    ``causal=False``), with ``window`` only those from position - window + 1 on. ``scale`` multiplies
+    the scores (default head_dim ** -0.5). Rows that see nothing (an empty sequence, a position before
+    its start) are zero. Returns (batch, queries, heads, head_dim), rounded once. Scores, softmax and sums
+    are in 32 bits at any length, the weights of the values in 22; the matrix instruction's cut-offs make
+    the error some units of 2^-24 of the values' size, a few times that of 32-bit operations
+    throughout. A length or page outside the table or the cache is left out and reported by the next
+    call as ``QRB200Error``; heads <= 65535, queries * heads / kv_heads <= 2^24.
     """
     return (_module or _native()).kv4_attention(q, _handle(cache), block_table, lengths, scale, causal, window)
