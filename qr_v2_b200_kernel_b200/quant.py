@@ -112,6 +112,9 @@ class KV4Cache:
     def __setattr__(self, name, value):  # the handle would go on with what it was made of
         raise AttributeError(f"a KV4Cache's {name} cannot be assigned")
 
+    def __reduce__(self):  # copy.copy shares the bytes, copy.deepcopy and pickle copy them
+        return KV4Cache, (self.data, self.page_size, self.head_dim, self.group_size, self.dtype)
+
 
 def kv4_cache(pages: int, page_size: int, kv_heads: int, head_dim: int, group_size: int | None = None,
               dtype: torch.dtype = torch.bfloat16, device="cuda") -> KV4Cache:

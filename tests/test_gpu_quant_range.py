@@ -4,6 +4,9 @@ numbers at either end of a type, indexes that no query needs, captured calls.
 Each check derives its own tolerance; U is the unit roundoff of a type.
 """
 
+import copy
+import pickle
+
 import pytest
 import torch
 from test_gpu_quant import BF, HF, SF, U, _attend64, _case, _check_rows, _randn, _values
@@ -408,3 +411,16 @@ def test_attention_with_one_large_channel(large, dtype):
     terms = ((q[0, 0].double().abs() @ keys.abs().T) * dim**-0.5).max()
     rms = lambda x: x.square().mean().sqrt()  # noqa: E731
     assert rms(got - want) <= (rms(want.to(dtype).double() - want).square() + (16 * 2.0**-24 * terms * rms(want)).square()).sqrt() * 1.02
+
+
+def test_copies_of_a_cache():
+    """copy.copy is another handle on the same bytes; copy.deepcopy and pickle have their own."""
+    q, cache, table, n = _case([20, 30], 1, 2, 2, 16, 64, 32, BF, seed=200)
+    want = qr.kv4_attention(q, cache, table, n)
+    shared, own, stored = copy.copy(cache), copy.deepcopy(cache), pickle.loads(pickle.dumps(cache))
+    for other in (shared, own, stored):
+        assert torch.equal(want, qr.kv4_attention(q, other, table, n))
+        assert (other.group_size, other.kv_heads, other.dtype) == (32, 2, BF)
+    cache.data.zero_()
+    assert not qr.kv4_attention(q, shared, table, n).any()
+    assert torch.equal(want, qr.kv4_attention(q, own, table, n)) and torch.equal(want, qr.kv4_attention(q, stored, table, n))
