@@ -217,7 +217,7 @@ int qrb200_kv4_read(const void* cache, const qrb200_kv4_shape* shape, void* k, v
  * lengths: batch, tokens in the cache, the queries' own among them: query i stands at position
  * lengths - queries + i. It sees the tokens up to its position (to the end when causal is 0), when
  * window > 0 only from its position - window + 1 on. out: batch x queries x q_heads x head_dim,
- * contiguous; zeros where nothing is seen. scale >= 0. q_heads <= 65535, queries x q_heads / kv_heads <= 2^24,
+ * contiguous; zeros where nothing is seen (values beyond 2^100 may sum past 32 bits' range before the division). scale >= 0. q_heads <= 65535, queries x q_heads / kv_heads <= 2^24,
  * batch x queries x q_heads < 2^31, (max_pages + 320) x page_size < 2^31. Workspace as the query says,
  * 256-byte aligned. */
 size_t qrb200_kv4_attention_workspace_bytes(const qrb200_kv4_shape* shape, int64_t batch, int64_t queries,

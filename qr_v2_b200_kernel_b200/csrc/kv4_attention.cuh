@@ -144,14 +144,10 @@ __device__ __forceinline__ float kv_exp2(float x) {
   return r;
 }
 // What a part with this (maximum, sum) counts against the maximum m of all: nothing where it saw
-// nothing, NaN where its scores were.
+// nothing, NaN where its scores were. (A part is added even if its weight underflows to 0: a value that is
+// NaN makes the result NaN, wherever the parts are cut. One that saw nothing holds zeros.)
 __device__ __forceinline__ float kv_part_weight(float2 ml, float m) {
   return ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : ml.y) : kv_exp2(ml.x - m);
-}
-// x and a part's sum that counts f. One that counts nothing may have left the range, but a value that
-// is NaN makes the result NaN, wherever the parts are cut.
-__device__ __forceinline__ float kv_join(float x, float f, float part) {
-  return f == 0.f && part == part ? x : fmaf(f, part, x);
 }
 template <int kWords>
 __device__ __forceinline__ void kv_load(uint32_t (&w)[kWords], const unsigned char* p) {  // from shared memory
@@ -700,7 +696,7 @@ __global__ void __launch_bounds__(32 * kKvWarps, kv_ctas(kGroups, kNT)) kv4_atte
   const auto joined = [&](int d) {
     float x = 0.f;
 #pragma unroll
-    for (int w = 0; w < kKvWarps; ++w) x = kv_join(x, f[w], s_o[w][r][d]);
+    for (int w = 0; w < kKvWarps; ++w) x = fmaf(f[w], s_o[w][r][d], x);
     return x;
   };
   if (P.splits == 1) {
@@ -746,9 +742,7 @@ __global__ void __launch_bounds__(32 * kKvWarps, kv_ctas(kGroups, kNT)) kv4_atte
 #pragma unroll
       for (int c = 0; c < kKvCluster; ++c) v[c] = c < P.splits ? __int_as_float(ld_cluster(smem_u32(&s_o[0][row][d]), c)) : 0.f;
 #pragma unroll
-      for (int c = 0; c < kKvCluster; ++c) {
-        x = kv_join(x, s_w[row][c], v[c]);
-      }
+      for (int c = 0; c < kKvCluster; ++c) x = fmaf(s_w[row][c], v[c], x);
       out_row(row)[d] = from_f32<T>(x * s_w[row][kKvCluster]);
     }
     cluster_sync();  // nobody leaves while its part is being read
@@ -771,10 +765,16 @@ __global__ void __launch_bounds__(32 * kKvJoinWarps) kv4_join_kernel(Kv4AttnPara
   const long long part =
       (((long long)b * P.sh.heads + head) * P.tiles + r / tile_rows) * P.splits * tile_rows + r % tile_rows;
   float m = -INFINITY, l = 0.f, x[kDim / 32] = {};
-  for (int s = lane; s < P.splits; s += 32) m = fmaxf(m, P.part_ml[part + (long long)s * tile_rows].x);
+  int end = 0;  // of the parts that saw something: a table wider than the sequence leaves the last ones empty
+  for (int s = lane; s < P.splits; s += 32) {
+    const float2 ml = P.part_ml[part + (long long)s * tile_rows];
+    m = fmaxf(m, ml.x);
+    if (!(ml.x == -INFINITY && ml.y == 0.f)) end = s + 1;
+  }
   for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(kFullMask, m, o));
+  end = __reduce_max_sync(kFullMask, end);
 #pragma unroll 8
-  for (int s = warp; s < P.splits; s += kKvJoinWarps) {
+  for (int s = warp; s < end; s += kKvJoinWarps) {
     const float2 ml = P.part_ml[part + (long long)s * tile_rows];
     const float* o = P.part_o + (part + (long long)s * tile_rows) * kDim;
     const float f = kv_part_weight(ml, m);
@@ -782,7 +782,7 @@ __global__ void __launch_bounds__(32 * kKvJoinWarps) kv4_join_kernel(Kv4AttnPara
 #pragma unroll
     for (int i = 0; i < kDim / 32; ++i) {
       const float v = o[32 * i + lane];
-      x[i] = kv_join(x[i], f, v);
+      x[i] = fmaf(f, v, x[i]);
     }
   }
 #pragma unroll
