@@ -199,8 +199,7 @@ int64_t qrb200_kv4_block_bytes(int64_t page_size, int64_t head_dim, int64_t grou
  * contiguous, other strides in elements) into the cache at slots (page * page_size + offset). A
  * negative slot is skipped; slots of one call must differ. A group's step and minimum are its
  * range / 15 (a step less in the last place if its top would pass the type's largest number) and its
- * least entry, its codes the nearest steps; a group with a NaN or an infinity
- * reads back as NaN. */
+ * least entry, its codes the nearest steps; a group with a NaN or an infinity reads back as NaN. */
 int qrb200_kv4_write(void* cache, const qrb200_kv4_shape* shape, const void* k, int64_t k_token_stride,
                      int64_t k_head_stride, const void* v, int64_t v_token_stride, int64_t v_head_stride,
                      const int64_t* slots, int64_t tokens, void* stream);
@@ -217,9 +216,9 @@ int qrb200_kv4_read(const void* cache, const qrb200_kv4_shape* shape, void* k, v
  * lengths: batch, tokens in the cache, the queries' own among them: query i stands at position
  * lengths - queries + i. It sees the tokens up to its position (to the end when causal is 0), when
  * window > 0 only from its position - window + 1 on. out: batch x queries x q_heads x head_dim,
- * contiguous; zeros where nothing is seen (values beyond 2^100 may sum past 32 bits' range before the division). scale >= 0. q_heads <= 65535, queries x q_heads / kv_heads <= 2^24,
- * batch x queries x q_heads < 2^31, (max_pages + 320) x page_size < 2^31. Workspace as the query says,
- * 256-byte aligned. */
+ * contiguous; zeros where nothing is seen (values beyond 2^100 may sum past 32 bits' range before the
+ * division). scale >= 0. q_heads <= 65535, queries x q_heads / kv_heads <= 2^24, batch x queries x
+ * q_heads < 2^31, (max_pages + 320) x page_size < 2^31. Workspace as the query says, 256-byte aligned. */
 size_t qrb200_kv4_attention_workspace_bytes(const qrb200_kv4_shape* shape, int64_t batch, int64_t queries,
                                             int64_t q_heads, int64_t max_pages, int64_t window);
 int qrb200_kv4_attention(const void* q, const int64_t* q_strides, const void* cache, const qrb200_kv4_shape* shape,
