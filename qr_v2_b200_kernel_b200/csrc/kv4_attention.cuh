@@ -104,8 +104,9 @@ __device__ __forceinline__ void kv_values(uint32_t (&a)[4], uint32_t w) {
   a[0] = w << 4 & kMask, a[1] = w & kMask, a[2] = ~(w >> 4) & kMask, a[3] = ~(w >> 8) & kMask;
 }
 // Where a query row's largest entry is put (its exponent), what its type makes of the code 1 (the
-// negative exponent), and the factor of the queries that meet nibbles 1 and 3. Scores are built from queries brought to 2^-kKvSpare, so that keys of any
-// size give finite ones, and multiplied by what that takes back, the scale included, as the last step.
+// negative exponent), and the factor of the queries that meet nibbles 1 and 3. Scores are built from
+// queries brought to 2^-kKvSpare, so that keys of any size give finite ones, and multiplied by what
+// takes that back, the scale included, as the last step.
 constexpr int kKvSpare = 8;
 template <typename T>
 struct KvKey;
