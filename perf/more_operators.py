@@ -243,8 +243,10 @@ def _to_fp8(x, tile):
     full[:rows, :cols] = f.abs()
     a = full.reshape(-1, tile, _blocks(cols), BLOCK).amax((1, 3))
     fine = a >= TINY
-    # The quotient in 64 bits: entries of 16 bits often lie midway between two codes, or next to that.
+    # In 64 bits: entries often lie midway between two codes, or so near that 32 bits lose on which side.
     q = f.double() * 448.0 / _spread(torch.where(fine, a, math.inf), rows, cols, tile)
+    power = torch.clamp(torch.frexp(q).exponent, min=-5) - 4  # of the codes' spacing
+    q = torch.ldexp(torch.round(torch.ldexp(q, -power)), power)
     return q.float().to(torch.float8_e4m3fn), torch.where(fine, a / 448.0, 0.0)
 
 
@@ -359,7 +361,7 @@ def _exact_fp8(x, tile):
         if tile > 1:
             top = torch.stack([t.amax() for t in top.split(tile)]).repeat_interleave(tile)[:rows]
         scale = top / 448
-        q = part / scale[:, None]
+        q = part * 448 / top[:, None]
         step = torch.exp2(torch.clamp(torch.floor(torch.log2(q.abs().clamp(min=2.0**-20))), min=-6) - 3)
         values[:, c : c + BLOCK] = (q / step).round() * step * scale[:, None]
         scales.append(scale[::tile])
