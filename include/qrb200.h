@@ -226,6 +226,66 @@ int qrb200_kv4_attention(const void* q, const int64_t* q_strides, const void* ca
                          int64_t batch, int64_t queries, int64_t q_heads, int64_t max_pages, int64_t window,
                          int causal, float scale, void* workspace, size_t workspace_bytes, void* stream);
 
+/* 8-bit floating point (e4m3: 448 is the largest number) with a scale for each block: 128 entries of a row
+ * (tile_rows 1), or 128 rows and 128 columns (tile_rows QRB200_FP8_BLOCK); the last blocks of a row or column
+ * may be smaller. scale = a / 448 with a = the block's largest magnitude; code = the number nearest to
+ * 448 x / a, ties to even, as if that quotient were exact (of QRB200_F32 entries as near as 64 bits tell). A
+ * block with a NaN or an infinity gets codes 0 and a NaN scale; one whose a is below 2^-100 codes and
+ * scale 0. x: rows x cols of dtype, q: rows x cols bytes, row strides in elements and bytes; scale:
+ * ceil(rows / tile_rows) x ceil(cols / 128), contiguous. cols <= QRB200_FP8_MAX_DEPTH. */
+#define QRB200_FP8_BLOCK 128
+#define QRB200_FP8_MAX_DEPTH 1048576
+int qrb200_quantize_fp8(const void* x, int64_t x_stride, uint8_t* q, int64_t q_stride, float* scale, int64_t rows, int64_t cols,
+                        int tile_rows, int dtype, void* stream);
+
+/* out (rows x cols of dtype, contiguous) = q * scale of its block, rounded once. */
+int qrb200_dequantize_fp8(const uint8_t* q, int64_t q_stride, const float* scale, void* out, int64_t rows, int64_t cols,
+                          int tile_rows, int dtype, void* stream);
+
+/* y[i, n] = sum_b (sum_{k in block b} x[i, k] w[n, k]) x_scale[i, b] w_scale[n / 128, b] + bias[n]: x and w of e4m3, blocks of 128
+ * along the depth. y: rows x outs of dtype, contiguous, 16-byte aligned; bias (may be NULL) of dtype; row strides of x and w in
+ * bytes; x_scale: rows x ceil(depth / 128), w_scale: ceil(outs / 128) x ceil(depth / 128), contiguous. Sums are in 32-bit floating point, a
+ * block's before its scales and theirs. Operands whose rows start on 16-byte boundaries are read as they lie; others
+ * may first be laid out in the workspace (256-byte aligned, its size from the query). */
+size_t qrb200_fp8_linear_workspace_bytes(const uint8_t* x, int64_t x_stride, const uint8_t* w, int64_t w_stride, int64_t rows,
+                                         int64_t outs, int64_t depth);
+int qrb200_fp8_linear(const uint8_t* x, int64_t x_stride, const float* x_scale, const uint8_t* w, int64_t w_stride,
+                      const float* w_scale, const void* bias, void* y, int64_t rows, int64_t outs, int64_t depth, int dtype,
+                      void* workspace, size_t workspace_bytes, void* stream);
+
+/* A paged key/value cache in 8 bits: codes, pages x kv_heads blocks of qrb200_kv8_block_bytes bytes, contiguous,
+ * 16-byte aligned, and range, pages x kv_heads x 2 floats (keys, values). A code c, from -127 to 127, of a page and head stands
+ * for c range / 127. dtype QRB200_BF16 or QRB200_F16, of the keys, values and queries; head_dim 64 or 128; page_size a power
+ * of two from 16 to 1024. */
+typedef struct qrb200_kv8_shape {
+  int64_t pages;
+  int32_t kv_heads, page_size, head_dim, dtype;
+} qrb200_kv8_shape;
+int64_t qrb200_kv8_block_bytes(int64_t page_size, int64_t head_dim);
+
+/* Writes keys and values (tokens x kv_heads x head_dim of the cache's type, channels contiguous, other strides in
+ * elements) at slots (page * page_size + offset), in any order, each at most once; a negative slot is skipped. A page's range
+ * becomes the largest of what it was and of the magnitudes written, rounded up to three significant bits; codes are
+ * rint(127 x / range), and those of its other tokens, where the range grew, rint(c old / range). A call that writes a page's
+ * first token begins it anew, the rest of it as zeros. A NaN or an infinity makes the range NaN until
+ * then. Only one call at a time may write a page. Workspace as the query says, 256-byte aligned. */
+size_t qrb200_kv8_write_workspace_bytes(const qrb200_kv8_shape* shape, int64_t tokens);
+int qrb200_kv8_write(void* codes, float* range, const qrb200_kv8_shape* shape, const void* k, int64_t k_token_stride,
+                     int64_t k_head_stride, const void* v, int64_t v_token_stride, int64_t v_head_stride, const int64_t* slots,
+                     int64_t tokens, void* workspace, size_t workspace_bytes, void* stream);
+
+/* The values at slots, as tokens x kv_heads x head_dim, contiguous, 16-byte aligned; zeros for a negative slot. */
+int qrb200_kv8_read(const void* codes, const float* range, const qrb200_kv8_shape* shape, void* k, void* v, const int64_t* slots,
+                    int64_t tokens, void* stream);
+
+/* qrb200_kv4_attention over this cache: operands, masks and limits as there. */
+size_t qrb200_kv8_attention_workspace_bytes(const qrb200_kv8_shape* shape, int64_t batch, int64_t queries, int64_t q_heads,
+                                            int64_t max_pages, int64_t window);
+int qrb200_kv8_attention(const void* q, const int64_t* q_strides, const void* codes, const float* range,
+                         const qrb200_kv8_shape* shape, const int32_t* block_table, int64_t table_stride, const int32_t* lengths,
+                         void* out, int64_t batch, int64_t queries, int64_t q_heads, int64_t max_pages, int64_t window, int causal,
+                         float scale, void* workspace, size_t workspace_bytes, void* stream);
+
 /* ---- diagnostics (no counterpart in the reference; used by bench.py) ---------------- */
 
 /* The three 3xTF32 tcgen05 GEMMs of the 128-wide trailing update on their own, for accuracy

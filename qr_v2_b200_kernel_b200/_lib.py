@@ -36,6 +36,13 @@ class KV4Shape(ctypes.Structure):
                 ("head_dim", ctypes.c_int32), ("groups", ctypes.c_int32), ("dtype", ctypes.c_int32)]
 
 
+class KV8Shape(ctypes.Structure):
+    """``qrb200_kv8_shape`` of include/qrb200.h."""
+
+    _fields_ = [("pages", ctypes.c_int64), ("kv_heads", ctypes.c_int32), ("page_size", ctypes.c_int32),
+                ("head_dim", ctypes.c_int32), ("dtype", ctypes.c_int32)]
+
+
 _P, _I64, _INT, _F32, _SIZE = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_float, ctypes.c_size_t
 
 # Every symbol include/qrb200.h declares, with its ctypes signature.
@@ -76,6 +83,17 @@ SIGNATURES = {
     "qrb200_kv4_read": (_INT, [_P, _P, _P, _P, _P, _I64, _P]),
     "qrb200_kv4_attention_workspace_bytes": (_SIZE, [_P, _I64, _I64, _I64, _I64, _I64]),
     "qrb200_kv4_attention": (_INT, [_P, _P, _P, _P, _P, _I64, _P, _P, _I64, _I64, _I64, _I64, _I64, _INT, _F32, _P,
+                                    _SIZE, _P]),
+    "qrb200_quantize_fp8": (_INT, [_P, _I64, _P, _I64, _P, _I64, _I64, _INT, _INT, _P]),
+    "qrb200_dequantize_fp8": (_INT, [_P, _I64, _P, _P, _I64, _I64, _INT, _INT, _P]),
+    "qrb200_fp8_linear_workspace_bytes": (_SIZE, [_P, _I64, _P, _I64, _I64, _I64, _I64]),
+    "qrb200_fp8_linear": (_INT, [_P, _I64, _P, _P, _I64, _P, _P, _P, _I64, _I64, _I64, _INT, _P, _SIZE, _P]),
+    "qrb200_kv8_block_bytes": (_I64, [_I64, _I64]),
+    "qrb200_kv8_write_workspace_bytes": (_SIZE, [_P, _I64]),
+    "qrb200_kv8_write": (_INT, [_P, _P, _P, _P, _I64, _I64, _P, _I64, _I64, _P, _I64, _P, _SIZE, _P]),
+    "qrb200_kv8_read": (_INT, [_P, _P, _P, _P, _P, _P, _I64, _P]),
+    "qrb200_kv8_attention_workspace_bytes": (_SIZE, [_P, _I64, _I64, _I64, _I64, _I64]),
+    "qrb200_kv8_attention": (_INT, [_P, _P, _P, _P, _P, _P, _I64, _P, _P, _I64, _I64, _I64, _I64, _I64, _INT, _F32, _P,
                                     _SIZE, _P]),
 }
 

@@ -19,7 +19,7 @@ REPO_DIR = os.path.dirname(PKG_DIR)
 CSRC = os.path.join(PKG_DIR, "csrc")
 LIB_NAME = "libqrb200.so"
 LIB_PATH = os.path.join(PKG_DIR, LIB_NAME)
-SOURCES = ["qrb200.cu", "quant.cu", "noalloc.cu"]
+SOURCES = ["qrb200.cu", "quant.cu", "fp8.cu", "kv8.cu", "noalloc.cu"]
 NATIVE_PATH = os.path.join(PKG_DIR, "_native.so")
 NATIVE_SOURCE = os.path.join(CSRC, "native.cpp")
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]

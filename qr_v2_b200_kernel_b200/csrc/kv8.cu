@@ -1,0 +1,156 @@
+// C ABI of the 8-bit key/value cache: argument checks, choice of kernel, launches.
+#include "launch.h"
+#include "kv8.cuh"
+#include "kv8_attention.cuh"
+
+namespace qrb200 {
+
+static bool shape_of(const qrb200_kv8_shape* s, Kv8Shape* h) {
+  if (!s || !type16_ok(s->dtype)) return false;
+  *h = Kv8Shape{s->kv_heads, s->page_size, s->head_dim, page_shift(s->page_size), s->pages};
+  return h->pages >= 0 && h->pages <= kMaxRows && h->heads > 0 && h->heads <= 65535 && (h->dim == 64 || h->dim == 128) &&
+         h->page >= 16 && h->page <= 1024 && (h->page & (h->page - 1)) == 0;
+}
+
+// f(type, dim) with both as types.
+template <typename F>
+static cudaError_t with_shape(int dtype, int dim, F&& f) {
+  if (dtype == QRB200_BF16) return dim == 64 ? f(__nv_bfloat16{}, Int<64>{}) : f(__nv_bfloat16{}, Int<128>{});
+  return dim == 64 ? f(__half{}, Int<64>{}) : f(__half{}, Int<128>{});
+}
+
+}  // namespace qrb200
+
+using namespace qrb200;
+
+int qrb200_internal_kv8_site() { return take_site(); }
+
+extern "C" {
+
+int64_t qrb200_kv8_block_bytes(int64_t page_size, int64_t head_dim) {
+  if (page_size < 16 || page_size > 1024 || (page_size & (page_size - 1)) != 0 || (head_dim != 64 && head_dim != 128)) return 0;
+  return 2 * page_size * head_dim;
+}
+
+size_t qrb200_kv8_write_workspace_bytes(const qrb200_kv8_shape* shape, int64_t tokens) {
+  Kv8Shape h;
+  if (!shape_of(shape, &h) || tokens <= kKv8Few) return 0;
+  return (size_t)h.pages * h.page * sizeof(int);
+}
+
+int qrb200_kv8_write(void* codes, float* range, const qrb200_kv8_shape* shape, const void* k, int64_t k_token_stride,
+                     int64_t k_head_stride, const void* v, int64_t v_token_stride, int64_t v_head_stride, const int64_t* slots,
+                     int64_t tokens, void* workspace, size_t workspace_bytes, void* stream) {
+  Kv8Shape h;
+  if (tokens < 0 || !shape_of(shape, &h) || tokens > kMaxRows / h.heads) return QRB200_ERR_ARG;
+  if (tokens == 0) return QRB200_OK;
+  if (!k || !v || !slots || (h.pages > 0 && (!codes || !range)) || (reinterpret_cast<uintptr_t>(codes) & 15u)) return QRB200_ERR_ARG;
+  const int st = quant_ready();
+  if (st != QRB200_OK) return st;
+  const size_t need = qrb200_kv8_write_workspace_bytes(shape, tokens);
+  if (need > 0 && (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 255u)))
+    return QRB200_ERR_WORKSPACE;
+  Kv8IoParams p{static_cast<unsigned char*>(codes), range, k, v, nullptr, nullptr, reinterpret_cast<const long long*>(slots),
+                need > 0 ? static_cast<int*>(workspace) : nullptr, tokens, k_token_stride, k_head_stride, v_token_stride,
+                v_head_stride, h, 1};
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (p.rows) {
+    LaunchShape l(dim3(ceil_div(tokens, 256)), 256, 0, s);
+    if (cudaLaunchKernelEx(&l.cfg, kv8_rows_kernel, p) != cudaSuccess) return QRB200_ERR_CUDA;
+    qrb200_internal_count_launch();
+    p.chunk = 32;
+  }
+  const cudaError_t e = with_shape(shape->dtype, h.dim, [&](auto type, auto dim) {
+    LaunchShape l(dim3(ceil_div(tokens, p.chunk), h.heads), 256, 0, s);
+    return cudaLaunchKernelEx(&l.cfg, kv8_write_kernel<decltype(type), dim()>, p);
+  });
+  if (e != cudaSuccess) return QRB200_ERR_CUDA;
+  return launched();
+}
+
+int qrb200_kv8_read(const void* codes, const float* range, const qrb200_kv8_shape* shape, void* k, void* v, const int64_t* slots,
+                    int64_t tokens, void* stream) {
+  Kv8Shape h;
+  if (tokens < 0 || !shape_of(shape, &h) || tokens > kMaxRows / h.heads) return QRB200_ERR_ARG;
+  if (tokens == 0) return QRB200_OK;
+  if (!k || !v || !slots || (h.pages > 0 && (!codes || !range)) ||
+      ((reinterpret_cast<uintptr_t>(codes) | reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15u))
+    return QRB200_ERR_ARG;
+  const int st = quant_ready();
+  if (st != QRB200_OK) return st;
+  const Kv8IoParams p{static_cast<unsigned char*>(const_cast<void*>(codes)), const_cast<float*>(range), nullptr, nullptr, k, v,
+                      reinterpret_cast<const long long*>(slots), nullptr, tokens, 0, 0, 0, 0, h, 1};
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const cudaError_t e = with_shape(shape->dtype, h.dim, [&](auto type, auto dim) {
+    LaunchShape l(dim3(ceil_div(tokens, 2048 / h.dim), h.heads), 256, 0, s);
+    return cudaLaunchKernelEx(&l.cfg, kv8_read_kernel<decltype(type), dim()>, p);
+  });
+  if (e != cudaSuccess) return QRB200_ERR_CUDA;
+  return launched();
+}
+
+// The launch grid is work x heads x batch, a large batch in several launches.
+constexpr int64_t kGridZ = 65535;
+static bool attention_args(const qrb200_kv8_shape* shape, int64_t batch, int64_t queries, int64_t q_heads, int64_t max_pages,
+                           Kv8Shape* h) {
+  if (batch < 0 || queries < 0 || q_heads < 0 || max_pages < 0 || !shape_of(shape, h)) return false;
+  return q_heads % h->heads == 0 && batch <= kMaxRows && q_heads <= 65535 && queries <= (1 << 24) &&
+         queries * (q_heads / h->heads) <= (1 << 24) && (queries * q_heads == 0 || batch <= kMaxRows / (queries * q_heads)) &&
+         max_pages <= kMaxRows / h->page - 320;
+}
+
+size_t qrb200_kv8_attention_workspace_bytes(const qrb200_kv8_shape* shape, int64_t batch, int64_t queries, int64_t q_heads,
+                                            int64_t max_pages, int64_t window) {
+  Kv8Shape h;
+  if (window < 0 || !attention_args(shape, batch, queries, q_heads, max_pages, &h)) return 0;
+  return 0;
+}
+
+int qrb200_kv8_attention(const void* q, const int64_t* q_strides, const void* codes, const float* range,
+                         const qrb200_kv8_shape* shape, const int32_t* block_table, int64_t table_stride, const int32_t* lengths,
+                         void* out, int64_t batch, int64_t queries, int64_t q_heads, int64_t max_pages, int64_t window, int causal,
+                         float scale, void* workspace, size_t workspace_bytes, void* stream) {
+  Kv8Shape h;
+  if (!q_strides || !(scale >= 0.f) || !(scale <= 3.0e38f) || window < 0 || !attention_args(shape, batch, queries, q_heads, max_pages, &h))
+    return QRB200_ERR_ARG;
+  if (batch == 0 || queries == 0 || q_heads == 0) return QRB200_OK;
+  if (!q || !out || !lengths || (max_pages > 0 && !block_table) || (reinterpret_cast<uintptr_t>(codes) & 15u) ||
+      (h.pages > 0 && (!codes || !range)) || table_stride < 0)
+    return QRB200_ERR_ARG;
+  const int st = quant_ready();
+  if (st != QRB200_OK) return st;
+  (void)workspace, (void)workspace_bytes;
+  Kv8AttnParams p{};
+  p.codes = static_cast<const unsigned char*>(codes);
+  p.range = range;
+  p.q = q;
+  p.out = out;
+  p.table = block_table;
+  p.lengths = lengths;
+  p.q_bs = q_strides[0], p.q_ts = q_strides[1], p.q_hs = q_strides[2], p.table_stride = table_stride;
+  p.batch = (int)batch, p.queries = (int)queries, p.q_heads = (int)q_heads, p.share = (int)(q_heads / h.heads);
+  // A window that reaches every token from every position is none (and cannot overflow a position).
+  p.window = window >= max_pages * h.page + queries ? 0 : (int)window;
+  p.max_pages = (int)max_pages, p.causal = causal;
+  p.scale = scale;
+  p.sh = h;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  for (int64_t b = 0; b < batch; b += kGridZ) {
+    Kv8AttnParams part = p;
+    part.batch = (int)std::min(kGridZ, batch - b);
+    part.q = static_cast<const char*>(q) + 2 * b * p.q_bs;
+    part.out = static_cast<char*>(out) + 2 * b * queries * q_heads * h.dim;
+    part.table += b * table_stride;
+    part.lengths += b;
+    const cudaError_t e = with_shape(shape->dtype, h.dim, [&](auto type, auto dim) {
+      LaunchShape l(dim3(ceil_div(queries, 4), q_heads, part.batch), 128, 0, s);
+      return cudaLaunchKernelEx(&l.cfg, kv8_simple_kernel<decltype(type), dim()>, part);
+    });
+    if (e != cudaSuccess) return QRB200_ERR_CUDA;
+    const int ended = launched();
+    if (ended != QRB200_OK) return ended;
+  }
+  return QRB200_OK;
+}
+
+}  // extern "C"

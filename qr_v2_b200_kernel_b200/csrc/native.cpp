@@ -217,7 +217,8 @@ Cache make_cache(const Tensor& data, int32_t page_size, int32_t head_dim, int32_
   return Cache{data, {data.size(0), (int32_t)data.size(1), page_size, head_dim, groups, type_code(type)}, type};
 }
 
-Tensor slots_operand(const Cache& c, const Tensor& slots) {
+template <typename C>  // either cache
+Tensor slots_operand(const C& c, const Tensor& slots) {
   operand(slots, "slots", {at::kLong}, &c.data);
   TORCH_CHECK_VALUE(slots.dim() == 1, "slots must be (tokens,), got ", shape_of(slots));
   return slots.contiguous();
@@ -250,8 +251,13 @@ py::tuple kv4_read(const Cache& c, const Tensor& slots) {
   return py::make_tuple(k, v);
 }
 
-Tensor kv4_attention(Tensor q, const Cache& c, Tensor table, Tensor lengths, std::optional<double> scale, bool causal,
-                     std::optional<int64_t> window) {
+// An attention call's operands, checked, and laid out where their strides need it.
+struct Reading {
+  int64_t batch, queries, heads, pages, window, strides[3];
+  float factor;
+};
+template <typename C>
+Reading reading(Tensor& q, const C& c, Tensor& table, Tensor& lengths, std::optional<double> scale, std::optional<int64_t> window) {
   operand(q, "q", {c.type}, &c.data);
   operand(table, "block_table", {at::kInt}, &c.data);
   operand(lengths, "lengths", {at::kInt}, &c.data);
@@ -270,17 +276,187 @@ Tensor kv4_attention(Tensor q, const Cache& c, Tensor table, Tensor lengths, std
   if (q.stride(3) != 1) q = q.contiguous();
   if (table.size(1) > 1 && table.stride(1) != 1) table = table.contiguous();
   lengths = lengths.contiguous();
+  return {batch, queries, heads, table.size(1), window.value_or(0), {q.stride(0), q.stride(1), q.stride(2)}, (float)factor};
+}
+
+Tensor kv4_attention(Tensor q, const Cache& c, Tensor table, Tensor lengths, std::optional<double> scale, bool causal,
+                     std::optional<int64_t> window) {
+  const Reading r = reading(q, c, table, lengths, scale, window);
+  OnDevice on(c.data);
   const Tensor out = empty(q.sizes(), c.type, c.data);
   if (out.numel() == 0) return out;
-  const int64_t pages = table.size(1);
-  const size_t need = qrb200_kv4_attention_workspace_bytes(&c.shape, batch, queries, heads, pages, window.value_or(0));
+  const size_t need = qrb200_kv4_attention_workspace_bytes(&c.shape, r.batch, r.queries, r.heads, r.pages, r.window);
   Tensor ws;
   if (need > 0) ws = empty({(int64_t)need}, at::kByte, c.data);
-  const int64_t strides[3] = {q.stride(0), q.stride(1), q.stride(2)};
-  check(qrb200_kv4_attention(ptr(q), strides, ptr(c.data), &c.shape, table.const_data_ptr<int32_t>(), table.stride(0),
-                             lengths.const_data_ptr<int32_t>(), out.data_ptr(), batch, queries, heads, pages,
-                             window.value_or(0), causal, (float)factor, need > 0 ? ws.data_ptr() : nullptr, need, on.stream),
+  check(qrb200_kv4_attention(ptr(q), r.strides, ptr(c.data), &c.shape, table.const_data_ptr<int32_t>(), table.stride(0),
+                             lengths.const_data_ptr<int32_t>(), out.data_ptr(), r.batch, r.queries, r.heads, r.pages, r.window,
+                             causal, r.factor, need > 0 ? ws.data_ptr() : nullptr, need, on.stream),
         "kv4_attention");
+  return out;
+}
+
+// ---- 8-bit floating point with a scale for each block ---------------------------------------
+
+int64_t blocks_of(int64_t n) { return (n + QRB200_FP8_BLOCK - 1) / QRB200_FP8_BLOCK; }
+
+void check_tile(const Tensor& t, const char* name, int64_t tile_rows) {
+  TORCH_CHECK_VALUE(tile_rows == 1 || tile_rows == QRB200_FP8_BLOCK, "tile_rows must be 1 or ", QRB200_FP8_BLOCK, ", got ", tile_rows);
+  TORCH_CHECK_VALUE(t.dim() > 0 && t.size(-1) <= QRB200_FP8_MAX_DEPTH && (tile_rows == 1 || t.dim() == 2), name, " must be ",
+                    tile_rows == 1 ? "(..., cols)" : "(rows, cols)", " with cols <= ", QRB200_FP8_MAX_DEPTH, ", got ", shape_of(t));
+}
+
+// The scales' shape for `t`: its leading shape, or the rows of its blocks, and the blocks of a row.
+c10::SmallVector<int64_t, 5> scale_sizes(const Tensor& t, int64_t tile_rows) {
+  c10::SmallVector<int64_t, 5> s(t.sizes().begin(), t.sizes().end());
+  if (tile_rows > 1) s[0] = blocks_of(s[0]);
+  s.back() = blocks_of(s.back());
+  return s;
+}
+
+const uint8_t* bytes(const Tensor& t) { return static_cast<const uint8_t*>(t.const_data_ptr()); }
+
+py::tuple quantize_fp8(const Tensor& x, int64_t tile_rows) {
+  operand(x, "x", {at::kFloat, at::kBFloat16, at::kHalf});
+  check_tile(x, "x", tile_rows);
+  OnDevice on(x);
+  const Tensor xr = as_rows(x);
+  const int64_t rows = xr.size(0), cols = xr.size(1), padded = (cols + 15) / 16 * 16;
+  Tensor q = empty({rows, padded}, at::kFloat8_e4m3fn, x);
+  if (padded != cols) q = q.slice(1, 0, cols);
+  const Tensor scale = empty(scale_sizes(x, tile_rows), at::kFloat, x);
+  if (rows > 0 && cols > 0)
+    check(qrb200_quantize_fp8(ptr(xr), xr.stride(0), static_cast<uint8_t*>(q.data_ptr()), q.stride(0), scale.data_ptr<float>(), rows,
+                              cols, (int)tile_rows, type_code(x.scalar_type()), on.stream),
+          "quantize_fp8");
+  return py::make_tuple(shaped(q, x), scale);
+}
+
+Tensor dequantize_fp8(const Tensor& codes, const Tensor& scale, at::ScalarType dtype, int64_t tile_rows) {
+  operand(codes, "codes", {at::kFloat8_e4m3fn});
+  operand(scale, "scale", {at::kFloat}, &codes);
+  TORCH_CHECK_TYPE(type_code(dtype) >= 0, "dtype must be float32, bfloat16 or float16, got ", c10::toString(dtype));
+  check_tile(codes, "codes", tile_rows);
+  const auto want = scale_sizes(codes, tile_rows);
+  TORCH_CHECK_VALUE(scale.sizes() == at::IntArrayRef(want), "scale must be ", at::IntArrayRef(want), " for codes ", shape_of(codes),
+                    ", got ", shape_of(scale));
+  OnDevice on(codes);
+  const Tensor q = as_rows(codes), s = scale.contiguous(), out = empty(codes.sizes(), dtype, codes);
+  if (q.numel() > 0)
+    check(qrb200_dequantize_fp8(bytes(q), q.stride(0), s.const_data_ptr<float>(), out.data_ptr(), q.size(0), q.size(1), (int)tile_rows,
+                                type_code(dtype), on.stream),
+          "dequantize_fp8");
+  return out;
+}
+
+Tensor fp8_linear(const Tensor& x, const Tensor& x_scale, const Tensor& weight, const Tensor& weight_scale, OptTensor bias,
+                  at::ScalarType dtype) {
+  operand(x, "x", {at::kFloat8_e4m3fn});
+  operand(weight, "weight", {at::kFloat8_e4m3fn}, &x);
+  operand(x_scale, "x_scale", {at::kFloat}, &x);
+  operand(weight_scale, "weight_scale", {at::kFloat}, &x);
+  TORCH_CHECK_TYPE(type_code(dtype) >= 0, "dtype must be float32, bfloat16 or float16, got ", c10::toString(dtype));
+  TORCH_CHECK_VALUE(x.dim() > 0 && weight.dim() == 2 && x.size(-1) == weight.size(1),
+                    "x must be (..., depth) and weight (outs, depth), got ", shape_of(x), " and ", shape_of(weight));
+  const int64_t outs = weight.size(0), depth = weight.size(1);
+  TORCH_CHECK_VALUE(depth >= 1 && depth <= QRB200_FP8_MAX_DEPTH, "depth must be from 1 to ", QRB200_FP8_MAX_DEPTH, ", got ", depth);
+  const auto want_x = scale_sizes(x, 1), want_w = scale_sizes(weight, QRB200_FP8_BLOCK);
+  TORCH_CHECK_VALUE(x_scale.sizes() == at::IntArrayRef(want_x), "x_scale must be ", at::IntArrayRef(want_x), " for x ", shape_of(x),
+                    ", got ", shape_of(x_scale));
+  TORCH_CHECK_VALUE(weight_scale.sizes() == at::IntArrayRef(want_w), "weight_scale must be ", at::IntArrayRef(want_w), " for weight ",
+                    shape_of(weight), ", got ", shape_of(weight_scale));
+  if (bias) {
+    operand(*bias, "bias", {dtype}, &x);
+    TORCH_CHECK_VALUE(bias->dim() == 1 && bias->size(0) == outs, "bias must be (", outs, ",), got ", shape_of(*bias));
+    bias = bias->contiguous();
+  }
+  OnDevice on(x);
+  const Tensor xr = as_rows(x), wr = as_rows(weight);
+  const int64_t rows = xr.size(0);
+  c10::SmallVector<int64_t, 5> sizes(x.sizes().begin(), x.sizes().end());
+  sizes.back() = outs;
+  const Tensor y = empty(sizes, dtype, x);
+  if (rows == 0 || outs == 0) return y;
+  const size_t need = qrb200_fp8_linear_workspace_bytes(bytes(xr), xr.stride(0), bytes(wr), wr.stride(0), rows, outs, depth);
+  Tensor ws;
+  if (need > 0) ws = empty({(int64_t)need}, at::kByte, x);
+  const Tensor sx = x_scale.contiguous(), sw = weight_scale.contiguous();
+  check(qrb200_fp8_linear(bytes(xr), xr.stride(0), sx.const_data_ptr<float>(), bytes(wr), wr.stride(0), sw.const_data_ptr<float>(),
+                          ptr(bias), y.data_ptr(), rows, outs, depth, type_code(dtype), need > 0 ? ws.data_ptr() : nullptr, need,
+                          on.stream),
+        "fp8_linear");
+  return y;
+}
+
+// ---- the 8-bit cache ------------------------------------------------------------------------
+
+struct Cache8 {
+  Tensor data, range;
+  qrb200_kv8_shape shape;
+  at::ScalarType type;
+};
+
+Cache8 make_cache8(const Tensor& data, const Tensor& range, int32_t page_size, int32_t head_dim, at::ScalarType type) {
+  TORCH_CHECK_TYPE(type == at::kBFloat16 || type == at::kHalf, "a cache's dtype must be bfloat16 or float16, got ",
+                   c10::toString(type));
+  operand(data, "data", {at::kByte});
+  operand(range, "range", {at::kFloat}, &data);
+  const int64_t size = qrb200_kv8_block_bytes(page_size, head_dim);
+  TORCH_CHECK_VALUE(size > 0 && data.dim() == 3 && data.size(2) == size && data.is_contiguous() && data.size(1) >= 1 &&
+                        data.size(1) <= 65535 && (reinterpret_cast<uintptr_t>(data.const_data_ptr()) & 15u) == 0,
+                    "data must be a contiguous, 16-byte aligned (pages, kv_heads, ", size,
+                    ") tensor for this page_size and head_dim, got ", shape_of(data));
+  const int64_t want[3] = {data.size(0), data.size(1), 2};
+  TORCH_CHECK_VALUE(range.sizes() == at::IntArrayRef(want) && range.is_contiguous(), "range must be a contiguous (", want[0], ", ",
+                    want[1], ", 2) tensor, got ", shape_of(range));
+  return Cache8{data, range, {data.size(0), (int32_t)data.size(1), page_size, head_dim, type_code(type)}, type};
+}
+
+void kv8_write(const Cache8& c, Tensor k, Tensor v, const Tensor& slots) {
+  operand(k, "k", {c.type}, &c.data);
+  operand(v, "v", {c.type}, &c.data);
+  const Tensor at = slots_operand(c, slots);
+  const int64_t want[3] = {at.size(0), c.shape.kv_heads, c.shape.head_dim};
+  TORCH_CHECK_VALUE(k.sizes() == at::IntArrayRef(want) && v.sizes() == at::IntArrayRef(want), "k and v must be (", want[0], ", ",
+                    want[1], ", ", want[2], "), got ", shape_of(k), " and ", shape_of(v));
+  if (want[0] == 0) return;
+  OnDevice on(c.data);
+  if (k.stride(2) != 1) k = k.contiguous();
+  if (v.stride(2) != 1) v = v.contiguous();
+  const size_t need = qrb200_kv8_write_workspace_bytes(&c.shape, want[0]);
+  Tensor ws;
+  if (need > 0) ws = empty({(int64_t)need}, at::kByte, c.data);
+  check(qrb200_kv8_write(c.data.data_ptr(), c.range.data_ptr<float>(), &c.shape, ptr(k), k.stride(0), k.stride(1), ptr(v),
+                         v.stride(0), v.stride(1), at.const_data_ptr<int64_t>(), want[0], need > 0 ? ws.data_ptr() : nullptr, need,
+                         on.stream),
+        "kv8_write");
+}
+
+py::tuple kv8_read(const Cache8& c, const Tensor& slots) {
+  const Tensor at = slots_operand(c, slots);
+  OnDevice on(c.data);
+  const int64_t sizes[3] = {at.size(0), c.shape.kv_heads, c.shape.head_dim};
+  const Tensor k = empty(sizes, c.type, c.data), v = empty(sizes, c.type, c.data);
+  if (sizes[0] > 0)
+    check(qrb200_kv8_read(ptr(c.data), c.range.const_data_ptr<float>(), &c.shape, k.data_ptr(), v.data_ptr(),
+                          at.const_data_ptr<int64_t>(), sizes[0], on.stream),
+          "kv8_read");
+  return py::make_tuple(k, v);
+}
+
+Tensor kv8_attention(Tensor q, const Cache8& c, Tensor table, Tensor lengths, std::optional<double> scale, bool causal,
+                     std::optional<int64_t> window) {
+  const Reading r = reading(q, c, table, lengths, scale, window);
+  OnDevice on(c.data);
+  const Tensor out = empty(q.sizes(), c.type, c.data);
+  if (out.numel() == 0) return out;
+  const size_t need = qrb200_kv8_attention_workspace_bytes(&c.shape, r.batch, r.queries, r.heads, r.pages, r.window);
+  Tensor ws;
+  if (need > 0) ws = empty({(int64_t)need}, at::kByte, c.data);
+  check(qrb200_kv8_attention(ptr(q), r.strides, ptr(c.data), c.range.const_data_ptr<float>(), &c.shape,
+                             table.const_data_ptr<int32_t>(), table.stride(0), lengths.const_data_ptr<int32_t>(), out.data_ptr(),
+                             r.batch, r.queries, r.heads, r.pages, r.window, causal, r.factor, need > 0 ? ws.data_ptr() : nullptr,
+                             need, on.stream),
+        "kv8_attention");
   return out;
 }
 
@@ -295,4 +471,11 @@ PYBIND11_MODULE(_native, m) {
   m.def("kv4_write", &kv4_write);
   m.def("kv4_read", &kv4_read);
   m.def("kv4_attention", &kv4_attention);
+  m.def("quantize_fp8", &quantize_fp8);
+  m.def("dequantize_fp8", &dequantize_fp8);
+  m.def("fp8_linear", &fp8_linear);
+  py::class_<Cache8>(m, "Cache8").def(py::init(&make_cache8));
+  m.def("kv8_write", &kv8_write);
+  m.def("kv8_read", &kv8_read);
+  m.def("kv8_attention", &kv8_attention);
 }

@@ -1317,8 +1317,12 @@ int qrb200_device_status(int* status_out) {
   if (!status_out) return QRB200_ERR_ARG;
   int v = 0;
   if (cudaMemcpyFromSymbol(&v, g_device_status, sizeof(int)) != cudaSuccess) return QRB200_ERR_CUDA;
-  const int q = qrb200_internal_quant_site();
-  if (q < 0) return QRB200_ERR_CUDA;
+  int q = 0;
+  for (int (*site)() : {qrb200_internal_quant_site, qrb200_internal_fp8_site, qrb200_internal_kv8_site}) {
+    const int found = site();
+    if (found < 0) return QRB200_ERR_CUDA;
+    if (q == 0) q = found;
+  }
   const int zero = 0;
   if (v != 0 && cudaMemcpyToSymbol(g_device_status, &zero, sizeof(int)) != cudaSuccess) return QRB200_ERR_CUDA;
   int dev = 0;

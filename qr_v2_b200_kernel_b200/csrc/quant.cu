@@ -1,59 +1,10 @@
 // C ABI of the operators on data in 8 and 4 bits: argument checks, choice of kernel, launches.
-#include <cuda.h>
-#include <cudaTypedefs.h>
-#include <cuda_runtime.h>
-
-#include <algorithm>
-#include <atomic>
-#include <cstdint>
-#include <mutex>
-#include <type_traits>
-
-#include "internal.h"
-#include "qrb200.h"
+#include "launch.h"
 #include "i8_linear.cuh"
 #include "kv4_attention.cuh"
 #include "quant_rows.cuh"
 
 namespace qrb200 {
-
-// This translation unit's failure words, registered once per device after the library's own check.
-static int quant_ready() {
-  static std::atomic<unsigned long long> ready{0};
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess) return QRB200_ERR_CUDA;
-  if (dev < 64 && ((ready.load(std::memory_order_acquire) >> dev) & 1ull)) return qrb200_last_status(nullptr);
-  const int st = qrb200_internal_check_device();
-  if (st != QRB200_OK) return st;
-  int* word = qrb200_internal_status_word(dev);
-  if (word && cudaMemcpyToSymbol(g_status_mapped, &word, sizeof(word)) != cudaSuccess) return QRB200_ERR_CUDA;
-  if (dev < 64) ready.fetch_or(1ull << dev, std::memory_order_acq_rel);
-  return qrb200_last_status(nullptr);
-}
-
-static int launched() {
-  qrb200_internal_count_launch();
-  return cudaGetLastError() == cudaSuccess ? QRB200_OK : QRB200_ERR_CUDA;
-}
-
-static bool type_ok(int t) { return t == QRB200_F32 || t == QRB200_BF16 || t == QRB200_F16; }
-static bool type16_ok(int t) { return t == QRB200_BF16 || t == QRB200_F16; }
-
-constexpr int kMaxCols = 32768;
-constexpr int64_t kMaxRows = (1ll << 31) - 1;
-
-static PFN_cuTensorMapEncodeTiled_v12000 map_encoder() {
-  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
-  static std::once_flag once;
-  std::call_once(once, [] {
-    void* p = nullptr;
-    cudaDriverEntryPointQueryResult q{};
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
-        q == cudaDriverEntryPointSuccess)
-      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
-  });
-  return fn;
-}
 
 // Boxes of 128 codes x `box_rows` rows, 128-byte swizzle; what lies outside the operand reads as zero.
 static bool encode_codes(CUtensorMap* map, const I8Operand& o, uint64_t depth, uint32_t box_rows) {
@@ -67,55 +18,6 @@ static bool encode_codes(CUtensorMap* map, const I8Operand& o, uint64_t depth, u
             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
-
-struct LaunchShape {
-  cudaLaunchConfig_t cfg{};
-  cudaLaunchAttribute attr[2];
-  // A kernel that begins with griddep_launch_wait() may be set up while its predecessor ends.
-  LaunchShape(dim3 grid, unsigned threads, size_t smem, cudaStream_t s) {
-    cfg.gridDim = grid;
-    cfg.blockDim = dim3(threads);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = s;
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.numAttrs = 1;
-    cfg.attrs = attr;
-  }
-  void cluster(unsigned x, unsigned y, unsigned z) {
-    attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = x;
-    attr[1].val.clusterDim.y = y;
-    attr[1].val.clusterDim.z = z;
-    cfg.numAttrs = 2;
-  }
-};
-
-// Whether a one-time set-up of a kernel has been done on the current device; the caller marks it.
-struct OncePerDevice {
-  std::atomic<unsigned long long> bits{0};
-  template <typename F>
-  cudaError_t run(F&& set_up) {
-    int dev = 0;
-    cudaGetDevice(&dev);
-    if (dev < 64 && ((bits.load(std::memory_order_acquire) >> dev) & 1ull)) return cudaSuccess;
-    const cudaError_t e = set_up();
-    if (e == cudaSuccess && dev < 64) bits.fetch_or(1ull << dev, std::memory_order_acq_rel);
-    return e;
-  }
-};
-
-static int sm_count() {
-  static std::atomic<int> sms[64];
-  int dev = 0, n = 0;
-  cudaGetDevice(&dev);
-  if (dev < 64 && (n = sms[dev].load(std::memory_order_relaxed)) > 0) return n;
-  cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
-  if (dev < 64) sms[dev].store(n, std::memory_order_relaxed);
-  return n;
-}
-
-static int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 
 // Packs of a row to a thread, by the row's length: four (enough loads in flight, few threads at the
 // two reductions), fewer where that would leave a warp idle. Short rows go several to a block, a
@@ -292,12 +194,6 @@ static cudaError_t launch_i8(const I8Params& p, I8Operand x, I8Operand w, uint4*
   }
 }
 
-static int page_shift(int page) {
-  int s = 0;
-  while (s < 10 && (1 << s) < page) ++s;
-  return s;
-}
-
 static bool shape_ok(const Kv4Shape& h) {
   return h.pages >= 0 && h.pages <= (1ll << 31) - 1 && h.heads > 0 && h.heads <= 65535 && (h.dim == 64 || h.dim == 128) &&
          h.page >= 16 && h.page <= 1024 && (h.page & (h.page - 1)) == 0 && h.groups > 0 && h.dim % h.groups == 0 &&
@@ -305,8 +201,6 @@ static bool shape_ok(const Kv4Shape& h) {
 }
 
 // f(dim, groups) with both as types, for the layouts that shape_ok admits.
-template <int kValue>
-using Int = std::integral_constant<int, kValue>;
 template <typename F>
 static cudaError_t with_layout(const Kv4Shape& h, F&& f) {
   if (h.dim == 64) return h.groups == 1 ? f(Int<64>{}, Int<1>{}) : f(Int<64>{}, Int<2>{});
@@ -412,13 +306,7 @@ static cudaError_t launch_attention_of(const Kv4AttnParams& p, const AttnPlan& p
 
 using namespace qrb200;
 
-int qrb200_internal_quant_site() {
-  int v = 0;
-  const int zero = 0;
-  if (cudaMemcpyFromSymbol(&v, g_device_status, sizeof(int)) != cudaSuccess) return -1;
-  if (v != 0 && cudaMemcpyToSymbol(g_device_status, &zero, sizeof(int)) != cudaSuccess) return -1;
-  return v;
-}
+int qrb200_internal_quant_site() { return take_site(); }
 
 extern "C" {
 
