@@ -1,5 +1,5 @@
 // C ABI of the operators on 8-bit floating point: argument checks, choice of kernel, launches.
-#include "launch.h"
+#include "codes.h"
 #include "fp8_linear.cuh"
 #include "fp8_rows.cuh"
 
@@ -40,14 +40,99 @@ static cudaError_t launch_values(const uint8_t* q, int64_t q_stride, const float
                             static_cast<T*>(out), (long long)rows, (int)cols, tile_rows);
 }
 
-template <typename T>
-static cudaError_t launch_fp8(const Fp8Params& p, const Fp8Operand& x, const Fp8Operand& w, cudaStream_t s) {
-  LaunchShape l(dim3(ceil_div(p.outs, 32), ceil_div(p.rows, 32)), 256, 0, s);
-  return cudaLaunchKernelEx(&l.cfg, fp8_simple_kernel<T>, p, x, w);
+static I8Operand codes_operand(const uint8_t* base, int64_t rows, int64_t stride) {
+  return i8_operand(reinterpret_cast<const int8_t*>(base), rows, stride);
 }
 
-static Fp8Operand fp8_operand(const uint8_t* base, int64_t rows, int64_t stride) {
-  return {base, rows, stride, !off16(base) && (rows == 1 || stride % 16 == 0)};
+template <typename T, int kBN>
+static cudaError_t launch_fp8_few(const Fp8Params& p, const I8Operand& x, const I8Operand& w, unsigned split, cudaStream_t s) {
+  using C = Fp8Few<kBN>;
+  static OncePerDevice once;
+  const cudaError_t e = once.run([] {
+    return cudaFuncSetAttribute(fp8_few_kernel<T, kBN>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::smem());
+  });
+  if (e != cudaSuccess) return e;
+  CUtensorMap tw, tx;
+  if (!encode_codes(&tw, w, p.depth, 128) || !encode_codes(&tx, x, p.depth, kBN)) return cudaErrorInvalidValue;
+  const int tn = ceil_div(p.outs, 128), tm = ceil_div(p.rows, kBN);
+  if (tm > 65535) return cudaErrorInvalidValue;
+  LaunchShape l(dim3(tn, tm, split), 192, C::smem(), s);
+  if (split > 1) l.cluster(1, 1, split);
+  return cudaLaunchKernelEx(&l.cfg, fp8_few_kernel<T, kBN>, p, tw, tx);
+}
+
+template <typename T>
+static cudaError_t launch_fp8_wide(Fp8Params p, const I8Operand& x, const I8Operand& w, cudaStream_t s) {
+  static OncePerDevice once;
+  const cudaError_t e = once.run([] {
+    return cudaFuncSetAttribute(fp8_wide_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)fp8_wide_smem());
+  });
+  if (e != cudaSuccess) return e;
+  CUtensorMap tw, tx;
+  if (!encode_codes(&tw, w, p.depth, 128) || !encode_codes(&tx, x, p.depth, 128)) return cudaErrorInvalidValue;
+  p.tiles_n = ceil_div(p.outs, 256);
+  const int64_t tiles = (int64_t)p.tiles_n * ceil_div(p.rows, 256);
+  if (tiles > (1 << 30)) return cudaErrorInvalidValue;
+  p.tiles = (int)tiles;
+  const int pairs = std::min(p.tiles, sm_count() / 2);
+  LaunchShape l(dim3(2 * pairs), 128 + 32 * kFp8WideEpi, fp8_wide_smem(), s);
+  return cudaLaunchKernelEx(&l.cfg, fp8_wide_kernel<T>, p, tx, tw);
+}
+
+// Which kernel, with how many rows a tile (`rows`) and over how many CTAs of the depth: the least
+// of the estimated clocks. A CTA takes in its stages at about 40 bytes a clock; joining a split
+// costs two cluster barriers (about 1500 clocks) and reading the sums at about 20 bytes a clock.
+// The wide kernel's pair takes 512 clocks a stage and a tile's last epilogue is bare.
+struct Fp8Plan {
+  int rows;  // 16, 32, 64 or 128 (few), 256 (wide)
+  unsigned split;
+};
+static Fp8Plan fp8_plan(int64_t rows, int64_t outs, int64_t nk) {
+  const int64_t sms = sm_count();
+  const int64_t pairs = (rows + 255) / 256 * ((outs + 255) / 256);
+  Fp8Plan best{256, 1};
+  int64_t least = (pairs + sms / 2 - 1) / (sms / 2) * (nk * 512 + 1500) + 3000;
+  for (int bn = 16; bn <= 128; bn *= 2) {
+    const int64_t tiles = (rows + bn - 1) / bn * ((outs + 127) / 128);
+    if ((rows + bn - 1) / bn > 65535) continue;
+    for (unsigned split = 1; split <= kFp8Split && split <= nk; split *= 2) {
+      const int64_t clocks = (tiles * split + sms - 1) / sms *
+                             ((nk + split - 1) / split * (128 + bn) * 128 / 40 + (split > 1 ? 1500 + bn * 24 : bn * 8));
+      if (clocks < least) {
+        least = clocks;
+        best = Fp8Plan{bn, split};
+      }
+    }
+    if (rows <= bn) break;
+  }
+  return best;
+}
+
+template <typename T>
+static cudaError_t launch_fp8_rows(const Fp8Params& p, const I8Operand& x, const I8Operand& w, cudaStream_t s) {
+  const Fp8RowsOperands r{p, x, w};
+  LaunchShape l(dim3(ceil_div(p.outs, 16)), 32 * kFp8RowsWarps, 0, s);
+  const bool aligned = x.aligned && w.aligned;
+  if (p.rows <= 8)
+    return cudaLaunchKernelEx(&l.cfg, aligned ? fp8_few_rows_kernel<T, 1, true> : fp8_few_rows_kernel<T, 1, false>, r);
+  return cudaLaunchKernelEx(&l.cfg, fp8_few_rows_kernel<T, 2, true>, r);  // never unaligned
+}
+
+static bool fp8_by_rows(int64_t rows, bool aligned) { return rows <= (aligned ? 16 : 8); }
+
+template <typename T>
+static cudaError_t launch_fp8(const Fp8Params& p, I8Operand x, I8Operand w, uint4* ws, cudaStream_t s) {
+  if (fp8_by_rows(p.rows, x.aligned && w.aligned)) return launch_fp8_rows<T>(p, x, w, s);
+  const cudaError_t e = lay_out(x, w, p.depth, ws, s);
+  if (e != cudaSuccess) return e;
+  const Fp8Plan plan = fp8_plan(p.rows, p.outs, p.blocks);
+  switch (plan.rows) {
+    case 16: return launch_fp8_few<T, 16>(p, x, w, plan.split, s);
+    case 32: return launch_fp8_few<T, 32>(p, x, w, plan.split, s);
+    case 64: return launch_fp8_few<T, 64>(p, x, w, plan.split, s);
+    case 128: return launch_fp8_few<T, 128>(p, x, w, plan.split, s);
+    default: return launch_fp8_wide<T>(p, x, w, s);
+  }
 }
 
 }  // namespace qrb200
@@ -96,8 +181,9 @@ int qrb200_dequantize_fp8(const uint8_t* q, int64_t q_stride, const float* scale
 
 size_t qrb200_fp8_linear_workspace_bytes(const uint8_t* x, int64_t x_stride, const uint8_t* w, int64_t w_stride, int64_t rows,
                                          int64_t outs, int64_t depth) {
-  (void)x, (void)x_stride, (void)w, (void)w_stride, (void)rows, (void)outs, (void)depth;
-  return 0;
+  if (rows <= 0 || outs <= 0 || depth <= 0 || depth > QRB200_FP8_MAX_DEPTH) return 0;
+  const I8Operand xo = codes_operand(x, rows, x_stride), wo = codes_operand(w, outs, w_stride);
+  return fp8_by_rows(rows, xo.aligned && wo.aligned) ? 0 : layout_bytes(xo, wo, depth);
 }
 
 int qrb200_fp8_linear(const uint8_t* x, int64_t x_stride, const float* x_scale, const uint8_t* w, int64_t w_stride,
@@ -113,12 +199,13 @@ int qrb200_fp8_linear(const uint8_t* x, int64_t x_stride, const float* x_scale, 
   const size_t need = qrb200_fp8_linear_workspace_bytes(x, x_stride, w, w_stride, rows, outs, depth);
   if (need > 0 && (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 255u)))
     return QRB200_ERR_WORKSPACE;
-  const Fp8Params p{x_scale, w_scale, bias, y, (int)rows, (int)outs, (int)depth, ceil_div(depth, kFp8Block)};
-  const Fp8Operand xo = fp8_operand(x, rows, x_stride), wo = fp8_operand(w, outs, w_stride);
+  const Fp8Params p{x_scale, w_scale, bias, y, (int)rows, (int)outs, (int)depth, ceil_div(depth, kFp8Block), 0, 0};
+  const I8Operand xo = codes_operand(x, rows, x_stride), wo = codes_operand(w, outs, w_stride);
+  uint4* ws = static_cast<uint4*>(workspace);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const cudaError_t e = dtype == QRB200_BF16  ? launch_fp8<__nv_bfloat16>(p, xo, wo, s)
-                        : dtype == QRB200_F16 ? launch_fp8<__half>(p, xo, wo, s)
-                                              : launch_fp8<float>(p, xo, wo, s);
+  const cudaError_t e = dtype == QRB200_BF16  ? launch_fp8<__nv_bfloat16>(p, xo, wo, ws, s)
+                        : dtype == QRB200_F16 ? launch_fp8<__half>(p, xo, wo, ws, s)
+                                              : launch_fp8<float>(p, xo, wo, ws, s);
   if (e != cudaSuccess) return QRB200_ERR_CUDA;
   return launched();
 }

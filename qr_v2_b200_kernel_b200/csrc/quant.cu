@@ -1,23 +1,10 @@
 // C ABI of the operators on data in 8 and 4 bits: argument checks, choice of kernel, launches.
-#include "launch.h"
+#include "codes.h"
 #include "i8_linear.cuh"
 #include "kv4_attention.cuh"
 #include "quant_rows.cuh"
 
 namespace qrb200 {
-
-// Boxes of 128 codes x `box_rows` rows, 128-byte swizzle; what lies outside the operand reads as zero.
-static bool encode_codes(CUtensorMap* map, const I8Operand& o, uint64_t depth, uint32_t box_rows) {
-  const PFN_cuTensorMapEncodeTiled_v12000 fn = map_encoder();
-  if (fn == nullptr) return false;
-  const cuuint64_t dims[2] = {depth, (cuuint64_t)o.rows};
-  const cuuint64_t strides[1] = {o.rows > 1 ? (cuuint64_t)o.stride : (depth + 15) / 16 * 16};
-  const cuuint32_t box[2] = {(cuuint32_t)kI8Depth, box_rows};
-  const cuuint32_t estr[2] = {1, 1};
-  return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<int8_t*>(o.base), dims, strides, box, estr,
-            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
 
 // Packs of a row to a thread, by the row's length: four (enough loads in flight, few threads at the
 // two reductions), fewer where that would leave a warp idle. Short rows go several to a block, a
@@ -165,25 +152,11 @@ static cudaError_t launch_i8_rows(const I8Params& p, const I8Operand& x, const I
 // tensor-core kernel.
 static bool i8_by_rows(int64_t rows, int64_t depth, bool aligned) { return rows <= (aligned ? 4 : 2) && depth <= 8192; }
 
-static I8Operand i8_operand(const int8_t* base, int64_t rows, int64_t stride) {
-  return {base, rows, stride, (reinterpret_cast<uintptr_t>(base) & 15u) == 0 && (rows == 1 || stride % 16 == 0)};
-}
-
 template <typename T>
 static cudaError_t launch_i8(const I8Params& p, I8Operand x, I8Operand w, uint4* ws, cudaStream_t s) {
   if (i8_by_rows(p.rows, p.depth, x.aligned && w.aligned)) return launch_i8_rows<T>(p, x, w, s);
-  if (!x.aligned || !w.aligned) {  // laid out anew in the workspace, x before w
-    const int packs = ceil_div(p.depth, 16);
-    uint4* to_x = x.aligned ? nullptr : ws;
-    uint4* to_w = w.aligned ? nullptr : ws + (x.aligned ? 0 : x.rows * packs);
-    const int64_t count = (to_x ? x.rows * packs : 0) + (to_w ? w.rows * packs : 0);
-    LaunchShape l(dim3(ceil_div(count, 256)), 256, 0, s);
-    const cudaError_t e = cudaLaunchKernelEx(&l.cfg, i8_pad_kernel, x, to_x, w, to_w, p.depth, packs);
-    if (e != cudaSuccess) return e;
-    qrb200_internal_count_launch();
-    if (to_x) x = {reinterpret_cast<const int8_t*>(to_x), x.rows, 16ll * packs, true};
-    if (to_w) w = {reinterpret_cast<const int8_t*>(to_w), w.rows, 16ll * packs, true};
-  }
+  const cudaError_t e = lay_out(x, w, p.depth, ws, s);
+  if (e != cudaSuccess) return e;
   const I8Plan plan = i8_plan(p.rows, p.outs, p.depth);
   switch (plan.rows) {
     case 16: return launch_i8_few<T, 16>(p, x, w, plan.split, s);
@@ -351,10 +324,8 @@ int qrb200_dequantize_int8(const int8_t* q, int64_t q_stride, const float* scale
 size_t qrb200_int8_linear_workspace_bytes(const int8_t* x, int64_t x_stride, const int8_t* w, int64_t w_stride,
                                           int64_t rows, int64_t outs, int64_t depth) {
   if (rows <= 0 || outs <= 0 || depth <= 0 || depth > QRB200_INT8_MAX_DEPTH) return 0;
-  const bool xa = i8_operand(x, rows, x_stride).aligned, wa = i8_operand(w, outs, w_stride).aligned;
-  if (i8_by_rows(rows, depth, xa && wa)) return 0;
-  const size_t pitch = (size_t)(depth + 15) / 16 * 16;
-  return (xa ? 0 : rows * pitch) + (wa ? 0 : outs * pitch);
+  const I8Operand xo = i8_operand(x, rows, x_stride), wo = i8_operand(w, outs, w_stride);
+  return i8_by_rows(rows, depth, xo.aligned && wo.aligned) ? 0 : layout_bytes(xo, wo, depth);
 }
 
 int qrb200_int8_linear(const int8_t* x, int64_t x_stride, const float* x_scale, const int8_t* w, int64_t w_stride,
