@@ -43,6 +43,21 @@ __device__ __forceinline__ void fp8_mma_pair(uint32_t d, uint64_t a, uint64_t b,
       : "memory");
 }
 
+// One lane of a converged warp. (The warp that issues MMAs runs its loop whole and lets one lane do so: its
+// descriptors then stay in the registers that the instruction wants.)
+__device__ __forceinline__ bool elect_one() {
+  uint32_t one;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}\n"
+      : "=r"(one));
+  return one != 0;
+}
+__device__ __forceinline__ void mbar_arrive(uint64_t* mbar) {  // of this CTA
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(mbar)) : "memory");
+}
+
 // Sixteen accumulator columns of this lane, asked for; they are there after tmem_arrived.
 __device__ __forceinline__ void tmem_ask16(uint32_t taddr, float (&v)[16]) {
   asm volatile(
@@ -216,7 +231,7 @@ __global__ void __launch_bounds__(192) fp8_few_kernel(Fp8Params P, const __grid_
     int issued = 0;
     for (int k = k_lo; k < k_hi; ++k, ++issued) {
       const int s = issued % C::kStages, turn = issued / C::kStages;
-      if (turn > 0 && !mbar_wait(&empty[s], (turn - 1) & 1)) {
+      if (turn > 0 && !mbar_wait_quick(&empty[s], (turn - 1) & 1)) {
         s_bad = 1;
         break;
       }
@@ -227,23 +242,27 @@ __global__ void __launch_bounds__(192) fp8_few_kernel(Fp8Params P, const __grid_
     }
     // Whatever happened, no load is in flight when this CTA ends.
     for (int j = max(0, issued - C::kStages); j < issued; ++j)
-      if (!mbar_wait(&full[j % C::kStages], (j / C::kStages) & 1)) s_bad = 1;
-  } else if (warp == 1 && lane == 0) {
+      if (!mbar_wait_quick(&full[j % C::kStages], (j / C::kStages) & 1)) s_bad = 1;
+  } else if (warp == 1) {
     constexpr uint32_t idesc = fp8_idesc(128, kBN);
-    int j = 0;
-    for (int k = k_lo; k < k_hi; ++k, ++j) {
-      const int s = j % C::kStages, buf = j & 1;
-      if ((j >= 2 && !mbar_wait(&acc_empty[buf], ((j >> 1) - 1) & 1)) || !mbar_wait(&full[s], (j / C::kStages) & 1)) {
+    const uint64_t w0 = i8_sdesc(smem_u32(ring)), x0 = i8_sdesc(smem_u32(ring) + 128 * kI8Depth);
+    uint32_t s = 0, turn = 0;
+    for (int j = 0; j < k_hi - k_lo; ++j) {
+      const uint32_t buf = j & 1;
+      if ((j >= 2 && !mbar_wait_quick(&acc_empty[buf], ((j >> 1) - 1) & 1)) || !mbar_wait_quick(&full[s], turn)) {
         s_bad = 1;
         break;
       }
       tc_fence_after();
-      const uint32_t at = smem_u32(ring) + s * C::kStage;
+      const uint64_t at = s * (C::kStage >> 4);
+      if (elect_one()) {
 #pragma unroll
-      for (int c = 0; c < kI8Depth / 32; ++c)
-        fp8_mma(tmem + buf * kBN, i8_sdesc(at + 32 * c), i8_sdesc(at + 128 * kI8Depth + 32 * c), idesc, c > 0);
-      mma_commit(&empty[s]);
-      mma_commit(&acc_full[buf]);
+        for (int c = 0; c < kI8Depth / 32; ++c) fp8_mma(tmem + buf * kBN, w0 + at + 2 * c, x0 + at + 2 * c, idesc, c > 0);
+        mma_commit(&empty[s]);
+        mma_commit(&acc_full[buf]);
+      }
+      __syncwarp();
+      if (++s == C::kStages) s = 0, turn ^= 1;
     }
     // The last products are over before anybody reuses the ring (the accumulators say so) or TMEM is freed.
   } else if (epi) {
@@ -272,7 +291,7 @@ __global__ void __launch_bounds__(192) fp8_few_kernel(Fp8Params P, const __grid_
       ask(k0 + kFp8Scales);
       for (int k = k0; k < min(k_hi, k0 + kFp8Scales); ++k, ++j) {
         const int buf = j & 1;
-        ok = ok && __all_sync(kFullMask, mbar_wait(&acc_full[buf], (j >> 1) & 1));
+        ok = ok && __all_sync(kFullMask, mbar_wait_quick(&acc_full[buf], (j >> 1) & 1));
         if (!ok) continue;
         tc_fence_after();
         float v[2][16];
@@ -283,7 +302,7 @@ __global__ void __launch_bounds__(192) fp8_few_kernel(Fp8Params P, const __grid_
           if (c + 1 < kBN / 16) tmem_ask16(lanes + buf * kBN + 16 * (c + 1), v[(c + 1) & 1]);
           if (c + 1 == kBN / 16) {  // every sum of this warp is in registers
             tc_fence_before();
-            if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(&acc_empty[buf])) : "memory");
+            if (lane == 0) mbar_arrive(&acc_empty[buf]);
           }
 #pragma unroll
           for (int q = 0; q < 16; q += 4) {
@@ -369,9 +388,19 @@ __global__ void __launch_bounds__(192) fp8_few_kernel(Fp8Params P, const __grid_
 // 4-11 add each block, scaled, to the 128 sums a lane that they hold in registers: a row to a lane, and the
 // 128 channels of one block of the weights to a warp, so that both scales are one factor. They take the
 // registers that warps 0-3 have no use for.
+//
+// A block's products take 512 clocks, and its accumulator must be free again 512 later. Between lie the
+// commit, the epilogue's loads and the other CTA's word, so what those wait for is kept short:
+// * one warp of a CTA asks the memory barriers for the eight, and passes the word on by named barriers (the
+//   eight asking for themselves, and arriving for themselves: 257 us);
+// * half of a block's sums are loaded at once, and the accumulator is free before the last half is added;
+// * the scales of four blocks come in one load (32 lines a warp's load, it holds up the barriers behind it).
+// 8192 x 8192 x 4096: 238 us, 2.3 P op/s; without the additions (one accumulator over the depth, one scale a row
+// and channel) the same products take 207 us under the power cap.
 constexpr int kFp8WideStage = 2 * 128 * kI8Depth;  // bytes per CTA and stage
 constexpr int kFp8WideStages = 5;
 constexpr int kFp8WideEpi = 8;  // epilogue warps
+constexpr int kFp8Hand = 32 * kFp8WideEpi + 32;  // threads of a named barrier between them and warp 2 or 3
 constexpr int kFp8Pitch = 144;  // bytes of a staged output row (128 and 16 to spread the banks)
 constexpr size_t fp8_wide_smem() { return 1024 + (size_t)kFp8WideStages * kFp8WideStage + kFp8WideEpi * 32 * kFp8Pitch; }
 
@@ -379,8 +408,9 @@ template <typename T>
 __global__ void __launch_bounds__(128 + 32 * kFp8WideEpi, 1) __cluster_dims__(2, 1, 1)
     fp8_wide_kernel(Fp8Params P, const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w) {
   extern __shared__ __align__(1024) unsigned char smem_raw[];
-  __shared__ uint64_t full[kFp8WideStages], empty[kFp8WideStages], acc_full[2], acc_empty[2];
+  __shared__ uint64_t full[kFp8WideStages], done[kFp8WideStages], acc_empty[2];
   __shared__ uint32_t s_tmem;
+  __shared__ volatile int s_bad;  // a wait ran out: keep to the barriers, write nothing
   unsigned char* ring = align1024(smem_raw);
   unsigned char* staged = ring + kFp8WideStages * kFp8WideStage;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -388,14 +418,12 @@ __global__ void __launch_bounds__(128 + 32 * kFp8WideEpi, 1) __cluster_dims__(2,
   const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1, nk = P.blocks;
 
   if (threadIdx.x == 0) {
+    s_bad = 0;
     for (int s = 0; s < kFp8WideStages; ++s) {
       mbar_init(&full[s], 1);
-      mbar_init(&empty[s], 1);
+      mbar_init(&done[s], 1);
     }
-    for (int s = 0; s < 2; ++s) {
-      mbar_init(&acc_full[s], 1);
-      mbar_init(&acc_empty[s], 2 * kFp8WideEpi);  // the epilogue warps of both CTAs
-    }
+    for (int s = 0; s < 2; ++s) mbar_init(&acc_empty[s], 2);  // both CTAs
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     fence_async_smem();
     prefetch_map(&tm_w);
@@ -432,7 +460,7 @@ __global__ void __launch_bounds__(128 + 32 * kFp8WideEpi, 1) __cluster_dims__(2,
         place(tile, m, n);
         for (int k = 0; k < nk; ++k, ++issued) {
           const int s = issued % kFp8WideStages, turn = issued / kFp8WideStages;
-          if (turn > 0 && !mbar_wait(&empty[s], (turn - 1) & 1)) {
+          if (turn > 0 && !mbar_wait_quick(&done[s], (turn - 1) & 1)) {
             ok = false;
             break;
           }
@@ -443,24 +471,50 @@ __global__ void __launch_bounds__(128 + 32 * kFp8WideEpi, 1) __cluster_dims__(2,
         }
       }
       // No load is in flight when the pair ends: the loads of both CTAs land on the leader's
-      // barriers, and `empty` says that the last use of each stage is over.
+      // barriers, and `done` says that the last use of each stage is over.
       for (int j = max(0, issued - kFp8WideStages); j < issued; ++j)
-        mbar_wait(&empty[j % kFp8WideStages], (j / kFp8WideStages) & 1);
-    } else if (warp == 1 && lane == 0 && rank == 0) {
+        mbar_wait_quick(&done[j % kFp8WideStages], (j / kFp8WideStages) & 1);
+    } else if (warp == 1 && rank == 0) {
       constexpr uint32_t idesc = fp8_idesc(256, 256);
-      const long long count = (long long)((P.tiles - pair + pairs - 1) / pairs) * nk;
-      for (long long j = 0; j < count; ++j) {
-        const int s = (int)(j % kFp8WideStages), buf = (int)(j & 1);
-        if (j >= 2 && !mbar_wait(&acc_empty[buf], ((j >> 1) - 1) & 1)) break;
-        if (!mbar_wait(&full[s], (j / kFp8WideStages) & 1)) break;
-        tc_fence_after();
-        const uint32_t at = smem_u32(ring) + s * kFp8WideStage;
+      const uint64_t x0 = i8_sdesc(smem_u32(ring)), w0 = i8_sdesc(smem_u32(ring) + 128 * kI8Depth);
+      uint32_t s = 0, turn = 0, j = 0;
+      bool ok = true;
+      for (int tile = pair; tile < P.tiles && ok; tile += pairs)
+        for (int k = 0; k < nk; ++k, ++j) {
+          const uint32_t buf = j & 1;
+          ok = mbar_wait_quick(&full[s], turn) && (j < 2 || mbar_wait_quick(&acc_empty[buf], ((j >> 1) - 1) & 1));
+          if (!ok) break;
+          tc_fence_after();
+          const uint64_t at = s * (kFp8WideStage >> 4);
+          if (elect_one()) {
 #pragma unroll
-        for (int c = 0; c < kI8Depth / 32; ++c)
-          fp8_mma_pair(tmem + buf * 256, i8_sdesc(at + 32 * c), i8_sdesc(at + 128 * kI8Depth + 32 * c), idesc, c > 0);
-        commit_pair(&empty[s]);
-        commit_pair(&acc_full[buf]);
-      }
+            for (int c = 0; c < kI8Depth / 32; ++c) fp8_mma_pair(tmem + buf * 256, x0 + at + 2 * c, w0 + at + 2 * c, idesc, c > 0);
+            commit_pair(&done[s]);
+          }
+          __syncwarp();
+          if (++s == kFp8WideStages) s = 0, turn ^= 1;
+        }
+    } else if (warp == 2) {
+      // Tells the epilogue warps that a block is done: one warp asks the barrier in their stead.
+      uint32_t s = 0, turn = 0, j = 0;
+      for (int tile = pair; tile < P.tiles; tile += pairs)
+        for (int k = 0; k < nk; ++k, ++j) {
+          if (!s_bad && !mbar_wait_quick(&done[s], turn)) s_bad = 1;
+          __syncwarp();
+          named_arrive(1 + (j & 1), kFp8Hand);
+          if (++s == kFp8WideStages) s = 0, turn ^= 1;
+        }
+    } else if (warp == 3) {
+      // Tells the MMAs' warp that the epilogue warps hold a block's sums. (Relaxed: nothing in memory hangs on it, and a
+      // release would wait for what has been asked for.)
+      uint32_t j = 0;
+      for (int tile = pair; tile < P.tiles; tile += pairs)
+        for (int k = 0; k < nk; ++k, ++j) {
+          named_sync(3 + (j & 1), kFp8Hand);
+          if (lane == 0)
+            asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(pair_leader(smem_u32(&acc_empty[j & 1])))
+                         : "memory");
+        }
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
@@ -469,9 +523,9 @@ __global__ void __launch_bounds__(128 + 32 * kFp8WideEpi, 1) __cluster_dims__(2,
     unsigned char* mine = staged + (warp - 4) * 32 * kFp8Pitch;
     const uint32_t lanes = tmem + ((uint32_t)(ew * 32) << 16) + 128 * half;
     const bool wide = P.outs % (16 / (int)sizeof(T)) == 0;  // 16-byte rows of y (y itself is 16-byte aligned)
+    const bool fours = nk % 4 == 0 && ((reinterpret_cast<uintptr_t>(P.sx) | reinterpret_cast<uintptr_t>(P.sw)) & 15u) == 0;
     T* y = static_cast<T*>(P.y);
     uint32_t j = 0;
-    bool bad = false;  // a wait ran out: touch nothing
     for (int tile = pair; tile < P.tiles; tile += pairs) {
       int m, n;
       place(tile, m, n);
@@ -479,36 +533,59 @@ __global__ void __launch_bounds__(128 + 32 * kFp8WideEpi, 1) __cluster_dims__(2,
       const bool real = row0 + lane < P.rows && n0 < P.outs;
       const float* sx = P.sx + (long long)(real ? row0 + lane : 0) * nk;
       const float* sw = P.sw + (long long)(real ? n0 / kFp8Block : 0) * nk;
+      // The scales of four blocks at a time, asked for four ahead.
+      alignas(16) float scale[4] = {}, next_x[4] = {}, next_w[4] = {};
+      const auto ask = [&](int k) {
+        if (fours) {
+          if (k < nk) {
+            *reinterpret_cast<float4*>(next_x) = __ldg(reinterpret_cast<const float4*>(sx + k));
+            *reinterpret_cast<float4*>(next_w) = __ldg(reinterpret_cast<const float4*>(sw + k));
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (k + i < nk) next_x[i] = __ldg(sx + k + i), next_w[i] = __ldg(sw + k + i);
+        }
+      };
+      ask(0);
       float2 acc[64];
 #pragma unroll
       for (int i = 0; i < 64; ++i) acc[i] = make_float2(0.f, 0.f);
-      float next_x = __ldg(sx), next_w = __ldg(sw);
       for (int k = 0; k < nk; ++k, ++j) {
-        const float scale = next_x * next_w;
-        if (k + 1 < nk) next_x = __ldg(sx + k + 1), next_w = __ldg(sw + k + 1);
         const int buf = j & 1;
-        bad = bad || !__all_sync(kFullMask, mbar_wait(&acc_full[buf], (j >> 1) & 1));
-        if (bad) continue;
-        tc_fence_after();
-        float v[2][16];
-        tmem_ask16(lanes + buf * 256, v[0]);
+        if ((k & 3) == 0) {
 #pragma unroll
-        for (int c = 0; c < 8; ++c) {
-          tmem_arrived(v[c & 1]);
-          if (c < 7) {
-            tmem_ask16(lanes + buf * 256 + 16 * (c + 1), v[(c + 1) & 1]);
-          } else {  // every sum of this warp is in registers: the accumulator is free
-            tc_fence_before();
-            if (lane == 0)
-              asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(pair_leader(smem_u32(&acc_empty[buf])))
-                           : "memory");
-          }
+          for (int i = 0; i < 4; ++i) scale[i] = next_x[i] * next_w[i];
+          ask(k + 4);
+        }
+        const float both = (k & 2) ? (k & 1) ? scale[3] : scale[2] : (k & 1) ? scale[1] : scale[0];
+        named_sync(1 + buf, kFp8Hand);
+        tc_fence_after();
+        // Half of the columns are asked for at once and the others as those are added, so that the accumulator
+        // is free before the last half is.
+        float v[4][16];
+        const auto add = [&](int c) {
 #pragma unroll
           for (int q = 0; q < 8; ++q)
-            acc[8 * c + q] = __ffma2_rn(make_float2(v[c & 1][2 * q], v[c & 1][2 * q + 1]), make_float2(scale, scale), acc[8 * c + q]);
+            acc[8 * c + q] = __ffma2_rn(make_float2(v[c & 3][2 * q], v[c & 3][2 * q + 1]), make_float2(both, both), acc[8 * c + q]);
+        };
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tmem_ask16(lanes + buf * 256 + 16 * c, v[c]);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tmem_arrived(v[c]);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          add(c);
+          tmem_ask16(lanes + buf * 256 + 16 * (c + 4), v[c]);
         }
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tmem_arrived(v[c]);
+        tc_fence_before();
+        named_arrive(3 + buf, kFp8Hand);
+#pragma unroll
+        for (int c = 4; c < 8; ++c) add(c);
       }
-      if (bad) continue;
+      if (s_bad) continue;
 #pragma unroll
       for (int c0 = 0; c0 < 128; c0 += kPer) {
         __syncwarp();
