@@ -265,7 +265,8 @@ int64_t qrb200_kv8_block_bytes(int64_t page_size, int64_t head_dim);
 
 /* Writes keys and values (tokens x kv_heads x head_dim of the cache's type, channels contiguous, other strides in
  * elements) at slots (page * page_size + offset), in any order, each at most once; a negative slot is skipped. A page's range
- * becomes the largest of what it was and of the magnitudes written, rounded up to three significant bits; codes are
+ * becomes the largest of what it was and of the magnitudes written, rounded up to three significant bits (unless those pass the
+ * type's largest number); codes are
  * rint(127 x / range), and those of its other tokens, where the range grew, rint(c old / range). A call that writes a page's
  * first token begins it anew, the rest of it as zeros. A NaN or an infinity makes the range NaN until
  * then. Only one call at a time may write a page. Workspace as the query says, 256-byte aligned. */

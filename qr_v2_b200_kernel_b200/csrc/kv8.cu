@@ -1,4 +1,6 @@
 // C ABI of the 8-bit key/value cache: argument checks, choice of kernel, launches.
+#include <cmath>
+
 #include "launch.h"
 #include "kv8.cuh"
 #include "kv8_attention.cuh"
@@ -17,6 +19,55 @@ template <typename F>
 static cudaError_t with_shape(int dtype, int dim, F&& f) {
   if (dtype == QRB200_BF16) return dim == 64 ? f(__nv_bfloat16{}, Int<64>{}) : f(__nv_bfloat16{}, Int<128>{});
   return dim == 64 ? f(__half{}, Int<64>{}) : f(__half{}, Int<128>{});
+}
+
+// How an attention call is cut: query rows per tile, and the token range over `splits` CTAs.
+struct Kv8Plan {
+  int tile_rows, tiles, splits;
+  size_t bytes;  // workspace: the parts and their (maximum, sum) pairs
+};
+
+// Eight rows a tile where a key head has no more than eight query rows, else sixteen. The token
+// range is cut over the CTAs that make the least estimated time, in fifths of a step's share of a
+// busy SM: a CTA alone takes 2.4 such shares for a step (1.8 with sixteen rows), so up to
+// that many share an SM for nothing, and its set-up takes two steps; joining costs 1.5 in a cluster
+// and 6 through memory. The length is the table's capacity or what a window leaves of it, all that
+// the host knows.
+static Kv8Plan attn_plan(const Kv8Shape& h, int64_t batch, int64_t queries, int64_t q_heads, int64_t max_pages, int64_t span) {
+  Kv8Plan p{};
+  const int64_t rows = queries * (q_heads / h.heads);
+  p.tile_rows = rows <= 8 ? 8 : 16;
+  p.tiles = ceil_div(rows, p.tile_rows);
+  const int64_t ctas = batch * h.heads * p.tiles, tokens = std::min(max_pages * h.page, span), sms = sm_count();
+  const int64_t unit = 16 * kv8_runs(h.dim) * kKvWarps, steps = std::max<int64_t>(1, (tokens + unit - 1) / unit);
+  int64_t best = -1;
+  for (int64_t n = 1; n <= std::min<int64_t>(steps, 128); ++n) {
+    const int64_t share = std::max<int64_t>(p.tile_rows == 8 ? 12 : 9, 5 * ((ctas * n + sms - 1) / sms));
+    const int64_t time = share * ((steps + n - 1) / n + 2) + (n > kKvCluster ? 30 : n > 1 ? 8 : 0);
+    if (best < 0 || time < best) {
+      best = time;
+      p.splits = (int)n;
+    }
+  }
+  if (p.splits > kKvCluster) p.bytes = (size_t)(ctas * p.splits * p.tile_rows) * (h.dim * sizeof(float) + sizeof(float2));
+  return p;
+}
+
+template <typename T, int kDim, int kNT>
+static cudaError_t launch_attention(const Kv8AttnParams& p, const Kv8Plan& plan, cudaStream_t s) {
+  constexpr int kSmem = kv8_smem_bytes(kDim, kNT);
+  static OncePerDevice once;
+  cudaError_t e = once.run([] {
+    return cudaFuncSetAttribute(kv8_attention_kernel<T, kDim, kNT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+  });
+  if (e != cudaSuccess) return e;
+  LaunchShape l(dim3(plan.splits * plan.tiles, p.sh.heads, p.batch), 32 * kKvWarps, kSmem, s);
+  if (plan.splits > 1 && plan.splits <= kKvCluster) l.cluster(plan.splits, 1, 1);
+  e = cudaLaunchKernelEx(&l.cfg, kv8_attention_kernel<T, kDim, kNT>, p);
+  if (e != cudaSuccess || plan.splits <= kKvCluster) return e;
+  qrb200_internal_count_launch();
+  LaunchShape j(dim3(p.batch * p.queries * p.q_heads), 32 * kKvJoinWarps, 0, s);
+  return cudaLaunchKernelEx(&j.cfg, kv_join_kernel<T, kDim, Kv8AttnParams>, p, plan.tile_rows);
 }
 
 }  // namespace qrb200
@@ -89,7 +140,10 @@ int qrb200_kv8_read(const void* codes, const float* range, const qrb200_kv8_shap
   return launched();
 }
 
-// The launch grid is work x heads x batch, a large batch in several launches.
+// The most tokens that a sequence's queries see between them.
+static int64_t token_span(int64_t queries, int64_t window) { return window > 0 ? std::min(window, kMaxRows) + queries : kMaxRows; }
+
+// The launch grid is (splits x row tiles) x key heads x batch, a large batch in several launches.
 constexpr int64_t kGridZ = 65535;
 static bool attention_args(const qrb200_kv8_shape* shape, int64_t batch, int64_t queries, int64_t q_heads, int64_t max_pages,
                            Kv8Shape* h) {
@@ -103,7 +157,7 @@ size_t qrb200_kv8_attention_workspace_bytes(const qrb200_kv8_shape* shape, int64
                                             int64_t max_pages, int64_t window) {
   Kv8Shape h;
   if (window < 0 || !attention_args(shape, batch, queries, q_heads, max_pages, &h)) return 0;
-  return 0;
+  return batch * queries * q_heads == 0 ? 0 : attn_plan(h, batch, queries, q_heads, max_pages, token_span(queries, window)).bytes;
 }
 
 int qrb200_kv8_attention(const void* q, const int64_t* q_strides, const void* codes, const float* range,
@@ -119,7 +173,9 @@ int qrb200_kv8_attention(const void* q, const int64_t* q_strides, const void* co
     return QRB200_ERR_ARG;
   const int st = quant_ready();
   if (st != QRB200_OK) return st;
-  (void)workspace, (void)workspace_bytes;
+  const Kv8Plan plan = attn_plan(h, batch, queries, q_heads, max_pages, token_span(queries, window));
+  if (plan.bytes > 0 && (!workspace || workspace_bytes < plan.bytes || (reinterpret_cast<uintptr_t>(workspace) & 255u)))
+    return QRB200_ERR_WORKSPACE;
   Kv8AttnParams p{};
   p.codes = static_cast<const unsigned char*>(codes);
   p.range = range;
@@ -131,20 +187,27 @@ int qrb200_kv8_attention(const void* q, const int64_t* q_strides, const void* co
   p.batch = (int)batch, p.queries = (int)queries, p.q_heads = (int)q_heads, p.share = (int)(q_heads / h.heads);
   // A window that reaches every token from every position is none (and cannot overflow a position).
   p.window = window >= max_pages * h.page + queries ? 0 : (int)window;
-  p.max_pages = (int)max_pages, p.causal = causal;
-  p.scale = scale;
+  p.max_pages = (int)max_pages, p.causal = causal, p.splits = plan.splits, p.tiles = plan.tiles;
+  p.scale_part = std::frexp(scale, &p.scale_power) * 2.f * 1.4426950408889634f;
+  p.scale_power -= 1;
   p.sh = h;
+  p.q_wide = (reinterpret_cast<uintptr_t>(q) & 7u) == 0 && ((q_strides[0] | q_strides[1] | q_strides[2]) & 3) == 0;
+  p.part_o = static_cast<float*>(workspace);
+  if (plan.splits > kKvCluster)
+    p.part_ml = reinterpret_cast<float2*>(p.part_o + batch * h.heads * plan.tiles * plan.splits * plan.tile_rows * h.dim);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   for (int64_t b = 0; b < batch; b += kGridZ) {
     Kv8AttnParams part = p;
+    const int64_t rows = b * queries * q_heads, parts = b * h.heads * plan.tiles * plan.splits * plan.tile_rows;
     part.batch = (int)std::min(kGridZ, batch - b);
     part.q = static_cast<const char*>(q) + 2 * b * p.q_bs;
-    part.out = static_cast<char*>(out) + 2 * b * queries * q_heads * h.dim;
+    part.out = static_cast<char*>(out) + 2 * rows * h.dim;
     part.table += b * table_stride;
     part.lengths += b;
+    if (p.part_ml) part.part_o += parts * h.dim, part.part_ml += parts;
     const cudaError_t e = with_shape(shape->dtype, h.dim, [&](auto type, auto dim) {
-      LaunchShape l(dim3(ceil_div(queries, 4), q_heads, part.batch), 128, 0, s);
-      return cudaLaunchKernelEx(&l.cfg, kv8_simple_kernel<decltype(type), dim()>, part);
+      return plan.tile_rows == 8 ? launch_attention<decltype(type), dim(), 1>(part, plan, s)
+                                 : launch_attention<decltype(type), dim(), 2>(part, plan, s);
     });
     if (e != cudaSuccess) return QRB200_ERR_CUDA;
     const int ended = launched();

@@ -2,7 +2,7 @@
 //
 // Keys and values of a page and head have a range R each, and a code stands for code R / 127. Tokens come
 // a few at a time, so R grows as they do: with a = the largest magnitude written,
-//   R = max(R, a rounded up to three significant bits),   code = rint(127 x / R),
+//   R = max(R, a rounded up to three significant bits),   code = rint(127 x / R)   (a half to the larger magnitude),
 // and where R grew from R' the codes of the page's other tokens become rint(code R' / R). (Rounded up, R
 // takes at most four steps to double, so a token is seldom rounded again; that costs at most a quarter
 // of the range, 9 % on average. It also makes the quotients safe: 127 x / R is midway between two
@@ -20,6 +20,8 @@
 //   values: rows are channels, columns tokens. Pieces of 32 channels; of each, 16 bytes for every lane: word w
 //     holds channel 16 (w / 2) + 8 (w % 2) + g, its bytes tokens 2t, 2t+1, 2t+8, 2t+9.
 #pragma once
+
+#include <type_traits>
 
 #include "quant_rows.cuh"
 #include "tc.cuh"
@@ -59,12 +61,15 @@ __device__ __forceinline__ int kv8_value_at(int dim, int token, int c) {
 constexpr uint32_t kKv8Zeros = 0x80808080u;
 constexpr int kKv8Few = 1024;  // rows up to which a CTA looks a page's rows up among all of them
 
-// Three significant bits, rounded up, of a magnitude's bits; NaN for what is not finite.
+// Three significant bits, rounded up, of a magnitude's bits (the magnitude itself where that would pass the type's
+// largest number, so that no value reads back as infinity); NaN for what is not finite.
+template <typename T>
 __device__ __forceinline__ float kv8_range(unsigned top) {
   if (top >= 0x7f800000u) return __int_as_float(0x7fffffff);
   if (__uint_as_float(top) < kTinyRow) return 0.f;
   const unsigned up = (top + 0x1fffffu) & ~0x1fffffu;
-  return __uint_as_float(up < 0x7f800000u ? up : top);
+  constexpr unsigned kMost = std::is_same<T, __half>::value ? 0x477fe000u : 0x7f7f0000u;  // 65504; 255 2^120
+  return __uint_as_float(up <= kMost ? up : top);
 }
 __device__ __forceinline__ float kv8_step(float range) { return range / 127.f; }
 // 127 / R, a little up: the one x between two codes, R / 2, goes to the upper one, and nothing else moves.
@@ -155,7 +160,7 @@ __global__ void __launch_bounds__(256) kv8_write_kernel(Kv8IoParams P) {
     float old[2], now[2];
 #pragma unroll
     for (int part = 0; part < 2; ++part) {
-      const float grown = kv8_range(__reduce_max_sync(kFullMask, s_top[part][tid & 7]));
+      const float grown = kv8_range<T>(__reduce_max_sync(kFullMask, s_top[part][tid & 7]));
       old[part] = fresh ? 0.f : range[part];
       now[part] = grown == grown && old[part] == old[part] ? fmaxf(grown, old[part]) : __int_as_float(0x7fffffff);
     }

@@ -1,7 +1,15 @@
 // Attention over the 8-bit cache (layout and formulas: kv8.cuh).
+//
+// With r_t and w_t the steps (range / 127) of token t's page for keys and values, c_t its codes:
+//   q . k_t = r_t (q . c_t),     o = sum_t (p_t w_t) c_t.
+// So the codes are the matrix operands, exact in 16 bits: a byte c + 128 under the exponent of 1024 is the fp16 number
+// 1152 + c, one addition away from c. No key or value is ever rounded; steps are applied in 32 bits.
 #pragma once
 
+#include <type_traits>
+
 #include "kv8.cuh"
+#include "kv_common.cuh"
 
 namespace qrb200 {
 
@@ -10,52 +18,450 @@ struct Kv8AttnParams {
   const float* range;
   const void* q;
   void* out;
+  float* part_o;   // [batch][head][tile][split][rows of a tile][dim], unnormalised, when splits > kKvCluster
+  float2* part_ml;  // [...][rows of a tile]: maximum (base 2) and sum
   const int* table;
   const int* lengths;
   long long q_bs, q_ts, q_hs, table_stride;  // strides in elements
-  int batch, queries, q_heads, share, max_pages, window, causal;
-  float scale;
+  int batch, queries, q_heads, share, max_pages, window, causal, splits, tiles;
+  int q_wide;    // four channels of q lie on an 8-byte boundary
+  float scale_part;  // the scale's significand times log2(e)
+  int scale_power;   // and its power of two
   Kv8Shape sh;
 };
 
-// A warp to a query row: token after token, its channels over the lanes.
-template <typename T, int kDim>
-__global__ void __launch_bounds__(128) kv8_simple_kernel(Kv8AttnParams P) {
-  constexpr int kPer = kDim / 32;
+// Two codes of a word (bytes 0 and 1, or 2 and 3) as fp16 numbers.
+template <int kHigh>
+__device__ __forceinline__ uint32_t kv8_codes(uint32_t w) {
+  const uint32_t x = __byte_perm(w, 0x64646464u, kHigh ? 0x4342 : 0x4140);
+  const __half2 c = __hsub2(reinterpret_cast<const __half2&>(x), __half2half2(__ushort_as_half(0x6480)));  // 1152
+  return reinterpret_cast<const uint32_t&>(c);
+}
+// An 8-bit number's significand in [1, 2), and its power of two.
+__device__ __forceinline__ float kv8_part(float x) { return __uint_as_float((__float_as_uint(x) & 0x807fffffu) | 0x3f800000u); }
+__device__ __forceinline__ int kv8_power(float x) { return (int)(__float_as_uint(x) >> 23 & 255) - 127; }
+
+constexpr int kKv8Top = 14;      // where a query row's largest entry is put (its exponent)
+constexpr int kKv8StepExp = 10;  // the largest value step's place: weights stay below 2^(10 + 4) in fp16
+constexpr int kKv8Aside = 8;     // steps between settings-aside
+
+// Runs of 16 tokens in a warp's step, steps in its ring, and CTAs to an SM that registers are kept for.
+__host__ __device__ constexpr int kv8_runs(int dim) { return dim == 64 ? 4 : 2; }
+__host__ __device__ constexpr int kv8_stages(int) { return 2; }
+__host__ __device__ constexpr int kv8_ctas(int nt) { return nt > 1 ? 2 : 2; }
+__host__ __device__ constexpr int kv8_ring_bytes(int dim, int nt) {
+  const int ring = kKvWarps * kv8_stages(nt) * kv8_runs(dim) * 32 * dim, parts = kKvWarps * 8 * nt * (dim + 4) * 4;
+  return ring > parts ? ring : parts;
+}
+// Dynamic shared memory: the warps' rings, reused at the end for their parts of the output, and
+// behind them the sums set aside.
+__host__ __device__ constexpr int kv8_smem_bytes(int dim, int nt) { return kv8_ring_bytes(dim, nt) + kKvWarps * 8 * nt * dim * 4; }
+
+template <typename T, int kDim, int kNT>
+__global__ void __launch_bounds__(32 * kKvWarps, kv8_ctas(kNT)) kv8_attention_kernel(Kv8AttnParams P) {
+  constexpr int kRows = 8 * kNT;      // query rows of a tile
+  constexpr int kSteps = kDim / 16;   // 16-channel steps of q . k; also 16-channel tiles of the output
+  constexpr int kRuns = kv8_runs(kDim), kUnit = 16 * kRuns;
+  constexpr int kRunBytes = 32 * kDim, kStage = kRuns * kRunBytes;
+  constexpr int kStages = kv8_stages(kNT);
+  constexpr float kNone = -INFINITY;
+  extern __shared__ __align__(128) unsigned char s_ring[];
+  __shared__ uint2 s_q[kNT][kSteps][32];
+  __shared__ unsigned s_qtop[kKvWarps][kNT][8];
+  __shared__ float2 s_step[kKvWarps][kStages][kRuns];  // a run's key and value steps
+  __shared__ float2 s_ml[kKvWarps][kRows];
+  __shared__ uint64_t s_full[kKvWarps][kStages];
+  __shared__ int s_bad;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int split = blockIdx.x % P.splits, tile = blockIdx.x / P.splits, head = blockIdx.y, b = blockIdx.z;
+  const int rows = P.queries * P.share, row0 = tile * kRows;
+
+  if (threadIdx.x == 0) s_bad = 0;
+  if (lane == 0) {
+    for (int i = 0; i < kStages; ++i) mbar_init(&s_full[warp][i], 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    fence_async_smem();
+  }
+  __syncwarp();
   griddep_launch_wait();
-  const int lane = threadIdx.x & 31, head = blockIdx.y, b = blockIdx.z;
-  const long long query = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
-  if (query >= P.queries) return;
   int len = P.lengths[b];
+  // The queries, asked for before anything waits: step j wants channels 16 j + 4 t + {0, 1} and {2,
+  // 3} of row g.
+  T qv[kNT][kSteps / kKvWarps][4];
+#pragma unroll
+  for (int n = 0; n < kNT; ++n) {
+    const int r = row0 + 8 * n + g;
+    const T* q = static_cast<const T*>(P.q) + b * P.q_bs + (long long)(r / P.share) * P.q_ts +
+                 (head * P.share + r % P.share) * P.q_hs + 4 * t;
+#pragma unroll
+    for (int i = 0; i < kSteps / kKvWarps; ++i) {
+      const T* at = q + 16 * (i * kKvWarps + warp);
+      if (P.q_wide) {
+        *reinterpret_cast<uint2*>(qv[n][i]) = r < rows ? __ldg(reinterpret_cast<const uint2*>(at)) : make_uint2(0, 0);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) qv[n][i][e] = r < rows ? at[e] : from_f32<T>(0.f);
+      }
+    }
+  }
   if (len < 0 || len > (long long)P.max_pages * P.sh.page || (len > 0 && P.sh.pages == 0)) {
-    if (lane == 0) report_device_failure(kSiteIndex);
+    if (threadIdx.x == 0) report_device_failure(kSiteIndex);
     len = 0;
   }
-  const T* q = static_cast<const T*>(P.q) + b * P.q_bs + query * P.q_ts + head * P.q_hs;
-  float qv[kPer], o[kPer] = {}, m = -INFINITY, l = 0.f;
-  for (int i = 0; i < kPer; ++i) qv[i] = to_f32(q[32 * i + lane]) * P.scale;
-  const int pos = len - P.queries + (int)query, hi = P.causal ? max(0, pos + 1) : len;
-  const int lo = P.window > 0 ? max(0, pos - P.window + 1) : 0;
-  for (int tok = lo; tok < hi; ++tok) {
-    const int page = P.table[b * P.table_stride + (tok >> P.sh.shift)], j = tok & (P.sh.page - 1);
-    if (page < 0 || page >= P.sh.pages) {
-      if (lane == 0) report_device_failure(kSiteIndex);
-      continue;
-    }
-    const long long at = (long long)page * P.sh.heads + head / P.share;
-    const unsigned char* block = P.codes + at * P.sh.block_bytes();
-    float s = 0.f;
-    for (int i = 0; i < kPer; ++i) s = fmaf(qv[i], (float)((int)block[kv8_key_at(kDim, j, 32 * i + lane)] - 128), s);
-    for (int x = 16; x; x >>= 1) s += __shfl_xor_sync(kFullMask, s, x);
-    s *= kv8_step(P.range[at * 2]);
-    const float step = kv8_step(P.range[at * 2 + 1]), next = fmaxf(m, s);
-    const float keep = m == -INFINITY ? 0.f : expf(m - next), p = expf(s - next);
-    l = fmaf(l, keep, p);
-    for (int i = 0; i < kPer; ++i) o[i] = fmaf(o[i], keep, p * step * (float)((int)block[kv8_value_at(kDim, j, 32 * i + lane)] - 128));
-    m = next;
+  // Tokens [lo, hi) that each row sees (lane r holds row r's), all rows together, and every row.
+  int my_lo = 0, my_hi = 0;
+  const bool real = lane < kRows && row0 + lane < rows;
+  if (real) {
+    const int pos = len - P.queries + (row0 + lane) / P.share;
+    my_hi = P.causal ? max(0, pos + 1) : len;
+    my_lo = P.window > 0 ? max(0, pos - P.window + 1) : 0;
   }
-  T* out = static_cast<T*>(P.out) + (((long long)b * P.queries + query) * P.q_heads + head) * kDim;
-  for (int i = 0; i < kPer; ++i) out[32 * i + lane] = from_f32<T>(l == 0.f ? 0.f : o[i] / l);
+  const bool sees = my_hi > my_lo;
+  const int all_lo = __reduce_min_sync(kFullMask, sees ? my_lo : 0x7fffffff);
+  const int all_hi = __reduce_max_sync(kFullMask, sees ? my_hi : 0);
+  const int in_lo = __reduce_max_sync(kFullMask, my_lo), in_hi = __reduce_min_sync(kFullMask, real ? my_hi : 0x7fffffff);
+  // This warp's steps [u, u_hi) of its CTA's share of the range.
+  const int u0 = all_hi > 0 ? all_lo / kUnit : 0, u1 = (all_hi + kUnit - 1) / kUnit;
+  const int per = (u1 - u0 + P.splits - 1) / P.splits;
+  const int cta_lo = min(u1, u0 + split * per), cta_hi = min(u1, cta_lo + per);
+  const int per_warp = (cta_hi - cta_lo + kKvWarps - 1) / kKvWarps;
+  int u = min(cta_hi, cta_lo + warp * per_warp);
+  const int u_hi = min(cta_hi, u + per_warp);
+
+  // The ring. Lane i of `page` holds the page of run `page_base` + i, -1 outside the range, before
+  // which pages may be gone from the table, or where the table is wrong; `steps` its steps.
+  unsigned char* ring = s_ring + warp * (kStages * kStage);
+  const int page_runs = P.sh.page / 16, page_shift = P.sh.shift - 4;
+  const int first_run = all_lo / 16, last_run = min(u_hi * kRuns, (len + 15) / 16);
+  int page_base = u * kRuns, page = -1;
+  float2 step = make_float2(0.f, 0.f);
+  auto look_up = [&]() {
+    page = -1;
+    step = make_float2(0.f, 0.f);
+    if (page_base + lane >= first_run && page_base + lane < last_run) {
+      page = __ldg(P.table + b * P.table_stride + ((page_base + lane) >> page_shift));
+      if (page < 0 || page >= P.sh.pages) {
+        report_device_failure(kSiteIndex);
+        page = -1;
+      } else {
+        step = __ldg(reinterpret_cast<const float2*>(P.range) + (long long)page * P.sh.heads + head);
+        step.x = kv8_step(step.x), step.y = kv8_step(step.y);
+      }
+    }
+  };
+  unsigned missing = 0;  // kRuns bits a stage: its runs without a page
+  auto issue = [&](int unit, int stage) {
+    if (unit * kRuns >= page_base + 32) {
+      page_base = unit * kRuns;
+      look_up();
+    }
+    const uint32_t bar = smem_u32(&s_full[warp][stage]), dst = smem_u32(ring + stage * kStage);
+    const int mine = page_base + lane - unit * kRuns;
+    if (mine >= 0 && mine < kRuns) s_step[warp][stage][mine] = step;
+    const auto at = [&](int pg, int run) {
+      return P.codes + ((long long)pg * P.sh.heads + head) * P.sh.block_bytes() + (run & (page_runs - 1)) * kRunBytes;
+    };
+    unsigned gone = 0;
+    if (page_runs >= kRuns && (unit + 1) * kRuns <= last_run) {  // one page, the last run's, holds the step: one copy
+      const int run = unit * kRuns, pg = __shfl_sync(kFullMask, page, run + kRuns - 1 - page_base);
+      if (pg < 0) gone = (1u << kRuns) - 1;
+      if (lane == 0) {
+        mbar_expect(bar, pg < 0 ? 0 : kStage);
+        if (pg >= 0) kv_copy(dst, at(pg, run), kStage, bar);
+      }
+    } else {
+      for (int i = 0; i < kRuns; ++i) gone |= __shfl_sync(kFullMask, page, unit * kRuns + i - page_base) < 0 ? 1u << i : 0u;
+      if (lane == 0) mbar_expect(bar, (kRuns - __popc(gone)) * kRunBytes);
+      for (int i = 0; i < kRuns; ++i) {
+        const int run = unit * kRuns + i, pg = __shfl_sync(kFullMask, page, run - page_base);
+        if (lane == 0 && pg >= 0) kv_copy(dst + i * kRunBytes, at(pg, run), kRunBytes, bar);
+      }
+    }
+    missing = (missing & ~(((1u << kRuns) - 1) << (8 * stage))) | gone << (8 * stage);
+  };
+  const int count = u_hi - u;
+  if (count > 0) look_up();
+  for (int i = 0; i < kStages && i < count; ++i) issue(u + i, i);
+
+  // Queries as the right operand, in fp16: each row brought by a power of two to the top of its range, where
+  // what the largest entry leaves of the others is 2^-38 of it. The warps share the work; first each row's
+  // largest entry.
+#pragma unroll
+  for (int n = 0; n < kNT; ++n) {
+    unsigned top = 0;
+#pragma unroll
+    for (int i = 0; i < kSteps / kKvWarps; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) top = max(top, __float_as_uint(to_f32(qv[n][i][e])) & 0x7fffffffu);
+#pragma unroll
+    for (int x = 1; x <= 2; x <<= 1) top = max(top, __shfl_xor_sync(kFullMask, top, x));
+    if (t == 0) s_qtop[warp][n][g] = top;
+  }
+  __syncthreads();
+  const auto power = [&](int n, int row) {  // of the row's largest entry; a row of zeros or of no numbers has any
+    unsigned top = 0;
+    for (int w = 0; w < kKvWarps; ++w) top = max(top, s_qtop[w][n][row]);
+    return max(1, min(254, (int)(top >> 23))) - 127;
+  };
+  // back: the power of two that takes a row's size and the scale's back, into the exponent's units (base 2).
+  int back[kNT][2];
+#pragma unroll
+  for (int n = 0; n < kNT; ++n) {
+    const int lift = kKv8Top - power(n, g);  // up to 140: in two factors
+    const float up = kv_power(lift / 2), more = kv_power(lift - lift / 2);
+#pragma unroll
+    for (int i = 0; i < kSteps / kKvWarps; ++i) {
+      alignas(8) __half x[4];
+      put2(x, to_f32(qv[n][i][0]) * up * more, to_f32(qv[n][i][1]) * up * more);
+      put2(x + 2, to_f32(qv[n][i][2]) * up * more, to_f32(qv[n][i][3]) * up * more);
+      s_q[n][i * kKvWarps + warp][lane] = *reinterpret_cast<uint2*>(x);
+    }
+    back[n][0] = power(n, 2 * t) - kKv8Top + P.scale_power;
+    back[n][1] = power(n, 2 * t + 1) - kKv8Top + P.scale_power;
+  }
+  __syncthreads();
+
+  float o[kNT][kSteps][4] = {};  // scaled by `unit`
+  float2 sum[kNT] = {};
+  // Weights are 2^(score + less), the reference being -less; bound is where a score moves it: 4
+  // above, rounded down where scores are so large (so the reference cannot be had back from it), and
+  // -inf while nothing has been seen. cap bounds the value steps, unit scales them.
+  float2 less[kNT] = {};
+  float bound[kNT][2], cap = 0.f, unit = 1.f;
+#pragma unroll
+  for (int n = 0; n < kNT; ++n) bound[n][0] = bound[n][1] = kNone;
+  const auto reference = [&](int n, int c) { return bound[n][c] == kNone ? kNone : -(c ? less[n].y : less[n].x); };
+
+  // This lane's sums set aside, 32 lanes apart; `aside` once there are some.
+  float4* apart = reinterpret_cast<float4*>(s_ring + kv8_ring_bytes(kDim, kNT)) + warp * (kRows * kDim / 4) + lane;
+  bool ok = true, aside = false;
+  int stage = 0, turn = 0;
+  for (int k = 0; ok && k < count;) {
+    const int pause = min(count, k + kKv8Aside);
+    for (; k < pause; ++k, ++u) {
+      const int tok0 = u * kUnit;
+      const unsigned char* runs = ring + stage * kStage;
+      const unsigned gone = missing >> (8 * stage) & ((1u << kRuns) - 1);
+      ok = ok && __all_sync(kFullMask, mbar_wait_quick(&s_full[warp][stage], turn));
+      if (!ok) break;
+      // Scores: s[i][n][h] holds token tok0 + 16 i + 8 h + g against rows 8 n + 2 t
+      // and the next.
+      float2 s[kRuns][kNT][2];
+      float2 steps[kRuns];
+      {
+        float acc[kRuns][kNT][4] = {};
+#pragma unroll
+        for (int c = 0; c < kDim / 64; ++c) {
+          uint32_t kc[kRuns][2][4];
+#pragma unroll
+          for (int i = 0; i < kRuns; ++i)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) kv_load(kc[i][h], runs + i * kRunBytes + h * (8 * kDim) + c * 512 + lane * 16);
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            uint2 q[kNT];
+#pragma unroll
+            for (int n = 0; n < kNT; ++n) q[n] = s_q[n][4 * c + w][lane];
+#pragma unroll
+            for (int i = 0; i < kRuns; ++i) {
+              const uint32_t a[4] = {kv8_codes<0>(kc[i][0][w]), kv8_codes<0>(kc[i][1][w]), kv8_codes<1>(kc[i][0][w]), kv8_codes<1>(kc[i][1][w])};
+#pragma unroll
+              for (int n = 0; n < kNT; ++n) kv_mma<__half>(acc[i][n], a, q[n].x, q[n].y);
+            }
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < kRuns; ++i) {
+          steps[i] = s_step[warp][stage][i];
+          const float keys = steps[i].x > 0.f ? kv8_part(steps[i].x) * P.scale_part : steps[i].x;  // 0 and NaN as they are
+          const int e = kv8_power(steps[i].x);
+#pragma unroll
+          for (int n = 0; n < kNT; ++n) {
+            const float2 f = make_float2(keys * kv_power(e + back[n][0]), keys * kv_power(e + back[n][1]));
+#pragma unroll
+            for (int h = 0; h < 2; ++h) s[i][n][h] = __fmul2_rn(make_float2(acc[i][n][2 * h], acc[i][n][2 * h + 1]), f);
+          }
+        }
+      }
+      const bool full = !gone && tok0 >= in_lo && tok0 + kUnit <= in_hi;  // every row sees every token
+      uint32_t seen[kNT];
+      if (!full) {
+#pragma unroll
+        for (int n = 0; n < kNT; ++n) {
+          int lo[2], hi[2];
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            lo[c] = __shfl_sync(kFullMask, my_lo, 8 * n + 2 * t + c);
+            hi[c] = __shfl_sync(kFullMask, my_hi, 8 * n + 2 * t + c);
+          }
+          seen[n] = 0;
+#pragma unroll
+          for (int i = 0; i < kRuns; ++i)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const int tok = tok0 + 16 * i + 8 * h + g;
+              const bool x = tok >= lo[0] && tok < hi[0] && !(gone >> i & 1);
+              const bool y = tok >= lo[1] && tok < hi[1] && !(gone >> i & 1);
+              seen[n] |= (x ? 1u : 0u) << (4 * i + 2 * h) | (y ? 2u : 0u) << (4 * i + 2 * h);
+              if (!x) s[i][n][h].x = kNone;
+              if (!y) s[i][n][h].y = kNone;
+            }
+        }
+      }
+      float up[kNT][2], most = 0.f;
+#pragma unroll
+      for (int i = 0; i < kRuns; ++i) most = fmaxf(most, steps[i].y);
+      bool move = most > cap;
+#pragma unroll
+      for (int n = 0; n < kNT; ++n) {
+        up[n][0] = s[0][n][0].x;
+        up[n][1] = s[0][n][0].y;
+#pragma unroll
+        for (int i = 0; i < kRuns; ++i)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            up[n][0] = fmaxf(up[n][0], s[i][n][h].x);
+            up[n][1] = fmaxf(up[n][1], s[i][n][h].y);
+          }
+        move = move || up[n][0] > bound[n][0] || up[n][1] > bound[n][1];
+      }
+      if (__any_sync(kFullMask, move)) {
+        most = fmaxf(most, cap);  // the same in every lane
+        float ratio = 1.f;
+        if (most > cap) {  // the power of two above the largest step, and the scale that puts it at 2^kKv8StepExp
+          const int e = max(-100, min(126, (int)(__float_as_uint(most) >> 23) - 126));
+          cap = __int_as_float((e + 127) << 23);
+          const float fresh = __int_as_float((kKv8StepExp - e + 127) << 23);
+          ratio = fresh / unit;
+          unit = fresh;
+        }
+#pragma unroll
+        for (int n = 0; n < kNT; ++n) {
+          float keep[2];
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+#pragma unroll
+            for (int x = 4; x < 32; x <<= 1) up[n][c] = fmaxf(up[n][c], __shfl_xor_sync(kFullMask, up[n][c], x));
+            const float last = reference(n, c), next = fmaxf(up[n][c], last);
+            keep[c] = next == kNone ? 0.f : kv_exp2(last - next);
+            bound[n][c] = __fadd_rd(next, kKvLazy);
+            // A row that has seen nothing has the reference -inf: its weights, 2^-inf, come from any
+            // finite one.
+            (c ? less[n].y : less[n].x) = next == kNone ? 0.f : -next;
+          }
+          sum[n] = make_float2(sum[n].x * keep[0], sum[n].y * keep[1]);
+#pragma unroll
+          for (int j = 0; j < kSteps; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[n][j][e] *= keep[e & 1] * ratio;
+          if (aside) {
+#pragma unroll
+            for (int j = 0; j < kSteps; ++j) {
+              float4 a = apart[32 * (n * kSteps + j)];
+              a.x *= keep[0] * ratio, a.y *= keep[1] * ratio, a.z *= keep[0] * ratio, a.w *= keep[1] * ratio;
+              apart[32 * (n * kSteps + j)] = a;
+            }
+          }
+        }
+      }
+      // Weights and output; kAll: every row sees every token (no tests in the common case).
+      auto finish = [&](auto all) {
+        constexpr bool kAll = decltype(all)::value;
+#pragma unroll
+        for (int i = 0; i < kRuns; ++i) {
+          uint32_t w[2][kNT][2];
+          const float scaled = steps[i].y * unit;
+#pragma unroll
+          for (int n = 0; n < kNT; ++n)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const float2 e = __fadd2_rn(s[i][n][h], less[n]), p = make_float2(kv_exp2(e.x), kv_exp2(e.y));
+              sum[n] = __fadd2_rn(sum[n], p);
+              float2 x = __fmul2_rn(p, make_float2(scaled, scaled));
+              if constexpr (!kAll) {  // what a row does not see may be NaN
+                if (!(seen[n] >> (4 * i + 2 * h) & 1)) x.x = 0.f;
+                if (!(seen[n] >> (4 * i + 2 * h) & 2)) x.y = 0.f;
+              }
+              const uint32_t high = kv_pack(x);
+              w[0][n][h] = kv_transpose(high);
+              const float2 top = __half22float2(__hneg2(reinterpret_cast<const __half2&>(high)));
+              w[1][n][h] = kv_transpose(kv_pack(__fadd2_rn(x, top)));
+            }
+#pragma unroll
+          for (int c = 0; c < kDim / 32; ++c) {
+            uint32_t vc[4];
+            kv_load(vc, runs + i * kRunBytes + 16 * kDim + c * 512 + lane * 16);
+#pragma unroll
+            for (int z = 0; z < 2; ++z) {
+              const uint32_t a[4] = {kv8_codes<0>(vc[2 * z]), kv8_codes<0>(vc[2 * z + 1]), kv8_codes<1>(vc[2 * z]), kv8_codes<1>(vc[2 * z + 1])};
+#pragma unroll
+              for (int n = 0; n < kNT; ++n)
+#pragma unroll
+                for (int half = 0; half < 2; ++half) kv_mma<__half>(o[n][2 * c + z], a, w[half][n][0], w[half][n][1]);
+            }
+          }
+        }
+      };
+      if (full) finish(std::true_type{});
+      else finish(std::false_type{});
+      __syncwarp();  // every lane has read this stage
+      if (k + kStages < count) issue(u + kStages, stage);
+      if (++stage == kStages) {
+        stage = 0;
+        turn ^= 1;
+      }
+    }
+    if (ok && k < count) {  // set the sums aside
+#pragma unroll
+      for (int n = 0; n < kNT; ++n)
+#pragma unroll
+        for (int j = 0; j < kSteps; ++j) {
+          float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (aside) a = apart[32 * (n * kSteps + j)];
+          a.x += o[n][j][0], a.y += o[n][j][1], a.z += o[n][j][2], a.w += o[n][j][3];
+          apart[32 * (n * kSteps + j)] = a;
+          o[n][j][0] = o[n][j][1] = o[n][j][2] = o[n][j][3] = 0.f;
+        }
+      aside = true;
+    }
+  }
+  if (!ok) {
+    // A copy did not arrive in time: nothing is written, and what is under way is waited for (with
+    // a limit) first.
+    for (int i = 0; i < kStages; ++i) mbar_wait(&s_full[warp][i], i < stage ? turn ^ 1 : turn);
+    s_bad = 1;
+  }
+  if (aside) {
+#pragma unroll
+    for (int n = 0; n < kNT; ++n)
+#pragma unroll
+      for (int j = 0; j < kSteps; ++j) {
+        const float4 a = apart[32 * (n * kSteps + j)];
+        o[n][j][0] += a.x, o[n][j][1] += a.y, o[n][j][2] += a.z, o[n][j][3] += a.w;
+      }
+  }
+  __syncthreads();  // the rings are free
+  float(*s_o)[kRows][kDim + 4] = reinterpret_cast<float(*)[kRows][kDim + 4]>(s_ring);
+
+  const float lower = 1.f / unit;
+  // The warps' parts: o[n][j][e] is channel 16 j + g + 8 (e / 2) of row 8 n + 2 t + e % 2.
+#pragma unroll
+  for (int n = 0; n < kNT; ++n)
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      float l = c ? sum[n].y : sum[n].x;
+#pragma unroll
+      for (int x = 4; x < 32; x <<= 1) l += __shfl_xor_sync(kFullMask, l, x);
+      if (g == 0) s_ml[warp][8 * n + 2 * t + c] = make_float2(reference(n, c), l);
+#pragma unroll
+      for (int j = 0; j < kSteps; ++j) {
+        s_o[warp][8 * n + 2 * t + c][16 * j + g] = o[n][j][c] * lower;
+        s_o[warp][8 * n + 2 * t + c][16 * j + g + 8] = o[n][j][2 + c] * lower;
+      }
+    }
+  __syncthreads();
+  kv_join_warps<T, kDim, kRows>(P, s_o, s_ml, reinterpret_cast<float*>(s_q), &s_bad, split, tile, head, b, rows, row0);
 }
 
 }  // namespace qrb200

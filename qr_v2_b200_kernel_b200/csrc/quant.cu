@@ -267,7 +267,7 @@ static cudaError_t launch_attention(Kv4AttnParams p, const AttnPlan& plan, cudaS
   if (e != cudaSuccess || plan.splits <= kKvCluster) return e;
   qrb200_internal_count_launch();
   LaunchShape j(dim3(p.batch * p.queries * p.q_heads), 32 * kKvJoinWarps, 0, s);
-  return cudaLaunchKernelEx(&j.cfg, kv4_join_kernel<T, kDim>, p, plan.tile_rows);
+  return cudaLaunchKernelEx(&j.cfg, kv_join_kernel<T, kDim, Kv4AttnParams>, p, plan.tile_rows);
 }
 
 template <typename T>
