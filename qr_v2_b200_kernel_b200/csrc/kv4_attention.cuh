@@ -54,7 +54,7 @@ struct Kv4AttnParams {
   const void* q;
   void* out;
   float* part_o;       // [batch][head][tile][split][rows of a tile][dim], unnormalised, when splits > kKvCluster
-  float2* part_ml;     // [...][rows of a tile]: maximum (base 2) and sum
+  float2* part_ml;     // [...][rows of a tile]: maximum (base 2) and sum; null where a cluster joins the parts
   const int* table;
   const int* lengths;
   long long q_bs, q_ts, q_hs, table_stride;  // strides in elements

@@ -21,50 +21,57 @@ static cudaError_t with_shape(int dtype, int dim, F&& f) {
   return dim == 64 ? f(__half{}, Int<64>{}) : f(__half{}, Int<128>{});
 }
 
-// How an attention call is cut: query rows per tile, and the token range over `splits` CTAs.
+// How an attention call is cut: query rows per tile, steps of 4 or 8 KB, and the token range over `splits` CTAs.
 struct Kv8Plan {
   int tile_rows, tiles, splits;
+  bool brief;   // short steps
+  bool memory;  // parts go through memory
   size_t bytes;  // workspace: the parts and their (maximum, sum) pairs
 };
 
-// Eight rows a tile where a key head has no more than eight query rows, else sixteen. The token
-// range is cut over the CTAs that make the least estimated time, in fifths of a step's share of a
-// busy SM: a CTA alone takes 2.4 such shares for a step (1.8 with sixteen rows), so up to
-// that many share an SM for nothing, and its set-up takes two steps; joining costs 1.5 in a cluster
-// and 6 through memory. The length is the table's capacity or what a window leaves of it, all that
-// the host knows.
+// Eight rows a tile where a key head has no more than eight query rows, else sixteen. Of both kinds of step and every number of
+// splits the least estimated time, in ns: waves of CTAs, a wave's steps at what one takes with so many CTAs on an SM
+// (measured with 128 channels), three steps for a CTA's set-up, 2 us for a join in a cluster and 4 through memory. Clusters place
+// badly where they fill the GPU (24 x 8192 tokens, 8 heads in threes: 99 us, through memory 70), so only what ends within one thin wave
+// joins so. The length is the table's capacity or what a window leaves of it, all that the host knows.
 static Kv8Plan attn_plan(const Kv8Shape& h, int64_t batch, int64_t queries, int64_t q_heads, int64_t max_pages, int64_t span) {
+  static const int kShort[5] = {0, 750, 1000, 1300, 1400}, kLong[3] = {0, 1000, 1400}, kLong16[3] = {0, 1500, 2300};
   Kv8Plan p{};
   const int64_t rows = queries * (q_heads / h.heads);
   p.tile_rows = rows <= 8 ? 8 : 16;
   p.tiles = ceil_div(rows, p.tile_rows);
   const int64_t ctas = batch * h.heads * p.tiles, tokens = std::min(max_pages * h.page, span), sms = sm_count();
-  const int64_t unit = 16 * kv8_runs(h.dim) * kKvWarps, steps = std::max<int64_t>(1, (tokens + unit - 1) / unit);
   int64_t best = -1;
-  for (int64_t n = 1; n <= std::min<int64_t>(steps, 128); ++n) {
-    const int64_t share = std::max<int64_t>(p.tile_rows == 8 ? 12 : 9, 5 * ((ctas * n + sms - 1) / sms));
-    const int64_t time = share * ((steps + n - 1) / n + 2) + (n > kKvCluster ? 30 : n > 1 ? 8 : 0);
-    if (best < 0 || time < best) {
-      best = time;
-      p.splits = (int)n;
+  for (int brief = 0; brief <= (p.tile_rows == 8 ? 1 : 0); ++brief) {
+    const int64_t unit = 16 * kv8_runs(h.dim, brief) * kKvWarps, steps = std::max<int64_t>(1, (tokens + unit - 1) / unit);
+    const int* ns = brief ? kShort : p.tile_rows == 8 ? kLong : kLong16;
+    const int per_sm = kv8_ctas(brief);
+    for (int64_t n = 1; n <= std::min<int64_t>(steps, 128); ++n) {
+      const int64_t all = ctas * n, waves = all / (per_sm * sms), rest = all - waves * per_sm * sms;
+      const bool memory = n > kKvCluster || (n > 1 && all > 2 * sms);
+      const int64_t time = ((steps + n - 1) / n + 3) * (waves * ns[per_sm] + ns[(rest + sms - 1) / sms]) + (memory ? 4000 : n > 1 ? 2000 : 0);
+      if (best < 0 || time < best) {
+        best = time;
+        p.splits = (int)n, p.brief = brief, p.memory = memory;
+      }
     }
   }
-  if (p.splits > kKvCluster) p.bytes = (size_t)(ctas * p.splits * p.tile_rows) * (h.dim * sizeof(float) + sizeof(float2));
+  if (p.memory) p.bytes = (size_t)(ctas * p.splits * p.tile_rows) * (h.dim * sizeof(float) + sizeof(float2));
   return p;
 }
 
-template <typename T, int kDim, int kNT>
+template <typename T, int kDim, int kNT, bool kBrief>
 static cudaError_t launch_attention(const Kv8AttnParams& p, const Kv8Plan& plan, cudaStream_t s) {
-  constexpr int kSmem = kv8_smem_bytes(kDim, kNT);
+  constexpr int kSmem = kv8_smem_bytes(kDim, kNT, kBrief);
   static OncePerDevice once;
   cudaError_t e = once.run([] {
-    return cudaFuncSetAttribute(kv8_attention_kernel<T, kDim, kNT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+    return cudaFuncSetAttribute(kv8_attention_kernel<T, kDim, kNT, kBrief>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
   });
   if (e != cudaSuccess) return e;
   LaunchShape l(dim3(plan.splits * plan.tiles, p.sh.heads, p.batch), 32 * kKvWarps, kSmem, s);
-  if (plan.splits > 1 && plan.splits <= kKvCluster) l.cluster(plan.splits, 1, 1);
-  e = cudaLaunchKernelEx(&l.cfg, kv8_attention_kernel<T, kDim, kNT>, p);
-  if (e != cudaSuccess || plan.splits <= kKvCluster) return e;
+  if (plan.splits > 1 && !plan.memory) l.cluster(plan.splits, 1, 1);
+  e = cudaLaunchKernelEx(&l.cfg, kv8_attention_kernel<T, kDim, kNT, kBrief>, p);
+  if (e != cudaSuccess || !plan.memory) return e;
   qrb200_internal_count_launch();
   LaunchShape j(dim3(p.batch * p.queries * p.q_heads), 32 * kKvJoinWarps, 0, s);
   return cudaLaunchKernelEx(&j.cfg, kv_join_kernel<T, kDim, Kv8AttnParams>, p, plan.tile_rows);
@@ -193,7 +200,7 @@ int qrb200_kv8_attention(const void* q, const int64_t* q_strides, const void* co
   p.sh = h;
   p.q_wide = (reinterpret_cast<uintptr_t>(q) & 7u) == 0 && ((q_strides[0] | q_strides[1] | q_strides[2]) & 3) == 0;
   p.part_o = static_cast<float*>(workspace);
-  if (plan.splits > kKvCluster)
+  if (plan.memory)
     p.part_ml = reinterpret_cast<float2*>(p.part_o + batch * h.heads * plan.tiles * plan.splits * plan.tile_rows * h.dim);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   for (int64_t b = 0; b < batch; b += kGridZ) {
@@ -206,8 +213,9 @@ int qrb200_kv8_attention(const void* q, const int64_t* q_strides, const void* co
     part.lengths += b;
     if (p.part_ml) part.part_o += parts * h.dim, part.part_ml += parts;
     const cudaError_t e = with_shape(shape->dtype, h.dim, [&](auto type, auto dim) {
-      return plan.tile_rows == 8 ? launch_attention<decltype(type), dim(), 1>(part, plan, s)
-                                 : launch_attention<decltype(type), dim(), 2>(part, plan, s);
+      using E = decltype(type);
+      if (plan.tile_rows == 16) return launch_attention<E, dim(), 2, false>(part, plan, s);
+      return plan.brief ? launch_attention<E, dim(), 1, true>(part, plan, s) : launch_attention<E, dim(), 1, false>(part, plan, s);
     });
     if (e != cudaSuccess) return QRB200_ERR_CUDA;
     const int ended = launched();

@@ -18,8 +18,8 @@ struct Kv8AttnParams {
   const float* range;
   const void* q;
   void* out;
-  float* part_o;   // [batch][head][tile][split][rows of a tile][dim], unnormalised, when splits > kKvCluster
-  float2* part_ml;  // [...][rows of a tile]: maximum (base 2) and sum
+  float* part_o;   // [batch][head][tile][split][rows of a tile][dim], unnormalised, where parts go through memory
+  float2* part_ml;  // [...][rows of a tile]: maximum (base 2) and sum; null where a cluster joins them
   const int* table;
   const int* lengths;
   long long q_bs, q_ts, q_hs, table_stride;  // strides in elements
@@ -45,25 +45,31 @@ constexpr int kKv8Top = 14;      // where a query row's largest entry is put (it
 constexpr int kKv8StepExp = 10;  // the largest value step's place: weights stay below 2^(10 + 4) in fp16
 constexpr int kKv8Aside = 8;     // steps between settings-aside
 
-// Runs of 16 tokens in a warp's step, steps in its ring, and CTAs to an SM that registers are kept for.
-__host__ __device__ constexpr int kv8_runs(int dim) { return dim == 64 ? 4 : 2; }
-__host__ __device__ constexpr int kv8_stages(int) { return 2; }
-__host__ __device__ constexpr int kv8_ctas(int nt) { return nt > 1 ? 2 : 2; }
-__host__ __device__ constexpr int kv8_ring_bytes(int dim, int nt) {
-  const int ring = kKvWarps * kv8_stages(nt) * kv8_runs(dim) * 32 * dim, parts = kKvWarps * 8 * nt * (dim + 4) * 4;
+// Bytes of a warp's step, 4 KB or 8: a step costs some 1000 clocks of instructions that wait for one another and 500 for each
+// 4 KB, so long steps suit few warps, and short ones leave shared memory for twice as many (four CTAs an SM for two,
+// at 128 registers for 168). With sixteen query rows, which take the registers of two CTAs anyway, long ones.
+// (64 x 8192 tokens, 8 heads: short 172 us, long 180; 16 x 8192 53, 51; 1 x 8192 13.8, 10.7; sixteen rows,
+// 64 x 8192 tokens, 4 heads: 159-174, 145.)
+__host__ __device__ constexpr int kv8_runs(int dim, bool brief) { return (brief ? 128 : 256) / dim; }
+constexpr int kKv8Stages = 2;  // steps in a warp's ring; more change nothing
+__host__ __device__ constexpr int kv8_ctas(bool brief) { return brief ? 4 : 2; }
+__host__ __device__ constexpr int kv8_ring_bytes(int dim, int nt, bool brief) {
+  const int ring = kKvWarps * kKv8Stages * kv8_runs(dim, brief) * 32 * dim, parts = kKvWarps * 8 * nt * (dim + 4) * 4;
   return ring > parts ? ring : parts;
 }
 // Dynamic shared memory: the warps' rings, reused at the end for their parts of the output, and
 // behind them the sums set aside.
-__host__ __device__ constexpr int kv8_smem_bytes(int dim, int nt) { return kv8_ring_bytes(dim, nt) + kKvWarps * 8 * nt * dim * 4; }
+__host__ __device__ constexpr int kv8_smem_bytes(int dim, int nt, bool brief) {
+  return kv8_ring_bytes(dim, nt, brief) + kKvWarps * 8 * nt * dim * 4;
+}
 
-template <typename T, int kDim, int kNT>
-__global__ void __launch_bounds__(32 * kKvWarps, kv8_ctas(kNT)) kv8_attention_kernel(Kv8AttnParams P) {
+template <typename T, int kDim, int kNT, bool kBrief>
+__global__ void __launch_bounds__(32 * kKvWarps, kv8_ctas(kBrief)) kv8_attention_kernel(Kv8AttnParams P) {
   constexpr int kRows = 8 * kNT;      // query rows of a tile
   constexpr int kSteps = kDim / 16;   // 16-channel steps of q . k; also 16-channel tiles of the output
-  constexpr int kRuns = kv8_runs(kDim), kUnit = 16 * kRuns;
+  constexpr int kRuns = kv8_runs(kDim, kBrief), kUnit = 16 * kRuns;
   constexpr int kRunBytes = 32 * kDim, kStage = kRuns * kRunBytes;
-  constexpr int kStages = kv8_stages(kNT);
+  constexpr int kStages = kKv8Stages;
   constexpr float kNone = -INFINITY;
   extern __shared__ __align__(128) unsigned char s_ring[];
   __shared__ uint2 s_q[kNT][kSteps][32];
@@ -234,7 +240,7 @@ __global__ void __launch_bounds__(32 * kKvWarps, kv8_ctas(kNT)) kv8_attention_ke
   const auto reference = [&](int n, int c) { return bound[n][c] == kNone ? kNone : -(c ? less[n].y : less[n].x); };
 
   // This lane's sums set aside, 32 lanes apart; `aside` once there are some.
-  float4* apart = reinterpret_cast<float4*>(s_ring + kv8_ring_bytes(kDim, kNT)) + warp * (kRows * kDim / 4) + lane;
+  float4* apart = reinterpret_cast<float4*>(s_ring + kv8_ring_bytes(kDim, kNT, kBrief)) + warp * (kRows * kDim / 4) + lane;
   bool ok = true, aside = false;
   int stage = 0, turn = 0;
   for (int k = 0; ok && k < count;) {
@@ -250,7 +256,7 @@ __global__ void __launch_bounds__(32 * kKvWarps, kv8_ctas(kNT)) kv8_attention_ke
       float2 s[kRuns][kNT][2];
       float2 steps[kRuns];
       {
-        float acc[kRuns][kNT][4] = {};
+        float acc[kRuns][kNT][4] = {};  // (even and odd steps apart, a chain of products half as long: 172 -> 182 us at 64 x 8192 tokens)
 #pragma unroll
         for (int c = 0; c < kDim / 64; ++c) {
           uint32_t kc[kRuns][2][4];

@@ -103,7 +103,7 @@ __device__ __forceinline__ void kv_join_warps(const Params& P, float (*s_o)[kRow
     const float inv = l == 0.f ? 0.f : 1.f / l;  // nothing seen: zeros
     if (row0 + r < rows && !*s_bad)
       for (int d = d0; d < kDim; d += kLanesRow) out_row(r)[d] = from_f32<T>(joined(d) * inv);
-  } else if (P.splits <= kKvCluster) {
+  } else if (!P.part_ml) {
     // The CTA's part takes its first warp's place; each CTA then joins every splits-th row of all
     // of them.
     for (int d = d0; d < kDim; d += kLanesRow) s_o[0][r][d] = joined(d);
