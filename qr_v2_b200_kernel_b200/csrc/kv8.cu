@@ -31,9 +31,9 @@ struct Kv8Plan {
 
 // Eight rows a tile where a key head has no more than eight query rows, else sixteen. Of both kinds of step and every number of
 // splits the least estimated time, in ns: waves of CTAs, a wave's steps at what one takes with so many CTAs on an SM
-// (measured with 128 channels), three steps for a CTA's set-up, 2 us for a join in a cluster and 4 through memory. Clusters place
-// badly where they fill the GPU (24 x 8192 tokens, 8 heads in threes: 99 us, through memory 70), so only what ends within one thin wave
-// joins so. The length is the table's capacity or what a window leaves of it, all that the host knows.
+// (measured with 128 channels), three steps for a CTA's set-up, 2 us for a join in a cluster and 4 through memory. Clusters of
+// other than two or four CTAs place badly where they fill the GPU (24 x 8192 tokens, 8 heads in threes: 99 us, through memory 70; in
+// pairs 64 x 8192 172, through memory 180), so those are left to thin waves. The length is the table's capacity or what a window leaves of it, all that the host knows.
 static Kv8Plan attn_plan(const Kv8Shape& h, int64_t batch, int64_t queries, int64_t q_heads, int64_t max_pages, int64_t span) {
   static const int kShort[5] = {0, 750, 1000, 1300, 1400}, kLong[3] = {0, 1000, 1400}, kLong16[3] = {0, 1500, 2300};
   Kv8Plan p{};
@@ -48,7 +48,7 @@ static Kv8Plan attn_plan(const Kv8Shape& h, int64_t batch, int64_t queries, int6
     const int per_sm = kv8_ctas(brief);
     for (int64_t n = 1; n <= std::min<int64_t>(steps, 128); ++n) {
       const int64_t all = ctas * n, waves = all / (per_sm * sms), rest = all - waves * per_sm * sms;
-      const bool memory = n > kKvCluster || (n > 1 && all > 2 * sms);
+      const bool memory = n > kKvCluster || (n != 1 && n != 2 && n != 4 && all > 2 * sms);
       const int64_t time = ((steps + n - 1) / n + 3) * (waves * ns[per_sm] + ns[(rest + sms - 1) / sms]) + (memory ? 4000 : n > 1 ? 2000 : 0);
       if (best < 0 || time < best) {
         best = time;
