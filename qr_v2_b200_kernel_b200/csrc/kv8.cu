@@ -4,6 +4,7 @@
 #include "launch.h"
 #include "kv8.cuh"
 #include "kv8_attention.cuh"
+#include "kv8_prompt.cuh"
 
 namespace qrb200 {
 
@@ -21,9 +22,12 @@ static cudaError_t with_shape(int dtype, int dim, F&& f) {
   return dim == 64 ? f(__half{}, Int<64>{}) : f(__half{}, Int<128>{});
 }
 
+constexpr int kPromptFrom = 64;  // query rows of a key head from which on kv8_prompt_kernel takes them
+
 // How an attention call is cut: query rows per tile, steps of 4 or 8 KB, and the token range over `splits` CTAs.
 struct Kv8Plan {
   int tile_rows, tiles, splits;
+  bool prompt;  // tiles of 256 rows on the tensor cores, not split; else
   bool brief;   // short steps
   bool memory;  // parts go through memory
   size_t bytes;  // workspace: the parts and their (maximum, sum) pairs
@@ -38,8 +42,11 @@ static Kv8Plan attn_plan(const Kv8Shape& h, int64_t batch, int64_t queries, int6
   static const int kShort[5] = {0, 750, 1000, 1300, 1400}, kLong[3] = {0, 1000, 1400}, kLong16[3] = {0, 1500, 2300};
   Kv8Plan p{};
   const int64_t rows = queries * (q_heads / h.heads);
-  p.tile_rows = rows <= 8 ? 8 : 16;
+  p.prompt = rows >= kPromptFrom;
+  p.tile_rows = p.prompt ? kPromptRows : rows <= 8 ? 8 : 16;
   p.tiles = ceil_div(rows, p.tile_rows);
+  p.splits = 1;
+  if (p.prompt) return p;
   const int64_t ctas = batch * h.heads * p.tiles, tokens = std::min(max_pages * h.page, span), sms = sm_count();
   int64_t best = -1;
   for (int brief = 0; brief <= (p.tile_rows == 8 ? 1 : 0); ++brief) {
@@ -75,6 +82,20 @@ static cudaError_t launch_attention(const Kv8AttnParams& p, const Kv8Plan& plan,
   qrb200_internal_count_launch();
   LaunchShape j(dim3(p.batch * p.queries * p.q_heads), 32 * kKvJoinWarps, 0, s);
   return cudaLaunchKernelEx(&j.cfg, kv_join_kernel<T, kDim, Kv8AttnParams>, p, plan.tile_rows);
+}
+
+template <typename T, int kDim>
+static cudaError_t launch_prompt(const Kv8AttnParams& p, cudaStream_t s) {
+  constexpr int kSmem = prompt_smem_bytes(kDim);
+  static OncePerDevice once;
+  const cudaError_t e = once.run([] {
+    return cudaFuncSetAttribute(kv8_prompt_kernel<T, kDim>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+  });
+  if (e != cudaSuccess) return e;
+  const int64_t ctas = (int64_t)p.tiles * p.sh.heads * p.batch;
+  if (ctas > kMaxRows) return cudaErrorInvalidValue;
+  LaunchShape l(dim3((unsigned)ctas), kPromptThreads, kSmem, s);
+  return cudaLaunchKernelEx(&l.cfg, kv8_prompt_kernel<T, kDim>, p);
 }
 
 }  // namespace qrb200
@@ -214,6 +235,7 @@ int qrb200_kv8_attention(const void* q, const int64_t* q_strides, const void* co
     if (p.part_ml) part.part_o += parts * h.dim, part.part_ml += parts;
     const cudaError_t e = with_shape(shape->dtype, h.dim, [&](auto type, auto dim) {
       using E = decltype(type);
+      if (plan.prompt) return launch_prompt<E, dim()>(part, s);
       if (plan.tile_rows == 16) return launch_attention<E, dim(), 2, false>(part, plan, s);
       return plan.brief ? launch_attention<E, dim(), 1, true>(part, plan, s) : launch_attention<E, dim(), 1, false>(part, plan, s);
     });

@@ -1,0 +1,455 @@
+// Attention of many queries (prompts, chunks of them) over the 8-bit cache (layout and formulas: kv8.cuh).
+//
+// Up to 256 query rows that share a key head to a CTA, as two tiles of 128 that take turns on the tensor cores: while
+// one tile's scores become weights, the other's products run. In steps of 128 tokens:
+//   S = Q K^T (fp16 x fp16, Q brought by a power of two to the top of fp16's range, K's codes exact),
+//   P = 2^(S r - reference) w,  O += P V  (V's codes exact; r and w the steps of the tokens' pages),
+// S, P and O in tensor memory (P takes S's place), the softmax of a row in one thread.
+//
+// Warps 0-3 and 4-7: the softmax of the first and the second tile. Warps 8-11: keys and values from bytes to
+// fp16 operands, through registers (16-bit numbers are twice the traffic, and what the cache saves); both land K-major in the
+// 128-byte swizzle, values transposed, which is how their bytes lie. Warp 12: the MMAs.
+//
+// P is one fp16 number for bf16 results (its error, 2^-12 of a weight, is a sixteenth of what the result's rounding
+// leaves) and two, high and low, for fp16 ones. It is scaled by a power of two that puts the largest step of the
+// values at 2^11, so weights keep their leading bits down to 2^-25 of the largest.
+#pragma once
+
+#include "codes.cuh"
+#include "kv8_attention.cuh"
+
+namespace qrb200 {
+
+constexpr int kPromptRows = 256, kPromptTokens = 128;
+constexpr int kPromptThreads = 32 * 16;  // (three warps idle: registers are dealt out by fours of warps)
+constexpr int kPromptStepExp = 11;
+__host__ __device__ constexpr int prompt_tile(int dim) { return 128 * dim * 2; }  // bytes of 128 rows of fp16
+__host__ __device__ constexpr int prompt_smem_bytes(int dim) { return 1024 + 2 * prompt_tile(dim) + 4 * prompt_tile(dim); }
+
+// kind::f16: fp16 operands, both K-major, 32-bit accumulator.
+__host__ __device__ constexpr uint32_t f16_idesc(int M, int N) { return (1u << 4) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24); }
+__device__ __forceinline__ void f16_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n"
+      :
+      : "r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate ? 1u : 0u)
+      : "memory");
+}
+__device__ __forceinline__ void f16_mma_tmem(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool accumulate) {  // A in tensor memory
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n"
+      :
+      : "r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate ? 1u : 0u)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_put16(uint32_t taddr, const uint32_t (&v)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
+      :
+      : "r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+        "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_put_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// Columns of S (rows of K in shared memory) in their order. Of 64 tokens, four runs of 16, column c holds token
+// prompt_token(c): the order that the values' bytes give a lane sixteen neighbours in.
+__host__ __device__ constexpr int prompt_run(int c) { return c >> 2 & 3; }
+__host__ __device__ constexpr int prompt_token(int c) { return 16 * prompt_run(c) + 2 * (c >> 4) + (c & 1) + 8 * (c >> 1 & 1); }
+// A row's 16-byte piece in the 128-byte swizzle.
+__device__ __forceinline__ uint32_t swizzled(int row, int piece) { return row * 128 + ((piece ^ (row & 7)) << 4); }
+
+template <typename T, int kDim>
+__global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(Kv8AttnParams P) {
+  constexpr int kTile = prompt_tile(kDim), kAtoms = kDim / 64;
+  constexpr bool kPrecise = std::is_same<T, __half>::value;  // weights in two halves
+  constexpr float kNone = -INFINITY;
+  extern __shared__ __align__(1024) unsigned char smem_raw[];
+  __shared__ uint64_t kv_full[2], kv_empty[2], s_full[2], p_full[2], o_full;
+  __shared__ uint32_t s_tmem;
+  __shared__ float s_key[2][8], s_value[2][8];  // steps of a stage's runs; values' scaled
+  __shared__ int s_power[2][8];                 // the keys' step's power of two (s_key holds its significand)
+  __shared__ unsigned s_most[16];
+  __shared__ volatile int s_bad;  // a wait ran out: keep to the barriers, write nothing
+  unsigned char* sq = align1024(smem_raw);
+  unsigned char* sk = sq + 2 * kTile;  // two stages of [keys][values]
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int units = P.batch * P.sh.heads;
+  // The last queries, which see most, first.
+  const int tile = P.tiles - 1 - (int)(blockIdx.x / units), unit = blockIdx.x % units, head = unit % P.sh.heads, b = unit / P.sh.heads;
+  const int rows = P.queries * P.share, row0 = tile * kPromptRows;
+  const int both = row0 + 128 < rows ? 2 : 1;  // tiles with rows
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&kv_full[i], 4);
+      mbar_init(&kv_empty[i], 1);
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_full[i], 4);
+    }
+    mbar_init(&o_full, 1);
+    s_bad = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    fence_async_smem();
+  }
+  griddep_launch_wait();  // before TMEM is taken: a kernel still running may need it
+  if (warp == 12) tmem_alloc(&s_tmem, 512);
+  int len = P.lengths[b];
+  if (len < 0 || len > (long long)P.max_pages * P.sh.page || (len > 0 && P.sh.pages == 0)) {
+    if (threadIdx.x == 0) report_device_failure(kSiteIndex);
+    len = 0;
+  }
+  // Tokens [lo, hi) that a row sees, and those of the CTA's rows together.
+  const auto range_of = [&](int row, int& lo, int& hi) {
+    const int pos = len - P.queries + row / P.share;
+    hi = P.causal ? max(0, pos + 1) : len;
+    lo = P.window > 0 ? max(0, pos - P.window + 1) : 0;
+    if (lo > hi) lo = hi;
+  };
+  int all_lo, all_hi, last_lo, last_hi;
+  range_of(row0, all_lo, all_hi);
+  const int last = min(rows, row0 + kPromptRows) - 1;
+  range_of(last, last_lo, last_hi);
+  // Positions grow with the row, and so do both ends; rows before the sequence's start see nothing.
+  if (all_hi <= all_lo) {
+    const int first = P.queries - len;  // the first query at a position
+    all_lo = last_lo;
+    if (first >= 0 && last >= first * P.share) {
+      int hi;
+      range_of(max(row0, first * P.share), all_lo, hi);
+    }
+  }
+  all_hi = last_hi;
+  const int block0 = all_lo / kPromptTokens, count = all_hi > all_lo ? (all_hi + kPromptTokens - 1) / kPromptTokens - block0 : 0;
+  const int first_run = all_lo / 16, last_run = (all_hi + 15) / 16;
+  // A run's page, -1 outside the range or where the table is wrong.
+  const auto page_of = [&](int run) {
+    if (run < first_run || run >= last_run) return -1;
+    const int page = __ldg(P.table + b * P.table_stride + (run >> (P.sh.shift - 4)));
+    if (page < 0 || page >= P.sh.pages) {
+      report_device_failure(kSiteIndex);
+      return -1;
+    }
+    return page;
+  };
+  const float2* steps = reinterpret_cast<const float2*>(P.range);
+
+  // The largest value step of the pages that are seen.
+  unsigned most = 0;
+  const int page_runs = P.sh.page / 16;
+  for (int page = first_run / page_runs + threadIdx.x; page * page_runs < last_run; page += kPromptThreads) {
+    const int at = page_of(max(first_run, page * page_runs));
+    if (at >= 0) {
+      const float w = kv8_step(__ldg(steps + (long long)at * P.sh.heads + head).y);
+      if (w == w) most = max(most, __float_as_uint(w));  // (not NaN)
+    }
+  }
+  most = __reduce_max_sync(kFullMask, most);
+  if (lane == 0) s_most[warp] = most;
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  most = __reduce_max_sync(kFullMask, s_most[lane & 15]);
+  const int cap = max(-100, min(126, (int)(most >> 23) - 126));  // 2^cap is above it
+  const float scaled = __int_as_float((kPromptStepExp - cap + 127) << 23), lower = __int_as_float((cap - kPromptStepExp + 127) << 23);
+  const uint32_t tmem = s_tmem;
+
+  if (warp < 8) {
+    // ---- the softmax of a tile, a row to a thread ----
+    const int mine = warp >> 2, in_tile = threadIdx.x & 127, row = row0 + 128 * mine + in_tile;
+    const bool real = row < rows;
+    const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16), s_at = lanes + 128 * mine, o_at = lanes + 256 + 128 * mine;
+    int lo = 0, hi = 0, back = 0;
+    if (real) range_of(row, lo, hi);
+    {
+      // The row's query, permuted as the keys' bytes are: piece k of 64 channels holds channels 16 w + 4 t + e with t =
+      // k / 2 and w = 2 (k & 1), 2 (k & 1) + 1.
+      const T* q = static_cast<const T*>(P.q) + b * P.q_bs + (long long)(row / P.share) * P.q_ts + (head * P.share + row % P.share) * P.q_hs;
+      const auto four = [&](T(&x)[4], int c) {
+        if (!real) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[e] = from_f32<T>(0.f);
+        } else if (P.q_wide) {
+          *reinterpret_cast<uint2*>(x) = __ldg(reinterpret_cast<const uint2*>(q + c));
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[e] = q[c + e];
+        }
+      };
+      unsigned top = 0;
+#pragma unroll 8
+      for (int c = 0; c < kDim; c += 4) {
+        alignas(8) T x[4];
+        four(x, c);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) top = max(top, __float_as_uint(to_f32(x[e])) & 0x7fffffffu);
+      }
+      const int power = max(1, min(254, (int)(top >> 23))) - 127, lift = kKv8Top - power;
+      const float up = kv_power(lift / 2), more = kv_power(lift - lift / 2);
+      back = power - kKv8Top + P.scale_power;
+#pragma unroll 1
+      for (int a = 0; a < kAtoms; ++a)
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          alignas(16) __half y[8];
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            alignas(8) T x[4];
+            four(x, 64 * a + 16 * (2 * (k & 1) + i) + 4 * (k >> 1));
+            put2(y + 4 * i, to_f32(x[0]) * up * more, to_f32(x[1]) * up * more);
+            put2(y + 4 * i + 2, to_f32(x[2]) * up * more, to_f32(x[3]) * up * more);
+          }
+          *reinterpret_cast<uint4*>(sq + mine * kTile + a * (128 * 128) + swizzled(in_tile, k)) = *reinterpret_cast<const uint4*>(y);
+        }
+    }
+    fence_async_smem();
+    named_sync(1, 288);  // with the MMAs' warp: both tiles' queries are there
+    if (mine < both) {
+      // What every row of the warp sees.
+      const int in_lo = __reduce_max_sync(kFullMask, lo), in_hi = __reduce_min_sync(kFullMask, real ? hi : 0x7fffffff);
+      float ref = kNone, sum = 0.f;  // weights are 2^(score - ref)
+      for (int j = 0; j < count; ++j) {
+        const int st = j & 1, tok0 = (block0 + j) * kPromptTokens;
+        if (!s_bad && !__all_sync(kFullMask, mbar_wait_quick(&s_full[mine], j & 1))) s_bad = 1;
+        tc_fence_after();
+        float f[8], v[2][16];
+#pragma unroll
+        for (int r = 0; r < 8; ++r) f[r] = s_key[st][r] * kv_power(s_power[st][r] + back);
+        const bool full = tok0 >= in_lo && tok0 + kPromptTokens <= in_hi;
+        // The largest score. (Factors are not negative, so a run's largest product gives its largest score.)
+        float top = kNone;
+        tmem_ask16(s_at, v[0]);
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+          tmem_arrived(v[c & 1]);
+          if (c < 7) tmem_ask16(s_at + 16 * (c + 1), v[(c + 1) & 1]);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            float m = kNone;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int at = tok0 + 64 * (c >> 2) + prompt_token(16 * (c & 3) + 4 * r + i);
+              const float x = v[c & 1][4 * r + i];
+              m = full || (at >= lo && at < hi) ? fmaxf(m, x) : m;
+            }
+            top = m > kNone ? fmaxf(top, m * f[4 * (c >> 2) + r]) : top;
+          }
+        }
+        const bool move = top > __fadd_rd(ref, kKvLazy) || (ref == kNone && top > kNone);
+        if (__any_sync(kFullMask, move)) {
+          const float next = fmaxf(ref, top), keep = ref == kNone ? 0.f : kv_exp2(ref - next);
+          if (j > 0) {  // (the products before these scores' are over)
+#pragma unroll 1
+            for (int c = 0; c < kDim; c += 16) {
+              float o[16];
+              tmem_ask16(o_at + c, o);
+              tmem_arrived(o);
+              uint32_t w[16];
+#pragma unroll
+              for (int i = 0; i < 16; ++i) w[i] = __float_as_uint(ref == kNone ? 0.f : o[i] * keep);
+              tmem_put16(o_at + c, w);
+            }
+            tmem_put_wait();
+          }
+          sum *= keep;
+          ref = next;
+        }
+        const float less = ref == kNone ? 0.f : -ref;
+        const float2 less2 = make_float2(less, less);
+        float2 sums = make_float2(0.f, 0.f);
+        tmem_ask16(s_at, v[0]);
+#pragma unroll
+        for (int c = 0; c < 8; c += 2) {
+          uint32_t high[16], low[16];
+#pragma unroll
+          for (int d = 0; d < 2; ++d) {
+            tmem_arrived(v[d]);
+            if (c + d < 7) tmem_ask16(s_at + 16 * (c + d + 1), v[d ^ 1]);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              const int run = 4 * (c >> 2) + r;
+              const float2 f2 = make_float2(f[run], f[run]), w2 = make_float2(s_value[st][run], s_value[st][run]);
+#pragma unroll
+              for (int i = 0; i < 4; i += 2) {
+                float2 x = __ffma2_rn(make_float2(v[d][4 * r + i], v[d][4 * r + i + 1]), f2, less2);
+                const int at = tok0 + 64 * (c >> 2) + prompt_token(16 * ((c + d) & 3) + 4 * r + i);  // and the next
+                const bool one = full || (at >= lo && at < hi), two = full || (at + 1 >= lo && at + 1 < hi);
+                float2 p = make_float2(one ? kv_exp2(x.x) : 0.f, two ? kv_exp2(x.y) : 0.f);
+                sums = __fadd2_rn(sums, p);
+                p = __fmul2_rn(p, w2);
+                if (!full) {  // what a row does not see may be NaN
+                  if (!one) p.x = 0.f;
+                  if (!two) p.y = 0.f;
+                }
+                high[8 * d + 2 * r + i / 2] = kv_pack(p);
+                if constexpr (kPrecise) {
+                  const float2 back2 = __half22float2(__hneg2(reinterpret_cast<const __half2&>(high[8 * d + 2 * r + i / 2])));
+                  low[8 * d + 2 * r + i / 2] = kv_pack(__fadd2_rn(p, back2));
+                }
+              }
+            }
+          }
+          // These 32 columns of S have been read; the next sixteen, asked for, are not among them.
+          tmem_put16(s_at + 16 * c, high);
+          if constexpr (kPrecise) tmem_put16(s_at + 16 * c + 16, low);
+        }
+        sum += sums.x + sums.y;
+        tmem_put_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[mine]);
+      }
+      if (count > 0) {
+        if (!s_bad && !__all_sync(kFullMask, mbar_wait_quick(&o_full, 0))) s_bad = 1;
+        tc_fence_after();
+      }
+      const float inv = sum == 0.f ? 0.f : lower / sum;  // nothing seen: zeros
+      T* out = static_cast<T*>(P.out) + (((long long)b * P.queries + row / P.share) * P.q_heads + head * P.share + row % P.share) * kDim;
+#pragma unroll 1
+      for (int c = 0; c < kDim; c += 16) {
+        float o[16] = {};
+        if (count > 0) {
+          tmem_ask16(o_at + c, o);
+          tmem_arrived(o);
+        }
+        alignas(16) T y[16];
+#pragma unroll
+        for (int i = 0; i < 16; i += 2) put2(y + i, sum == 0.f ? 0.f : o[i] * inv, sum == 0.f ? 0.f : o[i + 1] * inv);
+        if (real && !s_bad) {
+          *reinterpret_cast<uint4*>(out + c) = *reinterpret_cast<const uint4*>(y);
+          *reinterpret_cast<uint4*>(out + c + 8) = *reinterpret_cast<const uint4*>(y + 8);
+        }
+      }
+    }
+  } else if (warp < 12) {
+    // ---- keys and values to operands ----
+    const int cw = warp - 8, g = lane >> 2, t = lane & 3;
+    for (int j = 0; j < count; ++j) {
+      const int st = j & 1, run0 = (block0 + j) * 8;
+      unsigned char* keys = sk + st * 2 * kTile;
+      unsigned char* values = keys + kTile;
+      // Lane r's page is run r's.
+      const int page = page_of(run0 + (lane & 7));
+      const unsigned char* base[8];
+#pragma unroll
+      for (int r = 0; r < 8; ++r) {
+        const int pg = __shfl_sync(kFullMask, page, r);
+        base[r] = pg < 0 ? nullptr : P.codes + ((long long)pg * P.sh.heads + head) * P.sh.block_bytes() + ((run0 + r) & (page_runs - 1)) * (32 * kDim) + lane * 16;
+      }
+      const auto get = [&](int r, int at) {
+        return base[r] ? __ldg(reinterpret_cast<const uint4*>(base[r] + at)) : make_uint4(kKv8Zeros, kKv8Zeros, kKv8Zeros, kKv8Zeros);
+      };
+      // A warp takes two runs of keys, and values of half the 64-token pieces' channels.
+      uint4 kc[2][2][kAtoms];
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int a = 0; a < kAtoms; ++a) kc[i][h][a] = get(2 * cw + i, h * (8 * kDim) + a * 512);
+      if (j >= 2 && !s_bad && !__all_sync(kFullMask, mbar_wait_quick(&kv_empty[st], ((j >> 1) - 1) & 1))) s_bad = 1;
+      if (cw == 0 && lane < 8) {
+        float2 step = make_float2(0.f, 0.f);
+        if (page >= 0) step = __ldg(steps + (long long)page * P.sh.heads + head);
+        step.x = kv8_step(step.x), step.y = kv8_step(step.y);
+        s_key[st][lane] = step.x > 0.f ? kv8_part(step.x) * P.scale_part : step.x;  // 0 and NaN as they are
+        s_power[st][lane] = kv8_power(step.x);
+        s_value[st][lane] = step.y * scaled;
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int run = 2 * cw + i, row = 64 * (run >> 2) + 16 * (g >> 1) + 4 * (run & 3) + 2 * h + (g & 1);
+#pragma unroll
+          for (int a = 0; a < kAtoms; ++a) {
+            const uint4 w = kc[i][h][a];
+            unsigned char* to = keys + a * (128 * 128);
+            *reinterpret_cast<uint4*>(to + swizzled(row, 2 * t)) =
+                make_uint4(kv8_codes<0>(w.x), kv8_codes<1>(w.x), kv8_codes<0>(w.y), kv8_codes<1>(w.y));
+            *reinterpret_cast<uint4*>(to + swizzled(row, 2 * t + 1)) =
+                make_uint4(kv8_codes<0>(w.z), kv8_codes<1>(w.z), kv8_codes<0>(w.w), kv8_codes<1>(w.w));
+          }
+        }
+      // Values: 32 channels of 64 tokens at a time.
+#pragma unroll
+      for (int i = 0; i < kDim / 64; ++i) {
+        const int part = cw * (kDim / 64) + i, atom = part / (kDim / 32), piece = part % (kDim / 32);
+        uint4 vc[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) vc[r] = atom ? get(4 + r, 16 * kDim + piece * 512) : get(r, 16 * kDim + piece * 512);
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const int row = 32 * piece + 8 * w + g;
+          uint32_t x[4];
+#pragma unroll
+          for (int r = 0; r < 4; ++r) x[r] = reinterpret_cast<const uint32_t*>(&vc[r])[w];
+          unsigned char* to = values + atom * (kDim * 128);
+          *reinterpret_cast<uint4*>(to + swizzled(row, 2 * t)) =
+              make_uint4(kv8_codes<0>(x[0]), kv8_codes<1>(x[0]), kv8_codes<0>(x[1]), kv8_codes<1>(x[1]));
+          *reinterpret_cast<uint4*>(to + swizzled(row, 2 * t + 1)) =
+              make_uint4(kv8_codes<0>(x[2]), kv8_codes<1>(x[2]), kv8_codes<0>(x[3]), kv8_codes<1>(x[3]));
+        }
+      }
+      fence_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&kv_full[st]);
+    }
+  } else if (warp == 12) {
+    // ---- the MMAs ----
+    constexpr uint32_t to_s = f16_idesc(128, kPromptTokens), to_o = f16_idesc(128, kDim);
+    const uint64_t q0 = i8_sdesc(smem_u32(sq)), k0 = i8_sdesc(smem_u32(sk));
+    named_sync(1, 288);
+    const auto scores = [&](int x, int j) {
+      if (elect_one()) {
+#pragma unroll
+        for (int c = 0; c < kDim / 16; ++c)
+          f16_mma(tmem + 128 * x, q0 + ((x * kTile + (c >> 2) * (128 * 128)) >> 4) + 2 * (c & 3),
+                  k0 + (((j & 1) * 2 * kTile + (c >> 2) * (128 * 128)) >> 4) + 2 * (c & 3), to_s, c > 0);
+        mma_commit(&s_full[x]);
+      }
+      __syncwarp();
+    };
+    bool ok = true;
+    if (count > 0) {
+      ok = mbar_wait_quick(&kv_full[0], 0);
+      tc_fence_after();
+      if (ok)
+        for (int x = 0; x < both; ++x) scores(x, 0);
+    }
+    for (int j = 0; ok && j < count; ++j) {
+      const int st = j & 1;
+      if (j + 1 < count) ok = mbar_wait_quick(&kv_full[st ^ 1], ((j + 1) >> 1) & 1);
+      for (int x = 0; ok && x < both; ++x) {
+        ok = mbar_wait_quick(&p_full[x], j & 1);
+        if (!ok) break;
+        tc_fence_after();
+        if (elect_one()) {
+          const uint64_t v0 = k0 + ((st * 2 * kTile + kTile) >> 4);
+#pragma unroll
+          for (int c = 0; c < kPromptTokens / 16; ++c) {
+            const uint64_t v = v0 + ((c >> 2) * (kDim * 128) >> 4) + 2 * (c & 3);
+            const uint32_t p = tmem + 128 * x + 32 * (c >> 1) + 8 * (c & 1);
+            f16_mma_tmem(tmem + 256 + 128 * x, p, v, to_o, j > 0 || c > 0);
+            if constexpr (kPrecise) f16_mma_tmem(tmem + 256 + 128 * x, p + 16, v, to_o, true);
+          }
+          if (x == both - 1) mma_commit(&kv_empty[st]);
+          if (x == both - 1 && j == count - 1) mma_commit(&o_full);
+        }
+        __syncwarp();
+        if (j + 1 < count) scores(x, j + 1);
+      }
+    }
+    if (!ok) s_bad = 1;
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 12) tmem_dealloc(tmem, 512);
+}
+
+}  // namespace qrb200
