@@ -221,24 +221,29 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(Kv8AttnPa
         for (int r = 0; r < 8; ++r) f[r] = s_key[st][r] * kv_power(s_power[st][r] + back);
         const bool full = tok0 >= in_lo && tok0 + kPromptTokens <= in_hi;
         // The largest score. (Factors are not negative, so a run's largest product gives its largest score.)
-        float top = kNone;
-        tmem_ask16(s_at, v[0]);
+        const auto largest = [&](auto all) {
+          constexpr bool kAll = decltype(all)::value;
+          float top = kNone, m[4];
+          tmem_ask16(s_at, v[0]);
 #pragma unroll
-        for (int c = 0; c < 8; ++c) {
-          tmem_arrived(v[c & 1]);
-          if (c < 7) tmem_ask16(s_at + 16 * (c + 1), v[(c + 1) & 1]);
+          for (int c = 0; c < 8; ++c) {
+            tmem_arrived(v[c & 1]);
+            if (c < 7) tmem_ask16(s_at + 16 * (c + 1), v[(c + 1) & 1]);
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            float m = kNone;
+            for (int r = 0; r < 4; ++r) {
+              if ((c & 3) == 0) m[r] = kNone;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const int at = tok0 + 64 * (c >> 2) + prompt_token(16 * (c & 3) + 4 * r + i);
-              const float x = v[c & 1][4 * r + i];
-              m = full || (at >= lo && at < hi) ? fmaxf(m, x) : m;
+              for (int i = 0; i < 4; ++i) {
+                const int at = tok0 + 64 * (c >> 2) + prompt_token(16 * (c & 3) + 4 * r + i);
+                const float x = v[c & 1][4 * r + i];
+                m[r] = kAll || (at >= lo && at < hi) ? fmaxf(m[r], x) : m[r];
+              }
+              if ((c & 3) == 3) top = kAll || m[r] > kNone ? fmaxf(top, m[r] * f[4 * (c >> 2) + r]) : top;
             }
-            top = m > kNone ? fmaxf(top, m * f[4 * (c >> 2) + r]) : top;
           }
-        }
+          return top;
+        };
+        const float top = full ? largest(std::true_type{}) : largest(std::false_type{});
         const bool move = top > __fadd_rd(ref, kKvLazy) || (ref == kNone && top > kNone);
         if (__any_sync(kFullMask, move)) {
           const float next = fmaxf(ref, top), keep = ref == kNone ? 0.f : kv_exp2(ref - next);
@@ -261,42 +266,47 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(Kv8AttnPa
         const float less = ref == kNone ? 0.f : -ref;
         const float2 less2 = make_float2(less, less);
         float2 sums = make_float2(0.f, 0.f);
-        tmem_ask16(s_at, v[0]);
+        const auto weights = [&](auto all) {
+          constexpr bool kAll = decltype(all)::value;
+          tmem_ask16(s_at, v[0]);
 #pragma unroll
-        for (int c = 0; c < 8; c += 2) {
-          uint32_t high[16], low[16];
+          for (int c = 0; c < 8; c += 2) {
+            uint32_t high[16], low[16];
 #pragma unroll
-          for (int d = 0; d < 2; ++d) {
-            tmem_arrived(v[d]);
-            if (c + d < 7) tmem_ask16(s_at + 16 * (c + d + 1), v[d ^ 1]);
+            for (int d = 0; d < 2; ++d) {
+              tmem_arrived(v[d]);
+              if (c + d < 7) tmem_ask16(s_at + 16 * (c + d + 1), v[d ^ 1]);
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              const int run = 4 * (c >> 2) + r;
-              const float2 f2 = make_float2(f[run], f[run]), w2 = make_float2(s_value[st][run], s_value[st][run]);
+              for (int r = 0; r < 4; ++r) {
+                const int run = 4 * (c >> 2) + r;
+                const float2 f2 = make_float2(f[run], f[run]), w2 = make_float2(s_value[st][run], s_value[st][run]);
 #pragma unroll
-              for (int i = 0; i < 4; i += 2) {
-                float2 x = __ffma2_rn(make_float2(v[d][4 * r + i], v[d][4 * r + i + 1]), f2, less2);
-                const int at = tok0 + 64 * (c >> 2) + prompt_token(16 * ((c + d) & 3) + 4 * r + i);  // and the next
-                const bool one = full || (at >= lo && at < hi), two = full || (at + 1 >= lo && at + 1 < hi);
-                float2 p = make_float2(one ? kv_exp2(x.x) : 0.f, two ? kv_exp2(x.y) : 0.f);
-                sums = __fadd2_rn(sums, p);
-                p = __fmul2_rn(p, w2);
-                if (!full) {  // what a row does not see may be NaN
-                  if (!one) p.x = 0.f;
-                  if (!two) p.y = 0.f;
-                }
-                high[8 * d + 2 * r + i / 2] = kv_pack(p);
-                if constexpr (kPrecise) {
-                  const float2 back2 = __half22float2(__hneg2(reinterpret_cast<const __half2&>(high[8 * d + 2 * r + i / 2])));
-                  low[8 * d + 2 * r + i / 2] = kv_pack(__fadd2_rn(p, back2));
+                for (int i = 0; i < 4; i += 2) {
+                  float2 x = __ffma2_rn(make_float2(v[d][4 * r + i], v[d][4 * r + i + 1]), f2, less2);
+                  const int at = tok0 + 64 * (c >> 2) + prompt_token(16 * ((c + d) & 3) + 4 * r + i);  // and the next
+                  const bool one = kAll || (at >= lo && at < hi), two = kAll || (at + 1 >= lo && at + 1 < hi);
+                  float2 p = make_float2(one ? kv_exp2(x.x) : 0.f, two ? kv_exp2(x.y) : 0.f);
+                  sums = __fadd2_rn(sums, p);
+                  p = __fmul2_rn(p, w2);
+                  if constexpr (!kAll) {  // what a row does not see may be NaN
+                    if (!one) p.x = 0.f;
+                    if (!two) p.y = 0.f;
+                  }
+                  high[8 * d + 2 * r + i / 2] = kv_pack(p);
+                  if constexpr (kPrecise) {
+                    const float2 back2 = __half22float2(__hneg2(reinterpret_cast<const __half2&>(high[8 * d + 2 * r + i / 2])));
+                    low[8 * d + 2 * r + i / 2] = kv_pack(__fadd2_rn(p, back2));
+                  }
                 }
               }
             }
+            // These 32 columns of S have been read; the next sixteen, asked for, are not among them.
+            tmem_put16(s_at + 16 * c, high);
+            if constexpr (kPrecise) tmem_put16(s_at + 16 * c + 16, low);
           }
-          // These 32 columns of S have been read; the next sixteen, asked for, are not among them.
-          tmem_put16(s_at + 16 * c, high);
-          if constexpr (kPrecise) tmem_put16(s_at + 16 * c + 16, low);
-        }
+        };
+        if (full) weights(std::true_type{});
+        else weights(std::false_type{});
         sum += sums.x + sums.y;
         tmem_put_wait();
         tc_fence_before();
@@ -332,25 +342,33 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(Kv8AttnPa
       const int st = j & 1, run0 = (block0 + j) * 8;
       unsigned char* keys = sk + st * 2 * kTile;
       unsigned char* values = keys + kTile;
-      // Lane r's page is run r's.
+      // Lane r's page is run r's; where a run's bytes of this lane lie, or null.
       const int page = page_of(run0 + (lane & 7));
-      const unsigned char* base[8];
-#pragma unroll
-      for (int r = 0; r < 8; ++r) {
+      const auto base = [&](int r) -> const unsigned char* {
         const int pg = __shfl_sync(kFullMask, page, r);
-        base[r] = pg < 0 ? nullptr : P.codes + ((long long)pg * P.sh.heads + head) * P.sh.block_bytes() + ((run0 + r) & (page_runs - 1)) * (32 * kDim) + lane * 16;
-      }
-      const auto get = [&](int r, int at) {
-        return base[r] ? __ldg(reinterpret_cast<const uint4*>(base[r] + at)) : make_uint4(kKv8Zeros, kKv8Zeros, kKv8Zeros, kKv8Zeros);
+        if (pg < 0) return nullptr;
+        return P.codes + ((long long)pg * P.sh.heads + head) * P.sh.block_bytes() + ((run0 + r) & (page_runs - 1)) * (32 * kDim) + lane * 16;
+      };
+      const auto get = [&](const unsigned char* from, int at) {
+        return from ? __ldg(reinterpret_cast<const uint4*>(from + at)) : make_uint4(kKv8Zeros, kKv8Zeros, kKv8Zeros, kKv8Zeros);
       };
       // A warp takes two runs of keys, and values of half the 64-token pieces' channels.
       uint4 kc[2][2][kAtoms];
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
+      for (int i = 0; i < 2; ++i) {
+        const unsigned char* from = base(2 * cw + i);
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
-          for (int a = 0; a < kAtoms; ++a) kc[i][h][a] = get(2 * cw + i, h * (8 * kDim) + a * 512);
+          for (int a = 0; a < kAtoms; ++a) kc[i][h][a] = get(from, h * (8 * kDim) + a * 512);
+      }
+      uint4 vc[kDim / 64][4];  // 32 channels of 64 tokens at a time
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const unsigned char* from = base(4 * (cw / 2) + r);
+#pragma unroll
+        for (int i = 0; i < kDim / 64; ++i) vc[i][r] = get(from, 16 * kDim + ((cw & 1) * (kDim / 64) + i) * 512);
+      }
       if (j >= 2 && !s_bad && !__all_sync(kFullMask, mbar_wait_quick(&kv_empty[st], ((j >> 1) - 1) & 1))) s_bad = 1;
       if (cw == 0 && lane < 8) {
         float2 step = make_float2(0.f, 0.f);
@@ -375,19 +393,15 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(Kv8AttnPa
                 make_uint4(kv8_codes<0>(w.z), kv8_codes<1>(w.z), kv8_codes<0>(w.w), kv8_codes<1>(w.w));
           }
         }
-      // Values: 32 channels of 64 tokens at a time.
 #pragma unroll
       for (int i = 0; i < kDim / 64; ++i) {
-        const int part = cw * (kDim / 64) + i, atom = part / (kDim / 32), piece = part % (kDim / 32);
-        uint4 vc[4];
-#pragma unroll
-        for (int r = 0; r < 4; ++r) vc[r] = atom ? get(4 + r, 16 * kDim + piece * 512) : get(r, 16 * kDim + piece * 512);
+        const int atom = cw / 2, piece = (cw & 1) * (kDim / 64) + i;
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
           const int row = 32 * piece + 8 * w + g;
           uint32_t x[4];
 #pragma unroll
-          for (int r = 0; r < 4; ++r) x[r] = reinterpret_cast<const uint32_t*>(&vc[r])[w];
+          for (int r = 0; r < 4; ++r) x[r] = reinterpret_cast<const uint32_t*>(&vc[i][r])[w];
           unsigned char* to = values + atom * (kDim * 128);
           *reinterpret_cast<uint4*>(to + swizzled(row, 2 * t)) =
               make_uint4(kv8_codes<0>(x[0]), kv8_codes<1>(x[0]), kv8_codes<0>(x[1]), kv8_codes<1>(x[1]));
@@ -399,52 +413,54 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(Kv8AttnPa
       __syncwarp();
       if (lane == 0) mbar_arrive(&kv_full[st]);
     }
-  } else if (warp == 12) {
-    // ---- the MMAs ----
-    constexpr uint32_t to_s = f16_idesc(128, kPromptTokens), to_o = f16_idesc(128, kDim);
-    const uint64_t q0 = i8_sdesc(smem_u32(sq)), k0 = i8_sdesc(smem_u32(sk));
-    named_sync(1, 288);
-    const auto scores = [&](int x, int j) {
-      if (elect_one()) {
-#pragma unroll
-        for (int c = 0; c < kDim / 16; ++c)
-          f16_mma(tmem + 128 * x, q0 + ((x * kTile + (c >> 2) * (128 * 128)) >> 4) + 2 * (c & 3),
-                  k0 + (((j & 1) * 2 * kTile + (c >> 2) * (128 * 128)) >> 4) + 2 * (c & 3), to_s, c > 0);
-        mma_commit(&s_full[x]);
-      }
-      __syncwarp();
-    };
-    bool ok = true;
-    if (count > 0) {
-      ok = mbar_wait_quick(&kv_full[0], 0);
-      tc_fence_after();
-      if (ok)
-        for (int x = 0; x < both; ++x) scores(x, 0);
-    }
-    for (int j = 0; ok && j < count; ++j) {
-      const int st = j & 1;
-      if (j + 1 < count) ok = mbar_wait_quick(&kv_full[st ^ 1], ((j + 1) >> 1) & 1);
-      for (int x = 0; ok && x < both; ++x) {
-        ok = mbar_wait_quick(&p_full[x], j & 1);
-        if (!ok) break;
-        tc_fence_after();
+  } else {
+    // ---- the MMAs (warp 12) ----
+    if (warp == 12) {
+      constexpr uint32_t to_s = f16_idesc(128, kPromptTokens), to_o = f16_idesc(128, kDim);
+      const uint64_t q0 = i8_sdesc(smem_u32(sq)), k0 = i8_sdesc(smem_u32(sk));
+      named_sync(1, 288);
+      const auto scores = [&](int x, int j) {
         if (elect_one()) {
-          const uint64_t v0 = k0 + ((st * 2 * kTile + kTile) >> 4);
 #pragma unroll
-          for (int c = 0; c < kPromptTokens / 16; ++c) {
-            const uint64_t v = v0 + ((c >> 2) * (kDim * 128) >> 4) + 2 * (c & 3);
-            const uint32_t p = tmem + 128 * x + 32 * (c >> 1) + 8 * (c & 1);
-            f16_mma_tmem(tmem + 256 + 128 * x, p, v, to_o, j > 0 || c > 0);
-            if constexpr (kPrecise) f16_mma_tmem(tmem + 256 + 128 * x, p + 16, v, to_o, true);
-          }
-          if (x == both - 1) mma_commit(&kv_empty[st]);
-          if (x == both - 1 && j == count - 1) mma_commit(&o_full);
+          for (int c = 0; c < kDim / 16; ++c)
+            f16_mma(tmem + 128 * x, q0 + ((x * kTile + (c >> 2) * (128 * 128)) >> 4) + 2 * (c & 3),
+                    k0 + (((j & 1) * 2 * kTile + (c >> 2) * (128 * 128)) >> 4) + 2 * (c & 3), to_s, c > 0);
+          mma_commit(&s_full[x]);
         }
         __syncwarp();
-        if (j + 1 < count) scores(x, j + 1);
+      };
+      bool ok = true;
+      if (count > 0) {
+        ok = mbar_wait_quick(&kv_full[0], 0);
+        tc_fence_after();
+        if (ok)
+          for (int x = 0; x < both; ++x) scores(x, 0);
       }
+      for (int j = 0; ok && j < count; ++j) {
+        const int st = j & 1;
+        if (j + 1 < count) ok = mbar_wait_quick(&kv_full[st ^ 1], ((j + 1) >> 1) & 1);
+        for (int x = 0; ok && x < both; ++x) {
+          ok = mbar_wait_quick(&p_full[x], j & 1);
+          if (!ok) break;
+          tc_fence_after();
+          if (elect_one()) {
+            const uint64_t v0 = k0 + ((st * 2 * kTile + kTile) >> 4);
+#pragma unroll
+            for (int c = 0; c < kPromptTokens / 16; ++c) {
+              const uint64_t v = v0 + ((c >> 2) * (kDim * 128) >> 4) + 2 * (c & 3);
+              const uint32_t p = tmem + 128 * x + 32 * (c >> 1) + 8 * (c & 1);
+              f16_mma_tmem(tmem + 256 + 128 * x, p, v, to_o, j > 0 || c > 0);
+              if constexpr (kPrecise) f16_mma_tmem(tmem + 256 + 128 * x, p + 16, v, to_o, true);
+            }
+            if (x == both - 1) mma_commit(&kv_empty[st]);
+            if (x == both - 1 && j == count - 1) mma_commit(&o_full);
+          }
+          __syncwarp();
+          if (j + 1 < count) scores(x, j + 1);
+        }
+      }
+      if (!ok) s_bad = 1;
     }
-    if (!ok) s_bad = 1;
   }
   tc_fence_before();
   __syncthreads();
