@@ -1,10 +1,10 @@
 // Attention of many queries (prompts, chunks of them) over the 8-bit cache (layout and formulas: kv8.cuh).
 //
-// Up to 256 query rows that share a key head to a CTA, as two tiles of 128 that take turns on the tensor cores: while
-// one tile's scores become weights, the other's products run. In steps of 128 tokens:
+// Up to 256 query rows that share a key head to a CTA, as two tiles of 128. In steps of 64 tokens:
 //   S = Q K^T (fp16 x fp16, Q brought by a power of two to the top of fp16's range, K's codes exact),
 //   P = 2^(S r - reference) w,  O += P V  (V's codes exact; r and w the steps of the tokens' pages),
-// S, P and O in tensor memory (P takes S's place), the softmax of a row in one thread.
+// S, P and O in tensor memory (P takes S's place), the softmax of a row in one thread. Each tile has two S, so that
+// the scores of the next step are there when a softmax ends (one S of 128 tokens: 172 us for the chunk below).
 //
 // Warps 0-3 and 4-7: the softmax of the first and the second tile. Warps 8-11: keys and values from bytes to
 // fp16 operands, through registers (16-bit numbers are twice the traffic, and what the cache saves); both land K-major in the
@@ -20,30 +20,34 @@
 
 namespace qrb200 {
 
-constexpr int kPromptRows = 256, kPromptTokens = 128;
+constexpr int kPromptRows = 256, kPromptTokens = 64, kPromptStages = 4;
 constexpr int kPromptThreads = 32 * 16;  // (three warps idle: registers are dealt out by fours of warps)
 constexpr int kPromptStepExp = 11;
 __host__ __device__ constexpr int prompt_tile(int dim) { return 128 * dim * 2; }  // bytes of 128 rows of fp16
-__host__ __device__ constexpr int prompt_smem_bytes(int dim) { return 1024 + 2 * prompt_tile(dim) + 4 * prompt_tile(dim); }
+__host__ __device__ constexpr int prompt_smem_bytes(int dim) { return 1024 + (2 + kPromptStages) * prompt_tile(dim); }
 
 // kind::f16: fp16 operands, both K-major, 32-bit accumulator.
 __host__ __device__ constexpr uint32_t f16_idesc(int M, int N) { return (1u << 4) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24); }
-__device__ __forceinline__ void f16_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate) {
+// The operands' descriptors by their lower words, which hold the addresses; the upper word is the same for all.
+__device__ __forceinline__ void f16_mma(uint32_t d, uint32_t a, uint32_t b, uint32_t upper, uint32_t idesc, bool accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n"
+      "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\t"
+      "mov.b64 a, {%1, %3};\n\t"
+      "mov.b64 b, {%2, %3};\n\t"
+      "setp.ne.b32 p, %5, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %4, p;\n\t}\n"
       :
-      : "r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate ? 1u : 0u)
+      : "r"(d), "r"(a), "r"(b), "r"(upper), "r"(idesc), "r"(accumulate ? 1u : 0u)
       : "memory");
 }
-__device__ __forceinline__ void f16_mma_tmem(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool accumulate) {  // A in tensor memory
+__device__ __forceinline__ void f16_mma_tmem(uint32_t d, uint32_t a, uint32_t b, uint32_t upper, uint32_t idesc, bool accumulate) {  // A in tensor memory
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n"
+      "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\t"
+      "mov.b64 b, {%2, %3};\n\t"
+      "setp.ne.b32 p, %5, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n\t}\n"
       :
-      : "r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate ? 1u : 0u)
+      : "r"(d), "r"(a), "r"(b), "r"(upper), "r"(idesc), "r"(accumulate ? 1u : 0u)
       : "memory");
 }
 __device__ __forceinline__ void tmem_put16(uint32_t taddr, const uint32_t (&v)[16]) {
@@ -56,7 +60,7 @@ __device__ __forceinline__ void tmem_put16(uint32_t taddr, const uint32_t (&v)[1
 }
 __device__ __forceinline__ void tmem_put_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// Columns of S (rows of K in shared memory) in their order. Of 64 tokens, four runs of 16, column c holds token
+// Columns of S (rows of K in shared memory) in their order. Of a step's 64 tokens, four runs of 16, column c holds token
 // prompt_token(c): the order that the values' bytes give a lane sixteen neighbours in.
 __host__ __device__ constexpr int prompt_run(int c) { return c >> 2 & 3; }
 __host__ __device__ constexpr int prompt_token(int c) { return 16 * prompt_run(c) + 2 * (c >> 4) + (c & 1) + 8 * (c >> 1 & 1); }
@@ -69,14 +73,16 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(Kv8AttnPa
   constexpr bool kPrecise = std::is_same<T, __half>::value;  // weights in two halves
   constexpr float kNone = -INFINITY;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
-  __shared__ uint64_t kv_full[2], kv_empty[2], s_full[2], p_full[2], o_full;
+  __shared__ uint64_t kv_full[kPromptStages], kv_empty[kPromptStages], s_full[2][2], p_full[2][2], o_full[2][2];  // [tile][odd steps]
+  // (A softmax may be two steps ahead of the products with the values, and a barrier tells a phase only from the one before it:
+  // so each step waits for a barrier whose last phase but one is known to be over.)
   __shared__ uint32_t s_tmem;
-  __shared__ float s_key[2][8], s_value[2][8];  // steps of a stage's runs; values' scaled
-  __shared__ int s_power[2][8];                 // the keys' step's power of two (s_key holds its significand)
+  __shared__ float s_key[kPromptStages][4], s_value[kPromptStages][4];  // steps of a stage's runs; values' scaled
+  __shared__ int s_power[kPromptStages][4];  // the keys' step's power of two (s_key holds its significand)
   __shared__ unsigned s_most[16];
   __shared__ volatile int s_bad;  // a wait ran out: keep to the barriers, write nothing
   unsigned char* sq = align1024(smem_raw);
-  unsigned char* sk = sq + 2 * kTile;  // two stages of [keys][values]
+  unsigned char* sk = sq + 2 * kTile;  // stages of [keys][values], half a tile each
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int units = P.batch * P.sh.heads;
   // The last queries, which see most, first.
@@ -85,13 +91,18 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(Kv8AttnPa
   const int both = row0 + 128 < rows ? 2 : 1;  // tiles with rows
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < kPromptStages; ++i) {
       mbar_init(&kv_full[i], 4);
       mbar_init(&kv_empty[i], 1);
-      mbar_init(&s_full[i], 1);
-      mbar_init(&p_full[i], 4);
     }
-    mbar_init(&o_full, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&s_full[i][0], 1);
+      mbar_init(&s_full[i][1], 1);
+      mbar_init(&p_full[i][0], 4);
+      mbar_init(&p_full[i][1], 4);
+      mbar_init(&o_full[i][0], 1);
+      mbar_init(&o_full[i][1], 1);
+    }
     s_bad = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     fence_async_smem();
@@ -162,7 +173,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(Kv8AttnPa
     // ---- the softmax of a tile, a row to a thread ----
     const int mine = warp >> 2, in_tile = threadIdx.x & 127, row = row0 + 128 * mine + in_tile;
     const bool real = row < rows;
-    const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16), s_at = lanes + 128 * mine, o_at = lanes + 256 + 128 * mine;
+    const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16), o_at = lanes + 256 + 128 * mine;
     int lo = 0, hi = 0, back = 0;
     if (real) range_of(row, lo, hi);
     {
@@ -213,33 +224,34 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(Kv8AttnPa
       const int in_lo = __reduce_max_sync(kFullMask, lo), in_hi = __reduce_min_sync(kFullMask, real ? hi : 0x7fffffff);
       float ref = kNone, sum = 0.f;  // weights are 2^(score - ref)
       for (int j = 0; j < count; ++j) {
-        const int st = j & 1, tok0 = (block0 + j) * kPromptTokens;
-        if (!s_bad && !__all_sync(kFullMask, mbar_wait_quick(&s_full[mine], j & 1))) s_bad = 1;
+        const int st = j % kPromptStages, tok0 = (block0 + j) * kPromptTokens;
+        const uint32_t s_at = lanes + 128 * mine + 64 * (j & 1);
+        if (!s_bad && !__all_sync(kFullMask, mbar_wait_quick(&s_full[mine][j & 1], (j >> 1) & 1))) s_bad = 1;
         tc_fence_after();
-        float f[8], v[2][16];
+        float f[4], v[4][16];
 #pragma unroll
-        for (int r = 0; r < 8; ++r) f[r] = s_key[st][r] * kv_power(s_power[st][r] + back);
+        for (int c = 0; c < 4; ++c) tmem_ask16(s_at + 16 * c, v[c]);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) f[r] = s_key[st][r] * kv_power(s_power[st][r] + back);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tmem_arrived(v[c]);
         const bool full = tok0 >= in_lo && tok0 + kPromptTokens <= in_hi;
         // The largest score. (Factors are not negative, so a run's largest product gives its largest score.)
         const auto largest = [&](auto all) {
           constexpr bool kAll = decltype(all)::value;
-          float top = kNone, m[4];
-          tmem_ask16(s_at, v[0]);
+          float top = kNone;
 #pragma unroll
-          for (int c = 0; c < 8; ++c) {
-            tmem_arrived(v[c & 1]);
-            if (c < 7) tmem_ask16(s_at + 16 * (c + 1), v[(c + 1) & 1]);
+          for (int r = 0; r < 4; ++r) {
+            float m = kNone;
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              if ((c & 3) == 0) m[r] = kNone;
+            for (int c = 0; c < 4; ++c)
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
-                const int at = tok0 + 64 * (c >> 2) + prompt_token(16 * (c & 3) + 4 * r + i);
-                const float x = v[c & 1][4 * r + i];
-                m[r] = kAll || (at >= lo && at < hi) ? fmaxf(m[r], x) : m[r];
+                const int at = tok0 + prompt_token(16 * c + 4 * r + i);
+                const float x = v[c][4 * r + i];
+                m = kAll || (at >= lo && at < hi) ? fmaxf(m, x) : m;
               }
-              if ((c & 3) == 3) top = kAll || m[r] > kNone ? fmaxf(top, m[r] * f[4 * (c >> 2) + r]) : top;
-            }
+            top = kAll || m > kNone ? fmaxf(top, m * f[r]) : top;
           }
           return top;
         };
@@ -247,7 +259,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(Kv8AttnPa
         const bool move = top > __fadd_rd(ref, kKvLazy) || (ref == kNone && top > kNone);
         if (__any_sync(kFullMask, move)) {
           const float next = fmaxf(ref, top), keep = ref == kNone ? 0.f : kv_exp2(ref - next);
-          if (j > 0) {  // (the products before these scores' are over)
+          if (j > 0) {  // once the products before are over
+            if (!s_bad && !__all_sync(kFullMask, mbar_wait_quick(&o_full[mine][(j - 1) & 1], ((j - 1) >> 1) & 1))) s_bad = 1;
+            tc_fence_after();
 #pragma unroll 1
             for (int c = 0; c < kDim; c += 16) {
               float o[16];
@@ -268,22 +282,18 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(Kv8AttnPa
         float2 sums = make_float2(0.f, 0.f);
         const auto weights = [&](auto all) {
           constexpr bool kAll = decltype(all)::value;
-          tmem_ask16(s_at, v[0]);
 #pragma unroll
-          for (int c = 0; c < 8; c += 2) {
+          for (int c = 0; c < 4; c += 2) {
             uint32_t high[16], low[16];
 #pragma unroll
-            for (int d = 0; d < 2; ++d) {
-              tmem_arrived(v[d]);
-              if (c + d < 7) tmem_ask16(s_at + 16 * (c + d + 1), v[d ^ 1]);
+            for (int d = 0; d < 2; ++d)
 #pragma unroll
               for (int r = 0; r < 4; ++r) {
-                const int run = 4 * (c >> 2) + r;
-                const float2 f2 = make_float2(f[run], f[run]), w2 = make_float2(s_value[st][run], s_value[st][run]);
+                const float2 f2 = make_float2(f[r], f[r]), w2 = make_float2(s_value[st][r], s_value[st][r]);
 #pragma unroll
                 for (int i = 0; i < 4; i += 2) {
-                  float2 x = __ffma2_rn(make_float2(v[d][4 * r + i], v[d][4 * r + i + 1]), f2, less2);
-                  const int at = tok0 + 64 * (c >> 2) + prompt_token(16 * ((c + d) & 3) + 4 * r + i);  // and the next
+                  const float2 x = __ffma2_rn(make_float2(v[c + d][4 * r + i], v[c + d][4 * r + i + 1]), f2, less2);
+                  const int at = tok0 + prompt_token(16 * (c + d) + 4 * r + i);  // and the next
                   const bool one = kAll || (at >= lo && at < hi), two = kAll || (at + 1 >= lo && at + 1 < hi);
                   float2 p = make_float2(one ? kv_exp2(x.x) : 0.f, two ? kv_exp2(x.y) : 0.f);
                   sums = __fadd2_rn(sums, p);
@@ -299,8 +309,6 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(Kv8AttnPa
                   }
                 }
               }
-            }
-            // These 32 columns of S have been read; the next sixteen, asked for, are not among them.
             tmem_put16(s_at + 16 * c, high);
             if constexpr (kPrecise) tmem_put16(s_at + 16 * c + 16, low);
           }
@@ -311,12 +319,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(Kv8AttnPa
         tmem_put_wait();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[mine]);
+        if (lane == 0) mbar_arrive(&p_full[mine][j & 1]);
       }
-      if (count > 0) {
-        if (!s_bad && !__all_sync(kFullMask, mbar_wait_quick(&o_full, 0))) s_bad = 1;
-        tc_fence_after();
-      }
+      if (count > 0 && !s_bad && !__all_sync(kFullMask, mbar_wait_quick(&o_full[mine][(count - 1) & 1], ((count - 1) >> 1) & 1))) s_bad = 1;
+      tc_fence_after();
       const float inv = sum == 0.f ? 0.f : lower / sum;  // nothing seen: zeros
       T* out = static_cast<T*>(P.out) + (((long long)b * P.queries + row / P.share) * P.q_heads + head * P.share + row % P.share) * kDim;
 #pragma unroll 1
@@ -337,130 +343,117 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(Kv8AttnPa
     }
   } else if (warp < 12) {
     // ---- keys and values to operands ----
+    // 64 channels: two warps take two runs of keys each, two 32 channels of values. 128: each takes a run and 32 channels. The
+    // next step's bytes are asked for before this one's are converted, since only the stores wait for a stage.
     const int cw = warp - 8, g = lane >> 2, t = lane & 3;
+    constexpr bool kBoth = kAtoms == 2;
+    const bool has_keys = kBoth || cw < 2, has_values = kBoth || cw >= 2;
+    uint4 kc[4], vc[4];
+    const auto look_up = [&](int j) { return j < count ? page_of((block0 + j) * 4 + (lane & 3)) : -1; };
+    const auto ask = [&](int j, int pages) {
+      const auto get = [&](int r, int at) {
+        const int pg = __shfl_sync(kFullMask, pages, r);
+        const unsigned char* from = P.codes + ((long long)pg * P.sh.heads + head) * P.sh.block_bytes() +
+                                    (((block0 + j) * 4 + r) & (page_runs - 1)) * (32 * kDim) + lane * 16 + at;
+        return pg >= 0 ? __ldg(reinterpret_cast<const uint4*>(from)) : make_uint4(kKv8Zeros, kKv8Zeros, kKv8Zeros, kKv8Zeros);
+      };
+      if (has_keys)
+#pragma unroll
+        for (int l = 0; l < 4; ++l)
+          kc[l] = kBoth ? get(cw, (l >> 1) * (8 * kDim) + (l & 1) * 512) : get(2 * cw + (l >> 1), (l & 1) * (8 * kDim));
+      if (has_values)
+#pragma unroll
+        for (int l = 0; l < 4; ++l) vc[l] = get(l, 16 * kDim + (kBoth ? cw : cw - 2) * 512);
+    };
+    int page = look_up(0);
+    if (count > 0) ask(0, page);
     for (int j = 0; j < count; ++j) {
-      const int st = j & 1, run0 = (block0 + j) * 8;
-      unsigned char* keys = sk + st * 2 * kTile;
-      unsigned char* values = keys + kTile;
-      // Lane r's page is run r's; where a run's bytes of this lane lie, or null.
-      const int page = page_of(run0 + (lane & 7));
-      const auto base = [&](int r) -> const unsigned char* {
-        const int pg = __shfl_sync(kFullMask, page, r);
-        if (pg < 0) return nullptr;
-        return P.codes + ((long long)pg * P.sh.heads + head) * P.sh.block_bytes() + ((run0 + r) & (page_runs - 1)) * (32 * kDim) + lane * 16;
-      };
-      const auto get = [&](const unsigned char* from, int at) {
-        return from ? __ldg(reinterpret_cast<const uint4*>(from + at)) : make_uint4(kKv8Zeros, kKv8Zeros, kKv8Zeros, kKv8Zeros);
-      };
-      // A warp takes two runs of keys, and values of half the 64-token pieces' channels.
-      uint4 kc[2][2][kAtoms];
+      const int st = j % kPromptStages;
+      unsigned char* keys = sk + st * kTile;
+      unsigned char* values = keys + kTile / 2;
+      const int next = look_up(j + 1);
+      float2 step = make_float2(0.f, 0.f);
+      if (cw == 0 && page >= 0) step = __ldg(steps + (long long)page * P.sh.heads + head);
+      if (j >= kPromptStages && !s_bad && !__all_sync(kFullMask, mbar_wait_quick(&kv_empty[st], (j / kPromptStages - 1) & 1))) s_bad = 1;
+      if (has_keys)
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const unsigned char* from = base(2 * cw + i);
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-          for (int a = 0; a < kAtoms; ++a) kc[i][h][a] = get(from, h * (8 * kDim) + a * 512);
+        for (int l = 0; l < 4; ++l) {
+          const int run = kBoth ? cw : 2 * cw + (l >> 1), h = kBoth ? l >> 1 : l & 1, row = 16 * (g >> 1) + 4 * run + 2 * h + (g & 1);
+          const uint4 w = kc[l];
+          unsigned char* to = keys + (kBoth ? l & 1 : 0) * (64 * 128);
+          *reinterpret_cast<uint4*>(to + swizzled(row, 2 * t)) = make_uint4(kv8_codes<0>(w.x), kv8_codes<1>(w.x), kv8_codes<0>(w.y), kv8_codes<1>(w.y));
+          *reinterpret_cast<uint4*>(to + swizzled(row, 2 * t + 1)) = make_uint4(kv8_codes<0>(w.z), kv8_codes<1>(w.z), kv8_codes<0>(w.w), kv8_codes<1>(w.w));
+        }
+      if (has_values) {
+        const auto put = [&](int i, uint32_t w0, uint32_t w1, uint32_t w2, uint32_t w3) {
+          const int row = 32 * (kBoth ? cw : cw - 2) + 8 * i + g;
+          *reinterpret_cast<uint4*>(values + swizzled(row, 2 * t)) = make_uint4(kv8_codes<0>(w0), kv8_codes<1>(w0), kv8_codes<0>(w1), kv8_codes<1>(w1));
+          *reinterpret_cast<uint4*>(values + swizzled(row, 2 * t + 1)) = make_uint4(kv8_codes<0>(w2), kv8_codes<1>(w2), kv8_codes<0>(w3), kv8_codes<1>(w3));
+        };
+        put(0, vc[0].x, vc[1].x, vc[2].x, vc[3].x);
+        put(1, vc[0].y, vc[1].y, vc[2].y, vc[3].y);
+        put(2, vc[0].z, vc[1].z, vc[2].z, vc[3].z);
+        put(3, vc[0].w, vc[1].w, vc[2].w, vc[3].w);
       }
-      uint4 vc[kDim / 64][4];  // 32 channels of 64 tokens at a time
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const unsigned char* from = base(4 * (cw / 2) + r);
-#pragma unroll
-        for (int i = 0; i < kDim / 64; ++i) vc[i][r] = get(from, 16 * kDim + ((cw & 1) * (kDim / 64) + i) * 512);
-      }
-      if (j >= 2 && !s_bad && !__all_sync(kFullMask, mbar_wait_quick(&kv_empty[st], ((j >> 1) - 1) & 1))) s_bad = 1;
-      if (cw == 0 && lane < 8) {
-        float2 step = make_float2(0.f, 0.f);
-        if (page >= 0) step = __ldg(steps + (long long)page * P.sh.heads + head);
+      if (cw == 0 && lane < 4) {
         step.x = kv8_step(step.x), step.y = kv8_step(step.y);
         s_key[st][lane] = step.x > 0.f ? kv8_part(step.x) * P.scale_part : step.x;  // 0 and NaN as they are
         s_power[st][lane] = kv8_power(step.x);
         s_value[st][lane] = step.y * scaled;
       }
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int run = 2 * cw + i, row = 64 * (run >> 2) + 16 * (g >> 1) + 4 * (run & 3) + 2 * h + (g & 1);
-#pragma unroll
-          for (int a = 0; a < kAtoms; ++a) {
-            const uint4 w = kc[i][h][a];
-            unsigned char* to = keys + a * (128 * 128);
-            *reinterpret_cast<uint4*>(to + swizzled(row, 2 * t)) =
-                make_uint4(kv8_codes<0>(w.x), kv8_codes<1>(w.x), kv8_codes<0>(w.y), kv8_codes<1>(w.y));
-            *reinterpret_cast<uint4*>(to + swizzled(row, 2 * t + 1)) =
-                make_uint4(kv8_codes<0>(w.z), kv8_codes<1>(w.z), kv8_codes<0>(w.w), kv8_codes<1>(w.w));
-          }
-        }
-#pragma unroll
-      for (int i = 0; i < kDim / 64; ++i) {
-        const int atom = cw / 2, piece = (cw & 1) * (kDim / 64) + i;
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          const int row = 32 * piece + 8 * w + g;
-          uint32_t x[4];
-#pragma unroll
-          for (int r = 0; r < 4; ++r) x[r] = reinterpret_cast<const uint32_t*>(&vc[i][r])[w];
-          unsigned char* to = values + atom * (kDim * 128);
-          *reinterpret_cast<uint4*>(to + swizzled(row, 2 * t)) =
-              make_uint4(kv8_codes<0>(x[0]), kv8_codes<1>(x[0]), kv8_codes<0>(x[1]), kv8_codes<1>(x[1]));
-          *reinterpret_cast<uint4*>(to + swizzled(row, 2 * t + 1)) =
-              make_uint4(kv8_codes<0>(x[2]), kv8_codes<1>(x[2]), kv8_codes<0>(x[3]), kv8_codes<1>(x[3]));
-        }
-      }
+      if (j + 1 < count) ask(j + 1, next);
+      page = next;
       fence_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(&kv_full[st]);
     }
-  } else {
-    // ---- the MMAs (warp 12) ----
-    if (warp == 12) {
-      constexpr uint32_t to_s = f16_idesc(128, kPromptTokens), to_o = f16_idesc(128, kDim);
-      const uint64_t q0 = i8_sdesc(smem_u32(sq)), k0 = i8_sdesc(smem_u32(sk));
-      named_sync(1, 288);
-      const auto scores = [&](int x, int j) {
-        if (elect_one()) {
+  } else if (warp == 12) {
+    // ---- the MMAs ----
+    constexpr uint32_t to_s = f16_idesc(128, kPromptTokens), to_o = f16_idesc(128, kDim);
+    const uint32_t q0 = (uint32_t)i8_sdesc(smem_u32(sq)), k0 = (uint32_t)i8_sdesc(smem_u32(sk)), upper = (uint32_t)(i8_sdesc(0) >> 32);
+    named_sync(1, 288);
+    const auto scores = [&](int x, int j) {
+      if (elect_one()) {
+        const uint32_t q = q0 + x * (kTile >> 4), k = k0 + j % kPromptStages * (kTile >> 4), d = tmem + 128 * x + 64 * (j & 1);
 #pragma unroll
-          for (int c = 0; c < kDim / 16; ++c)
-            f16_mma(tmem + 128 * x, q0 + ((x * kTile + (c >> 2) * (128 * 128)) >> 4) + 2 * (c & 3),
-                    k0 + (((j & 1) * 2 * kTile + (c >> 2) * (128 * 128)) >> 4) + 2 * (c & 3), to_s, c > 0);
-          mma_commit(&s_full[x]);
+        for (int c = 0; c < kDim / 16; ++c)
+          f16_mma(d, q + (c >> 2) * (128 * 128 >> 4) + 2 * (c & 3), k + (c >> 2) * (64 * 128 >> 4) + 2 * (c & 3), upper, to_s, c > 0);
+        mma_commit(&s_full[x][j & 1]);
+      }
+      __syncwarp();
+    };
+    bool ok = true;
+    for (int j = 0; ok && j < 2 && j < count; ++j) {
+      ok = mbar_wait_quick(&kv_full[j], 0);
+      tc_fence_after();
+      for (int x = 0; ok && x < both; ++x) scores(x, j);
+    }
+    for (int j = 0; ok && j < count; ++j) {
+      const int st = j % kPromptStages;
+#pragma unroll 1
+      for (int x = 0; ok && x < both; ++x) {
+        ok = mbar_wait_quick(&p_full[x][j & 1], (j >> 1) & 1);
+        if (!ok) break;
+        tc_fence_after();
+        if (elect_one()) {
+          const uint32_t v = k0 + st * (kTile >> 4) + (kTile / 2 >> 4), p = tmem + 128 * x + 64 * (j & 1), d = tmem + 256 + 128 * x;
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            f16_mma_tmem(d, p + 32 * (c >> 1) + 8 * (c & 1), v + 2 * c, upper, to_o, j + c > 0);
+            if constexpr (kPrecise) f16_mma_tmem(d, p + 32 * (c >> 1) + 8 * (c & 1) + 16, v + 2 * c, upper, to_o, true);
+          }
+          if (x == both - 1) mma_commit(&kv_empty[st]);
+          mma_commit(&o_full[x][j & 1]);  // the last word to arrive in this CTA is one that is waited for
         }
         __syncwarp();
-      };
-      bool ok = true;
-      if (count > 0) {
-        ok = mbar_wait_quick(&kv_full[0], 0);
-        tc_fence_after();
-        if (ok)
-          for (int x = 0; x < both; ++x) scores(x, 0);
-      }
-      for (int j = 0; ok && j < count; ++j) {
-        const int st = j & 1;
-        if (j + 1 < count) ok = mbar_wait_quick(&kv_full[st ^ 1], ((j + 1) >> 1) & 1);
-        for (int x = 0; ok && x < both; ++x) {
-          ok = mbar_wait_quick(&p_full[x], j & 1);
-          if (!ok) break;
+        if (j + 2 < count) {
+          ok = x > 0 || mbar_wait_quick(&kv_full[(j + 2) % kPromptStages], ((j + 2) / kPromptStages) & 1);
           tc_fence_after();
-          if (elect_one()) {
-            const uint64_t v0 = k0 + ((st * 2 * kTile + kTile) >> 4);
-#pragma unroll
-            for (int c = 0; c < kPromptTokens / 16; ++c) {
-              const uint64_t v = v0 + ((c >> 2) * (kDim * 128) >> 4) + 2 * (c & 3);
-              const uint32_t p = tmem + 128 * x + 32 * (c >> 1) + 8 * (c & 1);
-              f16_mma_tmem(tmem + 256 + 128 * x, p, v, to_o, j > 0 || c > 0);
-              if constexpr (kPrecise) f16_mma_tmem(tmem + 256 + 128 * x, p + 16, v, to_o, true);
-            }
-            if (x == both - 1) mma_commit(&kv_empty[st]);
-            if (x == both - 1 && j == count - 1) mma_commit(&o_full);
-          }
-          __syncwarp();
-          if (j + 1 < count) scores(x, j + 1);
+          if (ok) scores(x, j + 2);
         }
       }
-      if (!ok) s_bad = 1;
     }
+    if (!ok) s_bad = 1;
   }
   tc_fence_before();
   __syncthreads();
