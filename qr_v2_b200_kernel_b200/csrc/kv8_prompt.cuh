@@ -6,9 +6,10 @@
 // S, P and O in tensor memory (P takes S's place), the softmax of a row in one thread. Each tile has two S, so that
 // the scores of the next step are there when a softmax ends (one S of 128 tokens: 172 us for the chunk below).
 //
-// Warps 0-3 and 4-7: the softmax of the first and the second tile. Warps 8-11: keys and values from bytes to
-// fp16 operands, through registers (16-bit numbers are twice the traffic, and what the cache saves); both land K-major in the
-// 128-byte swizzle, values transposed, which is how their bytes lie. Warp 12: the MMAs.
+// Warps 0-3 and 4-7: the softmax of the first and the second tile. Warp 13: bulk copies of the cache's bytes. Warps 8-11:
+// these into fp16 operands (16-bit numbers in memory are twice the traffic, and what the cache saves), K-major in the 128-byte
+// swizzle, values transposed, which is how their bytes lie. (Loads straight into these warps' registers are waited
+// for by the fence that the operands need: 166 us.) Warp 12: the MMAs.
 //
 // P is one fp16 number for bf16 results (its error, 2^-12 of a weight, is a sixteenth of what the result's rounding
 // leaves) and two, high and low, for fp16 ones. It is scaled by a power of two that puts the largest step of the
@@ -20,11 +21,12 @@
 
 namespace qrb200 {
 
-constexpr int kPromptRows = 256, kPromptTokens = 64, kPromptStages = 4;
-constexpr int kPromptThreads = 32 * 16;  // (three warps idle: registers are dealt out by fours of warps)
+constexpr int kPromptRows = 256, kPromptTokens = 64;
+constexpr int kPromptStages = 3, kPromptRaw = 3;  // steps of operands, and of bytes, in shared memory
+constexpr int kPromptThreads = 32 * 14;
 constexpr int kPromptStepExp = 11;
 __host__ __device__ constexpr int prompt_tile(int dim) { return 128 * dim * 2; }  // bytes of 128 rows of fp16
-__host__ __device__ constexpr int prompt_smem_bytes(int dim) { return 1024 + (2 + kPromptStages) * prompt_tile(dim); }
+__host__ __device__ constexpr int prompt_smem_bytes(int dim) { return 1024 + (2 + kPromptStages) * prompt_tile(dim) + kPromptRaw * prompt_tile(dim) / 2; }
 
 // kind::f16: fp16 operands, both K-major, 32-bit accumulator.
 __host__ __device__ constexpr uint32_t f16_idesc(int M, int N) { return (1u << 4) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24); }
@@ -73,16 +75,20 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(Kv8AttnPa
   constexpr bool kPrecise = std::is_same<T, __half>::value;  // weights in two halves
   constexpr float kNone = -INFINITY;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
-  __shared__ uint64_t kv_full[kPromptStages], kv_empty[kPromptStages], s_full[2][2], p_full[2][2], o_full[2][2];  // [tile][odd steps]
+  __shared__ uint64_t raw_full[kPromptRaw], raw_empty[kPromptRaw], kv_full[kPromptStages], kv_empty[kPromptStages], s_full[2][2], p_full[2][2], o_full[2][2];  // [tile][odd steps]
   // (A softmax may be two steps ahead of the products with the values, and a barrier tells a phase only from the one before it:
   // so each step waits for a barrier whose last phase but one is known to be over.)
   __shared__ uint32_t s_tmem;
   __shared__ float s_key[kPromptStages][4], s_value[kPromptStages][4];  // steps of a stage's runs; values' scaled
   __shared__ int s_power[kPromptStages][4];  // the keys' step's power of two (s_key holds its significand)
-  __shared__ unsigned s_most[16];
+  __shared__ int s_gone[kPromptStages];      // bits: runs without a page
+  __shared__ float2 s_step[kPromptRaw][4];
+  __shared__ int s_missing[kPromptRaw];
+  __shared__ unsigned s_most[14];
   __shared__ volatile int s_bad;  // a wait ran out: keep to the barriers, write nothing
   unsigned char* sq = align1024(smem_raw);
   unsigned char* sk = sq + 2 * kTile;  // stages of [keys][values], half a tile each
+  unsigned char* raw = sk + kPromptStages * kTile;  // steps of the cache's bytes
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int units = P.batch * P.sh.heads;
   // The last queries, which see most, first.
@@ -91,6 +97,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(Kv8AttnPa
   const int both = row0 + 128 < rows ? 2 : 1;  // tiles with rows
 
   if (threadIdx.x == 0) {
+    for (int i = 0; i < kPromptRaw; ++i) {
+      mbar_init(&raw_full[i], 1);
+      mbar_init(&raw_empty[i], 4);
+    }
     for (int i = 0; i < kPromptStages; ++i) {
       mbar_init(&kv_full[i], 4);
       mbar_init(&kv_empty[i], 1);
@@ -164,7 +174,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(Kv8AttnPa
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  most = __reduce_max_sync(kFullMask, s_most[lane & 15]);
+  most = __reduce_max_sync(kFullMask, lane < 14 ? s_most[lane] : 0u);
   const int cap = max(-100, min(126, (int)(most >> 23) - 126));  // 2^cap is above it
   const float scaled = __int_as_float((kPromptStepExp - cap + 127) << 23), lower = __int_as_float((cap - kPromptStepExp + 127) << 23);
   const uint32_t tmem = s_tmem;
@@ -235,7 +245,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(Kv8AttnPa
         for (int r = 0; r < 4; ++r) f[r] = s_key[st][r] * kv_power(s_power[st][r] + back);
 #pragma unroll
         for (int c = 0; c < 4; ++c) tmem_arrived(v[c]);
-        const bool full = tok0 >= in_lo && tok0 + kPromptTokens <= in_hi;
+        const int gone = s_gone[st];
+        const bool full = tok0 >= in_lo && tok0 + kPromptTokens <= in_hi && gone == 0;
         // The largest score. (Factors are not negative, so a run's largest product gives its largest score.)
         const auto largest = [&](auto all) {
           constexpr bool kAll = decltype(all)::value;
@@ -249,7 +260,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(Kv8AttnPa
               for (int i = 0; i < 4; ++i) {
                 const int at = tok0 + prompt_token(16 * c + 4 * r + i);
                 const float x = v[c][4 * r + i];
-                m = kAll || (at >= lo && at < hi) ? fmaxf(m, x) : m;
+                m = kAll || (at >= lo && at < hi && !(gone >> r & 1)) ? fmaxf(m, x) : m;
               }
             top = kAll || m > kNone ? fmaxf(top, m * f[r]) : top;
           }
@@ -294,7 +305,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(Kv8AttnPa
                 for (int i = 0; i < 4; i += 2) {
                   const float2 x = __ffma2_rn(make_float2(v[c + d][4 * r + i], v[c + d][4 * r + i + 1]), f2, less2);
                   const int at = tok0 + prompt_token(16 * (c + d) + 4 * r + i);  // and the next
-                  const bool one = kAll || (at >= lo && at < hi), two = kAll || (at + 1 >= lo && at + 1 < hi);
+                  const bool one = kAll || (at >= lo && at < hi && !(gone >> r & 1)), two = kAll || (at + 1 >= lo && at + 1 < hi && !(gone >> r & 1));
                   float2 p = make_float2(one ? kv_exp2(x.x) : 0.f, two ? kv_exp2(x.y) : 0.f);
                   sums = __fadd2_rn(sums, p);
                   p = __fmul2_rn(p, w2);
@@ -343,70 +354,85 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(Kv8AttnPa
     }
   } else if (warp < 12) {
     // ---- keys and values to operands ----
-    // 64 channels: two warps take two runs of keys each, two 32 channels of values. 128: each takes a run and 32 channels. The
-    // next step's bytes are asked for before this one's are converted, since only the stores wait for a stage.
+    // 64 channels: two warps take two runs of keys each, two 32 channels of values. 128: each takes a run and 32 channels.
     const int cw = warp - 8, g = lane >> 2, t = lane & 3;
     constexpr bool kBoth = kAtoms == 2;
-    const bool has_keys = kBoth || cw < 2, has_values = kBoth || cw >= 2;
-    uint4 kc[4], vc[4];
-    const auto look_up = [&](int j) { return j < count ? page_of((block0 + j) * 4 + (lane & 3)) : -1; };
-    const auto ask = [&](int j, int pages) {
-      const auto get = [&](int r, int at) {
-        const int pg = __shfl_sync(kFullMask, pages, r);
-        const unsigned char* from = P.codes + ((long long)pg * P.sh.heads + head) * P.sh.block_bytes() +
-                                    (((block0 + j) * 4 + r) & (page_runs - 1)) * (32 * kDim) + lane * 16 + at;
-        return pg >= 0 ? __ldg(reinterpret_cast<const uint4*>(from)) : make_uint4(kKv8Zeros, kKv8Zeros, kKv8Zeros, kKv8Zeros);
-      };
-      if (has_keys)
-#pragma unroll
-        for (int l = 0; l < 4; ++l)
-          kc[l] = kBoth ? get(cw, (l >> 1) * (8 * kDim) + (l & 1) * 512) : get(2 * cw + (l >> 1), (l & 1) * (8 * kDim));
-      if (has_values)
-#pragma unroll
-        for (int l = 0; l < 4; ++l) vc[l] = get(l, 16 * kDim + (kBoth ? cw : cw - 2) * 512);
-    };
-    int page = look_up(0);
-    if (count > 0) ask(0, page);
+    constexpr int kRun = 32 * kDim;
     for (int j = 0; j < count; ++j) {
-      const int st = j % kPromptStages;
+      const int st = j % kPromptStages, rs = j % kPromptRaw;
       unsigned char* keys = sk + st * kTile;
       unsigned char* values = keys + kTile / 2;
-      const int next = look_up(j + 1);
-      float2 step = make_float2(0.f, 0.f);
-      if (cw == 0 && page >= 0) step = __ldg(steps + (long long)page * P.sh.heads + head);
+      const unsigned char* from = raw + rs * (kTile / 2) + lane * 16;
+      if (!s_bad && !__all_sync(kFullMask, mbar_wait_quick(&raw_full[rs], (j / kPromptRaw) & 1))) s_bad = 1;
       if (j >= kPromptStages && !s_bad && !__all_sync(kFullMask, mbar_wait_quick(&kv_empty[st], (j / kPromptStages - 1) & 1))) s_bad = 1;
-      if (has_keys)
+      if (kBoth || cw < 2)
 #pragma unroll
         for (int l = 0; l < 4; ++l) {
-          const int run = kBoth ? cw : 2 * cw + (l >> 1), h = kBoth ? l >> 1 : l & 1, row = 16 * (g >> 1) + 4 * run + 2 * h + (g & 1);
-          const uint4 w = kc[l];
-          unsigned char* to = keys + (kBoth ? l & 1 : 0) * (64 * 128);
+          const int run = kBoth ? cw : 2 * cw + (l >> 1), h = kBoth ? l >> 1 : l & 1, a = kBoth ? l & 1 : 0;
+          const int row = 16 * (g >> 1) + 4 * run + 2 * h + (g & 1);
+          const uint4 w = *reinterpret_cast<const uint4*>(from + run * kRun + h * (8 * kDim) + a * 512);
+          unsigned char* to = keys + a * (64 * 128);
           *reinterpret_cast<uint4*>(to + swizzled(row, 2 * t)) = make_uint4(kv8_codes<0>(w.x), kv8_codes<1>(w.x), kv8_codes<0>(w.y), kv8_codes<1>(w.y));
           *reinterpret_cast<uint4*>(to + swizzled(row, 2 * t + 1)) = make_uint4(kv8_codes<0>(w.z), kv8_codes<1>(w.z), kv8_codes<0>(w.w), kv8_codes<1>(w.w));
         }
-      if (has_values) {
+      if (kBoth || cw >= 2) {
+        const int piece = kBoth ? cw : cw - 2;
+        uint4 w[4];
+#pragma unroll
+        for (int l = 0; l < 4; ++l) w[l] = *reinterpret_cast<const uint4*>(from + l * kRun + 16 * kDim + piece * 512);
         const auto put = [&](int i, uint32_t w0, uint32_t w1, uint32_t w2, uint32_t w3) {
-          const int row = 32 * (kBoth ? cw : cw - 2) + 8 * i + g;
+          const int row = 32 * piece + 8 * i + g;
           *reinterpret_cast<uint4*>(values + swizzled(row, 2 * t)) = make_uint4(kv8_codes<0>(w0), kv8_codes<1>(w0), kv8_codes<0>(w1), kv8_codes<1>(w1));
           *reinterpret_cast<uint4*>(values + swizzled(row, 2 * t + 1)) = make_uint4(kv8_codes<0>(w2), kv8_codes<1>(w2), kv8_codes<0>(w3), kv8_codes<1>(w3));
         };
-        put(0, vc[0].x, vc[1].x, vc[2].x, vc[3].x);
-        put(1, vc[0].y, vc[1].y, vc[2].y, vc[3].y);
-        put(2, vc[0].z, vc[1].z, vc[2].z, vc[3].z);
-        put(3, vc[0].w, vc[1].w, vc[2].w, vc[3].w);
+        put(0, w[0].x, w[1].x, w[2].x, w[3].x);
+        put(1, w[0].y, w[1].y, w[2].y, w[3].y);
+        put(2, w[0].z, w[1].z, w[2].z, w[3].z);
+        put(3, w[0].w, w[1].w, w[2].w, w[3].w);
       }
       if (cw == 0 && lane < 4) {
-        step.x = kv8_step(step.x), step.y = kv8_step(step.y);
+        const float2 step = s_step[rs][lane];
         s_key[st][lane] = step.x > 0.f ? kv8_part(step.x) * P.scale_part : step.x;  // 0 and NaN as they are
         s_power[st][lane] = kv8_power(step.x);
         s_value[st][lane] = step.y * scaled;
+        if (lane == 0) s_gone[st] = s_missing[rs];
       }
-      if (j + 1 < count) ask(j + 1, next);
-      page = next;
       fence_async_smem();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&kv_full[st]);
+      if (lane == 0) {
+        mbar_arrive(&kv_full[st]);
+        mbar_arrive(&raw_empty[rs]);
+      }
     }
+  } else if (warp == 13) {
+    // ---- bulk copies, a run of 16 tokens to each of four lanes ----
+    const auto look_up = [&](int j) { return j < count ? page_of((block0 + j) * 4 + (lane & 3)) : -1; };
+    constexpr int kRun = 32 * kDim;
+    int page = look_up(0);
+    for (int j = 0; j < count && !s_bad; ++j) {
+      const int rs = j % kPromptRaw, next = look_up(j + 1);
+      float2 step = make_float2(0.f, 0.f);
+      if (page >= 0) step = __ldg(steps + (long long)page * P.sh.heads + head);
+      const unsigned here = __ballot_sync(kFullMask, page >= 0) & 15u;
+      if (j >= kPromptRaw && !__all_sync(kFullMask, mbar_wait_quick(&raw_empty[rs], (j / kPromptRaw - 1) & 1))) {
+        s_bad = 1;
+        break;
+      }
+      if (lane < 4) s_step[rs][lane] = make_float2(kv8_step(step.x), kv8_step(step.y));
+      if (lane == 0) s_missing[rs] = 15 & ~here;
+      __syncwarp();
+      const uint32_t bar = smem_u32(&raw_full[rs]);
+      if (lane == 0) mbar_expect(bar, __popc(here) * kRun);
+      __syncwarp();
+      if (lane < 4 && page >= 0)
+        kv_copy(smem_u32(raw + rs * (kTile / 2) + lane * kRun),
+                P.codes + ((long long)page * P.sh.heads + head) * P.sh.block_bytes() + (((block0 + j) * 4 + lane) & (page_runs - 1)) * kRun,
+                kRun, bar);
+      page = next;
+    }
+    // Every copy is waited for by those who convert it; should they have given up, here, with a limit.
+    if (s_bad)
+      for (int rs = 0; rs < kPromptRaw; ++rs) mbar_wait_limit(&raw_full[rs], 0, 1u << 16, kSiteMbarrier), mbar_wait_limit(&raw_full[rs], 1, 1u << 16, kSiteMbarrier);
   } else if (warp == 12) {
     // ---- the MMAs ----
     constexpr uint32_t to_s = f16_idesc(128, kPromptTokens), to_o = f16_idesc(128, kDim);
