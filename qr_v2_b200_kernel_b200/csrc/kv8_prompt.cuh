@@ -6,10 +6,11 @@
 // S, P and O in tensor memory (P takes S's place), the softmax of a row in one thread. Each tile has two S, so that
 // the scores of the next step are there when a softmax ends (one S of 128 tokens: 172 us for the chunk below).
 //
-// Warps 0-3 and 4-7: the softmax of the first and the second tile. Warp 13: bulk copies of the cache's bytes. Warps 8-11:
+// Warps 0-3 and 4-7: the softmax of the first and the second tile. Warp 14: bulk copies of the cache's bytes. Warps 8-11:
 // these into fp16 operands (16-bit numbers in memory are twice the traffic, and what the cache saves), K-major in the 128-byte
 // swizzle, values transposed, which is how their bytes lie. (Loads straight into these warps' registers are waited
-// for by the fence that the operands need: 166 us.) Warp 12: the MMAs.
+// for by the fence that the operands need.) Warps 12 and 13: a tile's MMAs each (their issue takes some 45
+// clocks, as long as the smallest of them run).
 //
 // P is one fp16 number for bf16 results (its error, 2^-12 of a weight, is a sixteenth of what the result's rounding
 // leaves) and two, high and low, for fp16 ones. It is scaled by a power of two that puts the largest step of the
@@ -23,7 +24,7 @@ namespace qrb200 {
 
 constexpr int kPromptRows = 256, kPromptTokens = 64;
 constexpr int kPromptStages = 3, kPromptRaw = 3;  // steps of operands, and of bytes, in shared memory
-constexpr int kPromptThreads = 32 * 14;
+constexpr int kPromptThreads = 32 * 15;
 constexpr int kPromptStepExp = 11;
 __host__ __device__ constexpr int prompt_tile(int dim) { return 128 * dim * 2; }  // bytes of 128 rows of fp16
 __host__ __device__ constexpr int prompt_smem_bytes(int dim) { return 1024 + (2 + kPromptStages) * prompt_tile(dim) + kPromptRaw * prompt_tile(dim) / 2; }
@@ -79,12 +80,11 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(Kv8AttnPa
   // (A softmax may be two steps ahead of the products with the values, and a barrier tells a phase only from the one before it:
   // so each step waits for a barrier whose last phase but one is known to be over.)
   __shared__ uint32_t s_tmem;
-  __shared__ float s_key[kPromptStages][4], s_value[kPromptStages][4];  // steps of a stage's runs; values' scaled
-  __shared__ int s_power[kPromptStages][4];  // the keys' step's power of two (s_key holds its significand)
+  __shared__ float4 s_key[kPromptStages], s_value[kPromptStages];  // steps of a stage's runs, scaled
   __shared__ int s_gone[kPromptStages];      // bits: runs without a page
   __shared__ float2 s_step[kPromptRaw][4];
   __shared__ int s_missing[kPromptRaw];
-  __shared__ unsigned s_most[14];
+  __shared__ unsigned s_most[2][15];
   __shared__ volatile int s_bad;  // a wait ran out: keep to the barriers, write nothing
   unsigned char* sq = align1024(smem_raw);
   unsigned char* sk = sq + 2 * kTile;  // stages of [keys][values], half a tile each
@@ -103,7 +103,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(Kv8AttnPa
     }
     for (int i = 0; i < kPromptStages; ++i) {
       mbar_init(&kv_full[i], 4);
-      mbar_init(&kv_empty[i], 1);
+      mbar_init(&kv_empty[i], both);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s_full[i][0], 1);
@@ -159,23 +159,29 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(Kv8AttnPa
   };
   const float2* steps = reinterpret_cast<const float2*>(P.range);
 
-  // The largest value step of the pages that are seen.
-  unsigned most = 0;
+  // The largest steps of the pages that are seen.
+  unsigned most[2] = {0, 0};
   const int page_runs = P.sh.page / 16;
   for (int page = first_run / page_runs + threadIdx.x; page * page_runs < last_run; page += kPromptThreads) {
     const int at = page_of(max(first_run, page * page_runs));
     if (at >= 0) {
-      const float w = kv8_step(__ldg(steps + (long long)at * P.sh.heads + head).y);
-      if (w == w) most = max(most, __float_as_uint(w));  // (not NaN)
+      const float2 step = __ldg(steps + (long long)at * P.sh.heads + head);
+      if (step.x == step.x) most[0] = max(most[0], __float_as_uint(kv8_step(step.x)));  // (not NaN)
+      if (step.y == step.y) most[1] = max(most[1], __float_as_uint(kv8_step(step.y)));
     }
   }
-  most = __reduce_max_sync(kFullMask, most);
-  if (lane == 0) s_most[warp] = most;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    most[i] = __reduce_max_sync(kFullMask, most[i]);
+    if (lane == 0) s_most[i][warp] = most[i];
+  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  most = __reduce_max_sync(kFullMask, lane < 14 ? s_most[lane] : 0u);
-  const int cap = max(-100, min(126, (int)(most >> 23) - 126));  // 2^cap is above it
+  // The keys' steps are held relative to 2^key_power, a row's factor takes that back: together they are in range
+  // wherever the largest scores are. The values' are scaled by 2^kPromptStepExp / 2^cap, with 2^cap above the largest.
+  const int key_power = (int)(__reduce_max_sync(kFullMask, lane < 15 ? s_most[0][lane] : 0u) >> 23) - 127;
+  const int cap = max(-100, min(126, (int)(__reduce_max_sync(kFullMask, lane < 15 ? s_most[1][lane] : 0u) >> 23) - 126));
   const float scaled = __int_as_float((kPromptStepExp - cap + 127) << 23), lower = __int_as_float((cap - kPromptStepExp + 127) << 23);
   const uint32_t tmem = s_tmem;
 
@@ -184,7 +190,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(Kv8AttnPa
     const int mine = warp >> 2, in_tile = threadIdx.x & 127, row = row0 + 128 * mine + in_tile;
     const bool real = row < rows;
     const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16), o_at = lanes + 256 + 128 * mine;
-    int lo = 0, hi = 0, back = 0;
+    int lo = 0, hi = 0;
+    float back;  // the power of two that takes a row's size, the scale's and the keys' back, into the exponent's units (base 2)
     if (real) range_of(row, lo, hi);
     {
       // The row's query, permuted as the keys' bytes are: piece k of 64 channels holds channels 16 w + 4 t + e with t =
@@ -211,7 +218,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(Kv8AttnPa
       }
       const int power = max(1, min(254, (int)(top >> 23))) - 127, lift = kKv8Top - power;
       const float up = kv_power(lift / 2), more = kv_power(lift - lift / 2);
-      back = power - kKv8Top + P.scale_power;
+      back = kv_power(power - kKv8Top + P.scale_power + key_power);
 #pragma unroll 1
       for (int a = 0; a < kAtoms; ++a)
 #pragma unroll
@@ -228,21 +235,23 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(Kv8AttnPa
         }
     }
     fence_async_smem();
-    named_sync(1, 288);  // with the MMAs' warp: both tiles' queries are there
+    named_sync(1 + mine, 160);  // with the MMAs' warp: the tile's queries are there
     if (mine < both) {
       // What every row of the warp sees.
       const int in_lo = __reduce_max_sync(kFullMask, lo), in_hi = __reduce_min_sync(kFullMask, real ? hi : 0x7fffffff);
       float ref = kNone, sum = 0.f;  // weights are 2^(score - ref)
+      bool ok = true;
       for (int j = 0; j < count; ++j) {
         const int st = j % kPromptStages, tok0 = (block0 + j) * kPromptTokens;
         const uint32_t s_at = lanes + 128 * mine + 64 * (j & 1);
-        if (!s_bad && !__all_sync(kFullMask, mbar_wait_quick(&s_full[mine][j & 1], (j >> 1) & 1))) s_bad = 1;
+        ok = ok && mbar_wait_quick(&s_full[mine][j & 1], (j >> 1) & 1);
+        __syncwarp();
         tc_fence_after();
-        float f[4], v[4][16];
+        float v[4][16];
 #pragma unroll
         for (int c = 0; c < 4; ++c) tmem_ask16(s_at + 16 * c, v[c]);
-#pragma unroll
-        for (int r = 0; r < 4; ++r) f[r] = s_key[st][r] * kv_power(s_power[st][r] + back);
+        const float4 k4 = s_key[st], w4 = s_value[st];
+        const float f[4] = {k4.x * back, k4.y * back, k4.z * back, k4.w * back}, w[4] = {w4.x, w4.y, w4.z, w4.w};
 #pragma unroll
         for (int c = 0; c < 4; ++c) tmem_arrived(v[c]);
         const int gone = s_gone[st];
@@ -271,17 +280,18 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(Kv8AttnPa
         if (__any_sync(kFullMask, move)) {
           const float next = fmaxf(ref, top), keep = ref == kNone ? 0.f : kv_exp2(ref - next);
           if (j > 0) {  // once the products before are over
-            if (!s_bad && !__all_sync(kFullMask, mbar_wait_quick(&o_full[mine][(j - 1) & 1], ((j - 1) >> 1) & 1))) s_bad = 1;
+            ok = ok && mbar_wait_quick(&o_full[mine][(j - 1) & 1], ((j - 1) >> 1) & 1);
+            __syncwarp();
             tc_fence_after();
 #pragma unroll 1
             for (int c = 0; c < kDim; c += 16) {
               float o[16];
               tmem_ask16(o_at + c, o);
               tmem_arrived(o);
-              uint32_t w[16];
+              uint32_t kept[16];
 #pragma unroll
-              for (int i = 0; i < 16; ++i) w[i] = __float_as_uint(ref == kNone ? 0.f : o[i] * keep);
-              tmem_put16(o_at + c, w);
+              for (int i = 0; i < 16; ++i) kept[i] = __float_as_uint(ref == kNone ? 0.f : o[i] * keep);
+              tmem_put16(o_at + c, kept);
             }
             tmem_put_wait();
           }
@@ -300,7 +310,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(Kv8AttnPa
             for (int d = 0; d < 2; ++d)
 #pragma unroll
               for (int r = 0; r < 4; ++r) {
-                const float2 f2 = make_float2(f[r], f[r]), w2 = make_float2(s_value[st][r], s_value[st][r]);
+                const float2 f2 = make_float2(f[r], f[r]), w2 = make_float2(w[r], w[r]);
 #pragma unroll
                 for (int i = 0; i < 4; i += 2) {
                   const float2 x = __ffma2_rn(make_float2(v[c + d][4 * r + i], v[c + d][4 * r + i + 1]), f2, less2);
@@ -332,7 +342,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(Kv8AttnPa
         __syncwarp();
         if (lane == 0) mbar_arrive(&p_full[mine][j & 1]);
       }
-      if (count > 0 && !s_bad && !__all_sync(kFullMask, mbar_wait_quick(&o_full[mine][(count - 1) & 1], ((count - 1) >> 1) & 1))) s_bad = 1;
+      if (count > 0) ok = ok && mbar_wait_quick(&o_full[mine][(count - 1) & 1], ((count - 1) >> 1) & 1);
+      if (!ok) s_bad = 1;
+      __syncwarp();
       tc_fence_after();
       const float inv = sum == 0.f ? 0.f : lower / sum;  // nothing seen: zeros
       T* out = static_cast<T*>(P.out) + (((long long)b * P.queries + row / P.share) * P.q_heads + head * P.share + row % P.share) * kDim;
@@ -392,9 +404,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(Kv8AttnPa
       }
       if (cw == 0 && lane < 4) {
         const float2 step = s_step[rs][lane];
-        s_key[st][lane] = step.x > 0.f ? kv8_part(step.x) * P.scale_part : step.x;  // 0 and NaN as they are
-        s_power[st][lane] = kv8_power(step.x);
-        s_value[st][lane] = step.y * scaled;
+        reinterpret_cast<float*>(&s_key[st])[lane] = step.x > 0.f ? kv8_part(step.x) * P.scale_part * kv_power(kv8_power(step.x) - key_power) : step.x;  // 0 and NaN as they are
+        reinterpret_cast<float*>(&s_value[st])[lane] = step.y * scaled;
         if (lane == 0) s_gone[st] = s_missing[rs];
       }
       fence_async_smem();
@@ -404,7 +415,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(Kv8AttnPa
         mbar_arrive(&raw_empty[rs]);
       }
     }
-  } else if (warp == 13) {
+  } else if (warp == 14) {
     // ---- bulk copies, a run of 16 tokens to each of four lanes ----
     const auto look_up = [&](int j) { return j < count ? page_of((block0 + j) * 4 + (lane & 3)) : -1; };
     constexpr int kRun = 32 * kDim;
@@ -433,14 +444,15 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(Kv8AttnPa
     // Every copy is waited for by those who convert it; should they have given up, here, with a limit.
     if (s_bad)
       for (int rs = 0; rs < kPromptRaw; ++rs) mbar_wait_limit(&raw_full[rs], 0, 1u << 16, kSiteMbarrier), mbar_wait_limit(&raw_full[rs], 1, 1u << 16, kSiteMbarrier);
-  } else if (warp == 12) {
-    // ---- the MMAs ----
+  } else {
+    // ---- a tile's MMAs ----
     constexpr uint32_t to_s = f16_idesc(128, kPromptTokens), to_o = f16_idesc(128, kDim);
-    const uint32_t q0 = (uint32_t)i8_sdesc(smem_u32(sq)), k0 = (uint32_t)i8_sdesc(smem_u32(sk)), upper = (uint32_t)(i8_sdesc(0) >> 32);
-    named_sync(1, 288);
-    const auto scores = [&](int x, int j) {
+    const int x = warp - 12;
+    const uint32_t q = (uint32_t)i8_sdesc(smem_u32(sq)) + x * (kTile >> 4), k0 = (uint32_t)i8_sdesc(smem_u32(sk)), upper = (uint32_t)(i8_sdesc(0) >> 32);
+    named_sync(1 + x, 160);
+    const auto scores = [&](int j) {
       if (elect_one()) {
-        const uint32_t q = q0 + x * (kTile >> 4), k = k0 + j % kPromptStages * (kTile >> 4), d = tmem + 128 * x + 64 * (j & 1);
+        const uint32_t k = k0 + j % kPromptStages * (kTile >> 4), d = tmem + 128 * x + 64 * (j & 1);
 #pragma unroll
         for (int c = 0; c < kDim / 16; ++c)
           f16_mma(d, q + (c >> 2) * (128 * 128 >> 4) + 2 * (c & 3), k + (c >> 2) * (64 * 128 >> 4) + 2 * (c & 3), upper, to_s, c > 0);
@@ -449,34 +461,31 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(Kv8AttnPa
       __syncwarp();
     };
     bool ok = true;
-    for (int j = 0; ok && j < 2 && j < count; ++j) {
+    for (int j = 0; ok && x < both && j < 2 && j < count; ++j) {
       ok = mbar_wait_quick(&kv_full[j], 0);
       tc_fence_after();
-      for (int x = 0; ok && x < both; ++x) scores(x, j);
+      if (ok) scores(j);
     }
-    for (int j = 0; ok && j < count; ++j) {
+    for (int j = 0; ok && x < both && j < count; ++j) {
       const int st = j % kPromptStages;
-#pragma unroll 1
-      for (int x = 0; ok && x < both; ++x) {
-        ok = mbar_wait_quick(&p_full[x][j & 1], (j >> 1) & 1);
-        if (!ok) break;
-        tc_fence_after();
-        if (elect_one()) {
-          const uint32_t v = k0 + st * (kTile >> 4) + (kTile / 2 >> 4), p = tmem + 128 * x + 64 * (j & 1), d = tmem + 256 + 128 * x;
+      ok = mbar_wait_quick(&p_full[x][j & 1], (j >> 1) & 1);
+      if (!ok) break;
+      tc_fence_after();
+      if (elect_one()) {
+        const uint32_t v = k0 + st * (kTile >> 4) + (kTile / 2 >> 4), p = tmem + 128 * x + 64 * (j & 1), d = tmem + 256 + 128 * x;
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            f16_mma_tmem(d, p + 32 * (c >> 1) + 8 * (c & 1), v + 2 * c, upper, to_o, j + c > 0);
-            if constexpr (kPrecise) f16_mma_tmem(d, p + 32 * (c >> 1) + 8 * (c & 1) + 16, v + 2 * c, upper, to_o, true);
-          }
-          if (x == both - 1) mma_commit(&kv_empty[st]);
-          mma_commit(&o_full[x][j & 1]);  // the last word to arrive in this CTA is one that is waited for
+        for (int c = 0; c < 4; ++c) {
+          f16_mma_tmem(d, p + 32 * (c >> 1) + 8 * (c & 1), v + 2 * c, upper, to_o, j + c > 0);
+          if constexpr (kPrecise) f16_mma_tmem(d, p + 32 * (c >> 1) + 8 * (c & 1) + 16, v + 2 * c, upper, to_o, true);
         }
-        __syncwarp();
-        if (j + 2 < count) {
-          ok = x > 0 || mbar_wait_quick(&kv_full[(j + 2) % kPromptStages], ((j + 2) / kPromptStages) & 1);
-          tc_fence_after();
-          if (ok) scores(x, j + 2);
-        }
+        mma_commit(&kv_empty[st]);
+        mma_commit(&o_full[x][j & 1]);  // the last word to arrive in this CTA is one that is waited for
+      }
+      __syncwarp();
+      if (j + 2 < count) {
+        ok = mbar_wait_quick(&kv_full[(j + 2) % kPromptStages], ((j + 2) / kPromptStages) & 1);
+        tc_fence_after();
+        if (ok) scores(j + 2);
       }
     }
     if (!ok) s_bad = 1;
