@@ -22,8 +22,6 @@ static cudaError_t with_shape(int dtype, int dim, F&& f) {
   return dim == 64 ? f(__half{}, Int<64>{}) : f(__half{}, Int<128>{});
 }
 
-constexpr int kPromptFrom = 64;  // query rows of a key head from which on kv8_prompt_kernel takes them
-
 // How an attention call is cut: query rows per tile, steps of 4 or 8 KB, and the token range over `splits` CTAs.
 struct Kv8Plan {
   int tile_rows, tiles, splits;
@@ -42,11 +40,8 @@ static Kv8Plan attn_plan(const Kv8Shape& h, int64_t batch, int64_t queries, int6
   static const int kShort[5] = {0, 750, 1000, 1300, 1400}, kLong[3] = {0, 1000, 1400}, kLong16[3] = {0, 1500, 2300};
   Kv8Plan p{};
   const int64_t rows = queries * (q_heads / h.heads);
-  p.prompt = rows >= kPromptFrom;
-  p.tile_rows = p.prompt ? kPromptRows : rows <= 8 ? 8 : 16;
+  p.tile_rows = rows <= 8 ? 8 : 16;
   p.tiles = ceil_div(rows, p.tile_rows);
-  p.splits = 1;
-  if (p.prompt) return p;
   const int64_t ctas = batch * h.heads * p.tiles, tokens = std::min(max_pages * h.page, span), sms = sm_count();
   int64_t best = -1;
   for (int brief = 0; brief <= (p.tile_rows == 8 ? 1 : 0); ++brief) {
@@ -62,6 +57,15 @@ static Kv8Plan attn_plan(const Kv8Shape& h, int64_t batch, int64_t queries, int6
         p.splits = (int)n, p.brief = brief, p.memory = memory;
       }
     }
+  }
+  // The prompt kernel does not split the tokens: 1.15 us for each 64 of them and 8 for the rest of a CTA, one an SM. (2 x 2048
+  // queries over 4096 tokens, 16 heads on 4: 154 us for 647; 8 x 16 over 4096, 32 on 8: 73 for 63; 1 x 128 over 4096, 16
+  // on 4: 93 for 37.)
+  const int64_t tiles = (rows + kPromptRows - 1) / kPromptRows, wide = (tiles * batch * h.heads + sms - 1) / sms * (tokens / kPromptTokens * 1150 + 8000);
+  if (p.tile_rows == 16 && wide < best) {
+    p.prompt = true;
+    p.tile_rows = kPromptRows, p.tiles = (int)tiles, p.splits = 1, p.memory = false;
+    return p;
   }
   if (p.memory) p.bytes = (size_t)(ctas * p.splits * p.tile_rows) * (h.dim * sizeof(float) + sizeof(float2));
   return p;

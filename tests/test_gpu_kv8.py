@@ -349,6 +349,73 @@ def test_prompts(heads, share, queries, length, window, causal, dim, dtype):
         _check_attention(q, cache, table, lengths, values, window=window, causal=causal)
 
 
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("batch, heads, share, page, queries, capacity, window, causal", [
+    (40, 8, 4, 16, 40, 200, None, True), (40, 8, 4, 64, 33, 130, 50, True), (48, 4, 8, 32, 40, 190, None, False), (30, 8, 1, 64, 200, 260, 70, False),
+    (70, 3, 5, 128, 52, 100, 1, True), (4, 8, 2, 64, 500, 1000, None, True), (3, 8, 4, 16, 300, 1100, 333, True), (1, 4, 16, 1024, 700, 1300, None, True)])
+def test_many_prompts(batch, heads, share, page, queries, capacity, window, causal, dim, dtype):
+    # enough of them for tiles of 256 rows, whose rows begin and end anywhere, before the sequence's start too
+    cache, table, values = _filled(batch, capacity, heads, dim, page, dtype, seed=queries)
+    q = _randn(batch, queries, heads * share, dim, seed=9, dtype=dtype)
+    lengths = torch.randint(0, capacity + 1, (batch,), generator=_gen(7), device="cuda").int()
+    if batch >= 4:
+        lengths[:4] = torch.tensor([capacity, 0, 1, min(capacity, queries - 1)])
+    _check_attention(q, cache, table, lengths, values, window=window, causal=causal)
+
+
+def test_many_prompts_over_pages_that_are_wrong_or_not_finite():
+    batch, heads, dim, queries, n = 40, 8, 64, 40, 200
+    cache, table, values = _filled(batch, n, heads, dim, 16, BF, seed=5)
+    q = _randn(batch, queries, heads * 4, dim, seed=6)
+    lengths = torch.full((batch,), n, dtype=torch.int32, device="cuda")
+    want = qr.kv8_attention(q, cache, table, lengths)
+    seen = qr.kv8_attention(q, cache, table, lengths, window=30)
+    for part in (0, 1):  # a page shows in the queries that see it
+        spoiled = copy.deepcopy(cache)
+        spoiled.range[table[:, 11].long(), :, part] = float("nan")  # tokens 176 to 191
+        got = qr.kv8_attention(q, spoiled, table, lengths)
+        pos = n - queries + torch.arange(queries, device="cuda")
+        assert got[:, pos >= 176].isnan().all() and torch.equal(got[:, pos < 176], want[:, pos < 176])
+    # behind the window anything goes
+    spoiled = copy.deepcopy(cache)
+    spoiled.range[table[:, :8].long()] = float("nan")
+    gone = table.clone()
+    gone[:, :8] = 2**31 - 1
+    assert torch.equal(qr.kv8_attention(q, spoiled, table, lengths, window=30), seen)
+    assert torch.equal(qr.kv8_attention(q, spoiled, gone, lengths, window=30), seen)
+    # a page that the table has wrong is left out, and reported
+    gone = table.clone()
+    gone[:, 3] = -1
+    got = qr.kv8_attention(q, cache, gone, lengths, causal=False)
+    torch.cuda.synchronize()
+    with pytest.raises(QRB200Error):
+        qr.kv8_attention(q, cache, table, lengths)
+    without = [torch.cat([v[:, :48], v[:, 64:n]], 1) for v in values]
+    for b in (0, 39):
+        k, v = (x[b].repeat_interleave(4, 1) for x in without)
+        p = torch.softmax(torch.einsum("qhd,thd->hqt", q[b].double(), k) * dim**-0.5, -1)
+        exact = torch.einsum("hqt,thd->qhd", p, v)
+        size = torch.einsum("hqt,thd->qhd", p, v.abs())
+        assert torch.all((got[b].double() - exact).abs() <= U[BF] * exact.abs() + 2.0**-9 * size)
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_many_prompts_with_large_scores_and_ranges(dtype):
+    batch, heads, dim, queries, n = 40, 8, 128, 40, 160
+    for size in (2.0**30, 2.0**-30) if dtype == BF else (2.0**5, 2.0**-9):
+        cache, table, _ = _filled(batch, n, heads, dim, 32, dtype, seed=8)
+        grow = torch.exp2(torch.randint(-6, 6, cache.range.shape, generator=_gen(1), device="cuda").float())
+        cache.range.mul_(grow)
+        cache.range[..., 0] *= size
+        cache.range[table[:, 1].long(), :, 1] = 0.0
+        values = _values_of_codes(cache, table, n)
+        q = (_randn(batch, queries, heads * 4, dim, seed=6, dtype=torch.float32, size=0.3) / (size if dtype == BF or size < 1 else 1)).to(dtype)
+        q[..., 5] *= 64
+        q[3, 7] = 0
+        _check_attention(q, cache, table, torch.full((batch,), n, dtype=torch.int32, device="cuda"), values)
+
+
 @pytest.mark.parametrize("queries, share", [(1, 4), (3, 8), (150, 2)])
 def test_long_context_and_wide_table(queries, share):
     cache, table, values = _filled(2, 20000, 1, 128, 64, BF, seed=3)
