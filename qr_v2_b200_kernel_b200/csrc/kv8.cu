@@ -141,11 +141,14 @@ int qrb200_kv8_write(void* codes, float* range, const qrb200_kv8_shape* shape, c
     LaunchShape l(dim3(ceil_div(tokens, 256)), 256, 0, s);
     if (cudaLaunchKernelEx(&l.cfg, kv8_rows_kernel, p) != cudaSuccess) return QRB200_ERR_CUDA;
     qrb200_internal_count_launch();
-    p.chunk = 32;
+    p.chunk = 64;
   }
+  // 16-byte loads where every (token, head) starts on such a boundary.
+  const bool vec = ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15u) == 0 &&
+                   ((k_token_stride | k_head_stride | v_token_stride | v_head_stride) & 7) == 0;
   const cudaError_t e = with_shape(shape->dtype, h.dim, [&](auto type, auto dim) {
     LaunchShape l(dim3(ceil_div(tokens, p.chunk), h.heads), 256, 0, s);
-    return cudaLaunchKernelEx(&l.cfg, kv8_write_kernel<decltype(type), dim()>, p);
+    return cudaLaunchKernelEx(&l.cfg, vec ? kv8_write_kernel<decltype(type), dim(), true> : kv8_write_kernel<decltype(type), dim(), false>, p);
   });
   if (e != cudaSuccess) return QRB200_ERR_CUDA;
   return launched();
@@ -165,7 +168,7 @@ int qrb200_kv8_read(const void* codes, const float* range, const qrb200_kv8_shap
                       reinterpret_cast<const long long*>(slots), nullptr, tokens, 0, 0, 0, 0, h, 1};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const cudaError_t e = with_shape(shape->dtype, h.dim, [&](auto type, auto dim) {
-    LaunchShape l(dim3(ceil_div(tokens, 2048 / h.dim), h.heads), 256, 0, s);
+    LaunchShape l(dim3(ceil_div((tokens + 15) / 16 * h.heads, 8)), 256, 0, s);
     return cudaLaunchKernelEx(&l.cfg, kv8_read_kernel<decltype(type), dim()>, p);
   });
   if (e != cudaSuccess) return QRB200_ERR_CUDA;

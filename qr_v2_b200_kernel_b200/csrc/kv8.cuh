@@ -87,16 +87,51 @@ __global__ void __launch_bounds__(256) kv8_rows_kernel(Kv8IoParams P) {
   if (r < P.tokens && kv8_page(P, P.slots[r]) >= 0) P.rows[P.slots[r]] = (int)r;
 }
 
+// Threads and bytes. In a run of 16 tokens thread (chunk, t) holds channels 8 chunk to 8 chunk + 7 of tokens 2t, 2t + 1,
+// 2t + 8, 2t + 9: of the values whole words then, one a channel, 64 bytes apart, and of each key two words, 16 bytes apart.
+__device__ __forceinline__ int kv8_token(int t, int i) { return 2 * t + (i & 1) + 8 * (i >> 1); }
+
+// The largest magnitude of sixteen-bit numbers, as their bits: ordered as whole numbers, NaN above infinity.
+__device__ __forceinline__ uint32_t kv8_top(uint32_t top, const uint4& x) {
+  top = __vmaxu2(__vmaxu2(top, x.x & 0x7fff7fffu), x.y & 0x7fff7fffu);
+  return __vmaxu2(__vmaxu2(top, x.z & 0x7fff7fffu), x.w & 0x7fff7fffu);
+}
+template <typename T>
+__device__ __forceinline__ unsigned kv8_top_bits(uint32_t pair) {  // of a 32-bit float
+  const uint16_t top = (uint16_t)max(pair & 0xffffu, pair >> 16);
+  return __float_as_uint(to_f32(reinterpret_cast<const T&>(top)));
+}
+// Eight numbers to bytes code + 128, in the low bytes of floats: x inv + 128, under the exponent of 2^23, rounded once.
+template <typename T>
+__device__ __forceinline__ void kv8_bytes(uint32_t (&f)[8], const uint4& x, float inv) {
+  const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 two = make_float2(to_f32(reinterpret_cast<const T*>(&w[i])[0]), to_f32(reinterpret_cast<const T*>(&w[i])[1]));
+    f[2 * i] = __float_as_uint(fmaf(two.x, inv, 0x1.8p23f + 128.f));
+    f[2 * i + 1] = __float_as_uint(fmaf(two.y, inv, 0x1.8p23f + 128.f));
+  }
+}
+__device__ __forceinline__ uint32_t kv8_word(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {  // of low bytes
+  return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
+}
+
 // A CTA takes a stretch of rows and a head. Rows of one page are written by one CTA, whichever holds the
 // lowest of them, so that nothing is shared: it finds all of the page's rows (s_row: the row of each
-// slot), their largest magnitude, moves the older codes if the range grew, and writes the new ones.
-template <typename T, int kDim>
+// slot), their largest magnitude, and puts the runs that change together in shared memory, 64 tokens at a time: the
+// older codes, moved if the range grew, and the new ones over them. Up to 64 tokens a page, everything is read once.
+// 32768 tokens x 8 heads x 128 channels, bf16: see kv8_rows_kernel for what comes before.
+template <typename T, int kDim, bool kVec>
 __global__ void __launch_bounds__(256) kv8_write_kernel(Kv8IoParams P) {
-  constexpr int kSpan = kDim / 8, kAtOnce = 256 / kSpan;  // threads of a token, tokens at a time
+  constexpr int kChunks = kDim / 8, kRunThreads = 4 * kChunks;  // threads of a run
+  constexpr int kRuns = 256 / kRunThreads;                      // runs at a time: 4, or 8 with 64 channels
+  constexpr int kRun = 32 * kDim;
+  __shared__ uint4 s_image[kRuns * kRun / 16];
   __shared__ int s_row[1024];
   __shared__ unsigned s_low[8], s_top[2][8];
   griddep_launch_wait();
-  const int head = blockIdx.y, tid = threadIdx.x, warp = tid >> 5, c0 = 8 * (tid % kSpan);
+  const int head = blockIdx.y, tid = threadIdx.x, warp = tid >> 5;
+  const int t = tid & 3, chunk = (tid >> 2) % kChunks, mine = tid / kRunThreads;  // this thread's run of those at a time
   const long long row0 = (long long)blockIdx.x * P.chunk, row1 = min(P.tokens, row0 + P.chunk);
   for (long long r = row0; r < row1;) {
     const long long page = kv8_page(P, P.slots[r]);
@@ -105,11 +140,9 @@ __global__ void __launch_bounds__(256) kv8_write_kernel(Kv8IoParams P) {
       ++r;
       continue;
     }
-    long long end = r + 1;
-    while (end < row1 && kv8_page(P, P.slots[end]) == page) ++end;
-    // The rows of the page's slots, and the lowest of them.
+    // The rows of the page's slots, and the lowest of them; where this stretch leaves the page.
     __syncthreads();  // the page before is done
-    unsigned low = 0xffffffffu;
+    unsigned low = 0xffffffffu, end = (unsigned)(row1 - r);
     if (P.rows) {
       for (int j = tid; j < P.sh.page; j += 256) {
         const long long slot = (page << P.sh.shift) + j;
@@ -121,110 +154,226 @@ __global__ void __launch_bounds__(256) kv8_write_kernel(Kv8IoParams P) {
     } else {
       for (int j = tid; j < P.sh.page; j += 256) s_row[j] = -1;
       __syncthreads();
-      for (int at = tid; at < P.tokens; at += 256)
-        if (kv8_page(P, P.slots[at]) == page) {
-          atomicMax(&s_row[(int)P.slots[at] & (P.sh.page - 1)], at);
+      for (int at = tid; at < P.tokens; at += 256) {
+        const long long slot = P.slots[at];
+        if (kv8_page(P, slot) == page) {
+          atomicMax(&s_row[(int)slot & (P.sh.page - 1)], at);
           low = min(low, (unsigned)at);
         }
+      }
     }
+    for (long long i = r + 1 + (tid & 31); i < row1; i += 32)
+      if (kv8_page(P, P.slots[i]) != page) {
+        end = (unsigned)(i - r);
+        break;
+      }
+    end = __reduce_min_sync(kFullMask, end);
     low = __reduce_min_sync(kFullMask, low);
     if ((tid & 31) == 0) s_low[warp] = low;
     __syncthreads();
     low = __reduce_min_sync(kFullMask, s_low[tid & 7]);
-    const bool leads = low >= r && low < end;
-    r = end;
+    const bool leads = low >= r && low < r + end;
+    r += end;
     if (!leads) continue;
-    unsigned top[2] = {0, 0};
-    const auto each = [&](auto f) {
-      for (int j = tid / kSpan; j < P.sh.page; j += kAtOnce) {
-        const int row = s_row[j];
-        if (row < 0) continue;
-        const T* from[2] = {static_cast<const T*>(P.k) + row * P.k_ts + head * P.k_hs + c0,
-                            static_cast<const T*>(P.v) + row * P.v_ts + head * P.v_hs + c0};
+    const int runs = P.sh.page / 16;
+    uint4 x[2][4];  // this thread's tokens of a run: keys, values
+    int rows[4];
+    const auto fetch = [&](int run) {
 #pragma unroll
-        for (int part = 0; part < 2; ++part)
+      for (int i = 0; i < 4; ++i) rows[i] = run < runs ? s_row[16 * run + kv8_token(t, i)] : -1;
 #pragma unroll
-          for (int e = 0; e < 8; ++e) f(part, j, e, to_f32(from[part][e]));
-      }
+      for (int part = 0; part < 2; ++part)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          x[part][i] = make_uint4(0, 0, 0, 0);
+          if (rows[i] >= 0) {
+            const T* from = part ? static_cast<const T*>(P.v) + rows[i] * P.v_ts + head * P.v_hs : static_cast<const T*>(P.k) + rows[i] * P.k_ts + head * P.k_hs;
+            if constexpr (kVec) {
+              x[part][i] = __ldg(reinterpret_cast<const uint4*>(from + 8 * chunk));
+            } else {
+              alignas(16) T y[8];
+#pragma unroll
+              for (int e = 0; e < 8; ++e) y[e] = from[8 * chunk + e];
+              x[part][i] = *reinterpret_cast<const uint4*>(y);
+            }
+          }
+        }
     };
-    each([&](int part, int, int, float x) { top[part] = max(top[part], __float_as_uint(x) & 0x7fffffffu); });
+    uint32_t top[2] = {0, 0};
+    for (int base = 0; base < runs; base += kRuns) {
+      fetch(base + mine);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) top[0] = kv8_top(top[0], x[0][i]), top[1] = kv8_top(top[1], x[1][i]);
+    }
 #pragma unroll
     for (int part = 0; part < 2; ++part) {
-      top[part] = __reduce_max_sync(kFullMask, top[part]);
-      if ((tid & 31) == 0) s_top[part][warp] = top[part];
+      const unsigned most = __reduce_max_sync(kFullMask, kv8_top_bits<T>(top[part]));
+      if ((tid & 31) == 0) s_top[part][warp] = most;
     }
     __syncthreads();
     float* range = P.range + (page * P.sh.heads + head) * 2;
     unsigned char* block = P.codes + (page * P.sh.heads + head) * P.sh.block_bytes();
     const bool fresh = s_row[0] >= 0;
-    float old[2], now[2];
+    float old[2], now[2], inv[2];
 #pragma unroll
     for (int part = 0; part < 2; ++part) {
       const float grown = kv8_range<T>(__reduce_max_sync(kFullMask, s_top[part][tid & 7]));
       old[part] = fresh ? 0.f : range[part];
       now[part] = grown == grown && old[part] == old[part] ? fmaxf(grown, old[part]) : __int_as_float(0x7fffffff);
+      inv[part] = now[part] > 0.f ? kv8_inverse(now[part]) : 0.f;
     }
+    const bool move[2] = {now[0] == now[0] && (fresh || now[0] != old[0]), now[1] == now[1] && (fresh || now[1] != old[1])};
     __syncthreads();  // every thread has read the older range
     if (tid < 2) range[tid] = now[tid];
-    // Older codes to the new range (its quotient with the ranges 2^-8 of theirs, whose product with a code
-    // is finite, and exact): 16 bytes at a time, keys and values in runs of 16 tokens.
-    for (int at = tid; at < P.sh.block_bytes() / 16; at += 256) {
-      const int part = at / kDim & 1;
-      if (now[part] != now[part] || (!fresh && now[part] == old[part])) continue;
-      uint4 w = make_uint4(kKv8Zeros, kKv8Zeros, kKv8Zeros, kKv8Zeros);
-      if (old[part] > 0.f) {
-        w = reinterpret_cast<const uint4*>(block)[at];
-        uint32_t* word = reinterpret_cast<uint32_t*>(&w);
+    unsigned char* image = reinterpret_cast<unsigned char*>(s_image);
+    for (int base = 0; base < runs; base += kRuns) {
+      if (runs > kRuns) fetch(base + mine);
+      const bool any = rows[0] >= 0 || rows[1] >= 0 || rows[2] >= 0 || rows[3] >= 0;
+      const bool all = rows[0] >= 0 && rows[1] >= 0 && rows[2] >= 0 && rows[3] >= 0;
+      // Of each run, whether it is written at all and whether it is filled (a run's threads are whole warps).
+      const int count = __syncthreads_count(any);
+      if (count == 0 && !move[0] && !move[1]) continue;
+      const bool filled = __syncthreads_and(all || base + mine >= runs);
+      if (!filled) {
+        // The older codes first, moved to the new range (its quotient with the ranges 2^-8 of theirs, whose
+        // product with a code is finite, and exact), or zeros.
+        for (int at = tid; at < kRuns * kRun / 16; at += 256) {
+          if (base + at * 16 / kRun >= runs) break;
+          const int part = at / kDim & 1;
+          uint4 w = make_uint4(kKv8Zeros, kKv8Zeros, kKv8Zeros, kKv8Zeros);
+          if (!move[part] || old[part] > 0.f) w = reinterpret_cast<const uint4*>(block + (long long)base * kRun)[at];
+          if (move[part] && old[part] > 0.f) {
+            uint32_t* word = reinterpret_cast<uint32_t*>(&w);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              uint32_t next = 0;
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const int c = (int)(word[i] >> (8 * e) & 255) - 128;
+                next |= (uint32_t)(__float2int_rn(__fdiv_rn((float)c * (old[part] * 0x1p-8f), now[part] * 0x1p-8f)) + 128) << (8 * e);
+              }
+              word[i] = next;
+            }
+          }
+          s_image[at] = w;
+        }
+        __syncthreads();
+      }
+      if (any) {
+        unsigned char* run = image + mine * kRun;
+        uint32_t f[4][8];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          uint32_t next = 0;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int c = (int)(word[i] >> (8 * e) & 255) - 128;
-            next |= (uint32_t)(__float2int_rn(__fdiv_rn((float)c * (old[part] * 0x1p-8f), now[part] * 0x1p-8f)) + 128) << (8 * e);
+          kv8_bytes<T>(f[i], x[0][i], inv[0]);
+          if (rows[i] >= 0) {
+            uint32_t* to = reinterpret_cast<uint32_t*>(run + kv8_key_at(kDim, kv8_token(t, i), 8 * chunk));
+            to[0] = kv8_word(f[i][0], f[i][1], f[i][2], f[i][3]);
+            to[4] = kv8_word(f[i][4], f[i][5], f[i][6], f[i][7]);
           }
-          word[i] = next;
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) kv8_bytes<T>(f[i], x[1][i], inv[1]);
+        unsigned char* to = run + kv8_value_at(kDim, 2 * t, 8 * chunk);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          if (all) {
+            *reinterpret_cast<uint32_t*>(to + 64 * e) = kv8_word(f[0][e], f[1][e], f[2][e], f[3][e]);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (rows[i] >= 0) to[64 * e + i] = (unsigned char)f[i][e];
+          }
         }
       }
-      reinterpret_cast<uint4*>(block)[at] = w;
+      __syncthreads();
+      for (int at = tid; at < kRuns * kRun / 16; at += 256) {
+        if (base + at * 16 / kRun >= runs) break;
+        reinterpret_cast<uint4*>(block + (long long)base * kRun)[at] = s_image[at];
+      }
+      __syncthreads();  // the image is free
     }
-    __syncthreads();  // before the new codes go into the same words
-    const float inv[2] = {now[0] > 0.f ? kv8_inverse(now[0]) : 0.f, now[1] > 0.f ? kv8_inverse(now[1]) : 0.f};
-    each([&](int part, int j, int e, float x) {
-      const int code = inv[part] > 0.f ? __float2int_rn(x * inv[part]) : 0;
-      block[part ? kv8_value_at(kDim, j, c0 + e) : kv8_key_at(kDim, j, c0 + e)] = (unsigned char)(code + 128);
-    });
   }
 }
 
-// The values at slots; a negative slot reads as zeros. Eight channels to a thread.
+// The values at slots; a negative slot reads as zeros. A warp takes 16 rows of a head: a whole run, as sequences are read, goes
+// through shared memory, other rows come as they lie.
 template <typename T, int kDim>
 __global__ void __launch_bounds__(256) kv8_read_kernel(Kv8IoParams P) {
-  constexpr int kSpan = kDim / 8, kAtOnce = 256 / kSpan;
+  constexpr int kRun = 32 * kDim;
+  __shared__ uint4 s_run[8][kRun / 16];
   griddep_launch_wait();
-  const long long row = (long long)blockIdx.x * kAtOnce + threadIdx.x / kSpan;
-  const int head = blockIdx.y, c0 = 8 * (threadIdx.x % kSpan);
-  if (row >= P.tokens) return;
-  const long long slot = P.slots[row], page = kv8_page(P, slot);
-  if (page < 0 && slot >= 0 && head == 0 && c0 == 0) report_device_failure(kSiteIndex);
-  const int j = (int)slot & (P.sh.page - 1);
-  const long long at = page < 0 ? 0 : page * P.sh.heads + head;
-  const unsigned char* block = P.codes + at * P.sh.block_bytes();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, t = lane & 3;
+  const long long unit = (long long)blockIdx.x * 8 + warp, first = unit / P.sh.heads * 16;
+  const int head = (int)(unit % P.sh.heads);
+  if (first >= P.tokens) return;
+  const long long slot = lane < 16 && first + lane < P.tokens ? P.slots[first + lane] : -1, slot0 = __shfl_sync(kFullMask, slot, 0);
+  if (slot >= 0 && kv8_page(P, slot) < 0 && head == 0) report_device_failure(kSiteIndex);
+  const bool whole = __all_sync(kFullMask, lane >= 16 || slot == slot0 + lane) && (slot0 & 15) == 0 && kv8_page(P, slot0) >= 0;
+  const auto place = [&](long long s, float2& step) {  // the run that holds a slot
+    const long long page = kv8_page(P, s);
+    if (page < 0) return static_cast<const unsigned char*>(nullptr);
+    const float2 r = __ldg(reinterpret_cast<const float2*>(P.range) + page * P.sh.heads + head);
+    step = make_float2(kv8_step(r.x), kv8_step(r.y));
+    return static_cast<const unsigned char*>(P.codes) + (page * P.sh.heads + head) * P.sh.block_bytes() + ((int)s & (P.sh.page - 1)) / 16 * kRun;
+  };
+  const auto value = [&](uint32_t w, int e) {  // of byte e
+    return __uint_as_float(__byte_perm(w, 0x4b000000u, 0x7440 + e)) - 8388736.f;
+  };
+  if (whole) {
+    float2 step;
+    const unsigned char* run = place(slot0, step);
 #pragma unroll
-  for (int part = 0; part < 2; ++part) {
-    alignas(16) T out[8];
-    const float step = page < 0 ? 0.f : kv8_step(P.range[at * 2 + part]);
+    for (int i = 0; i < kRun / 512; ++i) s_run[warp][32 * i + lane] = __ldg(reinterpret_cast<const uint4*>(run) + 32 * i + lane);
+    __syncwarp();
+    const unsigned char* bytes = reinterpret_cast<const unsigned char*>(s_run[warp]);
 #pragma unroll
-    for (int e = 0; e < 8; e += 2) {
-      float c[2] = {0.f, 0.f};
-      if (page >= 0)
+    for (int chunk = lane >> 2; chunk < kDim / 8; chunk += 8) {
+      uint32_t v[8];
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
-          c[i] = (float)((int)block[part ? kv8_value_at(kDim, j, c0 + e + i) : kv8_key_at(kDim, j, c0 + e + i)] - 128);
-      put2(out + e, c[0] * step, c[1] * step);
+      for (int e = 0; e < 8; ++e) v[e] = *reinterpret_cast<const uint32_t*>(bytes + kv8_value_at(kDim, 2 * t, 8 * chunk) + 64 * e);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int token = kv8_token(t, i);
+        const uint32_t* from = reinterpret_cast<const uint32_t*>(bytes + kv8_key_at(kDim, token, 8 * chunk));
+        const uint32_t k[2] = {from[0], from[4]};
+        alignas(16) T out[8];
+        const long long at = ((first + token) * P.sh.heads + head) * kDim + 8 * chunk;
+#pragma unroll
+        for (int e = 0; e < 8; e += 2) put2(out + e, value(k[e >> 2], e & 3) * step.x, value(k[e >> 2], (e & 3) + 1) * step.x);
+        *reinterpret_cast<uint4*>(static_cast<T*>(P.k_out) + at) = *reinterpret_cast<const uint4*>(out);
+#pragma unroll
+        for (int e = 0; e < 8; e += 2) put2(out + e, value(v[e], i) * step.y, value(v[e + 1], i) * step.y);
+        *reinterpret_cast<uint4*>(static_cast<T*>(P.v_out) + at) = *reinterpret_cast<const uint4*>(out);
+      }
     }
-    *reinterpret_cast<uint4*>(static_cast<T*>(part ? P.v_out : P.k_out) + (row * P.sh.heads + head) * kDim + c0) =
-        *reinterpret_cast<const uint4*>(out);
+    return;
+  }
+  // Each row's place and steps at once, then eight channels of a row to a lane.
+  float2 step = make_float2(0.f, 0.f);
+  const unsigned char* run = place(slot, step);
+  constexpr int kSpan = kDim / 8;
+#pragma unroll 4
+  for (int i = 0; i < 16 * kSpan / 32; ++i) {
+    const int token = (32 * i + lane) / kSpan, c0 = 8 * (lane % kSpan);
+    const int j = __shfl_sync(kFullMask, (int)slot & 15, token);
+    const unsigned char* from = reinterpret_cast<const unsigned char*>(__shfl_sync(kFullMask, reinterpret_cast<unsigned long long>(run), token));
+    const float key = __shfl_sync(kFullMask, step.x, token), other = __shfl_sync(kFullMask, step.y, token);
+    uint32_t k[2] = {kKv8Zeros, kKv8Zeros}, v[8];
+    if (from) {
+      const uint32_t* keys = reinterpret_cast<const uint32_t*>(from + kv8_key_at(kDim, j, c0));
+      k[0] = __ldg(keys), k[1] = __ldg(keys + 4);
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = from ? (uint32_t)__ldg(from + kv8_value_at(kDim, j, c0) + 64 * e) : 128u;
+    if (first + token >= P.tokens) continue;
+    alignas(16) T out[8];
+    const long long at = ((first + token) * P.sh.heads + head) * kDim + c0;
+#pragma unroll
+    for (int e = 0; e < 8; e += 2) put2(out + e, value(k[e >> 2], e & 3) * key, value(k[e >> 2], (e & 3) + 1) * key);
+    *reinterpret_cast<uint4*>(static_cast<T*>(P.k_out) + at) = *reinterpret_cast<const uint4*>(out);
+#pragma unroll
+    for (int e = 0; e < 8; e += 2) put2(out + e, value(v[e], 0) * other, value(v[e + 1], 0) * other);
+    *reinterpret_cast<uint4*>(static_cast<T*>(P.v_out) + at) = *reinterpret_cast<const uint4*>(out);
   }
 }
 
