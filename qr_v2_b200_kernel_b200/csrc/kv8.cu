@@ -135,20 +135,29 @@ int qrb200_kv8_write(void* codes, float* range, const qrb200_kv8_shape* shape, c
     return QRB200_ERR_WORKSPACE;
   Kv8IoParams p{static_cast<unsigned char*>(codes), range, k, v, nullptr, nullptr, reinterpret_cast<const long long*>(slots),
                 need > 0 ? static_cast<int*>(workspace) : nullptr, tokens, k_token_stride, k_head_stride, v_token_stride,
-                v_head_stride, h, 1};
+                v_head_stride, h, 1, 1};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (p.rows) {
     LaunchShape l(dim3(ceil_div(tokens, 256)), 256, 0, s);
     if (cudaLaunchKernelEx(&l.cfg, kv8_rows_kernel, p) != cudaSuccess) return QRB200_ERR_CUDA;
     qrb200_internal_count_launch();
+    // As many heads to a CTA as leave four to an SM: the rows' look-up is shared, and the next head's loads are under way
+    // while one's bytes leave.
     p.chunk = 64;
+    p.span = (int)std::max<int64_t>(1, std::min<int64_t>(h.heads, (tokens + 63) / 64 * h.heads / (4 * sm_count())));
+    p.span = ceil_div(h.heads, ceil_div(h.heads, p.span));  // evenly
   }
   // 16-byte loads where every (token, head) starts on such a boundary.
   const bool vec = ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15u) == 0 &&
                    ((k_token_stride | k_head_stride | v_token_stride | v_head_stride) & 7) == 0;
   const cudaError_t e = with_shape(shape->dtype, h.dim, [&](auto type, auto dim) {
-    LaunchShape l(dim3(ceil_div(tokens, p.chunk), h.heads), 256, 0, s);
-    return cudaLaunchKernelEx(&l.cfg, vec ? kv8_write_kernel<decltype(type), dim(), true> : kv8_write_kernel<decltype(type), dim(), false>, p);
+    using E = decltype(type);
+    if (!p.rows) {
+      LaunchShape l(dim3((unsigned)tokens, ceil_div(h.heads, 8)), 256, 0, s);
+      return cudaLaunchKernelEx(&l.cfg, vec ? kv8_write_few_kernel<E, dim(), true> : kv8_write_few_kernel<E, dim(), false>, p);
+    }
+    LaunchShape l(dim3(ceil_div(tokens, p.chunk), ceil_div(h.heads, p.span)), 2 * h.dim, 0, s);
+    return cudaLaunchKernelEx(&l.cfg, vec ? kv8_write_kernel<E, dim(), true> : kv8_write_kernel<E, dim(), false>, p);
   });
   if (e != cudaSuccess) return QRB200_ERR_CUDA;
   return launched();
@@ -165,7 +174,7 @@ int qrb200_kv8_read(const void* codes, const float* range, const qrb200_kv8_shap
   const int st = quant_ready();
   if (st != QRB200_OK) return st;
   const Kv8IoParams p{static_cast<unsigned char*>(const_cast<void*>(codes)), const_cast<float*>(range), nullptr, nullptr, k, v,
-                      reinterpret_cast<const long long*>(slots), nullptr, tokens, 0, 0, 0, 0, h, 1};
+                      reinterpret_cast<const long long*>(slots), nullptr, tokens, 0, 0, 0, 0, h, 1, 1};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const cudaError_t e = with_shape(shape->dtype, h.dim, [&](auto type, auto dim) {
     LaunchShape l(dim3(ceil_div((tokens + 15) / 16 * h.heads, 8)), 256, 0, s);

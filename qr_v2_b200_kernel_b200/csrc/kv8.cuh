@@ -45,7 +45,7 @@ struct Kv8IoParams {
   int* rows;  // workspace: a slot's row of this call, where there are many
   long long tokens, k_ts, k_hs, v_ts, v_hs;  // strides in elements
   Kv8Shape sh;
-  int chunk;  // rows of a CTA
+  int chunk, span;  // rows and heads of a CTA
 };
 
 // Offsets of a token's code within its block: of channel c, as a key and as a value.
@@ -59,7 +59,7 @@ __device__ __forceinline__ int kv8_value_at(int dim, int token, int c) {
 }
 
 constexpr uint32_t kKv8Zeros = 0x80808080u;
-constexpr int kKv8Few = 1024;  // rows up to which a CTA looks a page's rows up among all of them
+constexpr int kKv8Few = 1024;  // rows up to which a page's are looked up among all of them
 
 // Three significant bits, rounded up, of a magnitude's bits (the magnitude itself where that would pass the type's
 // largest number, so that no value reads back as infinity); NaN for what is not finite.
@@ -116,21 +116,149 @@ __device__ __forceinline__ uint32_t kv8_word(uint32_t a, uint32_t b, uint32_t c,
   return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
 }
 
-// A CTA takes a stretch of rows and a head. Rows of one page are written by one CTA, whichever holds the
+// The older codes of a page and head to a new range: their quotient with the ranges 2^-8 of theirs, whose product with
+// a code is finite, and exact.
+__device__ __forceinline__ uint32_t kv8_moved(uint32_t word, float old, float now) {
+  uint32_t next = 0;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const int c = (int)(word >> (8 * e) & 255) - 128;
+    next |= (uint32_t)(__float2int_rn(__fdiv_rn((float)c * (old * 0x1p-8f), now * 0x1p-8f)) + 128) << (8 * e);
+  }
+  return next;
+}
+
+// Up to kKv8Few rows: a CTA to a row, a warp to a head. A page is written by the CTA of the lowest of its rows, which finds the
+// others among all. Tokens one by one, four channels to a lane, and bytes stored where they belong, since a step of decoding
+// brings a page one: 64 tokens x 8 heads 3.7 us (with the kernel below 11.2), 256 5.0 (35).
+template <typename T, int kDim, bool kVec>
+__global__ void __launch_bounds__(256) kv8_write_few_kernel(Kv8IoParams P) {
+  constexpr int kPer = kDim / 32;  // channels of a lane: 4, or 2
+  __shared__ int s_row[1024];
+  __shared__ unsigned s_low[8];
+  griddep_launch_wait();
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, r = blockIdx.x, head = blockIdx.y * 8 + warp;
+  const long long page = kv8_page(P, P.slots[r]);
+  if (page < 0) {
+    if (P.slots[r] >= 0 && tid == 0) report_device_failure(kSiteIndex);
+    return;
+  }
+  for (int j = tid; j < P.sh.page; j += 256) s_row[j] = -1;
+  __syncthreads();
+  unsigned low = 0xffffffffu;
+  for (int at = tid; at < P.tokens; at += 256) {
+    const long long slot = P.slots[at];
+    if (kv8_page(P, slot) == page) {
+      atomicMax(&s_row[(int)slot & (P.sh.page - 1)], at);
+      low = min(low, (unsigned)at);
+    }
+  }
+  low = __reduce_min_sync(kFullMask, low);
+  if (lane == 0) s_low[warp] = low;
+  __syncthreads();
+  low = __reduce_min_sync(kFullMask, s_low[lane & 7]);
+  if (low != (unsigned)r || head >= P.sh.heads) return;
+  const int c0 = kPer * lane;
+  const auto load = [&](T(&x)[2][kPer], int row) {
+#pragma unroll
+    for (int part = 0; part < 2; ++part) {
+      const T* from = (part ? static_cast<const T*>(P.v) + row * P.v_ts + head * P.v_hs : static_cast<const T*>(P.k) + row * P.k_ts + head * P.k_hs) + c0;
+      if constexpr (kVec && kPer == 4) {
+        *reinterpret_cast<uint2*>(x[part]) = __ldg(reinterpret_cast<const uint2*>(from));
+      } else if constexpr (kVec) {
+        *reinterpret_cast<uint32_t*>(x[part]) = __ldg(reinterpret_cast<const uint32_t*>(from));
+      } else {
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) x[part][e] = from[e];
+      }
+    }
+  };
+  // f(token, row) for the page's new tokens, eight at a time.
+  const auto each = [&](auto f) {
+    for (int base = 0; base < P.sh.page; base += 32) {
+      const int mine = base + lane < P.sh.page ? s_row[base + lane] : -1;
+      unsigned have = __ballot_sync(kFullMask, mine >= 0);
+      while (have) {
+        alignas(8) T x[4][2][kPer];
+        int token[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          token[i] = have ? __ffs(have) - 1 : -1;
+          have &= have - 1;
+          if (token[i] >= 0) load(x[i], __shfl_sync(kFullMask, mine, token[i]));
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (token[i] >= 0) f(base + token[i], x[i]);
+      }
+    }
+  };
+  unsigned top[2] = {0, 0};
+  each([&](int, const T(&x)[2][kPer]) {
+#pragma unroll
+    for (int part = 0; part < 2; ++part)
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) top[part] = max(top[part], __float_as_uint(to_f32(x[part][e])) & 0x7fffffffu);
+  });
+  float* range = P.range + (page * P.sh.heads + head) * 2;
+  unsigned char* block = P.codes + (page * P.sh.heads + head) * P.sh.block_bytes();
+  const bool fresh = s_row[0] >= 0;
+  float old[2], now[2], inv[2];
+  bool move[2];
+#pragma unroll
+  for (int part = 0; part < 2; ++part) {
+    const float grown = kv8_range<T>(__reduce_max_sync(kFullMask, top[part]));
+    old[part] = fresh ? 0.f : range[part];
+    now[part] = grown == grown && old[part] == old[part] ? fmaxf(grown, old[part]) : __int_as_float(0x7fffffff);
+    inv[part] = now[part] > 0.f ? kv8_inverse(now[part]) : 0.f;
+    move[part] = now[part] == now[part] && (fresh || now[part] != old[part]);
+  }
+  __syncwarp();  // every lane has read the older range
+  if (lane < 2) range[lane] = now[lane];
+  if (move[0] || move[1]) {
+#pragma unroll 4
+    for (int at = lane; at < P.sh.block_bytes() / 16; at += 32) {
+      const int part = at / kDim & 1;
+      if (!move[part]) continue;
+      uint4 w = make_uint4(kKv8Zeros, kKv8Zeros, kKv8Zeros, kKv8Zeros);
+      if (old[part] > 0.f) {
+        w = reinterpret_cast<const uint4*>(block)[at];
+        w = make_uint4(kv8_moved(w.x, old[part], now[part]), kv8_moved(w.y, old[part], now[part]), kv8_moved(w.z, old[part], now[part]),
+                       kv8_moved(w.w, old[part], now[part]));
+      }
+      reinterpret_cast<uint4*>(block)[at] = w;
+    }
+    __syncwarp();  // before the new codes go into the same words
+  }
+  each([&](int token, const T(&x)[2][kPer]) {
+    uint32_t f[2][kPer];
+#pragma unroll
+    for (int part = 0; part < 2; ++part)
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) f[part][e] = __float_as_uint(fmaf(to_f32(x[part][e]), inv[part], 0x1.8p23f + 128.f));
+    unsigned char* key = block + kv8_key_at(kDim, token, c0);
+    if constexpr (kPer == 4) *reinterpret_cast<uint32_t*>(key) = kv8_word(f[0][0], f[0][1], f[0][2], f[0][3]);
+    else *reinterpret_cast<uint16_t*>(key) = (uint16_t)__byte_perm(f[0][0], f[0][1], 0x0040);
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) block[kv8_value_at(kDim, token, c0 + e)] = (unsigned char)f[1][e];
+  });
+}
+
+// More rows: a CTA takes a stretch of them and some heads. Rows of one page are written by one CTA, whichever holds the
 // lowest of them, so that nothing is shared: it finds all of the page's rows (s_row: the row of each
 // slot), their largest magnitude, and puts the runs that change together in shared memory, 64 tokens at a time: the
 // older codes, moved if the range grew, and the new ones over them. Up to 64 tokens a page, everything is read once.
-// 32768 tokens x 8 heads x 128 channels, bf16: see kv8_rows_kernel for what comes before.
+// 32768 tokens x 8 heads x 128 channels, bf16, from a page's first token 61 us, from within one 83.
 template <typename T, int kDim, bool kVec>
-__global__ void __launch_bounds__(256) kv8_write_kernel(Kv8IoParams P) {
+__global__ void __launch_bounds__(2 * kDim) kv8_write_kernel(Kv8IoParams P) {
   constexpr int kChunks = kDim / 8, kRunThreads = 4 * kChunks;  // threads of a run
-  constexpr int kRuns = 256 / kRunThreads;                      // runs at a time: 4, or 8 with 64 channels
+  constexpr int kRuns = 4, kThreads = kRuns * kRunThreads;      // runs at a time
   constexpr int kRun = 32 * kDim;
   __shared__ uint4 s_image[kRuns * kRun / 16];
   __shared__ int s_row[1024];
-  __shared__ unsigned s_low[8], s_top[2][8];
+  __shared__ unsigned s_low[kThreads / 32], s_top[2][kThreads / 32];
   griddep_launch_wait();
-  const int head = blockIdx.y, tid = threadIdx.x, warp = tid >> 5;
+  const int head0 = blockIdx.y * P.span, heads = min(P.span, P.sh.heads - head0), tid = threadIdx.x, warp = tid >> 5;
   const int t = tid & 3, chunk = (tid >> 2) % kChunks, mine = tid / kRunThreads;  // this thread's run of those at a time
   const long long row0 = (long long)blockIdx.x * P.chunk, row1 = min(P.tokens, row0 + P.chunk);
   for (long long r = row0; r < row1;) {
@@ -143,24 +271,12 @@ __global__ void __launch_bounds__(256) kv8_write_kernel(Kv8IoParams P) {
     // The rows of the page's slots, and the lowest of them; where this stretch leaves the page.
     __syncthreads();  // the page before is done
     unsigned low = 0xffffffffu, end = (unsigned)(row1 - r);
-    if (P.rows) {
-      for (int j = tid; j < P.sh.page; j += 256) {
-        const long long slot = (page << P.sh.shift) + j;
-        const int at = P.rows[slot];  // whatever it held before, unless the row says so too
-        const bool is = at >= 0 && at < P.tokens && P.slots[at] == slot;
-        s_row[j] = is ? at : -1;
-        if (is) low = min(low, (unsigned)at);
-      }
-    } else {
-      for (int j = tid; j < P.sh.page; j += 256) s_row[j] = -1;
-      __syncthreads();
-      for (int at = tid; at < P.tokens; at += 256) {
-        const long long slot = P.slots[at];
-        if (kv8_page(P, slot) == page) {
-          atomicMax(&s_row[(int)slot & (P.sh.page - 1)], at);
-          low = min(low, (unsigned)at);
-        }
-      }
+    for (int j = tid; j < P.sh.page; j += kThreads) {
+      const long long slot = (page << P.sh.shift) + j;
+      const int at = P.rows[slot];  // whatever it held before, unless the row says so too
+      const bool is = at >= 0 && at < P.tokens && P.slots[at] == slot;
+      s_row[j] = is ? at : -1;
+      if (is) low = min(low, (unsigned)at);
     }
     for (long long i = r + 1 + (tid & 31); i < row1; i += 32)
       if (kv8_page(P, P.slots[i]) != page) {
@@ -171,14 +287,14 @@ __global__ void __launch_bounds__(256) kv8_write_kernel(Kv8IoParams P) {
     low = __reduce_min_sync(kFullMask, low);
     if ((tid & 31) == 0) s_low[warp] = low;
     __syncthreads();
-    low = __reduce_min_sync(kFullMask, s_low[tid & 7]);
+    low = __reduce_min_sync(kFullMask, s_low[tid & (kThreads / 32 - 1)]);
     const bool leads = low >= r && low < r + end;
     r += end;
     if (!leads) continue;
     const int runs = P.sh.page / 16;
     uint4 x[2][4];  // this thread's tokens of a run: keys, values
     int rows[4];
-    const auto fetch = [&](int run) {
+    const auto fetch = [&](int head, int run) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) rows[i] = run < runs ? s_row[16 * run + kv8_token(t, i)] : -1;
 #pragma unroll
@@ -199,98 +315,91 @@ __global__ void __launch_bounds__(256) kv8_write_kernel(Kv8IoParams P) {
           }
         }
     };
-    uint32_t top[2] = {0, 0};
-    for (int base = 0; base < runs; base += kRuns) {
-      fetch(base + mine);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) top[0] = kv8_top(top[0], x[0][i]), top[1] = kv8_top(top[1], x[1][i]);
-    }
-#pragma unroll
-    for (int part = 0; part < 2; ++part) {
-      const unsigned most = __reduce_max_sync(kFullMask, kv8_top_bits<T>(top[part]));
-      if ((tid & 31) == 0) s_top[part][warp] = most;
-    }
-    __syncthreads();
-    float* range = P.range + (page * P.sh.heads + head) * 2;
-    unsigned char* block = P.codes + (page * P.sh.heads + head) * P.sh.block_bytes();
-    const bool fresh = s_row[0] >= 0;
-    float old[2], now[2], inv[2];
-#pragma unroll
-    for (int part = 0; part < 2; ++part) {
-      const float grown = kv8_range<T>(__reduce_max_sync(kFullMask, s_top[part][tid & 7]));
-      old[part] = fresh ? 0.f : range[part];
-      now[part] = grown == grown && old[part] == old[part] ? fmaxf(grown, old[part]) : __int_as_float(0x7fffffff);
-      inv[part] = now[part] > 0.f ? kv8_inverse(now[part]) : 0.f;
-    }
-    const bool move[2] = {now[0] == now[0] && (fresh || now[0] != old[0]), now[1] == now[1] && (fresh || now[1] != old[1])};
-    __syncthreads();  // every thread has read the older range
-    if (tid < 2) range[tid] = now[tid];
     unsigned char* image = reinterpret_cast<unsigned char*>(s_image);
-    for (int base = 0; base < runs; base += kRuns) {
-      if (runs > kRuns) fetch(base + mine);
-      const bool any = rows[0] >= 0 || rows[1] >= 0 || rows[2] >= 0 || rows[3] >= 0;
-      const bool all = rows[0] >= 0 && rows[1] >= 0 && rows[2] >= 0 && rows[3] >= 0;
-      // Of each run, whether it is written at all and whether it is filled (a run's threads are whole warps).
-      const int count = __syncthreads_count(any);
-      if (count == 0 && !move[0] && !move[1]) continue;
-      const bool filled = __syncthreads_and(all || base + mine >= runs);
-      if (!filled) {
-        // The older codes first, moved to the new range (its quotient with the ranges 2^-8 of theirs, whose
-        // product with a code is finite, and exact), or zeros.
-        for (int at = tid; at < kRuns * kRun / 16; at += 256) {
-          if (base + at * 16 / kRun >= runs) break;
-          const int part = at / kDim & 1;
-          uint4 w = make_uint4(kKv8Zeros, kKv8Zeros, kKv8Zeros, kKv8Zeros);
-          if (!move[part] || old[part] > 0.f) w = reinterpret_cast<const uint4*>(block + (long long)base * kRun)[at];
-          if (move[part] && old[part] > 0.f) {
-            uint32_t* word = reinterpret_cast<uint32_t*>(&w);
+    if (runs <= kRuns) fetch(head0, mine);
+    for (int head = head0; head < head0 + heads; ++head) {
+      uint32_t top[2] = {0, 0};
+      for (int base = 0; base < runs; base += kRuns) {
+        if (runs > kRuns) fetch(head, base + mine);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              uint32_t next = 0;
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const int c = (int)(word[i] >> (8 * e) & 255) - 128;
-                next |= (uint32_t)(__float2int_rn(__fdiv_rn((float)c * (old[part] * 0x1p-8f), now[part] * 0x1p-8f)) + 128) << (8 * e);
-              }
-              word[i] = next;
-            }
-          }
-          s_image[at] = w;
-        }
-        __syncthreads();
+        for (int i = 0; i < 4; ++i) top[0] = kv8_top(top[0], x[0][i]), top[1] = kv8_top(top[1], x[1][i]);
       }
-      if (any) {
-        unsigned char* run = image + mine * kRun;
-        uint32_t f[4][8];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          kv8_bytes<T>(f[i], x[0][i], inv[0]);
-          if (rows[i] >= 0) {
-            uint32_t* to = reinterpret_cast<uint32_t*>(run + kv8_key_at(kDim, kv8_token(t, i), 8 * chunk));
-            to[0] = kv8_word(f[i][0], f[i][1], f[i][2], f[i][3]);
-            to[4] = kv8_word(f[i][4], f[i][5], f[i][6], f[i][7]);
-          }
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) kv8_bytes<T>(f[i], x[1][i], inv[1]);
-        unsigned char* to = run + kv8_value_at(kDim, 2 * t, 8 * chunk);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          if (all) {
-            *reinterpret_cast<uint32_t*>(to + 64 * e) = kv8_word(f[0][e], f[1][e], f[2][e], f[3][e]);
-          } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              if (rows[i] >= 0) to[64 * e + i] = (unsigned char)f[i][e];
-          }
-        }
+      for (int part = 0; part < 2; ++part) {
+        const unsigned most = __reduce_max_sync(kFullMask, kv8_top_bits<T>(top[part]));
+        if ((tid & 31) == 0) s_top[part][warp] = most;
       }
       __syncthreads();
-      for (int at = tid; at < kRuns * kRun / 16; at += 256) {
-        if (base + at * 16 / kRun >= runs) break;
-        reinterpret_cast<uint4*>(block + (long long)base * kRun)[at] = s_image[at];
+      float* range = P.range + (page * P.sh.heads + head) * 2;
+      unsigned char* block = P.codes + (page * P.sh.heads + head) * P.sh.block_bytes();
+      const bool fresh = s_row[0] >= 0;
+      float old[2], now[2], inv[2];
+#pragma unroll
+      for (int part = 0; part < 2; ++part) {
+        const float grown = kv8_range<T>(__reduce_max_sync(kFullMask, s_top[part][tid & (kThreads / 32 - 1)]));
+        old[part] = fresh ? 0.f : range[part];
+        now[part] = grown == grown && old[part] == old[part] ? fmaxf(grown, old[part]) : __int_as_float(0x7fffffff);
+        inv[part] = now[part] > 0.f ? kv8_inverse(now[part]) : 0.f;
       }
-      __syncthreads();  // the image is free
+      const bool move[2] = {now[0] == now[0] && (fresh || now[0] != old[0]), now[1] == now[1] && (fresh || now[1] != old[1])};
+      __syncthreads();  // every thread has read the older range
+      if (tid < 2) range[tid] = now[tid];
+      for (int base = 0; base < runs; base += kRuns) {
+        if (runs > kRuns) fetch(head, base + mine);
+        const bool any = rows[0] >= 0 || rows[1] >= 0 || rows[2] >= 0 || rows[3] >= 0;
+        const bool all = rows[0] >= 0 && rows[1] >= 0 && rows[2] >= 0 && rows[3] >= 0;
+        // Of each run, whether it is written at all and whether it is filled (a run's threads are whole warps).
+        const int count = __syncthreads_count(any);
+        if (count == 0 && !move[0] && !move[1]) continue;  // (never where the page is taken at once)
+        const bool filled = __syncthreads_and(all || base + mine >= runs);
+        if (!filled) {
+          // The older codes first, moved to the new range, or zeros.
+          for (int at = tid; at < kRuns * kRun / 16; at += kThreads) {
+            if (base + at * 16 / kRun >= runs) break;
+            const int part = at / kDim & 1;
+            uint4 w = make_uint4(kKv8Zeros, kKv8Zeros, kKv8Zeros, kKv8Zeros);
+            if (!move[part] || old[part] > 0.f) w = reinterpret_cast<const uint4*>(block + (long long)base * kRun)[at];
+              if (move[part] && old[part] > 0.f)
+              w = make_uint4(kv8_moved(w.x, old[part], now[part]), kv8_moved(w.y, old[part], now[part]), kv8_moved(w.z, old[part], now[part]),
+                             kv8_moved(w.w, old[part], now[part]));
+            s_image[at] = w;
+          }
+          __syncthreads();
+        }
+        if (any) {
+          unsigned char* run = image + mine * kRun;
+          uint32_t f[4][8];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            kv8_bytes<T>(f[i], x[0][i], inv[0]);
+            if (rows[i] >= 0) {
+              uint32_t* to = reinterpret_cast<uint32_t*>(run + kv8_key_at(kDim, kv8_token(t, i), 8 * chunk));
+              to[0] = kv8_word(f[i][0], f[i][1], f[i][2], f[i][3]);
+              to[4] = kv8_word(f[i][4], f[i][5], f[i][6], f[i][7]);
+            }
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i) kv8_bytes<T>(f[i], x[1][i], inv[1]);
+          unsigned char* to = run + kv8_value_at(kDim, 2 * t, 8 * chunk);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            if (all) {
+              *reinterpret_cast<uint32_t*>(to + 64 * e) = kv8_word(f[0][e], f[1][e], f[2][e], f[3][e]);
+            } else {
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                if (rows[i] >= 0) to[64 * e + i] = (unsigned char)f[i][e];
+            }
+          }
+        }
+        __syncthreads();
+        if (runs <= kRuns && head + 1 < head0 + heads) fetch(head + 1, mine);  // under way while this head's bytes leave
+        for (int at = tid; at < kRuns * kRun / 16; at += kThreads) {
+          if (base + at * 16 / kRun >= runs) break;
+          reinterpret_cast<uint4*>(block + (long long)base * kRun)[at] = s_image[at];
+        }
+        __syncthreads();  // the image is free
+      }
     }
   }
 }
