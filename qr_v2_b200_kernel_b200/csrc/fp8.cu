@@ -112,17 +112,15 @@ template <typename T>
 static cudaError_t launch_fp8_rows(const Fp8Params& p, const I8Operand& x, const I8Operand& w, cudaStream_t s) {
   const Fp8RowsOperands r{p, x, w};
   LaunchShape l(dim3(ceil_div(p.outs, 16)), 32 * kFp8RowsWarps, 0, s);
-  const bool aligned = x.aligned && w.aligned;
-  if (p.rows <= 8)
-    return cudaLaunchKernelEx(&l.cfg, aligned ? fp8_few_rows_kernel<T, 1, true> : fp8_few_rows_kernel<T, 1, false>, r);
-  return cudaLaunchKernelEx(&l.cfg, fp8_few_rows_kernel<T, 2, true>, r);  // never unaligned
+  return cudaLaunchKernelEx(&l.cfg, x.aligned && w.aligned ? fp8_rows_linear_kernel<T, true> : fp8_rows_linear_kernel<T, false>, r);
 }
 
-static bool fp8_by_rows(int64_t rows, bool aligned) { return rows <= (aligned ? 16 : 8); }
+// (4096 x 4096: up to eight rows 4.3-4.6 us, nine to sixteen through tcgen05 6.5.)
+constexpr int kFp8Rows = 8;
 
 template <typename T>
 static cudaError_t launch_fp8(const Fp8Params& p, I8Operand x, I8Operand w, uint4* ws, cudaStream_t s) {
-  if (fp8_by_rows(p.rows, x.aligned && w.aligned)) return launch_fp8_rows<T>(p, x, w, s);
+  if (p.rows <= kFp8Rows) return launch_fp8_rows<T>(p, x, w, s);
   const cudaError_t e = lay_out(x, w, p.depth, ws, s);
   if (e != cudaSuccess) return e;
   const Fp8Plan plan = fp8_plan(p.rows, p.outs, p.blocks);
@@ -183,7 +181,7 @@ size_t qrb200_fp8_linear_workspace_bytes(const uint8_t* x, int64_t x_stride, con
                                          int64_t outs, int64_t depth) {
   if (rows <= 0 || outs <= 0 || depth <= 0 || depth > QRB200_FP8_MAX_DEPTH) return 0;
   const I8Operand xo = codes_operand(x, rows, x_stride), wo = codes_operand(w, outs, w_stride);
-  return fp8_by_rows(rows, xo.aligned && wo.aligned) ? 0 : layout_bytes(xo, wo, depth);
+  return rows <= kFp8Rows ? 0 : layout_bytes(xo, wo, depth);
 }
 
 int qrb200_fp8_linear(const uint8_t* x, int64_t x_stride, const float* x_scale, const uint8_t* w, int64_t w_stride,

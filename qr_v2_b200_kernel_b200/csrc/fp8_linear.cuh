@@ -43,16 +43,18 @@ __device__ __forceinline__ void fp8_mma_pair(uint32_t d, uint64_t a, uint64_t b,
       : "memory");
 }
 
-// ---- up to sixteen rows ---------------------------------------------------------------------
+// ---- up to eight rows -----------------------------------------------------------------------
 //
-// The time is that of reading the weights once. A CTA takes 16 channels, a warp every eighth block of the
-// depth: weights, straight from memory, are the 16-row operand of the warp-level matrix instruction and
-// rows of x its columns; the order of a block's products is free, so a lane's 32 bytes of a row are two wide loads.
+// The time is that of reading the weights once, and at these sizes mostly latency. A CTA takes 16 channels, a warp every
+// sixteenth block of the depth: weights, straight from memory, are the 16-row operand of the warp-level matrix instruction and
+// rows of x its columns; the order of a block's products is free, so a lane's 32 bytes of a row are two wide loads. Many warps
+// with a block each in flight beat fewer with more (1 x 4096 x 4096: 4.3 us, 3.9 TB/s of weights; eight warps with four
+// blocks 7.5, one CTA an SM, or 5.0).
 struct Fp8RowsOperands {
   Fp8Params p;
   I8Operand x, w;
 };
-constexpr int kFp8RowsWarps = 8;
+constexpr int kFp8RowsWarps = 16;
 
 __device__ __forceinline__ void fp8_mma_warp(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -60,76 +62,52 @@ __device__ __forceinline__ void fp8_mma_warp(float (&d)[4], uint32_t a0, uint32_
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-template <typename T, int kNT, bool kAligned>  // kNT: eights of rows
-__global__ void __launch_bounds__(32 * kFp8RowsWarps) fp8_few_rows_kernel(Fp8RowsOperands R) {
-  constexpr int kUnroll = kNT == 1 ? 4 : 2;
-  __shared__ float s_sum[kFp8RowsWarps][8 * kNT][17];
+template <typename T, bool kAligned>
+__global__ void __launch_bounds__(32 * kFp8RowsWarps, 2) fp8_rows_linear_kernel(Fp8RowsOperands R) {
+  __shared__ float s_sum[kFp8RowsWarps][8][17];
   griddep_launch_wait();
   const Fp8Params& P = R.p;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int n0 = blockIdx.x * 16;
   const float* sw = P.sw + (long long)(n0 / kFp8Block) * P.blocks;
   const long long wr[2] = {min(n0 + g, P.outs - 1), min(n0 + g + 8, P.outs - 1)};
-  float acc[kNT][4] = {};
-  for (int b0 = warp; b0 < P.blocks; b0 += kFp8RowsWarps * kUnroll) {
-    uint4 w[kUnroll][2][2], x[kUnroll][kNT][2];
-    float s[kUnroll][kNT][2];
-    const bool whole = kAligned && (b0 + kFp8RowsWarps * (kUnroll - 1) + 1) * kFp8Block <= P.depth;
+  float acc[4] = {};
+  for (int b = warp; b < P.blocks; b += kFp8RowsWarps) {
+    uint4 w[2][2], x[2];
+    const bool whole = kAligned && (b + 1) * kFp8Block <= P.depth;
+    const auto get = [&](const I8Operand& o, long long row, int k) {
+      return whole         ? __ldg(reinterpret_cast<const uint4*>(o.base + row * o.stride + k))
+             : k < P.depth ? i8_codes16<kAligned>(o, row, k, P.depth)
+                           : make_uint4(0, 0, 0, 0);
+    };
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      const int b = b0 + u * kFp8RowsWarps;
+    for (int h = 0; h < 2; ++h) {
+      const int k = b * kFp8Block + 64 * h + 16 * t;
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int k = b * kFp8Block + 64 * h + 16 * t;
+      for (int r = 0; r < 2; ++r) w[r][h] = get(R.w, wr[r], k);
+      x[h] = g < P.rows ? get(R.x, g, k) : make_uint4(0, 0, 0, 0);
+    }
+    const float ws = __ldg(sw + b);
+    float s[2], d[4] = {};
 #pragma unroll
-        for (int r = 0; r < 2; ++r)
-          w[u][r][h] = whole ? __ldg(reinterpret_cast<const uint4*>(R.w.base + wr[r] * R.w.stride + k))
-                       : k < P.depth ? i8_codes16<kAligned>(R.w, wr[r], k, P.depth)
-                                     : make_uint4(0, 0, 0, 0);
+    for (int c = 0; c < 2; ++c) s[c] = 2 * t + c < P.rows ? __ldg(P.sx + (long long)(2 * t + c) * P.blocks + b) * ws : 0.f;
 #pragma unroll
-        for (int n = 0; n < kNT; ++n)
-          x[u][n][h] = 8 * n + g >= P.rows ? make_uint4(0, 0, 0, 0)
-                       : whole             ? __ldg(reinterpret_cast<const uint4*>(R.x.base + (8 * n + g) * R.x.stride + k))
-                       : k < P.depth       ? i8_codes16<kAligned>(R.x, 8 * n + g, k, P.depth)
-                                           : make_uint4(0, 0, 0, 0);
-      }
-      const bool in = b < P.blocks;
-      const float ws = in ? __ldg(sw + b) : 0.f;
-#pragma unroll
-      for (int n = 0; n < kNT; ++n)
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          const int row = 8 * n + 2 * t + c;
-          s[u][n][c] = in && row < P.rows ? __ldg(P.sx + (long long)row * P.blocks + b) * ws : 0.f;
-        }
+    for (int h = 0; h < 2; ++h) {
+      fp8_mma_warp(d, w[0][h].x, w[1][h].x, w[0][h].y, w[1][h].y, x[h].x, x[h].y);
+      fp8_mma_warp(d, w[0][h].z, w[1][h].z, w[0][h].w, w[1][h].w, x[h].z, x[h].w);
     }
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u)
-#pragma unroll
-      for (int n = 0; n < kNT; ++n) {
-        float d[4] = {};
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          fp8_mma_warp(d, w[u][0][h].x, w[u][1][h].x, w[u][0][h].y, w[u][1][h].y, x[u][n][h].x, x[u][n][h].y);
-          fp8_mma_warp(d, w[u][0][h].z, w[u][1][h].z, w[u][0][h].w, w[u][1][h].w, x[u][n][h].z, x[u][n][h].w);
-        }
-#pragma unroll
-        for (int e = 0; e < 4; ++e) acc[n][e] = fmaf(d[e], s[u][n][e & 1], acc[n][e]);
-      }
+    for (int e = 0; e < 4; ++e) acc[e] = fmaf(d[e], s[e & 1], acc[e]);
   }
 #pragma unroll
-  for (int n = 0; n < kNT; ++n)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) s_sum[warp][8 * n + 2 * t + (e & 1)][g + 8 * (e >> 1)] = acc[n][e];
+  for (int e = 0; e < 4; ++e) s_sum[warp][2 * t + (e & 1)][g + 8 * (e >> 1)] = acc[e];
   __syncthreads();
-  for (int at = threadIdx.x; at < 128 * kNT; at += 32 * kFp8RowsWarps) {
-    const int row = at >> 4, n = n0 + (at & 15);
-    if (row >= P.rows || n >= P.outs) continue;
-    float sum = P.bias ? to_f32(static_cast<const T*>(P.bias)[n]) : 0.f;
+  const int row = threadIdx.x >> 4, n = n0 + (threadIdx.x & 15);
+  if (row >= P.rows || n >= P.outs) return;
+  float sum = P.bias ? to_f32(static_cast<const T*>(P.bias)[n]) : 0.f;
 #pragma unroll
-    for (int i = 0; i < kFp8RowsWarps; ++i) sum += s_sum[i][row][at & 15];
-    static_cast<T*>(P.y)[(long long)row * P.outs + n] = from_f32<T>(sum);
-  }
+  for (int i = 0; i < kFp8RowsWarps; ++i) sum += s_sum[i][row][threadIdx.x & 15];
+  static_cast<T*>(P.y)[(long long)row * P.outs + n] = from_f32<T>(sum);
 }
 
 // ---- few rows ------------------------------------------------------------------------------
