@@ -8,12 +8,13 @@ namespace qrb200 {
 static bool off16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) != 0; }
 
 template <typename T, bool kAligned>
-static cudaError_t launch_quantise_of(const Fp8RowsParams& p, int tile_rows, cudaStream_t s) {
+static cudaError_t launch_quantise_of(Fp8RowsParams p, int tile_rows, cudaStream_t s) {
   constexpr int kPer = 256 / (kFp8Block * (int)sizeof(T) / 16);  // blocks that a CTA takes at a time
   if (tile_rows == 1) {
     // Four blocks to a thread where that leaves work for every SM.
     const int64_t units = p.rows * p.blocks;
     const int items = units > 4 * kPer * 8 * (int64_t)sm_count() ? 4 : 1;
+    p.step_rows = kPer / p.blocks, p.step_blocks = kPer % p.blocks;
     LaunchShape l(dim3(ceil_div(units, kPer * items)), 256, 0, s);
     return items == 4 ? cudaLaunchKernelEx(&l.cfg, fp8_rows_kernel<T, kAligned, 4>, p)
                       : cudaLaunchKernelEx(&l.cfg, fp8_rows_kernel<T, kAligned, 1>, p);
@@ -151,7 +152,7 @@ int qrb200_quantize_fp8(const void* x, int64_t x_stride, uint8_t* q, int64_t q_s
   if (rows > ((int64_t)1 << 33) / blocks) return QRB200_ERR_ARG;
   const int st = quant_ready();
   if (st != QRB200_OK) return st;
-  const Fp8RowsParams p{x, q, scale, rows, x_stride, q_stride, (int)cols, blocks, 0};
+  const Fp8RowsParams p{x, q, scale, rows, x_stride, q_stride, (int)cols, blocks, 0, 0, 0};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const cudaError_t e = dtype == QRB200_BF16  ? launch_quantise<__nv_bfloat16>(p, tile_rows, s)
                         : dtype == QRB200_F16 ? launch_quantise<__half>(p, tile_rows, s)

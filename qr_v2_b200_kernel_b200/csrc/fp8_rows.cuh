@@ -21,6 +21,7 @@ struct Fp8RowsParams {
   long long rows, x_stride, q_stride;
   int cols, blocks;  // of a row
   int q_aligned;     // rows of q start on 16-byte boundaries
+  int step_rows, step_blocks;  // rows and blocks from a thread's block to its next
 };
 
 __device__ __forceinline__ uint32_t fp8_pair(float a, float b) {  // a in the low byte
@@ -34,10 +35,17 @@ __device__ __forceinline__ float2 fp8_values(uint32_t two) {  // of the low and 
   return __half22float2(reinterpret_cast<const __half2&>(h));
 }
 
-// What a block's entries are divided by: a / 512 and its reciprocal (a from 2^-100 on, so both are normal).
+// What a block's entries are divided by: a / 512 and its reciprocal, to within two units in the last place (a from
+// 2^-100 on, so both are normal).
 struct Fp8Block {
   float div, inv;
 };
+__device__ __forceinline__ Fp8Block fp8_block(unsigned top) {
+  Fp8Block b;
+  b.div = __uint_as_float(top) * 0x1p-9f;
+  asm("rcp.approx.f32 %0, %1;" : "=f"(b.inv) : "f"(b.div));
+  return b;
+}
 
 // An entry for which 32 bits leave open on which side of a border between codes 448 x / a lies: the
 // quotient in 64 bits, rounded to 32 with its last bit standing for all that is cut off.
@@ -47,40 +55,58 @@ static __device__ __noinline__ float fp8_next_to_border(float x, float div) {
   return (double)r == q ? r : __uint_as_float(__float_as_uint(r) | 1u);
 }
 
-// 448 x / a, as a 32-bit number that rounds to the code that the exact quotient does.
+// 448 x / a of two entries, as 32-bit numbers that round to the codes that the exact quotients do.
 template <typename T>
-__device__ __forceinline__ float fp8_quotient(T x, const Fp8Block& b) {
-  const float v = to_f32(x), p = v * 0.875f;
-  const float q = p * b.inv;
+__device__ __forceinline__ float2 fp8_quotients(float2 v, const Fp8Block& b) {
+  const float2 div = make_float2(-b.div, -b.div), inv = make_float2(b.inv, b.inv);
+  const float2 p = __fmul2_rn(v, make_float2(0.875f, 0.875f));
+  float2 q = __fmul2_rn(p, inv);
   if constexpr (sizeof(T) == 2) {
-    // p is exact, and the remainder's correction makes the quotient the nearest of 32 bits: a border is
-    // one of those, and no other quotient of 16-bit numbers is near enough to round to one.
-    return fmaf(fmaf(-q, b.div, p), b.inv, q);
+    // p is exact, and the remainder's correction makes the quotient right to some 2^-44 before it is rounded: a
+    // quotient of 16-bit numbers that lies on a border becomes that border, and no other is near enough to round to one.
+    return __ffma2_rn(__ffma2_rn(q, div, p), inv, q);
   } else {
     // A border has four bits and a half: of the 20 behind them only the first is set. From 2^-11 to 2^-6
     // the codes lie 2^-9 apart, and borders elsewhere; below, there is nothing but 0.
-    const uint32_t bits = __float_as_uint(q);
-    const bool near = ((bits - 0x80000u + 8) & 0xfffffu) <= 16u || (bits & 0x7fffffffu) - 0x3a000000u < 0x02800010u;
-    return near ? fp8_next_to_border(v, b.div) : q;
+    const auto near = [](float x) {
+      const uint32_t bits = __float_as_uint(x);
+      return ((bits - 0x80000u + 8) & 0xfffffu) <= 16u || (bits & 0x7fffffffu) - 0x3a000000u < 0x02800010u;
+    };
+    if (near(q.x)) q.x = fp8_next_to_border(v.x, b.div);
+    if (near(q.y)) q.y = fp8_next_to_border(v.y, b.div);
+    return q;
   }
 }
 
-// A block's largest magnitude (as bits: NaN above infinity) to its scale; whether it has codes at all.
-__device__ __forceinline__ bool fp8_scale(unsigned top, float* scale) {
-  const float a = __uint_as_float(top);
-  if (top >= 0x7f800000u) *scale = __int_as_float(0x7fffffff);
-  else *scale = a < kTinyRow ? 0.f : a / 448.f;
-  return top < 0x7f800000u && a >= kTinyRow;
+// The largest magnitude of a pack, as the bits of a 32-bit float: ordered as whole numbers, NaN above infinity.
+template <typename T, int kVec>
+__device__ __forceinline__ unsigned fp8_top(const T (&x)[kVec]) {
+  const uint32_t* w = reinterpret_cast<const uint32_t*>(x);
+  if constexpr (sizeof(T) == 2) {
+    const uint32_t top = __vmaxu2(__vmaxu2(w[0] & 0x7fff7fffu, w[1] & 0x7fff7fffu), __vmaxu2(w[2] & 0x7fff7fffu, w[3] & 0x7fff7fffu));
+    const uint16_t most = (uint16_t)max(top & 0xffffu, top >> 16);
+    return __float_as_uint(to_f32(reinterpret_cast<const T&>(most)));
+  } else {
+    return max(max(w[0] & 0x7fffffffu, w[1] & 0x7fffffffu), max(w[2] & 0x7fffffffu, w[3] & 0x7fffffffu));
+  }
 }
+// a / 448, rounded once (the remainder's correction of a product with 1 / 448).
+__device__ __forceinline__ float fp8_scale(unsigned top) {
+  const float a = __uint_as_float(top), q = a * (1.f / 448.f);
+  const float scale = fmaf(fmaf(-q, 448.f, a), 1.f / 448.f, q);
+  return top >= 0x7f800000u ? __int_as_float(0x7fffffff) : a < kTinyRow ? 0.f : scale;
+}
+__device__ __forceinline__ bool fp8_has_codes(unsigned top) { return top < 0x7f800000u && __uint_as_float(top) >= kTinyRow; }
 
 template <typename T, int kVec>
 __device__ __forceinline__ void fp8_codes(uint32_t (&word)[kVec / 4], const T (&x)[kVec], unsigned top) {
-  const float div = __uint_as_float(top) * 0x1p-9f;
-  const Fp8Block b{div, __frcp_rn(div)};
+  const Fp8Block b = fp8_block(top);
 #pragma unroll
-  for (int i = 0; i < kVec / 4; ++i)
-    word[i] = fp8_pair(fp8_quotient(x[4 * i], b), fp8_quotient(x[4 * i + 1], b)) |
-              fp8_pair(fp8_quotient(x[4 * i + 2], b), fp8_quotient(x[4 * i + 3], b)) << 16;
+  for (int i = 0; i < kVec / 4; ++i) {
+    const float2 lo = fp8_quotients<T>(make_float2(to_f32(x[4 * i]), to_f32(x[4 * i + 1])), b);
+    const float2 hi = fp8_quotients<T>(make_float2(to_f32(x[4 * i + 2]), to_f32(x[4 * i + 3])), b);
+    word[i] = fp8_pair(lo.x, lo.y) | fp8_pair(hi.x, hi.y) << 16;
+  }
 }
 
 template <bool kAligned, typename T, int kVec>
@@ -102,43 +128,42 @@ __global__ void __launch_bounds__(256) fp8_rows_kernel(Fp8RowsParams P) {
   constexpr int kVec = 16 / sizeof(T), kSpan = kFp8Block / kVec, kPer = 256 / kSpan;  // threads of a block; blocks at a time
   griddep_launch_wait();
   const int lane = threadIdx.x % kSpan;
-  const long long total = P.rows * P.blocks, first = (long long)blockIdx.x * (kPer * kItems) + threadIdx.x / kSpan;
+  const long long first = (long long)blockIdx.x * (kPer * kItems) + threadIdx.x / kSpan;
   const char* lo = static_cast<const char*>(P.x);
   const Span in{lo, lo + ((P.rows - 1) * P.x_stride + P.cols) * (long long)sizeof(T)};
   alignas(16) T x[kItems][kVec];
-  const auto place = [&](int i, long long& row, int& col) {
-    const long long at = first + i * kPer;
-    row = total <= 0xffffffffll ? (long long)((uint32_t)at / (uint32_t)P.blocks) : at / P.blocks;
-    col = (int)(at - row * P.blocks) * kFp8Block + lane * kVec;
-    return at < total && col < P.cols;
+  // A thread's block and, step_rows rows and step_blocks blocks on, its next.
+  const long long row0 = first <= 0xffffffffll ? (long long)((uint32_t)first / (uint32_t)P.blocks) : first / P.blocks;
+  const int block0 = (int)(first - row0 * P.blocks);
+  long long row = row0;
+  int block = block0;
+  const auto advance = [&]() {
+    row += P.step_rows, block += P.step_blocks;
+    if (block >= P.blocks) block -= P.blocks, ++row;
   };
 #pragma unroll
   for (int i = 0; i < kItems; ++i) {
-    long long row;
-    int col;
-    const bool mine = place(i, row, col);
-    if (mine) load_pack<kAligned>(x[i], static_cast<const T*>(P.x) + row * P.x_stride + col, P.cols - col, in);
+    const int col = block * kFp8Block + lane * kVec;
+    if (row < P.rows && col < P.cols) load_pack<kAligned>(x[i], static_cast<const T*>(P.x) + row * P.x_stride + col, P.cols - col, in);
     else
 #pragma unroll
       for (int e = 0; e < kVec; ++e) x[i][e] = from_f32<T>(0.f);
+    advance();
   }
+  row = row0, block = block0;
 #pragma unroll
   for (int i = 0; i < kItems; ++i) {
-    long long row;
-    int col;
-    const bool mine = place(i, row, col);
-    unsigned top = 0;
-#pragma unroll
-    for (int e = 0; e < kVec; ++e) top = max(top, __float_as_uint(to_f32(x[i][e])) & 0x7fffffffu);
+    const int col = block * kFp8Block + lane * kVec;
+    unsigned top = fp8_top(x[i]);
 #pragma unroll
     for (int o = kSpan / 2; o; o >>= 1) top = max(top, __shfl_xor_sync(kFullMask, top, o));
-    float scale;
-    const bool codes = fp8_scale(top, &scale);
-    if (!mine) continue;
-    if (lane == 0) P.scale[first + i * kPer] = scale;
-    uint32_t word[kVec / 4] = {};
-    if (codes) fp8_codes<T, kVec>(word, x[i], top);
-    fp8_store<kAligned, T, kVec>(P.q + row * P.q_stride + col, word, P.cols - col, P.q_aligned);
+    if (row < P.rows && col < P.cols) {
+      if (lane == 0) P.scale[first + i * kPer] = fp8_scale(top);
+      uint32_t word[kVec / 4] = {};
+      if (fp8_has_codes(top)) fp8_codes<T, kVec>(word, x[i], top);
+      fp8_store<kAligned, T, kVec>(P.q + row * P.q_stride + col, word, P.cols - col, P.q_aligned);
+    }
+    advance();
   }
 }
 
@@ -165,15 +190,13 @@ __global__ void __launch_bounds__(512) fp8_tiles_kernel(Fp8RowsParams P) {
   }
 #pragma unroll
   for (int i = 0; i < kItems; ++i)
-#pragma unroll
-    for (int e = 0; e < kVec; ++e) top = max(top, __float_as_uint(to_f32(x[i][e])) & 0x7fffffffu);
+    top = max(top, fp8_top(x[i]));
   top = __reduce_max_sync(kFullMask, top);
   if ((threadIdx.x & 31) == 0) s_top[threadIdx.x >> 5] = top;
   __syncthreads();
   top = __reduce_max_sync(kFullMask, s_top[threadIdx.x & 15]);
-  float scale;
-  const bool codes = fp8_scale(top, &scale);
-  if (threadIdx.x == 0) P.scale[tile] = scale;
+  const bool codes = fp8_has_codes(top);
+  if (threadIdx.x == 0) P.scale[tile] = fp8_scale(top);
 #pragma unroll
   for (int i = 0; i < kItems; ++i) {
     const long long row = row0 + i * kStep;
