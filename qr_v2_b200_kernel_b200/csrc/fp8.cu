@@ -34,11 +34,12 @@ static cudaError_t launch_quantise(Fp8RowsParams p, int tile_rows, cudaStream_t 
 template <typename T>
 static cudaError_t launch_values(const uint8_t* q, int64_t q_stride, const float* scale, void* out, int64_t rows, int64_t cols,
                                  int tile_rows, cudaStream_t s) {
-  const bool packed = cols * sizeof(T) % 16 == 0 && q_stride % 16 == 0 && !off16(q) && !off16(out);
-  const int64_t units = rows * (packed ? ceil_div(cols, 16) : cols);
-  LaunchShape l(dim3(ceil_div(units, 256)), 256, 0, s);
-  return cudaLaunchKernelEx(&l.cfg, packed ? fp8_values_kernel<T, true> : fp8_values_kernel<T, false>, q, (long long)q_stride, scale,
-                            static_cast<T*>(out), (long long)rows, (int)cols, tile_rows);
+  constexpr int kVec = 16 / sizeof(T);
+  const bool packed = cols % kVec == 0 && q_stride % 16 == 0 && !off16(q) && !off16(out);
+  Fp8ValuesParams p{q, scale, out, rows, q_stride, (int)cols, ceil_div(cols, kFp8Block), tile_rows, packed ? (int)(cols / kVec) : ceil_div(cols, 256), 0, 0};
+  p.step_rows = 256 / p.units, p.step_units = 256 % p.units;
+  LaunchShape l(dim3(ceil_div(rows * p.units, packed ? 1024 : 8)), 256, 0, s);
+  return cudaLaunchKernelEx(&l.cfg, packed ? fp8_values_kernel<T, true> : fp8_values_kernel<T, false>, p);
 }
 
 static I8Operand codes_operand(const uint8_t* base, int64_t rows, int64_t stride) {

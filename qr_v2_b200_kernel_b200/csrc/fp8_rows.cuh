@@ -207,41 +207,73 @@ __global__ void __launch_bounds__(512) fp8_tiles_kernel(Fp8RowsParams P) {
   }
 }
 
-// value = code * scale of its block, rounded once: sixteen codes to a thread where both sides' rows start on
-// 16-byte boundaries (kPacked), else one, a warp's side by side.
+// value = code * scale of its block, rounded once: four packs of 16 bytes of values to a thread, a CTA's width apart,
+// where both sides' rows start on 16-byte boundaries (kPacked), else eight values, a warp on 256 neighbouring ones.
+struct Fp8ValuesParams {
+  const uint8_t* q;
+  const float* scale;
+  void* out;
+  long long rows, q_stride;
+  int cols, blocks, tile_rows;
+  int units;                  // packs of a row, or its spans of 256
+  int step_rows, step_units;  // from a thread's pack to its next
+};
 template <typename T, bool kPacked>
-__global__ void __launch_bounds__(256) fp8_values_kernel(const uint8_t* q, long long q_stride, const float* scale, T* out,
-                                                         long long rows, int cols, int tile_rows) {
-  constexpr int kSpan = kPacked ? 16 : 1;
+__global__ void __launch_bounds__(256) fp8_values_kernel(Fp8ValuesParams P) {
   griddep_launch_wait();
-  const int spans = (cols + kSpan - 1) / kSpan, blocks = (cols + kFp8Block - 1) / kFp8Block;
-  const long long at = (long long)blockIdx.x * 256 + threadIdx.x;
-  const long long row = at <= 0xffffffffll ? (long long)((uint32_t)at / (uint32_t)spans) : at / spans;
-  if (row >= rows) return;
-  const int c = (int)(at - row * spans) * kSpan;
-  const float s = scale[(tile_rows == 1 ? row : row / kFp8Block) * blocks + c / kFp8Block];
-  q += row * q_stride + c;
-  out += row * cols + c;
+  const auto scale_at = [&](long long row, int c) {
+    return __ldg(P.scale + (P.tile_rows == 1 ? row : row / kFp8Block) * P.blocks + c / kFp8Block);
+  };
+  const auto split = [&](long long at, long long& row, int& unit) {
+    row = at <= 0xffffffffll ? (long long)((uint32_t)at / (uint32_t)P.units) : at / P.units;
+    unit = (int)(at - row * P.units);
+  };
   if constexpr (kPacked) {
-    const int n = cols - c;  // a multiple of a pack of the values
-    uint32_t word[4] = {};
-    if (n >= 16) *reinterpret_cast<uint4*>(word) = __ldg(reinterpret_cast<const uint4*>(q));
-    else
+    constexpr int kVec = 16 / sizeof(T), kItems = 4;
+    long long row[kItems];
+    int unit[kItems];
+    uint32_t word[kItems][kVec / 4];
+    float s[kItems];
+    split((long long)blockIdx.x * (256 * kItems) + threadIdx.x, row[0], unit[0]);
 #pragma unroll
-      for (int e = 0; e < 16; ++e) word[e / 4] |= e < n ? (uint32_t)q[e] << (8 * (e & 3)) : 0u;
-    constexpr int kPart = 16 / sizeof(T);
-#pragma unroll
-    for (int h = 0; h < 16; h += kPart) {
-      alignas(16) T v[kPart];
-#pragma unroll
-      for (int e = 0; e < kPart; e += 2) {
-        const float2 two = fp8_values(word[(h + e) / 4] >> (8 * ((h + e) & 2)));
-        put2(&v[e], two.x * s, two.y * s);
+    for (int i = 0; i < kItems; ++i) {
+      if (i > 0) {
+        row[i] = row[i - 1] + P.step_rows, unit[i] = unit[i - 1] + P.step_units;
+        if (unit[i] >= P.units) unit[i] -= P.units, ++row[i];
       }
-      if (h < n) store_pack<true>(out + h, v, kPart);
+      if (row[i] >= P.rows) continue;
+      const uint8_t* q = P.q + row[i] * P.q_stride + unit[i] * kVec;
+      if constexpr (kVec == 8) *reinterpret_cast<uint2*>(word[i]) = __ldg(reinterpret_cast<const uint2*>(q));
+      else word[i][0] = __ldg(reinterpret_cast<const uint32_t*>(q));
+      s[i] = scale_at(row[i], unit[i] * kVec);
+    }
+#pragma unroll
+    for (int i = 0; i < kItems; ++i) {
+      if (row[i] >= P.rows) continue;
+      alignas(16) T v[kVec];
+#pragma unroll
+      for (int e = 0; e < kVec; e += 2) {
+        const float2 two = fp8_values(word[i][e / 4] >> (8 * (e & 2)));
+        put2(&v[e], two.x * s[i], two.y * s[i]);
+      }
+      *reinterpret_cast<uint4*>(static_cast<T*>(P.out) + row[i] * P.cols + unit[i] * kVec) = *reinterpret_cast<const uint4*>(v);
     }
   } else {
-    *out = from_f32<T>(fp8_values(*q).x * s);
+    const int lane = threadIdx.x & 31;
+    long long row;
+    int unit;
+    split((long long)blockIdx.x * 8 + (threadIdx.x >> 5), row, unit);
+    if (row >= P.rows) return;
+    const int c = unit * 256;
+    const uint8_t* q = P.q + row * P.q_stride + c;
+    T* out = static_cast<T*>(P.out) + row * P.cols + c;
+    uint32_t code[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) code[i] = c + lane + 32 * i < P.cols ? __ldg(q + lane + 32 * i) : 0;
+    const float s[2] = {scale_at(row, c), c + kFp8Block < P.cols ? scale_at(row, c + kFp8Block) : 0.f};
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (c + lane + 32 * i < P.cols) out[lane + 32 * i] = from_f32<T>(fp8_values(code[i]).x * s[i / 4]);
   }
 }
 
