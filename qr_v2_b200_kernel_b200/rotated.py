@@ -1,7 +1,7 @@
 """A quantised attention layer in rotated coordinates: what the orthogonal matrices of this package
     are for.
 
-    python -m qr_v2_b200_kernel_b200.rotated [--hidden 1024] [--tokens 200] [--steps 8]
+    python -m qr_v2_b200_kernel_b200.rotated [--hidden 1024] [--tokens 200] [--steps 8] [--cache-bits 4] [--products int8]
 
     The residual stream of a transformer has a few channels far larger than the rest, and a scale
     for a whole row then wastes the 8 bits of the others. An orthogonal ``Q`` (hidden x hidden, from
@@ -12,6 +12,11 @@
     output projection takes ``R`` back. Nothing is added to a step:
 
     rms_norm_int8 -> int8_linear -> kv4_write -> kv4_attention -> quantize_int8 -> int8_linear
+
+    With ``--cache-bits 8`` keys and values go into the 8-bit cache, and with ``--products fp8`` the
+    projections are products of 8-bit floating point with a scale for each block of 128, which need the rotation
+    less: quantize_fp8 -> fp8_linear -> kv8_write -> kv8_attention -> quantize_fp8 -> fp8_linear, the
+    norm's factor multiplied into the scales.
 
     The command runs a prompt and some single tokens through one layer, with and without the
     rotation, and prints how far each is from the same layer in 64 bits. (No positional rotation:
@@ -26,21 +31,29 @@ import json
 import torch
 
 from . import gen
-from .quant import int8_linear, kv4_attention, kv4_cache, kv4_write, quantize_int8, rms_norm_int8
+from .quant import (fp8_linear, int8_linear, kv4_attention, kv4_cache, kv4_write, kv8_attention, kv8_cache, kv8_write,
+                    quantize_fp8, quantize_int8, rms_norm_int8)
 
 __all__ = ["RotatedAttention"]
 
 
 class RotatedAttention:
-    """One attention layer: int8 projections, a 4-bit cache, one sequence per row of ``block_table``.
+    """One attention layer: 8-bit projections, a 4- or 8-bit cache, one sequence per row of ``block_table``.
 
     ``wq`` (heads * head_dim, hidden), ``wk`` and ``wv`` (kv_heads * head_dim, hidden), ``wo``
     (hidden, heads * head_dim) and ``gain`` (hidden,): floating point, on a CUDA device.
     ``q_hidden`` (hidden, hidden) and ``q_head`` (head_dim, head_dim): orthogonal, or ``None`` for
-    no rotation. Weights are rotated in 64 bits and quantised once.
+    no rotation. ``products``: "int8" (a scale for each row and channel) or "fp8" (8-bit floating point, a scale for each
+    block of 128); ``cache_bits``: 4 or 8. Weights are rotated in 64 bits and quantised once.
     """
 
-    def __init__(self, wq, wk, wv, wo, gain, head_dim: int, q_hidden=None, q_head=None, dtype=torch.bfloat16):
+    def __init__(self, wq, wk, wv, wo, gain, head_dim: int, q_hidden=None, q_head=None, dtype=torch.bfloat16,
+                 products: str = "int8", cache_bits: int = 4):
+        if products not in ("int8", "fp8"):
+            raise ValueError(f'products must be "int8" or "fp8", got {products!r}')
+        if cache_bits not in (4, 8):
+            raise ValueError(f"cache_bits must be 4 or 8, got {cache_bits}")
+        self.products, self.cache_bits = products, cache_bits
         self.head_dim, self.dtype = head_dim, dtype
         self.heads, self.kv_heads = wq.shape[0] // head_dim, wk.shape[0] // head_dim
         eye = lambda n: torch.eye(n, dtype=torch.float64, device=wq.device)  # noqa: E731
@@ -52,11 +65,21 @@ class RotatedAttention:
             return torch.einsum("de,hdi,ij->hej", r, w.unflatten(0, (-1, head_dim)), q).flatten(0, 1)
 
         out = torch.einsum("ij,ihd,de->jhe", q, wo.double().unflatten(1, (-1, head_dim)), r).flatten(1)
-        self.qkv, self.qkv_scale = quantize_int8(torch.cat([into_heads(w) for w in (wq, wk, wv)]).float())
-        self.out, self.out_scale = quantize_int8(out.float())
+        quantize = quantize_int8 if products == "int8" else lambda w: quantize_fp8(w, tile_rows=128)
+        self.qkv, self.qkv_scale = quantize(torch.cat([into_heads(w) for w in (wq, wk, wv)]).float())
+        self.out, self.out_scale = quantize(out.float())
 
     def new_cache(self, pages: int, page_size: int = 64):
-        return kv4_cache(pages, page_size, self.kv_heads, self.head_dim, dtype=self.dtype, device=self.qkv.device)
+        make = kv4_cache if self.cache_bits == 4 else kv8_cache
+        return make(pages, page_size, self.kv_heads, self.head_dim, dtype=self.dtype, device=self.qkv.device)
+
+    def _normed(self, x, residual):
+        """Codes and scales of the norm's output, and the stream."""
+        if self.products == "int8":
+            return rms_norm_int8(x, residual=residual)
+        stream = x if residual is None else x + residual
+        codes, scale = quantize_fp8(stream)
+        return codes, scale * torch.rsqrt(stream.float().square().mean(-1, keepdim=True) + 1e-6), stream
 
     def __call__(self, x, residual, cache, block_table, lengths, slots):
         """``(update, residual)`` for ``x`` (batch, queries, hidden), added to ``residual`` first (``None``:
@@ -67,13 +90,15 @@ class RotatedAttention:
         norm.
         """
         batch, queries, _ = x.shape
-        codes, scale, stream = rms_norm_int8(x, residual=residual)
-        qkv = int8_linear(codes, scale, self.qkv, self.qkv_scale, dtype=self.dtype)
+        linear, quantize = (int8_linear, quantize_int8) if self.products == "int8" else (fp8_linear, quantize_fp8)
+        write, attend = (kv4_write, kv4_attention) if self.cache_bits == 4 else (kv8_write, kv8_attention)
+        codes, scale, stream = self._normed(x, residual)
+        qkv = linear(codes, scale, self.qkv, self.qkv_scale, dtype=self.dtype)
         q, k, v = qkv.unflatten(-1, (-1, self.head_dim)).split([self.heads, self.kv_heads, self.kv_heads], dim=2)
-        kv4_write(cache, k.flatten(0, 1), v.flatten(0, 1), slots)
-        o = kv4_attention(q, cache, block_table, lengths)
-        codes, scale = quantize_int8(o.flatten(2))
-        return int8_linear(codes, scale, self.out, self.out_scale, dtype=self.dtype), stream
+        write(cache, k.flatten(0, 1), v.flatten(0, 1), slots)
+        o = attend(q, cache, block_table, lengths)
+        codes, scale = quantize(o.flatten(2))
+        return linear(codes, scale, self.out, self.out_scale, dtype=self.dtype), stream
 
 
 def exact_layer(stream, wq, wk, wv, wo, gain, head_dim):
@@ -89,7 +114,7 @@ def exact_layer(stream, wq, wk, wv, wo, gain, head_dim):
 
 
 def run(hidden: int = 1024, head_dim: int = 128, kv_heads: int = 2, batch: int = 3, tokens: int = 200, steps: int = 8,
-        seed: int = 0, device="cuda") -> dict:
+        seed: int = 0, device="cuda", products: str = "int8", cache_bits: int = 4) -> dict:
     """Relative error of the layer's updates, rotated and plain, over a prompt of ``tokens - steps`` tokens and ``steps`` single ones."""
     g = torch.Generator(device=device).manual_seed(seed)
     heads = hidden // head_dim
@@ -104,7 +129,7 @@ def run(hidden: int = 1024, head_dim: int = 128, kv_heads: int = 2, batch: int =
     q_head = gen.haar_orthogonal(1, head_dim, g, device)[0].double()
     errors = {}
     for name, q, r in (("rotated", q_hidden, q_head), ("plain", None, None)):
-        layer = RotatedAttention(*weights, gain, head_dim, q, r)
+        layer = RotatedAttention(*weights, gain, head_dim, q, r, products=products, cache_bits=cache_bits)
         page, per = 64, -(-tokens // 64)
         cache = layer.new_cache(batch * per, page)
         table = torch.randperm(batch * per, generator=g, device=device).reshape(batch, per).int()
@@ -128,8 +153,11 @@ def main() -> None:
     ap.add_argument("--hidden", type=int, default=1024)
     ap.add_argument("--tokens", type=int, default=200)
     ap.add_argument("--steps", type=int, default=8)
+    ap.add_argument("--products", choices=("int8", "fp8"), default="int8")
+    ap.add_argument("--cache-bits", type=int, choices=(4, 8), default=4)
     a = ap.parse_args()
-    print(json.dumps({"relative_error": run(hidden=a.hidden, tokens=a.tokens, steps=a.steps)}))
+    errors = run(hidden=a.hidden, tokens=a.tokens, steps=a.steps, products=a.products, cache_bits=a.cache_bits)
+    print(json.dumps({"relative_error": errors}))
 
 
 if __name__ == "__main__":
