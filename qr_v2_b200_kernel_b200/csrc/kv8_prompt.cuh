@@ -23,7 +23,7 @@
 namespace qrb200 {
 
 constexpr int kPromptRows = 256, kPromptTokens = 64;
-constexpr int kPromptStages = 3, kPromptRaw = 3;  // steps of operands, and of bytes, in shared memory
+constexpr int kPromptStages = 3, kPromptRaw = 2;  // steps of operands, and of bytes, in shared memory
 constexpr int kPromptThreads = 32 * 15;
 constexpr int kPromptStepExp = 11;
 __host__ __device__ constexpr int prompt_tile(int dim) { return 128 * dim * 2; }  // bytes of 128 rows of fp16
