@@ -141,10 +141,10 @@ int qrb200_kv8_write(void* codes, float* range, const qrb200_kv8_shape* shape, c
     LaunchShape l(dim3(ceil_div(tokens, 256)), 256, 0, s);
     if (cudaLaunchKernelEx(&l.cfg, kv8_rows_kernel, p) != cudaSuccess) return QRB200_ERR_CUDA;
     qrb200_internal_count_launch();
-    // As many heads to a CTA as leave four to an SM: the rows' look-up is shared, and the next head's loads are under way
+    // As many heads to a CTA as leave eight to an SM: the rows' look-up is shared, and the next head's loads are under way
     // while one's bytes leave.
     p.chunk = 64;
-    p.span = (int)std::max<int64_t>(1, std::min<int64_t>(h.heads, (tokens + 63) / 64 * h.heads / (4 * sm_count())));
+    p.span = (int)std::max<int64_t>(1, std::min<int64_t>(h.heads, (tokens + 63) / 64 * h.heads / (8 * sm_count())));
     p.span = ceil_div(h.heads, ceil_div(h.heads, p.span));  // evenly
   }
   // 16-byte loads where every (token, head) starts on such a boundary.

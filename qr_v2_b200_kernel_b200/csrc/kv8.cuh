@@ -248,7 +248,7 @@ __global__ void __launch_bounds__(256) kv8_write_few_kernel(Kv8IoParams P) {
 // lowest of them, so that nothing is shared: it finds all of the page's rows (s_row: the row of each
 // slot), their largest magnitude, and puts the runs that change together in shared memory, 64 tokens at a time: the
 // older codes, moved if the range grew, and the new ones over them. Up to 64 tokens a page, everything is read once.
-// 32768 tokens x 8 heads x 128 channels, bf16, from a page's first token 61 us, from within one 83.
+// 32768 tokens x 8 heads x 128 channels, bf16, from a page's first token 61 us, from within one 75.
 template <typename T, int kDim, bool kVec>
 __global__ void __launch_bounds__(2 * kDim) kv8_write_kernel(Kv8IoParams P) {
   constexpr int kChunks = kDim / 8, kRunThreads = 4 * kChunks;  // threads of a run
