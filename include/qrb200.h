@@ -254,7 +254,7 @@ int qrb200_fp8_linear(const uint8_t* x, int64_t x_stride, const float* x_scale, 
                       void* workspace, size_t workspace_bytes, void* stream);
 
 /* A paged key/value cache in 8 bits: codes, pages x kv_heads blocks of qrb200_kv8_block_bytes bytes, contiguous,
- * 16-byte aligned, and range, pages x kv_heads x 2 floats (keys, values). A code c, from -127 to 127, of a page and head stands
+ * 16-byte aligned, and range, pages x kv_heads x 2 floats (keys, values), 8-byte aligned. A code c, from -127 to 127, of a page and head stands
  * for c range / 127. dtype QRB200_BF16 or QRB200_F16, of the keys, values and queries; head_dim 64 or 128; page_size a power
  * of two from 16 to 1024. */
 typedef struct qrb200_kv8_shape {

@@ -15,6 +15,11 @@ static bool shape_of(const qrb200_kv8_shape* s, Kv8Shape* h) {
          h->page >= 16 && h->page <= 1024 && (h->page & (h->page - 1)) == 0;
 }
 
+// Codes by sixteen bytes, ranges by pairs.
+static bool cache_ok(const Kv8Shape& h, const void* codes, const void* range) {
+  return (h.pages == 0 || (codes && range)) && ((reinterpret_cast<uintptr_t>(codes) & 15u) | (reinterpret_cast<uintptr_t>(range) & 7u)) == 0;
+}
+
 // f(type, dim) with both as types.
 template <typename F>
 static cudaError_t with_shape(int dtype, int dim, F&& f) {
@@ -127,7 +132,7 @@ int qrb200_kv8_write(void* codes, float* range, const qrb200_kv8_shape* shape, c
   Kv8Shape h;
   if (tokens < 0 || !shape_of(shape, &h) || tokens > kMaxRows / h.heads) return QRB200_ERR_ARG;
   if (tokens == 0) return QRB200_OK;
-  if (!k || !v || !slots || (h.pages > 0 && (!codes || !range)) || (reinterpret_cast<uintptr_t>(codes) & 15u)) return QRB200_ERR_ARG;
+  if (!k || !v || !slots || !cache_ok(h, codes, range)) return QRB200_ERR_ARG;
   const int st = quant_ready();
   if (st != QRB200_OK) return st;
   const size_t need = qrb200_kv8_write_workspace_bytes(shape, tokens);
@@ -168,8 +173,7 @@ int qrb200_kv8_read(const void* codes, const float* range, const qrb200_kv8_shap
   Kv8Shape h;
   if (tokens < 0 || !shape_of(shape, &h) || tokens > kMaxRows / h.heads) return QRB200_ERR_ARG;
   if (tokens == 0) return QRB200_OK;
-  if (!k || !v || !slots || (h.pages > 0 && (!codes || !range)) ||
-      ((reinterpret_cast<uintptr_t>(codes) | reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15u))
+  if (!k || !v || !slots || !cache_ok(h, codes, range) || ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15u))
     return QRB200_ERR_ARG;
   const int st = quant_ready();
   if (st != QRB200_OK) return st;
@@ -212,8 +216,7 @@ int qrb200_kv8_attention(const void* q, const int64_t* q_strides, const void* co
   if (!q_strides || !(scale >= 0.f) || !(scale <= 3.0e38f) || window < 0 || !attention_args(shape, batch, queries, q_heads, max_pages, &h))
     return QRB200_ERR_ARG;
   if (batch == 0 || queries == 0 || q_heads == 0) return QRB200_OK;
-  if (!q || !out || !lengths || (max_pages > 0 && !block_table) || (reinterpret_cast<uintptr_t>(codes) & 15u) ||
-      (h.pages > 0 && (!codes || !range)) || table_stride < 0)
+  if (!q || !out || !lengths || (max_pages > 0 && !block_table) || !cache_ok(h, codes, range) || table_stride < 0)
     return QRB200_ERR_ARG;
   const int st = quant_ready();
   if (st != QRB200_OK) return st;
@@ -229,8 +232,7 @@ int qrb200_kv8_attention(const void* q, const int64_t* q_strides, const void* co
   p.lengths = lengths;
   p.q_bs = q_strides[0], p.q_ts = q_strides[1], p.q_hs = q_strides[2], p.table_stride = table_stride;
   p.batch = (int)batch, p.queries = (int)queries, p.q_heads = (int)q_heads, p.share = (int)(q_heads / h.heads);
-  // A window that reaches every token from every position is none (and cannot overflow a position).
-  p.window = window >= max_pages * h.page + queries ? 0 : (int)window;
+  p.window = window >= max_pages * h.page ? 0 : (int)window;  // one that reaches every token from every position is none
   p.max_pages = (int)max_pages, p.causal = causal, p.splits = plan.splits, p.tiles = plan.tiles;
   p.scale_part = std::frexp(scale, &p.scale_power) * 2.f * 1.4426950408889634f;
   p.scale_power -= 1;

@@ -359,7 +359,7 @@ __global__ void __launch_bounds__(2 * kDim) kv8_write_kernel(Kv8IoParams P) {
             const int part = at / kDim & 1;
             uint4 w = make_uint4(kKv8Zeros, kKv8Zeros, kKv8Zeros, kKv8Zeros);
             if (!move[part] || old[part] > 0.f) w = reinterpret_cast<const uint4*>(block + (long long)base * kRun)[at];
-              if (move[part] && old[part] > 0.f)
+            if (move[part] && old[part] > 0.f)
               w = make_uint4(kv8_moved(w.x, old[part], now[part]), kv8_moved(w.y, old[part], now[part]), kv8_moved(w.z, old[part], now[part]),
                              kv8_moved(w.w, old[part], now[part]));
             s_image[at] = w;

@@ -121,7 +121,7 @@ __global__ void __launch_bounds__(32 * kKvWarps, kv8_ctas(kBrief)) kv8_attention
   if (real) {
     const int pos = len - P.queries + (row0 + lane) / P.share;
     my_hi = P.causal ? max(0, pos + 1) : len;
-    my_lo = P.window > 0 ? max(0, pos - P.window + 1) : 0;
+    my_lo = P.window > 0 && pos >= P.window ? pos - P.window + 1 : 0;
   }
   const bool sees = my_hi > my_lo;
   const int all_lo = __reduce_min_sync(kFullMask, sees ? my_lo : 0x7fffffff);

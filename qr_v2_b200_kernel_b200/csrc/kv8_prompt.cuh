@@ -128,7 +128,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(Kv8AttnPa
   const auto range_of = [&](int row, int& lo, int& hi) {
     const int pos = len - P.queries + row / P.share;
     hi = P.causal ? max(0, pos + 1) : len;
-    lo = P.window > 0 ? max(0, pos - P.window + 1) : 0;
+    lo = P.window > 0 && pos >= P.window ? pos - P.window + 1 : 0;
     if (lo > hi) lo = hi;
   };
   int all_lo, all_hi, last_lo, last_hi;

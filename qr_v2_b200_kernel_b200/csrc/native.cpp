@@ -406,8 +406,9 @@ Cache8 make_cache8(const Tensor& data, const Tensor& range, int32_t page_size, i
                     "data must be a contiguous, 16-byte aligned (pages, kv_heads, ", size,
                     ") tensor for this page_size and head_dim, got ", shape_of(data));
   const int64_t want[3] = {data.size(0), data.size(1), 2};
-  TORCH_CHECK_VALUE(range.sizes() == at::IntArrayRef(want) && range.is_contiguous(), "range must be a contiguous (", want[0], ", ",
-                    want[1], ", 2) tensor, got ", shape_of(range));
+  TORCH_CHECK_VALUE(range.sizes() == at::IntArrayRef(want) && range.is_contiguous() &&
+                        (reinterpret_cast<uintptr_t>(range.const_data_ptr()) & 7u) == 0,
+                    "range must be a contiguous, 8-byte aligned (", want[0], ", ", want[1], ", 2) tensor, got ", shape_of(range));
   return Cache8{data, range, {data.size(0), (int32_t)data.size(1), page_size, head_dim, type_code(type)}, type};
 }
 

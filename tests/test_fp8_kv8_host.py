@@ -56,6 +56,8 @@ def test_kv8_entries_check_their_arguments(lib):
     assert write(tokens=0) == OK and write(tokens=-1) == ARG
     assert write(codes=None) == ARG and write(rng=None) == ARG and write(k=None) == ARG and write(slots=None) == ARG
     assert write(codes=ctypes.c_void_p(264)) == ARG  # not 16-byte aligned
+    odd = ctypes.c_void_p(260)  # not 8-byte aligned, as pairs of ranges are read
+    assert write(rng=odd) == ARG and r(P, odd, ctypes.byref(good), P, P, P, 3, None) == ARG
     for shape in (_lib.KV8Shape(4, 2, 16, 64, 0), _lib.KV8Shape(4, 0, 16, 64, 1), _lib.KV8Shape(4, 2, 24, 64, 1),
                   _lib.KV8Shape(4, 2, 16, 96, 1), _lib.KV8Shape(-1, 2, 16, 64, 1)):
         assert write(shape=shape) == ARG
@@ -74,6 +76,7 @@ def test_kv8_entries_check_their_arguments(lib):
     assert attend(heads=3) == ARG and attend(batch=-1) == ARG and attend(window=-1) == ARG and attend(pages=-1) == ARG
     assert attend(q=None) == ARG and attend(table=None) == ARG and attend(lengths=None) == ARG and attend(st=None) == ARG
     assert attend(codes=None) == ARG and attend(rng=None) == ARG and attend(scale=-1.0) == ARG and attend(scale=float("nan")) == ARG
+    assert attend(rng=odd) == ARG
     assert attend(queries=1 << 25) == ARG and attend(pages=1 << 30) == ARG
 
 

@@ -243,6 +243,7 @@ def test_copies_and_refusals():
             (lambda: qr.kv8_read(cache, slots.cpu()), RuntimeError), (lambda: qr.kv8_read(qr.kv4_cache(2, 16, 2, 64), slots), TypeError),
             (lambda: qr.KV8Cache(cache.data, cache.range[:1], 16, 64, BF), ValueError), (lambda: qr.KV8Cache(cache.data, cache.range, 32, 64, BF), ValueError),
             (lambda: qr.KV8Cache(cache.data, cache.range, 16, 64, torch.float32), TypeError),
+            (lambda: qr.KV8Cache(cache.data, torch.zeros(9, device="cuda")[1:].view(2, 2, 2), 16, 64, BF), ValueError),  # off 8 bytes
             (lambda: qr.kv8_attention(q.half(), cache, table, lengths), TypeError), (lambda: qr.kv8_attention(q[:, :, :3], cache, table, lengths), ValueError),
             (lambda: qr.kv8_attention(q, cache, table.long(), lengths), TypeError), (lambda: qr.kv8_attention(q, cache, table[0], lengths), ValueError),
             (lambda: qr.kv8_attention(q, cache, table, lengths, window=0), ValueError), (lambda: qr.kv8_attention(q, cache, table, lengths, scale=-1.0), ValueError),
@@ -544,6 +545,27 @@ def test_empty_calls():
         assert torch.all(out == 0)
         none = qr.kv8_cache(0, 16, 1, 64)
         assert torch.all(qr.kv8_attention(_randn(2, queries, 2, 64), none, table, _lengths(0, 0)) == 0)
+
+
+def test_a_batch_past_one_launch_grid():
+    batch = 65540  # a launch's third dimension holds 65535
+    cache, table, values = _filled(5, 16, 1, 64, 16, BF)
+    pick = torch.arange(batch, device="cuda") % 5
+    lengths = (torch.arange(batch, device="cuda") % 17).int()
+    q = _randn(batch, 1, 1, 64)
+    out = qr.kv8_attention(q, cache, table[pick].contiguous(), lengths)
+    at = torch.cat([torch.arange(40, device="cuda"), torch.arange(batch - 40, batch, device="cuda")])
+    part = _check_attention(q[at].contiguous(), cache, table[pick[at]].contiguous(), lengths[at], [x[pick[at]] for x in values])
+    assert torch.equal(out[at], part)
+
+
+@pytest.mark.parametrize("queries", [1, 30])
+def test_windows_up_to_the_largest(queries):
+    cache, table, values = _filled(2, 64, 2, 64, 16, BF)
+    q, lengths = _randn(2, queries, 4, 64), _lengths(64, 5)
+    whole = _check_attention(q, cache, table, lengths, values)
+    for window in (63, 64, 65, 64 + queries, 2**31 - 2, 2**31 - 1):
+        assert torch.equal(_check_attention(q, cache, table, lengths, values, window=window), whole) or window == 63
 
 
 def test_offsets_past_two_gibibytes():
