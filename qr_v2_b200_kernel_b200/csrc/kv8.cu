@@ -27,6 +27,9 @@ static cudaError_t with_shape(int dtype, int dim, F&& f) {
   return dim == 64 ? f(__half{}, Int<64>{}) : f(__half{}, Int<128>{});
 }
 
+// The pages' number and their list, before the slots' rows.
+static size_t write_list_bytes(int64_t tokens) { return 256 + (size_t)(tokens + 63) / 64 * 256; }
+
 // How an attention call is cut: query rows per tile, steps of 4 or 8 KB, and the token range over `splits` CTAs.
 struct Kv8Plan {
   int tile_rows, tiles, splits;
@@ -123,7 +126,7 @@ int64_t qrb200_kv8_block_bytes(int64_t page_size, int64_t head_dim) {
 size_t qrb200_kv8_write_workspace_bytes(const qrb200_kv8_shape* shape, int64_t tokens) {
   Kv8Shape h;
   if (!shape_of(shape, &h) || tokens <= kKv8Few) return 0;
-  return (size_t)h.pages * h.page * sizeof(int);
+  return write_list_bytes(tokens) + (size_t)h.pages * h.page * sizeof(int);
 }
 
 int qrb200_kv8_write(void* codes, float* range, const qrb200_kv8_shape* shape, const void* k, int64_t k_token_stride,
@@ -139,18 +142,18 @@ int qrb200_kv8_write(void* codes, float* range, const qrb200_kv8_shape* shape, c
   if (need > 0 && (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 255u)))
     return QRB200_ERR_WORKSPACE;
   Kv8IoParams p{static_cast<unsigned char*>(codes), range, k, v, nullptr, nullptr, reinterpret_cast<const long long*>(slots),
-                need > 0 ? static_cast<int*>(workspace) : nullptr, tokens, k_token_stride, k_head_stride, v_token_stride,
-                v_head_stride, h, 1, 1};
+                nullptr, nullptr, nullptr, tokens, k_token_stride, k_head_stride, v_token_stride, v_head_stride, h, 0};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (p.rows) {
+  if (need > 0) {
+    p.pages = static_cast<int*>(workspace);
+    p.list = p.pages + 64;
+    p.rows = p.pages + write_list_bytes(tokens) / sizeof(int);
     LaunchShape l(dim3(ceil_div(tokens, 256)), 256, 0, s);
     if (cudaLaunchKernelEx(&l.cfg, kv8_rows_kernel, p) != cudaSuccess) return QRB200_ERR_CUDA;
+    LaunchShape m(dim3(ceil_div(tokens, 8 * kKv8Seek)), 256, 0, s);
+    if (cudaLaunchKernelEx(&m.cfg, kv8_pages_kernel, p) != cudaSuccess) return QRB200_ERR_CUDA;
     qrb200_internal_count_launch();
-    // As many heads to a CTA as leave eight to an SM: the rows' look-up is shared, and the next head's loads are under way
-    // while one's bytes leave.
-    p.chunk = 64;
-    p.span = (int)std::max<int64_t>(1, std::min<int64_t>(h.heads, (tokens + 63) / 64 * h.heads / (8 * sm_count())));
-    p.span = ceil_div(h.heads, ceil_div(h.heads, p.span));  // evenly
+    qrb200_internal_count_launch();
   }
   // 16-byte loads where every (token, head) starts on such a boundary.
   const bool vec = ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15u) == 0 &&
@@ -158,10 +161,19 @@ int qrb200_kv8_write(void* codes, float* range, const qrb200_kv8_shape* shape, c
   const cudaError_t e = with_shape(shape->dtype, h.dim, [&](auto type, auto dim) {
     using E = decltype(type);
     if (!p.rows) {
-      LaunchShape l(dim3((unsigned)tokens, ceil_div(h.heads, 8)), 256, 0, s);
+      // (64 tokens of a page x 8 heads 9.4 us with two heads to a CTA, 15.9 with four; 256 single tokens 11.3, 6.6.)
+      p.span = tokens <= 64 ? 2 : 4;
+      LaunchShape l(dim3((unsigned)tokens, ceil_div(h.heads, p.span)), 2 * h.dim, 0, s);
       return cudaLaunchKernelEx(&l.cfg, vec ? kv8_write_few_kernel<E, dim(), true> : kv8_write_few_kernel<E, dim(), false>, p);
     }
-    LaunchShape l(dim3(ceil_div(tokens, p.chunk), ceil_div(h.heads, p.span)), 2 * h.dim, 0, s);
+    // Eight CTAs to an SM: a page's rows are looked up once for several heads then, and the next head's loads are under
+    // way while one's bytes leave.
+    const unsigned ctas = (unsigned)std::min<int64_t>(8 * sm_count(), tokens * h.heads);
+    LaunchShape m(dim3(std::min<unsigned>(ctas, 4 * sm_count())), 32 * kKv8ThinWarps, 0, s);
+    const cudaError_t thin = cudaLaunchKernelEx(&m.cfg, vec ? kv8_write_thin_kernel<E, dim(), true> : kv8_write_thin_kernel<E, dim(), false>, p);
+    if (thin != cudaSuccess) return thin;
+    qrb200_internal_count_launch();
+    LaunchShape l(dim3(ctas), 2 * h.dim, 0, s);
     return cudaLaunchKernelEx(&l.cfg, vec ? kv8_write_kernel<E, dim(), true> : kv8_write_kernel<E, dim(), false>, p);
   });
   if (e != cudaSuccess) return QRB200_ERR_CUDA;
@@ -178,7 +190,7 @@ int qrb200_kv8_read(const void* codes, const float* range, const qrb200_kv8_shap
   const int st = quant_ready();
   if (st != QRB200_OK) return st;
   const Kv8IoParams p{static_cast<unsigned char*>(const_cast<void*>(codes)), const_cast<float*>(range), nullptr, nullptr, k, v,
-                      reinterpret_cast<const long long*>(slots), nullptr, tokens, 0, 0, 0, 0, h, 1, 1};
+                      reinterpret_cast<const long long*>(slots), nullptr, nullptr, nullptr, tokens, 0, 0, 0, 0, h, 0};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const cudaError_t e = with_shape(shape->dtype, h.dim, [&](auto type, auto dim) {
     LaunchShape l(dim3(ceil_div((tokens + 15) / 16 * h.heads, 8)), 256, 0, s);

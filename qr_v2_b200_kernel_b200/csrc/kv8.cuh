@@ -42,10 +42,12 @@ struct Kv8IoParams {
   void* k_out;
   void* v_out;
   const long long* slots;
-  int* rows;  // workspace: a slot's row of this call, where there are many
+  // Workspace, where there are many rows: how many pages get few of them and how many more, a row of each page (the first kind
+  // from the list's front, the second from its end), and the row of each slot.
+  int *pages, *list, *rows;
   long long tokens, k_ts, k_hs, v_ts, v_hs;  // strides in elements
   Kv8Shape sh;
-  int chunk, span;  // rows and heads of a CTA
+  int span;  // heads of a CTA, where rows are few
 };
 
 // Offsets of a token's code within its block: of channel c, as a key and as a value.
@@ -60,6 +62,7 @@ __device__ __forceinline__ int kv8_value_at(int dim, int token, int c) {
 
 constexpr uint32_t kKv8Zeros = 0x80808080u;
 constexpr int kKv8Few = 1024;  // rows up to which a page's are looked up among all of them
+constexpr int kKv8Thin = 8;    // rows of a page up to which a warp takes a head, else a CTA
 
 // Three significant bits, rounded up, of a magnitude's bits (the magnitude itself where that would pass the type's
 // largest number, so that no value reads back as infinity); NaN for what is not finite.
@@ -81,10 +84,55 @@ __device__ __forceinline__ long long kv8_page(const Kv8IoParams& P, long long sl
   return slot < 0 || page >= P.sh.pages ? -1 : page;
 }
 
+// Many rows: which row a slot has (whichever was stored last where a slot is given twice), and, once that is known, the
+// pages: each by the lowest of its rows, in any order.
 __global__ void __launch_bounds__(256) kv8_rows_kernel(Kv8IoParams P) {
   griddep_launch_wait();
   const long long r = (long long)blockIdx.x * 256 + threadIdx.x;
-  if (r < P.tokens && kv8_page(P, P.slots[r]) >= 0) P.rows[P.slots[r]] = (int)r;
+  if (r < 2) P.pages[r] = 0;
+  if (r >= P.tokens) return;
+  const long long slot = P.slots[r];
+  if (kv8_page(P, slot) >= 0) P.rows[slot] = (int)r;
+  else if (slot >= 0) report_device_failure(kSiteIndex);
+}
+// The row of a slot, or -1; P.rows holds anything where this call gives none.
+__device__ __forceinline__ int kv8_row(const Kv8IoParams& P, long long slot) {
+  const int at = P.rows[slot];
+  return at >= 0 && at < P.tokens && P.slots[at] == slot ? at : -1;
+}
+constexpr int kKv8Seek = 4;  // rows of a warp, so that their look-ups wait together
+__global__ void __launch_bounds__(256) kv8_pages_kernel(Kv8IoParams P) {
+  griddep_launch_wait();
+  const int lane = threadIdx.x & 31;
+  const long long first = ((long long)blockIdx.x * 8 + (threadIdx.x >> 5)) * kKv8Seek;
+  long long page[kKv8Seek];
+  unsigned low[kKv8Seek];
+  int rows[kKv8Seek] = {};
+#pragma unroll
+  for (int i = 0; i < kKv8Seek; ++i) {
+    const long long r = first + i;
+    page[i] = r < P.tokens ? kv8_page(P, P.slots[r]) : -1;
+    low[i] = 0xffffffffu;
+    // The row before is lower, where it is the one that its slot has.
+    if (r > 0 && page[i] >= 0 && kv8_page(P, P.slots[r - 1]) == page[i] && P.rows[P.slots[r - 1]] == r - 1) page[i] = -1;
+  }
+  for (int j = lane; j < P.sh.page; j += 32)
+#pragma unroll
+    for (int i = 0; i < kKv8Seek; ++i)
+      if (page[i] >= 0) {
+        const int at = kv8_row(P, (page[i] << P.sh.shift) + j);
+        low[i] = min(low[i], (unsigned)at);  // (-1 is the largest)
+        rows[i] += at >= 0;
+      }
+#pragma unroll
+  for (int i = 0; i < kKv8Seek; ++i)
+    if (page[i] >= 0 && __reduce_min_sync(kFullMask, low[i]) == first + i) {
+      const bool thin = __reduce_add_sync(kFullMask, rows[i]) <= kKv8Thin;
+      if (lane == 0) {
+        const int at = atomicAdd(P.pages + !thin, 1);
+        P.list[thin ? at : P.tokens - 1 - at] = (int)(first + i);
+      }
+    }
 }
 
 // Threads and bytes. In a run of 16 tokens thread (chunk, t) holds channels 8 chunk to 8 chunk + 7 of tokens 2t, 2t + 1,
@@ -128,36 +176,12 @@ __device__ __forceinline__ uint32_t kv8_moved(uint32_t word, float old, float no
   return next;
 }
 
-// Up to kKv8Few rows: a CTA to a row, a warp to a head. A page is written by the CTA of the lowest of its rows, which finds the
-// others among all. Tokens one by one, four channels to a lane, and bytes stored where they belong, since a step of decoding
-// brings a page one: 64 tokens x 8 heads 3.7 us (with the kernel below 11.2), 256 5.0 (35).
+// A page's head whose new rows are few, by a warp: tokens one by one, four channels (64: two) to a lane, and bytes stored where they
+// belong, since a step of decoding brings a page one.
 template <typename T, int kDim, bool kVec>
-__global__ void __launch_bounds__(256) kv8_write_few_kernel(Kv8IoParams P) {
-  constexpr int kPer = kDim / 32;  // channels of a lane: 4, or 2
-  __shared__ int s_row[1024];
-  __shared__ unsigned s_low[8];
-  griddep_launch_wait();
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, r = blockIdx.x, head = blockIdx.y * 8 + warp;
-  const long long page = kv8_page(P, P.slots[r]);
-  if (page < 0) {
-    if (P.slots[r] >= 0 && tid == 0) report_device_failure(kSiteIndex);
-    return;
-  }
-  for (int j = tid; j < P.sh.page; j += 256) s_row[j] = -1;
-  __syncthreads();
-  unsigned low = 0xffffffffu;
-  for (int at = tid; at < P.tokens; at += 256) {
-    const long long slot = P.slots[at];
-    if (kv8_page(P, slot) == page) {
-      atomicMax(&s_row[(int)slot & (P.sh.page - 1)], at);
-      low = min(low, (unsigned)at);
-    }
-  }
-  low = __reduce_min_sync(kFullMask, low);
-  if (lane == 0) s_low[warp] = low;
-  __syncthreads();
-  low = __reduce_min_sync(kFullMask, s_low[lane & 7]);
-  if (low != (unsigned)r || head >= P.sh.heads) return;
+__device__ __forceinline__ void kv8_write_thin(const Kv8IoParams& P, const int* s_row, long long page, int head) {
+  constexpr int kPer = kDim / 32;  // channels of a lane
+  const int lane = threadIdx.x & 31;
   const int c0 = kPer * lane;
   const auto load = [&](T(&x)[2][kPer], int row) {
 #pragma unroll
@@ -244,163 +268,222 @@ __global__ void __launch_bounds__(256) kv8_write_few_kernel(Kv8IoParams P) {
   });
 }
 
-// More rows: a CTA takes a stretch of them and some heads. Rows of one page are written by one CTA, whichever holds the
-// lowest of them, so that nothing is shared: it finds all of the page's rows (s_row: the row of each
-// slot), their largest magnitude, and puts the runs that change together in shared memory, 64 tokens at a time: the
-// older codes, moved if the range grew, and the new ones over them. Up to 64 tokens a page, everything is read once.
-// 32768 tokens x 8 heads x 128 channels, bf16, from a page's first token 61 us, from within one 75.
+// Some heads of a page with more new rows, by the CTA: their largest magnitude, then the runs that change, put together in
+// shared memory, 64 tokens at a time: the older codes, moved if the range grew, and the new ones over them. Up to 64
+// tokens a page, everything is read once.
+template <int kDim>
+struct Kv8Thick {
+  static constexpr int kChunks = kDim / 8, kRunThreads = 4 * kChunks;  // threads of a run
+  static constexpr int kRuns = 4, kThreads = kRuns * kRunThreads;      // runs at a time
+  uint4 image[kRuns * 2 * kDim];
+  unsigned top[2][kThreads / 32];
+  unsigned char has[2][kThreads / 32];
+};
 template <typename T, int kDim, bool kVec>
-__global__ void __launch_bounds__(2 * kDim) kv8_write_kernel(Kv8IoParams P) {
-  constexpr int kChunks = kDim / 8, kRunThreads = 4 * kChunks;  // threads of a run
-  constexpr int kRuns = 4, kThreads = kRuns * kRunThreads;      // runs at a time
-  constexpr int kRun = 32 * kDim;
-  __shared__ uint4 s_image[kRuns * kRun / 16];
-  __shared__ int s_row[1024];
-  __shared__ unsigned s_low[kThreads / 32], s_top[2][kThreads / 32];
-  griddep_launch_wait();
-  const int head0 = blockIdx.y * P.span, heads = min(P.span, P.sh.heads - head0), tid = threadIdx.x, warp = tid >> 5;
-  const int t = tid & 3, chunk = (tid >> 2) % kChunks, mine = tid / kRunThreads;  // this thread's run of those at a time
-  const long long row0 = (long long)blockIdx.x * P.chunk, row1 = min(P.tokens, row0 + P.chunk);
-  for (long long r = row0; r < row1;) {
-    const long long page = kv8_page(P, P.slots[r]);
-    if (page < 0) {
-      if (P.slots[r] >= 0 && tid == 0) report_device_failure(kSiteIndex);
-      ++r;
-      continue;
-    }
-    // The rows of the page's slots, and the lowest of them; where this stretch leaves the page.
-    __syncthreads();  // the page before is done
-    unsigned low = 0xffffffffu, end = (unsigned)(row1 - r);
-    for (int j = tid; j < P.sh.page; j += kThreads) {
-      const long long slot = (page << P.sh.shift) + j;
-      const int at = P.rows[slot];  // whatever it held before, unless the row says so too
-      const bool is = at >= 0 && at < P.tokens && P.slots[at] == slot;
-      s_row[j] = is ? at : -1;
-      if (is) low = min(low, (unsigned)at);
-    }
-    for (long long i = r + 1 + (tid & 31); i < row1; i += 32)
-      if (kv8_page(P, P.slots[i]) != page) {
-        end = (unsigned)(i - r);
-        break;
+__device__ __forceinline__ void kv8_write_thick(const Kv8IoParams& P, Kv8Thick<kDim>& S, const int* s_row, long long page, int head0, int heads) {
+  using K = Kv8Thick<kDim>;
+  constexpr int kRuns = K::kRuns, kThreads = K::kThreads, kRunWarps = K::kRunThreads / 32, kRun = 32 * kDim;
+  const int tid = threadIdx.x, warp = tid >> 5;
+  const int t = tid & 3, chunk = (tid >> 2) % K::kChunks, mine = tid / K::kRunThreads;  // this thread's run of those at a time
+  const int runs = P.sh.page / 16;
+  uint4 x[2][4];  // this thread's tokens of a run: keys, values
+  int rows[4];
+  const auto fetch = [&](int head, int run) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) rows[i] = run < runs ? s_row[16 * run + kv8_token(t, i)] : -1;
+#pragma unroll
+    for (int part = 0; part < 2; ++part)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        x[part][i] = make_uint4(0, 0, 0, 0);
+        if (rows[i] >= 0) {
+          const T* from = part ? static_cast<const T*>(P.v) + rows[i] * P.v_ts + head * P.v_hs : static_cast<const T*>(P.k) + rows[i] * P.k_ts + head * P.k_hs;
+          if constexpr (kVec) {
+            x[part][i] = __ldg(reinterpret_cast<const uint4*>(from + 8 * chunk));
+          } else {
+            alignas(16) T y[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) y[e] = from[8 * chunk + e];
+            x[part][i] = *reinterpret_cast<const uint4*>(y);
+          }
+        }
       }
-    end = __reduce_min_sync(kFullMask, end);
-    low = __reduce_min_sync(kFullMask, low);
-    if ((tid & 31) == 0) s_low[warp] = low;
+  };
+  unsigned char* image = reinterpret_cast<unsigned char*>(S.image);
+  if (runs <= kRuns) fetch(head0, mine);
+  for (int head = head0; head < head0 + heads; ++head) {
+    uint32_t top[2] = {0, 0};
+    for (int base = 0; base < runs; base += kRuns) {
+      if (runs > kRuns) fetch(head, base + mine);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) top[0] = kv8_top(top[0], x[0][i]), top[1] = kv8_top(top[1], x[1][i]);
+    }
+#pragma unroll
+    for (int part = 0; part < 2; ++part) {
+      const unsigned most = __reduce_max_sync(kFullMask, kv8_top_bits<T>(top[part]));
+      if ((tid & 31) == 0) S.top[part][warp] = most;
+    }
     __syncthreads();
-    low = __reduce_min_sync(kFullMask, s_low[tid & (kThreads / 32 - 1)]);
-    const bool leads = low >= r && low < r + end;
-    r += end;
-    if (!leads) continue;
-    const int runs = P.sh.page / 16;
-    uint4 x[2][4];  // this thread's tokens of a run: keys, values
-    int rows[4];
-    const auto fetch = [&](int head, int run) {
+    float* range = P.range + (page * P.sh.heads + head) * 2;
+    unsigned char* block = P.codes + (page * P.sh.heads + head) * P.sh.block_bytes();
+    const bool fresh = s_row[0] >= 0;
+    float old[2], now[2], inv[2];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) rows[i] = run < runs ? s_row[16 * run + kv8_token(t, i)] : -1;
-#pragma unroll
-      for (int part = 0; part < 2; ++part)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          x[part][i] = make_uint4(0, 0, 0, 0);
-          if (rows[i] >= 0) {
-            const T* from = part ? static_cast<const T*>(P.v) + rows[i] * P.v_ts + head * P.v_hs : static_cast<const T*>(P.k) + rows[i] * P.k_ts + head * P.k_hs;
-            if constexpr (kVec) {
-              x[part][i] = __ldg(reinterpret_cast<const uint4*>(from + 8 * chunk));
-            } else {
-              alignas(16) T y[8];
-#pragma unroll
-              for (int e = 0; e < 8; ++e) y[e] = from[8 * chunk + e];
-              x[part][i] = *reinterpret_cast<const uint4*>(y);
-            }
-          }
-        }
-    };
-    unsigned char* image = reinterpret_cast<unsigned char*>(s_image);
-    if (runs <= kRuns) fetch(head0, mine);
-    for (int head = head0; head < head0 + heads; ++head) {
-      uint32_t top[2] = {0, 0};
-      for (int base = 0; base < runs; base += kRuns) {
-        if (runs > kRuns) fetch(head, base + mine);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) top[0] = kv8_top(top[0], x[0][i]), top[1] = kv8_top(top[1], x[1][i]);
-      }
-#pragma unroll
-      for (int part = 0; part < 2; ++part) {
-        const unsigned most = __reduce_max_sync(kFullMask, kv8_top_bits<T>(top[part]));
-        if ((tid & 31) == 0) s_top[part][warp] = most;
-      }
+    for (int part = 0; part < 2; ++part) {
+      const float grown = kv8_range<T>(__reduce_max_sync(kFullMask, S.top[part][tid & (kThreads / 32 - 1)]));
+      old[part] = fresh ? 0.f : range[part];
+      now[part] = grown == grown && old[part] == old[part] ? fmaxf(grown, old[part]) : __int_as_float(0x7fffffff);
+      inv[part] = now[part] > 0.f ? kv8_inverse(now[part]) : 0.f;
+    }
+    const bool move[2] = {now[0] == now[0] && (fresh || now[0] != old[0]), now[1] == now[1] && (fresh || now[1] != old[1])};
+    __syncthreads();  // every thread has read the older range
+    if (tid < 2) range[tid] = now[tid];
+    for (int base = 0; base < runs; base += kRuns) {
+      if (runs > kRuns) fetch(head, base + mine);
+      const bool any = rows[0] >= 0 || rows[1] >= 0 || rows[2] >= 0 || rows[3] >= 0;
+      const bool all = rows[0] >= 0 && rows[1] >= 0 && rows[2] >= 0 && rows[3] >= 0;
+      // Of each run, whether anything is written and whether it is filled (a run's threads are whole warps).
+      const bool some = __any_sync(kFullMask, any), whole = __all_sync(kFullMask, all);
+      unsigned char* has = S.has[base / kRuns & 1];
+      if ((tid & 31) == 0) has[warp] = (some ? 1 : 0) | (whole ? 2 : 0);
       __syncthreads();
-      float* range = P.range + (page * P.sh.heads + head) * 2;
-      unsigned char* block = P.codes + (page * P.sh.heads + head) * P.sh.block_bytes();
-      const bool fresh = s_row[0] >= 0;
-      float old[2], now[2], inv[2];
+      unsigned changed = 0, filled = 0;
 #pragma unroll
-      for (int part = 0; part < 2; ++part) {
-        const float grown = kv8_range<T>(__reduce_max_sync(kFullMask, s_top[part][tid & (kThreads / 32 - 1)]));
-        old[part] = fresh ? 0.f : range[part];
-        now[part] = grown == grown && old[part] == old[part] ? fmaxf(grown, old[part]) : __int_as_float(0x7fffffff);
-        inv[part] = now[part] > 0.f ? kv8_inverse(now[part]) : 0.f;
+      for (int i = 0; i < kRuns; ++i) {
+        unsigned either = has[i * kRunWarps], both = either;
+        if (kRunWarps == 2) either |= has[2 * i + 1], both &= has[2 * i + 1];
+        if (base + i < runs) changed |= ((either & 1) || move[0] || move[1] ? 1u : 0u) << i;
+        filled |= (both >> 1) << i;
       }
-      const bool move[2] = {now[0] == now[0] && (fresh || now[0] != old[0]), now[1] == now[1] && (fresh || now[1] != old[1])};
-      __syncthreads();  // every thread has read the older range
-      if (tid < 2) range[tid] = now[tid];
-      for (int base = 0; base < runs; base += kRuns) {
-        if (runs > kRuns) fetch(head, base + mine);
-        const bool any = rows[0] >= 0 || rows[1] >= 0 || rows[2] >= 0 || rows[3] >= 0;
-        const bool all = rows[0] >= 0 && rows[1] >= 0 && rows[2] >= 0 && rows[3] >= 0;
-        // Of each run, whether it is written at all and whether it is filled (a run's threads are whole warps).
-        const int count = __syncthreads_count(any);
-        if (count == 0 && !move[0] && !move[1]) continue;  // (never where the page is taken at once)
-        const bool filled = __syncthreads_and(all || base + mine >= runs);
-        if (!filled) {
-          // The older codes first, moved to the new range, or zeros.
-          for (int at = tid; at < kRuns * kRun / 16; at += kThreads) {
-            if (base + at * 16 / kRun >= runs) break;
-            const int part = at / kDim & 1;
-            uint4 w = make_uint4(kKv8Zeros, kKv8Zeros, kKv8Zeros, kKv8Zeros);
-            if (!move[part] || old[part] > 0.f) w = reinterpret_cast<const uint4*>(block + (long long)base * kRun)[at];
-            if (move[part] && old[part] > 0.f)
-              w = make_uint4(kv8_moved(w.x, old[part], now[part]), kv8_moved(w.y, old[part], now[part]), kv8_moved(w.z, old[part], now[part]),
-                             kv8_moved(w.w, old[part], now[part]));
-            s_image[at] = w;
-          }
-          __syncthreads();
-        }
-        if (any) {
-          unsigned char* run = image + mine * kRun;
-          uint32_t f[4][8];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            kv8_bytes<T>(f[i], x[0][i], inv[0]);
-            if (rows[i] >= 0) {
-              uint32_t* to = reinterpret_cast<uint32_t*>(run + kv8_key_at(kDim, kv8_token(t, i), 8 * chunk));
-              to[0] = kv8_word(f[i][0], f[i][1], f[i][2], f[i][3]);
-              to[4] = kv8_word(f[i][4], f[i][5], f[i][6], f[i][7]);
-            }
-          }
-#pragma unroll
-          for (int i = 0; i < 4; ++i) kv8_bytes<T>(f[i], x[1][i], inv[1]);
-          unsigned char* to = run + kv8_value_at(kDim, 2 * t, 8 * chunk);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            if (all) {
-              *reinterpret_cast<uint32_t*>(to + 64 * e) = kv8_word(f[0][e], f[1][e], f[2][e], f[3][e]);
-            } else {
-#pragma unroll
-              for (int i = 0; i < 4; ++i)
-                if (rows[i] >= 0) to[64 * e + i] = (unsigned char)f[i][e];
-            }
-          }
+      if (changed == 0) continue;  // (never where the page is taken at once)
+      if (changed & ~filled) {
+        // The older codes first, moved to the new range, or zeros.
+#pragma unroll 4
+        for (int at = tid; at < kRuns * kRun / 16; at += kThreads) {
+          if (!((changed & ~filled) >> (at * 16 / kRun) & 1)) continue;
+          const int part = at / kDim & 1;
+          uint4 w = make_uint4(kKv8Zeros, kKv8Zeros, kKv8Zeros, kKv8Zeros);
+          if (!move[part] || old[part] > 0.f) w = reinterpret_cast<const uint4*>(block + (long long)base * kRun)[at];
+          if (move[part] && old[part] > 0.f)
+            w = make_uint4(kv8_moved(w.x, old[part], now[part]), kv8_moved(w.y, old[part], now[part]), kv8_moved(w.z, old[part], now[part]),
+                           kv8_moved(w.w, old[part], now[part]));
+          S.image[at] = w;
         }
         __syncthreads();
-        if (runs <= kRuns && head + 1 < head0 + heads) fetch(head + 1, mine);  // under way while this head's bytes leave
-        for (int at = tid; at < kRuns * kRun / 16; at += kThreads) {
-          if (base + at * 16 / kRun >= runs) break;
-          reinterpret_cast<uint4*>(block + (long long)base * kRun)[at] = s_image[at];
-        }
-        __syncthreads();  // the image is free
       }
+      if (any) {
+        unsigned char* run = image + mine * kRun;
+        uint32_t f[4][8];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          kv8_bytes<T>(f[i], x[0][i], inv[0]);
+          if (rows[i] >= 0) {
+            uint32_t* to = reinterpret_cast<uint32_t*>(run + kv8_key_at(kDim, kv8_token(t, i), 8 * chunk));
+            to[0] = kv8_word(f[i][0], f[i][1], f[i][2], f[i][3]);
+            to[4] = kv8_word(f[i][4], f[i][5], f[i][6], f[i][7]);
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) kv8_bytes<T>(f[i], x[1][i], inv[1]);
+        unsigned char* to = run + kv8_value_at(kDim, 2 * t, 8 * chunk);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          if (all) {
+            *reinterpret_cast<uint32_t*>(to + 64 * e) = kv8_word(f[0][e], f[1][e], f[2][e], f[3][e]);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (rows[i] >= 0) to[64 * e + i] = (unsigned char)f[i][e];
+          }
+        }
+      }
+      __syncthreads();
+      if (runs <= kRuns && head + 1 < head0 + heads) fetch(head + 1, mine);  // under way while this head's bytes leave
+      for (int at = tid; at < kRuns * kRun / 16; at += kThreads) {
+        if (changed >> (at * 16 / kRun) & 1) reinterpret_cast<uint4*>(block + (long long)base * kRun)[at] = S.image[at];
+      }
+      __syncthreads();  // the image is free
     }
+  }
+}
+
+// Up to kKv8Few rows, in one launch: a CTA to a row and two heads or four. The CTA of the lowest of a page's rows finds the
+// others among all. (8 heads x 128 channels: single tokens of 64 sequences 3.7 us, of 256 6.5, of 1024 20.5; 64 tokens of one 9.3,
+// 500 17.5. Through the lists below: 14, 14, 23; 16, 18, and 12 for a chunk of 128.)
+template <typename T, int kDim, bool kVec>
+__global__ void __launch_bounds__(2 * kDim) kv8_write_few_kernel(Kv8IoParams P) {
+  constexpr int kThreads = 2 * kDim;
+  __shared__ Kv8Thick<kDim> s_thick;
+  __shared__ int s_row[1024];
+  __shared__ unsigned s_low[kThreads / 32];
+  griddep_launch_wait();
+  const int tid = threadIdx.x, r = blockIdx.x;
+  const long long page = kv8_page(P, P.slots[r]);
+  if (page < 0) {
+    if (P.slots[r] >= 0 && tid == 0) report_device_failure(kSiteIndex);
+    return;
+  }
+  for (int j = tid; j < P.sh.page; j += kThreads) s_row[j] = -1;
+  __syncthreads();
+  unsigned low = 0xffffffffu;
+  int rows = 0;
+  for (int at = tid; at < P.tokens; at += kThreads) {
+    const long long slot = P.slots[at];
+    if (kv8_page(P, slot) == page) {
+      atomicMax(&s_row[(int)slot & (P.sh.page - 1)], at);
+      low = min(low, (unsigned)at);
+      rows = 1;
+    }
+  }
+  low = __reduce_min_sync(kFullMask, low);
+  if ((tid & 31) == 0) s_low[tid >> 5] = low;
+  rows = __syncthreads_count(rows > 0);
+  low = __reduce_min_sync(kFullMask, s_low[tid & (kThreads / 32 - 1)]);
+  if (low != (unsigned)r) return;
+  const int head0 = blockIdx.y * P.span;
+  const int heads = min(P.span, P.sh.heads - head0);
+  if (rows > kKv8Thin) kv8_write_thick<T, kDim, kVec>(P, s_thick, s_row, page, head0, heads);
+  else if (tid >> 5 < heads) kv8_write_thin<T, kDim, kVec>(P, s_row, page, head0 + (tid >> 5));
+}
+
+// More: of the pages' heads, in order, each warp takes as many as any other, (2048 single tokens x 8 heads x 128 channels 33 us;
+// by CTAs, as below, 202)
+constexpr int kKv8ThinWarps = 4;
+template <typename T, int kDim, bool kVec>
+__global__ void __launch_bounds__(32 * kKv8ThinWarps) kv8_write_thin_kernel(Kv8IoParams P) {
+  __shared__ int s_row[kKv8ThinWarps][1024];
+  griddep_launch_wait();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const long long units = (long long)P.pages[0] * P.sh.heads, warps = gridDim.x * (long long)kKv8ThinWarps, per = (units + warps - 1) / warps;
+  const long long first = (blockIdx.x * (long long)kKv8ThinWarps + warp) * per, end = min(units, first + per);
+  for (long long unit = first; unit < end; ++unit) {
+    const int head = (int)(unit % P.sh.heads);
+    const long long page = kv8_page(P, P.slots[P.list[unit / P.sh.heads]]);
+    if (unit == first || head == 0) {
+      __syncwarp();  // the page before is done
+      for (int j = lane; j < P.sh.page; j += 32) s_row[warp][j] = kv8_row(P, (page << P.sh.shift) + j);
+      __syncwarp();
+    }
+    kv8_write_thin<T, kDim, kVec>(P, s_row[warp], page, head);
+  }
+}
+// and each CTA. 32768 tokens x 8 heads x 128 channels, bf16: 71 us from a page's first token, 73 from within one, 2.9 TB/s of
+// keys, values and codes; in instructions and their order, the two kernels before it 8 of them. (Both sorts of pages in one kernel:
+// 75 and 80, the registers of the one hold up the other.)
+template <typename T, int kDim, bool kVec>
+__global__ void __launch_bounds__(2 * kDim) kv8_write_kernel(Kv8IoParams P) {
+  __shared__ Kv8Thick<kDim> s_thick;
+  __shared__ int s_row[1024];
+  griddep_launch_wait();
+  const long long units = (long long)P.pages[1] * P.sh.heads, per = (units + gridDim.x - 1) / gridDim.x, end = min(units, (blockIdx.x + 1) * per);
+  for (long long unit = blockIdx.x * per; unit < end;) {
+    const int head0 = (int)(unit % P.sh.heads), heads = (int)min((long long)(P.sh.heads - head0), end - unit);
+    const long long page = kv8_page(P, P.slots[P.list[P.tokens - 1 - unit / P.sh.heads]]);
+    unit += heads;
+    __syncthreads();  // the page before is done
+    for (int j = threadIdx.x; j < P.sh.page; j += 2 * kDim) s_row[j] = kv8_row(P, (page << P.sh.shift) + j);
+    __syncthreads();
+    kv8_write_thick<T, kDim, kVec>(P, s_thick, s_row, page, head0, heads);
   }
 }
 

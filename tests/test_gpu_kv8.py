@@ -132,6 +132,22 @@ def test_many_tokens_as_few(tokens):
     short.check(caches[2], slots)
 
 
+@pytest.mark.parametrize("dtype, dim, page, pages", [(BF, 128, 64, 300), (HF, 64, 16, 400), (BF, 64, 256, 120), (HF, 128, 1024, 12)])
+def test_pages_that_get_few_tokens_and_pages_that_get_many(dtype, dim, page, pages):
+    # more than 1024 rows in a call, from one to all of a page's; a second call over the first, larger, so that codes move
+    heads = 3
+    cache, model = qr.kv8_cache(pages, page, heads, dim, dtype=dtype), Model(pages, page, heads, dim)
+    for turn in range(2):
+        counts = [1, 8, 9, 2, page, 7, 10][turn:]
+        slots = torch.cat([p * page + torch.randperm(page, generator=_gen(100 * turn + p), device="cuda")[: min(page, counts[p % len(counts)])] for p in range(pages)])
+        slots = slots[torch.randperm(len(slots), generator=_gen(turn), device="cuda")]
+        assert len(slots) > 1024
+        k, v = _randn(len(slots), heads, dim, seed=turn, dtype=dtype, size=1 + 2 * turn), _randn(len(slots), heads, dim, seed=7 + turn, dtype=dtype, size=4 - 3 * turn)
+        qr.kv8_write(cache, k, v, slots)
+        model.write(k, v, slots)
+        model.check(cache, _all(cache))
+
+
 def test_rest_of_a_page_begun_anew_reads_as_zeros():
     cache = qr.kv8_cache(2, 32, 1, 64)
     qr.kv8_write(cache, _randn(64, 1, 64, seed=1), _randn(64, 1, 64, seed=2), torch.arange(64, device="cuda"))
