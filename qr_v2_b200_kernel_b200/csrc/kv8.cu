@@ -161,9 +161,11 @@ int qrb200_kv8_write(void* codes, float* range, const qrb200_kv8_shape* shape, c
   const cudaError_t e = with_shape(shape->dtype, h.dim, [&](auto type, auto dim) {
     using E = decltype(type);
     if (!p.rows) {
-      // (64 tokens of a page x 8 heads 9.4 us with two heads to a CTA, 15.9 with four; 256 single tokens 11.3, 6.6.)
-      p.span = tokens <= 64 ? 2 : 4;
-      LaunchShape l(dim3((unsigned)tokens, ceil_div(h.heads, p.span)), 2 * h.dim, 0, s);
+      // The fewer CTAs, the better this kernel and the next overlap (64 single tokens x 8 heads, written and read back: with
+      // eight heads to a CTA 9.2 us, four 14.1, two 14.2; from 128 on all the same); the more, the sooner a chunk of one
+      // sequence is done (12 tokens 22.6, 12.3, 7.3; 64 42.9, 22.3, 12.6).
+      p.span = tokens <= 16 ? 2 : tokens <= 32 ? 4 : tokens <= 64 ? 8 : 4;
+      LaunchShape l(dim3((unsigned)tokens, ceil_div(h.heads, p.span)), 256, 0, s);
       return cudaLaunchKernelEx(&l.cfg, vec ? kv8_write_few_kernel<E, dim(), true> : kv8_write_few_kernel<E, dim(), false>, p);
     }
     // Eight CTAs to an SM: a page's rows are looked up once for several heads then, and the next head's loads are under

@@ -104,7 +104,7 @@ def test_token_by_token_and_begun_anew(dtype, dim):
             model.check(cache, _all(cache))
 
 
-@pytest.mark.parametrize("tokens", [1024, 1025, 5000])
+@pytest.mark.parametrize("tokens", [255, 256, 257, 1024, 1025, 5000])
 def test_many_tokens_as_few(tokens):
     # the same rows in one call, whichever way their pages are looked up, and in the order of time
     heads, dim, page, batch = 2, 64, 64, 5
@@ -134,7 +134,7 @@ def test_many_tokens_as_few(tokens):
 
 @pytest.mark.parametrize("dtype, dim, page, pages", [(BF, 128, 64, 300), (HF, 64, 16, 400), (BF, 64, 256, 120), (HF, 128, 1024, 12)])
 def test_pages_that_get_few_tokens_and_pages_that_get_many(dtype, dim, page, pages):
-    # more than 1024 rows in a call, from one to all of a page's; a second call over the first, larger, so that codes move
+    # many rows in a call, from one to all of a page's; a second call over the first, larger, so that codes move
     heads = 3
     cache, model = qr.kv8_cache(pages, page, heads, dim, dtype=dtype), Model(pages, page, heads, dim)
     for turn in range(2):
