@@ -117,7 +117,8 @@ __global__ void __launch_bounds__(32 * kFp8RowsWarps, 2) fp8_rows_linear_kernel(
 // CTA then adds all the CTAs' sums of some rows of x, in their order, through distributed shared memory.
 //
 // Warp 0 issues the loads, warp 1 the MMAs into two accumulators in turn, warps 2-5 hold one output
-// channel a lane and kBN sums each.
+// channel a lane and kBN sums each. 4096 x 4096: 16 rows 6.3 us, 64 8.2, 128 10.7, that is 2.7 to 1.6 TB/s of weights: the
+// set-up, the first loads and the join of the cut depth are most of it (333 x 1000 x 2000 8.3).
 constexpr int kFp8Split = 4;  // the most CTAs that share a tile's depth
 constexpr int kFp8Scales = 8;  // blocks whose scales are held at a time
 template <int kBN>

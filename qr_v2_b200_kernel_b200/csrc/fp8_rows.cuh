@@ -122,7 +122,8 @@ __device__ __forceinline__ void fp8_store(uint8_t* q, const uint32_t (&word)[kVe
 }
 
 // Blocks of a row: a pack (16 bytes) to a thread, so 16 (32-bit entries: 32) threads to a block, kItems
-// blocks to a thread, all asked for before the first is used.
+// blocks to a thread, all asked for before the first is used. 16384 x 4096 bf16: 40 us, 5.0 TB/s (one block to a thread, and
+// unpacked maxima and quotients: 75); the quotients' instructions and the bytes are about level.
 template <typename T, bool kAligned, int kItems>
 __global__ void __launch_bounds__(256) fp8_rows_kernel(Fp8RowsParams P) {
   constexpr int kVec = 16 / sizeof(T), kSpan = kFp8Block / kVec, kPer = 256 / kSpan;  // threads of a block; blocks at a time
@@ -167,9 +168,10 @@ __global__ void __launch_bounds__(256) fp8_rows_kernel(Fp8RowsParams P) {
   }
 }
 
-// Blocks of 128 rows and 128 columns, one to a CTA, held in registers between the maximum and the codes.
+// Blocks of 128 rows and 128 columns, one to a CTA, held in registers between the maximum and the codes. 5000 x 2040 fp32: 14 us,
+// 3.7 TB/s (three CTAs an SM; two, in the registers that it would take, 17); 16384 x 4096 bf16 38, 5.3.
 template <typename T, bool kAligned>
-__global__ void __launch_bounds__(512) fp8_tiles_kernel(Fp8RowsParams P) {
+__global__ void __launch_bounds__(512, 3) fp8_tiles_kernel(Fp8RowsParams P) {
   constexpr int kVec = 16 / sizeof(T), kSpan = kFp8Block / kVec, kStep = 512 / kSpan, kItems = kFp8Block / kStep;
   __shared__ unsigned s_top[16];
   griddep_launch_wait();
@@ -208,7 +210,8 @@ __global__ void __launch_bounds__(512) fp8_tiles_kernel(Fp8RowsParams P) {
 }
 
 // value = code * scale of its block, rounded once: four packs of 16 bytes of values to a thread, a CTA's width apart,
-// where both sides' rows start on 16-byte boundaries (kPacked), else eight values, a warp on 256 neighbouring ones.
+// where both sides' rows start on 16-byte boundaries (kPacked), else eight values, a warp on 256 neighbouring ones. 16384 x 4096
+// to bf16 32 us, 6.3 TB/s; 8192 x 2047 to fp16 14 us, 3.6.
 struct Fp8ValuesParams {
   const uint8_t* q;
   const float* scale;

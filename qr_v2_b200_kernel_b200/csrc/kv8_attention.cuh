@@ -4,6 +4,10 @@
 //   q . k_t = r_t (q . c_t),     o = sum_t (p_t w_t) c_t.
 // So the codes are the matrix operands, exact in 16 bits: a byte c + 128 under the exponent of 1024 is the fp16 number
 // 1152 + c, one addition away from c. No key or value is ever rounded; steps are applied in 32 bits.
+//
+// 64 sequences of 8192 tokens, 8 heads of 128 channels with 8 query rows each, bf16: 172 us for 1.07 GB, 6.2 TB/s (under the power
+// cap, 208). The bytes bound it there, with issue slots 64 % busy; fewer or shorter sequences wait for a chain of latencies (one
+// of 513 tokens 7.3 us). A CTA's four warps take a quarter of its tokens each, so nothing is shared until the end.
 #pragma once
 
 #include <type_traits>
