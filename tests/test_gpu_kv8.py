@@ -649,3 +649,45 @@ def test_repeated_calls_agree():
         out = qr.kv8_attention(q, cache, table, _lengths(3000, 1777, 2048))
         for _ in range(5):
             assert torch.equal(qr.kv8_attention(q, cache, table, _lengths(3000, 1777, 2048)), out)
+
+
+def test_calls_at_the_same_time():
+    # writes by lists of pages, attention through memory, of prompts and of single tokens, and products, each on its own
+    # stream and at once, eager and from two graphs
+    heads, dim, page = 2, 128, 64
+    cache, table, _ = _filled(2, 8192, heads, dim, page, BF)
+    one, many = _randn(1, 1, 8, dim), _randn(2, 300, 8, dim, seed=1)
+    x, sx = qr.quantize_fp8(_randn(700, 512, seed=2))
+    w, sw = qr.quantize_fp8(_randn(1024, 512, seed=3), tile_rows=128)
+    k = _randn(1500, heads, dim, seed=4)
+    order = [torch.randperm(64 * page, generator=_gen(i), device="cuda")[:1500] for i in range(2)]
+    own = [qr.kv8_cache(64, page, heads, dim) for _ in range(2)]
+
+    def write(i):
+        qr.kv8_write(own[i], k, k, order[i])
+        return qr.kv8_read(own[i], order[i])[0]
+
+    calls = [lambda: write(0), lambda: write(1), lambda: qr.kv8_attention(one, cache, table[:1], _lengths_of),
+             lambda: qr.kv8_attention(many, cache, table, _lengths_two), lambda: qr.fp8_linear(x, sx, w, sw), lambda: qr.fp8_linear(x[:40], sx[:40], w, sw)]
+    _lengths_of, _lengths_two = _lengths(8192), _lengths(5000, 8192)
+    want = [f().clone() for f in calls]
+    streams = [torch.cuda.Stream() for _ in calls]
+    torch.cuda.synchronize()
+    for _ in range(3):
+        got = []
+        for f, s in zip(calls, streams):
+            with torch.cuda.stream(s):
+                got.append([f() for _ in range(4)])
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for out, b in zip(got, want) for a in out)
+    graphs, outs = [], []
+    for part in (0, 1):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            outs.append([f() for f in calls[part::2]])
+    for _ in range(3):
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for part in (0, 1) for a, b in zip(outs[part], want[part::2]))
