@@ -163,7 +163,7 @@ int qrb200_kv8_write(void* codes, float* range, const qrb200_kv8_shape* shape, c
     if (!p.rows) {
       // The fewer CTAs, the better this kernel and the next overlap (64 single tokens x 8 heads, written and read back: with
       // eight heads to a CTA 9.2 us, four 14.1, two 14.2; from 128 on all the same); the more, the sooner a chunk of one
-      // sequence is done (12 tokens 22.6, 12.3, 7.3; 64 42.9, 22.3, 12.6).
+      // sequence is done (128 tokens 34, 26, 25).
       p.span = tokens <= 16 ? 2 : tokens <= 32 ? 4 : tokens <= 64 ? 8 : 4;
       LaunchShape l(dim3((unsigned)tokens, ceil_div(h.heads, p.span)), 256, 0, s);
       return cudaLaunchKernelEx(&l.cfg, vec ? kv8_write_few_kernel<E, dim(), true> : kv8_write_few_kernel<E, dim(), false>, p);

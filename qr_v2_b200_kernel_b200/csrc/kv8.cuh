@@ -176,16 +176,12 @@ __device__ __forceinline__ uint32_t kv8_moved(uint32_t word, float old, float no
   return next;
 }
 
-// A page's head whose new rows are few, by a warp or (kTeam) a CTA of eight, four rows at a time to each: tokens one by one, four
-// channels (64: two) to a lane, and bytes stored where they belong, since a step of decoding brings a page one.
-template <typename T, int kDim, bool kVec, bool kTeam>
-__device__ __forceinline__ void kv8_write_thin(const Kv8IoParams& P, const int* s_row, unsigned (*s_top)[2], long long page, int head) {
+// A page's head whose new rows are few, by a warp: tokens one by one, four channels (64: two) to a lane, and bytes stored where they
+// belong, since a step of decoding brings a page one.
+template <typename T, int kDim, bool kVec>
+__device__ __forceinline__ void kv8_write_thin(const Kv8IoParams& P, const int* s_row, long long page, int head) {
   constexpr int kPer = kDim / 32;  // channels of a lane
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const auto sync = [&]() {
-    if (kTeam) __syncthreads();
-    else __syncwarp();
-  };
+  const int lane = threadIdx.x & 31;
   const int c0 = kPer * lane;
   const auto load = [&](T(&x)[2][kPer], int row) {
 #pragma unroll
@@ -201,11 +197,11 @@ __device__ __forceinline__ void kv8_write_thin(const Kv8IoParams& P, const int* 
       }
     }
   };
-  // f(token, row) for the page's new tokens, eight at a time.
+  // f(token, row) for the page's new tokens, loaded four at a time (eight change nothing).
   const auto each = [&](auto f) {
     for (int base = 0; base < P.sh.page; base += 32) {
       const int mine = base + lane < P.sh.page ? s_row[base + lane] : -1;
-      unsigned have = __ballot_sync(kFullMask, mine >= 0 && (!kTeam || ((base + lane) >> 2 & 7) == warp));
+      unsigned have = __ballot_sync(kFullMask, mine >= 0);
       while (have) {
         alignas(8) T x[4][2][kPer];
         int token[4];
@@ -229,11 +225,6 @@ __device__ __forceinline__ void kv8_write_thin(const Kv8IoParams& P, const int* 
       for (int e = 0; e < kPer; ++e) top[part] = max(top[part], __float_as_uint(to_f32(x[part][e])) & 0x7fffffffu);
   });
   for (int part = 0; part < 2; ++part) top[part] = __reduce_max_sync(kFullMask, top[part]);
-  if constexpr (kTeam) {
-    if (lane == 0) s_top[warp][0] = top[0], s_top[warp][1] = top[1];
-    __syncthreads();
-    for (int part = 0; part < 2; ++part) top[part] = __reduce_max_sync(kFullMask, s_top[lane & 7][part]);
-  }
   float* range = P.range + (page * P.sh.heads + head) * 2;
   unsigned char* block = P.codes + (page * P.sh.heads + head) * P.sh.block_bytes();
   const bool fresh = s_row[0] >= 0;
@@ -247,11 +238,11 @@ __device__ __forceinline__ void kv8_write_thin(const Kv8IoParams& P, const int* 
     inv[part] = now[part] > 0.f ? kv8_inverse(now[part]) : 0.f;
     move[part] = now[part] == now[part] && (fresh || now[part] != old[part]);
   }
-  sync();  // every lane has read the older range
-  if (lane < 2 && (!kTeam || warp == 0)) range[lane] = now[lane];
+  __syncwarp();  // every lane has read the older range
+  if (lane < 2) range[lane] = now[lane];
   if (move[0] || move[1]) {
 #pragma unroll 4
-    for (int at = kTeam ? threadIdx.x : lane; at < P.sh.block_bytes() / 16; at += kTeam ? 256 : 32) {
+    for (int at = lane; at < P.sh.block_bytes() / 16; at += 32) {
       const int part = at / kDim & 1;
       if (!move[part]) continue;
       uint4 w = make_uint4(kKv8Zeros, kKv8Zeros, kKv8Zeros, kKv8Zeros);
@@ -262,7 +253,7 @@ __device__ __forceinline__ void kv8_write_thin(const Kv8IoParams& P, const int* 
       }
       reinterpret_cast<uint4*>(block)[at] = w;
     }
-    sync();  // before the new codes go into the same words
+    __syncwarp();  // before the new codes go into the same words
   }
   each([&](int token, const T(&x)[2][kPer]) {
     uint32_t f[2][kPer];
@@ -279,13 +270,13 @@ __device__ __forceinline__ void kv8_write_thin(const Kv8IoParams& P, const int* 
 }
 
 // Up to kKv8Few rows, in one launch: a CTA to a row and some heads. The CTA of the lowest of a page's rows finds the others
-// among all. (8 heads x 128 channels: single tokens of 16 sequences 3.7 us, of 256 4.4, of 1024 13.2; 128 tokens of one 25.8,
-// 500 31.9. Through the lists below: 14 for 128 to 256 single tokens, 18 for 512, 23 for 1024; 12 and 18 for the chunks.)
+// among all. (8 heads x 128 channels: single tokens of 16 sequences 3.5 us, of 256 4.2; 64 tokens of one 29, 128 26; a CTA's
+// eight warps to a head, one head after another, 43 and 26. Through the lists below: 14 for 128 to 256 single tokens, 18 for 512, 23 for 1024; 12 and 18 for the chunks.)
 template <typename T, int kDim, bool kVec>
 __global__ void __launch_bounds__(256) kv8_write_few_kernel(Kv8IoParams P) {
   constexpr int kThreads = 256;
   __shared__ int s_row[1024];
-  __shared__ unsigned s_low[8], s_top[8][2];
+  __shared__ unsigned s_low[8];
   griddep_launch_wait();
   const int tid = threadIdx.x, r = blockIdx.x;
   const long long page = kv8_page(P, P.slots[r]);
@@ -296,26 +287,21 @@ __global__ void __launch_bounds__(256) kv8_write_few_kernel(Kv8IoParams P) {
   for (int j = tid; j < P.sh.page; j += kThreads) s_row[j] = -1;
   __syncthreads();
   unsigned low = 0xffffffffu;
-  int rows = 0;
   for (int at = tid; at < P.tokens; at += kThreads) {
     const long long slot = P.slots[at];
     if (kv8_page(P, slot) == page) {
       atomicMax(&s_row[(int)slot & (P.sh.page - 1)], at);
       low = min(low, (unsigned)at);
-      rows = 1;
     }
   }
   low = __reduce_min_sync(kFullMask, low);
   if ((tid & 31) == 0) s_low[tid >> 5] = low;
-  rows = __syncthreads_count(rows > 0);
+  __syncthreads();
   low = __reduce_min_sync(kFullMask, s_low[tid & 7]);
   if (low != (unsigned)r) return;
   const int head0 = blockIdx.y * P.span;
   const int heads = min(P.span, P.sh.heads - head0);
-  if (rows > kKv8Thin)
-    for (int head = 0; head < heads; ++head) kv8_write_thin<T, kDim, kVec, true>(P, s_row, s_top, page, head0 + head);
-  else if (tid >> 5 < heads)
-    kv8_write_thin<T, kDim, kVec, false>(P, s_row, s_top, page, head0 + (tid >> 5));
+  if (tid >> 5 < heads) kv8_write_thin<T, kDim, kVec>(P, s_row, page, head0 + (tid >> 5));
 }
 
 // Some heads of a page with more new rows, by the CTA: their largest magnitude, then the runs that change, put together in
@@ -475,7 +461,7 @@ __global__ void __launch_bounds__(32 * kKv8ThinWarps) kv8_write_thin_kernel(Kv8I
       for (int j = lane; j < P.sh.page; j += 32) s_row[warp][j] = kv8_row(P, (page << P.sh.shift) + j);
       __syncwarp();
     }
-    kv8_write_thin<T, kDim, kVec, false>(P, s_row[warp], nullptr, page, head);
+    kv8_write_thin<T, kDim, kVec>(P, s_row[warp], page, head);
   }
 }
 // and each CTA. 32768 tokens x 8 heads x 128 channels, bf16: 71 us from a page's first token, 73 from within one, 2.9 TB/s of
