@@ -270,8 +270,9 @@ __device__ __forceinline__ void kv8_write_thin(const Kv8IoParams& P, const int* 
 }
 
 // Up to kKv8Few rows, in one launch: a CTA to a row and some heads. The CTA of the lowest of a page's rows finds the others
-// among all. (8 heads x 128 channels: single tokens of 16 sequences 3.5 us, of 256 4.2; 64 tokens of one 29, 128 26; a CTA's
-// eight warps to a head, one head after another, 43 and 26. Through the lists below: 14 for 128 to 256 single tokens, 18 for 512, 23 for 1024; 12 and 18 for the chunks.)
+// among all. (8 heads x 128 channels: single tokens of 16 sequences 3.5 us, of 256 4.2; 64 tokens of one 29, 128 26; with a
+// CTA's eight warps to a head, one head after another, 43 and 26. Through the lists below: 14 for 128 to 256 single tokens, 12 for
+// 128 of one sequence, 18 for 500.)
 template <typename T, int kDim, bool kVec>
 __global__ void __launch_bounds__(256) kv8_write_few_kernel(Kv8IoParams P) {
   constexpr int kThreads = 256;
