@@ -142,7 +142,7 @@ int qrb200_kv8_write(void* codes, float* range, const qrb200_kv8_shape* shape, c
   if (need > 0 && (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 255u)))
     return QRB200_ERR_WORKSPACE;
   Kv8IoParams p{static_cast<unsigned char*>(codes), range, k, v, nullptr, nullptr, reinterpret_cast<const long long*>(slots),
-                nullptr, nullptr, nullptr, tokens, k_token_stride, k_head_stride, v_token_stride, v_head_stride, h, 0};
+                nullptr, nullptr, nullptr, tokens, k_token_stride, k_head_stride, v_token_stride, v_head_stride, h};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (need > 0) {
     p.pages = static_cast<int*>(workspace);
@@ -161,11 +161,7 @@ int qrb200_kv8_write(void* codes, float* range, const qrb200_kv8_shape* shape, c
   const cudaError_t e = with_shape(shape->dtype, h.dim, [&](auto type, auto dim) {
     using E = decltype(type);
     if (!p.rows) {
-      // The fewer CTAs, the better this kernel and the next overlap (64 single tokens x 8 heads, written and read back: with
-      // eight heads to a CTA 9.2 us, four 14.1, two 14.2; from 128 on all the same); the more, the sooner a chunk of one
-      // sequence is done (128 tokens 34, 26, 25).
-      p.span = tokens <= 16 ? 2 : tokens <= 32 ? 4 : tokens <= 64 ? 8 : 4;
-      LaunchShape l(dim3((unsigned)tokens, ceil_div(h.heads, p.span)), 256, 0, s);
+      LaunchShape l(dim3((unsigned)tokens, ceil_div(h.heads, 8)), 256, 0, s);
       return cudaLaunchKernelEx(&l.cfg, vec ? kv8_write_few_kernel<E, dim(), true> : kv8_write_few_kernel<E, dim(), false>, p);
     }
     // Eight CTAs to an SM: a page's rows are looked up once for several heads then, and the next head's loads are under
@@ -192,7 +188,7 @@ int qrb200_kv8_read(const void* codes, const float* range, const qrb200_kv8_shap
   const int st = quant_ready();
   if (st != QRB200_OK) return st;
   const Kv8IoParams p{static_cast<unsigned char*>(const_cast<void*>(codes)), const_cast<float*>(range), nullptr, nullptr, k, v,
-                      reinterpret_cast<const long long*>(slots), nullptr, nullptr, nullptr, tokens, 0, 0, 0, 0, h, 0};
+                      reinterpret_cast<const long long*>(slots), nullptr, nullptr, nullptr, tokens, 0, 0, 0, 0, h};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const cudaError_t e = with_shape(shape->dtype, h.dim, [&](auto type, auto dim) {
     LaunchShape l(dim3(ceil_div((tokens + 15) / 16 * h.heads, 8)), 256, 0, s);

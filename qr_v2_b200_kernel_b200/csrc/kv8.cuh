@@ -47,7 +47,6 @@ struct Kv8IoParams {
   int *pages, *list, *rows;
   long long tokens, k_ts, k_hs, v_ts, v_hs;  // strides in elements
   Kv8Shape sh;
-  int span;  // heads of a CTA, where rows are few
 };
 
 // Offsets of a token's code within its block: of channel c, as a key and as a value.
@@ -61,7 +60,7 @@ __device__ __forceinline__ int kv8_value_at(int dim, int token, int c) {
 }
 
 constexpr uint32_t kKv8Zeros = 0x80808080u;
-constexpr int kKv8Few = 256;  // rows up to which a page's are looked up among all of them
+constexpr int kKv8Few = 1024;  // rows up to which a page's are looked up among all of them
 constexpr int kKv8Thin = 8;    // rows of a page up to which a warp takes a head, else a CTA
 
 // Three significant bits, rounded up, of a magnitude's bits (the magnitude itself where that would pass the type's
@@ -176,12 +175,16 @@ __device__ __forceinline__ uint32_t kv8_moved(uint32_t word, float old, float no
   return next;
 }
 
-// A page's head whose new rows are few, by a warp: tokens one by one, four channels (64: two) to a lane, and bytes stored where they
-// belong, since a step of decoding brings a page one.
-template <typename T, int kDim, bool kVec>
-__device__ __forceinline__ void kv8_write_thin(const Kv8IoParams& P, const int* s_row, long long page, int head) {
+// A page's head whose new rows are few, by a warp or (kTeam) a CTA of eight, four rows at a time to each: tokens one by one, four
+// channels (64: two) to a lane, and bytes stored where they belong, since a step of decoding brings a page one.
+template <typename T, int kDim, bool kVec, bool kTeam>
+__device__ __forceinline__ void kv8_write_thin(const Kv8IoParams& P, const int* s_row, unsigned (*s_top)[2], long long page, int head) {
   constexpr int kPer = kDim / 32;  // channels of a lane
-  const int lane = threadIdx.x & 31;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const auto sync = [&]() {
+    if (kTeam) __syncthreads();
+    else __syncwarp();
+  };
   const int c0 = kPer * lane;
   const auto load = [&](T(&x)[2][kPer], int row) {
 #pragma unroll
@@ -201,7 +204,7 @@ __device__ __forceinline__ void kv8_write_thin(const Kv8IoParams& P, const int* 
   const auto each = [&](auto f) {
     for (int base = 0; base < P.sh.page; base += 32) {
       const int mine = base + lane < P.sh.page ? s_row[base + lane] : -1;
-      unsigned have = __ballot_sync(kFullMask, mine >= 0);
+      unsigned have = __ballot_sync(kFullMask, mine >= 0 && (!kTeam || ((base + lane) >> 2 & 7) == warp));
       while (have) {
         alignas(8) T x[4][2][kPer];
         int token[4];
@@ -225,6 +228,11 @@ __device__ __forceinline__ void kv8_write_thin(const Kv8IoParams& P, const int* 
       for (int e = 0; e < kPer; ++e) top[part] = max(top[part], __float_as_uint(to_f32(x[part][e])) & 0x7fffffffu);
   });
   for (int part = 0; part < 2; ++part) top[part] = __reduce_max_sync(kFullMask, top[part]);
+  if constexpr (kTeam) {
+    if (lane == 0) s_top[warp][0] = top[0], s_top[warp][1] = top[1];
+    __syncthreads();
+    for (int part = 0; part < 2; ++part) top[part] = __reduce_max_sync(kFullMask, s_top[lane & 7][part]);
+  }
   float* range = P.range + (page * P.sh.heads + head) * 2;
   unsigned char* block = P.codes + (page * P.sh.heads + head) * P.sh.block_bytes();
   const bool fresh = s_row[0] >= 0;
@@ -238,11 +246,11 @@ __device__ __forceinline__ void kv8_write_thin(const Kv8IoParams& P, const int* 
     inv[part] = now[part] > 0.f ? kv8_inverse(now[part]) : 0.f;
     move[part] = now[part] == now[part] && (fresh || now[part] != old[part]);
   }
-  __syncwarp();  // every lane has read the older range
-  if (lane < 2) range[lane] = now[lane];
+  sync();  // every lane has read the older range
+  if (lane < 2 && (!kTeam || warp == 0)) range[lane] = now[lane];
   if (move[0] || move[1]) {
 #pragma unroll 4
-    for (int at = lane; at < P.sh.block_bytes() / 16; at += 32) {
+    for (int at = kTeam ? threadIdx.x : lane; at < P.sh.block_bytes() / 16; at += kTeam ? 256 : 32) {
       const int part = at / kDim & 1;
       if (!move[part]) continue;
       uint4 w = make_uint4(kKv8Zeros, kKv8Zeros, kKv8Zeros, kKv8Zeros);
@@ -253,7 +261,7 @@ __device__ __forceinline__ void kv8_write_thin(const Kv8IoParams& P, const int* 
       }
       reinterpret_cast<uint4*>(block)[at] = w;
     }
-    __syncwarp();  // before the new codes go into the same words
+    sync();  // before the new codes go into the same words
   }
   each([&](int token, const T(&x)[2][kPer]) {
     uint32_t f[2][kPer];
@@ -269,40 +277,44 @@ __device__ __forceinline__ void kv8_write_thin(const Kv8IoParams& P, const int* 
   });
 }
 
-// Up to kKv8Few rows, in one launch: a CTA to a row and some heads. The CTA of the lowest of a page's rows finds the others
-// among all. (8 heads x 128 channels: single tokens of 16 sequences 3.5 us, of 256 4.2; 64 tokens of one 29, 128 26; with a
-// CTA's eight warps to a head, one head after another, 43 and 26. Through the lists below: 14 for 128 to 256 single tokens, 12 for
-// 128 of one sequence, 18 for 500.)
+// Up to kKv8Few rows, in one launch: a CTA to a row and eight heads. It finds the page's other rows among all, and the CTAs of a
+// page's rows share the heads, by their rows' order: a warp to a head where they are few, a CTA to a head where there are as many
+// CTAs. Few and light CTAs, so that this kernel and the next overlap. (8 heads x 128 channels: single tokens of 16 sequences 3.6 us,
+// of 256 5.1, of 1024 9.2; 12 tokens of one 3.8, 64 6.1, 500 10.9, 1000 14.9. Through the lists below: 14 for 256 single
+// tokens, 23 for 1024; 12 and 18 for 128 and 500 of one sequence.)
 template <typename T, int kDim, bool kVec>
 __global__ void __launch_bounds__(256) kv8_write_few_kernel(Kv8IoParams P) {
-  constexpr int kThreads = 256;
   __shared__ int s_row[1024];
-  __shared__ unsigned s_low[8];
+  __shared__ unsigned s_count[8], s_top[8][2];
   griddep_launch_wait();
-  const int tid = threadIdx.x, r = blockIdx.x;
+  const int tid = threadIdx.x, warp = tid >> 5, r = blockIdx.x;
   const long long page = kv8_page(P, P.slots[r]);
   if (page < 0) {
     if (P.slots[r] >= 0 && tid == 0) report_device_failure(kSiteIndex);
     return;
   }
-  for (int j = tid; j < P.sh.page; j += kThreads) s_row[j] = -1;
+  for (int j = tid; j < P.sh.page; j += 256) s_row[j] = -1;
   __syncthreads();
-  unsigned low = 0xffffffffu;
-  for (int at = tid; at < P.tokens; at += kThreads) {
+  unsigned count = 0;  // the page's rows, and above 2^16 those before this one
+  for (int at = tid; at < P.tokens; at += 256) {
     const long long slot = P.slots[at];
     if (kv8_page(P, slot) == page) {
       atomicMax(&s_row[(int)slot & (P.sh.page - 1)], at);
-      low = min(low, (unsigned)at);
+      count += at < r ? 0x10001u : 1u;
     }
   }
-  low = __reduce_min_sync(kFullMask, low);
-  if ((tid & 31) == 0) s_low[tid >> 5] = low;
+  count = __reduce_add_sync(kFullMask, count);
+  if ((tid & 31) == 0) s_count[warp] = count;
   __syncthreads();
-  low = __reduce_min_sync(kFullMask, s_low[tid & 7]);
-  if (low != (unsigned)r) return;
-  const int head0 = blockIdx.y * P.span;
-  const int heads = min(P.span, P.sh.heads - head0);
-  if (tid >> 5 < heads) kv8_write_thin<T, kDim, kVec>(P, s_row, page, head0 + (tid >> 5));
+  count = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) count += s_count[i];
+  const int rows = count & 0xffff, rank = count >> 16, head0 = 8 * blockIdx.y, heads = min(8, P.sh.heads - head0);
+  if (rows < 8) {
+    if (rank + rows * warp < heads) kv8_write_thin<T, kDim, kVec, false>(P, s_row, s_top, page, head0 + rank + rows * warp);
+  } else if (rank < heads) {
+    kv8_write_thin<T, kDim, kVec, true>(P, s_row, s_top, page, head0 + rank);
+  }
 }
 
 // Some heads of a page with more new rows, by the CTA: their largest magnitude, then the runs that change, put together in
@@ -444,15 +456,18 @@ __device__ __forceinline__ void kv8_write_thick(const Kv8IoParams& P, Kv8Thick<k
   }
 }
 
-// More: of the pages' heads, in order, each warp takes as many as any other, (2048 single tokens x 8 heads x 128 channels 33 us;
+// More: of the pages with few rows, unless they are so few themselves that the next kernel does them by the way (the ends of
+// sequences), each warp takes as many heads, in order, as any other, (2048 single tokens x 8 heads x 128 channels 33 us;
 // by CTAs, as below, 202)
 constexpr int kKv8ThinWarps = 4;
+// (Up to 256 of their heads: two sequences' 936 tokens x 4 heads 19.3 -> 12.1 us, sixteen's 512 x 8 37.6 -> 28.6.)
+__device__ __forceinline__ int kv8_thin_pages(const Kv8IoParams& P) { return (long long)P.pages[0] * P.sh.heads > 256 ? P.pages[0] : 0; }
 template <typename T, int kDim, bool kVec>
 __global__ void __launch_bounds__(32 * kKv8ThinWarps) kv8_write_thin_kernel(Kv8IoParams P) {
   __shared__ int s_row[kKv8ThinWarps][1024];
   griddep_launch_wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const long long units = (long long)P.pages[0] * P.sh.heads, warps = gridDim.x * (long long)kKv8ThinWarps, per = (units + warps - 1) / warps;
+  const long long units = (long long)kv8_thin_pages(P) * P.sh.heads, warps = gridDim.x * (long long)kKv8ThinWarps, per = (units + warps - 1) / warps;
   const long long first = (blockIdx.x * (long long)kKv8ThinWarps + warp) * per, end = min(units, first + per);
   for (long long unit = first; unit < end; ++unit) {
     const int head = (int)(unit % P.sh.heads);
@@ -462,21 +477,23 @@ __global__ void __launch_bounds__(32 * kKv8ThinWarps) kv8_write_thin_kernel(Kv8I
       for (int j = lane; j < P.sh.page; j += 32) s_row[warp][j] = kv8_row(P, (page << P.sh.shift) + j);
       __syncwarp();
     }
-    kv8_write_thin<T, kDim, kVec>(P, s_row[warp], page, head);
+    kv8_write_thin<T, kDim, kVec, false>(P, s_row[warp], nullptr, page, head);
   }
 }
 // and each CTA. 32768 tokens x 8 heads x 128 channels, bf16: 71 us from a page's first token, 73 from within one, 2.9 TB/s of
-// keys, values and codes; in instructions and their order, the two kernels before it 8 of them. (Both sorts of pages in one kernel:
+// keys, values and codes; in instructions and their order, the three kernels before it 8 of them. (Both sorts of pages in one kernel:
 // 75 and 80, the registers of the one hold up the other.)
 template <typename T, int kDim, bool kVec>
 __global__ void __launch_bounds__(2 * kDim) kv8_write_kernel(Kv8IoParams P) {
   __shared__ Kv8Thick<kDim> s_thick;
   __shared__ int s_row[1024];
   griddep_launch_wait();
-  const long long units = (long long)P.pages[1] * P.sh.heads, per = (units + gridDim.x - 1) / gridDim.x, end = min(units, (blockIdx.x + 1) * per);
+  const int thick = P.pages[1], pages = thick + P.pages[0] - kv8_thin_pages(P);
+  const long long units = (long long)pages * P.sh.heads, per = (units + gridDim.x - 1) / gridDim.x, end = min(units, (blockIdx.x + 1) * per);
   for (long long unit = blockIdx.x * per; unit < end;) {
     const int head0 = (int)(unit % P.sh.heads), heads = (int)min((long long)(P.sh.heads - head0), end - unit);
-    const long long page = kv8_page(P, P.slots[P.list[P.tokens - 1 - unit / P.sh.heads]]);
+    const int at = (int)(unit / P.sh.heads);
+    const long long page = kv8_page(P, P.slots[P.list[at < thick ? P.tokens - 1 - at : at - thick]]);
     unit += heads;
     __syncthreads();  // the page before is done
     for (int j = threadIdx.x; j < P.sh.page; j += 2 * kDim) s_row[j] = kv8_row(P, (page << P.sh.shift) + j);

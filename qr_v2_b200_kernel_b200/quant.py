@@ -284,7 +284,7 @@ def kv8_write(cache: KV8Cache, k: torch.Tensor, v: torch.Tensor, slots: torch.Te
     127 steps either way, and where the range grew the page's older codes are rounded to the new
     steps. A call that writes a page's first token begins the page anew: the rest of it reads as zeros. A
     NaN or an infinity makes what the page holds of its head NaN, until the page begins anew. Calls that
-    run at the same time may not write the same page. More than 256 tokens take a workspace of 4 bytes a slot of the cache. A slot past the cache is skipped and reported by the next call as
+    run at the same time may not write the same page. More than 1024 tokens take a workspace of 4 bytes a slot of the cache. A slot past the cache is skipped and reported by the next call as
     ``QRB200Error``.
     """
     (_module or _native()).kv8_write(_handle(cache, KV8Cache), k, v, slots)
