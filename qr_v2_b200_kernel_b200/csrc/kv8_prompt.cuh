@@ -17,8 +17,8 @@
 // for by the fence that the operands need.) Warps 12 and 13: a tile's MMAs each (their issue takes some 45
 // clocks, as long as the smallest of them run).
 //
-// P is one fp16 number for bf16 results (its error, 2^-12 of a weight, is a sixteenth of what the result's rounding
-// leaves) and two, high and low, for fp16 ones. It is scaled by a power of two that puts the largest step of the
+// P is two fp16 numbers, high and low, 22 bits. (One would do for bf16 results but for a tenth of them, which then are
+// not the nearest.) It is scaled by a power of two that puts the largest step of the
 // values at 2^11, so weights keep their leading bits down to 2^-25 of the largest.
 #pragma once
 
@@ -78,7 +78,6 @@ __device__ __forceinline__ uint32_t swizzled(int row, int piece) { return row * 
 template <typename T, int kDim>
 __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(Kv8AttnParams P) {
   constexpr int kTile = prompt_tile(kDim), kAtoms = kDim / 64;
-  constexpr bool kPrecise = std::is_same<T, __half>::value;  // weights in two halves
   constexpr float kNone = -INFINITY;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   __shared__ uint64_t raw_full[kPromptRaw], raw_empty[kPromptRaw], kv_full[kPromptStages], kv_empty[kPromptStages], s_full[2][2], p_full[2][2], o_full[2][2];  // [tile][odd steps]
@@ -329,14 +328,12 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(Kv8AttnPa
                     if (!two) p.y = 0.f;
                   }
                   high[8 * d + 2 * r + i / 2] = kv_pack(p);
-                  if constexpr (kPrecise) {
-                    const float2 back2 = __half22float2(__hneg2(reinterpret_cast<const __half2&>(high[8 * d + 2 * r + i / 2])));
-                    low[8 * d + 2 * r + i / 2] = kv_pack(__fadd2_rn(p, back2));
-                  }
+                  const float2 back2 = __half22float2(__hneg2(reinterpret_cast<const __half2&>(high[8 * d + 2 * r + i / 2])));
+                  low[8 * d + 2 * r + i / 2] = kv_pack(__fadd2_rn(p, back2));
                 }
               }
             tmem_put16(s_at + 16 * c, high);
-            if constexpr (kPrecise) tmem_put16(s_at + 16 * c + 16, low);
+            tmem_put16(s_at + 16 * c + 16, low);
           }
         };
         if (full) weights(std::true_type{});
@@ -481,7 +478,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(Kv8AttnPa
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
           f16_mma_tmem(d, p + 32 * (c >> 1) + 8 * (c & 1), v + 2 * c, upper, to_o, j + c > 0);
-          if constexpr (kPrecise) f16_mma_tmem(d, p + 32 * (c >> 1) + 8 * (c & 1) + 16, v + 2 * c, upper, to_o, true);
+          f16_mma_tmem(d, p + 32 * (c >> 1) + 8 * (c & 1) + 16, v + 2 * c, upper, to_o, true);
         }
         mma_commit(&kv_empty[st]);
         mma_commit(&o_full[x][j & 1]);  // the last word to arrive in this CTA is one that is waited for

@@ -302,6 +302,6 @@ def kv8_attention(q: torch.Tensor, cache: KV8Cache, block_table: torch.Tensor, l
     """Softmax attention of each sequence's newest tokens over its 8-bit cache.
 
     Operands, masks, limits and failures as in :func:`kv4_attention`; single tokens, drafts and long prompts alike. Weights
-    are held in 22 bits, in prompts with bfloat16 results in 11 (a sixteenth of the results' own rounding).
+    are held in 22 bits.
     """
     return (_module or _native()).kv8_attention(q, _handle(cache, KV8Cache), block_table, lengths, scale, causal, window)

@@ -1,0 +1,112 @@
+"""How exact attention over the 8-bit cache is, against 64 bits: the weights' bits, long sums, and that a row depends on what it sees only (GPU).
+
+Each bound is relative to `size`, the sum of |weight x value| of a row and channel: by that much may 32-bit arithmetic be off, and
+no more. It holds for prompts and single tokens, and for both types, alike.
+"""
+
+import math
+
+import pytest
+import torch
+
+import qr_v2_b200_kernel_b200 as qr
+
+pytestmark = pytest.mark.gpu
+
+BF, HF = torch.bfloat16, torch.float16
+
+
+def _gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def _randn(*shape, seed=0, dtype=BF, size=1.0):
+    return (torch.randn(*shape, generator=_gen(seed), device="cuda") * size).to(dtype)
+
+
+def _pages(batch, tokens, heads, dim, page, dtype, seed=0):
+    """An empty cache, the table of its sequences and their slots (batch, tokens)."""
+    per = -(-tokens // page)
+    table = torch.randperm(batch * per + 1, generator=_gen(seed), device="cuda")[: batch * per].reshape(batch, per).int()
+    cache = qr.kv8_cache(batch * per + 1, page, heads, dim, dtype=dtype)
+    at = torch.arange(tokens, device="cuda")
+    return cache, table, table.long()[:, at // page] * page + at % page
+
+
+def _write(cache, slots, k, v):
+    qr.kv8_write(cache, k.flatten(0, 1).to(cache.dtype), v.flatten(0, 1).to(cache.dtype), slots.reshape(-1))
+
+
+def _values(cache, slots):
+    """What the cache stands for at slots (tokens,), in 64 bits, and the steps of its values (tokens, heads)."""
+    plain = qr.KV8Cache(cache.data, torch.full_like(cache.range, 127.0), cache.page_size, cache.head_dim, cache.dtype)
+    step = cache.range.double()[slots // cache.page_size] / 127
+    k, v = (x.double() * step[:, :, i, None] for i, x in enumerate(qr.kv8_read(plain, slots)))
+    return k, v, step[..., 1]
+
+
+def _check(out, q, cache, slots, lengths, terms, window=None, rows=None, scale=None, causal=True):
+    """Of `terms` products of a score that are not zero, each is exact; their sum, and what scales it, is off by terms + 4 units of
+    2^-23 of their magnitudes, and a weight by twice that (its own score's and the largest one's). A weight is held in 22 bits (half a
+    unit: 2^-23) with an exponential of two units of 2^-23 and a scaling: 2^-20. Sums: 64 products join a sum of the matrix instruction's before
+    it is added to others in 32 bits, each cut off by up to a unit, 2^-23, of the sum so far: 2^-17, and 2^-20 for the rest.
+
+    And weights times their steps are put, in fp16 pairs, within 2^24 / 2^10 of fp16's smallest by the largest of the row: 2^-25 2^-10 each of the
+    largest weight times range; n of them, and a factor of two for the power of two above: n 2^-34 (127 w <= R).
+    """
+    batch, queries, heads, dim = q.shape
+    share = heads // cache.kv_heads
+    factor = dim**-0.5 if scale is None else scale
+    worst = 0.0
+    for b in range(batch):
+        n = int(lengths[b])
+        if n == 0:
+            continue
+        k, v, step = _values(cache, slots[b, :n])
+        k, v = (x.repeat_interleave(share, 1) for x in (k, v))
+        reach = 127 * step.repeat_interleave(share, 1)  # tokens, heads
+        at = torch.arange(n, device="cuda")
+        for i in range(queries) if rows is None else rows:
+            i = i % queries
+            pos = n - queries + i
+            seen = (at <= pos) if causal else torch.ones(n, dtype=torch.bool, device="cuda")
+            if window:
+                seen = seen & (at > pos - window)
+            if not seen.any():
+                assert torch.all(out[b, i] == 0)
+                continue
+            k_, v_, r_, qi = k[seen], v[seen], reach[seen], q[b, i].double()
+            p = torch.softmax(torch.einsum("hd,thd->ht", qi, k_) * factor, -1)
+            d = (torch.einsum("hd,thd->ht", qi.abs(), k_.abs()) * factor).amax(-1) * (terms + 4) * 2.0**-23
+            want = torch.einsum("ht,thd->hd", p, v_)
+            size = torch.einsum("ht,thd->hd", p, v_.abs())
+            bound = torch.finfo(q.dtype).eps / 2 * want.abs() + ((2 * d).expm1()[:, None] + 2.0**-20 + 2.0**-17 + 2.0**-20) * size
+            bound += len(p[0]) * 2.0**-34 * (p.T * r_).amax(0)[:, None] + (2.0**-24 if q.dtype == HF else 0.0)
+            worst = max(worst, ((out[b, i].double() - want).abs() / bound).max().item())
+    assert worst <= 1.0, worst
+
+
+def _few_channels(batch, queries, heads, dim, dtype, size, channels=4, seed=9):
+    """Queries of few channels that are not zero: their scores are sums of as many products."""
+    q = _randn(batch, queries, heads, dim, seed=seed, dtype=dtype, size=size)
+    q[..., channels:] = 0
+    return q
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("batch, heads, share, queries", [(40, 8, 4, 40), (2, 2, 8, 5), (2, 2, 8, 1), (1, 1, 1, 1)])
+def test_weights_are_held_in_22_bits(batch, heads, share, queries, dim, dtype):
+    # Values come in pairs of opposite ones under nearly the same weights: what is left of a pair is the weights' error, and no
+    # rounding of the result hides it. (Held in 11 bits the larger of two weights is off by up to 2^-12.)
+    n = 200
+    cache, table, slots = _pages(batch, n, heads, dim, 16, dtype)
+    k = torch.randn(batch, n // 2, heads, dim, generator=_gen(1), device="cuda").repeat_interleave(2, 1)
+    v = torch.randn(batch, n // 2, heads, dim, generator=_gen(2), device="cuda").repeat_interleave(2, 1)
+    k[:, 1::2, :, 1] += 0.02
+    v[:, 1::2] *= -1
+    _write(cache, slots, k, v)
+    q = _few_channels(batch, queries, heads * share, dim, dtype, 1.5 * dim**0.5)
+    lengths = torch.full((batch,), n, dtype=torch.int32, device="cuda")
+    out = qr.kv8_attention(q, cache, table, lengths)
+    _check(out[:2], q[:2], cache, slots, lengths, 4)
