@@ -36,7 +36,7 @@ struct Kv8Plan {
   bool prompt;  // tiles of 256 rows on the tensor cores, not split; else
   bool brief;   // short steps
   bool memory;  // parts go through memory
-  size_t bytes;  // workspace: the parts and their (maximum, sum) pairs
+  size_t bytes;  // workspace: the parts and their (maximum, sum) pairs, or a prompt's sums set aside
 };
 
 // Eight rows a tile where a key head has no more than eight query rows, else sixteen. Of both kinds of step and every number of
@@ -44,7 +44,7 @@ struct Kv8Plan {
 // (measured with 128 channels), three steps for a CTA's set-up, 2 us for a join in a cluster and 4 through memory. Clusters of
 // other than two or four CTAs place badly where they fill the GPU (24 x 8192 tokens, 8 heads in threes: 99 us, through memory 70; in
 // pairs 64 x 8192 172, through memory 180), so those are left to thin waves. The length is the table's capacity or what a window leaves of it, all that the host knows.
-static Kv8Plan attn_plan(const Kv8Shape& h, int64_t batch, int64_t queries, int64_t q_heads, int64_t max_pages, int64_t span) {
+static Kv8Plan attn_plan(const Kv8Shape& h, bool half, int64_t batch, int64_t queries, int64_t q_heads, int64_t max_pages, int64_t span) {
   static const int kShort[5] = {0, 750, 1000, 1300, 1400}, kLong[3] = {0, 1000, 1400}, kLong16[3] = {0, 1500, 2300};
   Kv8Plan p{};
   const int64_t rows = queries * (q_heads / h.heads);
@@ -73,6 +73,8 @@ static Kv8Plan attn_plan(const Kv8Shape& h, int64_t batch, int64_t queries, int6
   if (p.tile_rows == 16 && wide < best) {
     p.prompt = true;
     p.tile_rows = kPromptRows, p.tiles = (int)tiles, p.splits = 1, p.memory = false;
+    if (tokens / kPromptTokens + 2 > prompt_aside(half))  // (the most steps, begun anywhere)
+      p.bytes = (size_t)(tiles * batch * h.heads * kPromptRows) * (h.dim * sizeof(float));
     return p;
   }
   if (p.memory) p.bytes = (size_t)(ctas * p.splits * p.tile_rows) * (h.dim * sizeof(float) + sizeof(float2));
@@ -215,7 +217,7 @@ size_t qrb200_kv8_attention_workspace_bytes(const qrb200_kv8_shape* shape, int64
                                             int64_t max_pages, int64_t window) {
   Kv8Shape h;
   if (window < 0 || !attention_args(shape, batch, queries, q_heads, max_pages, &h)) return 0;
-  return batch * queries * q_heads == 0 ? 0 : attn_plan(h, batch, queries, q_heads, max_pages, token_span(queries, window)).bytes;
+  return batch * queries * q_heads == 0 ? 0 : attn_plan(h, shape->dtype == QRB200_F16, batch, queries, q_heads, max_pages, token_span(queries, window)).bytes;
 }
 
 int qrb200_kv8_attention(const void* q, const int64_t* q_strides, const void* codes, const float* range,
@@ -230,7 +232,7 @@ int qrb200_kv8_attention(const void* q, const int64_t* q_strides, const void* co
     return QRB200_ERR_ARG;
   const int st = quant_ready();
   if (st != QRB200_OK) return st;
-  const Kv8Plan plan = attn_plan(h, batch, queries, q_heads, max_pages, token_span(queries, window));
+  const Kv8Plan plan = attn_plan(h, shape->dtype == QRB200_F16, batch, queries, q_heads, max_pages, token_span(queries, window));
   if (plan.bytes > 0 && (!workspace || workspace_bytes < plan.bytes || (reinterpret_cast<uintptr_t>(workspace) & 255u)))
     return QRB200_ERR_WORKSPACE;
   Kv8AttnParams p{};
@@ -248,7 +250,7 @@ int qrb200_kv8_attention(const void* q, const int64_t* q_strides, const void* co
   p.scale_power -= 1;
   p.sh = h;
   p.q_wide = (reinterpret_cast<uintptr_t>(q) & 7u) == 0 && ((q_strides[0] | q_strides[1] | q_strides[2]) & 3) == 0;
-  p.part_o = static_cast<float*>(workspace);
+  p.part_o = plan.bytes > 0 ? static_cast<float*>(workspace) : nullptr;
   if (plan.memory)
     p.part_ml = reinterpret_cast<float2*>(p.part_o + batch * h.heads * plan.tiles * plan.splits * plan.tile_rows * h.dim);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
@@ -260,7 +262,8 @@ int qrb200_kv8_attention(const void* q, const int64_t* q_strides, const void* co
     part.out = static_cast<char*>(out) + 2 * rows * h.dim;
     part.table += b * table_stride;
     part.lengths += b;
-    if (p.part_ml) part.part_o += parts * h.dim, part.part_ml += parts;
+    if (p.part_o) part.part_o += parts * h.dim;
+    if (p.part_ml) part.part_ml += parts;
     const cudaError_t e = with_shape(shape->dtype, h.dim, [&](auto type, auto dim) {
       using E = decltype(type);
       if (plan.prompt) return launch_prompt<E, dim()>(part, s);

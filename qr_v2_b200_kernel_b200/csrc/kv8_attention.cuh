@@ -22,7 +22,8 @@ struct Kv8AttnParams {
   const float* range;
   const void* q;
   void* out;
-  float* part_o;   // [batch][head][tile][split][rows of a tile][dim], unnormalised, where parts go through memory
+  float* part_o;   // [batch][head][tile][split][rows of a tile][dim], unnormalised, where parts go through memory;
+                   // of prompts, a CTA's sums set aside; else null
   float2* part_ml;  // [...][rows of a tile]: maximum (base 2) and sum; null where a cluster joins them
   const int* table;
   const int* lengths;

@@ -17,6 +17,10 @@
 // for by the fence that the operands need.) Warps 12 and 13: a tile's MMAs each (their issue takes some 45
 // clocks, as long as the smallest of them run).
 //
+// A matrix instruction cuts off what it adds, so a sum over many tokens comes out small (over 131072 by 2^-10). So O is added in 32 bits
+// to sums in global memory every 32 steps, every 16 for fp16 results: of 2 x 2048 queries over 4096 tokens 0.2 % of the bf16
+// and 0.7 % of the fp16 results are then not the nearest (of elementary 32-bit operations 0.1 % of the bf16 ones).
+//
 // P is two fp16 numbers, high and low, 22 bits. (One would do for bf16 results but for a tenth of them, which then are
 // not the nearest.) It is scaled by a power of two that puts the largest step of the
 // values at 2^11, so weights keep their leading bits down to 2^-25 of the largest.
@@ -31,6 +35,8 @@ constexpr int kPromptRows = 256, kPromptTokens = 64;
 constexpr int kPromptStages = 3, kPromptRaw = 2;  // steps of operands, and of bytes, in shared memory (four and two 151 us)
 constexpr int kPromptThreads = 32 * 15;
 constexpr int kPromptStepExp = 11;
+// Steps between settings-aside, a power of two. (Both types, 2 x 2048 queries over 4096 tokens: never 158 us, 32 166, 16 183, 8 209.)
+__host__ __device__ constexpr int prompt_aside(bool half) { return half ? 16 : 32; }
 __host__ __device__ constexpr int prompt_tile(int dim) { return 128 * dim * 2; }  // bytes of 128 rows of fp16
 __host__ __device__ constexpr int prompt_smem_bytes(int dim) { return 1024 + (2 + kPromptStages) * prompt_tile(dim) + kPromptRaw * prompt_tile(dim) / 2; }
 
@@ -68,12 +74,53 @@ __device__ __forceinline__ void tmem_put16(uint32_t taddr, const uint32_t (&v)[1
 }
 __device__ __forceinline__ void tmem_put_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+// Sums set aside in global memory, by one thread each: added to where they lie, so that nothing waits for them.
+__device__ __forceinline__ void aside_store(float4* to, const float4& x) {
+  asm volatile("st.relaxed.gpu.global.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(to), "f"(x.x), "f"(x.y), "f"(x.z), "f"(x.w) : "memory");
+}
+__device__ __forceinline__ void aside_add(float4* to, const float4& x) {
+  asm volatile("red.relaxed.gpu.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(to), "f"(x.x), "f"(x.y), "f"(x.z), "f"(x.w) : "memory");
+}
+__device__ __forceinline__ float4 aside_load(const float4* from) {
+  float4 x;
+  asm volatile("ld.relaxed.gpu.global.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(x.x), "=f"(x.y), "=f"(x.z), "=f"(x.w) : "l"(from) : "memory");
+  return x;
+}
+
 // Columns of S (rows of K in shared memory) in their order. Of a step's 64 tokens, four runs of 16, column c holds token
 // prompt_token(c): the order that the values' bytes give a lane sixteen neighbours in.
 __host__ __device__ constexpr int prompt_run(int c) { return c >> 2 & 3; }
 __host__ __device__ constexpr int prompt_token(int c) { return 16 * prompt_run(c) + 2 * (c >> 4) + (c & 1) + 8 * (c >> 1 & 1); }
 // A row's 16-byte piece in the 128-byte swizzle.
 __device__ __forceinline__ uint32_t swizzled(int row, int piece) { return row * 128 + ((piece ^ (row & 7)) << 4); }
+
+// A row's sums join those set aside. Out of line: the loop around it has no registers to spare.
+template <int kDim>
+static __device__ __noinline__ void prompt_set_aside(uint32_t o_at, float4* to, float lag, bool first) {
+  const bool moved = __any_sync(kFullMask, lag != 1.f);
+#pragma unroll 1
+  for (int c = 0; c < kDim; c += 32) {
+    float o[2][16];
+    tmem_ask16(o_at + c, o[0]);
+    tmem_ask16(o_at + c + 16, o[1]);
+    tmem_arrived(o[0]);
+    tmem_arrived(o[1]);
+#pragma unroll
+    for (int i = 0; i < 8; ++i, to += kPromptRows) {
+      const float* x = &o[i >> 2][4 * (i & 3)];
+      float4 y = make_float4(x[0], x[1], x[2], x[3]);
+      if (first || moved) {
+        if (!first) {
+          const float4 a = aside_load(to);
+          y = make_float4(fmaf(a.x, lag, y.x), fmaf(a.y, lag, y.y), fmaf(a.z, lag, y.z), fmaf(a.w, lag, y.w));
+        }
+        aside_store(to, y);
+      } else {
+        aside_add(to, y);
+      }
+    }
+  }
+}
 
 template <typename T, int kDim>
 __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(Kv8AttnParams P) {
@@ -188,6 +235,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(Kv8AttnPa
   const int cap = max(-100, min(126, (int)(__reduce_max_sync(kFullMask, lane < 15 ? s_most[1][lane] : 0u) >> 23) - 126));
   const float scaled = __int_as_float((kPromptStepExp - cap + 127) << 23), lower = __int_as_float((cap - kPromptStepExp + 127) << 23);
   const uint32_t tmem = s_tmem;
+  const int aside_every = P.part_o ? prompt_aside(std::is_same<T, __half>::value) : 1 << 30;
 
   if (warp < 8) {
     // ---- the softmax of a tile, a row to a thread ----
@@ -244,105 +292,122 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(Kv8AttnPa
       // What every row of the warp sees.
       const int in_lo = __reduce_max_sync(kFullMask, lo), in_hi = __reduce_min_sync(kFullMask, real ? hi : 0x7fffffff);
       float ref = kNone, sum = 0.f;  // weights are 2^(score - ref)
+      // Set aside, four channels of a row beside the next row's: the sums of earlier steps, against the reference of then, which `lag`
+      // brings to the present one.
+      const auto set_aside = [&]() {
+        return reinterpret_cast<float4*>(P.part_o) + (long long)blockIdx.x * (kDim / 4 * kPromptRows) + 128 * (threadIdx.x >> 7) + (threadIdx.x & 127);
+      };
+      float lag = 1.f;
       bool ok = true;
-      for (int j = 0; j < count; ++j) {
-        const int st = j % kPromptStages, tok0 = (block0 + j) * kPromptTokens;
-        const uint32_t s_at = lanes + 128 * mine + 64 * (j & 1);
-        ok = ok && mbar_wait_quick(&s_full[mine][j & 1], (j >> 1) & 1);
-        __syncwarp();
-        tc_fence_after();
-        float v[4][16];
+      for (int j = 0; j < count;) {
+        const int pause = min(count, j + aside_every);
+        for (; j < pause; ++j) {
+          const int st = j % kPromptStages, tok0 = (block0 + j) * kPromptTokens;
+          const uint32_t s_at = lanes + 128 * mine + 64 * (j & 1);
+          ok = ok && mbar_wait_quick(&s_full[mine][j & 1], (j >> 1) & 1);
+          __syncwarp();
+          tc_fence_after();
+          float v[4][16];
 #pragma unroll
-        for (int c = 0; c < 4; ++c) tmem_ask16(s_at + 16 * c, v[c]);
-        const float4 k4 = s_key[st], w4 = s_value[st];
-        const float f[4] = {k4.x * back, k4.y * back, k4.z * back, k4.w * back}, w[4] = {w4.x, w4.y, w4.z, w4.w};
+          for (int c = 0; c < 4; ++c) tmem_ask16(s_at + 16 * c, v[c]);
+          const float4 k4 = s_key[st], w4 = s_value[st];
+          const float f[4] = {k4.x * back, k4.y * back, k4.z * back, k4.w * back}, w[4] = {w4.x, w4.y, w4.z, w4.w};
 #pragma unroll
-        for (int c = 0; c < 4; ++c) tmem_arrived(v[c]);
-        const int gone = s_gone[st];
-        const bool full = tok0 >= in_lo && tok0 + kPromptTokens <= in_hi && gone == 0;
-        // The largest score. (Factors are not negative, so a run's largest product gives its largest score.)
-        const auto largest = [&](auto all) {
-          constexpr bool kAll = decltype(all)::value;
-          float top = kNone;
+          for (int c = 0; c < 4; ++c) tmem_arrived(v[c]);
+          const int gone = s_gone[st];
+          const bool full = tok0 >= in_lo && tok0 + kPromptTokens <= in_hi && gone == 0;
+          // The largest score. (Factors are not negative, so a run's largest product gives its largest score.)
+          const auto largest = [&](auto all) {
+            constexpr bool kAll = decltype(all)::value;
+            float top = kNone;
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            float m = kNone;
+            for (int r = 0; r < 4; ++r) {
+              float m = kNone;
 #pragma unroll
-            for (int c = 0; c < 4; ++c)
+              for (int c = 0; c < 4; ++c)
 #pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const int at = tok0 + prompt_token(16 * c + 4 * r + i);
-                const float x = v[c][4 * r + i];
-                m = kAll || (at >= lo && at < hi && !(gone >> r & 1)) ? fmaxf(m, x) : m;
-              }
-            top = kAll || m > kNone ? fmaxf(top, m * f[r]) : top;
-          }
-          return top;
-        };
-        const float top = full ? largest(std::true_type{}) : largest(std::false_type{});
-        const bool move = top > __fadd_rd(ref, kKvLazy) || (ref == kNone && top > kNone);
-        if (__any_sync(kFullMask, move)) {
-          const float next = fmaxf(ref, top), keep = ref == kNone ? 0.f : kv_exp2(ref - next);
-          if (j > 0) {  // once the products before are over
-            ok = ok && mbar_wait_quick(&o_full[mine][(j - 1) & 1], ((j - 1) >> 1) & 1);
-            __syncwarp();
-            tc_fence_after();
-#pragma unroll 1
-            for (int c = 0; c < kDim; c += 16) {
-              float o[16];
-              tmem_ask16(o_at + c, o);
-              tmem_arrived(o);
-              uint32_t kept[16];
-#pragma unroll
-              for (int i = 0; i < 16; ++i) kept[i] = __float_as_uint(ref == kNone ? 0.f : o[i] * keep);
-              tmem_put16(o_at + c, kept);
-            }
-            tmem_put_wait();
-          }
-          sum *= keep;
-          ref = next;
-        }
-        const float less = ref == kNone ? 0.f : -ref;
-        const float2 less2 = make_float2(less, less);
-        float2 sums = make_float2(0.f, 0.f);
-        const auto weights = [&](auto all) {
-          constexpr bool kAll = decltype(all)::value;
-#pragma unroll
-          for (int c = 0; c < 4; c += 2) {
-            uint32_t high[16], low[16];
-#pragma unroll
-            for (int d = 0; d < 2; ++d)
-#pragma unroll
-              for (int r = 0; r < 4; ++r) {
-                const float2 f2 = make_float2(f[r], f[r]), w2 = make_float2(w[r], w[r]);
-#pragma unroll
-                for (int i = 0; i < 4; i += 2) {
-                  const float2 x = __ffma2_rn(make_float2(v[c + d][4 * r + i], v[c + d][4 * r + i + 1]), f2, less2);
-                  const int at = tok0 + prompt_token(16 * (c + d) + 4 * r + i);  // and the next
-                  const bool one = kAll || (at >= lo && at < hi && !(gone >> r & 1)), two = kAll || (at + 1 >= lo && at + 1 < hi && !(gone >> r & 1));
-                  float2 p = make_float2(one ? kv_exp2(x.x) : 0.f, two ? kv_exp2(x.y) : 0.f);
-                  sums = __fadd2_rn(sums, p);
-                  p = __fmul2_rn(p, w2);
-                  if constexpr (!kAll) {  // what a row does not see may be NaN
-                    if (!one) p.x = 0.f;
-                    if (!two) p.y = 0.f;
-                  }
-                  high[8 * d + 2 * r + i / 2] = kv_pack(p);
-                  const float2 back2 = __half22float2(__hneg2(reinterpret_cast<const __half2&>(high[8 * d + 2 * r + i / 2])));
-                  low[8 * d + 2 * r + i / 2] = kv_pack(__fadd2_rn(p, back2));
+                for (int i = 0; i < 4; ++i) {
+                  const int at = tok0 + prompt_token(16 * c + 4 * r + i);
+                  const float x = v[c][4 * r + i];
+                  m = kAll || (at >= lo && at < hi && !(gone >> r & 1)) ? fmaxf(m, x) : m;
                 }
+              top = kAll || m > kNone ? fmaxf(top, m * f[r]) : top;
+            }
+            return top;
+          };
+          const float top = full ? largest(std::true_type{}) : largest(std::false_type{});
+          const bool move = top > __fadd_rd(ref, kKvLazy) || (ref == kNone && top > kNone);
+          if (__any_sync(kFullMask, move)) {
+            const float next = fmaxf(ref, top), keep = ref == kNone ? 0.f : kv_exp2(ref - next);
+            if ((j & (aside_every - 1)) != 0) {  // once the products before are over
+              ok = ok && mbar_wait_quick(&o_full[mine][(j - 1) & 1], ((j - 1) >> 1) & 1);
+              __syncwarp();
+              tc_fence_after();
+#pragma unroll 1
+              for (int c = 0; c < kDim; c += 16) {
+                float o[16];
+                tmem_ask16(o_at + c, o);
+                tmem_arrived(o);
+                uint32_t kept[16];
+#pragma unroll
+                for (int i = 0; i < 16; ++i) kept[i] = __float_as_uint(ref == kNone ? 0.f : o[i] * keep);
+                tmem_put16(o_at + c, kept);
               }
-            tmem_put16(s_at + 16 * c, high);
-            tmem_put16(s_at + 16 * c + 16, low);
+              tmem_put_wait();
+            }
+            sum *= keep;
+            lag *= keep;
+            ref = next;
           }
-        };
-        if (full) weights(std::true_type{});
-        else weights(std::false_type{});
-        sum += sums.x + sums.y;
-        tmem_put_wait();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[mine][j & 1]);
+          const float less = ref == kNone ? 0.f : -ref;
+          const float2 less2 = make_float2(less, less);
+          float2 sums = make_float2(0.f, 0.f);
+          const auto weights = [&](auto all) {
+            constexpr bool kAll = decltype(all)::value;
+#pragma unroll
+            for (int c = 0; c < 4; c += 2) {
+              uint32_t high[16], low[16];
+#pragma unroll
+              for (int d = 0; d < 2; ++d)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                  const float2 f2 = make_float2(f[r], f[r]), w2 = make_float2(w[r], w[r]);
+#pragma unroll
+                  for (int i = 0; i < 4; i += 2) {
+                    const float2 x = __ffma2_rn(make_float2(v[c + d][4 * r + i], v[c + d][4 * r + i + 1]), f2, less2);
+                    const int at = tok0 + prompt_token(16 * (c + d) + 4 * r + i);  // and the next
+                    const bool one = kAll || (at >= lo && at < hi && !(gone >> r & 1)), two = kAll || (at + 1 >= lo && at + 1 < hi && !(gone >> r & 1));
+                    float2 p = make_float2(one ? kv_exp2(x.x) : 0.f, two ? kv_exp2(x.y) : 0.f);
+                    sums = __fadd2_rn(sums, p);
+                    p = __fmul2_rn(p, w2);
+                    if constexpr (!kAll) {  // what a row does not see may be NaN
+                      if (!one) p.x = 0.f;
+                      if (!two) p.y = 0.f;
+                    }
+                    high[8 * d + 2 * r + i / 2] = kv_pack(p);
+                    const float2 back2 = __half22float2(__hneg2(reinterpret_cast<const __half2&>(high[8 * d + 2 * r + i / 2])));
+                    low[8 * d + 2 * r + i / 2] = kv_pack(__fadd2_rn(p, back2));
+                  }
+                }
+              tmem_put16(s_at + 16 * c, high);
+              tmem_put16(s_at + 16 * c + 16, low);
+            }
+          };
+          if (full) weights(std::true_type{});
+          else weights(std::false_type{});
+          sum += sums.x + sums.y;
+          tmem_put_wait();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&p_full[mine][j & 1]);
+        }
+        if (j < count) {  // the next product with the values begins new sums
+          ok = ok && mbar_wait_quick(&o_full[mine][(j - 1) & 1], ((j - 1) >> 1) & 1);
+          __syncwarp();
+          tc_fence_after();
+          prompt_set_aside<kDim>(o_at, set_aside(), lag, j == aside_every);
+          lag = 1.f;
+        }
       }
       if (count > 0) ok = ok && mbar_wait_quick(&o_full[mine][(count - 1) & 1], ((count - 1) >> 1) & 1);
       if (!ok) s_bad = 1;
@@ -350,12 +415,29 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(Kv8AttnPa
       tc_fence_after();
       const float inv = sum == 0.f ? 0.f : lower / sum;  // nothing seen: zeros
       T* out = static_cast<T*>(P.out) + (((long long)b * P.queries + row / P.share) * P.q_heads + head * P.share + row % P.share) * kDim;
-#pragma unroll 1
+      const bool apart = count > aside_every;
+      float4 a[2][8];
+      const auto ask = [&](int c) {
+        if (apart && c < kDim)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) a[c >> 5 & 1][i] = aside_load(set_aside() + (c / 4 + i) * kPromptRows);
+      };
+      ask(0);
+#pragma unroll
       for (int c = 0; c < kDim; c += 16) {
+        if ((c & 31) == 0) ask(c + 32);
         float o[16] = {};
         if (count > 0) {
           tmem_ask16(o_at + c, o);
           tmem_arrived(o);
+        }
+        if (apart) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float4 x = a[c >> 5 & 1][(c >> 2 & 4) + i];
+            o[4 * i] = fmaf(x.x, lag, o[4 * i]), o[4 * i + 1] = fmaf(x.y, lag, o[4 * i + 1]);
+            o[4 * i + 2] = fmaf(x.z, lag, o[4 * i + 2]), o[4 * i + 3] = fmaf(x.w, lag, o[4 * i + 3]);
+          }
         }
         alignas(16) T y[16];
 #pragma unroll
@@ -477,7 +559,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(Kv8AttnPa
         const uint32_t v = k0 + st * (kTile >> 4) + (kTile / 2 >> 4), p = tmem + 128 * x + 64 * (j & 1), d = tmem + 256 + 128 * x;
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          f16_mma_tmem(d, p + 32 * (c >> 1) + 8 * (c & 1), v + 2 * c, upper, to_o, j + c > 0);
+          f16_mma_tmem(d, p + 32 * (c >> 1) + 8 * (c & 1), v + 2 * c, upper, to_o, (j & (aside_every - 1)) + c > 0);
           f16_mma_tmem(d, p + 32 * (c >> 1) + 8 * (c & 1) + 16, v + 2 * c, upper, to_o, true);
         }
         mma_commit(&kv_empty[st]);

@@ -48,8 +48,9 @@ def _values(cache, slots):
 def _check(out, q, cache, slots, lengths, terms, window=None, rows=None, scale=None, causal=True):
     """Of `terms` products of a score that are not zero, each is exact; their sum, and what scales it, is off by terms + 4 units of
     2^-23 of their magnitudes, and a weight by twice that (its own score's and the largest one's). A weight is held in 22 bits (half a
-    unit: 2^-23) with an exponential of two units of 2^-23 and a scaling: 2^-20. Sums: 64 products join a sum of the matrix instruction's before
-    it is added to others in 32 bits, each cut off by up to a unit, 2^-23, of the sum so far: 2^-17, and 2^-20 for the rest.
+    unit: 2^-23) with an exponential of two units of 2^-23 and a scaling: 2^-20. Sums: up to 256 products, 128 for
+    fp16, join a sum of the matrix instruction's before it is added to others in 32 bits, each cut off by up to a unit, 2^-23, of the sum so far: 2^-15 or
+    2^-16, and 2^-20 for the rest.
 
     And weights times their steps are put, in fp16 pairs, within 2^24 / 2^10 of fp16's smallest by the largest of the row: 2^-25 2^-10 each of the
     largest weight times range; n of them, and a factor of two for the power of two above: n 2^-34 (127 w <= R).
@@ -80,7 +81,7 @@ def _check(out, q, cache, slots, lengths, terms, window=None, rows=None, scale=N
             d = (torch.einsum("hd,thd->ht", qi.abs(), k_.abs()) * factor).amax(-1) * (terms + 4) * 2.0**-23
             want = torch.einsum("ht,thd->hd", p, v_)
             size = torch.einsum("ht,thd->hd", p, v_.abs())
-            bound = torch.finfo(q.dtype).eps / 2 * want.abs() + ((2 * d).expm1()[:, None] + 2.0**-20 + 2.0**-17 + 2.0**-20) * size
+            bound = torch.finfo(q.dtype).eps / 2 * want.abs() + ((2 * d).expm1()[:, None] + 2.0**-20 + (2.0**-16 if q.dtype == HF else 2.0**-15) + 2.0**-20) * size
             bound += len(p[0]) * 2.0**-34 * (p.T * r_).amax(0)[:, None] + (2.0**-24 if q.dtype == HF else 0.0)
             worst = max(worst, ((out[b, i].double() - want).abs() / bound).max().item())
     assert worst <= 1.0, worst
@@ -110,3 +111,35 @@ def test_weights_are_held_in_22_bits(batch, heads, share, queries, dim, dtype):
     lengths = torch.full((batch,), n, dtype=torch.int32, device="cuda")
     out = qr.kv8_attention(q, cache, table, lengths)
     _check(out[:2], q[:2], cache, slots, lengths, 4)
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("dim, queries, share, n, window", [(128, 2048, 8, 32768, None), (64, 1024, 8, 40000, None), (128, 1024, 8, 20000, 16000), (128, 1, 8, 32768, None),
+                                                            (64, 5, 4, 40000, None)])
+def test_long_sums_keep_32_bits(dim, queries, share, n, window, dtype):
+    # Positive values under nearly even weights: whatever a sum cuts off, it cuts off in one direction.
+    heads = 2
+    cache, table, slots = _pages(1, n, heads, dim, 64, dtype)
+    k = 0.05 * torch.randn(1, n, heads, dim, generator=_gen(1), device="cuda")
+    v = 0.5 + torch.rand(1, n, heads, dim, generator=_gen(2), device="cuda")
+    _write(cache, slots, k, v)
+    q = _few_channels(1, queries, heads * share, dim, dtype, 1.0)
+    lengths = torch.tensor([n], dtype=torch.int32, device="cuda")
+    out = qr.kv8_attention(q, cache, table, lengths, window=window)
+    _check(out, q, cache, slots, lengths, 4, window=window, rows=[0, 1, 300, -2, -1])
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_long_sums_under_rising_scores(dim, dtype):
+    # The largest score keeps growing, so what has been summed, and what was set aside, keeps being scaled down.
+    heads, share, queries, n = 2, 8, 1024, 6000
+    cache, table, slots = _pages(1, n, heads, dim, 64, dtype)
+    k = 0.05 * torch.randn(1, n, heads, dim, generator=_gen(1), device="cuda")
+    k[..., 0] = torch.linspace(0, 4, n, device="cuda")[None, :, None]
+    v = 0.5 + torch.rand(1, n, heads, dim, generator=_gen(2), device="cuda")
+    _write(cache, slots, k, v)
+    q = _few_channels(1, queries, heads * share, dim, dtype, 1.0)
+    q[..., 0] = torch.linspace(1, 8, heads * share, device="cuda") * dim**0.5 / 4
+    lengths = torch.tensor([n], dtype=torch.int32, device="cuda")
+    _check(qr.kv8_attention(q, cache, table, lengths), q, cache, slots, lengths, 4, rows=[0, 1, 300, -2, -1])
