@@ -22,8 +22,8 @@
 // and 0.7 % of the fp16 results are then not the nearest (of elementary 32-bit operations 0.1 % of the bf16 ones).
 //
 // P is two fp16 numbers, high and low, 22 bits. (One would do for bf16 results but for a tenth of them, which then are
-// not the nearest.) It is scaled by a power of two that puts the largest step of the
-// values at 2^11, so weights keep their leading bits down to 2^-25 of the largest.
+// not the nearest.) It is scaled, a row at a time, by a power of two that puts the largest weight times step that the row has met
+// at 2^11, so weights keep their leading bits down to 2^-25 of the largest, whatever pages the row does not see or has no weight for.
 #pragma once
 
 #include "codes.cuh"
@@ -34,7 +34,7 @@ namespace qrb200 {
 constexpr int kPromptRows = 256, kPromptTokens = 64;
 constexpr int kPromptStages = 3, kPromptRaw = 2;  // steps of operands, and of bytes, in shared memory (four and two 151 us)
 constexpr int kPromptThreads = 32 * 15;
-constexpr int kPromptStepExp = 11;
+constexpr int kPromptTop = 11;  // a row's largest weight times step is put below this power of two, and stays below 2^(11 + 4)
 // Steps between settings-aside, a power of two. (Both types, 2 x 2048 queries over 4096 tokens: never 158 us, 32 166, 16 183, 8 209.)
 __host__ __device__ constexpr int prompt_aside(bool half) { return half ? 16 : 32; }
 __host__ __device__ constexpr int prompt_tile(int dim) { return 128 * dim * 2; }  // bytes of 128 rows of fp16
@@ -73,6 +73,14 @@ __device__ __forceinline__ void tmem_put16(uint32_t taddr, const uint32_t (&v)[1
       : "memory");
 }
 __device__ __forceinline__ void tmem_put_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// A value's step times a row's unit. (Beyond 2^100 only where weights are below 2^-100: bounded, so that none of them times
+// this is infinite. NaN stays.)
+__device__ __forceinline__ float prompt_scaled(float step, float unit) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(step * unit), "f"(0x1p100f));
+  return r;
+}
 
 // Sums set aside in global memory, by one thread each: added to where they lie, so that nothing waits for them.
 __device__ __forceinline__ void aside_store(float4* to, const float4& x) {
@@ -131,11 +139,11 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(Kv8AttnPa
   // (A softmax may be two steps ahead of the products with the values, and a barrier tells a phase only from the one before it:
   // so each step waits for a barrier whose last phase but one is known to be over.)
   __shared__ uint32_t s_tmem;
-  __shared__ float4 s_key[kPromptStages], s_value[kPromptStages];  // steps of a stage's runs, scaled
+  __shared__ float4 s_key[kPromptStages], s_value[kPromptStages];  // steps of a stage's runs, the keys' scaled
   __shared__ int s_gone[kPromptStages];      // bits: runs without a page
   __shared__ float2 s_step[kPromptRaw][4];
   __shared__ int s_missing[kPromptRaw];
-  __shared__ unsigned s_most[2][15];
+  __shared__ unsigned s_most[15];
   __shared__ volatile int s_bad;  // a wait ran out: keep to the barriers, write nothing
   unsigned char* sq = align1024(smem_raw);
   unsigned char* sk = sq + 2 * kTile;  // stages of [keys][values], half a tile each
@@ -210,30 +218,24 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(Kv8AttnPa
   };
   const float2* steps = reinterpret_cast<const float2*>(P.range);
 
-  // The largest steps of the pages that are seen.
-  unsigned most[2] = {0, 0};
+  // The largest step of the keys' pages that are seen.
+  unsigned most = 0;
   const int page_runs = P.sh.page / 16;
   for (int page = first_run / page_runs + threadIdx.x; page * page_runs < last_run; page += kPromptThreads) {
     const int at = page_of(max(first_run, page * page_runs));
     if (at >= 0) {
-      const float2 step = __ldg(steps + (long long)at * P.sh.heads + head);
-      if (step.x == step.x) most[0] = max(most[0], __float_as_uint(kv8_step(step.x)));  // (not NaN)
-      if (step.y == step.y) most[1] = max(most[1], __float_as_uint(kv8_step(step.y)));
+      const float range = __ldg(P.range + ((long long)at * P.sh.heads + head) * 2);
+      if (range == range) most = max(most, __float_as_uint(kv8_step(range)));  // (not NaN)
     }
   }
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    most[i] = __reduce_max_sync(kFullMask, most[i]);
-    if (lane == 0) s_most[i][warp] = most[i];
-  }
+  most = __reduce_max_sync(kFullMask, most);
+  if (lane == 0) s_most[warp] = most;
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   // The keys' steps are held relative to 2^key_power, a row's factor takes that back: together they are in range
-  // wherever the largest scores are. The values' are scaled by 2^kPromptStepExp / 2^cap, with 2^cap above the largest.
-  const int key_power = (int)(__reduce_max_sync(kFullMask, lane < 15 ? s_most[0][lane] : 0u) >> 23) - 127;
-  const int cap = max(-100, min(126, (int)(__reduce_max_sync(kFullMask, lane < 15 ? s_most[1][lane] : 0u) >> 23) - 126));
-  const float scaled = __int_as_float((kPromptStepExp - cap + 127) << 23), lower = __int_as_float((cap - kPromptStepExp + 127) << 23);
+  // wherever the largest scores are.
+  const int key_power = (int)(__reduce_max_sync(kFullMask, lane < 15 ? s_most[lane] : 0u) >> 23) - 127;
   const uint32_t tmem = s_tmem;
   const int aside_every = P.part_o ? prompt_aside(std::is_same<T, __half>::value) : 1 << 30;
 
@@ -291,7 +293,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(Kv8AttnPa
     if (mine < both) {
       // What every row of the warp sees.
       const int in_lo = __reduce_max_sync(kFullMask, lo), in_hi = __reduce_min_sync(kFullMask, real ? hi : 0x7fffffff);
-      float ref = kNone, sum = 0.f;  // weights are 2^(score - ref)
+      // Weights are 2^(score - ref); with their steps they are held times `unit`, which puts the largest that the row has met, 2^(reach
+      // - ref) at most, at 2^kPromptTop. A row's numbers hang on nothing but what the row sees.
+      float ref = kNone, sum = 0.f, reach = kNone, unit = 1.f;
       // Set aside, four channels of a row beside the next row's: the sums of earlier steps, against the reference of then, which `lag`
       // brings to the present one.
       const auto set_aside = [&]() {
@@ -316,10 +320,11 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(Kv8AttnPa
           for (int c = 0; c < 4; ++c) tmem_arrived(v[c]);
           const int gone = s_gone[st];
           const bool full = tok0 >= in_lo && tok0 + kPromptTokens <= in_hi && gone == 0;
-          // The largest score. (Factors are not negative, so a run's largest product gives its largest score.)
+          // The largest score, and the largest one with the power of two above its value's step. (Factors are not negative, so a run's
+          // largest product gives its largest score.)
           const auto largest = [&](auto all) {
             constexpr bool kAll = decltype(all)::value;
-            float top = kNone;
+            float2 top = make_float2(kNone, kNone);
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
               float m = kNone;
@@ -331,14 +336,26 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(Kv8AttnPa
                   const float x = v[c][4 * r + i];
                   m = kAll || (at >= lo && at < hi && !(gone >> r & 1)) ? fmaxf(m, x) : m;
                 }
-              top = kAll || m > kNone ? fmaxf(top, m * f[r]) : top;
+              const float score = kAll || m > kNone ? m * f[r] : kNone;
+              top.x = fmaxf(top.x, score);
+              top.y = fmaxf(top.y, score + (__uint_as_float(__float_as_uint(w[r]) >> 23 | 0x4b000000u) - (8388608.f + 126.f)));
             }
             return top;
           };
-          const float top = full ? largest(std::true_type{}) : largest(std::false_type{});
-          const bool move = top > __fadd_rd(ref, kKvLazy) || (ref == kNone && top > kNone);
+          const float2 top = full ? largest(std::true_type{}) : largest(std::false_type{});
+          const bool move = top.x > __fadd_rd(ref, kKvLazy) || top.y > __fadd_rd(reach, kKvLazy) || (ref == kNone && top.x > kNone);
           if (__any_sync(kFullMask, move)) {
-            const float next = fmaxf(ref, top), keep = ref == kNone ? 0.f : kv_exp2(ref - next);
+            float keep = 1.f, ratio = 1.f;
+            const bool none = ref == kNone;
+            if (move) {
+              const float next = fmaxf(ref, top.x);
+              reach = fmaxf(reach, top.y);
+              const int power = min(100, max(-126, kPromptTop - (int)ceilf(reach - next))), by = power - kv8_power(unit);
+              keep = none ? 0.f : kv_exp2(ref - next);
+              ratio = by < -126 ? 0.f : kv_power(by);
+              unit = kv_power(power);
+              ref = next;
+            }
             if ((j & (aside_every - 1)) != 0) {  // once the products before are over
               ok = ok && mbar_wait_quick(&o_full[mine][(j - 1) & 1], ((j - 1) >> 1) & 1);
               __syncwarp();
@@ -350,15 +367,15 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(Kv8AttnPa
                 tmem_arrived(o);
                 uint32_t kept[16];
 #pragma unroll
-                for (int i = 0; i < 16; ++i) kept[i] = __float_as_uint(ref == kNone ? 0.f : o[i] * keep);
+                for (int i = 0; i < 16; ++i) kept[i] = __float_as_uint(none ? 0.f : o[i] * (keep * ratio));
                 tmem_put16(o_at + c, kept);
               }
               tmem_put_wait();
             }
             sum *= keep;
-            lag *= keep;
-            ref = next;
+            lag *= keep * ratio;
           }
+          const float scaled[4] = {prompt_scaled(w[0], unit), prompt_scaled(w[1], unit), prompt_scaled(w[2], unit), prompt_scaled(w[3], unit)};
           const float less = ref == kNone ? 0.f : -ref;
           const float2 less2 = make_float2(less, less);
           float2 sums = make_float2(0.f, 0.f);
@@ -371,7 +388,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(Kv8AttnPa
               for (int d = 0; d < 2; ++d)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                  const float2 f2 = make_float2(f[r], f[r]), w2 = make_float2(w[r], w[r]);
+                  const float2 f2 = make_float2(f[r], f[r]), w2 = make_float2(scaled[r], scaled[r]);
 #pragma unroll
                   for (int i = 0; i < 4; i += 2) {
                     const float2 x = __ffma2_rn(make_float2(v[c + d][4 * r + i], v[c + d][4 * r + i + 1]), f2, less2);
@@ -413,7 +430,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(Kv8AttnPa
       if (!ok) s_bad = 1;
       __syncwarp();
       tc_fence_after();
-      const float inv = sum == 0.f ? 0.f : lower / sum;  // nothing seen: zeros
+      const float inv = sum == 0.f ? 0.f : kv_power(-kv8_power(unit)) / sum;  // nothing seen: zeros
       T* out = static_cast<T*>(P.out) + (((long long)b * P.queries + row / P.share) * P.q_heads + head * P.share + row % P.share) * kDim;
       const bool apart = count > aside_every;
       float4 a[2][8];
@@ -489,7 +506,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(Kv8AttnPa
       if (cw == 0 && lane < 4) {
         const float2 step = s_step[rs][lane];
         reinterpret_cast<float*>(&s_key[st])[lane] = step.x > 0.f ? kv8_part(step.x) * P.scale_part * kv_power(kv8_power(step.x) - key_power) : step.x;  // 0 and NaN as they are
-        reinterpret_cast<float*>(&s_value[st])[lane] = step.y * scaled;
+        reinterpret_cast<float*>(&s_value[st])[lane] = step.y;
         if (lane == 0) s_gone[st] = s_missing[rs];
       }
       fence_async_smem();

@@ -143,3 +143,52 @@ def test_long_sums_under_rising_scores(dim, dtype):
     q[..., 0] = torch.linspace(1, 8, heads * share, device="cuda") * dim**0.5 / 4
     lengths = torch.tensor([n], dtype=torch.int32, device="cuda")
     _check(qr.kv8_attention(q, cache, table, lengths), q, cache, slots, lengths, 4, rows=[0, 1, 300, -2, -1])
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("batch, heads, share, queries", [(40, 8, 4, 40)])
+@pytest.mark.parametrize("window", [None, 60])
+def test_large_values_that_a_row_does_not_see(window, batch, heads, share, queries, dim, dtype):
+    # the last page's values reach far beyond the others'; so do, with a window, those of the page that the first queries see last
+    n, page = 200, 16
+    cache, table, slots = _pages(batch, n, heads, dim, page, dtype)
+    _write(cache, slots, _randn(batch, n, heads, dim, seed=1), _randn(batch, n, heads, dim, seed=2))
+    cache.range[..., 1] *= 2.0**-16
+    q = _few_channels(batch, queries, heads * share, dim, dtype, 1.5 * dim**0.5)
+    lengths = torch.full((batch,), n, dtype=torch.int32, device="cuda")
+    pos = n - queries + torch.arange(queries, device="cuda")
+    blind = pos < 192  # pages 12 (tokens 192 on) and, with a window, 6 (tokens 96 to 111, which queries from 172 on do not see)
+    pages = [12]
+    if window:
+        blind &= pos >= 172
+        pages.append(6)
+    want = qr.kv8_attention(q, cache, table, lengths, window=window)
+    for up in (2.0**26, 2.0**29 if dtype == HF else 2.0**40):  # within fp16's range
+        grown = qr.KV8Cache(cache.data, cache.range.clone(), page, dim, dtype)
+        grown.range[table[:, pages].long(), :, 1] *= up
+        out = qr.kv8_attention(q, grown, table, lengths, window=window)
+        assert torch.equal(out[:, blind], want[:, blind]) and not torch.equal(out[:, ~blind], want[:, ~blind])
+        _check(out[:1], q[:1], grown, slots, lengths, 4, window=window)
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("batch, heads, share, queries", [(40, 8, 4, 40)])
+def test_large_values_without_weight(batch, heads, share, queries, dim, dtype):
+    # pages of values 2^50 times the others', whose scores leave them a weight of about 2^-90
+    n, page = 200, 16
+    cache, table, slots = _pages(batch, n, heads, dim, page, dtype)
+    k = torch.randn(batch, n, heads, dim, generator=_gen(1), device="cuda")
+    k[..., 0] = 0
+    k[:, 16:32, :, 0] = -8
+    k[:, 192:, :, 0] = -8
+    _write(cache, slots, k, _randn(batch, n, heads, dim, seed=2))
+    cache.range[..., 1] *= 2.0**-20
+    cache.range[table[:, [1, 12]].long(), :, 1] *= 2.0**50
+    q = _few_channels(batch, queries, heads * share, dim, dtype, 0.5 * dim**0.5)
+    q[..., 0] = 8 * dim**0.5
+    lengths = torch.full((batch,), n, dtype=torch.int32, device="cuda")
+    out = qr.kv8_attention(q, cache, table, lengths)
+    assert out.float().abs().amax() < 2.0**-14
+    _check(out[:2], q[:2], cache, slots, lengths, 4)
