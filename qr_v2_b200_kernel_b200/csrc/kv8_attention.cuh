@@ -46,8 +46,18 @@ __device__ __forceinline__ uint32_t kv8_codes(uint32_t w) {
 __device__ __forceinline__ float kv8_part(float x) { return __uint_as_float((__float_as_uint(x) & 0x807fffffu) | 0x3f800000u); }
 __device__ __forceinline__ int kv8_power(float x) { return (int)(__float_as_uint(x) >> 23 & 255) - 127; }
 
+// The power of two above a step, as its exponent.
+__device__ __forceinline__ float kv8_above(float step) { return __uint_as_float(__float_as_uint(step) >> 23 | 0x4b000000u) - (8388608.f + 126.f); }
+// A value's step times a row's unit. (Beyond 2^100 only where weights are below 2^-100: bounded, so that none of them times
+// this is infinite. NaN stays.)
+__device__ __forceinline__ float kv8_scaled(float step, float unit) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(step * unit), "f"(0x1p100f));
+  return r;
+}
+
 constexpr int kKv8Top = 14;      // where a query row's largest entry is put (its exponent)
-constexpr int kKv8StepExp = 10;  // the largest value step's place: weights stay below 2^(10 + 4) in fp16
+constexpr int kKv8StepExp = 10;  // a row's largest weight times step is put below this power of two, and stays below 2^(10 + 4)
 constexpr int kKv8Aside = 8;     // steps between settings-aside
 
 // Bytes of a warp's step, 4 KB or 8: a step costs some 1000 clocks of instructions that wait for one another and 500 for each
@@ -237,11 +247,16 @@ __global__ void __launch_bounds__(32 * kKvWarps, kv8_ctas(kBrief)) kv8_attention
   float2 sum[kNT] = {};
   // Weights are 2^(score + less), the reference being -less; bound is where a score moves it: 4
   // above, rounded down where scores are so large (so the reference cannot be had back from it), and
-  // -inf while nothing has been seen. cap bounds the value steps, unit scales them.
-  float2 less[kNT] = {};
-  float bound[kNT][2], cap = 0.f, unit = 1.f;
+  // -inf while nothing has been seen. With their steps weights are held times `unit`, which puts the largest that the row has met
+  // at 2^kKv8StepExp; reach is where a score with the power of two above its value's step moves it, 4 above. A row's numbers hang on
+  // nothing but what the row sees.
+  float2 less[kNT] = {}, unit[kNT];
+  float bound[kNT][2], reach[kNT][2];
 #pragma unroll
-  for (int n = 0; n < kNT; ++n) bound[n][0] = bound[n][1] = kNone;
+  for (int n = 0; n < kNT; ++n) {
+    bound[n][0] = bound[n][1] = reach[n][0] = reach[n][1] = kNone;
+    unit[n] = make_float2(1.f, 1.f);
+  }
   const auto reference = [&](int n, int c) { return bound[n][c] == kNone ? kNone : -(c ? less[n].y : less[n].x); };
 
   // This lane's sums set aside, 32 lanes apart; `aside` once there are some.
@@ -320,57 +335,53 @@ __global__ void __launch_bounds__(32 * kKvWarps, kv8_ctas(kBrief)) kv8_attention
             }
         }
       }
-      float up[kNT][2], most = 0.f;
-#pragma unroll
-      for (int i = 0; i < kRuns; ++i) most = fmaxf(most, steps[i].y);
-      bool move = most > cap;
+      float up[kNT][2], far[kNT][2];  // the largest score, and with the power of two above its value's step
+      bool move = false;
 #pragma unroll
       for (int n = 0; n < kNT; ++n) {
-        up[n][0] = s[0][n][0].x;
-        up[n][1] = s[0][n][0].y;
+        up[n][0] = up[n][1] = far[n][0] = far[n][1] = kNone;
 #pragma unroll
-        for (int i = 0; i < kRuns; ++i)
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            up[n][0] = fmaxf(up[n][0], s[i][n][h].x);
-            up[n][1] = fmaxf(up[n][1], s[i][n][h].y);
-          }
-        move = move || up[n][0] > bound[n][0] || up[n][1] > bound[n][1];
+        for (int i = 0; i < kRuns; ++i) {
+          const float e = kv8_above(steps[i].y), x = fmaxf(s[i][n][0].x, s[i][n][1].x), y = fmaxf(s[i][n][0].y, s[i][n][1].y);
+          up[n][0] = fmaxf(up[n][0], x), far[n][0] = fmaxf(far[n][0], x + e);
+          up[n][1] = fmaxf(up[n][1], y), far[n][1] = fmaxf(far[n][1], y + e);
+        }
+        move = move || up[n][0] > bound[n][0] || up[n][1] > bound[n][1] || far[n][0] > reach[n][0] || far[n][1] > reach[n][1];
       }
       if (__any_sync(kFullMask, move)) {
-        most = fmaxf(most, cap);  // the same in every lane
-        float ratio = 1.f;
-        if (most > cap) {  // the power of two above the largest step, and the scale that puts it at 2^kKv8StepExp
-          const int e = max(-100, min(126, (int)(__float_as_uint(most) >> 23) - 126));
-          cap = __int_as_float((e + 127) << 23);
-          const float fresh = __int_as_float((kKv8StepExp - e + 127) << 23);
-          ratio = fresh / unit;
-          unit = fresh;
-        }
 #pragma unroll
         for (int n = 0; n < kNT; ++n) {
-          float keep[2];
+          float keep[2], all[2];
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
 #pragma unroll
-            for (int x = 4; x < 32; x <<= 1) up[n][c] = fmaxf(up[n][c], __shfl_xor_sync(kFullMask, up[n][c], x));
-            const float last = reference(n, c), next = fmaxf(up[n][c], last);
-            keep[c] = next == kNone ? 0.f : kv_exp2(last - next);
-            bound[n][c] = __fadd_rd(next, kKvLazy);
-            // A row that has seen nothing has the reference -inf: its weights, 2^-inf, come from any
-            // finite one.
-            (c ? less[n].y : less[n].x) = next == kNone ? 0.f : -next;
+            for (int x = 4; x < 32; x <<= 1) {
+              up[n][c] = fmaxf(up[n][c], __shfl_xor_sync(kFullMask, up[n][c], x));
+              far[n][c] = fmaxf(far[n][c], __shfl_xor_sync(kFullMask, far[n][c], x));
+            }
+            keep[c] = all[c] = 1.f;
+            if (up[n][c] > bound[n][c] || far[n][c] > reach[n][c]) {
+              const float last = reference(n, c), next = fmaxf(up[n][c], last), was = c ? unit[n].y : unit[n].x;
+              const float top = reach[n][c] == kNone ? far[n][c] : fmaxf(far[n][c], reach[n][c] - kKvLazy);
+              const int power = min(100, max(-126, kKv8StepExp - (int)ceilf(top - next))), by = power - kv8_power(was);
+              keep[c] = kv_exp2(last - next);
+              all[c] = keep[c] * (by < -126 ? 0.f : kv_power(by));
+              bound[n][c] = __fadd_rd(next, kKvLazy);
+              reach[n][c] = __fadd_rd(top, kKvLazy);
+              (c ? less[n].y : less[n].x) = -next;
+              (c ? unit[n].y : unit[n].x) = kv_power(power);
+            }
           }
           sum[n] = make_float2(sum[n].x * keep[0], sum[n].y * keep[1]);
 #pragma unroll
           for (int j = 0; j < kSteps; ++j)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) o[n][j][e] *= keep[e & 1] * ratio;
+            for (int e = 0; e < 4; ++e) o[n][j][e] *= all[e & 1];
           if (aside) {
 #pragma unroll
             for (int j = 0; j < kSteps; ++j) {
               float4 a = apart[32 * (n * kSteps + j)];
-              a.x *= keep[0] * ratio, a.y *= keep[1] * ratio, a.z *= keep[0] * ratio, a.w *= keep[1] * ratio;
+              a.x *= all[0], a.y *= all[1], a.z *= all[0], a.w *= all[1];
               apart[32 * (n * kSteps + j)] = a;
             }
           }
@@ -382,14 +393,14 @@ __global__ void __launch_bounds__(32 * kKvWarps, kv8_ctas(kBrief)) kv8_attention
 #pragma unroll
         for (int i = 0; i < kRuns; ++i) {
           uint32_t w[2][kNT][2];
-          const float scaled = steps[i].y * unit;
 #pragma unroll
-          for (int n = 0; n < kNT; ++n)
+          for (int n = 0; n < kNT; ++n) {
+            const float2 scaled = make_float2(kv8_scaled(steps[i].y, unit[n].x), kv8_scaled(steps[i].y, unit[n].y));
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
               const float2 e = __fadd2_rn(s[i][n][h], less[n]), p = make_float2(kv_exp2(e.x), kv_exp2(e.y));
               sum[n] = __fadd2_rn(sum[n], p);
-              float2 x = __fmul2_rn(p, make_float2(scaled, scaled));
+              float2 x = __fmul2_rn(p, scaled);
               if constexpr (!kAll) {  // what a row does not see may be NaN
                 if (!(seen[n] >> (4 * i + 2 * h) & 1)) x.x = 0.f;
                 if (!(seen[n] >> (4 * i + 2 * h) & 2)) x.y = 0.f;
@@ -399,6 +410,7 @@ __global__ void __launch_bounds__(32 * kKvWarps, kv8_ctas(kBrief)) kv8_attention
               const float2 top = __half22float2(__hneg2(reinterpret_cast<const __half2&>(high)));
               w[1][n][h] = kv_transpose(kv_pack(__fadd2_rn(x, top)));
             }
+          }
 #pragma unroll
           for (int c = 0; c < kDim / 32; ++c) {
             uint32_t vc[4];
@@ -455,13 +467,13 @@ __global__ void __launch_bounds__(32 * kKvWarps, kv8_ctas(kBrief)) kv8_attention
   __syncthreads();  // the rings are free
   float(*s_o)[kRows][kDim + 4] = reinterpret_cast<float(*)[kRows][kDim + 4]>(s_ring);
 
-  const float lower = 1.f / unit;
   // The warps' parts: o[n][j][e] is channel 16 j + g + 8 (e / 2) of row 8 n + 2 t + e % 2.
 #pragma unroll
   for (int n = 0; n < kNT; ++n)
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
       float l = c ? sum[n].y : sum[n].x;
+      const float lower = kv_power(-kv8_power(c ? unit[n].y : unit[n].x));
 #pragma unroll
       for (int x = 4; x < 32; x <<= 1) l += __shfl_xor_sync(kFullMask, l, x);
       if (g == 0) s_ml[warp][8 * n + 2 * t + c] = make_float2(reference(n, c), l);

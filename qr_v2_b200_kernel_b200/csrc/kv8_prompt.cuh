@@ -74,14 +74,6 @@ __device__ __forceinline__ void tmem_put16(uint32_t taddr, const uint32_t (&v)[1
 }
 __device__ __forceinline__ void tmem_put_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// A value's step times a row's unit. (Beyond 2^100 only where weights are below 2^-100: bounded, so that none of them times
-// this is infinite. NaN stays.)
-__device__ __forceinline__ float prompt_scaled(float step, float unit) {
-  float r;
-  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(step * unit), "f"(0x1p100f));
-  return r;
-}
-
 // Sums set aside in global memory, by one thread each: added to where they lie, so that nothing waits for them.
 __device__ __forceinline__ void aside_store(float4* to, const float4& x) {
   asm volatile("st.relaxed.gpu.global.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(to), "f"(x.x), "f"(x.y), "f"(x.z), "f"(x.w) : "memory");
@@ -338,7 +330,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(Kv8AttnPa
                 }
               const float score = kAll || m > kNone ? m * f[r] : kNone;
               top.x = fmaxf(top.x, score);
-              top.y = fmaxf(top.y, score + (__uint_as_float(__float_as_uint(w[r]) >> 23 | 0x4b000000u) - (8388608.f + 126.f)));
+              top.y = fmaxf(top.y, score + kv8_above(w[r]));
             }
             return top;
           };
@@ -375,7 +367,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(Kv8AttnPa
             sum *= keep;
             lag *= keep * ratio;
           }
-          const float scaled[4] = {prompt_scaled(w[0], unit), prompt_scaled(w[1], unit), prompt_scaled(w[2], unit), prompt_scaled(w[3], unit)};
+          const float scaled[4] = {kv8_scaled(w[0], unit), kv8_scaled(w[1], unit), kv8_scaled(w[2], unit), kv8_scaled(w[3], unit)};
           const float less = ref == kNone ? 0.f : -ref;
           const float2 less2 = make_float2(less, less);
           float2 sums = make_float2(0.f, 0.f);

@@ -147,22 +147,23 @@ def test_long_sums_under_rising_scores(dim, dtype):
 
 @pytest.mark.parametrize("dtype", [BF, HF])
 @pytest.mark.parametrize("dim", [64, 128])
-@pytest.mark.parametrize("batch, heads, share, queries", [(40, 8, 4, 40)])
-@pytest.mark.parametrize("window", [None, 60])
-def test_large_values_that_a_row_does_not_see(window, batch, heads, share, queries, dim, dtype):
-    # the last page's values reach far beyond the others'; so do, with a window, those of the page that the first queries see last
-    n, page = 200, 16
+@pytest.mark.parametrize("batch, heads, share, queries, n, window", [
+    (40, 8, 4, 40, 200, None), (40, 8, 4, 40, 200, 60), (2, 2, 8, 12, 200, None), (2, 2, 8, 12, 200, 78), (2, 3, 1, 8, 197, None), (2, 3, 1, 8, 197, 79)])
+def test_large_values_that_a_row_does_not_see(batch, heads, share, queries, n, window, dim, dtype):
+    # the last page's values reach far beyond the others'; so do, with a window, those of a page that only the first queries see
+    page = 16
     cache, table, slots = _pages(batch, n, heads, dim, page, dtype)
     _write(cache, slots, _randn(batch, n, heads, dim, seed=1), _randn(batch, n, heads, dim, seed=2))
     cache.range[..., 1] *= 2.0**-16
     q = _few_channels(batch, queries, heads * share, dim, dtype, 1.5 * dim**0.5)
     lengths = torch.full((batch,), n, dtype=torch.int32, device="cuda")
     pos = n - queries + torch.arange(queries, device="cuda")
-    blind = pos < 192  # pages 12 (tokens 192 on) and, with a window, 6 (tokens 96 to 111, which queries from 172 on do not see)
+    blind = pos < 192  # pages 12 (tokens 192 on) and, with a window, 6 (tokens 96 to 111)
     pages = [12]
     if window:
-        blind &= pos >= 172
+        blind &= pos - window >= 111
         pages.append(6)
+    assert blind.any() and not blind.all()
     want = qr.kv8_attention(q, cache, table, lengths, window=window)
     for up in (2.0**26, 2.0**29 if dtype == HF else 2.0**40):  # within fp16's range
         grown = qr.KV8Cache(cache.data, cache.range.clone(), page, dim, dtype)
@@ -174,7 +175,7 @@ def test_large_values_that_a_row_does_not_see(window, batch, heads, share, queri
 
 @pytest.mark.parametrize("dtype", [BF, HF])
 @pytest.mark.parametrize("dim", [64, 128])
-@pytest.mark.parametrize("batch, heads, share, queries", [(40, 8, 4, 40)])
+@pytest.mark.parametrize("batch, heads, share, queries", [(40, 8, 4, 40), (2, 2, 8, 5), (2, 2, 8, 1), (1, 1, 1, 1)])
 def test_large_values_without_weight(batch, heads, share, queries, dim, dtype):
     # pages of values 2^50 times the others', whose scores leave them a weight of about 2^-90
     n, page = 200, 16
