@@ -301,10 +301,10 @@ __global__ void __launch_bounds__(32 * kKvWarps, kv8_ctas(kBrief)) kv8_attention
         for (int i = 0; i < kRuns; ++i) {
           steps[i] = s_step[warp][stage][i];
           const float keys = steps[i].x > 0.f ? kv8_part(steps[i].x) * P.scale_part : steps[i].x;  // 0 and NaN as they are
-          const int e = kv8_power(steps[i].x);
+          const int e = kv8_power(steps[i].x);  // (factors below 2^97, products below 2^29: no score is infinite, nor 0 times one NaN)
 #pragma unroll
           for (int n = 0; n < kNT; ++n) {
-            const float2 f = make_float2(keys * kv_power(e + back[n][0]), keys * kv_power(e + back[n][1]));
+            const float2 f = make_float2(keys * kv_power(min(94, e + back[n][0])), keys * kv_power(min(94, e + back[n][1])));
 #pragma unroll
             for (int h = 0; h < 2; ++h) s[i][n][h] = __fmul2_rn(make_float2(acc[i][n][2 * h], acc[i][n][2 * h + 1]), f);
           }

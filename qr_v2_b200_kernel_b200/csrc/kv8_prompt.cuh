@@ -74,6 +74,14 @@ __device__ __forceinline__ void tmem_put16(uint32_t taddr, const uint32_t (&v)[1
 }
 __device__ __forceinline__ void tmem_put_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+// What turns a row's products with a run's codes into scores. (Products are 2^-24 to 2^29, if not 0: bounded, so that none of them
+// times this is infinite, nor 0 times it NaN. NaN stays.)
+__device__ __forceinline__ float kv8_factor(float step, float2 back) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(step * back.x * back.y), "f"(0x1p97f));
+  return r;
+}
+
 // Sums set aside in global memory, by one thread each: added to where they lie, so that nothing waits for them.
 __device__ __forceinline__ void aside_store(float4* to, const float4& x) {
   asm volatile("st.relaxed.gpu.global.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(to), "f"(x.x), "f"(x.y), "f"(x.z), "f"(x.w) : "memory");
@@ -135,7 +143,6 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(Kv8AttnPa
   __shared__ int s_gone[kPromptStages];      // bits: runs without a page
   __shared__ float2 s_step[kPromptRaw][4];
   __shared__ int s_missing[kPromptRaw];
-  __shared__ unsigned s_most[15];
   __shared__ volatile int s_bad;  // a wait ran out: keep to the barriers, write nothing
   unsigned char* sq = align1024(smem_raw);
   unsigned char* sk = sq + 2 * kTile;  // stages of [keys][values], half a tile each
@@ -209,25 +216,11 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(Kv8AttnPa
     return page;
   };
   const float2* steps = reinterpret_cast<const float2*>(P.range);
-
-  // The largest step of the keys' pages that are seen.
-  unsigned most = 0;
   const int page_runs = P.sh.page / 16;
-  for (int page = first_run / page_runs + threadIdx.x; page * page_runs < last_run; page += kPromptThreads) {
-    const int at = page_of(max(first_run, page * page_runs));
-    if (at >= 0) {
-      const float range = __ldg(P.range + ((long long)at * P.sh.heads + head) * 2);
-      if (range == range) most = max(most, __float_as_uint(kv8_step(range)));  // (not NaN)
-    }
-  }
-  most = __reduce_max_sync(kFullMask, most);
-  if (lane == 0) s_most[warp] = most;
+
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  // The keys' steps are held relative to 2^key_power, a row's factor takes that back: together they are in range
-  // wherever the largest scores are.
-  const int key_power = (int)(__reduce_max_sync(kFullMask, lane < 15 ? s_most[lane] : 0u) >> 23) - 127;
   const uint32_t tmem = s_tmem;
   const int aside_every = P.part_o ? prompt_aside(std::is_same<T, __half>::value) : 1 << 30;
 
@@ -237,7 +230,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(Kv8AttnPa
     const bool real = row < rows;
     const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16), o_at = lanes + 256 + 128 * mine;
     int lo = 0, hi = 0;
-    float back;  // the power of two that takes a row's size, the scale's and the keys' back, into the exponent's units (base 2)
+    float2 back;  // two powers of two that take a row's size and the scale's back, into the exponent's units (base 2)
     if (real) range_of(row, lo, hi);
     {
       // The row's query, permuted as the keys' bytes are: piece k of 64 channels holds channels 16 w + 4 t + e with t =
@@ -264,7 +257,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(Kv8AttnPa
       }
       const int power = max(1, min(254, (int)(top >> 23))) - 127, lift = kKv8Top - power;
       const float up = kv_power(lift / 2), more = kv_power(lift - lift / 2);
-      back = kv_power(power - kKv8Top + P.scale_power + key_power);
+      const int by = power - kKv8Top + P.scale_power;
+      back = make_float2(kv_power(by / 2), kv_power(by - by / 2));
 #pragma unroll 1
       for (int a = 0; a < kAtoms; ++a)
 #pragma unroll
@@ -307,7 +301,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(Kv8AttnPa
 #pragma unroll
           for (int c = 0; c < 4; ++c) tmem_ask16(s_at + 16 * c, v[c]);
           const float4 k4 = s_key[st], w4 = s_value[st];
-          const float f[4] = {k4.x * back, k4.y * back, k4.z * back, k4.w * back}, w[4] = {w4.x, w4.y, w4.z, w4.w};
+          const float f[4] = {kv8_factor(k4.x, back), kv8_factor(k4.y, back), kv8_factor(k4.z, back), kv8_factor(k4.w, back)}, w[4] = {w4.x, w4.y, w4.z, w4.w};
 #pragma unroll
           for (int c = 0; c < 4; ++c) tmem_arrived(v[c]);
           const int gone = s_gone[st];
@@ -497,7 +491,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(Kv8AttnPa
       }
       if (cw == 0 && lane < 4) {
         const float2 step = s_step[rs][lane];
-        reinterpret_cast<float*>(&s_key[st])[lane] = step.x > 0.f ? kv8_part(step.x) * P.scale_part * kv_power(kv8_power(step.x) - key_power) : step.x;  // 0 and NaN as they are
+        reinterpret_cast<float*>(&s_key[st])[lane] = step.x * P.scale_part;  // (steps are 2^-107 to 2^121, the scale's part below 3)
         reinterpret_cast<float*>(&s_value[st])[lane] = step.y;
         if (lane == 0) s_gone[st] = s_missing[rs];
       }

@@ -193,3 +193,34 @@ def test_large_values_without_weight(batch, heads, share, queries, dim, dtype):
     out = qr.kv8_attention(q, cache, table, lengths)
     assert out.float().abs().amax() < 2.0**-14
     _check(out[:2], q[:2], cache, slots, lengths, 4)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("batch, heads, share, queries", [(40, 8, 4, 40), (2, 2, 8, 12)])
+def test_large_keys_that_a_row_does_not_see(batch, heads, share, queries, dim):
+    # queries near 2^60 over keys near 2^-60, the last page's keys near 2^100 (of bf16's range)
+    n, page = 200, 16
+    cache, table, slots = _pages(batch, n, heads, dim, page, BF)
+    _write(cache, slots, _randn(batch, n, heads, dim, seed=1), _randn(batch, n, heads, dim, seed=2))
+    cache.range[..., 0] *= 2.0**-60
+    q = _few_channels(batch, queries, heads * share, dim, BF, 1.5 * dim**0.5 * 2.0**60)
+    lengths = torch.full((batch,), n, dtype=torch.int32, device="cuda")
+    want = qr.kv8_attention(q, cache, table, lengths)
+    _check(want[:1], q[:1], cache, slots, lengths, 4)
+    blind = n - queries + torch.arange(queries, device="cuda") < 192
+    cache.range[table[:, 12].long(), :, 0] *= 2.0**160
+    assert torch.equal(qr.kv8_attention(q, cache, table, lengths)[:, blind], want[:, blind])
+
+
+@pytest.mark.parametrize("batch, heads, share, queries", [(40, 8, 4, 40), (2, 2, 8, 12), (1, 1, 1, 1)])
+def test_scores_of_nothing_under_a_factor_beyond_32_bits(batch, heads, share, queries):
+    # keys of zeros in pages whose range, with queries near 2^60, leaves 32 bits: their scores are 0
+    n, page, dim = 200, 16, 128
+    cache, table, slots = _pages(batch, n, heads, dim, page, BF)
+    k = torch.zeros(batch, n, heads, dim, device="cuda")
+    k[..., 10] = 1
+    _write(cache, slots, k, _randn(batch, n, heads, dim, seed=2))
+    cache.range[..., 0] *= 2.0**100
+    q = _few_channels(batch, queries, heads * share, dim, BF, 2.0**60)
+    lengths = torch.full((batch,), n, dtype=torch.int32, device="cuda")
+    _check(qr.kv8_attention(q, cache, table, lengths)[:2], q[:2], cache, slots, lengths, 0)
