@@ -467,16 +467,17 @@ __global__ void __launch_bounds__(32 * kKvWarps, kv8_ctas(kBrief)) kv8_attention
   __syncthreads();  // the rings are free
   float(*s_o)[kRows][kDim + 4] = reinterpret_cast<float(*)[kRows][kDim + 4]>(s_ring);
 
-  // The warps' parts: o[n][j][e] is channel 16 j + g + 8 (e / 2) of row 8 n + 2 t + e % 2.
+  // The warps' parts: o[n][j][e] is channel 16 j + g + 8 (e / 2) of row 8 n + 2 t + e % 2. With their sums of weights they are
+  // held times 2^-24, so that many of the type's largest values add up to a number still.
 #pragma unroll
   for (int n = 0; n < kNT; ++n)
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
       float l = c ? sum[n].y : sum[n].x;
-      const float lower = kv_power(-kv8_power(c ? unit[n].y : unit[n].x));
+      const float lower = kv_power(-24 - kv8_power(c ? unit[n].y : unit[n].x));
 #pragma unroll
       for (int x = 4; x < 32; x <<= 1) l += __shfl_xor_sync(kFullMask, l, x);
-      if (g == 0) s_ml[warp][8 * n + 2 * t + c] = make_float2(reference(n, c), l);
+      if (g == 0) s_ml[warp][8 * n + 2 * t + c] = make_float2(reference(n, c), l * 0x1p-24f);
 #pragma unroll
       for (int j = 0; j < kSteps; ++j) {
         s_o[warp][8 * n + 2 * t + c][16 * j + g] = o[n][j][c] * lower;

@@ -223,3 +223,19 @@ def test_scores_of_nothing_under_a_factor_beyond_32_bits(batch, heads, share, qu
     q = _few_channels(batch, queries, heads * share, dim, BF, 2.0**60)
     lengths = torch.full((batch,), n, dtype=torch.int32, device="cuda")
     _check(qr.kv8_attention(q, cache, table, lengths)[:2], q[:2], cache, slots, lengths, 0)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("batch, heads, share, queries, n", [(40, 8, 4, 40, 200), (2, 2, 8, 12, 200), (1, 1, 1, 1, 200), (1, 1, 4, 1, 8192), (1, 2, 2, 1, 70000)])
+@pytest.mark.parametrize("size", [2.0**126, 2.0**-100])
+def test_values_near_the_largest_and_the_smallest(size, batch, heads, share, queries, n, dim):
+    # of one sign under even weights: their unnormalised sum is beyond 32 bits' range, their mean is not
+    cache, table, slots = _pages(batch, n, heads, dim, 16, BF)
+    k = 0.05 * torch.randn(batch, n, heads, dim, generator=_gen(1), device="cuda")
+    _write(cache, slots, k, 0.5 + 0.5 * torch.rand(batch, n, heads, dim, generator=_gen(2), device="cuda"))
+    cache.range[..., 1] *= size
+    q = _few_channels(batch, queries, heads * share, dim, BF, 1.0)
+    lengths = torch.full((batch,), n, dtype=torch.int32, device="cuda")
+    out = qr.kv8_attention(q, cache, table, lengths)
+    assert out.isfinite().all()
+    _check(out[:2], q[:2], cache, slots, lengths, 4)
