@@ -8,13 +8,9 @@ namespace qrb200 {
 
 constexpr unsigned kFullMask = 0xffffffffu;
 
-// Named CTA barriers (id 0 is __syncthreads): bar.sync waits for nthreads arrivals, bar.arrive
-// adds this warp's arrival without waiting.
+// Named CTA barriers (id 0 is __syncthreads): waits for nthreads arrivals.
 __device__ __forceinline__ void named_sync(int id, int nthreads) {
   asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(nthreads) : "memory");
-}
-__device__ __forceinline__ void named_arrive(int id, int nthreads) {
-  asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(nthreads) : "memory");
 }
 
 // Programmatic dependent launch: let the next kernel in the stream be scheduled now, and wait
