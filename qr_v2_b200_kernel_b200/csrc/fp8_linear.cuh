@@ -196,7 +196,7 @@ __global__ void __launch_bounds__(192) fp8_few_kernel(Fp8Params P, const __grid_
     uint32_t s = 0, turn = 0;
     for (int j = 0; j < k_hi - k_lo; ++j) {
       const uint32_t buf = j & 1;
-      if ((j >= 2 && !mbar_wait_quick(&acc_empty[buf], ((j >> 1) - 1) & 1)) || !mbar_wait_quick(&full[s], turn)) {
+      if (!__all_sync(kFullMask, (j < 2 || mbar_wait_quick(&acc_empty[buf], ((j >> 1) - 1) & 1)) && mbar_wait_quick(&full[s], turn))) {
         s_bad = 1;
         break;
       }
@@ -238,7 +238,7 @@ __global__ void __launch_bounds__(192) fp8_few_kernel(Fp8Params P, const __grid_
       ask(k0 + kFp8Scales);
       for (int k = k0; k < min(k_hi, k0 + kFp8Scales); ++k, ++j) {
         const int buf = j & 1;
-        ok = ok && __all_sync(kFullMask, mbar_wait_quick(&acc_full[buf], (j >> 1) & 1));
+        ok = ok && warp_wait_quick(&acc_full[buf], (j >> 1) & 1);
         if (!ok) continue;
         tc_fence_after();
         float v[2][16];
@@ -431,7 +431,7 @@ __global__ void __launch_bounds__(128 + 32 * kFp8WideEpi, 1) __cluster_dims__(2,
       for (int tile = pair; tile < P.tiles && ok; tile += pairs)
         for (int k = 0; k < nk; ++k, ++j) {
           const uint32_t buf = j & 1;
-          ok = mbar_wait_quick(&full[s], turn) && (j < 2 || mbar_wait_quick(&acc_empty[buf], ((j >> 1) - 1) & 1));
+          ok = __all_sync(kFullMask, mbar_wait_quick(&full[s], turn) && (j < 2 || mbar_wait_quick(&acc_empty[buf], ((j >> 1) - 1) & 1)));
           if (!ok) break;
           tc_fence_after();
           const uint64_t at = s * (kFp8WideStage >> 4);

@@ -269,7 +269,7 @@ __global__ void __launch_bounds__(32 * kKvWarps, kv8_ctas(kBrief)) kv8_attention
       const int tok0 = u * kUnit;
       const unsigned char* runs = ring + stage * kStage;
       const unsigned gone = missing >> (8 * stage) & ((1u << kRuns) - 1);
-      ok = ok && __all_sync(kFullMask, mbar_wait_quick(&s_full[warp][stage], turn));
+      ok = ok && warp_wait_quick(&s_full[warp][stage], turn);
       if (!ok) break;
       // Scores: s[i][n][h] holds token tok0 + 16 i + 8 h + g against rows 8 n + 2 t
       // and the next.

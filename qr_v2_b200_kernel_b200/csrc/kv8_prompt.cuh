@@ -222,6 +222,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(Kv8AttnPa
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = s_tmem;
+  const auto gave_up = [&]() { return __any_sync(kFullMask, s_bad) != 0; };  // the same to a whole warp, whenever its lanes look
   const int aside_every = P.part_o ? prompt_aside(std::is_same<T, __half>::value) : 1 << 30;
 
   if (warp < 8) {
@@ -462,8 +463,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(Kv8AttnPa
       unsigned char* keys = sk + st * kTile;
       unsigned char* values = keys + kTile / 2;
       const unsigned char* from = raw + rs * (kTile / 2) + lane * 16;
-      if (!s_bad && !__all_sync(kFullMask, mbar_wait_quick(&raw_full[rs], (j / kPromptRaw) & 1))) s_bad = 1;
-      if (j >= kPromptStages && !s_bad && !__all_sync(kFullMask, mbar_wait_quick(&kv_empty[st], (j / kPromptStages - 1) & 1))) s_bad = 1;
+      bool bad = gave_up() || !warp_wait_quick(&raw_full[rs], (j / kPromptRaw) & 1);
+      bad = bad || (j >= kPromptStages && !warp_wait_quick(&kv_empty[st], (j / kPromptStages - 1) & 1));
+      if (bad) s_bad = 1;
       if (kBoth || cw < 2)
 #pragma unroll
         for (int l = 0; l < 4; ++l) {
@@ -507,12 +509,12 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(Kv8AttnPa
     const auto look_up = [&](int j) { return j < count ? page_of((block0 + j) * 4 + (lane & 3)) : -1; };
     constexpr int kRun = 32 * kDim;
     int page = look_up(0);
-    for (int j = 0; j < count && !s_bad; ++j) {
+    for (int j = 0; j < count && !gave_up(); ++j) {
       const int rs = j % kPromptRaw, next = look_up(j + 1);
       float2 step = make_float2(0.f, 0.f);
       if (page >= 0) step = __ldg(steps + (long long)page * P.sh.heads + head);
       const unsigned here = __ballot_sync(kFullMask, page >= 0) & 15u;
-      if (j >= kPromptRaw && !__all_sync(kFullMask, mbar_wait_quick(&raw_empty[rs], (j / kPromptRaw - 1) & 1))) {
+      if (j >= kPromptRaw && !warp_wait_quick(&raw_empty[rs], (j / kPromptRaw - 1) & 1)) {
         s_bad = 1;
         break;
       }
@@ -549,13 +551,13 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(Kv8AttnPa
     };
     bool ok = true;
     for (int j = 0; ok && x < both && j < 2 && j < count; ++j) {
-      ok = mbar_wait_quick(&kv_full[j], 0);
+      ok = warp_wait_quick(&kv_full[j], 0);
       tc_fence_after();
       if (ok) scores(j);
     }
     for (int j = 0; ok && x < both && j < count; ++j) {
       const int st = j % kPromptStages;
-      ok = mbar_wait_quick(&p_full[x][j & 1], (j >> 1) & 1);
+      ok = warp_wait_quick(&p_full[x][j & 1], (j >> 1) & 1);
       if (!ok) break;
       tc_fence_after();
       if (elect_one()) {
@@ -570,7 +572,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(Kv8AttnPa
       }
       __syncwarp();
       if (j + 2 < count) {
-        ok = mbar_wait_quick(&kv_full[(j + 2) % kPromptStages], ((j + 2) / kPromptStages) & 1);
+        ok = warp_wait_quick(&kv_full[(j + 2) % kPromptStages], ((j + 2) / kPromptStages) & 1);
         tc_fence_after();
         if (ok) scores(j + 2);
       }

@@ -205,6 +205,11 @@ __device__ __forceinline__ bool mbar_wait_quick(uint64_t* mbar, uint32_t parity)
   return __builtin_expect(done != 0, 1) || mbar_wait_on(mbar, parity);
 }
 
+// By a whole warp, with one answer for it: where the limit runs out as the phase ends, lanes could part otherwise.
+__device__ __forceinline__ bool warp_wait_quick(uint64_t* mbar, uint32_t parity) {
+  return __all_sync(kFullMask, mbar_wait_quick(mbar, parity));
+}
+
 __device__ __forceinline__ void fence_async_smem() {
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
 }
