@@ -140,6 +140,7 @@ static cudaError_t launch_fp8(const Fp8Params& p, I8Operand x, I8Operand w, uint
 using namespace qrb200;
 
 int qrb200_internal_fp8_site() { return take_site(); }
+bool qrb200_internal_fp8_register(int* word) { return register_word(word); }
 
 extern "C" {
 

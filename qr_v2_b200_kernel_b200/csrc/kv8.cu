@@ -117,6 +117,7 @@ static cudaError_t launch_prompt(const Kv8AttnParams& p, cudaStream_t s) {
 using namespace qrb200;
 
 int qrb200_internal_kv8_site() { return take_site(); }
+bool qrb200_internal_kv8_register(int* word) { return register_word(word); }
 
 extern "C" {
 

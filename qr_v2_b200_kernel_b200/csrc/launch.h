@@ -18,19 +18,13 @@
 
 namespace qrb200 {
 
-// This translation unit's failure words, registered once per device after the library's own check.
+// The device checked, and what an earlier kernel on it has reported. (Every source file's failure words are registered by the first
+// call of any operator on a device: a symbol's copy could not be captured.)
 static int quant_ready() {
-  static std::atomic<unsigned long long> ready{0};
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess) return QRB200_ERR_CUDA;
-  if (dev < 64 && ((ready.load(std::memory_order_acquire) >> dev) & 1ull)) return qrb200_last_status(nullptr);
   const int st = qrb200_internal_check_device();
-  if (st != QRB200_OK) return st;
-  int* word = qrb200_internal_status_word(dev);
-  if (word && cudaMemcpyToSymbol(g_status_mapped, &word, sizeof(word)) != cudaSuccess) return QRB200_ERR_CUDA;
-  if (dev < 64) ready.fetch_or(1ull << dev, std::memory_order_acq_rel);
-  return qrb200_last_status(nullptr);
+  return st != QRB200_OK ? st : qrb200_last_status(nullptr);
 }
+static inline bool register_word(int* word) { return cudaMemcpyToSymbol(g_status_mapped, &word, sizeof(word)) == cudaSuccess; }
 
 // Reads and clears this translation unit's device failure word; a site, 0, or -1 for a CUDA error.
 static inline int take_site() {

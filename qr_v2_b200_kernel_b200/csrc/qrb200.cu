@@ -205,12 +205,14 @@ static int register_status_word(int dev) {
   if (cudaHostGetDevicePointer(&dptr, g_status_host + dev, 0) != cudaSuccess) return QRB200_ERR_CUDA;
   int* word = static_cast<int*>(dptr);
   if (cudaMemcpyToSymbol(g_status_mapped, &word, sizeof(word)) != cudaSuccess) return QRB200_ERR_CUDA;
+  for (bool (*set)(int*) : {qrb200_internal_quant_register, qrb200_internal_fp8_register, qrb200_internal_kv8_register})
+    if (!set(word)) return QRB200_ERR_CUDA;
   return QRB200_OK;
 }
 
-// The current device must be an sm_100 GPU. The first call per device also registers its
-// mapped failure word (a synchronous symbol copy: make the first call on a device before any
-// stream capture on it).
+// The current device must be an sm_100 GPU. The first call per device, of any operator, also registers its
+// mapped failure word with every source file that has device code (synchronous symbol copies: make the first call on a device
+// before any stream capture on it).
 static int check_device() {
   static PerDevice ok, bad;
   int dev = 0;
@@ -1131,14 +1133,6 @@ __global__ void selftest_wait_kernel(uint32_t polls) {
 using namespace qrb200;
 
 int qrb200_internal_check_device() { return check_device(); }
-int* qrb200_internal_status_word(int dev) {
-  void* d = nullptr;
-  std::lock_guard<std::mutex> lk(g_status_mu);
-  if (!g_status_host || dev < 0 || dev >= kStatusWords ||
-      cudaHostGetDevicePointer(&d, g_status_host + dev, 0) != cudaSuccess)
-    return nullptr;
-  return static_cast<int*>(d);
-}
 void qrb200_internal_count_launch() { g_launches.fetch_add(1, std::memory_order_relaxed); }
 
 static int geqrf_impl(const float* A, float* H, float* tau, int64_t batch, int64_t n,

@@ -280,6 +280,7 @@ static cudaError_t launch_attention_of(const Kv4AttnParams& p, const AttnPlan& p
 using namespace qrb200;
 
 int qrb200_internal_quant_site() { return take_site(); }
+bool qrb200_internal_quant_register(int* word) { return register_word(word); }
 
 extern "C" {
 
