@@ -66,10 +66,10 @@ static Kv8Plan attn_plan(const Kv8Shape& h, bool half, int64_t batch, int64_t qu
       }
     }
   }
-  // The prompt kernel does not split the tokens: 1.15 us for each 64 of them and 8 for the rest of a CTA, one an SM. (2 x 2048
-  // queries over 4096 tokens, 16 heads on 4: 146 us for 647; 8 x 16 over 4096, 32 on 8: 73 for 63; 1 x 128 over 4096, 16
-  // on 4: 93 for 37.)
-  const int64_t tiles = (rows + kPromptRows - 1) / kPromptRows, wide = (tiles * batch * h.heads + sms - 1) / sms * (tokens / kPromptTokens * 1150 + 8000);
+  // The prompt kernel does not split the tokens: 1.4 us for each 64 of them and 8 for the rest of a CTA, one an SM. (16 heads on 4 of 128
+  // channels, over 4096 tokens: 1 x 512 queries 104 us for 122, 1 x 128 104 for 38; 32 on 8, 8 x 16 queries over 4096: 78 for
+  // 65, 16 x 24 over 2048: 46 for 103.)
+  const int64_t tiles = (rows + kPromptRows - 1) / kPromptRows, wide = (tiles * batch * h.heads + sms - 1) / sms * (tokens / kPromptTokens * 1400 + 8000);
   if (p.tile_rows == 16 && wide < best) {
     p.prompt = true;
     p.tile_rows = kPromptRows, p.tiles = (int)tiles, p.splits = 1, p.memory = false;
