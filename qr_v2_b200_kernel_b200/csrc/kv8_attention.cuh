@@ -89,7 +89,7 @@ __global__ void __launch_bounds__(32 * kKvWarps, kv8_ctas(kBrief)) kv8_attention
   extern __shared__ __align__(128) unsigned char s_ring[];
   __shared__ uint2 s_q[kNT][kSteps][32];
   __shared__ unsigned s_qtop[kKvWarps][kNT][8];
-  __shared__ float2 s_step[kKvWarps][kStages][kRuns];  // a run's key and value steps
+  __shared__ float4 s_step[kKvWarps][kStages][kRuns];  // a run's key and value steps, and the power of two above the latter
   __shared__ float2 s_ml[kKvWarps][kRows];
   __shared__ uint64_t s_full[kKvWarps][kStages];
   __shared__ int s_bad;
@@ -179,7 +179,7 @@ __global__ void __launch_bounds__(32 * kKvWarps, kv8_ctas(kBrief)) kv8_attention
     }
     const uint32_t bar = smem_u32(&s_full[warp][stage]), dst = smem_u32(ring + stage * kStage);
     const int mine = page_base + lane - unit * kRuns;
-    if (mine >= 0 && mine < kRuns) s_step[warp][stage][mine] = step;
+    if (mine >= 0 && mine < kRuns) s_step[warp][stage][mine] = make_float4(step.x, step.y, kv8_above(step.y), 0.f);
     const auto at = [&](int pg, int run) {
       return P.codes + ((long long)pg * P.sh.heads + head) * P.sh.block_bytes() + (run & (page_runs - 1)) * kRunBytes;
     };
@@ -248,7 +248,7 @@ __global__ void __launch_bounds__(32 * kKvWarps, kv8_ctas(kBrief)) kv8_attention
   // Weights are 2^(score + less), the reference being -less; bound is where a score moves it: 4
   // above, rounded down where scores are so large (so the reference cannot be had back from it), and
   // -inf while nothing has been seen. With their steps weights are held times `unit`, which puts the largest that the row has met
-  // at 2^kKv8StepExp; reach is where a score with the power of two above its value's step moves it, 4 above. A row's numbers hang on
+  // at 2^kKv8StepExp; reach is where a weight with the power of two above its value's step, in exponents, moves it, 4 above. A row's numbers hang on
   // nothing but what the row sees.
   float2 less[kNT] = {}, unit[kNT];
   float bound[kNT][2], reach[kNT][2];
@@ -275,6 +275,7 @@ __global__ void __launch_bounds__(32 * kKvWarps, kv8_ctas(kBrief)) kv8_attention
       // and the next.
       float2 s[kRuns][kNT][2];
       float2 steps[kRuns];
+      float above = kNone;  // of all of them
       {
         float acc[kRuns][kNT][4] = {};  // (even and odd steps apart, a chain of products half as long: 172 -> 182 us at 64 x 8192 tokens)
 #pragma unroll
@@ -299,7 +300,9 @@ __global__ void __launch_bounds__(32 * kKvWarps, kv8_ctas(kBrief)) kv8_attention
         }
 #pragma unroll
         for (int i = 0; i < kRuns; ++i) {
-          steps[i] = s_step[warp][stage][i];
+          const float4 of_run = s_step[warp][stage][i];
+          steps[i] = make_float2(of_run.x, of_run.y);
+          above = fmaxf(above, of_run.z);
           const float keys = steps[i].x > 0.f ? kv8_part(steps[i].x) * P.scale_part : steps[i].x;  // 0 and NaN as they are
           const int e = kv8_power(steps[i].x);  // (factors below 2^97, products below 2^29: no score is infinite, nor 0 times one NaN)
 #pragma unroll
@@ -335,18 +338,21 @@ __global__ void __launch_bounds__(32 * kKvWarps, kv8_ctas(kBrief)) kv8_attention
             }
         }
       }
-      float up[kNT][2], far[kNT][2];  // the largest score, and with the power of two above its value's step
+      // The largest score, and whether a weight with the power of two above its value's step may be further up than any before. (That is
+      // added to the difference: next to a large score it would be lost.)
+      float up[kNT][2];
       bool move = false;
 #pragma unroll
       for (int n = 0; n < kNT; ++n) {
-        up[n][0] = up[n][1] = far[n][0] = far[n][1] = kNone;
+        up[n][0] = up[n][1] = kNone;
 #pragma unroll
-        for (int i = 0; i < kRuns; ++i) {
-          const float e = kv8_above(steps[i].y), x = fmaxf(s[i][n][0].x, s[i][n][1].x), y = fmaxf(s[i][n][0].y, s[i][n][1].y);
-          up[n][0] = fmaxf(up[n][0], x), far[n][0] = fmaxf(far[n][0], x + e);
-          up[n][1] = fmaxf(up[n][1], y), far[n][1] = fmaxf(far[n][1], y + e);
-        }
-        move = move || up[n][0] > bound[n][0] || up[n][1] > bound[n][1] || far[n][0] > reach[n][0] || far[n][1] > reach[n][1];
+        for (int i = 0; i < kRuns; ++i)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            up[n][0] = fmaxf(up[n][0], s[i][n][h].x);
+            up[n][1] = fmaxf(up[n][1], s[i][n][h].y);
+          }
+        move = move || up[n][0] > bound[n][0] || up[n][1] > bound[n][1] || up[n][0] + less[n].x + above > reach[n][0] || up[n][1] + less[n].y + above > reach[n][1];
       }
       if (__any_sync(kFullMask, move)) {
 #pragma unroll
@@ -354,20 +360,34 @@ __global__ void __launch_bounds__(32 * kKvWarps, kv8_ctas(kBrief)) kv8_attention
           float keep[2], all[2];
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
+            // The row's largest score in each run. (Shuffles by the whole warp, whatever its rows need; all of a row's lanes decide alike.)
+            float high[kRuns];
 #pragma unroll
-            for (int x = 4; x < 32; x <<= 1) {
-              up[n][c] = fmaxf(up[n][c], __shfl_xor_sync(kFullMask, up[n][c], x));
-              far[n][c] = fmaxf(far[n][c], __shfl_xor_sync(kFullMask, far[n][c], x));
+            for (int i = 0; i < kRuns; ++i) {
+              high[i] = c ? fmaxf(s[i][n][0].y, s[i][n][1].y) : fmaxf(s[i][n][0].x, s[i][n][1].x);
+#pragma unroll
+              for (int x = 4; x < 32; x <<= 1) high[i] = fmaxf(high[i], __shfl_xor_sync(kFullMask, high[i], x));
             }
+            const float last = reference(n, c), was = c ? unit[n].y : unit[n].x;
+            float next = last;
+#pragma unroll
+            for (int i = 0; i < kRuns; ++i) next = fmaxf(next, high[i]);
+            // The largest weight with the power of two above its value's step, in exponents, against a reference.
+            const auto furthest = [&](float base) {
+              float x = kNone;
+#pragma unroll
+              for (int i = 0; i < kRuns; ++i) x = fmaxf(x, high[i] - base + kv8_above(steps[i].y));
+              return x;
+            };
+            const bool mine = next > bound[n][c] || furthest(last) > reach[n][c];
+            const float top = fmaxf(furthest(next), reach[n][c] - kKvLazy - (next - last));
             keep[c] = all[c] = 1.f;
-            if (up[n][c] > bound[n][c] || far[n][c] > reach[n][c]) {
-              const float last = reference(n, c), next = fmaxf(up[n][c], last), was = c ? unit[n].y : unit[n].x;
-              const float top = reach[n][c] == kNone ? far[n][c] : fmaxf(far[n][c], reach[n][c] - kKvLazy);
-              const int power = min(100, max(-126, kKv8StepExp - (int)ceilf(top - next))), by = power - kv8_power(was);
+            if (mine) {
+              const int power = min(100, max(-126, kKv8StepExp - (int)ceilf(fmaxf(top, -200.f)))), by = power - kv8_power(was);
               keep[c] = kv_exp2(last - next);
               all[c] = keep[c] * (by < -126 ? 0.f : kv_power(by));
               bound[n][c] = __fadd_rd(next, kKvLazy);
-              reach[n][c] = __fadd_rd(top, kKvLazy);
+              reach[n][c] = top + kKvLazy;
               (c ? less[n].y : less[n].x) = -next;
               (c ? unit[n].y : unit[n].x) = kv_power(power);
             }

@@ -140,6 +140,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(Kv8AttnPa
   // so each step waits for a barrier whose last phase but one is known to be over.)
   __shared__ uint32_t s_tmem;
   __shared__ float4 s_key[kPromptStages], s_value[kPromptStages];  // steps of a stage's runs, the keys' scaled
+  __shared__ float s_above[kPromptStages];  // the power of two above the largest of the values' steps
   __shared__ int s_gone[kPromptStages];      // bits: runs without a page
   __shared__ float2 s_step[kPromptRaw][4];
   __shared__ int s_missing[kPromptRaw];
@@ -280,9 +281,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(Kv8AttnPa
     if (mine < both) {
       // What every row of the warp sees.
       const int in_lo = __reduce_max_sync(kFullMask, lo), in_hi = __reduce_min_sync(kFullMask, real ? hi : 0x7fffffff);
-      // Weights are 2^(score - ref); with their steps they are held times `unit`, which puts the largest that the row has met, 2^(reach
-      // - ref) at most, at 2^kPromptTop. A row's numbers hang on nothing but what the row sees.
+      // Weights are 2^(score - ref); with their steps they are held times `unit`, which puts the largest that the row has met, 2^reach
+      // at most, at 2^kPromptTop. A row's numbers hang on nothing but what the row sees.
       float ref = kNone, sum = 0.f, reach = kNone, unit = 1.f;
+      bool calm = true;  // no row's reference in the warp is so large that its rounding matters
       // Set aside, four channels of a row beside the next row's: the sums of earlier steps, against the reference of then, which `lag`
       // brings to the present one.
       const auto set_aside = [&]() {
@@ -307,11 +309,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(Kv8AttnPa
           for (int c = 0; c < 4; ++c) tmem_arrived(v[c]);
           const int gone = s_gone[st];
           const bool full = tok0 >= in_lo && tok0 + kPromptTokens <= in_hi && gone == 0;
-          // The largest score, and the largest one with the power of two above its value's step. (Factors are not negative, so a run's
-          // largest product gives its largest score.)
+          // The largest score of each run. (Factors are not negative, so the largest product gives it.)
+          float score[4];
           const auto largest = [&](auto all) {
             constexpr bool kAll = decltype(all)::value;
-            float2 top = make_float2(kNone, kNone);
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
               float m = kNone;
@@ -323,21 +324,25 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(Kv8AttnPa
                   const float x = v[c][4 * r + i];
                   m = kAll || (at >= lo && at < hi && !(gone >> r & 1)) ? fmaxf(m, x) : m;
                 }
-              const float score = kAll || m > kNone ? m * f[r] : kNone;
-              top.x = fmaxf(top.x, score);
-              top.y = fmaxf(top.y, score + kv8_above(w[r]));
+              score[r] = kAll || m > kNone ? __fmul_rn(m, f[r]) : kNone;  // (rounded before anything is taken from it)
             }
-            return top;
           };
-          const float2 top = full ? largest(std::true_type{}) : largest(std::false_type{});
-          const bool move = top.x > __fadd_rd(ref, kKvLazy) || top.y > __fadd_rd(reach, kKvLazy) || (ref == kNone && top.x > kNone);
-          if (__any_sync(kFullMask, move)) {
+          if (full) largest(std::true_type{});
+          else largest(std::false_type{});
+          // Of all, and with the power of two above its value's step, which is added to the difference: next to a large score it would be lost.
+          const float top = fmaxf(fmaxf(score[0], score[1]), fmaxf(score[2], score[3])), base = ref == kNone ? top : ref;
+          // (First with the largest of the steps, which the row need not see.)
+          if (__any_sync(kFullMask, top > __fadd_rd(ref, kKvLazy) || top - base + s_above[st] > reach + kKvLazy || (ref == kNone && top > kNone))) {
+            float far = kNone;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) far = fmaxf(far, score[r] - base + kv8_above(w[r]));
+            const bool move = top > __fadd_rd(ref, kKvLazy) || far > reach + kKvLazy || (ref == kNone && top > kNone);
             float keep = 1.f, ratio = 1.f;
             const bool none = ref == kNone;
             if (move) {
-              const float next = fmaxf(ref, top.x);
-              reach = fmaxf(reach, top.y);
-              const int power = min(100, max(-126, kPromptTop - (int)ceilf(reach - next))), by = power - kv8_power(unit);
+              const float next = fmaxf(ref, top);
+              reach = fmaxf(reach, far) - (next - base);
+              const int power = min(100, max(-126, kPromptTop - (int)ceilf(fmaxf(reach, -200.f)))), by = power - kv8_power(unit);
               keep = none ? 0.f : kv_exp2(ref - next);
               ratio = by < -126 ? 0.f : kv_power(by);
               unit = kv_power(power);
@@ -361,6 +366,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(Kv8AttnPa
             }
             sum *= keep;
             lag *= keep * ratio;
+            calm = __all_sync(kFullMask, ref == kNone || fabsf(ref) < 0x1p20f);
           }
           const float scaled[4] = {kv8_scaled(w[0], unit), kv8_scaled(w[1], unit), kv8_scaled(w[2], unit), kv8_scaled(w[3], unit)};
           const float less = ref == kNone ? 0.f : -ref;
@@ -378,7 +384,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(Kv8AttnPa
                   const float2 f2 = make_float2(f[r], f[r]), w2 = make_float2(scaled[r], scaled[r]);
 #pragma unroll
                   for (int i = 0; i < 4; i += 2) {
-                    const float2 x = __ffma2_rn(make_float2(v[c + d][4 * r + i], v[c + d][4 * r + i + 1]), f2, less2);
+                    // (In one operation the difference from a large reference is that of the unrounded score, which may be far above 0;
+                    // paired products and sums would be made one.)
+                    const float2 v2 = make_float2(v[c + d][4 * r + i], v[c + d][4 * r + i + 1]);
+                    const float2 x = kAll ? __ffma2_rn(v2, f2, less2) : make_float2(__fmul_rn(v2.x, f[r]) + less, __fmul_rn(v2.y, f[r]) + less);
                     const int at = tok0 + prompt_token(16 * (c + d) + 4 * r + i);  // and the next
                     const bool one = kAll || (at >= lo && at < hi && !(gone >> r & 1)), two = kAll || (at + 1 >= lo && at + 1 < hi && !(gone >> r & 1));
                     float2 p = make_float2(one ? kv_exp2(x.x) : 0.f, two ? kv_exp2(x.y) : 0.f);
@@ -397,7 +406,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(Kv8AttnPa
               tmem_put16(s_at + 16 * c + 16, low);
             }
           };
-          if (full) weights(std::true_type{});
+          if (full && calm) weights(std::true_type{});
           else weights(std::false_type{});
           sum += sums.x + sums.y;
           tmem_put_wait();
@@ -495,7 +504,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(Kv8AttnPa
         const float2 step = s_step[rs][lane];
         reinterpret_cast<float*>(&s_key[st])[lane] = step.x * P.scale_part;  // (steps are 2^-107 to 2^121, the scale's part below 3)
         reinterpret_cast<float*>(&s_value[st])[lane] = step.y;
-        if (lane == 0) s_gone[st] = s_missing[rs];
+        const float above = kv8_above(step.y), other = fmaxf(above, __shfl_xor_sync(15u, above, 1));
+        const float most = fmaxf(other, __shfl_xor_sync(15u, other, 2));
+        if (lane == 0) s_gone[st] = s_missing[rs], s_above[st] = most;
       }
       fence_async_smem();
       __syncwarp();

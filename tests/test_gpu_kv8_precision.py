@@ -239,3 +239,32 @@ def test_values_near_the_largest_and_the_smallest(size, batch, heads, share, que
     out = qr.kv8_attention(q, cache, table, lengths)
     assert out.isfinite().all()
     _check(out[:2], q[:2], cache, slots, lengths, 4)
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("batch, heads, share, queries", [(40, 8, 4, 40), (2, 2, 8, 12), (1, 1, 1, 1)])
+@pytest.mark.parametrize("power", [10, 24, 27, 40])
+def test_scores_next_to_which_a_values_step_is_lost(power, batch, heads, share, queries, dim, dtype):
+    # every 29th token's score is near 2^power, the others' are 0; values reach 2^12, steps are near 2^5, and later pages' larger still
+    n, page = 200, 16
+    cache, table, slots = _pages(batch, n, heads, dim, page, dtype)
+    k = torch.zeros(batch, n, heads, dim, device="cuda")
+    k[:, ::29, :, 0] = 1
+    v = torch.randn(batch, n, heads, dim, generator=_gen(1), device="cuda") * torch.linspace(3, 2000, n, device="cuda")[None, :, None, None]
+    _write(cache, slots, k, v)
+    q = torch.zeros(batch, queries, heads * share, dim, device="cuda")
+    q[..., 0] = 8
+    q = q.to(dtype)
+    cache.range[..., 0] *= 2.0 ** (power - 3)  # a score is 8 / 8 of a key's entry, by the scale
+    lengths = torch.full((batch,), n, dtype=torch.int32, device="cuda")
+    out = qr.kv8_attention(q, cache, table, lengths, scale=1.0)
+    assert out.isfinite().all()
+    if power == 10:
+        return
+    for b in range(min(batch, 2)):  # the same score for each of the tokens, and nothing for the others
+        _, values, _ = _values(cache, slots[b])
+        for i in range(queries):
+            at = values[: n - queries + i + 1 : 29].repeat_interleave(share, 1)
+            want, size = at.mean(0), at.abs().mean(0)
+            assert torch.all((out[b, i].double() - want).abs() <= torch.finfo(dtype).eps / 2 * want.abs() + 2.0**-15 * size)
