@@ -117,7 +117,7 @@ static cudaError_t launch_fp8_rows(const Fp8Params& p, const I8Operand& x, const
   return cudaLaunchKernelEx(&l.cfg, x.aligned && w.aligned ? fp8_rows_linear_kernel<T, true> : fp8_rows_linear_kernel<T, false>, r);
 }
 
-// (4096 x 4096: up to eight rows 4.3-4.6 us, nine to sixteen through tcgen05 6.5.)
+// (4096 x 4096: up to eight rows 4.3-4.7 us, nine to sixteen through tcgen05 6.3-6.5.)
 constexpr int kFp8Rows = 8;
 
 template <typename T>

@@ -48,8 +48,7 @@ __device__ __forceinline__ void fp8_mma_pair(uint32_t d, uint64_t a, uint64_t b,
 // The time is that of reading the weights once, and at these sizes mostly latency. A CTA takes 16 channels, a warp every
 // sixteenth block of the depth: weights, straight from memory, are the 16-row operand of the warp-level matrix instruction and
 // rows of x its columns; the order of a block's products is free, so a lane's 32 bytes of a row are two wide loads. Many warps
-// with a block each in flight beat fewer with more (1 x 4096 x 4096: 4.3 us, 3.9 TB/s of weights; eight warps with four
-// blocks 7.5, one CTA an SM, or 5.0).
+// with a block each in flight: 1 x 4096 x 4096 4.3 us, 3.9 TB/s of weights.
 struct Fp8RowsOperands {
   Fp8Params p;
   I8Operand x, w;
@@ -117,8 +116,8 @@ __global__ void __launch_bounds__(32 * kFp8RowsWarps, 2) fp8_rows_linear_kernel(
 // CTA then adds all the CTAs' sums of some rows of x, in their order, through distributed shared memory.
 //
 // Warp 0 issues the loads, warp 1 the MMAs into two accumulators in turn, warps 2-5 hold one output
-// channel a lane and kBN sums each. 4096 x 4096: 16 rows 6.3 us, 64 8.2, 128 10.7, that is 2.7 to 1.6 TB/s of weights: the
-// set-up, the first loads and the join of the cut depth are most of it (333 x 1000 x 2000 8.3).
+// channel a lane and kBN sums each. 4096 x 4096: 9 to 16 rows 6.3-6.5 us, 64 8.4, 128 10.7, that is 2.6 to 1.6 TB/s of weights: the
+// set-up, the first loads and the join of the cut depth, one after another (issue slots 16 % busy, tensor pipe 11 %; 333 x 1000 x 2000 8.4).
 constexpr int kFp8Split = 4;  // the most CTAs that share a tile's depth
 constexpr int kFp8Scales = 8;  // blocks whose scales are held at a time
 template <int kBN>
@@ -338,13 +337,12 @@ __global__ void __launch_bounds__(192) fp8_few_kernel(Fp8Params P, const __grid_
 //
 // A block's products take 512 clocks, and its accumulator must be free again 512 later. Between lie the
 // commit, the epilogue's loads and the other CTA's word, so what those wait for is kept short:
-// * one warp of a CTA asks the memory barriers for the eight, and passes the word on by named barriers (the
-//   eight asking for themselves, and arriving for themselves: 257 us).
+// * one warp of a CTA asks the memory barriers for the eight, and passes the word on by named barriers.
 //   On each of those the same nine warps wait for one another, block after block, so that they stay in step where a wait for the memory ran
 //   out and nothing else holds them back;
 // * half of a block's sums are loaded at once, and the accumulator is free before the last half is added;
 // * the scales of four blocks come in one load (32 lines a warp's load, it holds up the barriers behind it).
-// 8192 x 8192 x 4096: 238 us, 2.3 P op/s; without the additions (one accumulator over the depth, one scale a row
+// 8192 x 8192 x 4096: 239 us, 2.3 P op/s; without the additions (one accumulator over the depth, one scale a row
 // and channel) the same products take 207 us under the power cap.
 constexpr int kFp8WideStage = 2 * 128 * kI8Depth;  // bytes per CTA and stage
 constexpr int kFp8WideStages = 5;

@@ -480,9 +480,9 @@ __global__ void __launch_bounds__(32 * kKv8ThinWarps) kv8_write_thin_kernel(Kv8I
     kv8_write_thin<T, kDim, kVec, false>(P, s_row[warp], nullptr, page, head);
   }
 }
-// and each CTA. 32768 tokens x 8 heads x 128 channels, bf16: 71 us from a page's first token, 73 from within one, 2.9 TB/s of
-// keys, values and codes; in instructions and their order, the three kernels before it 8 of them. (Both sorts of pages in one kernel:
-// 75 and 80, the registers of the one hold up the other.)
+// and each CTA. 32768 tokens x 8 heads x 128 channels, bf16: 69 us from a page's first token, 71 from within one, 3.0 TB/s of
+// keys, values and codes, the three kernels before it 8 of them. No pipe is full (issue slots 41 %, memory 31 %): a head's loads,
+// maximum, packing and stores follow one another, and 128 registers leave sixteen warps an SM.
 template <typename T, int kDim, bool kVec>
 __global__ void __launch_bounds__(2 * kDim) kv8_write_kernel(Kv8IoParams P) {
   __shared__ Kv8Thick<kDim> s_thick;

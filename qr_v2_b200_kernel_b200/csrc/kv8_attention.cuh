@@ -5,9 +5,9 @@
 // So the codes are the matrix operands, exact in 16 bits: a byte c + 128 under the exponent of 1024 is the fp16 number
 // 1152 + c, one addition away from c. No key or value is ever rounded; steps are applied in 32 bits.
 //
-// 64 sequences of 8192 tokens, 8 heads of 128 channels with 8 query rows each, bf16: 172 us for 1.07 GB, 6.2 TB/s (under the power
-// cap, 208). The bytes bound it there, with issue slots 64 % busy; fewer or shorter sequences wait for a chain of latencies (one
-// of 513 tokens 7.3 us). A CTA's four warps take a quarter of its tokens each, so nothing is shared until the end.
+// 64 sequences of 8192 tokens, 8 heads of 128 channels with 8 query rows each, bf16: 176 us for 1.07 GB, 6.1 TB/s (under the power
+// cap, 213). The bytes bound it there, with issue slots 65 % busy; fewer or shorter sequences wait for a chain of latencies (one
+// of 513 tokens 7.2 us). A CTA's four warps take a quarter of its tokens each, so nothing is shared until the end.
 #pragma once
 
 #include <type_traits>
@@ -63,10 +63,9 @@ constexpr int kKv8Aside = 8;     // steps between settings-aside
 // Bytes of a warp's step, 4 KB or 8: a step costs some 1000 clocks of instructions that wait for one another and 500 for each
 // 4 KB, so long steps suit few warps, and short ones leave shared memory for twice as many (four CTAs an SM for two,
 // at 128 registers for 168). With sixteen query rows, which take the registers of two CTAs anyway, long ones.
-// (64 x 8192 tokens, 8 heads: short 172 us, long 180; 16 x 8192 53, 51; 1 x 8192 13.8, 10.7; sixteen rows,
-// 64 x 8192 tokens, 4 heads: 159-174, 145.)
+// (64 x 8192 tokens, 8 heads: short 172 us, long 180; 1 x 8192 13.8, 10.7.)
 __host__ __device__ constexpr int kv8_runs(int dim, bool brief) { return (brief ? 128 : 256) / dim; }
-constexpr int kKv8Stages = 2;  // steps in a warp's ring; more change nothing
+constexpr int kKv8Stages = 2;  // steps in a warp's ring
 __host__ __device__ constexpr int kv8_ctas(bool brief) { return brief ? 4 : 2; }
 __host__ __device__ constexpr int kv8_ring_bytes(int dim, int nt, bool brief) {
   const int ring = kKvWarps * kKv8Stages * kv8_runs(dim, brief) * 32 * dim, parts = kKvWarps * 8 * nt * (dim + 4) * 4;
@@ -277,7 +276,7 @@ __global__ void __launch_bounds__(32 * kKvWarps, kv8_ctas(kBrief)) kv8_attention
       float2 steps[kRuns];
       float above = kNone;  // of all of them
       {
-        float acc[kRuns][kNT][4] = {};  // (even and odd steps apart, a chain of products half as long: 172 -> 182 us at 64 x 8192 tokens)
+        float acc[kRuns][kNT][4] = {};
 #pragma unroll
         for (int c = 0; c < kDim / 64; ++c) {
           uint32_t kc[kRuns][2][4];

@@ -4,12 +4,11 @@
 //   S = Q K^T (fp16 x fp16, Q brought by a power of two to the top of fp16's range, K's codes exact),
 //   P = 2^(S r - reference) w,  O += P V  (V's codes exact; r and w the steps of the tokens' pages),
 // S, P and O in tensor memory (P takes S's place), the softmax of a row in one thread. Each tile has two S, so that
-// the scores of the next step are there when a softmax ends (one S of 128 tokens: 172 us for the chunk below).
+// the scores of the next step are there when a softmax ends.
 //
-// Two sequences' 2048 queries over 4096 tokens, 16 heads on 4 of 128 channels, bf16: 146 us, 0.71 PFLOP/s (64 channels 117). No
-// pipe is full (tensor 36 %, exponentials 37 %, issue slots 46 %): a tile's step is a chain of its products, the
-// loads of its scores, its softmax and its stores, which two tiles and two S fill by half. Two threads to a row took 212 us and
-// more, since the registers of twice the threads do not hold a row's scores.
+// Two sequences' 2048 queries over 4096 tokens, 16 heads on 4 of 128 channels, bf16: 172 us, 0.60 PFLOP/s (fp16 192, 64 channels
+// 143). No pipe is full (tensor 46 %, exponentials 31 %, issue slots 49 %): a tile's step is a chain of its products, the
+// loads of its scores, its softmax and its stores, which two tiles and two S fill by half.
 //
 // Warps 0-3 and 4-7: the softmax of the first and the second tile. Warp 14: bulk copies of the cache's bytes. Warps 8-11:
 // these into fp16 operands (16-bit numbers in memory are twice the traffic, and what the cache saves), K-major in the 128-byte
@@ -32,7 +31,7 @@
 namespace qrb200 {
 
 constexpr int kPromptRows = 256, kPromptTokens = 64;
-constexpr int kPromptStages = 3, kPromptRaw = 2;  // steps of operands, and of bytes, in shared memory (four and two 151 us)
+constexpr int kPromptStages = 3, kPromptRaw = 2;  // steps of operands, and of bytes, in shared memory
 constexpr int kPromptThreads = 32 * 15;
 constexpr int kPromptTop = 11;  // a row's largest weight times step is put below this power of two, and stays below 2^(11 + 4)
 // Steps between settings-aside, a power of two. (Both types, 2 x 2048 queries over 4096 tokens: never 158 us, 32 166, 16 183, 8 209.)

@@ -284,8 +284,8 @@ def kv8_write(cache: KV8Cache, k: torch.Tensor, v: torch.Tensor, slots: torch.Te
     127 steps either way, and where the range grew the page's older codes are rounded to the new
     steps. A call that writes a page's first token begins the page anew: the rest of it reads as zeros. A
     NaN or an infinity makes what the page holds of its head NaN, until the page begins anew. Calls that
-    run at the same time may not write the same page. More than 1024 tokens take a workspace of 4 bytes a slot of the cache. A slot past the cache is skipped and reported by the next call as
-    ``QRB200Error``.
+    run at the same time may not write the same page. More than 1024 tokens take a workspace of 4 bytes a slot of the
+    cache. A slot past the cache is skipped and reported by the next call as ``QRB200Error``.
     """
     (_module or _native()).kv8_write(_handle(cache, KV8Cache), k, v, slots)
 
@@ -302,6 +302,7 @@ def kv8_attention(q: torch.Tensor, cache: KV8Cache, block_table: torch.Tensor, l
     """Softmax attention of each sequence's newest tokens over its 8-bit cache.
 
     Operands, masks, limits and failures as in :func:`kv4_attention`; single tokens, drafts and long prompts alike. Weights
-    are held in 22 bits.
+    are held in 22 bits; in prompts over more than some 2000 tokens (float16 1000) the matrix instruction's cut-offs make
+    the error up to 2^-16 (2^-17) of the values' size. What a row does not see does not enter its result.
     """
     return (_module or _native()).kv8_attention(q, _handle(cache, KV8Cache), block_table, lengths, scale, causal, window)

@@ -14,8 +14,8 @@
     rms_norm_int8 -> int8_linear -> kv4_write -> kv4_attention -> quantize_int8 -> int8_linear
 
     With ``--cache-bits 8`` keys and values go into the 8-bit cache, and with ``--products fp8`` the
-    projections are products of 8-bit floating point with a scale for each block of 128, which need the rotation
-    less: quantize_fp8 -> fp8_linear -> kv8_write -> kv8_attention -> quantize_fp8 -> fp8_linear, the
+    projections are products of 8-bit floating point with a scale for each block of 128, for which the rotation
+    does little: quantize_fp8 -> fp8_linear -> kv8_write -> kv8_attention -> quantize_fp8 -> fp8_linear, the
     norm's factor multiplied into the scales.
 
     The command runs a prompt and some single tokens through one layer, with and without the
