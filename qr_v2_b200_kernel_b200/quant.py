@@ -303,6 +303,6 @@ def kv8_attention(q: torch.Tensor, cache: KV8Cache, block_table: torch.Tensor, l
 
     Operands, masks, limits and failures as in :func:`kv4_attention`; single tokens, drafts and long prompts alike. Weights
     are held in 22 bits; in prompts over more than some 2000 tokens (float16 1000) the matrix instruction's cut-offs make
-    the error up to 2^-16 (2^-17) of the values' size. What a row does not see does not enter its result.
+    the error some 2^-16 (2^-17) of the values' size. What a row does not see does not enter its result.
     """
     return (_module or _native()).kv8_attention(q, _handle(cache, KV8Cache), block_table, lengths, scale, causal, window)
