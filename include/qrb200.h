@@ -147,8 +147,8 @@ int qrb200_geqrf_f32_noalloc(const float* A, float* H, float* tau, int64_t batch
  * hold no outlying channels, and are kept in 8 bits, keys and values in 4. All entries are
  * asynchronous on `stream`, allocate nothing, return a status, and first report (launching
  * nothing) a failure that a kernel of an earlier call has recorded, as qrb200_last_status does.
- * Their first call on each device registers the failure word for these kernels too, with a
- * synchronous symbol copy: make it before any stream capture on that device. */
+ * The first call on each device, of these or of any other entry that launches, registers its failure word for all kernels, with
+ * synchronous symbol copies: make it before any stream capture on that device. */
 
 enum { QRB200_F32 = 0, QRB200_BF16 = 1, QRB200_F16 = 2 }; /* element types */
 
